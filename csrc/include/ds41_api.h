@@ -552,6 +552,25 @@ int ds41_latent_attend(const ds41_latent_attend_args* args, void* stream);
 int ds41_latent_merge(const float* part_o, const float* part_ml, const float* sink, int n_splits, int rows, int heads,
                       int kv_pad, void* out, int ld_out, int f32, void* stream);
 
+// Attention of rows whose page tables begin with the same pages: the common keys are read once for all of them (prefix_attn.cu),
+// every row's other keys by the forms below, which also join the parts.  Device arrays of the plan, made on the host:
+typedef struct ds41_prefix_plan {
+  const int* items;               // [max_items][8]: {slot, first, rows, first key, end key, part, 0, 0}
+  const int* n_items;             // how many there are
+  const int* order;               // pass rows by prefix: an item's rows are order[first] .. order[first + rows - 1]
+  const int* own;                 // [rows] first key that a row reads by itself
+  const int* cell;                // [rows] the row's first cell of part_o / part_ml
+  const int* parts;               // [rows] how many it has
+  float* part_o;                  // [cells][heads][value width] unnormalised results
+  float* part_ml;                 // [cells][heads]{maximum, sum}; grouped attention: of scores in units of log 2, latent: natural
+  int max_items, rows_per_item, grid;      // `grid`: blocks of the first launch, which walk the items
+} ds41_prefix_plan;
+// latent attention: the common keys, the own keys (ds41_latent_attend's partial results over them), and the join of both
+int ds41_prefix_latent_shared(const ds41_latent_attend_args* args, const ds41_prefix_plan* plan, int n_pages, void* stream);
+int ds41_prefix_latent_own(const ds41_latent_attend_args* args, const ds41_prefix_plan* plan, void* stream);
+int ds41_prefix_latent_merge(const float* part_o, const float* part_ml, const float* sink, const ds41_prefix_plan* plan,
+                             int n_splits, int rows, int heads, int kv_pad, void* out, int ld_out, int f32, void* stream);
+
 // Long prompt pass of one request over expanded keys and values (latent_prefill.cu): pass row r stands at position pos0 + r.
 typedef struct ds41_latent_prefill_args {
   const void* q;                  // bf16 [rows][ld_q]: head h at h * (dim_pad + rot_pad): [unrotated | rotated]
@@ -626,6 +645,9 @@ typedef struct ds41_group_attend_args {
 } ds41_group_attend_args;
 // Any mix of rows; n_splits <= 16 CTAs share a row's keys.
 int ds41_group_attend(const ds41_group_attend_args* args, void* stream);
+// The same in two launches for rows that share prefixes: the common keys, then the own ones and the join of the parts.
+int ds41_prefix_group_shared(const ds41_group_attend_args* args, const ds41_prefix_plan* plan, void* stream);
+int ds41_prefix_group_own(const ds41_group_attend_args* args, const ds41_prefix_plan* plan, void* stream);
 // Long prompt pass of one request (bf16, dim_pad <= 256, vdim_pad <= 128, pages of 32, 64 or 128 tokens): row r stands at
 // position pos0 + r.
 int ds41_group_prefill(const ds41_group_attend_args* args, void* stream);

@@ -1,0 +1,316 @@
+// Attention over the common keys of rows that share a prefix, for every type and size, and the join of latent attention's parts.
+//
+// A block takes sixteen queries (head and row) of an item and walks its keys 32 at a time through shared memory, so that a cached
+// value that was read once serves sixteen queries: scores by 256 threads of two (query, key) pairs each, a softmax state per query
+// (running maximum and sum), results in registers.  It serves 32-bit rows and the sizes that the tensor-core forms
+// (prefix_group.cu, prefix_latent.cu) leave out, and is bound by its 32-bit products and their operands from shared memory.
+#include "ds41_prefix.cuh"
+#include "ds41_tma.h"
+
+namespace ds41 {
+
+constexpr int kSimpleQueries = 16;
+constexpr int kSimpleKeys = 32;
+
+struct SimpleArgs {
+  const void *q, *q2, *pool;         // a query is [d1 values of q | d2 of q2]
+  const int *page_table, *row_pos, *row_slot;
+  long long ld_q, ld_q2;
+  int q_head, q2_head;               // values between a row's heads
+  int d1, d2, vp, row_len;
+  int k_lane, v_at, v_lane;          // key / value head g of a cache row: keys at g * k_lane, values at v_at + g * v_lane
+  int lanes, per_lane, heads, chunk, max_pages, page_tokens;
+  float scale, unit;                 // of the maximum that is stored, in units of log 2
+};
+
+inline int simple_smem(const SimpleArgs& p) {
+  const int dp = p.d1 + p.d2;
+  return 4 * (kSimpleQueries * (dp + 4) + kSimpleKeys * (dp + 4) + kSimpleKeys * p.vp + kSimpleQueries * (kSimpleKeys + 1)) +
+         16 * kSimpleQueries;
+}
+
+__device__ __forceinline__ float4 four(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 four(const __nv_bfloat16* p) {
+  const uint2 v = *reinterpret_cast<const uint2*>(p);
+  return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16),
+                     __uint_as_float(v.y & 0xffff0000u));
+}
+
+// QPT: queries whose columns a thread accumulates
+template <typename T, int QPT>
+__global__ void __launch_bounds__(256) prefix_simple_kernel(const SimpleArgs p, const ds41_prefix_plan plan) {
+  extern __shared__ __align__(16) float ps_smem[];
+  const int dp = p.d1 + p.d2, ds = dp + 4, nc = p.vp / 4;
+  float* qs = ps_smem;                                        // [16][ds]
+  float* ks = qs + kSimpleQueries * ds;                       // [32][ds]
+  float* vs = ks + kSimpleKeys * ds;                          // [32][vp]
+  float* sc = vs + kSimpleKeys * p.vp;                        // [16][33] scores, then weights
+  float* ms = sc + kSimpleQueries * (kSimpleKeys + 1);        // [16] maxima
+  float* ls = ms + kSimpleQueries;                            // [16] sums
+  float* keep = ls + kSimpleQueries;                          // [16] factor on what was summed before
+  int* lim = reinterpret_cast<int*>(keep + kSimpleQueries);   // [16] end of what a query sees
+  __shared__ int low[kSimpleQueries], row_of[kSimpleQueries];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int subs = (plan.rows_per_item * p.per_lane + kSimpleQueries - 1) / kSimpleQueries;
+  const int units = *plan.n_items * p.lanes * subs;
+  for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    const PrefixItem it = prefix_item(plan, unit / (p.lanes * subs));
+    const int g = unit / subs % p.lanes, i0 = unit % subs * kSimpleQueries, count = it.rows * p.per_lane;
+    if (i0 >= count) continue;
+    __syncthreads();                     // the last unit's shared memory is no longer read
+    if (tid < kSimpleQueries) {
+      int r = -1, lo = 0, hi = 0;
+      if (i0 + tid < count) {
+        r = plan.order[it.first + (i0 + tid) / p.per_lane];
+        const int pos = p.row_pos[r];
+        if (p.row_slot[r] >= 0) {
+          lo = p.chunk > 0 ? pos - pos % p.chunk : 0;
+          hi = min(min(plan.own[r], pos + 1), it.key1);
+        }
+      }
+      row_of[tid] = r;
+      low[tid] = lo;
+      lim[tid] = hi;
+      ms[tid] = -INFINITY;
+      ls[tid] = 0.f;
+    }
+    __syncthreads();
+    for (int i = 4 * tid; i < kSimpleQueries * dp; i += 1024) {
+      const int u = i / dp, d = i % dp, r = row_of[u], h = g * p.per_lane + (i0 + u) % p.per_lane;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r >= 0)
+        v = d < p.d1 ? four(static_cast<const T*>(p.q) + r * p.ld_q + 1ll * h * p.q_head + d)
+                     : four(static_cast<const T*>(p.q2) + r * p.ld_q2 + 1ll * h * p.q2_head + (d - p.d1));
+      *reinterpret_cast<float4*>(qs + u * ds + d) = v;
+    }
+    int from = INT_MAX, to = 0;
+#pragma unroll
+    for (int u = 0; u < kSimpleQueries; ++u) {
+      if (low[u] < lim[u]) from = min(from, low[u]);
+      to = max(to, lim[u]);
+    }
+    from = max(it.key0, from);
+    float4 acc[QPT];
+#pragma unroll
+    for (int u = 0; u < QPT; ++u) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int col = tid % nc, u0 = tid / nc * QPT;
+    for (int t0 = from; t0 < to; t0 += kSimpleKeys) {
+      __syncthreads();
+      for (int i = 4 * tid; i < kSimpleKeys * (dp + p.vp); i += 1024) {
+        const int j = i / (dp + p.vp), d = i % (dp + p.vp), key = t0 + j, pg = key / p.page_tokens;
+        const int id = key < to && pg < p.max_pages ? p.page_table[1ll * it.slot * p.max_pages + pg] : -1;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (id >= 0) {
+          const T* row = static_cast<const T*>(p.pool) + (1ll * id * p.page_tokens + (key - pg * p.page_tokens)) * p.row_len;
+          v = four(d < dp ? row + g * p.k_lane + d : row + p.v_at + g * p.v_lane + (d - dp));
+        }
+        *reinterpret_cast<float4*>(d < dp ? ks + j * ds + d : vs + j * p.vp + (d - dp)) = v;
+      }
+      __syncthreads();
+      {
+        const int u = tid >> 4, j = tid & 15;
+        float a = 0.f, b = 0.f;
+        for (int d = 0; d < dp; d += 4) {
+          const float4 x = four(qs + u * ds + d), y = four(ks + j * ds + d), z = four(ks + (j + 16) * ds + d);
+          a += x.x * y.x + x.y * y.y + x.z * y.z + x.w * y.w;
+          b += x.x * z.x + x.y * z.y + x.z * z.z + x.w * z.w;
+        }
+        const int key = t0 + j;
+        sc[u * 33 + j] = key >= low[u] && key < lim[u] ? a * p.scale : -INFINITY;
+        sc[u * 33 + j + 16] = key + 16 >= low[u] && key + 16 < lim[u] ? b * p.scale : -INFINITY;
+      }
+      __syncthreads();
+      for (int u = 2 * warp; u < 2 * warp + 2; ++u) {
+        const float s = sc[u * 33 + lane], top = fmaxf(ms[u], warp_max(s));
+        const float e = s == -INFINITY ? 0.f : expf(s - top);
+        const float f = ms[u] == -INFINITY ? 0.f : expf(ms[u] - top), sum = warp_sum(e);
+        __syncwarp();
+        sc[u * 33 + lane] = e;
+        if (lane == 0) {
+          ls[u] = ls[u] * f + sum;
+          ms[u] = top;
+          keep[u] = f;
+        }
+      }
+      __syncthreads();
+      if (u0 < kSimpleQueries) {
+#pragma unroll
+        for (int u = 0; u < QPT; ++u) {
+          const float f = keep[u0 + u];
+          acc[u].x *= f;
+          acc[u].y *= f;
+          acc[u].z *= f;
+          acc[u].w *= f;
+        }
+        for (int j = 0; j < kSimpleKeys; ++j) {
+          const float4 v = four(vs + j * p.vp + 4 * col);
+#pragma unroll
+          for (int u = 0; u < QPT; ++u) {
+            const float w = sc[(u0 + u) * 33 + j];
+            if (w != 0.f) {              // what a query does not see may be anything
+              acc[u].x += w * v.x;
+              acc[u].y += w * v.y;
+              acc[u].z += w * v.z;
+              acc[u].w += w * v.w;
+            }
+          }
+        }
+      }
+    }
+    __syncthreads();
+    if (u0 < kSimpleQueries)
+#pragma unroll
+      for (int u = 0; u < QPT; ++u) {
+        const int r = row_of[u0 + u];
+        if (r < 0) continue;
+        const int h = g * p.per_lane + (i0 + u0 + u) % p.per_lane;
+        const long long cell = (1ll * plan.cell[r] + it.split) * p.heads + h;
+        *reinterpret_cast<float4*>(plan.part_o + cell * p.vp + 4 * col) = acc[u];
+        if (col == 0) *reinterpret_cast<float2*>(plan.part_ml + 2 * cell) = make_float2(ms[u0 + u] * p.unit, ls[u0 + u]);
+      }
+  }
+}
+
+template <typename T, int QPT>
+static int launch_simple(const SimpleArgs& p, const ds41_prefix_plan& plan, cudaStream_t st) {
+  const int smem = simple_smem(p);
+  if (smem > 220 * 1024) return cudaErrorInvalidValue;
+  const cudaError_t e = cudaFuncSetAttribute(prefix_simple_kernel<T, QPT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  const long long most = 1ll * plan.max_items * p.lanes * ((plan.rows_per_item * p.per_lane + kSimpleQueries - 1) / kSimpleQueries);
+  const int blocks = static_cast<int>(most < 4 * sm_count() ? most : 4 * sm_count());
+  return launch_pdl(prefix_simple_kernel<T, QPT>, dim3(blocks), dim3(256), smem, st, p, plan);
+}
+
+template <typename T>
+static int dispatch_simple(const SimpleArgs& p, const ds41_prefix_plan& plan, cudaStream_t st) {
+  const int nc = p.vp / 4;
+  if (16 * nc <= 256) return launch_simple<T, 1>(p, plan, st);
+  if (8 * nc <= 256) return launch_simple<T, 2>(p, plan, st);
+  if (4 * nc <= 256) return launch_simple<T, 4>(p, plan, st);
+  if (2 * nc <= 256) return launch_simple<T, 8>(p, plan, st);
+  if (nc <= 256) return launch_simple<T, 16>(p, plan, st);
+  return cudaErrorInvalidValue;
+}
+
+static int run_simple(const SimpleArgs& p, const ds41_prefix_plan& plan, int f32, cudaStream_t st) {
+  // rows of four values at a time
+  if ((p.ld_q & 3) || (p.ld_q2 & 3) || (p.q_head & 3) || (p.q2_head & 3) || (p.row_len & 3) || (p.d1 & 3) || (p.d2 & 3) || (p.vp & 3) ||
+      ((reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.q2) | reinterpret_cast<uintptr_t>(p.pool)) & (f32 ? 15 : 7)))
+    return cudaErrorInvalidValue;
+  return f32 ? dispatch_simple<float>(p, plan, st) : dispatch_simple<__nv_bfloat16>(p, plan, st);
+}
+
+// One block per (head, row): the cells are the row's own splits, then the parts of its prefix.
+constexpr int kMaxCells = 256;
+template <typename T>
+__global__ void __launch_bounds__(128) prefix_merge_kernel(const float* part_o, const float* part_ml, const float* sink,
+                                                           const ds41_prefix_plan plan, int n_splits, int heads, int kv_pad, T* out,
+                                                           int ld_out) {
+  __shared__ float wt[kMaxCells];
+  __shared__ float red[33], tops[4];
+  const int h = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int parts = min(plan.parts[r], kMaxCells - n_splits), n = n_splits + parts;
+  const long long own0 = 1ll * r * n_splits * heads + h, far0 = 1ll * plan.cell[r] * heads + h;
+  const float sk = sink != nullptr ? sink[h] : -INFINITY;
+  float2 ml[kMaxCells / 128];
+  float m = sk;
+#pragma unroll
+  for (int j = 0; j < kMaxCells / 128; ++j) {
+    const int s = tid + 128 * j;
+    ml[j] = make_float2(-INFINITY, 0.f);
+    if (s < n)
+      ml[j] = s < n_splits ? *reinterpret_cast<const float2*>(part_ml + 2 * (own0 + 1ll * s * heads))
+                           : *reinterpret_cast<const float2*>(plan.part_ml + 2 * (far0 + 1ll * (s - n_splits) * heads));
+    m = fmaxf(m, ml[j].x);
+  }
+  m = warp_max(m);
+  if ((tid & 31) == 0) tops[tid >> 5] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 4; ++w) m = fmaxf(m, tops[w]);
+  float den = 0.f;
+#pragma unroll
+  for (int j = 0; j < kMaxCells / 128; ++j) {
+    const float e = ml[j].x > -INFINITY ? expf(ml[j].x - m) : 0.f;
+    if (tid + 128 * j < n) wt[tid + 128 * j] = e;
+    den += e * ml[j].y;
+  }
+  den = block_sum(den, red) + (sink != nullptr && m > -INFINITY ? expf(sk - m) : 0.f);
+  const float inv = den > 0.f ? 1.0f / den : 0.f;
+  for (int i = 4 * tid; i < kv_pad; i += 512) {
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    const long long step = 1ll * heads * kv_pad;
+    const float* own = part_o + own0 * kv_pad + i;
+    const float* far = plan.part_o + far0 * kv_pad + i;
+#pragma unroll 8
+    for (int s = 0; s < n; ++s) {
+      const float e = wt[s];
+      if (e > 0.f) {
+        const float4 o = *reinterpret_cast<const float4*>(s < n_splits ? own + s * step : far + (s - n_splits) * step);
+        a.x += e * o.x;
+        a.y += e * o.y;
+        a.z += e * o.z;
+        a.w += e * o.w;
+      }
+    }
+    store4(out + 1ll * r * ld_out + h * kv_pad + i, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
+  }
+}
+
+}  // namespace ds41
+
+using namespace ds41;
+
+extern "C" int ds41_prefix_group_shared(const ds41_group_attend_args* a, const ds41_prefix_plan* plan, void* stream) {
+  if (!prefix_plan_ok(plan) || a == nullptr || a->rows <= 0 || a->heads <= 0 || a->kv_heads <= 0 || a->heads % a->kv_heads != 0 ||
+      a->dim_pad <= 0 || (a->dim_pad & 15) || a->vdim_pad <= 0 || (a->vdim_pad & 15) || a->chunk < 0 || a->max_pages <= 0 ||
+      a->page_tokens <= 0 || a->q == nullptr || a->pool == nullptr || a->page_table == nullptr || a->row_pos == nullptr ||
+      a->row_slot == nullptr || a->ld_q < 1ll * a->heads * a->dim_pad)
+    return cudaErrorInvalidValue;
+  SimpleArgs p{};
+  p.q = a->q; p.q2 = a->q; p.pool = a->pool;
+  p.page_table = a->page_table; p.row_pos = a->row_pos; p.row_slot = a->row_slot;
+  p.ld_q = a->ld_q; p.q_head = a->dim_pad; p.d1 = a->dim_pad; p.vp = a->vdim_pad;
+  p.row_len = a->kv_heads * (a->dim_pad + a->vdim_pad);
+  p.k_lane = a->dim_pad; p.v_at = a->kv_heads * a->dim_pad; p.v_lane = a->vdim_pad;
+  p.lanes = a->kv_heads; p.per_lane = a->heads / a->kv_heads; p.heads = a->heads;
+  p.chunk = a->chunk; p.max_pages = a->max_pages; p.page_tokens = a->page_tokens;
+  p.scale = a->scale; p.unit = 1.4426950408889634f;
+  return run_simple(p, *plan, a->f32, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int ds41_prefix_latent_shared(const ds41_latent_attend_args* a, const ds41_prefix_plan* plan, int n_pages, void* stream) {
+  if (!prefix_plan_ok(plan) || a == nullptr || a->rows <= 0 || a->heads <= 0 || a->kv_pad <= 0 || (a->kv_pad & 3) ||
+      a->row_len < a->kv_pad || (a->row_len & 3) || n_pages <= 0 || a->max_pages <= 0 || a->page_tokens <= 0 || a->q_abs == nullptr ||
+      (a->row_len > a->kv_pad && a->q_rot == nullptr) || a->pool == nullptr || a->page_table == nullptr || a->row_pos == nullptr ||
+      a->row_slot == nullptr)
+    return cudaErrorInvalidValue;
+  SimpleArgs p{};
+  p.q = a->q_abs; p.q2 = a->q_rot; p.pool = a->pool;
+  p.page_table = a->page_table; p.row_pos = a->row_pos; p.row_slot = a->row_slot;
+  p.ld_q = a->ld_q_abs; p.q_head = a->kv_pad; p.ld_q2 = a->ld_q_rot; p.q2_head = a->q_rot_stride;
+  p.d1 = a->kv_pad; p.d2 = a->row_len - a->kv_pad; p.vp = a->kv_pad; p.row_len = a->row_len;
+  p.lanes = 1; p.per_lane = a->heads; p.heads = a->heads;
+  p.max_pages = a->max_pages; p.page_tokens = a->page_tokens;
+  p.scale = a->scale; p.unit = 1.f;
+  return run_simple(p, *plan, a->f32, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int ds41_prefix_latent_merge(const float* part_o, const float* part_ml, const float* sink, const ds41_prefix_plan* plan,
+                                        int n_splits, int rows, int heads, int kv_pad, void* out, int ld_out, int f32, void* stream) {
+  if (!prefix_plan_ok(plan) || part_o == nullptr || part_ml == nullptr || n_splits <= 0 || n_splits > 64 || (kv_pad & 3) || kv_pad <= 0 ||
+      rows <= 0 || rows > 65535 || heads <= 0 || out == nullptr || ld_out < heads * kv_pad || (ld_out & 3))
+    return cudaErrorInvalidValue;
+  const dim3 grid(heads, rows);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto launch = [&](auto kernel, auto* o) {
+    return launch_pdl(kernel, grid, dim3(128), 0, st, part_o, part_ml, sink, *plan, n_splits, heads, kv_pad, o, ld_out);
+  };
+  return f32 ? launch(prefix_merge_kernel<float>, static_cast<float*>(out))
+             : launch(prefix_merge_kernel<__nv_bfloat16>, static_cast<__nv_bfloat16*>(out));
+}

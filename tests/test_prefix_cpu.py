@@ -1,0 +1,216 @@
+"""Plans of attention over a shared prefix: which rows share what, how the keys are divided, and what the calls refuse (no GPU)."""
+import itertools
+import random
+
+import numpy as np
+import pytest
+import torch
+
+from ds41rt_b200.ops import prefix
+from ds41rt_b200.ops.prefix import PrefixPlan, common_runs, key_span
+
+BF16 = torch.bfloat16
+
+
+def table(*rows, width=12):
+    t = np.full((len(rows), width), -1, dtype=np.int32)
+    for i, r in enumerate(rows):
+        t[i, :len(r)] = r
+    return t
+
+
+def test_rows_are_grouped_by_their_leading_pages():
+    t = table([1, 2, 3, 4, 5], [1, 2, 3, 7, 8, 9], [1, 2, 3, 11], [1, 20, 21], [30, 31, 32], [30, 31, 33, 34], [])
+    got = {tuple(sorted(rows)): pages for rows, pages in common_runs(t)}
+    assert got == {(0, 1, 2): 3, (4, 5): 2}
+
+
+def test_one_row_that_shares_little_does_not_cost_the_others_their_prefix():
+    t = table(*[[1, 2, 3, 4, 5, 6, 7, 8, 100 + i] for i in range(6)], [1, 200, 201])
+    assert [(sorted(r), p) for r, p in common_runs(t)] == [(list(range(6)), 8)]
+
+
+def test_leading_pages_alone_count_and_free_places_never_do():
+    assert common_runs(table([1, 2, 3], [4, 2, 3])) == []
+    assert common_runs(table([], [])) == []
+    assert common_runs(table([5])) == []
+    assert common_runs(table([1, 2], [1, 2], width=2)) == [([0, 1], 2)]
+
+
+def best_saving(t):
+    """Most page reads that any division of the rows into groups saves, by trying them all."""
+    n = len(t)
+
+    def run(rows):
+        k = 0
+        while k < t.shape[1] and t[rows[0], k] >= 0 and all(t[r, k] == t[rows[0], k] for r in rows):
+            k += 1
+        return k
+
+    best = 0
+    for size in range(2, n + 1):
+        for rows in itertools.combinations(range(n), size):
+            best = max(best, (size - 1) * run(rows))
+    return best
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_the_first_group_saves_most_and_groups_are_true(seed):
+    rng = random.Random(seed)
+    rows = []
+    for _ in range(rng.randint(2, 7)):                       # paths of a small random tree
+        rows.append([10 * d + rng.randint(0, 1 + d // 3) for d in range(rng.randint(0, 6))])
+    t = table(*rows)
+    groups = common_runs(t)
+    seen = [r for g, _ in groups for r in g]
+    assert len(seen) == len(set(seen))
+    for members, pages in groups:
+        assert len(members) > 1 and pages > 0
+        assert all((t[m, :pages] == t[members[0], :pages]).all() and (t[m, :pages] >= 0).all() for m in members)
+    assert max([(len(m) - 1) * p for m, p in groups], default=0) == best_saving(t)
+
+
+@pytest.mark.parametrize("seed", range(20))
+def test_items_cover_every_prefix_once(seed):
+    rng = random.Random(seed)
+    P = rng.choice([32, 64, 128])
+    kind, heads, kv = rng.choice([("grouped", 16, 4), ("grouped", 6, 2), ("latent", 16, 1), ("latent", 5, 1)])
+    rows = rng.randint(2, 90)
+    width = 80
+    t = np.full((rows + 4, width), -1, dtype=np.int32)
+    pages = iter(rng.sample(range(100000), 20000))
+    slots = rng.sample(range(rows + 4), rows)
+    parts = [[next(pages) for _ in range(rng.randint(1, 70))] for _ in range(rng.randint(1, 4))]
+    for s in slots:
+        lead = rng.choice(parts + [[]])
+        row = lead + [next(pages) for _ in range(rng.randint(1, width - len(lead)))]
+        t[s, :len(row)] = row
+    row_slots = [s if rng.random() < 0.9 else -1 for s in slots]
+    plan = PrefixPlan(kind, rows=rows, heads=heads, kv_heads=kv, vdim=64, page_tokens=P, device="cpu")
+    plan.set(row_slots, torch.from_numpy(t))
+    d = plan.data.numpy()
+    items, order, own, cell, count = (d[a:b] for a, b in zip(plan._at, plan._at[1:] + [len(d)]))
+    assert d[0] == plan.n_items <= plan.max_items
+    covered = {}
+    for slot, first, n, k0, k1, part, _, _ in items[:8 * plan.n_items].reshape(-1, 8):
+        assert 0 < n <= plan.rows_per_item and 0 <= k0 < k1 and k0 % P == 0 and k1 % P == 0
+        for r in order[first:first + n]:
+            assert (t[row_slots[r], :k1 // P] == t[slot, :k1 // P]).all() and row_slots[r] >= 0
+            assert part < count[r] and cell[r] + count[r] <= plan.max_cells
+            covered.setdefault(int(r), []).append((int(k0), int(k1), int(part)))
+    for r in range(rows):
+        got = sorted(covered.get(r, []))
+        assert [x[2] for x in got] == list(range(count[r]))
+        assert [x[0] for x in got] + [own[r]] == [0] + [x[1] for x in got]          # adjacent, from 0 to the row's own keys
+    used = [c for r in covered for c in range(cell[r], cell[r] + count[r])]
+    assert len(used) == len(set(used))                                                # no cell has two writers
+
+
+def test_a_new_plan_replaces_the_old_one_whole():
+    t = table([1, 2, 3, 4], [1, 2, 3, 5], [9, 8])
+    plan = PrefixPlan("grouped", rows=3, heads=4, kv_heads=2, vdim=16, page_tokens=64, device="cpu")
+    plan.set([0, 1, 2], t)
+    assert plan.n_items > 0 and plan.shared == [([0, 1], 192)]
+    plan.set([0, 2], t)
+    assert plan.n_items == 0 and plan.shared == [] and int(plan.data.abs().sum()) == 0
+
+
+def test_rows_of_one_slot_share_with_other_slots_only():
+    t = table([1, 2, 3, 4], [1, 2, 3, 5])
+    plan = PrefixPlan("latent", rows=4, heads=4, vdim=16, page_tokens=64, device="cpu")
+    plan.set([0, 0, 0], t)
+    assert plan.shared == []
+    plan.set([0, 0, 1, -1], t)
+    assert plan.shared == [([0, 1, 2], 192)]
+
+
+def test_short_prefixes_are_left_to_the_rows():
+    t = table([1, 2], [1, 3])
+    plan = PrefixPlan("grouped", rows=2, heads=4, kv_heads=2, vdim=16, page_tokens=32, device="cpu", min_tokens=64)
+    plan.set([0, 1], t)
+    assert plan.shared == [] and plan.n_items == 0
+
+
+def test_key_ranges_fill_one_wave_and_stay_within_the_parts_of_a_row():
+    assert key_span([(1, 4096)], 18, 128) == 256              # 16 ranges of 18
+    for pieces, keys in ((1, 100), (3, 100000), (40, 5000), (200, 300), (1, 1 << 24)):
+        span = key_span([(pieces, keys)], 37, 128)
+        assert span >= 1 and -(-keys // span) <= prefix.MAX_PARTS
+
+
+@pytest.mark.parametrize("kw", [dict(kind="other"), dict(heads=0), dict(heads=6, kv_heads=4), dict(vdim=24), dict(rows=0),
+                                dict(kind="latent", kv_heads=2), dict(dtype=torch.float16), dict(page_tokens=0)])
+def test_plans_refuse_what_they_cannot_describe(kw):
+    args = dict(kind="grouped", rows=4, heads=8, kv_heads=2, vdim=32, page_tokens=64, device="cpu")
+    args.update(kw)
+    if args["kind"] == "latent" and "kv_heads" not in kw:
+        args["kv_heads"] = 1
+    with pytest.raises(ValueError):
+        PrefixPlan(args.pop("kind"), **args)
+
+
+@pytest.mark.parametrize("slots,tables", [([0] * 5, table([1])), ([1], table([1])), ([0], table([1]).astype(np.int64)),
+                                          ([0], table([1])[0]), ([[0]], table([1]))])
+def test_plans_refuse_rows_and_tables_that_do_not_fit(slots, tables):
+    plan = PrefixPlan("grouped", rows=4, heads=8, kv_heads=2, vdim=32, page_tokens=64, device="cpu")
+    with pytest.raises(ValueError):
+        plan.set(slots, tables)
+
+
+def call(kind="grouped", **change):
+    """A call that is right but for its device (everything lies on the CPU), with some arguments changed."""
+    H, D, V, P, R = 8, 32, 32, 64, 3
+    G = 2 if kind == "grouped" else 1
+    plan = PrefixPlan(kind, rows=4, heads=H, kv_heads=G, vdim=V, page_tokens=P, device="cpu")
+    z = lambda *s, dtype=BF16: torch.zeros(*s, dtype=dtype)
+    a = dict(page_table=z(4, 5, dtype=torch.int32), row_pos=z(R, dtype=torch.int32), row_slot=z(R, dtype=torch.int32), plan=plan,
+             scale=1.0, out=z(R, H, V))
+    if kind == "grouped":
+        a.update(q=z(R, H, D), pool=z(10 * P, G * (D + V)), gate=z(R, H, dtype=torch.float32))
+        fn = prefix.group_attend
+    else:
+        a.update(q_abs=z(R, H, V), q_rot=z(R, H, 16), pool=z(10 * P, V + 16), sink=z(H, dtype=torch.float32))
+        fn = prefix.latent_attend
+    for k, v in change.items():
+        a[k] = v(a[k]) if callable(v) else v
+    return fn(**a)
+
+
+COMMON = [
+    (dict(page_table=lambda t: t.long()), "32-bit"), (dict(row_pos=lambda t: t.float()), "32-bit"),
+    (dict(row_slot=lambda t: t[:2]), "entry per row"), (dict(page_table=lambda t: t[0]), "slots, pages"),
+    (dict(page_table=lambda t: t.t()), "contiguous"), (dict(pool=lambda t: t[:100]), "whole pages"),
+    (dict(pool=lambda t: t[:, :-1]), "contiguous rows"), (dict(pool=lambda t: t.float()), "pool is"),
+    (dict(out=lambda t: t[:2]), "out must be"), (dict(out=lambda t: t.float()), "out is"),
+    (dict(out=lambda t: t.transpose(0, 1)), "out must be"), (dict(), "current CUDA device"),
+]
+
+
+@pytest.mark.parametrize("kind", ["grouped", "latent"])
+@pytest.mark.parametrize("change,why", COMMON)
+def test_calls_refuse_what_does_not_fit(kind, change, why):
+    if not change and torch.cuda.is_available():
+        pytest.skip("the device check is the one that is asked here")
+    with pytest.raises(ValueError, match=why):
+        call(kind, **change)
+
+
+@pytest.mark.parametrize("change", [
+    dict(q=lambda t: t.float()), dict(q=lambda t: t[:, :4]), dict(q=lambda t: t[..., :24]), dict(q=lambda t: t[..., ::2]),
+    dict(q=lambda t: t[0]), dict(q=lambda t: torch.zeros(5, 8, 32, dtype=BF16)), dict(q=lambda t: torch.zeros(0, 8, 32, dtype=BF16)),
+    dict(q=lambda t: torch.zeros(3 * 8 * 32 + 1, dtype=BF16)[1:].view(3, 8, 32)), dict(q=lambda t: t[:1].expand(3, 8, 32)),
+    dict(q=lambda t: torch.zeros(3, 8, 48, dtype=BF16)[..., :32]),
+    dict(gate=lambda t: t.to(BF16)), dict(gate=lambda t: t[:2]), dict(gate=lambda t: t.t().contiguous().t()), dict(chunk=-1),
+    dict(plan=lambda p: PrefixPlan("latent", rows=4, heads=8, vdim=32, page_tokens=64, device="cpu"))])
+def test_grouped_calls_refuse(change):
+    with pytest.raises(ValueError):
+        call("grouped", **change)
+
+
+@pytest.mark.parametrize("change", [
+    dict(q_abs=lambda t: t[..., :16]), dict(q_abs=lambda t: t.float()), dict(q_rot=lambda t: t[:2]), dict(q_rot=lambda t: t[..., :8]),
+    dict(q_rot=None), dict(sink=lambda t: t[:4]), dict(sink=lambda t: t.to(BF16)), dict(sink=lambda t: torch.zeros(16)[::2]),
+    dict(plan=lambda p: PrefixPlan("grouped", rows=4, heads=8, kv_heads=1, vdim=32, page_tokens=64, device="cpu"))])
+def test_latent_calls_refuse(change):
+    with pytest.raises(ValueError):
+        call("latent", **change)
