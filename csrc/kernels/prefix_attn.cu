@@ -9,6 +9,8 @@
 
 namespace ds41 {
 
+int launch_prefix_group(const ds41_group_attend_args& a, const ds41_prefix_plan& plan, cudaStream_t st);
+
 constexpr int kSimpleQueries = 16;
 constexpr int kSimpleKeys = 32;
 
@@ -272,6 +274,8 @@ extern "C" int ds41_prefix_group_shared(const ds41_group_attend_args* a, const d
       a->page_tokens <= 0 || a->q == nullptr || a->pool == nullptr || a->page_table == nullptr || a->row_pos == nullptr ||
       a->row_slot == nullptr || a->ld_q < 1ll * a->heads * a->dim_pad)
     return cudaErrorInvalidValue;
+  const int done = launch_prefix_group(*a, *plan, static_cast<cudaStream_t>(stream));
+  if (done != cudaErrorNotSupported) return done;
   SimpleArgs p{};
   p.q = a->q; p.q2 = a->q; p.pool = a->pool;
   p.page_table = a->page_table; p.row_pos = a->row_pos; p.row_slot = a->row_slot;

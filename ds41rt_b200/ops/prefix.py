@@ -81,7 +81,7 @@ def key_span(work: Sequence[Tuple[int, int]], budget: int, unit: int) -> int:
         cost = waves * (lo * unit + ITEM_COST)
         if best is None or cost < best[0]:
             best = (cost, lo * unit)
-    return max(best[1] if best else longest, -(-longest // MAX_PARTS))
+    return max(best[1] if best else longest, -(-longest // (MAX_PARTS * unit)) * unit)
 
 
 ITEM_COST = 512          # fixed cost of an item, in keys
