@@ -10,6 +10,7 @@
 namespace ds41 {
 
 int launch_prefix_group(const ds41_group_attend_args& a, const ds41_prefix_plan& plan, cudaStream_t st);
+int launch_prefix_latent(const ds41_latent_attend_args& a, const ds41_prefix_plan& plan, int n_pages, cudaStream_t st);
 
 constexpr int kSimpleQueries = 16;
 constexpr int kSimpleKeys = 32;
@@ -294,6 +295,8 @@ extern "C" int ds41_prefix_latent_shared(const ds41_latent_attend_args* a, const
       (a->row_len > a->kv_pad && a->q_rot == nullptr) || a->pool == nullptr || a->page_table == nullptr || a->row_pos == nullptr ||
       a->row_slot == nullptr)
     return cudaErrorInvalidValue;
+  const int done = launch_prefix_latent(*a, *plan, n_pages, static_cast<cudaStream_t>(stream));
+  if (done != cudaErrorNotSupported) return done;
   SimpleArgs p{};
   p.q = a->q_abs; p.q2 = a->q_rot; p.pool = a->pool;
   p.page_table = a->page_table; p.row_pos = a->row_pos; p.row_slot = a->row_slot;

@@ -1,0 +1,465 @@
+// Latent attention over the common keys of rows that share a prefix, on tcgen05.
+//
+// Every head reads the same key rows, so the (row, head) pairs of an item's rows are packed into the 128 rows of a tensor-core tile.
+// A key row is [latent | rotated part], the latent being the value as well: with 512 latent values the result of 128 queries alone
+// would fill the 512 columns of a CTA's tensor memory.  So two CTAs of a cluster divide the columns of queries, keys and values between
+// them: each multiplies its half of the columns, S = S_0 + S_1, they exchange these partial scores through distributed shared memory,
+// both compute the whole softmax (the sum of two numbers is the same in either order, so they agree bit for bit), and each
+// accumulates its half of the values from the key tile that it has loaded.  No product and no load is made twice.  Up to 256 latent
+// values fit one CTA.
+//   tensor memory : O 256 columns, Q 160 (the first product's A operand: it never touches shared memory again), S 64, P 32
+//   shared memory : a ring of tiles of 64 keys (up to five chunks of 64 columns), two buffers for the other CTA's scores
+//   warps 0-3, 4-7: columns 0-31 / 32-63 of a tile's scores, one thread per query in each half: exchange, softmax, partial results
+//   warp 8        : TMA producer, page by page
+//   warp 9        : tcgen05.mma issue: S = Q K^T of the next tile while this tile's softmax runs, then O += P V
+// The running maximum is raised when it grew by more than 2^8 only.  P is rounded to bf16 as the operand of the second product; sums
+// stay in 32 bits.
+#include <cuda.h>
+
+#include "ds41_prefix.cuh"
+#include "ds41_tma.h"
+
+namespace ds41 {
+
+constexpr int kPlThreads = 320;
+constexpr int kPlQueries = 128, kPlKeys = 64;
+constexpr int kPlChunk = kPlKeys * 128;        // bytes of 64 keys x 64 bf16 columns
+constexpr int kPlMost = 5;                     // chunks of columns of a CTA
+constexpr int kPlStages = 8;
+constexpr uint32_t kPlQ = 256, kPlS = 416, kPlP = 480;      // columns of tensor memory behind O
+
+struct PrefixLatentParams {
+  const __nv_bfloat16 *q_abs, *q_rot;
+  const int *page_table, *row_pos, *row_slot;
+  long long ld_q_abs, ld_q_rot;
+  int q_rot_stride, heads, kvp, rp;
+  int chunks, stages;                                       // of a stage, of the ring
+  int v_col[3], rot_step[3];                                // CTA c: latent columns [v_col[c], v_col[c + 1]), rotated steps of 16 likewise
+  int max_pages, page_tokens, box, hidden_row;
+  float scale_log2;
+  int* status;
+};
+
+// ------------------------------------------------------------------ cluster helpers
+__device__ __forceinline__ void remote_store(uint32_t addr, float a, float b, float c, float d) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
+}
+__device__ __forceinline__ void remote_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred P;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 P, [%1], %2;\n\t"
+      "selp.b32 %0, 1, 0, P;\n\t}"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+// mbar_wait for what the other CTA has written (bounded like it)
+__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, int* status, int where) {
+  if (try_wait_cluster(bar, parity)) return true;
+  const long long start = clock64();
+  uint32_t spins = 0;
+  while (!try_wait_cluster(bar, parity)) {
+    if ((++spins & 0x3ff) == 0 && (clock64() - start > DS41_WAIT_LIMIT_CYCLES ||
+                                   (status != nullptr && *reinterpret_cast<volatile int*>(status) != kStatusOk))) {
+      if (status != nullptr && atomicCAS(status, kStatusOk, kStatusMbarTimeout) == kStatusOk) {
+        status[1] = where;
+        status[2] = static_cast<int>(blockIdx.x);
+        status[3] = static_cast<int>(parity);
+      }
+      return false;
+    }
+  }
+  return true;
+}
+__device__ __forceinline__ void cluster_meet() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <bool PAIR>
+__global__ void __launch_bounds__(kPlThreads, 1)
+prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLatentParams p, const ds41_prefix_plan plan) {
+  extern __shared__ __align__(1024) uint8_t pl_smem[];       // no room to align it here: four stages leave 800 bytes
+  uint8_t* smem = pl_smem;
+  const int stage_bytes = p.chunks * kPlChunk;
+  uint8_t* s_kv = smem;
+  float* s_x = reinterpret_cast<float*>(s_kv + p.stages * stage_bytes);      // [2][16 columns of four][128 queries][4]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_x + (PAIR ? 2 * kPlKeys * kPlQueries : 0));
+  uint64_t* kv_full = bars;                                  // [stages]
+  uint64_t* kv_empty = kv_full + kPlStages;
+  uint64_t* q_full = kv_empty + kPlStages;
+  uint64_t* s_full = q_full + 1;                             // S complete
+  uint64_t* s_free = s_full + 1;                             // S read by all eight warps
+  uint64_t* p_full = s_free + 1;                             // P written, O rescaled
+  uint64_t* pv_done = p_full + 1;                            // O += P V complete
+  uint64_t* x_full = pv_done + 1;                            // [2] the other CTA's scores are here
+  uint64_t* x_free = x_full + 2;                             // [2] and have been read there
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(x_free + 2);
+  float* s_top = reinterpret_cast<float*>(tmem_slot + 2);    // [2][2][128] maxima of the two halves, by tile parity
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = PAIR ? static_cast<int>(blockIdx.x & 1) : 0;
+
+  pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kPlStages; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
+    }
+    mbar_init(q_full, 8);
+    mbar_init(s_full, 1);
+    mbar_init(s_free, 8);
+    mbar_init(p_full, 8);
+    mbar_init(pv_done, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&x_full[i], 8);
+      mbar_init(&x_free[i], 8);
+    }
+    mbar_init_fence();
+    tma_prefetch_desc(&pool);
+  }
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (PAIR) cluster_meet();                                  // the other CTA's barriers are ready, too
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+
+  const int units = *plan.n_items, first_unit = PAIR ? blockIdx.x >> 1 : blockIdx.x, unit_step = PAIR ? gridDim.x >> 1 : gridDim.x;
+  const int v0 = p.v_col[rank], v1 = p.v_col[rank + 1], r0 = p.rot_step[rank], r1 = p.rot_step[rank + 1];
+  const int v_chunks = (v1 - v0 + 63) / 64, r_chunk0 = r0 >> 2, r_chunks = r1 > r0 ? (r1 + 3) / 4 - r_chunk0 : 0;
+
+  if (warp == 8) {
+    const int boxes = kPlKeys / p.box;
+    int kt = 0;
+    bool ok = true;
+    for (int unit = first_unit; unit < units && ok; unit += unit_step) {
+      const PrefixItem it = prefix_item(plan, unit);
+      const int n = (it.key1 - it.key0 + kPlKeys - 1) / kPlKeys;
+      const int* table = p.page_table + 1ll * it.slot * p.max_pages;
+      int row = 0, u = 0;
+      for (int j = 0; j < n; ++j, ++kt) {
+        int at[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i < boxes) {
+            if ((u & 31) == 0) {                             // lane i: pool row of box i of the walk, 32 boxes at a time
+              const int key = it.key0 + (u + lane) * p.box, pg = key / p.page_tokens;
+              const int id = key < it.key1 && pg < p.max_pages ? table[pg] : -1;
+              row = id >= 0 ? id * p.page_tokens + (key - pg * p.page_tokens) : p.hidden_row;
+            }
+            at[i] = __shfl_sync(0xffffffffu, row, u & 31);
+            ++u;
+          }
+        const int stage = kt % p.stages;
+        ok = __all_sync(0xffffffffu, mbar_wait(&kv_empty[stage], ((kt / p.stages) & 1) ^ 1, p.status, 500)) != 0;
+        if (!ok) break;
+        if (lane == 0) {
+          uint8_t* dst = s_kv + stage * stage_bytes;
+          mbar_expect_tx(&kv_full[stage], (v_chunks + r_chunks) * kPlChunk);
+          for (int c = 0; c < v_chunks + r_chunks; ++c) {
+            const int x = c < v_chunks ? v0 + 64 * c : p.kvp + 64 * (r_chunk0 + c - v_chunks);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (i < boxes) tma_load_3d(dst + c * kPlChunk + i * p.box * 128, &pool, &kv_full[stage], x, at[i], 0);
+          }
+        }
+        __syncwarp();
+      }
+    }
+    if (!ok && lane == 0)                                    // let the copies under way land before the shared memory goes away
+      for (int b = max(0, kt - p.stages); b < kt; ++b)
+        for (int i = 0; i < (1 << 18) && !mbar_test_wait(&kv_full[b % p.stages], (b / p.stages) & 1); ++i) {
+        }
+  } else if (warp == 9) {
+    const bool leader = elect_one();
+    const uint32_t idesc_s = umma_idesc(kPlQueries, kPlKeys, 1u, 1u);
+    const uint32_t idesc_pv = umma_idesc_bmn(kPlQueries, v1 - v0, 1u, 1u);
+    const uint64_t k_desc = umma_desc_sw128(smem_u32(s_kv)), v_desc = umma_desc_sw128_mn(smem_u32(s_kv), kPlChunk, 1024);
+    const int v_steps = (v1 - v0) / 16;
+    auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
+      const bool ok = mbar_wait(bar, parity, p.status, where);
+      return __all_sync(0xffffffffu, ok) != 0;
+    };
+    bool ok = true;
+    int kt = 0, live = 0;
+    auto scores = [&](int tile) {                            // S of a tile, once its keys are here and the last S has been read
+      const int stage = tile % p.stages;
+      if (!wait(&kv_full[stage], (tile / p.stages) & 1, 511)) return false;
+      if (tile > 0 && !wait(s_free, (tile - 1) & 1, 512)) return false;
+      tc_fence_after();
+      const uint64_t kd = k_desc + static_cast<uint64_t>(stage * stage_bytes / 16);
+      for (int k = 0; k < v_steps; ++k)
+        umma_bf16_ts_if(leader, tmem + kPlS, tmem + kPlQ + 8 * k, kd + static_cast<uint64_t>((k >> 2) * (kPlChunk / 16) + (k & 3) * 2),
+                        idesc_s, k > 0 ? 1u : 0u);
+      for (int k = r0; k < r1; ++k) {
+        const int x = 4 * v_chunks + k - 4 * r_chunk0;       // the step's place behind the value chunks
+        umma_bf16_ts_if(leader, tmem + kPlS, tmem + kPlQ + 8 * x, kd + static_cast<uint64_t>((x >> 2) * (kPlChunk / 16) + (x & 3) * 2),
+                        idesc_s, v_steps + k > r0 ? 1u : 0u);
+      }
+      tc_commit_if(leader, s_full);
+      return true;
+    };
+    for (int unit = first_unit; unit < units && ok; unit += unit_step) {
+      const PrefixItem it = prefix_item(plan, unit);
+      const int n = (it.key1 - it.key0 + kPlKeys - 1) / kPlKeys;
+      ok = wait(q_full, live & 1, 510);
+      ++live;
+      if (ok) {
+        tc_fence_after();
+        ok = scores(kt);
+      }
+      for (int j = 0; j < n && ok; ++j) {
+        if (j + 1 < n) ok = scores(kt + j + 1);
+        if (ok) ok = wait(p_full, (kt + j) & 1, 513);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t vd = v_desc + static_cast<uint64_t>((kt + j) % p.stages * stage_bytes / 16);
+#pragma unroll
+        for (int k = 0; k < kPlKeys / 16; ++k)
+          umma_bf16_ts_if(leader, tmem, tmem + kPlP + 8 * k, vd + 128 * k, idesc_pv, j == 0 && k == 0 ? 0u : 1u);
+        tc_commit_if(leader, &kv_empty[(kt + j) % p.stages]);
+        tc_commit_if(leader, pv_done);
+      }
+      kt += n;
+    }
+  } else {
+    const int half = warp >> 2, quad = warp & 3, mine = quad * 32 + lane;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    const uint32_t x_there = PAIR ? cluster_addr(smem_u32(s_x), rank ^ 1) : 0;
+    const uint32_t full_there = PAIR ? cluster_addr(smem_u32(x_full), rank ^ 1) : 0;
+    const uint32_t free_there = PAIR ? cluster_addr(smem_u32(x_free), rank ^ 1) : 0;
+    int kt = 0;
+    bool ok = true;
+    // loops run to their ends whatever happened: the two warps of a quadrant meet at barriers
+    for (int unit = first_unit; unit < units; unit += unit_step) {
+      const PrefixItem it = prefix_item(plan, unit);
+      const int n = (it.key1 - it.key0 + kPlKeys - 1) / kPlKeys;
+      int r = -1, hi = 0, h = 0;
+      if (mine < it.rows * p.heads) {
+        r = plan.order[it.first + mine / p.heads];
+        h = mine % p.heads;
+        if (p.row_slot[r] >= 0) hi = min(min(plan.own[r], p.row_pos[r] + 1), it.key1);
+      }
+      // queries into tensor memory: 32 values at a time, the two halves in turn
+      for (int c = half; c < 2 * (v_chunks + r_chunks); c += 2) {
+        uint32_t w[16];
+        const bool lat = c < 2 * v_chunks;
+        const int d0 = lat ? v0 + 32 * c : 64 * r_chunk0 + 32 * (c - 2 * v_chunks), width = lat ? v1 : p.rp;
+        const __nv_bfloat16* src = r < 0 ? nullptr
+                                   : lat ? p.q_abs + r * p.ld_q_abs + 1ll * h * p.kvp + d0
+                                         : p.q_rot + r * p.ld_q_rot + 1ll * h * p.q_rot_stride + d0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (src != nullptr && d0 + 8 * i < width) v = *reinterpret_cast<const uint4*>(src + 8 * i);
+          w[4 * i] = v.x;
+          w[4 * i + 1] = v.y;
+          w[4 * i + 2] = v.z;
+          w[4 * i + 3] = v.w;
+        }
+        __syncwarp();
+        tmem_st_32x16(lanes + kPlQ + 16 * c, w);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+      int high = hi > 0 ? hi : 0x7fffffff;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) high = min(high, __shfl_xor_sync(0xffffffffu, high, o));
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < n; ++j, ++kt) {
+        const int buf = kt & 1, use = kt >> 1;
+        float s[32];
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(s_full, kt & 1, p.status, 520)) != 0;
+        if (ok) {
+          tc_fence_after();
+          uint32_t v[32];
+          tmem_ld_32x32(lanes + kPlS + 32 * half, v);
+          tmem_wait_ld();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(s_free);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) s[i] = __uint_as_float(v[i]);
+          if (PAIR) {
+            // [buffer][column / 4][query]: neighbouring lanes, neighbouring 16 bytes
+            const uint32_t at = 16u * (static_cast<uint32_t>((16 * buf + 8 * half) * kPlQueries) + mine);
+            if (use > 0) ok = __all_sync(0xffffffffu, wait_cluster(&x_free[buf], (use - 1) & 1, p.status, 521)) != 0;
+            if (ok) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) remote_store(x_there + at + 16 * kPlQueries * i, s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
+              __syncwarp();
+              if (lane == 0) remote_arrive(full_there + 8 * buf);
+              ok = __all_sync(0xffffffffu, wait_cluster(&x_full[buf], use & 1, p.status, 522)) != 0;
+            }
+            if (ok) {
+              const float4* x = reinterpret_cast<const float4*>(s_x) + (16 * buf + 8 * half) * kPlQueries + mine;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float4 y = x[i * kPlQueries];
+                s[4 * i] += y.x;
+                s[4 * i + 1] += y.y;
+                s[4 * i + 2] += y.z;
+                s[4 * i + 3] += y.w;
+              }
+              __syncwarp();
+              if (lane == 0) remote_arrive(free_there + 8 * buf);
+            }
+          }
+        }
+        const int key0 = it.key0 + j * kPlKeys + 32 * half;
+        const bool edge = it.key0 + (j + 1) * kPlKeys > high;
+        const int shown = hi - key0;
+        float top = -INFINITY;
+        if (ok) {
+          if (edge) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) s[i] = i < shown ? s[i] : -INFINITY;
+          }
+#pragma unroll
+          for (int i = 0; i < 32; ++i) top = fmaxf(top, s[i]);
+          top *= p.scale_log2;
+        }
+        s_top[(2 * buf + half) * kPlQueries + mine] = top;
+        named_barrier(1 + quad, 64);
+        if (!ok) continue;
+        top = fmaxf(top, s_top[(2 * buf + (half ^ 1)) * kPlQueries + mine]);
+        const bool grow = top > m + 8.f || (m == -INFINITY && top > m);
+        if (kt > 0) ok = __all_sync(0xffffffffu, mbar_wait(pv_done, (kt - 1) & 1, p.status, 523)) != 0;
+        if (!ok) continue;
+        tc_fence_after();
+        if (__any_sync(0xffffffffu, grow)) {
+          const float m_new = grow ? top : m, keep = grow ? (m == -INFINITY ? 0.f : ex2_approx(m - m_new)) : 1.f;
+          l *= keep;
+          m = m_new;
+          if (j > 0) {
+            const int cols = (v1 - v0) / 32 * 16;              // the two halves share the columns
+            for (int c = half ? cols : 0; c < (half ? v1 - v0 : cols); c += 16) {
+              uint32_t o[16];
+              tmem_ld_32x16(lanes + c, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
+              tmem_st_32x16(lanes + c, o);
+            }
+          }
+        }
+        const float neg = m == -INFINITY ? 0.f : -m;
+        uint32_t w[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float a = ex2_approx(fmaf(s[2 * i], p.scale_log2, neg)), b = ex2_approx(fmaf(s[2 * i + 1], p.scale_log2, neg));
+          l += a + b;
+          const __nv_bfloat162 q = __floats2bfloat162_rn(a, b);
+          w[i] = *reinterpret_cast<const uint32_t*>(&q);
+        }
+        tmem_st_32x16(lanes + kPlP + 16 * half, w);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full);
+      }
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(pv_done, (kt - 1) & 1, p.status, 524)) != 0;
+      tc_fence_after();
+      // the halves' sums, in the buffer of maxima that the last tile did not use
+      s_top[(2 * (kt & 1) + half) * kPlQueries + mine] = l;
+      named_barrier(1 + quad, 64);
+      l += s_top[(2 * (kt & 1) + (half ^ 1)) * kPlQueries + mine];
+      if (ok) {
+        const bool write = r >= 0, seen = hi > it.key0;
+        const long long cell = write ? (1ll * plan.cell[r] + it.split) * p.heads + h : 0;
+        if (write && half == 0 && rank == 0)
+          *reinterpret_cast<float2*>(plan.part_ml + 2 * cell) =
+              make_float2(seen ? m * 0.6931471805599453f : -INFINITY, seen ? l : 0.f);
+        float* dst = plan.part_o + cell * p.kvp + v0;
+        const int cols = (v1 - v0) / 32 * 16;
+        for (int c = half ? cols : 0; c < (half ? v1 - v0 : cols); c += 16) {
+          uint32_t o[16];
+          tmem_ld_32x16(lanes + c, o);
+          tmem_wait_ld();
+          if (write) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+              *reinterpret_cast<float4*>(dst + c + i) = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]),
+                                                                    __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
+          }
+          __syncwarp();
+        }
+      }
+      tc_fence_before();
+      named_barrier(1 + quad, 64);                             // the buffers of maxima may be written again
+    }
+  }
+  __syncthreads();
+  if (PAIR) cluster_meet();                                    // nothing of this CTA's memory is written or signalled any more
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <bool PAIR>
+static int launch_form(const CUtensorMap& pool, const PrefixLatentParams& p, const ds41_prefix_plan& plan, int smem, cudaStream_t st) {
+  const cudaError_t e = cudaFuncSetAttribute(prefix_latent_kernel<PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  if (!PAIR) return launch_pdl(prefix_latent_kernel<PAIR>, dim3(plan.grid), dim3(kPlThreads), smem, st, pool, p, plan);
+  const int pairs = plan.grid < sm_count() / 2 ? plan.grid : sm_count() / 2;
+  return launch_pdl_cluster(prefix_latent_kernel<PAIR>, dim3(2 * pairs), dim3(kPlThreads), 2, smem, st, pool, p, plan);
+}
+
+// cudaErrorNotSupported: these sizes are for the simple form
+int launch_prefix_latent(const ds41_latent_attend_args& a, const ds41_prefix_plan& plan, int n_pages, cudaStream_t st) {
+  const int rp = a.row_len - a.kv_pad, v_chunks = (a.kv_pad + 63) / 64;
+  if (a.f32 || (a.kv_pad & 15) || (rp & 15) || a.kv_pad > 512 || plan.rows_per_item * a.heads > kPlQueries || (a.ld_q_abs & 7) ||
+      (a.ld_q_rot & 7) || (a.q_rot_stride & 7) || 1ll * n_pages * a.page_tokens >= (1ll << 31) - 1 ||
+      ((reinterpret_cast<uintptr_t>(a.q_abs) | reinterpret_cast<uintptr_t>(a.q_rot) | reinterpret_cast<uintptr_t>(a.pool)) & 15))
+    return cudaErrorNotSupported;
+  PrefixLatentParams p{};
+  if (a.page_tokens % kPlKeys == 0) p.box = kPlKeys;
+  else if (kPlKeys % a.page_tokens == 0 && a.page_tokens >= 8) p.box = a.page_tokens;
+  else return cudaErrorNotSupported;
+  const bool pair = v_chunks > 4 || v_chunks + (rp + 63) / 64 > kPlMost;
+  const int r_steps = rp / 16;
+  p.v_col[1] = pair ? (v_chunks + 1) / 2 * 64 : a.kv_pad;
+  if (p.v_col[1] > a.kv_pad) p.v_col[1] = a.kv_pad;
+  p.v_col[2] = a.kv_pad;
+  // the rotated steps go where they balance the first product
+  int first = (a.kv_pad / 16 + r_steps) / 2 - p.v_col[1] / 16;
+  first = first < 0 ? 0 : (first > r_steps ? r_steps : first);
+  p.rot_step[1] = pair ? first : r_steps;
+  p.rot_step[2] = r_steps;
+  for (int c = 0; c < (pair ? 2 : 1); ++c) {
+    const int r0 = p.rot_step[c], r1 = p.rot_step[c + 1];
+    const int n = (p.v_col[c + 1] - p.v_col[c] + 63) / 64 + (r1 > r0 ? (r1 + 3) / 4 - r0 / 4 : 0);
+    if (n > kPlMost || p.v_col[c + 1] <= p.v_col[c]) return cudaErrorNotSupported;
+    p.chunks = n > p.chunks ? n : p.chunks;
+  }
+  constexpr int kExtra = 8 * (2 * kPlStages + 9) + 8 + 4 * 4 * kPlQueries;
+  const int room = 227 * 1024 - kExtra - (pair ? 2 * 4 * kPlKeys * kPlQueries : 0);
+  p.stages = room / (p.chunks * kPlChunk);
+  if (p.stages > kPlStages) p.stages = kPlStages;
+  const int smem = kExtra + (pair ? 2 * 4 * kPlKeys * kPlQueries : 0) + p.stages * p.chunks * kPlChunk;
+  p.q_abs = static_cast<const __nv_bfloat16*>(a.q_abs);
+  p.q_rot = static_cast<const __nv_bfloat16*>(a.q_rot);
+  p.page_table = a.page_table; p.row_pos = a.row_pos; p.row_slot = a.row_slot;
+  p.ld_q_abs = a.ld_q_abs; p.ld_q_rot = a.ld_q_rot; p.q_rot_stride = a.q_rot_stride;
+  p.heads = a.heads; p.kvp = a.kv_pad; p.rp = rp;
+  p.max_pages = a.max_pages; p.page_tokens = a.page_tokens; p.hidden_row = n_pages * a.page_tokens;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.status = a.status;
+  CUtensorMap pool;
+  const cudaError_t e = make_tensor_map_3d(&pool, a.pool, TmaDtype::kBF16, a.row_len, p.hidden_row, 1, 2ull * a.row_len, 0, 64, p.box, true);
+  if (e != cudaSuccess) return e;
+  return pair ? launch_form<true>(pool, p, plan, smem, st) : launch_form<false>(pool, p, plan, smem, st);
+}
+
+}  // namespace ds41

@@ -108,7 +108,8 @@ class PrefixPlan:
         self.min_tokens = min_tokens
         per_lane = heads // kv_heads
         self.rows_per_item = max(1, (256 if kind == "grouped" else 128) // per_lane)
-        self.budget = max(1, (SMS if kind == "grouped" else SMS // 2) // kv_heads)
+        pair = kind == "latent" and vdim > 256               # two CTAs to an item
+        self.budget = max(1, (SMS // 2 if pair else SMS) // kv_heads)
         self.max_items = 2 * self.budget + rows
         self.max_cells = 2 * self.budget * min(self.rows_per_item, rows) + rows
         self.own_cells = rows * self._own_splits(rows, 1 << 30) if kind == "latent" else 0
