@@ -41,40 +41,11 @@ struct PrefixLatentParams {
 };
 
 // ------------------------------------------------------------------ cluster helpers
-__device__ __forceinline__ void remote_store(uint32_t addr, float a, float b, float c, float d) {
-  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
-}
-__device__ __forceinline__ void remote_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n\t.reg .pred P;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 P, [%1], %2;\n\t"
-      "selp.b32 %0, 1, 0, P;\n\t}"
-      : "=r"(done)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return done != 0;
-}
-// mbar_wait for what the other CTA has written (bounded like it)
-__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, int* status, int where) {
-  if (try_wait_cluster(bar, parity)) return true;
-  const long long start = clock64();
-  uint32_t spins = 0;
-  while (!try_wait_cluster(bar, parity)) {
-    if ((++spins & 0x3ff) == 0 && (clock64() - start > DS41_WAIT_LIMIT_CYCLES ||
-                                   (status != nullptr && *reinterpret_cast<volatile int*>(status) != kStatusOk))) {
-      if (status != nullptr && atomicCAS(status, kStatusOk, kStatusMbarTimeout) == kStatusOk) {
-        status[1] = where;
-        status[2] = static_cast<int>(blockIdx.x);
-        status[3] = static_cast<int>(parity);
-      }
-      return false;
-    }
-  }
-  return true;
+// Sixteen bytes into the other CTA's shared memory, counted by its barrier.
+__device__ __forceinline__ void remote_store(uint32_t addr, uint32_t bar, float a, float b, float c, float d) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%2, %3, %4, %5}, [%1];" ::"r"(addr), "r"(bar),
+               "f"(a), "f"(b), "f"(c), "f"(d)
+               : "memory");
 }
 __device__ __forceinline__ void cluster_meet() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -97,8 +68,7 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
   uint64_t* p_full = s_free + 1;                             // P written, O rescaled
   uint64_t* pv_done = p_full + 1;                            // O += P V complete
   uint64_t* x_full = pv_done + 1;                            // [2] the other CTA's scores are here
-  uint64_t* x_free = x_full + 2;                             // [2] and have been read there
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(x_free + 2);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(x_full + 2);
   float* s_top = reinterpret_cast<float*>(tmem_slot + 2);    // [2][2][128] maxima of the two halves, by tile parity
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = PAIR ? static_cast<int>(blockIdx.x & 1) : 0;
@@ -114,10 +84,7 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
     mbar_init(s_free, 8);
     mbar_init(p_full, 8);
     mbar_init(pv_done, 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&x_full[i], 8);
-      mbar_init(&x_free[i], 8);
-    }
+    for (int i = 0; i < 2; ++i) mbar_init(&x_full[i], 1);
     mbar_init_fence();
     tma_prefetch_desc(&pool);
   }
@@ -235,7 +202,6 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     const uint32_t x_there = PAIR ? cluster_addr(smem_u32(s_x), rank ^ 1) : 0;
     const uint32_t full_there = PAIR ? cluster_addr(smem_u32(x_full), rank ^ 1) : 0;
-    const uint32_t free_there = PAIR ? cluster_addr(smem_u32(x_free), rank ^ 1) : 0;
     int kt = 0;
     bool ok = true;
     // loops run to their ends whatever happened: the two warps of a quadrant meet at barriers
@@ -291,16 +257,14 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
 #pragma unroll
           for (int i = 0; i < 32; ++i) s[i] = __uint_as_float(v[i]);
           if (PAIR) {
-            // [buffer][column / 4][query]: neighbouring lanes, neighbouring 16 bytes
+            // [buffer][column / 4][query]: neighbouring lanes, neighbouring 16 bytes.  The buffer is free: the scores of the last tile
+            // came after the other CTA had read what this one sent for the tile before it.
             const uint32_t at = 16u * (static_cast<uint32_t>((16 * buf + 8 * half) * kPlQueries) + mine);
-            if (use > 0) ok = __all_sync(0xffffffffu, wait_cluster(&x_free[buf], (use - 1) & 1, p.status, 521)) != 0;
-            if (ok) {
+            if (threadIdx.x == 0) mbar_expect_tx(&x_full[buf], 4 * kPlKeys * kPlQueries);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) remote_store(x_there + at + 16 * kPlQueries * i, s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
-              __syncwarp();
-              if (lane == 0) remote_arrive(full_there + 8 * buf);
-              ok = __all_sync(0xffffffffu, wait_cluster(&x_full[buf], use & 1, p.status, 522)) != 0;
-            }
+            for (int i = 0; i < 8; ++i)
+              remote_store(x_there + at + 16 * kPlQueries * i, full_there + 8 * buf, s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
+            ok = __all_sync(0xffffffffu, mbar_wait(&x_full[buf], use & 1, p.status, 522)) != 0;
             if (ok) {
               const float4* x = reinterpret_cast<const float4*>(s_x) + (16 * buf + 8 * half) * kPlQueries + mine;
 #pragma unroll
@@ -311,8 +275,6 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
                 s[4 * i + 2] += y.z;
                 s[4 * i + 3] += y.w;
               }
-              __syncwarp();
-              if (lane == 0) remote_arrive(free_there + 8 * buf);
             }
           }
         }
