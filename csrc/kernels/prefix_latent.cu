@@ -9,9 +9,10 @@
 // values fit one CTA.
 //   tensor memory : O 256 columns, Q 160 (the first product's A operand: it never touches shared memory again), S 64, P 32
 //   shared memory : a ring of tiles of 64 keys (up to five chunks of 64 columns), two buffers for the other CTA's scores
-//   warps 0-3, 4-7: columns 0-31 / 32-63 of a tile's scores, one thread per query in each half: exchange, softmax, partial results
+//   warps 0-3, 4-7: even / odd tiles, one thread per query: exchange, softmax, partial results.  A tile's way from S to P is a chain of
+//                   latencies; two are under way, and hand the running maximum on as soon as a tile's own is known
 //   warp 8        : TMA producer, page by page
-//   warp 9        : tcgen05.mma issue: S = Q K^T of the next tile while this tile's softmax runs, then O += P V
+//   warp 9        : tcgen05.mma issue: S = Q K^T of the next tile as soon as this tile's S is in registers, then O += P V
 // The running maximum is raised when it grew by more than 2^8 only.  P is rounded to bf16 as the operand of the second product; sums
 // stay in 32 bits.
 #include <cuda.h>
@@ -47,6 +48,10 @@ __device__ __forceinline__ void remote_store(uint32_t addr, uint32_t bar, float 
                "f"(a), "f"(b), "f"(c), "f"(d)
                : "memory");
 }
+// The other CTA's barrier.  What was read before has been used by now, so nothing needs to be ordered but the arrival itself.
+__device__ __forceinline__ void remote_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 __device__ __forceinline__ void cluster_meet() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -54,7 +59,7 @@ __device__ __forceinline__ void cluster_meet() {
 template <bool PAIR>
 __global__ void __launch_bounds__(kPlThreads, 1)
 prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLatentParams p, const ds41_prefix_plan plan) {
-  extern __shared__ __align__(1024) uint8_t pl_smem[];       // no room to align it here: four stages leave 800 bytes
+  extern __shared__ __align__(1024) uint8_t pl_smem[];       // no room to align it here: four stages leave 200 bytes
   uint8_t* smem = pl_smem;
   const int stage_bytes = p.chunks * kPlChunk;
   uint8_t* s_kv = smem;
@@ -63,13 +68,17 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
   uint64_t* kv_full = bars;                                  // [stages]
   uint64_t* kv_empty = kv_full + kPlStages;
   uint64_t* q_full = kv_empty + kPlStages;
-  uint64_t* s_full = q_full + 1;                             // S complete
-  uint64_t* s_free = s_full + 1;                             // S read by all eight warps
+  uint64_t* s_free = q_full + 1;                             // S in registers
   uint64_t* p_full = s_free + 1;                             // P written, O rescaled
-  uint64_t* pv_done = p_full + 1;                            // O += P V complete
-  uint64_t* x_full = pv_done + 1;                            // [2] the other CTA's scores are here
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(x_full + 2);
-  float* s_top = reinterpret_cast<float*>(tmem_slot + 2);    // [2][2][128] maxima of the two halves, by tile parity
+  // by parity of the tile, as each half of the warps waits for every other one only:
+  uint64_t* s_full = p_full + 1;                             // [2] S complete
+  uint64_t* pv_done = s_full + 2;                            // [2] O += P V complete
+  uint64_t* x_full = pv_done + 2;                            // [2] the other CTA's scores are here
+  uint64_t* x_free = x_full + 2;                             // [2] this CTA's have been read there
+  uint64_t* known = x_free + 2;                              // [2][4] the maximum after a tile, by quadrant
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(known + 8);
+  float* s_top = reinterpret_cast<float*>(tmem_slot + 2);    // [128] the running maximum
+  float2* s_ml = reinterpret_cast<float2*>(s_top + kPlQueries);      // [2][128] the halves' maxima and sums
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = PAIR ? static_cast<int>(blockIdx.x & 1) : 0;
 
@@ -80,11 +89,15 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
       mbar_init(&kv_empty[i], 1);
     }
     mbar_init(q_full, 8);
-    mbar_init(s_full, 1);
-    mbar_init(s_free, 8);
-    mbar_init(p_full, 8);
-    mbar_init(pv_done, 1);
-    for (int i = 0; i < 2; ++i) mbar_init(&x_full[i], 1);
+    mbar_init(s_free, 4);
+    mbar_init(p_full, 4);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&pv_done[i], 1);
+      mbar_init(&x_full[i], 1);
+      mbar_init(&x_free[i], 4);
+      for (int q = 0; q < 4; ++q) mbar_init(&known[4 * i + q], 1);
+    }
     mbar_init_fence();
     tma_prefetch_desc(&pool);
   }
@@ -171,7 +184,7 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
         umma_bf16_ts_if(leader, tmem + kPlS, tmem + kPlQ + 8 * x, kd + static_cast<uint64_t>((x >> 2) * (kPlChunk / 16) + (x & 3) * 2),
                         idesc_s, v_steps + k > r0 ? 1u : 0u);
       }
-      tc_commit_if(leader, s_full);
+      tc_commit_if(leader, &s_full[tile & 1]);
       return true;
     };
     for (int unit = first_unit; unit < units && ok; unit += unit_step) {
@@ -193,18 +206,20 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
         for (int k = 0; k < kPlKeys / 16; ++k)
           umma_bf16_ts_if(leader, tmem, tmem + kPlP + 8 * k, vd + 128 * k, idesc_pv, j == 0 && k == 0 ? 0u : 1u);
         tc_commit_if(leader, &kv_empty[(kt + j) % p.stages]);
-        tc_commit_if(leader, pv_done);
+        tc_commit_if(leader, &pv_done[(kt + j) & 1]);
       }
       kt += n;
     }
   } else {
     const int half = warp >> 2, quad = warp & 3, mine = quad * 32 + lane;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-    const uint32_t x_there = PAIR ? cluster_addr(smem_u32(s_x), rank ^ 1) : 0;
-    const uint32_t full_there = PAIR ? cluster_addr(smem_u32(x_full), rank ^ 1) : 0;
+    const uint32_t x_there = PAIR ? cluster_addr(smem_u32(s_x + half * kPlKeys * kPlQueries) + 16 * mine, rank ^ 1) : 0;
+    const uint32_t full_there = PAIR ? cluster_addr(smem_u32(&x_full[half]), rank ^ 1) : 0;
+    const uint32_t free_there = PAIR ? cluster_addr(smem_u32(&x_free[half]), rank ^ 1) : 0;
+    const float* x_here = s_x + half * kPlKeys * kPlQueries;
     int kt = 0;
     bool ok = true;
-    // loops run to their ends whatever happened: the two warps of a quadrant meet at barriers
+    // the loop runs to its end whatever happened: the two warps of a quadrant meet at barriers
     for (int unit = first_unit; unit < units; unit += unit_step) {
       const PrefixItem it = prefix_item(plan, unit);
       const int n = (it.key1 - it.key0 + kPlKeys - 1) / kPlKeys;
@@ -241,71 +256,70 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
       int high = hi > 0 ? hi : 0x7fffffff;
 #pragma unroll
       for (int o = 16; o; o >>= 1) high = min(high, __shfl_xor_sync(0xffffffffu, high, o));
-      float m = -INFINITY, l = 0.f;
-      for (int j = 0; j < n; ++j, ++kt) {
-        const int buf = kt & 1, use = kt >> 1;
-        float s[32];
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(s_full, kt & 1, p.status, 520)) != 0;
-        if (ok) {
-          tc_fence_after();
-          uint32_t v[32];
-          tmem_ld_32x32(lanes + kPlS + 32 * half, v);
+      float m = -INFINITY, l = 0.f;                              // the maximum that l is relative to
+      for (int j = (kt ^ half) & 1; j < n && ok; j += 2) {
+        const int tile = kt + j, use = tile >> 1;
+        float s[kPlKeys];
+        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[half], use & 1, p.status, 520)) != 0;
+        if (!ok) break;
+        tc_fence_after();
+        {
+          uint32_t a[32], b[32];
+          tmem_ld_32x32(lanes + kPlS, a);
+          tmem_ld_32x32(lanes + kPlS + 32, b);
           tmem_wait_ld();
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(s_free);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) s[i] = __uint_as_float(v[i]);
-          if (PAIR) {
-            // [buffer][column / 4][query]: neighbouring lanes, neighbouring 16 bytes.  The buffer is free: the scores of the last tile
-            // came after the other CTA had read what this one sent for the tile before it.
-            const uint32_t at = 16u * (static_cast<uint32_t>((16 * buf + 8 * half) * kPlQueries) + mine);
-            if (threadIdx.x == 0) mbar_expect_tx(&x_full[buf], 4 * kPlKeys * kPlQueries);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              remote_store(x_there + at + 16 * kPlQueries * i, full_there + 8 * buf, s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
-            ok = __all_sync(0xffffffffu, mbar_wait(&x_full[buf], use & 1, p.status, 522)) != 0;
-            if (ok) {
-              const float4* x = reinterpret_cast<const float4*>(s_x) + (16 * buf + 8 * half) * kPlQueries + mine;
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const float4 y = x[i * kPlQueries];
-                s[4 * i] += y.x;
-                s[4 * i + 1] += y.y;
-                s[4 * i + 2] += y.z;
-                s[4 * i + 3] += y.w;
-              }
-            }
+          for (int i = 0; i < 32; ++i) {
+            s[i] = __uint_as_float(a[i]);
+            s[32 + i] = __uint_as_float(b[i]);
           }
         }
-        const int key0 = it.key0 + j * kPlKeys + 32 * half;
-        const bool edge = it.key0 + (j + 1) * kPlKeys > high;
-        const int shown = hi - key0;
-        float top = -INFINITY;
-        if (ok) {
-          if (edge) {
+        if (PAIR) {                                            // [column / 4][query]: neighbouring lanes, neighbouring 16 bytes
+          if (use > 0) ok = __all_sync(0xffffffffu, mbar_wait(&x_free[half], (use - 1) & 1, p.status, 521)) != 0;
+          if (!ok) break;
+          if (quad == 0 && lane == 0) mbar_expect_tx(&x_full[half], 4 * kPlKeys * kPlQueries);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) s[i] = i < shown ? s[i] : -INFINITY;
+          for (int i = 0; i < kPlKeys / 4; ++i)
+            remote_store(x_there + 16 * kPlQueries * i, full_there, s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
+          ok = __all_sync(0xffffffffu, mbar_wait(&x_full[half], use & 1, p.status, 522)) != 0;
+          if (!ok) break;
+          const float4* x = reinterpret_cast<const float4*>(x_here) + mine;
+#pragma unroll
+          for (int i = 0; i < kPlKeys / 4; ++i) {
+            const float4 y = x[i * kPlQueries];
+            s[4 * i] += y.x;
+            s[4 * i + 1] += y.y;
+            s[4 * i + 2] += y.z;
+            s[4 * i + 3] += y.w;
           }
-#pragma unroll
-          for (int i = 0; i < 32; ++i) top = fmaxf(top, s[i]);
-          top *= p.scale_log2;
         }
-        s_top[(2 * buf + half) * kPlQueries + mine] = top;
-        named_barrier(1 + quad, 64);
-        if (!ok) continue;
-        top = fmaxf(top, s_top[(2 * buf + (half ^ 1)) * kPlQueries + mine]);
-        const bool grow = top > m + 8.f || (m == -INFINITY && top > m);
-        if (kt > 0) ok = __all_sync(0xffffffffu, mbar_wait(pv_done, (kt - 1) & 1, p.status, 523)) != 0;
-        if (!ok) continue;
-        tc_fence_after();
+        const int key0 = it.key0 + j * kPlKeys;
+        if (key0 + kPlKeys > high) {                           // the tile holds keys that a query of this warp does not see
+          const int shown = hi - key0;
+#pragma unroll
+          for (int i = 0; i < kPlKeys; ++i) s[i] = i < shown ? s[i] : -INFINITY;
+        }
+        float top = s[0];
+#pragma unroll
+        for (int i = 1; i < kPlKeys; ++i) top = fmaxf(top, s[i]);
+        top *= p.scale_log2;
+        if (tile > 0) ok = __all_sync(0xffffffffu, mbar_wait(&known[4 * (half ^ 1) + quad], ((tile - 1) >> 1) & 1, p.status, 523)) != 0;
+        if (!ok) break;
+        float now = j > 0 ? s_top[mine] : -INFINITY;           // what O is relative to
+        const bool grow = top > now + 8.f || (now == -INFINITY && top > now);
+        bool last_done = tile == 0;
         if (__any_sync(0xffffffffu, grow)) {
-          const float m_new = grow ? top : m, keep = grow ? (m == -INFINITY ? 0.f : ex2_approx(m - m_new)) : 1.f;
-          l *= keep;
-          m = m_new;
+          const float next = grow ? top : now, keep = grow ? (now == -INFINITY ? 0.f : ex2_approx(now - next)) : 1.f;
           if (j > 0) {
-            const int cols = (v1 - v0) / 32 * 16;              // the two halves share the columns
-            for (int c = half ? cols : 0; c < (half ? v1 - v0 : cols); c += 16) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[half ^ 1], ((tile - 1) >> 1) & 1, p.status, 524)) != 0;
+            if (!ok) break;
+            last_done = true;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < v1 - v0; c += 16) {
               uint32_t o[16];
               tmem_ld_32x16(lanes + c, o);
               tmem_wait_ld();
@@ -313,29 +327,43 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
               for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
               tmem_st_32x16(lanes + c, o);
             }
+            tmem_wait_st();
+            tc_fence_before();
           }
+          now = next;
         }
+        s_top[mine] = now;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&known[4 * half + quad]);
+        if (now > m) l *= m == -INFINITY ? 0.f : ex2_approx(m - now);
+        m = now;
         const float neg = m == -INFINITY ? 0.f : -m;
-        uint32_t w[16];
+        uint32_t w[kPlKeys / 2];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
+        for (int i = 0; i < kPlKeys / 2; ++i) {
           const float a = ex2_approx(fmaf(s[2 * i], p.scale_log2, neg)), b = ex2_approx(fmaf(s[2 * i + 1], p.scale_log2, neg));
           l += a + b;
           const __nv_bfloat162 q = __floats2bfloat162_rn(a, b);
           w[i] = *reinterpret_cast<const uint32_t*>(&q);
         }
-        tmem_st_32x16(lanes + kPlP + 16 * half, w);
+        if (PAIR && lane == 0) remote_arrive(free_there);
+        if (!last_done) ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[half ^ 1], ((tile - 1) >> 1) & 1, p.status, 525)) != 0;
+        if (!ok) break;
+        tc_fence_after();
+        tmem_st_32x32(lanes + kPlP, w);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full);
       }
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(pv_done, (kt - 1) & 1, p.status, 524)) != 0;
+      kt += n;
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[(kt - 1) & 1], ((kt - 1) >> 1) & 1, p.status, 526)) != 0;
       tc_fence_after();
-      // the halves' sums, in the buffer of maxima that the last tile did not use
-      s_top[(2 * (kt & 1) + half) * kPlQueries + mine] = l;
+      s_ml[half * kPlQueries + mine] = make_float2(m, l);
       named_barrier(1 + quad, 64);
-      l += s_top[(2 * (kt & 1) + (half ^ 1)) * kPlQueries + mine];
+      const float2 ma = s_ml[mine], mb = s_ml[kPlQueries + mine];
+      m = fmaxf(ma.x, mb.x);                                     // the last one, as it only grows
+      l = (ma.x == -INFINITY ? 0.f : ma.y * ex2_approx(ma.x - m)) + (mb.x == -INFINITY ? 0.f : mb.y * ex2_approx(mb.x - m));
       if (ok) {
         const bool write = r >= 0, seen = hi > it.key0;
         const long long cell = write ? (1ll * plan.cell[r] + it.split) * p.heads + h : 0;
@@ -358,7 +386,7 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
         }
       }
       tc_fence_before();
-      named_barrier(1 + quad, 64);                             // the buffers of maxima may be written again
+      named_barrier(1 + quad, 64);                             // O, the maxima and the sums may be written again
     }
   }
   __syncthreads();
@@ -405,7 +433,7 @@ int launch_prefix_latent(const ds41_latent_attend_args& a, const ds41_prefix_pla
     if (n > kPlMost || p.v_col[c + 1] <= p.v_col[c]) return cudaErrorNotSupported;
     p.chunks = n > p.chunks ? n : p.chunks;
   }
-  constexpr int kExtra = 8 * (2 * kPlStages + 9) + 8 + 4 * 4 * kPlQueries;
+  constexpr int kExtra = 8 * (2 * kPlStages + 19) + 8 + 4 * 5 * kPlQueries;
   const int room = 227 * 1024 - kExtra - (pair ? 2 * 4 * kPlKeys * kPlQueries : 0);
   p.stages = room / (p.chunks * kPlChunk);
   if (p.stages > kPlStages) p.stages = kPlStages;

@@ -218,9 +218,12 @@ def own_cluster(rows: int, heads: int, kv_heads: int, tokens: int) -> int:
 
 
 # ---------------------------------------------------------------------------------------------------- front end
-def _check(plan: PrefixPlan, kind: str, q: torch.Tensor, pool, page_table, row_pos, row_slot, out, width: int, named) -> int:
+def _check(plan: PrefixPlan, kind: str, q: torch.Tensor, pool, page_table, row_pos, row_slot, out, width: int, scale: float,
+           named) -> int:
     if plan.kind != kind:
         raise ValueError(f"the plan is for {plan.kind} attention")
+    if not scale > 0:
+        raise ValueError("scale must be positive")
     R = q.shape[0]
     if not 0 < R <= plan.rows:
         raise ValueError(f"a pass has 1 to {plan.rows} rows, not {R}")
@@ -269,7 +272,8 @@ def group_attend(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, 
         raise ValueError("q: a row's heads must lie side by side")
     if out is None:
         out = torch.empty(R, H, plan.vdim, dtype=plan.dtype, device=q.device)
-    _check(plan, "grouped", q, pool, page_table, row_pos, row_slot, out, plan.kv_heads * (D + plan.vdim), (("q", q), ("gate", gate)))
+    _check(plan, "grouped", q, pool, page_table, row_pos, row_slot, out, plan.kv_heads * (D + plan.vdim), scale,
+           (("q", q), ("gate", gate)))
     if chunk < 0:
         raise ValueError("chunk must not be negative")
     if gate is not None and (gate.shape != (R, H) or gate.stride(1) != 1):
@@ -310,7 +314,8 @@ def latent_attend(q_abs: torch.Tensor, q_rot: Optional[torch.Tensor], pool: torc
     rot = 0 if q_rot is None else q_rot.shape[2]
     if out is None:
         out = torch.empty(R, H, V, dtype=plan.dtype, device=q_abs.device)
-    _check(plan, "latent", q_abs, pool, page_table, row_pos, row_slot, out, V + rot, (("q_abs", q_abs), ("q_rot", q_rot), ("sink", sink)))
+    _check(plan, "latent", q_abs, pool, page_table, row_pos, row_slot, out, V + rot, scale,
+           (("q_abs", q_abs), ("q_rot", q_rot), ("sink", sink)))
     if sink is not None and (sink.shape != (H,) or not sink.is_contiguous()):
         raise ValueError(f"sink must be {H} contiguous values")
     a = S.LatentAttendArgs()

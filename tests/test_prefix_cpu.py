@@ -182,7 +182,7 @@ COMMON = [
     (dict(page_table=lambda t: t.t()), "contiguous"), (dict(pool=lambda t: t[:100]), "whole pages"),
     (dict(pool=lambda t: t[:, :-1]), "contiguous rows"), (dict(pool=lambda t: t.float()), "pool is"),
     (dict(out=lambda t: t[:2]), "out must be"), (dict(out=lambda t: t.float()), "out is"),
-    (dict(out=lambda t: t.transpose(0, 1)), "out must be"), (dict(), "current CUDA device"),
+    (dict(out=lambda t: t.transpose(0, 1)), "out must be"), (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(), "current CUDA device"),
 ]
 
 
