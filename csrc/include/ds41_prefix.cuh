@@ -31,6 +31,23 @@ struct NoPrefix {};
 template <typename X>
 constexpr bool kHasPrefix = !std::is_same<X, NoPrefix>::value;
 
+// Two 32-bit operations in one instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)),
+        "l"(reinterpret_cast<unsigned long long&>(c)));
+  return d;
+}
+
 inline bool prefix_plan_ok(const ds41_prefix_plan* p) {
   return p != nullptr && p->items != nullptr && p->n_items != nullptr && p->order != nullptr && p->own != nullptr &&
          p->cell != nullptr && p->parts != nullptr && p->part_o != nullptr && p->part_ml != nullptr && p->max_items > 0 &&

@@ -124,34 +124,26 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
       const PrefixItem it = prefix_item(plan, unit);
       const int n = (it.key1 - it.key0 + kPlKeys - 1) / kPlKeys;
       const int* table = p.page_table + 1ll * it.slot * p.max_pages;
-      int row = 0, u = 0;
+      int row = 0, u = 0;                                    // lane i: pool row of box i of the walk, 32 boxes at a time
       for (int j = 0; j < n; ++j, ++kt) {
-        int at[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i < boxes) {
-            if ((u & 31) == 0) {                             // lane i: pool row of box i of the walk, 32 boxes at a time
-              const int key = it.key0 + (u + lane) * p.box, pg = key / p.page_tokens;
-              const int id = key < it.key1 && pg < p.max_pages ? table[pg] : -1;
-              row = id >= 0 ? id * p.page_tokens + (key - pg * p.page_tokens) : p.hidden_row;
-            }
-            at[i] = __shfl_sync(0xffffffffu, row, u & 31);
-            ++u;
-          }
         const int stage = kt % p.stages;
         ok = __all_sync(0xffffffffu, mbar_wait(&kv_empty[stage], ((kt / p.stages) & 1) ^ 1, p.status, 500)) != 0;
         if (!ok) break;
-        if (lane == 0) {
-          uint8_t* dst = s_kv + stage * stage_bytes;
-          mbar_expect_tx(&kv_full[stage], (v_chunks + r_chunks) * kPlChunk);
-          for (int c = 0; c < v_chunks + r_chunks; ++c) {
-            const int x = c < v_chunks ? v0 + 64 * c : p.kvp + 64 * (r_chunk0 + c - v_chunks);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (i < boxes) tma_load_3d(dst + c * kPlChunk + i * p.box * 128, &pool, &kv_full[stage], x, at[i], 0);
+        uint8_t* dst = s_kv + stage * stage_bytes;
+        mbar_expect_tx_if(lane == 0, &kv_full[stage], (v_chunks + r_chunks) * kPlChunk);
+#pragma unroll 1
+        for (int i = 0; i < boxes; ++i, ++u, dst += p.box * 128) {
+          if ((u & 31) == 0) {
+            const int key = it.key0 + (u + lane) * p.box, pg = key / p.page_tokens;
+            const int id = key < it.key1 && pg < p.max_pages ? table[pg] : -1;
+            row = id >= 0 ? id * p.page_tokens + (key - pg * p.page_tokens) : p.hidden_row;
           }
+          const int at = __shfl_sync(0xffffffffu, row, u & 31);
+#pragma unroll 1
+          for (int c = 0; c < v_chunks + r_chunks; ++c)
+            tma_load_3d_if(lane == 0, dst + c * kPlChunk, &pool, &kv_full[stage],
+                           c < v_chunks ? v0 + 64 * c : p.kvp + 64 * (r_chunk0 + c - v_chunks), at, 0);
         }
-        __syncwarp();
       }
     }
     if (!ok && lane == 0)                                    // let the copies under way land before the shared memory goes away
@@ -176,14 +168,13 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
       if (tile > 0 && !wait(s_free, (tile - 1) & 1, 512)) return false;
       tc_fence_after();
       const uint64_t kd = k_desc + static_cast<uint64_t>(stage * stage_bytes / 16);
+      // steps of 16 columns: four to a chunk of 128 bytes
+#pragma unroll 1
       for (int k = 0; k < v_steps; ++k)
-        umma_bf16_ts_if(leader, tmem + kPlS, tmem + kPlQ + 8 * k, kd + static_cast<uint64_t>((k >> 2) * (kPlChunk / 16) + (k & 3) * 2),
-                        idesc_s, k > 0 ? 1u : 0u);
-      for (int k = r0; k < r1; ++k) {
-        const int x = 4 * v_chunks + k - 4 * r_chunk0;       // the step's place behind the value chunks
-        umma_bf16_ts_if(leader, tmem + kPlS, tmem + kPlQ + 8 * x, kd + static_cast<uint64_t>((x >> 2) * (kPlChunk / 16) + (x & 3) * 2),
-                        idesc_s, v_steps + k > r0 ? 1u : 0u);
-      }
+        umma_bf16_ts_if(leader, tmem + kPlS, tmem + kPlQ + 8 * k, kd + (k >> 2) * (kPlChunk / 16) + 2 * (k & 3), idesc_s, k > 0);
+#pragma unroll 1
+      for (int k = 4 * v_chunks + r0 - 4 * r_chunk0; k < 4 * v_chunks + r1 - 4 * r_chunk0; ++k)
+        umma_bf16_ts_if(leader, tmem + kPlS, tmem + kPlQ + 8 * k, kd + (k >> 2) * (kPlChunk / 16) + 2 * (k & 3), idesc_s, 1u);
       tc_commit_if(leader, &s_full[tile & 1]);
       return true;
     };
@@ -196,8 +187,9 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
         tc_fence_after();
         ok = scores(kt);
       }
+      if (ok && n > 1) ok = scores(kt + 1);
       for (int j = 0; j < n && ok; ++j) {
-        if (j + 1 < n) ok = scores(kt + j + 1);
+        if (j + 2 < n) ok = scores(kt + j + 2);                // waits in tensor memory for the half that is at tile j
         if (ok) ok = wait(p_full, (kt + j) & 1, 513);
         if (!ok) break;
         tc_fence_after();
@@ -259,7 +251,7 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
       float m = -INFINITY, l = 0.f;                              // the maximum that l is relative to
       for (int j = (kt ^ half) & 1; j < n && ok; j += 2) {
         const int tile = kt + j, use = tile >> 1;
-        float s[kPlKeys];
+        float2 s[kPlKeys / 2];
         ok = __all_sync(0xffffffffu, mbar_wait(&s_full[half], use & 1, p.status, 520)) != 0;
         if (!ok) break;
         tc_fence_after();
@@ -272,9 +264,9 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
           __syncwarp();
           if (lane == 0) mbar_arrive(s_free);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            s[i] = __uint_as_float(a[i]);
-            s[32 + i] = __uint_as_float(b[i]);
+          for (int i = 0; i < 16; ++i) {
+            s[i] = make_float2(__uint_as_float(a[2 * i]), __uint_as_float(a[2 * i + 1]));
+            s[16 + i] = make_float2(__uint_as_float(b[2 * i]), __uint_as_float(b[2 * i + 1]));
           }
         }
         if (PAIR) {                                            // [column / 4][query]: neighbouring lanes, neighbouring 16 bytes
@@ -283,29 +275,30 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
           if (quad == 0 && lane == 0) mbar_expect_tx(&x_full[half], 4 * kPlKeys * kPlQueries);
 #pragma unroll
           for (int i = 0; i < kPlKeys / 4; ++i)
-            remote_store(x_there + 16 * kPlQueries * i, full_there, s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
+            remote_store(x_there + 16 * kPlQueries * i, full_there, s[2 * i].x, s[2 * i].y, s[2 * i + 1].x, s[2 * i + 1].y);
           ok = __all_sync(0xffffffffu, mbar_wait(&x_full[half], use & 1, p.status, 522)) != 0;
           if (!ok) break;
           const float4* x = reinterpret_cast<const float4*>(x_here) + mine;
 #pragma unroll
           for (int i = 0; i < kPlKeys / 4; ++i) {
             const float4 y = x[i * kPlQueries];
-            s[4 * i] += y.x;
-            s[4 * i + 1] += y.y;
-            s[4 * i + 2] += y.z;
-            s[4 * i + 3] += y.w;
+            s[2 * i] = add2(s[2 * i], make_float2(y.x, y.y));
+            s[2 * i + 1] = add2(s[2 * i + 1], make_float2(y.z, y.w));
           }
         }
         const int key0 = it.key0 + j * kPlKeys;
         if (key0 + kPlKeys > high) {                           // the tile holds keys that a query of this warp does not see
           const int shown = hi - key0;
 #pragma unroll
-          for (int i = 0; i < kPlKeys; ++i) s[i] = i < shown ? s[i] : -INFINITY;
+          for (int i = 0; i < kPlKeys / 2; ++i) {
+            s[i].x = 2 * i < shown ? s[i].x : -INFINITY;
+            s[i].y = 2 * i + 1 < shown ? s[i].y : -INFINITY;
+          }
         }
-        float top = s[0];
+        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 1; i < kPlKeys; ++i) top = fmaxf(top, s[i]);
-        top *= p.scale_log2;
+        for (int i = 0; i < kPlKeys / 2; ++i) tops[i & 3] = fmaxf(tops[i & 3], fmaxf(s[i].x, s[i].y));
+        const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * p.scale_log2;
         if (tile > 0) ok = __all_sync(0xffffffffu, mbar_wait(&known[4 * (half ^ 1) + quad], ((tile - 1) >> 1) & 1, p.status, 523)) != 0;
         if (!ok) break;
         float now = j > 0 ? s_top[mine] : -INFINITY;           // what O is relative to
@@ -339,13 +332,18 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
         m = now;
         const float neg = m == -INFINITY ? 0.f : -m;
         uint32_t w[kPlKeys / 2];
+        float2 sums[2] = {};
+        const float2 by = make_float2(p.scale_log2, p.scale_log2), off = make_float2(neg, neg);
 #pragma unroll
         for (int i = 0; i < kPlKeys / 2; ++i) {
-          const float a = ex2_approx(fmaf(s[2 * i], p.scale_log2, neg)), b = ex2_approx(fmaf(s[2 * i + 1], p.scale_log2, neg));
-          l += a + b;
-          const __nv_bfloat162 q = __floats2bfloat162_rn(a, b);
+          float2 e = fma2(s[i], by, off);
+          e = make_float2(ex2_approx(e.x), ex2_approx(e.y));
+          sums[i & 1] = add2(sums[i & 1], e);
+          const __nv_bfloat162 q = __floats2bfloat162_rn(e.x, e.y);
           w[i] = *reinterpret_cast<const uint32_t*>(&q);
         }
+        sums[0] = add2(sums[0], sums[1]);
+        l += sums[0].x + sums[0].y;
         if (PAIR && lane == 0) remote_arrive(free_there);
         if (!last_done) ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[half ^ 1], ((tile - 1) >> 1) & 1, p.status, 525)) != 0;
         if (!ok) break;
