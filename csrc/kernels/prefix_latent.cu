@@ -155,7 +155,6 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
     const uint32_t idesc_s = umma_idesc(kPlQueries, kPlKeys, 1u, 1u);
     const uint32_t idesc_pv = umma_idesc_bmn(kPlQueries, v1 - v0, 1u, 1u);
     const uint64_t k_desc = umma_desc_sw128(smem_u32(s_kv)), v_desc = umma_desc_sw128_mn(smem_u32(s_kv), kPlChunk, 1024);
-    const int v_steps = (v1 - v0) / 16;
     auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
       const bool ok = mbar_wait(bar, parity, p.status, where);
       return __all_sync(0xffffffffu, ok) != 0;
@@ -164,17 +163,24 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
     int kt = 0, live = 0;
     auto scores = [&](int tile) {                            // S of a tile, once its keys are here and the last S has been read
       const int stage = tile % p.stages;
-      if (!wait(&kv_full[stage], (tile / p.stages) & 1, 511)) return false;
-      if (tile > 0 && !wait(s_free, (tile - 1) & 1, 512)) return false;
+      const bool here = mbar_wait(&kv_full[stage], (tile / p.stages) & 1, p.status, 511) &&
+                        (tile == 0 || mbar_wait(s_free, (tile - 1) & 1, p.status, 512));
+      if (!__all_sync(0xffffffffu, here)) return false;
       tc_fence_after();
       const uint64_t kd = k_desc + static_cast<uint64_t>(stage * stage_bytes / 16);
-      // steps of 16 columns: four to a chunk of 128 bytes
+      // steps of 16 columns, four to a chunk of 128 bytes; queries are zero behind the last latent column
+      uint64_t b = kd;
+      uint32_t a = tmem + kPlQ;
 #pragma unroll 1
-      for (int k = 0; k < v_steps; ++k)
-        umma_bf16_ts_if(leader, tmem + kPlS, tmem + kPlQ + 8 * k, kd + (k >> 2) * (kPlChunk / 16) + 2 * (k & 3), idesc_s, k > 0);
+      for (int c = 0; c < v_chunks; ++c, a += 32, b += kPlChunk / 16) {
+        umma_bf16_ts_if(leader, tmem + kPlS, a, b, idesc_s, c);
+        umma_bf16_ts_if(leader, tmem + kPlS, a + 8, b + 2, idesc_s, 1u);
+        umma_bf16_ts_if(leader, tmem + kPlS, a + 16, b + 4, idesc_s, 1u);
+        umma_bf16_ts_if(leader, tmem + kPlS, a + 24, b + 6, idesc_s, 1u);
+      }
 #pragma unroll 1
-      for (int k = 4 * v_chunks + r0 - 4 * r_chunk0; k < 4 * v_chunks + r1 - 4 * r_chunk0; ++k)
-        umma_bf16_ts_if(leader, tmem + kPlS, tmem + kPlQ + 8 * k, kd + (k >> 2) * (kPlChunk / 16) + 2 * (k & 3), idesc_s, 1u);
+      for (int k = r0 - 4 * r_chunk0; k < r1 - 4 * r_chunk0; ++k)
+        umma_bf16_ts_if(leader, tmem + kPlS, a + 8 * k, b + (k >> 2) * (kPlChunk / 16) + 2 * (k & 3), idesc_s, 1u);
       tc_commit_if(leader, &s_full[tile & 1]);
       return true;
     };
