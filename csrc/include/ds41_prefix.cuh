@@ -48,6 +48,36 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return d;
 }
 
+// Four products of 16 columns of K each in one go, by the one thread that calls this; `accumulate` is the first one's.  Between two
+// products written one by one the compiler moves every operand to the uniform registers again: 128 x 64 x 16 took 83 cycles each
+// with A in tensor memory and 52 with A in shared memory, 34 and 50 so (32 is the tensor core's time, 48 that of two operands from
+// shared memory).  ASTEP / BSTEP: from one product's operands to the next one's, in columns of tensor memory or units of 16 bytes.
+template <int BSTEP>
+__device__ __forceinline__ void umma4_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b32 x;\n\t.reg .b64 y;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 q, 0, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "add.s32 x, %1, 8;\n\tadd.s64 y, %2, %5;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %3, q;\n\t"
+      "add.s32 x, %1, 16;\n\tadd.s64 y, %2, %6;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %3, q;\n\t"
+      "add.s32 x, %1, 24;\n\tadd.s64 y, %2, %7;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %3, q;\n\t}"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "n"(BSTEP), "n"(2 * BSTEP), "n"(3 * BSTEP)
+      : "memory");
+}
+template <int ASTEP, int BSTEP>
+__device__ __forceinline__ void umma4_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 x, y;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 q, 0, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+      "add.s64 x, %1, %5;\n\tadd.s64 y, %2, %8;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, q;\n\t"
+      "add.s64 x, %1, %6;\n\tadd.s64 y, %2, %9;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, q;\n\t"
+      "add.s64 x, %1, %7;\n\tadd.s64 y, %2, %10;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, q;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "n"(ASTEP), "n"(2 * ASTEP), "n"(3 * ASTEP), "n"(BSTEP), "n"(2 * BSTEP),
+        "n"(3 * BSTEP)
+      : "memory");
+}
+
 inline bool prefix_plan_ok(const ds41_prefix_plan* p) {
   return p != nullptr && p->items != nullptr && p->n_items != nullptr && p->order != nullptr && p->own != nullptr &&
          p->cell != nullptr && p->parts != nullptr && p->part_o != nullptr && p->part_ml != nullptr && p->max_items > 0 &&

@@ -9,10 +9,11 @@
 // values fit one CTA.
 //   tensor memory : O 256 columns, Q 160 (the first product's A operand: it never touches shared memory again), S 64, P 32
 //   shared memory : a ring of tiles of 64 keys (up to five chunks of 64 columns), two buffers for the other CTA's scores
-//   warps 0-3, 4-7: even / odd tiles, one thread per query: exchange, softmax, partial results.  A tile's way from S to P is a chain of
-//                   latencies; two are under way, and hand the running maximum on as soon as a tile's own is known
+//   warps 0-7     : two sets of four take the tiles in turn, one thread per query: exchange, softmax, partial results.  A tile's way
+//                   from S to P is a chain of latencies; two are under way, and hand the running maximum on as soon as a tile's
+//                   own is known
 //   warp 8        : TMA producer, page by page
-//   warp 9        : tcgen05.mma issue: S = Q K^T of the next tile as soon as this tile's S is in registers, then O += P V
+//   warp 9        : tcgen05.mma issue, in whichever order their inputs come: S = Q K^T as soon as the last S is in registers, O += P V
 // The running maximum is raised when it grew by more than 2^8 only.  P is rounded to bf16 as the operand of the second product; sums
 // stay in 32 bits.
 #include <cuda.h>
@@ -22,9 +23,9 @@
 
 namespace ds41 {
 
-constexpr int kPlThreads = 320;
+constexpr int kPlSets = 2, kPlThreads = 128 * kPlSets + 64, kPlTma = 4 * kPlSets, kPlMma = kPlTma + 1;
 constexpr int kPlQueries = 128, kPlKeys = 64;
-constexpr int kPlChunk = kPlKeys * 128;        // bytes of 64 keys x 64 bf16 columns
+constexpr int kPlChunk = kPlKeys * 128;        // bytes of a tile's keys x 64 bf16 columns
 constexpr int kPlMost = 5;                     // chunks of columns of a CTA
 constexpr int kPlStages = 8;
 constexpr uint32_t kPlQ = 256, kPlS = 416, kPlP = 480;      // columns of tensor memory behind O
@@ -37,6 +38,7 @@ struct PrefixLatentParams {
   int chunks, stages;                                       // of a stage, of the ring
   int v_col[3], rot_step[3];                                // CTA c: latent columns [v_col[c], v_col[c + 1]), rotated steps of 16 likewise
   int max_pages, page_tokens, box, hidden_row;
+  int deep;                                                 // a CTA's latent chunks of a box in one copy
   float scale_log2;
   int* status;
 };
@@ -58,27 +60,27 @@ __device__ __forceinline__ void cluster_meet() {
 
 template <bool PAIR>
 __global__ void __launch_bounds__(kPlThreads, 1)
-prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLatentParams p, const ds41_prefix_plan plan) {
-  extern __shared__ __align__(1024) uint8_t pl_smem[];       // no room to align it here: four stages leave 200 bytes
+prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_constant__ CUtensorMap chunks, const PrefixLatentParams p, const ds41_prefix_plan plan) {
+  extern __shared__ __align__(1024) uint8_t pl_smem[];       // no room to align it here: it is a multiple of 1024 as it is
   uint8_t* smem = pl_smem;
   const int stage_bytes = p.chunks * kPlChunk;
   uint8_t* s_kv = smem;
-  float* s_x = reinterpret_cast<float*>(s_kv + p.stages * stage_bytes);      // [2][16 columns of four][128 queries][4]
+  float* s_x = reinterpret_cast<float*>(s_kv + p.stages * stage_bytes);      // [2][columns of four][128 queries][4]
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_x + (PAIR ? 2 * kPlKeys * kPlQueries : 0));
   uint64_t* kv_full = bars;                                  // [stages]
   uint64_t* kv_empty = kv_full + kPlStages;
   uint64_t* q_full = kv_empty + kPlStages;
   uint64_t* s_free = q_full + 1;                             // S in registers
-  uint64_t* p_full = s_free + 1;                             // P written, O rescaled
-  // by parity of the tile, as each half of the warps waits for every other one only:
-  uint64_t* s_full = p_full + 1;                             // [2] S complete
-  uint64_t* pv_done = s_full + 2;                            // [2] O += P V complete
-  uint64_t* x_full = pv_done + 2;                            // [2] the other CTA's scores are here
-  uint64_t* x_free = x_full + 2;                             // [2] this CTA's have been read there
-  uint64_t* known = x_free + 2;                              // [2][4] the maximum after a tile, by quadrant
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(known + 8);
+  // by tile % 2, so that each is waited for by one set (which sees every phase of it):
+  uint64_t* p_full = s_free + 1;                             // [2] P written, O rescaled
+  uint64_t* s_full = p_full + kPlSets;                       // [2] S complete
+  uint64_t* pv_done = s_full + kPlSets;                      // [2] O += P V complete
+  uint64_t* x_full = pv_done + kPlSets;                      // [2] the other CTA's scores are here
+  uint64_t* x_free = x_full + kPlSets;                       // [2] this CTA's have been read there
+  uint64_t* known = x_free + kPlSets;                        // [2][4] the maximum after a tile, by quadrant
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(known + 4 * kPlSets);
   float* s_top = reinterpret_cast<float*>(tmem_slot + 2);    // [128] the running maximum
-  float2* s_ml = reinterpret_cast<float2*>(s_top + kPlQueries);      // [2][128] the halves' maxima and sums
+  float* s_sum = s_top + kPlQueries;                         // [2][128] the sets' sums
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = PAIR ? static_cast<int>(blockIdx.x & 1) : 0;
 
@@ -88,10 +90,10 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
       mbar_init(&kv_full[i], 1);
       mbar_init(&kv_empty[i], 1);
     }
-    mbar_init(q_full, 8);
+    mbar_init(q_full, 4 * kPlSets);
     mbar_init(s_free, 4);
-    mbar_init(p_full, 4);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kPlSets; ++i) {
+      mbar_init(&p_full[i], 4);
       mbar_init(&s_full[i], 1);
       mbar_init(&pv_done[i], 1);
       mbar_init(&x_full[i], 1);
@@ -100,8 +102,9 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
     }
     mbar_init_fence();
     tma_prefetch_desc(&pool);
+    if (p.deep) tma_prefetch_desc(&chunks);
   }
-  if (warp == 9) {
+  if (warp == kPlMma) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
@@ -116,9 +119,12 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
   const int v0 = p.v_col[rank], v1 = p.v_col[rank + 1], r0 = p.rot_step[rank], r1 = p.rot_step[rank + 1];
   const int v_chunks = (v1 - v0 + 63) / 64, r_chunk0 = r0 >> 2, r_chunks = r1 > r0 ? (r1 + 3) / 4 - r_chunk0 : 0;
 
-  if (warp == 8) {
-    const int boxes = kPlKeys / p.box;
-    int kt = 0;
+  if (warp == kPlTma) {
+    // A copy costs the issuing thread 50 to 100 cycles: where a tile lies in one page and the chunks in one row of them, all of a CTA's
+    // latent chunks come in one (a box of 64 columns x 64 rows x chunks).
+    const int boxes = kPlKeys / p.box, singles = p.deep ? r_chunks : v_chunks + r_chunks, first_single = p.deep ? v_chunks : 0;
+    int stage = 0, kt = 0;
+    uint32_t free_phase = 1;
     bool ok = true;
     for (int unit = first_unit; unit < units && ok; unit += unit_step) {
       const PrefixItem it = prefix_item(plan, unit);
@@ -126,11 +132,10 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
       const int* table = p.page_table + 1ll * it.slot * p.max_pages;
       int row = 0, u = 0;                                    // lane i: pool row of box i of the walk, 32 boxes at a time
       for (int j = 0; j < n; ++j, ++kt) {
-        const int stage = kt % p.stages;
-        ok = __all_sync(0xffffffffu, mbar_wait(&kv_empty[stage], ((kt / p.stages) & 1) ^ 1, p.status, 500)) != 0;
+        ok = __all_sync(0xffffffffu, mbar_wait(&kv_empty[stage], free_phase, p.status, 500)) != 0;
         if (!ok) break;
         uint8_t* dst = s_kv + stage * stage_bytes;
-        mbar_expect_tx_if(lane == 0, &kv_full[stage], (v_chunks + r_chunks) * kPlChunk);
+        if (lane == 0) mbar_expect_tx(&kv_full[stage], (v_chunks + r_chunks) * kPlChunk);
 #pragma unroll 1
         for (int i = 0; i < boxes; ++i, ++u, dst += p.box * 128) {
           if ((u & 31) == 0) {
@@ -139,10 +144,18 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
             row = id >= 0 ? id * p.page_tokens + (key - pg * p.page_tokens) : p.hidden_row;
           }
           const int at = __shfl_sync(0xffffffffu, row, u & 31);
+          if (lane == 0) {
+            if (p.deep) tma_load_3d(dst, &chunks, &kv_full[stage], 0, at, v0 >> 6);
 #pragma unroll 1
-          for (int c = 0; c < v_chunks + r_chunks; ++c)
-            tma_load_3d_if(lane == 0, dst + c * kPlChunk, &pool, &kv_full[stage],
-                           c < v_chunks ? v0 + 64 * c : p.kvp + 64 * (r_chunk0 + c - v_chunks), at, 0);
+            for (int c = first_single; c < first_single + singles; ++c)
+              tma_load_3d(dst + c * kPlChunk, &pool, &kv_full[stage],
+                          c < v_chunks ? v0 + 64 * c : p.kvp + 64 * (r_chunk0 + c - v_chunks), at, 0);
+          }
+          __syncwarp();
+        }
+        if (++stage == p.stages) {
+          stage = 0;
+          free_phase ^= 1;
         }
       }
     }
@@ -150,74 +163,83 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
       for (int b = max(0, kt - p.stages); b < kt; ++b)
         for (int i = 0; i < (1 << 18) && !mbar_test_wait(&kv_full[b % p.stages], (b / p.stages) & 1); ++i) {
         }
-  } else if (warp == 9) {
-    const bool leader = elect_one();
-    const uint32_t idesc_s = umma_idesc(kPlQueries, kPlKeys, 1u, 1u);
-    const uint32_t idesc_pv = umma_idesc_bmn(kPlQueries, v1 - v0, 1u, 1u);
-    const uint64_t k_desc = umma_desc_sw128(smem_u32(s_kv)), v_desc = umma_desc_sw128_mn(smem_u32(s_kv), kPlChunk, 1024);
-    auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
-      const bool ok = mbar_wait(bar, parity, p.status, where);
-      return __all_sync(0xffffffffu, ok) != 0;
-    };
-    bool ok = true;
-    int kt = 0, live = 0;
-    auto scores = [&](int tile) {                            // S of a tile, once its keys are here and the last S has been read
-      const int stage = tile % p.stages;
-      const bool here = mbar_wait(&kv_full[stage], (tile / p.stages) & 1, p.status, 511) &&
-                        (tile == 0 || mbar_wait(s_free, (tile - 1) & 1, p.status, 512));
-      if (!__all_sync(0xffffffffu, here)) return false;
-      tc_fence_after();
-      const uint64_t kd = k_desc + static_cast<uint64_t>(stage * stage_bytes / 16);
-      // steps of 16 columns, four to a chunk of 128 bytes; queries are zero behind the last latent column
-      uint64_t b = kd;
-      uint32_t a = tmem + kPlQ;
-#pragma unroll 1
-      for (int c = 0; c < v_chunks; ++c, a += 32, b += kPlChunk / 16) {
-        umma_bf16_ts_if(leader, tmem + kPlS, a, b, idesc_s, c);
-        umma_bf16_ts_if(leader, tmem + kPlS, a + 8, b + 2, idesc_s, 1u);
-        umma_bf16_ts_if(leader, tmem + kPlS, a + 16, b + 4, idesc_s, 1u);
-        umma_bf16_ts_if(leader, tmem + kPlS, a + 24, b + 6, idesc_s, 1u);
-      }
-#pragma unroll 1
-      for (int k = r0 - 4 * r_chunk0; k < r1 - 4 * r_chunk0; ++k)
-        umma_bf16_ts_if(leader, tmem + kPlS, a + 8 * k, b + (k >> 2) * (kPlChunk / 16) + 2 * (k & 3), idesc_s, 1u);
-      tc_commit_if(leader, &s_full[tile & 1]);
-      return true;
-    };
-    for (int unit = first_unit; unit < units && ok; unit += unit_step) {
-      const PrefixItem it = prefix_item(plan, unit);
-      const int n = (it.key1 - it.key0 + kPlKeys - 1) / kPlKeys;
-      ok = wait(q_full, live & 1, 510);
-      ++live;
-      if (ok) {
-        tc_fence_after();
-        ok = scores(kt);
-      }
-      if (ok && n > 1) ok = scores(kt + 1);
-      for (int j = 0; j < n && ok; ++j) {
-        if (j + 2 < n) ok = scores(kt + j + 2);                // waits in tensor memory for the half that is at tile j
-        if (ok) ok = wait(p_full, (kt + j) & 1, 513);
+  } else if (warp == kPlMma) {
+    // one thread: votes and the like between two products cost as much as the products
+    if (elect_one()) {
+      const uint32_t idesc_s = umma_idesc(kPlQueries, kPlKeys, 1u, 1u);
+      const uint32_t idesc_pv = umma_idesc_bmn(kPlQueries, v1 - v0, 1u, 1u);
+      const uint64_t k_desc = umma_desc_sw128(smem_u32(s_kv)), v_desc = umma_desc_sw128_mn(smem_u32(s_kv), kPlChunk, 1024);
+      bool ok = true;
+      int kt = 0, live = 0, s_stage = 0, p_stage = 0;          // tiles so far; the ring's places of the next scores and values
+      uint32_t s_phase = 0;
+      for (int unit = first_unit; unit < units && ok; unit += unit_step) {
+        const PrefixItem it = prefix_item(plan, unit);
+        const int n = (it.key1 - it.key0 + kPlKeys - 1) / kPlKeys;
+        ok = mbar_wait(q_full, live & 1, p.status, 510);
+        ++live;
         if (!ok) break;
         tc_fence_after();
-        const uint64_t vd = v_desc + static_cast<uint64_t>((kt + j) % p.stages * stage_bytes / 16);
-#pragma unroll
-        for (int k = 0; k < kPlKeys / 16; ++k)
-          umma_bf16_ts_if(leader, tmem, tmem + kPlP + 8 * k, vd + 128 * k, idesc_pv, j == 0 && k == 0 ? 0u : 1u);
-        tc_commit_if(leader, &kv_empty[(kt + j) % p.stages]);
-        tc_commit_if(leader, &pv_done[(kt + j) & 1]);
+        int sj = 0, pj = 0;                                    // next scores, next values
+        uint32_t idle = 0;
+        long long since = 0;
+        while (pj < n) {
+          const int st = kt + sj, pt = kt + pj;
+          if (pj < sj && mbar_test_wait(&p_full[pt % kPlSets], (pt / kPlSets) & 1)) {
+            tc_fence_after();
+            umma4_ts<128>(tmem, tmem + kPlP, v_desc + static_cast<uint64_t>(p_stage * stage_bytes / 16), idesc_pv, pj > 0);
+            tc_commit_if(true, &kv_empty[p_stage]);
+            tc_commit_if(true, &pv_done[pt % kPlSets]);
+            ++pj;
+            if (++p_stage == p.stages) p_stage = 0;
+          } else if (sj < n && mbar_test_wait(&kv_full[s_stage], s_phase) && (st == 0 || mbar_test_wait(s_free, (st - 1) & 1))) {
+            tc_fence_after();
+            // steps of 16 columns, four to a chunk of 128 bytes; queries are zero behind the last latent column
+            uint64_t b = k_desc + static_cast<uint64_t>(s_stage * stage_bytes / 16);
+            uint32_t a = tmem + kPlQ;
+#pragma unroll 1
+            for (int c = 0; c < v_chunks; ++c, a += 32, b += kPlChunk / 16) umma4_ts<2>(tmem + kPlS, a, b, idesc_s, c);
+#pragma unroll 1
+            for (int k = r0 - 4 * r_chunk0; k < r1 - 4 * r_chunk0; ++k)
+              umma_bf16_ts_if(true, tmem + kPlS, a + 8 * k, b + (k >> 2) * (kPlChunk / 16) + 2 * (k & 3), idesc_s, 1u);
+            tc_commit_if(true, &s_full[st % kPlSets]);
+            ++sj;
+            if (++s_stage == p.stages) {
+              s_stage = 0;
+              s_phase ^= 1;
+            }
+          } else if ((++idle & 0x3ff) == 0) {                  // as long as any other wait: see mbar_wait
+            if (since == 0) since = clock64();
+            if (clock64() - since > DS41_WAIT_LIMIT_CYCLES ||
+                (p.status != nullptr && *reinterpret_cast<volatile int*>(p.status) != kStatusOk)) {
+              if (p.status != nullptr && atomicCAS(p.status, kStatusOk, kStatusMbarTimeout) == kStatusOk) {
+                p.status[1] = 511;
+                p.status[2] = static_cast<int>(blockIdx.x);
+                p.status[3] = pj;
+              }
+              ok = false;
+              break;
+            }
+            continue;
+          } else {
+            continue;
+          }
+          idle = 0;
+          since = 0;
+        }
+        kt += n;
       }
-      kt += n;
     }
+    __syncwarp();
   } else {
-    const int half = warp >> 2, quad = warp & 3, mine = quad * 32 + lane;
+    const int set = warp >> 2, quad = warp & 3, mine = quad * 32 + lane;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-    const uint32_t x_there = PAIR ? cluster_addr(smem_u32(s_x + half * kPlKeys * kPlQueries) + 16 * mine, rank ^ 1) : 0;
-    const uint32_t full_there = PAIR ? cluster_addr(smem_u32(&x_full[half]), rank ^ 1) : 0;
-    const uint32_t free_there = PAIR ? cluster_addr(smem_u32(&x_free[half]), rank ^ 1) : 0;
-    const float* x_here = s_x + half * kPlKeys * kPlQueries;
+    const uint32_t x_there = PAIR ? cluster_addr(smem_u32(s_x) + 16 * mine, rank ^ 1) : 0;
+    const uint32_t full_there = PAIR ? cluster_addr(smem_u32(&x_full[set]), rank ^ 1) : 0;
+    const uint32_t free_there = PAIR ? cluster_addr(smem_u32(&x_free[set]), rank ^ 1) : 0;
+    const int before = (set + kPlSets - 1) % kPlSets;              // the set of the last tile
     int kt = 0;
     bool ok = true;
-    // the loop runs to its end whatever happened: the two warps of a quadrant meet at barriers
+    // the loop runs to its end whatever happened: the warps of a quadrant meet at barriers
     for (int unit = first_unit; unit < units; unit += unit_step) {
       const PrefixItem it = prefix_item(plan, unit);
       const int n = (it.key1 - it.key0 + kPlKeys - 1) / kPlKeys;
@@ -227,8 +249,8 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
         h = mine % p.heads;
         if (p.row_slot[r] >= 0) hi = min(min(plan.own[r], p.row_pos[r] + 1), it.key1);
       }
-      // queries into tensor memory: 32 values at a time, the two halves in turn
-      for (int c = half; c < 2 * (v_chunks + r_chunks); c += 2) {
+      // queries into tensor memory: 32 values at a time, the sets in turn
+      for (int c = set; c < 2 * (v_chunks + r_chunks); c += kPlSets) {
         uint32_t w[16];
         const bool lat = c < 2 * v_chunks;
         const int d0 = lat ? v0 + 32 * c : 64 * r_chunk0 + 32 * (c - 2 * v_chunks), width = lat ? v1 : p.rp;
@@ -255,10 +277,10 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
 #pragma unroll
       for (int o = 16; o; o >>= 1) high = min(high, __shfl_xor_sync(0xffffffffu, high, o));
       float m = -INFINITY, l = 0.f;                              // the maximum that l is relative to
-      for (int j = (kt ^ half) & 1; j < n && ok; j += 2) {
-        const int tile = kt + j, use = tile >> 1;
+      for (int j = (set + kPlSets - kt % kPlSets) % kPlSets; j < n && ok; j += kPlSets) {
+        const int tile = kt + j, use = tile / kPlSets;
         float2 s[kPlKeys / 2];
-        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[half], use & 1, p.status, 520)) != 0;
+        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[set], use & 1, p.status, 520)) != 0;
         if (!ok) break;
         tc_fence_after();
         {
@@ -276,15 +298,17 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
           }
         }
         if (PAIR) {                                            // [column / 4][query]: neighbouring lanes, neighbouring 16 bytes
-          if (use > 0) ok = __all_sync(0xffffffffu, mbar_wait(&x_free[half], (use - 1) & 1, p.status, 521)) != 0;
+          const uint32_t buf = (tile & 1) * kPlKeys * kPlQueries;      // its last scores, of the tile before last, have been read
+          if (tile > 1)
+            ok = __all_sync(0xffffffffu, mbar_wait(&x_free[(tile - 2) % kPlSets], ((tile - 2) / kPlSets) & 1, p.status, 521)) != 0;
           if (!ok) break;
-          if (quad == 0 && lane == 0) mbar_expect_tx(&x_full[half], 4 * kPlKeys * kPlQueries);
+          if (quad == 0 && lane == 0) mbar_expect_tx(&x_full[set], 4 * kPlKeys * kPlQueries);
 #pragma unroll
           for (int i = 0; i < kPlKeys / 4; ++i)
-            remote_store(x_there + 16 * kPlQueries * i, full_there, s[2 * i].x, s[2 * i].y, s[2 * i + 1].x, s[2 * i + 1].y);
-          ok = __all_sync(0xffffffffu, mbar_wait(&x_full[half], use & 1, p.status, 522)) != 0;
+            remote_store(x_there + 4 * buf + 16 * kPlQueries * i, full_there, s[2 * i].x, s[2 * i].y, s[2 * i + 1].x, s[2 * i + 1].y);
+          ok = __all_sync(0xffffffffu, mbar_wait(&x_full[set], use & 1, p.status, 522)) != 0;
           if (!ok) break;
-          const float4* x = reinterpret_cast<const float4*>(x_here) + mine;
+          const float4* x = reinterpret_cast<const float4*>(s_x + buf) + mine;
 #pragma unroll
           for (int i = 0; i < kPlKeys / 4; ++i) {
             const float4 y = x[i * kPlQueries];
@@ -305,7 +329,8 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
 #pragma unroll
         for (int i = 0; i < kPlKeys / 2; ++i) tops[i & 3] = fmaxf(tops[i & 3], fmaxf(s[i].x, s[i].y));
         const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * p.scale_log2;
-        if (tile > 0) ok = __all_sync(0xffffffffu, mbar_wait(&known[4 * (half ^ 1) + quad], ((tile - 1) >> 1) & 1, p.status, 523)) != 0;
+        if (PAIR && lane == 0) remote_arrive(free_there);          // every score has been used for the maximum
+        if (tile > 0) ok = __all_sync(0xffffffffu, mbar_wait(&known[4 * before + quad], ((tile - 1) / kPlSets) & 1, p.status, 523)) != 0;
         if (!ok) break;
         float now = j > 0 ? s_top[mine] : -INFINITY;           // what O is relative to
         const bool grow = top > now + 8.f || (now == -INFINITY && top > now);
@@ -313,7 +338,7 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
         if (__any_sync(0xffffffffu, grow)) {
           const float next = grow ? top : now, keep = grow ? (now == -INFINITY ? 0.f : ex2_approx(now - next)) : 1.f;
           if (j > 0) {
-            ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[half ^ 1], ((tile - 1) >> 1) & 1, p.status, 524)) != 0;
+            ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[before], ((tile - 1) / kPlSets) & 1, p.status, 524)) != 0;
             if (!ok) break;
             last_done = true;
             tc_fence_after();
@@ -333,7 +358,7 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
         }
         s_top[mine] = now;
         __syncwarp();
-        if (lane == 0) mbar_arrive(&known[4 * half + quad]);
+        if (lane == 0) mbar_arrive(&known[4 * set + quad]);
         if (now > m) l *= m == -INFINITY ? 0.f : ex2_approx(m - now);
         m = now;
         const float neg = m == -INFINITY ? 0.f : -m;
@@ -350,33 +375,37 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
         }
         sums[0] = add2(sums[0], sums[1]);
         l += sums[0].x + sums[0].y;
-        if (PAIR && lane == 0) remote_arrive(free_there);
-        if (!last_done) ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[half ^ 1], ((tile - 1) >> 1) & 1, p.status, 525)) != 0;
+        // the last tile's P has been used
+        if (!last_done) ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[before], ((tile - 1) / kPlSets) & 1, p.status, 525)) != 0;
         if (!ok) break;
         tc_fence_after();
         tmem_st_32x32(lanes + kPlP, w);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_full);
+        if (lane == 0) mbar_arrive(&p_full[set]);
       }
       kt += n;
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[(kt - 1) & 1], ((kt - 1) >> 1) & 1, p.status, 526)) != 0;
+      // the last maximum is there; and the set of the last tile has seen the products up to the one before the last complete, so that the
+      // wait that follows cannot take an earlier phase for its own
+      named_barrier(1 + quad, 32 * kPlSets);
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[(kt - 1) % kPlSets], ((kt - 1) / kPlSets) & 1, p.status, 526)) != 0;
       tc_fence_after();
-      s_ml[half * kPlQueries + mine] = make_float2(m, l);
-      named_barrier(1 + quad, 64);
-      const float2 ma = s_ml[mine], mb = s_ml[kPlQueries + mine];
-      m = fmaxf(ma.x, mb.x);                                     // the last one, as it only grows
-      l = (ma.x == -INFINITY ? 0.f : ma.y * ex2_approx(ma.x - m)) + (mb.x == -INFINITY ? 0.f : mb.y * ex2_approx(mb.x - m));
+      const float all = s_top[mine];
+      s_sum[set * kPlQueries + mine] = m == -INFINITY ? 0.f : l * ex2_approx(m - all);
+      named_barrier(1 + quad, 32 * kPlSets);
+      l = s_sum[mine];
+#pragma unroll
+      for (int i = 1; i < kPlSets; ++i) l += s_sum[i * kPlQueries + mine];
+      m = all;
       if (ok) {
         const bool write = r >= 0, seen = hi > it.key0;
         const long long cell = write ? (1ll * plan.cell[r] + it.split) * p.heads + h : 0;
-        if (write && half == 0 && rank == 0)
+        if (write && set == 0 && rank == 0)
           *reinterpret_cast<float2*>(plan.part_ml + 2 * cell) =
               make_float2(seen ? m * 0.6931471805599453f : -INFINITY, seen ? l : 0.f);
         float* dst = plan.part_o + cell * p.kvp + v0;
-        const int cols = (v1 - v0) / 32 * 16;
-        for (int c = half ? cols : 0; c < (half ? v1 - v0 : cols); c += 16) {
+        for (int c = 16 * set; c < v1 - v0; c += 16 * kPlSets) {
           uint32_t o[16];
           tmem_ld_32x16(lanes + c, o);
           tmem_wait_ld();
@@ -390,24 +419,24 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const PrefixLaten
         }
       }
       tc_fence_before();
-      named_barrier(1 + quad, 64);                             // O, the maxima and the sums may be written again
+      named_barrier(1 + quad, 32 * kPlSets);                     // O, the maxima and the sums may be written again
     }
   }
   __syncthreads();
   if (PAIR) cluster_meet();                                    // nothing of this CTA's memory is written or signalled any more
-  if (warp == 9) {
+  if (warp == kPlMma) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
 }
 
 template <bool PAIR>
-static int launch_form(const CUtensorMap& pool, const PrefixLatentParams& p, const ds41_prefix_plan& plan, int smem, cudaStream_t st) {
+static int launch_form(const CUtensorMap& pool, const CUtensorMap& chunks, const PrefixLatentParams& p, const ds41_prefix_plan& plan, int smem, cudaStream_t st) {
   const cudaError_t e = cudaFuncSetAttribute(prefix_latent_kernel<PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  if (!PAIR) return launch_pdl(prefix_latent_kernel<PAIR>, dim3(plan.grid), dim3(kPlThreads), smem, st, pool, p, plan);
+  if (!PAIR) return launch_pdl(prefix_latent_kernel<PAIR>, dim3(plan.grid), dim3(kPlThreads), smem, st, pool, chunks, p, plan);
   const int pairs = plan.grid < sm_count() / 2 ? plan.grid : sm_count() / 2;
-  return launch_pdl_cluster(prefix_latent_kernel<PAIR>, dim3(2 * pairs), dim3(kPlThreads), 2, smem, st, pool, p, plan);
+  return launch_pdl_cluster(prefix_latent_kernel<PAIR>, dim3(2 * pairs), dim3(kPlThreads), 2, smem, st, pool, chunks, p, plan);
 }
 
 // cudaErrorNotSupported: these sizes are for the simple form
@@ -437,7 +466,7 @@ int launch_prefix_latent(const ds41_latent_attend_args& a, const ds41_prefix_pla
     if (n > kPlMost || p.v_col[c + 1] <= p.v_col[c]) return cudaErrorNotSupported;
     p.chunks = n > p.chunks ? n : p.chunks;
   }
-  constexpr int kExtra = 8 * (2 * kPlStages + 19) + 8 + 4 * 5 * kPlQueries;
+  constexpr int kExtra = 8 * (2 * kPlStages + 2 + 9 * kPlSets) + 8 + 4 * (1 + kPlSets) * kPlQueries;
   const int room = 227 * 1024 - kExtra - (pair ? 2 * 4 * kPlKeys * kPlQueries : 0);
   p.stages = room / (p.chunks * kPlChunk);
   if (p.stages > kPlStages) p.stages = kPlStages;
@@ -453,7 +482,14 @@ int launch_prefix_latent(const ds41_latent_attend_args& a, const ds41_prefix_pla
   CUtensorMap pool;
   const cudaError_t e = make_tensor_map_3d(&pool, a.pool, TmaDtype::kBF16, a.row_len, p.hidden_row, 1, 2ull * a.row_len, 0, 64, p.box, true);
   if (e != cudaSuccess) return e;
-  return pair ? launch_form<true>(pool, p, plan, smem, st) : launch_form<false>(pool, p, plan, smem, st);
+  CUtensorMap chunks = pool;
+  p.deep = p.box == kPlKeys && a.row_len % 64 == 0 && a.kv_pad % 64 == 0 && (!pair || 2 * p.v_col[1] == a.kv_pad);
+  if (p.deep) {
+    const cudaError_t d = make_tensor_map_3d(&chunks, a.pool, TmaDtype::kBF16, 64, p.hidden_row, a.row_len / 64, 2ull * a.row_len, 128, 64,
+                                             kPlKeys, true, p.v_col[1] / 64);
+    if (d != cudaSuccess) return d;
+  }
+  return pair ? launch_form<true>(pool, chunks, p, plan, smem, st) : launch_form<false>(pool, chunks, p, plan, smem, st);
 }
 
 }  // namespace ds41

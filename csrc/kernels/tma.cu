@@ -26,7 +26,7 @@ static int g_last_result = 0;     // driver result of the most recent encode (di
 
 cudaError_t make_tensor_map_3d(CUtensorMap* out, const void* base, TmaDtype dtype, uint64_t cols, uint64_t rows,
                                uint64_t batch, uint64_t row_stride_bytes, uint64_t batch_stride_bytes,
-                               uint32_t box_cols, uint32_t box_rows, bool swizzle128) {
+                               uint32_t box_cols, uint32_t box_rows, bool swizzle128, uint32_t box_batch) {
   std::call_once(g_once, resolve);
   if (g_encode == nullptr) return cudaErrorNotSupported;
   CUtensorMapDataType dt;
@@ -46,14 +46,14 @@ cudaError_t make_tensor_map_3d(CUtensorMap* out, const void* base, TmaDtype dtyp
   const uint64_t align = padded4 ? 31 : 15;
   if ((reinterpret_cast<uintptr_t>(base) & align) != 0 || (row_stride_bytes & align) != 0 ||
       (batch > 1 && (batch_stride_bytes & align) != 0) || (box_smem_bytes & 15) != 0 ||
-      box_rows == 0 || box_rows > 256 || box_cols == 0 || box_cols > 256 || (padded4 && (box_cols != 128 || cols % 128))) {
+      box_rows == 0 || box_rows > 256 || box_batch == 0 || box_batch > 256 || box_cols == 0 || box_cols > 256 || (padded4 && (box_cols != 128 || cols % 128))) {
     return cudaErrorInvalidValue;
   }
   if (swizzle128 && box_smem_bytes != 128) return cudaErrorInvalidValue;
   cuuint64_t dims[3] = {cols, rows, batch == 0 ? 1 : batch};
   cuuint64_t strides[2] = {row_stride_bytes, batch > 1 ? batch_stride_bytes : row_stride_bytes * rows};
   if ((strides[1] & align) != 0) strides[1] = (strides[1] + align) & ~align;
-  cuuint32_t box[3] = {box_cols, box_rows, 1};
+  cuuint32_t box[3] = {box_cols, box_rows, box_batch};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = g_encode(out, dt, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
