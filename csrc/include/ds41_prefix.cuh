@@ -78,11 +78,18 @@ __device__ __forceinline__ void umma4_ss(uint32_t d, uint64_t a, uint64_t b, uin
       : "memory");
 }
 
+// Eight neighbouring values, 32-byte aligned: a whole sector of L2 per thread, as neighbouring threads store to rows far apart.
+__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]),
+               "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
+}
+
 inline bool prefix_plan_ok(const ds41_prefix_plan* p) {
   return p != nullptr && p->items != nullptr && p->n_items != nullptr && p->order != nullptr && p->own != nullptr &&
          p->cell != nullptr && p->parts != nullptr && p->part_o != nullptr && p->part_ml != nullptr && p->max_items > 0 &&
          p->rows_per_item > 0 && p->grid > 0 && !(reinterpret_cast<uintptr_t>(p->items) & 15) &&
-         !(reinterpret_cast<uintptr_t>(p->part_o) & 15) && !(reinterpret_cast<uintptr_t>(p->part_ml) & 7);
+         !(reinterpret_cast<uintptr_t>(p->part_o) & 31) && !(reinterpret_cast<uintptr_t>(p->part_ml) & 7);
 }
 
 }  // namespace ds41

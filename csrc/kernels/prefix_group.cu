@@ -95,7 +95,8 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
 
   if (warp == 8) {
     const int boxes = kPgTile / p.box;
-    int kt = 0;                                          // key tiles so far: key and value rings
+    int kt = 0, k_stage = 0, v_stage = 0;                // key tiles so far, places in the rings
+    uint32_t k_free = 1, v_free = 1;
     bool ok = true;
     for (int unit = blockIdx.x; unit < units && ok; unit += gridDim.x) {
       const PrefixItem it = prefix_item(plan, unit / p.kv_heads);
@@ -103,49 +104,42 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
       int first;
       const int n = span(it, first);
       const int* table = p.page_table + 1ll * it.slot * p.max_pages;
-      int row = 0, u = 0, u_row = 0;                     // lane i: pool row of box i of the walk, 32 boxes at a time
-      for (int j = 0; j < n && ok; ++j, ++kt) {
-        int at[16];                                      // this tile's boxes (at most 128 / 8)
-        auto locate = [&](int i) {
-          if ((u & 31) == 0) {
-            const int key = first + (u + lane) * p.box, pg = key / p.page_tokens;
-            const int id = key < it.key1 && pg < p.max_pages ? table[pg] : -1;
-            row = id >= 0 ? id * p.page_tokens + (key - pg * p.page_tokens) : p.hidden_row;
-          }
-          u_row = __shfl_sync(0xffffffffu, row, u & 31);
-          ++u;
-          return u_row;
-        };
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (i < boxes) at[i] = locate(i);
-        const int ks = kt % p.k_stages, vs = kt % p.v_stages;
-        ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[ks], ((kt / p.k_stages) & 1) ^ 1, p.status, 460)) != 0;
-        if (!ok) break;
-        if (lane == 0) {
-          mbar_expect_tx(&k_full[ks], k_bytes);
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (i < boxes)
-              for (int c = 0; c < p.kd; ++c)
-                tma_load_3d(s_k + ks * k_bytes + c * kPgChunk + i * p.box * 128, &pool, &k_full[ks], g * p.dp + 64 * c, at[i], 0);
+      int row = 0, u = 0;                                // lane i: pool row of box i of the walk, 32 boxes at a time
+      for (int j = 0; j < n; ++j, ++kt, u += boxes) {
+        if ((u & 31) == 0) {                             // boxes divides 32
+          const int key = first + (u + lane) * p.box, pg = key / p.page_tokens;
+          const int id = key < it.key1 && pg < p.max_pages ? table[pg] : -1;
+          row = id >= 0 ? id * p.page_tokens + (key - pg * p.page_tokens) : p.hidden_row;
         }
-        __syncwarp();
-        ok = __all_sync(0xffffffffu, mbar_wait(&v_empty[vs], ((kt / p.v_stages) & 1) ^ 1, p.status, 461)) != 0;
+        // one tile of keys or values: `chunks` chunks of 64 columns from column x on
+        auto fetch = [&](uint8_t* dst, uint64_t* bar, int x, int chunks) {
+          if (lane == 0) mbar_expect_tx(bar, chunks * kPgChunk);
+#pragma unroll 1
+          for (int i = 0; i < boxes; ++i) {
+            const int at = __shfl_sync(0xffffffffu, row, (u + i) & 31);
+            if (lane == 0)
+#pragma unroll 1
+              for (int c = 0; c < chunks; ++c) tma_load_3d(dst + c * kPgChunk + i * p.box * 128, &pool, bar, x + 64 * c, at, 0);
+            __syncwarp();
+          }
+        };
+        ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[k_stage], k_free, p.status, 460)) != 0;
+        if (!ok) break;
+        fetch(s_k + k_stage * k_bytes, &k_full[k_stage], g * p.dp, p.kd);
+        if (++k_stage == p.k_stages) {
+          k_stage = 0;
+          k_free ^= 1;
+        }
+        ok = __all_sync(0xffffffffu, mbar_wait(&v_empty[v_stage], v_free, p.status, 461)) != 0;
         if (!ok) {
           ++kt;
           break;
         }
-        if (lane == 0) {
-          mbar_expect_tx(&v_full[vs], v_bytes);
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (i < boxes)
-              for (int c = 0; c < p.vc; ++c)
-                tma_load_3d(s_v + vs * v_bytes + c * kPgChunk + i * p.box * 128, &pool, &v_full[vs],
-                            p.kv_heads * p.dp + g * p.vp + 64 * c, at[i], 0);
+        fetch(s_v + v_stage * v_bytes, &v_full[v_stage], p.kv_heads * p.dp + g * p.vp, p.vc);
+        if (++v_stage == p.v_stages) {
+          v_stage = 0;
+          v_free ^= 1;
         }
-        __syncwarp();
       }
     }
     if (!ok && lane == 0) {
@@ -163,26 +157,7 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
     const uint32_t idesc_pv = umma_idesc_bmn(kPgTile, p.vp, 1u, 1u);
     const uint64_t q_desc = umma_desc_sw128(smem_u32(s_q)), k_desc = umma_desc_sw128(smem_u32(s_k));
     const uint64_t v_desc = umma_desc_sw128_mn(smem_u32(s_v), kPgChunk, 1024);
-    const int kd16 = p.dp / 16;
-    auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
-      const bool ok = mbar_wait(bar, parity, p.status, where);
-      return __all_sync(0xffffffffu, ok) != 0;
-    };
-    auto issue_s = [&](int t, int q_tile, int stage) {
-      const uint64_t qd = q_desc + static_cast<uint64_t>(q_tile * q_bytes / 16);
-      const uint64_t kd = k_desc + static_cast<uint64_t>(stage * k_bytes / 16);
-      for (int k = 0; k < kd16; ++k) {
-        const uint64_t off = static_cast<uint64_t>((k >> 2) * (kPgChunk / 16) + (k & 3) * 2);
-        umma_bf16_if(leader, tmem + t * 128, qd + off, kd + off, idesc_s, k > 0 ? 1u : 0u);
-      }
-      tc_commit_if(leader, &s_full[t]);
-    };
-    auto issue_pv = [&](int t, int stage, bool first) {
-      const uint64_t vd = v_desc + static_cast<uint64_t>(stage * v_bytes / 16);
-#pragma unroll
-      for (int k = 0; k < kPgTile / 16; ++k)
-        umma_bf16_ts_if(leader, tmem + 256 + t * 128, tmem + t * 128 + 8 * k, vd + 128 * k, idesc_pv, first && k == 0 ? 0u : 1u);
-    };
+    const int whole = p.dp / 64, rest = p.dp / 16 - 4 * whole;
     bool ok = true;
     int kt = 0, done[2] = {0, 0}, live = 0;              // key tiles; products of each tile; units with work so far
     for (int unit = blockIdx.x; unit < units && ok; unit += gridDim.x) {
@@ -190,64 +165,70 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
       int first;
       const int n = span(it, first);
       if (n == 0) continue;
-      ok = wait(q_full, live & 1, 470);
-      ++live;
-      if (!ok) break;
-      tc_fence_after();
-      auto key_ready = [&](int j) { return wait(&k_full[(kt + j) % p.k_stages], ((kt + j) / p.k_stages) & 1, 471); };
-      auto value_ready = [&](int j) { return wait(&v_full[(kt + j) % p.v_stages], ((kt + j) / p.v_stages) & 1, 472); };
-      if (it.rows * p.n > kPgTile) {
-        ok = key_ready(0);
-        if (!ok) break;
+      if (leader) {                                      // one thread: votes and the like between two products cost as much as the products
+        ok = mbar_wait(q_full, live & 1, p.status, 470);
+        ++live;
         tc_fence_after();
-        issue_s(0, 0, kt % p.k_stages);
-        issue_s(1, 1, kt % p.k_stages);
-        tc_commit_if(leader, &k_empty[kt % p.k_stages]);
-        for (int j = 0; j < n && ok; ++j) {
-          const int vs = (kt + j) % p.v_stages, ks = (kt + j + 1) % p.k_stages;
-          ok = value_ready(j);
-          if (ok && j + 1 < n) ok = key_ready(j + 1);
-          if (!ok) break;
+        const bool both = it.rows * p.n <= kPgTile;
+        const int step = both ? 2 : 1;
+        // per tile: its next scores and next values, as numbers of key tiles; scores overwrite the P that the values before them read
+        int sj[2] = {0, both ? 1 : 0}, pj[2] = {0, both ? 1 : 0};
+        uint32_t idle = 0;
+        long long since = 0;
+        while (ok && (pj[0] < n || pj[1] < n)) {
+          bool moved = false;
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            if (ok) ok = wait(&p_full[t], done[t] & 1, 473 + t);
-            if (!ok) break;
-            ++done[t];
-            tc_fence_after();
-            issue_pv(t, vs, j == 0);
-            if (j == n - 1) tc_commit_if(leader, &o_full[t]);
-            if (t == 1) tc_commit_if(leader, &v_empty[vs]);
-            if (j + 1 < n) issue_s(t, t, ks);
+            if (pj[t] < sj[t] && pj[t] < n) {
+              const int at = kt + pj[t], stage = p.v_stages == 2 ? at & 1 : 0, phase = p.v_stages == 2 ? (at >> 1) & 1 : at & 1;
+              if (mbar_test_wait(&p_full[t], done[t] & 1) && mbar_test_wait(&v_full[stage], phase)) {
+                tc_fence_after();
+                const uint64_t vd = v_desc + static_cast<uint64_t>(stage * v_bytes / 16);
+                const uint32_t o = tmem + 256 + t * 128, a = tmem + t * 128;
+                umma4_ts<128>(o, a, vd, idesc_pv, pj[t] >= step);
+                umma4_ts<128>(o, a + 32, vd + 512, idesc_pv, 1u);
+                ++done[t];
+                if (both || pj[t ^ 1] > pj[t]) tc_commit_if(true, &v_empty[stage]);      // the tile's last reader
+                pj[t] += step;
+                if (pj[t] >= n) tc_commit_if(true, &o_full[t]);
+                moved = true;
+              }
+            }
+            if (sj[t] < n && sj[t] == pj[t]) {
+              const int at = kt + sj[t], stage = p.k_stages == 2 ? at & 1 : 0, phase = p.k_stages == 2 ? (at >> 1) & 1 : at & 1;
+              if (mbar_test_wait(&k_full[stage], phase)) {
+                tc_fence_after();
+                uint64_t a = q_desc + static_cast<uint64_t>(both ? 0 : t * q_bytes / 16), b = k_desc + static_cast<uint64_t>(stage * k_bytes / 16);
+#pragma unroll 1
+                for (int c = 0; c < whole; ++c, a += kPgChunk / 16, b += kPgChunk / 16) umma4_ss<2, 2>(tmem + t * 128, a, b, idesc_s, c);
+#pragma unroll 1
+                for (int k = 0; k < rest; ++k) umma_bf16(tmem + t * 128, a + 2 * k, b + 2 * k, idesc_s, whole > 0 || k > 0);
+                tc_commit_if(true, &s_full[t]);
+                if (both || sj[t ^ 1] > sj[t]) tc_commit_if(true, &k_empty[stage]);
+                sj[t] += step;
+                moved = true;
+              }
+            }
           }
-          if (ok && j + 1 < n) tc_commit_if(leader, &k_empty[ks]);
-        }
-      } else {
-        for (int j = 0; j < 2 && j < n && ok; ++j) {
-          ok = key_ready(j);
-          if (!ok) break;
-          tc_fence_after();
-          issue_s(j, 0, (kt + j) % p.k_stages);
-          tc_commit_if(leader, &k_empty[(kt + j) % p.k_stages]);
-        }
-        for (int j = 0; j < n && ok; ++j) {
-          const int t = j & 1, vs = (kt + j) % p.v_stages;
-          ok = value_ready(j) && wait(&p_full[t], done[t] & 1, 473 + t);
-          if (!ok) break;
-          ++done[t];
-          tc_fence_after();
-          issue_pv(t, vs, j < 2);
-          if (j + 2 >= n) tc_commit_if(leader, &o_full[t]);
-          tc_commit_if(leader, &v_empty[vs]);
-          if (j + 2 < n) {
-            ok = key_ready(j + 2);
-            if (!ok) break;
-            tc_fence_after();
-            issue_s(t, 0, (kt + j + 2) % p.k_stages);
-            tc_commit_if(leader, &k_empty[(kt + j + 2) % p.k_stages]);
+          if (moved) {
+            idle = 0;
+            since = 0;
+          } else if ((++idle & 0x3ff) == 0) {            // as long as any other wait: see mbar_wait
+            if (since == 0) since = clock64();
+            if (clock64() - since > DS41_WAIT_LIMIT_CYCLES ||
+                (p.status != nullptr && *reinterpret_cast<volatile int*>(p.status) != kStatusOk)) {
+              if (p.status != nullptr && atomicCAS(p.status, kStatusOk, kStatusMbarTimeout) == kStatusOk) {
+                p.status[1] = 471;
+                p.status[2] = static_cast<int>(blockIdx.x);
+                p.status[3] = pj[0];
+              }
+              ok = false;
+            }
           }
         }
+        kt += n;
       }
-      kt += n;
+      ok = __ballot_sync(0xffffffffu, leader && ok) != 0;
     }
   } else {
     const int t = warp >> 2, quad = warp & 3, tid = threadIdx.x, mine = quad * 32 + lane;
@@ -275,12 +256,22 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
       s_row[t * kPgTile + mine] = r;                     // equal in both halves where the queries are
       named_barrier(1, 2 * kPgTile);
       if (n > 0) {
-        const int pieces = p.dp / 8, q_tiles = both ? 1 : 2;
-        for (int i = tid; i < q_tiles * kPgTile * pieces; i += 2 * kPgTile) {
-          const int x = i / pieces, c = i % pieces, row = s_row[x], y = x & (kPgTile - 1);
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (row >= 0) v = *reinterpret_cast<const uint4*>(p.q + row * p.ld_q + 1ll * (g * p.n + x % p.n) * p.dp + 8 * c);
-          *reinterpret_cast<uint4*>(s_q + (x >> 7) * q_bytes + (c >> 3) * kPgChunk + y * 128 + (((c & 7) ^ (y & 7)) << 4)) = v;
+        // a row's 16-byte pieces by neighbouring lanes, four rows of a lane under way together
+        const int pieces = p.dp / 8, per = 32 / pieces, sub = lane / pieces, c = lane % pieces, rows = (both ? 1 : 2) * kPgTile;
+        for (int x0 = warp * per + sub; x0 < rows; x0 += 32 * per) {
+          uint4 v[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int x = x0 + 8 * per * k, row = sub < per && x < rows ? s_row[x] : -1;
+            v[k] = make_uint4(0, 0, 0, 0);
+            if (row >= 0) v[k] = *reinterpret_cast<const uint4*>(p.q + row * p.ld_q + 1ll * (g * p.n + x % p.n) * p.dp + 8 * c);
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int x = x0 + 8 * per * k, y = x & (kPgTile - 1);
+            if (sub < per && x < rows)
+              *reinterpret_cast<uint4*>(s_q + (x >> 7) * q_bytes + (c >> 3) * kPgChunk + y * 128 + (((c & 7) ^ (y & 7)) << 4)) = v[k];
+          }
         }
         fence_async_smem();
         mbar_arrive(q_full);
@@ -302,21 +293,28 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
         const int key0 = first + j * kPgTile;
         const bool edge = key0 < low || key0 + kPgTile > high;
         const int shown = hi - key0, hidden = lo - key0;             // columns [hidden, shown) of this tile are visible
+        // Two halves of 64 columns, each read twice: the loops' bodies have to stay in the instruction cache, which this code shares
+        // with the other roles' (unrolled over the tile, 42 % of all cycles were waits for instructions)
         float top = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t v[32];
-          tmem_ld_32x32(s_t + 32 * c, v);
+        uint32_t v[64];
+        auto load = [&](int c) {
+          tmem_ld_32x32(s_t + c, reinterpret_cast<uint32_t(&)[32]>(v[0]));
+          tmem_ld_32x32(s_t + c + 32, reinterpret_cast<uint32_t(&)[32]>(v[32]));
           tmem_wait_ld();
           if (edge) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (32 * c + i < shown && 32 * c + i >= hidden) top = fmaxf(top, __uint_as_float(v[i]) * p.scale_log2);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(v[i]) * p.scale_log2);
+            for (int i = 0; i < 64; ++i) v[i] = c + i < shown && c + i >= hidden ? v[i] : 0xff800000u;
           }
+        };
+#pragma unroll 1
+        for (int c = 0; c < kPgTile; c += 64) {
+          load(c);
+          float tops[4] = {top, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < 64; i += 2) tops[(i >> 1) & 3] = fmaxf(tops[(i >> 1) & 3], fmaxf(__uint_as_float(v[i]), __uint_as_float(v[i + 1])));
+          top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
         }
+        top *= p.scale_log2;
         const bool grow = top > m + 8.f || (m == -INFINITY && top > m);
         if (__any_sync(0xffffffffu, grow)) {
           const float m_new = grow ? top : m;
@@ -325,6 +323,7 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
           m = m_new;
           if (j > from) {
             const float keep = grow ? alpha : 1.f;
+#pragma unroll 1
             for (int c = 0; c < p.vp; c += 16) {
               uint32_t o[16];
               tmem_ld_32x16(o_t + c, o);
@@ -336,26 +335,24 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
           }
         }
         const float neg = m == -INFINITY ? 0.f : -m;
+        const float2 by = make_float2(p.scale_log2, p.scale_log2), off = make_float2(neg, neg);
+        float2 sums[2] = {};
+#pragma unroll 1
+        for (int c = 0; c < kPgTile; c += 64) {
+          load(c);
+          uint32_t w[32];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t v[32], w[16];
-          tmem_ld_32x32(s_t + 32 * c, v);
-          tmem_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float a = ex2_approx(fmaf(__uint_as_float(v[2 * i]), p.scale_log2, neg));
-            float b = ex2_approx(fmaf(__uint_as_float(v[2 * i + 1]), p.scale_log2, neg));
-            if (edge) {
-              const int x = 32 * c + 2 * i;
-              a = x < shown && x >= hidden ? a : 0.f;
-              b = x + 1 < shown && x + 1 >= hidden ? b : 0.f;
-            }
-            l += a + b;
-            const __nv_bfloat162 q = __floats2bfloat162_rn(a, b);
+          for (int i = 0; i < 32; ++i) {
+            float2 e = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), by, off);
+            e = make_float2(ex2_approx(e.x), ex2_approx(e.y));
+            sums[i & 1] = add2(sums[i & 1], e);
+            const __nv_bfloat162 q = __floats2bfloat162_rn(e.x, e.y);
             w[i] = *reinterpret_cast<const uint32_t*>(&q);
           }
-          tmem_st_32x16(s_t + 16 * c, w);                // columns whose S this thread has read
+          tmem_st_32x32(s_t + c / 2, w);                 // columns whose S this thread has read
         }
+        sums[0] = add2(sums[0], sums[1]);
+        l += sums[0].x + sums[0].y;
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&p_full[t]);
@@ -396,14 +393,14 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
           tmem_wait_ld();
           if (write) {
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-              float o[4];
+            for (int i = 0; i < 16; i += 8) {
+              float o[8];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
+              for (int e = 0; e < 8; ++e) {
                 o[e] = f0 * __uint_as_float(a[i + e]);
                 if (has[1] && both) o[e] += f1 * __uint_as_float(b[i + e]);
               }
-              *reinterpret_cast<float4*>(dst + c + i) = make_float4(o[0], o[1], o[2], o[3]);
+              store8(dst + c + i, o);
             }
           }
           __syncwarp();

@@ -249,25 +249,27 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
         h = mine % p.heads;
         if (p.row_slot[r] >= 0) hi = min(min(plan.own[r], p.row_pos[r] + 1), it.key1);
       }
-      // queries into tensor memory: 32 values at a time, the sets in turn
-      for (int c = set; c < 2 * (v_chunks + r_chunks); c += kPlSets) {
-        uint32_t w[16];
-        const bool lat = c < 2 * v_chunks;
-        const int d0 = lat ? v0 + 32 * c : 64 * r_chunk0 + 32 * (c - 2 * v_chunks), width = lat ? v1 : p.rp;
-        const __nv_bfloat16* src = r < 0 ? nullptr
-                                   : lat ? p.q_abs + r * p.ld_q_abs + 1ll * h * p.kvp + d0
+      // queries into tensor memory, the sets in turn: all of a thread's loads are under way together
+      {
+        constexpr int kMine = 2 * kPlMost / kPlSets;             // pieces of 32 values
+        uint4 v[kMine][4];
+#pragma unroll
+        for (int k = 0; k < kMine; ++k) {
+          const int c = set + kPlSets * k;
+          const bool lat = c < 2 * v_chunks;
+          const int d0 = lat ? v0 + 32 * c : 64 * r_chunk0 + 32 * (c - 2 * v_chunks), width = lat ? v1 : p.rp;
+          const __nv_bfloat16* src = lat ? p.q_abs + r * p.ld_q_abs + 1ll * h * p.kvp + d0
                                          : p.q_rot + r * p.ld_q_rot + 1ll * h * p.q_rot_stride + d0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (src != nullptr && d0 + 8 * i < width) v = *reinterpret_cast<const uint4*>(src + 8 * i);
-          w[4 * i] = v.x;
-          w[4 * i + 1] = v.y;
-          w[4 * i + 2] = v.z;
-          w[4 * i + 3] = v.w;
+          for (int i = 0; i < 4; ++i)
+            v[k][i] = r >= 0 && c < 2 * (v_chunks + r_chunks) && d0 + 8 * i < width ? *reinterpret_cast<const uint4*>(src + 8 * i)
+                                                                                   : make_uint4(0, 0, 0, 0);
         }
-        __syncwarp();
-        tmem_st_32x16(lanes + kPlQ + 16 * c, w);
+#pragma unroll
+        for (int k = 0; k < kMine; ++k) {
+          const int c = set + kPlSets * k;
+          if (c < 2 * (v_chunks + r_chunks)) tmem_st_32x16(lanes + kPlQ + 16 * c, reinterpret_cast<const uint32_t(&)[16]>(v[k][0]));
+        }
       }
       tmem_wait_st();
       tc_fence_before();
@@ -410,10 +412,8 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
           tmem_ld_32x16(lanes + c, o);
           tmem_wait_ld();
           if (write) {
-#pragma unroll
-            for (int i = 0; i < 16; i += 4)
-              *reinterpret_cast<float4*>(dst + c + i) = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]),
-                                                                    __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
+            store8(dst + c, reinterpret_cast<const float(&)[8]>(o[0]));
+            store8(dst + c + 8, reinterpret_cast<const float(&)[8]>(o[8]));
           }
           __syncwarp();
         }
