@@ -552,24 +552,21 @@ int ds41_latent_attend(const ds41_latent_attend_args* args, void* stream);
 int ds41_latent_merge(const float* part_o, const float* part_ml, const float* sink, int n_splits, int rows, int heads,
                       int kv_pad, void* out, int ld_out, int f32, void* stream);
 
-// Attention of rows whose page tables begin with the same pages: the common keys are read once for all of them (prefix_attn.cu),
-// every row's other keys by the forms below, which also join the parts.  Device arrays of the plan, made on the host:
+// Attention of rows whose page tables begin with the same pages (prefix_attn.cu, prefix_group.cu, prefix_latent.cu): common keys are
+// read once for all rows that share them.  Device arrays of the plan, made on the host:
 typedef struct ds41_prefix_plan {
-  const int* items;               // [max_items][8]: {slot, first, rows, first key, end key, part, 0, 0}
-  const int* n_items;             // how many there are
-  const int* order;               // pass rows by prefix: an item's rows are order[first] .. order[first + rows - 1]
-  const int* own;                 // [rows] first key that a row reads by itself
+  const int* units;               // [max_units][8]: {slot, first row, rows (0: none), first key, end key, part, tail, key/value head}
+  const int* n_units;             // how many there are
+  const int* order;               // pass rows by prefix: a unit's rows are order[first] .. order[first + rows - 1]; a tail's: first + i
   const int* cell;                // [rows] the row's first cell of part_o / part_ml
   const int* parts;               // [rows] how many it has
   float* part_o;                  // [cells][heads][value width] unnormalised results
-  float* part_ml;                 // [cells][heads]{maximum, sum}; grouped attention: of scores in units of log 2, latent: natural
-  int max_items, rows_per_item, grid;      // `grid`: blocks of the first launch, which walk the items
+  float* part_ml;                 // [cells][heads]{maximum in units of log 2, sum}
+  int max_units, rows_per_unit, grid;      // `grid`: blocks (or pairs of them) that walk the units
 } ds41_prefix_plan;
-// latent attention: the common keys, the own keys (ds41_latent_attend's partial results over them), and the join of both
-int ds41_prefix_latent_shared(const ds41_latent_attend_args* args, const ds41_prefix_plan* plan, int n_pages, void* stream);
-int ds41_prefix_latent_own(const ds41_latent_attend_args* args, const ds41_prefix_plan* plan, void* stream);
-int ds41_prefix_latent_merge(const float* part_o, const float* part_ml, const float* sink, const ds41_prefix_plan* plan,
-                             int n_splits, int rows, int heads, int kv_pad, void* out, int ld_out, int f32, void* stream);
+// Latent attention: ds41_latent_attend and ds41_latent_merge in two launches (part_o, part_ml, n_splits of the arguments are not used).
+int ds41_prefix_latent(const ds41_latent_attend_args* args, const ds41_prefix_plan* plan, int n_pages, const float* sink, void* out,
+                       int ld_out, void* stream);
 
 // Long prompt pass of one request over expanded keys and values (latent_prefill.cu): pass row r stands at position pos0 + r.
 typedef struct ds41_latent_prefill_args {
@@ -645,9 +642,8 @@ typedef struct ds41_group_attend_args {
 } ds41_group_attend_args;
 // Any mix of rows; n_splits <= 16 CTAs share a row's keys.
 int ds41_group_attend(const ds41_group_attend_args* args, void* stream);
-// The same in two launches for rows that share prefixes: the common keys, then the own ones and the join of the parts.
-int ds41_prefix_group_shared(const ds41_group_attend_args* args, const ds41_prefix_plan* plan, void* stream);
-int ds41_prefix_group_own(const ds41_group_attend_args* args, const ds41_prefix_plan* plan, void* stream);
+// The same in two launches for rows that share prefixes (n_splits is not used).
+int ds41_prefix_group(const ds41_group_attend_args* args, const ds41_prefix_plan* plan, void* stream);
 // Long prompt pass of one request (bf16, dim_pad <= 256, vdim_pad <= 128, pages of 32, 64 or 128 tokens): row r stands at
 // position pos0 + r.
 int ds41_group_prefill(const ds41_group_attend_args* args, void* stream);

@@ -1,35 +1,51 @@
-// What the kernels of attention over a shared prefix share (prefix_attn.cu, prefix_group.cu, prefix_latent.cu, and the forms of
-// group_attn.cu / latent_attn.cu that finish it).
+// What the kernels of attention over a shared prefix share (prefix_attn.cu, prefix_group.cu, prefix_latent.cu).
 //
-// Row r's keys are divided at own[r], a multiple of the page size: the positions below it lie in pages that several requests' page
-// tables begin with, and are read once for all of them; the row reads the others by itself.  Softmax over a divided set of keys
-// needs of every part only its maximum m, its sum l = sum exp(s - m) and its unnormalised result o = sum exp(s - m) v: with
-// M = max m_i the whole is sum exp(m_i - M) o_i / sum exp(m_i - M) l_i.
+// A row's keys are divided into parts: ranges of pages that several requests' page tables begin with, read once for all of them, and
+// ranges of its own.  Softmax over a divided set of keys needs of every part only its maximum m, its sum l = sum exp(s - m) and its
+// unnormalised result o = sum exp(s - m) v: with M = max m_i the whole is sum exp(m_i - M) o_i / sum exp(m_i - M) l_i.
 //
-// The plan is made on the host from the page tables (ops/prefix.py).  An item is a range of keys of one prefix and some of the
-// rows that share it; the parts of row r are the cells cell[r] .. cell[r] + parts[r] - 1 of [cell][head].
+// The plan is made on the host from the page tables (ops/prefix.py).  A unit is a range of keys, the rows that see them and a key/value
+// head; the parts of row r are the cells cell[r] .. cell[r] + parts[r] - 1 of [cell][head].  A tail is a range behind the shared
+// pages: its rows belong to one request, and it ends at the last of their positions, which the host does not know.
 #pragma once
-#include <type_traits>
-
 #include "ds41_stack.cuh"
 
 namespace ds41 {
 
-struct PrefixItem {
-  int slot, first, rows, key0, key1, split;      // rows order[first] .. of the pass; keys [key0, key1) of the slot's page table
+struct PrefixUnit {
+  int slot, first, rows, key0, key1, part, tail, head;
 };
-constexpr int kItemInts = 8;
+constexpr int kUnitInts = 8;
 
-__device__ __forceinline__ PrefixItem prefix_item(const ds41_prefix_plan& p, int i) {
-  const int4 a = *reinterpret_cast<const int4*>(p.items + 1ll * i * kItemInts);
-  const int2 b = *reinterpret_cast<const int2*>(p.items + 1ll * i * kItemInts + 4);
-  return {a.x, a.y, a.z, a.w, b.x, b.y};
+__device__ __forceinline__ PrefixUnit prefix_unit(const ds41_prefix_plan& p, int i) {
+  const int4 a = *reinterpret_cast<const int4*>(p.units + 1ll * i * kUnitInts);
+  const int4 b = *reinterpret_cast<const int4*>(p.units + 1ll * i * kUnitInts + 4);
+  return {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 }
-
-// a launch without a prefix
-struct NoPrefix {};
-template <typename X>
-constexpr bool kHasPrefix = !std::is_same<X, NoPrefix>::value;
+__device__ __forceinline__ int prefix_row(const ds41_prefix_plan& p, const PrefixUnit& u, int i) {
+  return u.tail ? u.first + i : p.order[u.first + i];
+}
+// Whole warps: the keys [first, end) that a unit's rows see.  A chunk's border may lie inside; `first` is a page's.
+__device__ __forceinline__ void prefix_span(const ds41_prefix_plan& p, const PrefixUnit& u, const int* row_pos, const int* row_slot,
+                                            int chunk, int page_tokens, int& first, int& end) {
+  first = u.key0;
+  end = u.key1;
+  if (chunk == 0 && !u.tail) return;
+  int low = u.key1, high = 0;
+  for (int i = threadIdx.x & 31; i < u.rows; i += 32) {
+    const int r = prefix_row(p, u, i), pos = row_pos[r];
+    if (row_slot[r] < 0) continue;
+    low = min(low, chunk > 0 ? pos - pos % chunk : 0);
+    high = max(high, pos + 1);
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    low = min(low, __shfl_xor_sync(0xffffffffu, low, o));
+    high = max(high, __shfl_xor_sync(0xffffffffu, high, o));
+  }
+  first = max(first, low - low % page_tokens);
+  end = max(first, min(end, high));
+}
 
 // Two 32-bit operations in one instruction.
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
@@ -86,10 +102,10 @@ __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
 }
 
 inline bool prefix_plan_ok(const ds41_prefix_plan* p) {
-  return p != nullptr && p->items != nullptr && p->n_items != nullptr && p->order != nullptr && p->own != nullptr &&
-         p->cell != nullptr && p->parts != nullptr && p->part_o != nullptr && p->part_ml != nullptr && p->max_items > 0 &&
-         p->rows_per_item > 0 && p->grid > 0 && !(reinterpret_cast<uintptr_t>(p->items) & 15) &&
-         !(reinterpret_cast<uintptr_t>(p->part_o) & 31) && !(reinterpret_cast<uintptr_t>(p->part_ml) & 7);
+  return p != nullptr && p->units != nullptr && p->n_units != nullptr && p->order != nullptr && p->cell != nullptr &&
+         p->parts != nullptr && p->part_o != nullptr && p->part_ml != nullptr && p->max_units > 0 && p->rows_per_unit > 0 &&
+         p->grid > 0 && !(reinterpret_cast<uintptr_t>(p->units) & 15) && !(reinterpret_cast<uintptr_t>(p->part_o) & 31) &&
+         !(reinterpret_cast<uintptr_t>(p->part_ml) & 7);
 }
 
 }  // namespace ds41

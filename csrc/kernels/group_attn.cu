@@ -16,7 +16,6 @@
 
 #include "ds41_group.cuh"
 #include "ds41_mma.cuh"
-#include "ds41_prefix.cuh"
 #include "ds41_tma.h"
 
 namespace ds41 {
@@ -416,47 +415,9 @@ static int launch_post_fast(const ds41_attn_post_args& a, cudaStream_t st, bool&
   return cudaSuccess;
 }
 
-// First key that a row reads by itself.
-__device__ __forceinline__ int own_start(const NoPrefix&, int, int first) { return first; }
-__device__ __forceinline__ int own_start(const ds41_prefix_plan& x, int r, int first) { return max(first, x.own[r]); }
-
-// Four columns of head h of row r over all parts: the row's own result o with maximum `top` (in units of log 2) and sum `sum`, and
-// the parts of its prefix.
-__device__ __forceinline__ void join_parts(const NoPrefix&, int, int, int, int, int, float4&, float&, float) {}
-__device__ __forceinline__ void join_parts(const ds41_prefix_plan& x, int r, int h, int heads, int vp, int c, float4& o, float& sum,
-                                           float top) {
-  const int n = x.parts[r];
-  if (n == 0) return;
-  const long long cell = 1ll * x.cell[r] * heads + h;
-  const float2* ml = reinterpret_cast<const float2*>(x.part_ml) + cell;
-  const float* part = x.part_o + cell * vp + c;
-  float all = top;
-#pragma unroll 4
-  for (int s = 0; s < n; ++s) all = fmaxf(all, ml[1ll * s * heads].x);
-  if (all == -INFINITY) return;
-  const float keep = top == -INFINITY ? 0.f : exp2f(top - all);
-  o.x *= keep;
-  o.y *= keep;
-  o.z *= keep;
-  o.w *= keep;
-  sum *= keep;
-#pragma unroll 4
-  for (int s = 0; s < n; ++s) {
-    const float2 t = ml[1ll * s * heads];
-    if (t.x == -INFINITY) continue;                  // the part holds nothing that this row sees: its values were not written
-    const float w = exp2f(t.x - all);
-    const float4 v = *reinterpret_cast<const float4*>(part + 1ll * s * heads * vp);
-    sum += w * t.y;
-    o.x += w * v.x;
-    o.y += w * v.y;
-    o.z += w * v.z;
-    o.w += w * v.w;
-  }
-}
-
 // Plain form for every type and size: one block per (head, row), a tile of 32 keys at a time.
-template <typename T, typename X>
-__global__ void __launch_bounds__(128) group_attend_plain_kernel(ds41_group_attend_args p, X prefix) {
+template <typename T>
+__global__ void __launch_bounds__(128) group_attend_plain_kernel(ds41_group_attend_args p) {
   extern __shared__ __align__(16) float ga_smem[];
   float* qs = ga_smem;                   // [dim_pad]
   float* os = qs + p.dim_pad;            // [vdim_pad] running output
@@ -481,7 +442,7 @@ __global__ void __launch_bounds__(128) group_attend_plain_kernel(ds41_group_atte
   auto at = [&](int key) {
     return cache_row(static_cast<const T*>(p.pool), p.page_table, p.max_pages, p.page_tokens, row_len, slot, key);
   };
-  for (int t0 = own_start(prefix, r, chunk_start(pos, p.chunk)); t0 <= pos; t0 += 32) {
+  for (int t0 = chunk_start(pos, p.chunk); t0 <= pos; t0 += 32) {
     for (int j = warp; j < 32; j += 4) {
       const T* kv = t0 + j <= pos ? at(t0 + j) : nullptr;
       float a = 0.f;
@@ -510,19 +471,8 @@ __global__ void __launch_bounds__(128) group_attend_plain_kernel(ds41_group_atte
     }
     __syncthreads();
   }
-  const float gate = p.gate.data != nullptr ? sigmoid_f32(proj_at(p.gate, r, h)) : 1.f;
-  if constexpr (kHasPrefix<X>) {
-    for (int i = 4 * tid; i < p.vdim_pad; i += 512) {
-      float4 o = *reinterpret_cast<const float4*>(os + i);
-      float sum = l;
-      join_parts(prefix, r, h, p.heads, p.vdim_pad, i, o, sum, m * 1.4426950408889634f);
-      const float f = (sum > 0.f ? 1.0f / sum : 0.f) * gate;
-      store4(out + i, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
-    }
-  } else {
-    const float f = (l > 0.f ? 1.0f / l : 0.f) * gate;
-    for (int i = tid; i < p.vdim_pad; i += 128) out[i] = from_f32<T>(os[i] * f);
-  }
+  const float f = (l > 0.f ? 1.0f / l : 0.f) * (p.gate.data != nullptr ? sigmoid_f32(proj_at(p.gate, r, h)) : 1.f);
+  for (int i = tid; i < p.vdim_pad; i += 128) out[i] = from_f32<T>(os[i] * f);
 }
 
 // bf16 form: CTA (split, key/value head and 16 of its query heads, row).  A producer warp brings tiles of 16 NW keys and values
@@ -567,10 +517,9 @@ inline bool plan_attend(const ds41_group_attend_args& a, AttendPlan& t) {
   return false;
 }
 
-template <int NW, int KD, int NP, typename X>
+template <int NW, int KD, int NP>
 __global__ void __launch_bounds__(32 * (NW + 1))
-group_attend_mma_kernel(const __grid_constant__ CUtensorMap pool, const ds41_group_attend_args p, const AttendPlan plan,
-                        const X prefix) {
+group_attend_mma_kernel(const __grid_constant__ CUtensorMap pool, const ds41_group_attend_args p, const AttendPlan plan) {
   constexpr int kTileKeys = 16 * NW, kTileChunk = kTileKeys * 128;      // bytes of a tile's rows x 64 bf16 columns
   extern __shared__ uint8_t gm_raw[];
   uint8_t* stages = gm_raw + ((1024u - (smem_u32(gm_raw) & 1023u)) & 1023u);
@@ -596,8 +545,8 @@ group_attend_mma_kernel(const __grid_constant__ CUtensorMap pool, const ds41_gro
   __syncthreads();                       // the barriers are ready
   pdl_wait();
   const int slot = p.row_slot[r], pos = p.row_pos[r];
-  const int first = own_start(prefix, r, chunk_start(pos, p.chunk)), base = first - first % plan.box;      // this CTA's tiles of keys
-  const int tiles = kHasPrefix<X> && first > pos ? 0 : (pos - base) / kTileKeys + 1, per = (tiles + p.n_splits - 1) / p.n_splits;
+  const int first = chunk_start(pos, p.chunk), base = first - first % plan.box;      // this CTA's tiles of keys
+  const int tiles = (pos - base) / kTileKeys + 1, per = (tiles + p.n_splits - 1) / p.n_splits;
   const int t0 = min(tiles, split * per), t1 = min(tiles, t0 + per);
   __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) + 1ll * r * p.ld_out;
   if (slot < 0) {                        // the same in every CTA of the cluster
@@ -740,30 +689,13 @@ group_attend_mma_kernel(const __grid_constant__ CUtensorMap pool, const ds41_gro
         // the accumulator layout of 16 x 16 scores is the operand layout of one 16-key product
         const uint32_t wa[4] = {pack_bf16(w[0][0], w[0][1]), pack_bf16(w[0][2], w[0][3]), pack_bf16(w[1][0], w[1][1]),
                                 pack_bf16(w[1][2], w[1][3])};
-        // what lies in the hidden places of a page is nobody's: a weight of zero does not take a NaN or an infinity away
-        bool edge = false;
-        uint32_t shown[2] = {~0u, ~0u};
-        if constexpr (kHasPrefix<X>) {
-          edge = key0 < first || key0 + 15 > pos;
-          if (edge)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const int key = key0 + 8 * u + q2;
-              shown[u] = (key >= first && key <= pos ? 0xffffu : 0u) | (key + 1 >= first && key + 1 <= pos ? 0xffff0000u : 0u);
-            }
-        }
 #pragma unroll
         for (int i0 = 0; i0 < NP; i0 += 4) {
           uint32_t b[4][4];
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (16 * (i0 + i) < vp) {
+            if (16 * (i0 + i) < vp)
               ldmatrix_x4_trans(b[i][0], b[i][1], b[i][2], b[i][3], swizzled(vt, vrow, 2 * (i0 + i) + vpiece));
-              if (edge) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) b[i][e] &= shown[e & 1];
-              }
-            }
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             if (16 * (i0 + i) < vp) {
@@ -800,10 +732,9 @@ group_attend_mma_kernel(const __grid_constant__ CUtensorMap pool, const ds41_gro
   }
   __syncthreads();
   const bool alone = p.n_splits == 1;
-  auto finish = [&](int row, int c, float4 o, float sum, float top) {
+  auto finish = [&](int row, int c, float4 o, float sum) {
     const int h = h0 + row;
     if (h >= h_end) return;
-    join_parts(prefix, r, h, p.heads, vp, c, o, sum, top);
     const float f = (sum > 0.f ? 1.0f / sum : 0.f) * (p.gate.data != nullptr ? sigmoid_f32(proj_at(p.gate, r, h)) : 1.f);
     store4(out + h * vp + c, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
   };
@@ -825,7 +756,7 @@ group_attend_mma_kernel(const __grid_constant__ CUtensorMap pool, const ds41_gro
       o.w += wk * v.w;
     }
     if (alone) {
-      finish(row, c, o, sum, top);
+      finish(row, c, o, sum);
     } else {
       *reinterpret_cast<float4*>(co + row * vp + c) = o;
       if (c == 0) {
@@ -853,21 +784,20 @@ group_attend_mma_kernel(const __grid_constant__ CUtensorMap pool, const ds41_gro
       o.z += wk * v.z;
       o.w += wk * v.w;
     }
-    finish(row, c, o, sum, top);
+    finish(row, c, o, sum);
   }
   cluster.sync();                        // peers may still read this CTA's partial results
 }
 
-template <int NW, int KD, int NP, typename X>
-static int launch_group_attend(const ds41_group_attend_args& a, const AttendPlan& plan, const X& prefix, cudaStream_t st) {
-  constexpr auto kernel = group_attend_mma_kernel<NW, KD, NP, X>;
+template <int NW, int KD, int NP>
+static int launch_group_attend(const ds41_group_attend_args& a, const AttendPlan& plan, cudaStream_t st) {
   const int smem = attend_smem(plan, a.dim_pad), row_len = a.kv_heads * (a.dim_pad + a.vdim_pad);
   static bool ready = false;
   cudaError_t e;
   if (!ready) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
+    e = cudaFuncSetAttribute(group_attend_mma_kernel<NW, KD, NP>, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
     if (e != cudaSuccess) return e;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    e = cudaFuncSetAttribute(group_attend_mma_kernel<NW, KD, NP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
     ready = true;
   }
@@ -877,36 +807,21 @@ static int launch_group_attend(const ds41_group_attend_args& a, const AttendPlan
   if (e != cudaSuccess) return e;
   const int m_tiles = (a.heads / a.kv_heads + 15) / 16;
   const dim3 grid(a.n_splits, a.kv_heads * m_tiles, a.rows), block(32 * (NW + 1));
-  if (a.n_splits == 1) return launch_pdl(kernel, grid, block, smem, st, pool, a, plan, prefix);
-  return launch_pdl_cluster(kernel, grid, block, a.n_splits, smem, st, pool, a, plan, prefix);
+  if (a.n_splits == 1) return launch_pdl(group_attend_mma_kernel<NW, KD, NP>, grid, block, smem, st, pool, a, plan);
+  return launch_pdl_cluster(group_attend_mma_kernel<NW, KD, NP>, grid, block, a.n_splits, smem, st, pool, a, plan);
 }
 
-template <typename X>
-static int dispatch_group_attend(const ds41_group_attend_args& a, const AttendPlan& plan, const X& prefix, cudaStream_t st) {
+static int dispatch_group_attend(const ds41_group_attend_args& a, const AttendPlan& plan, cudaStream_t st) {
   if (plan.warps == 8) {
-    if (a.dim_pad > 128) return launch_group_attend<8, 16, 8>(a, plan, prefix, st);
+    if (a.dim_pad > 128) return launch_group_attend<8, 16, 8>(a, plan, st);
     if (a.dim_pad > 64)
-      return a.vdim_pad <= 64 ? launch_group_attend<8, 8, 4>(a, plan, prefix, st) : launch_group_attend<8, 8, 8>(a, plan, prefix, st);
-    return a.vdim_pad <= 64 ? launch_group_attend<8, 4, 4>(a, plan, prefix, st) : launch_group_attend<8, 4, 8>(a, plan, prefix, st);
+      return a.vdim_pad <= 64 ? launch_group_attend<8, 8, 4>(a, plan, st) : launch_group_attend<8, 8, 8>(a, plan, st);
+    return a.vdim_pad <= 64 ? launch_group_attend<8, 4, 4>(a, plan, st) : launch_group_attend<8, 4, 8>(a, plan, st);
   }
-  if (a.dim_pad > 128) return launch_group_attend<4, 16, 16>(a, plan, prefix, st);
-  if (a.vdim_pad > 128) return launch_group_attend<4, 8, 16>(a, plan, prefix, st);
-  if (a.dim_pad > 64) return launch_group_attend<4, 8, 8>(a, plan, prefix, st);
-  return a.vdim_pad <= 64 ? launch_group_attend<4, 4, 4>(a, plan, prefix, st) : launch_group_attend<4, 4, 8>(a, plan, prefix, st);
-}
-
-template <typename X>
-static int run_group_attend(const ds41_group_attend_args* a, const X& prefix, void* stream) {
-  if (!group_attend_ok(a) || a->n_splits < 1 || a->n_splits > kAttendSplits || a->rows > 65535) return cudaErrorInvalidValue;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  AttendPlan plan;
-  if (plan_attend(*a, plan) && a->kv_heads * ((a->heads / a->kv_heads + 15) / 16) <= 65535)
-    return dispatch_group_attend(*a, plan, prefix, st);
-  const size_t smem = (1ull * a->dim_pad + a->vdim_pad + 32) * sizeof(float);
-  if (smem > 48 * 1024) return cudaErrorInvalidValue;
-  const dim3 grid(a->heads, a->rows);
-  return a->f32 ? launch_pdl(group_attend_plain_kernel<float, X>, grid, dim3(128), smem, st, *a, prefix)
-                : launch_pdl(group_attend_plain_kernel<__nv_bfloat16, X>, grid, dim3(128), smem, st, *a, prefix);
+  if (a.dim_pad > 128) return launch_group_attend<4, 16, 16>(a, plan, st);
+  if (a.vdim_pad > 128) return launch_group_attend<4, 8, 16>(a, plan, st);
+  if (a.dim_pad > 64) return launch_group_attend<4, 8, 8>(a, plan, st);
+  return a.vdim_pad <= 64 ? launch_group_attend<4, 4, 4>(a, plan, st) : launch_group_attend<4, 4, 8>(a, plan, st);
 }
 
 }  // namespace ds41
@@ -944,9 +859,15 @@ extern "C" int ds41_attn_post(const ds41_attn_post_args* a, void* stream) {
                 : launch_pdl(attn_post_kernel<__nv_bfloat16>, dim3(a->rows), block, smem, st, *a);
 }
 
-extern "C" int ds41_group_attend(const ds41_group_attend_args* a, void* stream) { return run_group_attend(a, NoPrefix{}, stream); }
-
-extern "C" int ds41_prefix_group_own(const ds41_group_attend_args* a, const ds41_prefix_plan* plan, void* stream) {
-  if (!prefix_plan_ok(plan) || a == nullptr || (a->ld_out & 3)) return cudaErrorInvalidValue;
-  return run_group_attend(a, *plan, stream);
+extern "C" int ds41_group_attend(const ds41_group_attend_args* a, void* stream) {
+  if (!group_attend_ok(a) || a->n_splits < 1 || a->n_splits > kAttendSplits || a->rows > 65535) return cudaErrorInvalidValue;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  AttendPlan plan;
+  if (plan_attend(*a, plan) && a->kv_heads * ((a->heads / a->kv_heads + 15) / 16) <= 65535)
+    return dispatch_group_attend(*a, plan, st);
+  const size_t smem = (1ull * a->dim_pad + a->vdim_pad + 32) * sizeof(float);
+  if (smem > 48 * 1024) return cudaErrorInvalidValue;
+  const dim3 grid(a->heads, a->rows);
+  return a->f32 ? launch_pdl(group_attend_plain_kernel<float>, grid, dim3(128), smem, st, *a)
+                : launch_pdl(group_attend_plain_kernel<__nv_bfloat16>, grid, dim3(128), smem, st, *a);
 }

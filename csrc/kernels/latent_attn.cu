@@ -11,7 +11,7 @@
 #include <type_traits>
 
 #include "ds41_mma.cuh"
-#include "ds41_prefix.cuh"
+#include "ds41_stack.cuh"
 #include "ds41_tma.h"
 
 namespace ds41 {
@@ -198,13 +198,9 @@ __global__ void __launch_bounds__(256) latent_gather_kernel(const T* pool, const
   }
 }
 
-// First key that a row reads by itself (past L1 where it is asked for again behind the wait).
-__device__ __forceinline__ int own_start(const NoPrefix&, int) { return 0; }
-__device__ __forceinline__ int own_start(const ds41_prefix_plan& x, int r) { return __ldcg(x.own + r); }
-
 // Plain form for every type and size: one block per (row, head, split), a tile of 32 keys at a time.
-template <typename T, typename X>
-__global__ void __launch_bounds__(128) latent_attend_plain_kernel(ds41_latent_attend_args p, X prefix) {
+template <typename T>
+__global__ void __launch_bounds__(128) latent_attend_plain_kernel(ds41_latent_attend_args p) {
   extern __shared__ float att_smem[];
   float* qs = att_smem;                  // [kv_pad + rot_pad] query, scaled
   float* os = qs + p.row_len;            // [kv_pad] running output
@@ -214,10 +210,10 @@ __global__ void __launch_bounds__(128) latent_attend_plain_kernel(ds41_latent_at
   pdl_launch_dependents();
   pdl_wait();
   const int slot = p.row_slot[r], pos = p.row_pos[r];
-  const int first = own_start(prefix, r), n_keys = slot < 0 ? 0 : pos + 1;
-  int per = (max(0, n_keys - first) + p.n_splits - 1) / p.n_splits;
+  const int n_keys = slot < 0 ? 0 : pos + 1;
+  int per = (n_keys + p.n_splits - 1) / p.n_splits;
   per = (per + 63) / 64 * 64;
-  const int k0 = first + split * per, k1 = min(n_keys, k0 + per);
+  const int k0 = split * per, k1 = min(n_keys, k0 + per);
   const long long cell = (1ll * r * p.n_splits + split) * p.heads + h;
   if (k0 >= k1) {
     if (tid == 0) {
@@ -286,8 +282,8 @@ __host__ __device__ constexpr int attend_mma_bytes(int mt, int row_len) {
   return (mt * 16 + 2 * kKeyTile) * (row_len + 8) * 2 + mt * 16 * kProbStride * 2 + mt * 64 * 4 + 3 * 8;
 }
 
-template <int MT, int PW, int NP, typename X>
-__global__ void __launch_bounds__(MT * PW * 32) latent_attend_mma_kernel(ds41_latent_attend_args p, int early, X prefix) {
+template <int MT, int PW, int NP>
+__global__ void __launch_bounds__(MT * PW * 32) latent_attend_mma_kernel(ds41_latent_attend_args p, int early) {
   extern __shared__ __align__(16) uint8_t la_smem[];
   const int RL = p.row_len, RS = RL + 8;
   __nv_bfloat16* sq = reinterpret_cast<__nv_bfloat16*>(la_smem);              // [MT * 16][RS]
@@ -309,9 +305,8 @@ __global__ void __launch_bounds__(MT * PW * 32) latent_attend_mma_kernel(ds41_la
   auto find = [&]() {
     slot = __ldcg(p.row_slot + r);       // again behind the wait: past L1, which may hold what stood there before
     const int n_keys = slot < 0 ? 0 : __ldcg(p.row_pos + r) + 1;
-    const int first = own_start(prefix, r);
-    const int per = ((max(0, n_keys - first) + kKeyTile - 1) / kKeyTile + p.n_splits - 1) / p.n_splits * kKeyTile;
-    k0 = first + split * per;
+    const int per = ((n_keys + kKeyTile - 1) / kKeyTile + p.n_splits - 1) / p.n_splits * kKeyTile;
+    k0 = split * per;
     k1 = min(n_keys, k0 + per);
   };
   auto locate = [&](int key) {           // threads of the first two warps: where the row of a key lies
@@ -515,13 +510,12 @@ __global__ void __launch_bounds__(MT * PW * 32) latent_attend_mma_kernel(ds41_la
   }
 }
 
-template <int MT, int PW, int NP, typename X>
-static int launch_attend_mma(const ds41_latent_attend_args& a, const X& prefix, cudaStream_t st) {
-  constexpr auto kernel = latent_attend_mma_kernel<MT, PW, NP, X>;
+template <int MT, int PW, int NP>
+static int launch_attend_mma(const ds41_latent_attend_args& a, cudaStream_t st) {
   const int smem = attend_mma_bytes(MT, a.row_len);
   static int allowed = 47 * 1024;
   if (smem > allowed) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const cudaError_t e = cudaFuncSetAttribute(latent_attend_mma_kernel<MT, PW, NP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     allowed = smem;
   }
@@ -529,17 +523,17 @@ static int launch_attend_mma(const ds41_latent_attend_args& a, const X& prefix, 
   // Keys are asked for early by grids that run at once: later blocks would only ask twice.  32 rows x 32 heads (160 blocks) over 300 keys
   // 16.2 us with it, 15.2 without; 4097 keys 63.6 and 60.5; one row over 64 keys from memory 4.7 and 5.8.
   const int early = 1ll * grid.x * grid.y * grid.z <= sm_count();
-  return launch_pdl(kernel, grid, dim3(MT * PW * 32), smem, st, a, early, prefix);
+  return launch_pdl(latent_attend_mma_kernel<MT, PW, NP>, grid, dim3(MT * PW * 32), smem, st, a, early);
 }
 
 // eight warps in every form: for 16 heads the second four share the latent columns only
-template <int MT, typename X>
-static int dispatch_attend_mma(const ds41_latent_attend_args& a, const X& prefix, cudaStream_t st) {
+template <int MT>
+static int dispatch_attend_mma(const ds41_latent_attend_args& a, cudaStream_t st) {
   constexpr int PW = 8 / MT;
-  if (a.kv_pad <= 16 * PW) return launch_attend_mma<MT, PW, 1>(a, prefix, st);
-  if (a.kv_pad <= 32 * PW) return launch_attend_mma<MT, PW, 2>(a, prefix, st);
-  if (MT == 1 || a.kv_pad <= 64 * PW) return launch_attend_mma<MT, PW, 4>(a, prefix, st);      // at most 512 values
-  return launch_attend_mma<MT, MT == 1 ? 8 : PW, MT == 1 ? 4 : 8>(a, prefix, st);
+  if (a.kv_pad <= 16 * PW) return launch_attend_mma<MT, PW, 1>(a, st);
+  if (a.kv_pad <= 32 * PW) return launch_attend_mma<MT, PW, 2>(a, st);
+  if (MT == 1 || a.kv_pad <= 64 * PW) return launch_attend_mma<MT, PW, 4>(a, st);      // at most 512 values
+  return launch_attend_mma<MT, MT == 1 ? 8 : PW, MT == 1 ? 4 : 8>(a, st);
 }
 
 // heads per CTA of the tensor-core form for this row length (0: it does not fit, the plain form runs)
@@ -702,8 +696,7 @@ extern "C" int ds41_latent_gather(const void* pool, const int* page_table, int m
                     static_cast<__nv_bfloat16*>(lat), static_cast<__nv_bfloat16*>(rot));
 }
 
-template <typename X>
-static int run_latent_attend(const ds41_latent_attend_args* a, const X& prefix, void* stream) {
+extern "C" int ds41_latent_attend(const ds41_latent_attend_args* a, void* stream) {
   if (a == nullptr || a->rows <= 0 || a->rows > 65535 || a->heads <= 0 || a->n_splits <= 0 || a->n_splits > 65535 ||
       a->kv_pad <= 0 || a->row_len < a->kv_pad || a->page_tokens <= 0 || a->max_pages <= 0 || a->q_abs == nullptr ||
       (a->row_len > a->kv_pad && a->q_rot == nullptr) || a->pool == nullptr || a->page_table == nullptr ||
@@ -711,22 +704,13 @@ static int run_latent_attend(const ds41_latent_attend_args* a, const X& prefix, 
     return cudaErrorInvalidValue;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int mma_heads = attend_mma_heads(*a);
-  if (mma_heads == 32) return dispatch_attend_mma<2>(*a, prefix, st);
-  if (mma_heads == 16) return dispatch_attend_mma<1>(*a, prefix, st);
+  if (mma_heads == 32) return dispatch_attend_mma<2>(*a, st);
+  if (mma_heads == 16) return dispatch_attend_mma<1>(*a, st);
   const size_t smem = (1ull * a->row_len + a->kv_pad + 32) * sizeof(float);
   if (smem > 48 * 1024) return cudaErrorInvalidValue;
   const dim3 grid(a->heads, a->n_splits, a->rows);
-  return a->f32 ? launch_pdl(latent_attend_plain_kernel<float, X>, grid, dim3(128), smem, st, *a, prefix)
-                : launch_pdl(latent_attend_plain_kernel<__nv_bfloat16, X>, grid, dim3(128), smem, st, *a, prefix);
-}
-
-extern "C" int ds41_latent_attend(const ds41_latent_attend_args* a, void* stream) {
-  return run_latent_attend(a, NoPrefix{}, stream);
-}
-
-extern "C" int ds41_prefix_latent_own(const ds41_latent_attend_args* a, const ds41_prefix_plan* plan, void* stream) {
-  if (!prefix_plan_ok(plan)) return cudaErrorInvalidValue;
-  return run_latent_attend(a, *plan, stream);
+  return a->f32 ? launch_pdl(latent_attend_plain_kernel<float>, grid, dim3(128), smem, st, *a)
+                : launch_pdl(latent_attend_plain_kernel<__nv_bfloat16>, grid, dim3(128), smem, st, *a);
 }
 
 extern "C" int ds41_latent_merge(const float* part_o, const float* part_ml, const float* sink, int n_splits, int rows,

@@ -1,9 +1,10 @@
-// Attention over the common keys of rows that share a prefix, for every type and size, and the join of latent attention's parts.
+// Attention of rows that share prefixes: its parts for every type and size, and their join.
 //
-// A block takes sixteen queries (head and row) of an item and walks its keys 32 at a time through shared memory, so that a cached
+// A block takes sixteen queries (head and row) of a unit and walks its keys 32 at a time through shared memory, so that a cached
 // value that was read once serves sixteen queries: scores by 256 threads of two (query, key) pairs each, a softmax state per query
 // (running maximum and sum), results in registers.  It serves 32-bit rows and the sizes that the tensor-core forms
 // (prefix_group.cu, prefix_latent.cu) leave out, and is bound by its 32-bit products and their operands from shared memory.
+#include "ds41_group.cuh"
 #include "ds41_prefix.cuh"
 #include "ds41_tma.h"
 
@@ -23,7 +24,7 @@ struct SimpleArgs {
   int d1, d2, vp, row_len;
   int k_lane, v_at, v_lane;          // key / value head g of a cache row: keys at g * k_lane, values at v_at + g * v_lane
   int lanes, per_lane, heads, chunk, max_pages, page_tokens;
-  float scale, unit;                 // of the maximum that is stored, in units of log 2
+  float scale;
 };
 
 inline int simple_smem(const SimpleArgs& p) {
@@ -56,21 +57,21 @@ __global__ void __launch_bounds__(256) prefix_simple_kernel(const SimpleArgs p, 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_launch_dependents();
   pdl_wait();
-  const int subs = (plan.rows_per_item * p.per_lane + kSimpleQueries - 1) / kSimpleQueries;
-  const int units = *plan.n_items * p.lanes * subs;
+  const int subs = (plan.rows_per_unit * p.per_lane + kSimpleQueries - 1) / kSimpleQueries;
+  const int units = *plan.n_units * subs;
   for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
-    const PrefixItem it = prefix_item(plan, unit / (p.lanes * subs));
-    const int g = unit / subs % p.lanes, i0 = unit % subs * kSimpleQueries, count = it.rows * p.per_lane;
+    const PrefixUnit it = prefix_unit(plan, unit / subs);
+    const int g = it.head, i0 = unit % subs * kSimpleQueries, count = it.rows * p.per_lane;
     if (i0 >= count) continue;
     __syncthreads();                     // the last unit's shared memory is no longer read
     if (tid < kSimpleQueries) {
       int r = -1, lo = 0, hi = 0;
       if (i0 + tid < count) {
-        r = plan.order[it.first + (i0 + tid) / p.per_lane];
+        r = prefix_row(plan, it, (i0 + tid) / p.per_lane);
         const int pos = p.row_pos[r];
         if (p.row_slot[r] >= 0) {
           lo = p.chunk > 0 ? pos - pos % p.chunk : 0;
-          hi = min(min(plan.own[r], pos + 1), it.key1);
+          hi = min(pos + 1, it.key1);
         }
       }
       row_of[tid] = r;
@@ -169,9 +170,9 @@ __global__ void __launch_bounds__(256) prefix_simple_kernel(const SimpleArgs p, 
         const int r = row_of[u0 + u];
         if (r < 0) continue;
         const int h = g * p.per_lane + (i0 + u0 + u) % p.per_lane;
-        const long long cell = (1ll * plan.cell[r] + it.split) * p.heads + h;
+        const long long cell = (1ll * plan.cell[r] + it.part) * p.heads + h;
         *reinterpret_cast<float4*>(plan.part_o + cell * p.vp + 4 * col) = acc[u];
-        if (col == 0) *reinterpret_cast<float2*>(plan.part_ml + 2 * cell) = make_float2(ms[u0 + u] * p.unit, ls[u0 + u]);
+        if (col == 0) *reinterpret_cast<float2*>(plan.part_ml + 2 * cell) = make_float2(ms[u0 + u] * 1.4426950408889634f, ls[u0 + u]);
       }
   }
 }
@@ -182,7 +183,7 @@ static int launch_simple(const SimpleArgs& p, const ds41_prefix_plan& plan, cuda
   if (smem > 220 * 1024) return cudaErrorInvalidValue;
   const cudaError_t e = cudaFuncSetAttribute(prefix_simple_kernel<T, QPT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  const long long most = 1ll * plan.max_items * p.lanes * ((plan.rows_per_item * p.per_lane + kSimpleQueries - 1) / kSimpleQueries);
+  const long long most = 1ll * plan.max_units * ((plan.rows_per_unit * p.per_lane + kSimpleQueries - 1) / kSimpleQueries);
   const int blocks = static_cast<int>(most < 4 * sm_count() ? most : 4 * sm_count());
   return launch_pdl(prefix_simple_kernel<T, QPT>, dim3(blocks), dim3(256), smem, st, p, plan);
 }
@@ -206,118 +207,119 @@ static int run_simple(const SimpleArgs& p, const ds41_prefix_plan& plan, int f32
   return f32 ? dispatch_simple<float>(p, plan, st) : dispatch_simple<__nv_bfloat16>(p, plan, st);
 }
 
-// One block per (head, row): the cells are the row's own splits, then the parts of its prefix.
-constexpr int kMaxCells = 256;
+// A warp joins 128 columns of a (row, head): the lanes find the parts' weights, then every lane sums four columns over the parts, eight
+// of them under way together.  Rows without a slot have no parts and become zero.  The launch also keeps the convolution's last
+// inputs where the attention has one (ds41_group.cuh).
 template <typename T>
-__global__ void __launch_bounds__(128) prefix_merge_kernel(const float* part_o, const float* part_ml, const float* sink,
-                                                           const ds41_prefix_plan plan, int n_splits, int heads, int kv_pad, T* out,
-                                                           int ld_out) {
-  __shared__ float wt[kMaxCells];
-  __shared__ float red[33], tops[4];
-  const int h = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
+__global__ void __launch_bounds__(128) prefix_join_kernel(const ds41_prefix_plan plan, const float* sink, const ds41_proj gate, int rows,
+                                                          int heads, int vp, T* out, int ld_out, const ds41_group_attend_args keep) {
+  const int lane = threadIdx.x & 31, strips = (vp + 127) / 128;
+  const long long w = 4ll * blockIdx.x + (threadIdx.x >> 5);
+  const int r = static_cast<int>(w / (heads * strips)), h = static_cast<int>(w / strips % heads), c = static_cast<int>(w % strips) * 128 + 4 * lane;
   pdl_launch_dependents();
   pdl_wait();
-  const int parts = min(plan.parts[r], kMaxCells - n_splits), n = n_splits + parts;
-  const long long own0 = 1ll * r * n_splits * heads + h, far0 = 1ll * plan.cell[r] * heads + h;
-  const float sk = sink != nullptr ? sink[h] : -INFINITY;
-  float2 ml[kMaxCells / 128];
-  float m = sk;
+  if (r >= rows) return;
+  if (keep.taps > 1 && keep.row_slot[r] >= 0)
+    keep_inputs(keep, r, keep.row_slot[r], keep.row_pos[r], static_cast<int>(w % (heads * strips)), heads * strips, lane, 32);
+  const int n = plan.parts[r];
+  const long long cell = 1ll * plan.cell[r] * heads + h;
+  const float2* ml = reinterpret_cast<const float2*>(plan.part_ml) + cell;
+  const float* part = plan.part_o + cell * vp + c;
+  const long long step = 1ll * heads * vp;
+  const float sk = sink != nullptr ? sink[h] * 1.4426950408889634f : -INFINITY;
+  float all = sk;
+  for (int s = lane; s < n; s += 32) all = fmaxf(all, ml[1ll * s * heads].x);
+  all = warp_max(all);
+  float den = sink != nullptr && lane == 0 && all > -INFINITY ? exp2f(sk - all) : 0.f;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s0 = 0; s0 < n; s0 += 32) {
+    float2 mine = make_float2(-INFINITY, 0.f);
+    if (s0 + lane < n) mine = ml[1ll * (s0 + lane) * heads];
+    const float e = mine.x > -INFINITY ? exp2f(mine.x - all) : 0.f;
+    den += e * mine.y;
+    for (int k0 = 0; k0 < 32 && s0 + k0 < n; k0 += 8) {
+      float4 o[8];
+      float f[8];
 #pragma unroll
-  for (int j = 0; j < kMaxCells / 128; ++j) {
-    const int s = tid + 128 * j;
-    ml[j] = make_float2(-INFINITY, 0.f);
-    if (s < n)
-      ml[j] = s < n_splits ? *reinterpret_cast<const float2*>(part_ml + 2 * (own0 + 1ll * s * heads))
-                           : *reinterpret_cast<const float2*>(plan.part_ml + 2 * (far0 + 1ll * (s - n_splits) * heads));
-    m = fmaxf(m, ml[j].x);
-  }
-  m = warp_max(m);
-  if ((tid & 31) == 0) tops[tid >> 5] = m;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < 4; ++w) m = fmaxf(m, tops[w]);
-  float den = 0.f;
-#pragma unroll
-  for (int j = 0; j < kMaxCells / 128; ++j) {
-    const float e = ml[j].x > -INFINITY ? expf(ml[j].x - m) : 0.f;
-    if (tid + 128 * j < n) wt[tid + 128 * j] = e;
-    den += e * ml[j].y;
-  }
-  den = block_sum(den, red) + (sink != nullptr && m > -INFINITY ? expf(sk - m) : 0.f);
-  const float inv = den > 0.f ? 1.0f / den : 0.f;
-  for (int i = 4 * tid; i < kv_pad; i += 512) {
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    const long long step = 1ll * heads * kv_pad;
-    const float* own = part_o + own0 * kv_pad + i;
-    const float* far = plan.part_o + far0 * kv_pad + i;
-#pragma unroll 8
-    for (int s = 0; s < n; ++s) {
-      const float e = wt[s];
-      if (e > 0.f) {
-        const float4 o = *reinterpret_cast<const float4*>(s < n_splits ? own + s * step : far + (s - n_splits) * step);
-        a.x += e * o.x;
-        a.y += e * o.y;
-        a.z += e * o.z;
-        a.w += e * o.w;
+      for (int k = 0; k < 8; ++k) {
+        f[k] = __shfl_sync(0xffffffffu, e, k0 + k);
+        // a part without a weight may hold anything: nothing may have been written
+        if (f[k] > 0.f && c < vp) o[k] = *reinterpret_cast<const float4*>(part + (s0 + k0 + k) * step);
       }
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (f[k] > 0.f && c < vp) {
+          a.x += f[k] * o[k].x;
+          a.y += f[k] * o[k].y;
+          a.z += f[k] * o[k].z;
+          a.w += f[k] * o[k].w;
+        }
     }
-    store4(out + 1ll * r * ld_out + h * kv_pad + i, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
   }
+  den = warp_sum(den);
+  const float f = (den > 0.f ? 1.0f / den : 0.f) * (gate.data != nullptr ? sigmoid_f32(proj_at(gate, r, h)) : 1.f);
+  if (c < vp) store4(out + 1ll * r * ld_out + h * vp + c, make_float4(a.x * f, a.y * f, a.z * f, a.w * f));
+}
+
+template <typename T>
+static int launch_join(const ds41_prefix_plan& plan, const float* sink, const ds41_proj& gate, int rows, int heads, int vp, void* out,
+                       int ld_out, const ds41_group_attend_args& keep, cudaStream_t st) {
+  const long long warps = 1ll * rows * heads * ((vp + 127) / 128);
+  return launch_pdl(prefix_join_kernel<T>, dim3(static_cast<unsigned>((warps + 3) / 4)), dim3(128), 0, st, plan, sink, gate, rows, heads,
+                    vp, static_cast<T*>(out), ld_out, keep);
 }
 
 }  // namespace ds41
 
 using namespace ds41;
 
-extern "C" int ds41_prefix_group_shared(const ds41_group_attend_args* a, const ds41_prefix_plan* plan, void* stream) {
-  if (!prefix_plan_ok(plan) || a == nullptr || a->rows <= 0 || a->heads <= 0 || a->kv_heads <= 0 || a->heads % a->kv_heads != 0 ||
-      a->dim_pad <= 0 || (a->dim_pad & 15) || a->vdim_pad <= 0 || (a->vdim_pad & 15) || a->chunk < 0 || a->max_pages <= 0 ||
-      a->page_tokens <= 0 || a->q == nullptr || a->pool == nullptr || a->page_table == nullptr || a->row_pos == nullptr ||
-      a->row_slot == nullptr || a->ld_q < 1ll * a->heads * a->dim_pad)
+extern "C" int ds41_prefix_group(const ds41_group_attend_args* a, const ds41_prefix_plan* plan, void* stream) {
+  if (!prefix_plan_ok(plan) || !group_attend_ok(a) || (a->ld_out & 3) || (reinterpret_cast<uintptr_t>(a->out) & (a->f32 ? 15 : 7)))
     return cudaErrorInvalidValue;
-  const int done = launch_prefix_group(*a, *plan, static_cast<cudaStream_t>(stream));
-  if (done != cudaErrorNotSupported) return done;
-  SimpleArgs p{};
-  p.q = a->q; p.q2 = a->q; p.pool = a->pool;
-  p.page_table = a->page_table; p.row_pos = a->row_pos; p.row_slot = a->row_slot;
-  p.ld_q = a->ld_q; p.q_head = a->dim_pad; p.d1 = a->dim_pad; p.vp = a->vdim_pad;
-  p.row_len = a->kv_heads * (a->dim_pad + a->vdim_pad);
-  p.k_lane = a->dim_pad; p.v_at = a->kv_heads * a->dim_pad; p.v_lane = a->vdim_pad;
-  p.lanes = a->kv_heads; p.per_lane = a->heads / a->kv_heads; p.heads = a->heads;
-  p.chunk = a->chunk; p.max_pages = a->max_pages; p.page_tokens = a->page_tokens;
-  p.scale = a->scale; p.unit = 1.4426950408889634f;
-  return run_simple(p, *plan, a->f32, static_cast<cudaStream_t>(stream));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  int e = launch_prefix_group(*a, *plan, st);
+  if (e == cudaErrorNotSupported) {
+    SimpleArgs p{};
+    p.q = a->q; p.q2 = a->q; p.pool = a->pool;
+    p.page_table = a->page_table; p.row_pos = a->row_pos; p.row_slot = a->row_slot;
+    p.ld_q = a->ld_q; p.q_head = a->dim_pad; p.d1 = a->dim_pad; p.vp = a->vdim_pad;
+    p.row_len = a->kv_heads * (a->dim_pad + a->vdim_pad);
+    p.k_lane = a->dim_pad; p.v_at = a->kv_heads * a->dim_pad; p.v_lane = a->vdim_pad;
+    p.lanes = a->kv_heads; p.per_lane = a->heads / a->kv_heads; p.heads = a->heads;
+    p.chunk = a->chunk; p.max_pages = a->max_pages; p.page_tokens = a->page_tokens;
+    p.scale = a->scale;
+    e = run_simple(p, *plan, a->f32, st);
+  }
+  if (e != cudaSuccess) return e;
+  return a->f32 ? launch_join<float>(*plan, nullptr, a->gate, a->rows, a->heads, a->vdim_pad, a->out, a->ld_out, *a, st)
+                : launch_join<__nv_bfloat16>(*plan, nullptr, a->gate, a->rows, a->heads, a->vdim_pad, a->out, a->ld_out, *a, st);
 }
 
-extern "C" int ds41_prefix_latent_shared(const ds41_latent_attend_args* a, const ds41_prefix_plan* plan, int n_pages, void* stream) {
-  if (!prefix_plan_ok(plan) || a == nullptr || a->rows <= 0 || a->heads <= 0 || a->kv_pad <= 0 || (a->kv_pad & 3) ||
+extern "C" int ds41_prefix_latent(const ds41_latent_attend_args* a, const ds41_prefix_plan* plan, int n_pages, const float* sink, void* out,
+                                  int ld_out, void* stream) {
+  if (!prefix_plan_ok(plan) || a == nullptr || a->rows <= 0 || a->heads <= 0 || a->heads > 65535 || a->kv_pad <= 0 || (a->kv_pad & 3) ||
       a->row_len < a->kv_pad || (a->row_len & 3) || n_pages <= 0 || a->max_pages <= 0 || a->page_tokens <= 0 || a->q_abs == nullptr ||
       (a->row_len > a->kv_pad && a->q_rot == nullptr) || a->pool == nullptr || a->page_table == nullptr || a->row_pos == nullptr ||
-      a->row_slot == nullptr)
+      a->row_slot == nullptr || out == nullptr || ld_out < a->heads * a->kv_pad || (ld_out & 3) ||
+      (reinterpret_cast<uintptr_t>(out) & (a->f32 ? 15 : 7)))
     return cudaErrorInvalidValue;
-  const int done = launch_prefix_latent(*a, *plan, n_pages, static_cast<cudaStream_t>(stream));
-  if (done != cudaErrorNotSupported) return done;
-  SimpleArgs p{};
-  p.q = a->q_abs; p.q2 = a->q_rot; p.pool = a->pool;
-  p.page_table = a->page_table; p.row_pos = a->row_pos; p.row_slot = a->row_slot;
-  p.ld_q = a->ld_q_abs; p.q_head = a->kv_pad; p.ld_q2 = a->ld_q_rot; p.q2_head = a->q_rot_stride;
-  p.d1 = a->kv_pad; p.d2 = a->row_len - a->kv_pad; p.vp = a->kv_pad; p.row_len = a->row_len;
-  p.lanes = 1; p.per_lane = a->heads; p.heads = a->heads;
-  p.max_pages = a->max_pages; p.page_tokens = a->page_tokens;
-  p.scale = a->scale; p.unit = 1.f;
-  return run_simple(p, *plan, a->f32, static_cast<cudaStream_t>(stream));
-}
-
-extern "C" int ds41_prefix_latent_merge(const float* part_o, const float* part_ml, const float* sink, const ds41_prefix_plan* plan,
-                                        int n_splits, int rows, int heads, int kv_pad, void* out, int ld_out, int f32, void* stream) {
-  if (!prefix_plan_ok(plan) || part_o == nullptr || part_ml == nullptr || n_splits <= 0 || n_splits > 64 || (kv_pad & 3) || kv_pad <= 0 ||
-      rows <= 0 || rows > 65535 || heads <= 0 || out == nullptr || ld_out < heads * kv_pad || (ld_out & 3))
-    return cudaErrorInvalidValue;
-  const dim3 grid(heads, rows);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  auto launch = [&](auto kernel, auto* o) {
-    return launch_pdl(kernel, grid, dim3(128), 0, st, part_o, part_ml, sink, *plan, n_splits, heads, kv_pad, o, ld_out);
-  };
-  return f32 ? launch(prefix_merge_kernel<float>, static_cast<float*>(out))
-             : launch(prefix_merge_kernel<__nv_bfloat16>, static_cast<__nv_bfloat16*>(out));
+  int e = launch_prefix_latent(*a, *plan, n_pages, st);
+  if (e == cudaErrorNotSupported) {
+    SimpleArgs p{};
+    p.q = a->q_abs; p.q2 = a->q_rot; p.pool = a->pool;
+    p.page_table = a->page_table; p.row_pos = a->row_pos; p.row_slot = a->row_slot;
+    p.ld_q = a->ld_q_abs; p.q_head = a->kv_pad; p.ld_q2 = a->ld_q_rot; p.q2_head = a->q_rot_stride;
+    p.d1 = a->kv_pad; p.d2 = a->row_len - a->kv_pad; p.vp = a->kv_pad; p.row_len = a->row_len;
+    p.lanes = 1; p.per_lane = a->heads; p.heads = a->heads;
+    p.max_pages = a->max_pages; p.page_tokens = a->page_tokens;
+    p.scale = a->scale;
+    e = run_simple(p, *plan, a->f32, st);
+  }
+  if (e != cudaSuccess) return e;
+  const ds41_proj none{};
+  ds41_group_attend_args keep{};
+  keep.taps = 1;
+  return a->f32 ? launch_join<float>(*plan, sink, none, a->rows, a->heads, a->kv_pad, out, ld_out, keep, st)
+                : launch_join<__nv_bfloat16>(*plan, sink, none, a->rows, a->heads, a->kv_pad, out, ld_out, keep, st);
 }

@@ -1,7 +1,8 @@
-// Grouped-query attention over the common keys of rows that share a prefix, on tcgen05.
+// Parts of grouped-query attention for rows that share prefixes, on tcgen05.
 //
-// The queries of one key/value head are packed: (row, head) pairs of an item's rows are the 128 rows of a tensor-core tile, so that a
-// tile of keys and values is read once for all of them and the products have the shape of a prompt's.  A CTA has two tiles:
+// The queries of one key/value head are packed: (row, head) pairs of a unit's rows are the 128 rows of a tensor-core tile, so that a
+// tile of keys and values is read once for all of them and the products have the shape of a prompt's.  A CTA walks units, its copies
+// running ahead into the next one, and has two tiles:
 //   more than 128 queries : two tiles of queries that walk the same keys;
 //   up to 128             : the same queries twice, over the even and the odd tiles of keys, joined through tensor memory at the end.
 // Either way one tile's softmax runs while the tensor core works on the other's products.
@@ -79,18 +80,11 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
 
-  const int units = *plan.n_items * p.kv_heads;
-  // keys [first, first + 128 tiles) that an item's rows walk: a chunk's border may lie inside (whole warps)
-  auto span = [&](const PrefixItem& it, int& first) {
-    first = it.key0;
-    if (p.chunk > 0) {
-      int low = it.key1;
-      for (int i = lane; i < it.rows; i += 32) low = min(low, chunk_start(p.row_pos[plan.order[it.first + i]], p.chunk));
-#pragma unroll
-      for (int o = 16; o; o >>= 1) low = min(low, __shfl_xor_sync(0xffffffffu, low, o));
-      first = max(first, low - low % p.page_tokens);
-    }
-    return first < it.key1 ? (it.key1 - first + kPgTile - 1) / kPgTile : 0;
+  const int units = *plan.n_units;
+  // the key tiles of a unit (whole warps)
+  auto span = [&](const PrefixUnit& it, int& first, int& end) {
+    prefix_span(plan, it, p.row_pos, p.row_slot, p.chunk, p.page_tokens, first, end);
+    return (end - first + kPgTile - 1) / kPgTile;
   };
 
   if (warp == 8) {
@@ -99,16 +93,17 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
     uint32_t k_free = 1, v_free = 1;
     bool ok = true;
     for (int unit = blockIdx.x; unit < units && ok; unit += gridDim.x) {
-      const PrefixItem it = prefix_item(plan, unit / p.kv_heads);
-      const int g = unit % p.kv_heads;
-      int first;
-      const int n = span(it, first);
+      const PrefixUnit it = prefix_unit(plan, unit);
+      if (it.rows == 0) continue;
+      const int g = it.head;
+      int first, end;
+      const int n = span(it, first, end);
       const int* table = p.page_table + 1ll * it.slot * p.max_pages;
       int row = 0, u = 0;                                // lane i: pool row of box i of the walk, 32 boxes at a time
       for (int j = 0; j < n; ++j, ++kt, u += boxes) {
         if ((u & 31) == 0) {                             // boxes divides 32
           const int key = first + (u + lane) * p.box, pg = key / p.page_tokens;
-          const int id = key < it.key1 && pg < p.max_pages ? table[pg] : -1;
+          const int id = key < end && pg < p.max_pages ? table[pg] : -1;
           row = id >= 0 ? id * p.page_tokens + (key - pg * p.page_tokens) : p.hidden_row;
         }
         // one tile of keys or values: `chunks` chunks of 64 columns from column x on
@@ -161,9 +156,10 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
     bool ok = true;
     int kt = 0, done[2] = {0, 0}, live = 0;              // key tiles; products of each tile; units with work so far
     for (int unit = blockIdx.x; unit < units && ok; unit += gridDim.x) {
-      const PrefixItem it = prefix_item(plan, unit / p.kv_heads);
-      int first;
-      const int n = span(it, first);
+      const PrefixUnit it = prefix_unit(plan, unit);
+      if (it.rows == 0) continue;
+      int first, end;
+      const int n = span(it, first, end);
       if (n == 0) continue;
       if (leader) {                                      // one thread: votes and the like between two products cost as much as the products
         ok = mbar_wait(q_full, live & 1, p.status, 470);
@@ -231,26 +227,27 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
       ok = __ballot_sync(0xffffffffu, leader && ok) != 0;
     }
   } else {
-    const int t = warp >> 2, quad = warp & 3, tid = threadIdx.x, mine = quad * 32 + lane;
+    const int t = warp >> 2, quad = warp & 3, mine = quad * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
     const uint32_t s_t = tmem + lanes + t * 128, o_t = tmem + lanes + 256 + t * 128;
-    int tiles = 0, outs[2] = {0, 0};                     // tiles of S seen by this half; finished results of both
+    int kt = 0, tiles = 0, outs[2] = {0, 0};             // key tiles so far; tiles of S seen by this half; finished results of both
     bool ok = true;
     // the loop runs to its end whatever happened: its barriers are for all eight warps
     for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
-      const PrefixItem it = prefix_item(plan, unit / p.kv_heads);
-      const int g = unit % p.kv_heads, count = it.rows * p.n;
+      const PrefixUnit it = prefix_unit(plan, unit);
+      if (it.rows == 0) continue;
+      const int g = it.head, count = it.rows * p.n;
       const bool both = count <= kPgTile;                // the same queries in both tiles
-      int first;
-      const int n = span(it, first);
+      int first, end;
+      const int n = span(it, first, end);
       const int mine_q = both ? mine : t * kPgTile + mine;
       int r = -1, lo = 0, hi = 0;
       if (mine_q < count) {
-        r = plan.order[it.first + mine_q / p.n];
+        r = prefix_row(plan, it, mine_q / p.n);
         const int pos = p.row_pos[r];
         if (p.row_slot[r] >= 0) {
           lo = chunk_start(pos, p.chunk);
-          hi = min(min(plan.own[r], pos + 1), it.key1);
+          hi = min(pos + 1, it.key1);
         }
       }
       s_row[t * kPgTile + mine] = r;                     // equal in both halves where the queries are
@@ -353,10 +350,22 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
         }
         sums[0] = add2(sums[0], sums[1]);
         l += sums[0].x + sums[0].y;
+        if (it.tail && key0 + kPgTile > end) {
+          // Places behind the last position belong to nobody, and a weight of zero does not take a NaN or an infinity away: their values
+          // become zeros, a thread to a place.
+          const int at = kt + j, stage = p.v_stages == 2 ? at & 1 : 0, phase = p.v_stages == 2 ? (at >> 1) & 1 : at & 1;
+          ok = __all_sync(0xffffffffu, mbar_wait(&v_full[stage], phase, p.status, 484 + t)) != 0;
+          if (!ok) break;
+          if (key0 + mine >= end)
+            for (int i = 0; i < 8 * p.vc; ++i)
+              *reinterpret_cast<uint4*>(s_v + stage * v_bytes + (i >> 3) * kPgChunk + mine * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+          fence_async_smem();
+        }
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&p_full[t]);
       }
+      kt += n;
       if (hi <= lo) {                                    // a query that sees nothing here: tiles without an edge did not look
         m = -INFINITY;
         l = 0.f;
@@ -373,7 +382,7 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
       tc_fence_after();
       named_barrier(1, 2 * kPgTile);                     // s_ml is there
       const bool write = ok && r >= 0;
-      const long long cell = write ? (1ll * plan.cell[r] + it.split) * p.heads + g * p.n + mine_q % p.n : 0;
+      const long long cell = write ? (1ll * plan.cell[r] + it.part) * p.heads + g * p.n + mine_q % p.n : 0;
       float f0 = 1.f, f1 = 0.f;                          // factors on the two tiles' results
       if (both) {
         const float2 a = s_ml[mine], b = s_ml[kPgTile + mine];
@@ -420,7 +429,7 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
 // Stages and shared memory of a launch; false: the sizes do not fit.
 static bool plan_prefix_group(const ds41_group_attend_args& a, const ds41_prefix_plan& plan, PrefixGroupParams& p, int& smem) {
   p.n = a.heads / a.kv_heads;
-  if (a.f32 || a.n_pages <= 0 || a.vdim_pad > 128 || (a.ld_q & 7) || plan.rows_per_item * p.n > 2 * kPgTile ||
+  if (a.f32 || a.n_pages <= 0 || a.vdim_pad > 128 || (a.ld_q & 7) || plan.rows_per_unit * p.n > 2 * kPgTile ||
       ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.pool)) & 15) ||
       1ll * a.n_pages * a.page_tokens >= (1ll << 31) - 1)
     return false;

@@ -1,6 +1,6 @@
-// Latent attention over the common keys of rows that share a prefix, on tcgen05.
+// Parts of latent attention for rows that share prefixes, on tcgen05.
 //
-// Every head reads the same key rows, so the (row, head) pairs of an item's rows are packed into the 128 rows of a tensor-core tile.
+// Every head reads the same key rows, so the (row, head) pairs of a unit's rows are packed into the 128 rows of a tensor-core tile.
 // A key row is [latent | rotated part], the latent being the value as well: with 512 latent values the result of 128 queries alone
 // would fill the 512 columns of a CTA's tensor memory.  So two CTAs of a cluster divide the columns of queries, keys and values between
 // them: each multiplies its half of the columns, S = S_0 + S_1, they exchange these partial scores through distributed shared memory,
@@ -115,9 +115,15 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
 
-  const int units = *plan.n_items, first_unit = PAIR ? blockIdx.x >> 1 : blockIdx.x, unit_step = PAIR ? gridDim.x >> 1 : gridDim.x;
+  const int units = *plan.n_units, first_unit = PAIR ? blockIdx.x >> 1 : blockIdx.x, unit_step = PAIR ? gridDim.x >> 1 : gridDim.x;
   const int v0 = p.v_col[rank], v1 = p.v_col[rank + 1], r0 = p.rot_step[rank], r1 = p.rot_step[rank + 1];
   const int v_chunks = (v1 - v0 + 63) / 64, r_chunk0 = r0 >> 2, r_chunks = r1 > r0 ? (r1 + 3) / 4 - r_chunk0 : 0;
+
+  auto span = [&](const PrefixUnit& it, int& end) {            // the key tiles of a unit (whole warps)
+    int first;
+    prefix_span(plan, it, p.row_pos, p.row_slot, 0, p.page_tokens, first, end);
+    return (end - first + kPlKeys - 1) / kPlKeys;
+  };
 
   if (warp == kPlTma) {
     // A copy costs the issuing thread 50 to 100 cycles: where a tile lies in one page and the chunks in one row of them, all of a CTA's
@@ -127,8 +133,10 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
     uint32_t free_phase = 1;
     bool ok = true;
     for (int unit = first_unit; unit < units && ok; unit += unit_step) {
-      const PrefixItem it = prefix_item(plan, unit);
-      const int n = (it.key1 - it.key0 + kPlKeys - 1) / kPlKeys;
+      const PrefixUnit it = prefix_unit(plan, unit);
+      if (it.rows == 0) continue;
+      int end;
+      const int n = span(it, end);
       const int* table = p.page_table + 1ll * it.slot * p.max_pages;
       int row = 0, u = 0;                                    // lane i: pool row of box i of the walk, 32 boxes at a time
       for (int j = 0; j < n; ++j, ++kt) {
@@ -140,7 +148,7 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
         for (int i = 0; i < boxes; ++i, ++u, dst += p.box * 128) {
           if ((u & 31) == 0) {
             const int key = it.key0 + (u + lane) * p.box, pg = key / p.page_tokens;
-            const int id = key < it.key1 && pg < p.max_pages ? table[pg] : -1;
+            const int id = key < end && pg < p.max_pages ? table[pg] : -1;
             row = id >= 0 ? id * p.page_tokens + (key - pg * p.page_tokens) : p.hidden_row;
           }
           const int at = __shfl_sync(0xffffffffu, row, u & 31);
@@ -164,25 +172,27 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
         for (int i = 0; i < (1 << 18) && !mbar_test_wait(&kv_full[b % p.stages], (b / p.stages) & 1); ++i) {
         }
   } else if (warp == kPlMma) {
-    // one thread: votes and the like between two products cost as much as the products
-    if (elect_one()) {
-      const uint32_t idesc_s = umma_idesc(kPlQueries, kPlKeys, 1u, 1u);
-      const uint32_t idesc_pv = umma_idesc_bmn(kPlQueries, v1 - v0, 1u, 1u);
-      const uint64_t k_desc = umma_desc_sw128(smem_u32(s_kv)), v_desc = umma_desc_sw128_mn(smem_u32(s_kv), kPlChunk, 1024);
-      bool ok = true;
-      int kt = 0, live = 0, s_stage = 0, p_stage = 0;          // tiles so far; the ring's places of the next scores and values
-      uint32_t s_phase = 0;
-      for (int unit = first_unit; unit < units && ok; unit += unit_step) {
-        const PrefixItem it = prefix_item(plan, unit);
-        const int n = (it.key1 - it.key0 + kPlKeys - 1) / kPlKeys;
+    const bool leader = elect_one();
+    const uint32_t idesc_s = umma_idesc(kPlQueries, kPlKeys, 1u, 1u);
+    const uint32_t idesc_pv = umma_idesc_bmn(kPlQueries, v1 - v0, 1u, 1u);
+    const uint64_t k_desc = umma_desc_sw128(smem_u32(s_kv)), v_desc = umma_desc_sw128_mn(smem_u32(s_kv), kPlChunk, 1024);
+    bool ok = true;
+    int kt = 0, live = 0, s_stage = 0, p_stage = 0;            // tiles so far; the ring's places of the next scores and values
+    uint32_t s_phase = 0;
+    for (int unit = first_unit; unit < units && ok; unit += unit_step) {
+      const PrefixUnit it = prefix_unit(plan, unit);
+      if (it.rows == 0) continue;
+      int end;
+      const int n = span(it, end);
+      if (n == 0) continue;
+      if (leader) {                                            // one thread: votes and the like between two products cost as much as the products
         ok = mbar_wait(q_full, live & 1, p.status, 510);
         ++live;
-        if (!ok) break;
         tc_fence_after();
         int sj = 0, pj = 0;                                    // next scores, next values
         uint32_t idle = 0;
         long long since = 0;
-        while (pj < n) {
+        while (ok && pj < n) {
           const int st = kt + sj, pt = kt + pj;
           if (pj < sj && mbar_test_wait(&p_full[pt % kPlSets], (pt / kPlSets) & 1)) {
             tc_fence_after();
@@ -217,7 +227,6 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
                 p.status[3] = pj;
               }
               ok = false;
-              break;
             }
             continue;
           } else {
@@ -228,8 +237,8 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
         }
         kt += n;
       }
+      ok = __ballot_sync(0xffffffffu, leader && ok) != 0;
     }
-    __syncwarp();
   } else {
     const int set = warp >> 2, quad = warp & 3, mine = quad * 32 + lane;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16);
@@ -241,13 +250,20 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
     bool ok = true;
     // the loop runs to its end whatever happened: the warps of a quadrant meet at barriers
     for (int unit = first_unit; unit < units; unit += unit_step) {
-      const PrefixItem it = prefix_item(plan, unit);
-      const int n = (it.key1 - it.key0 + kPlKeys - 1) / kPlKeys;
+      const PrefixUnit it = prefix_unit(plan, unit);
+      if (it.rows == 0) continue;
+      int end;
+      const int n = span(it, end);
       int r = -1, hi = 0, h = 0;
       if (mine < it.rows * p.heads) {
-        r = plan.order[it.first + mine / p.heads];
+        r = prefix_row(plan, it, mine / p.heads);
         h = mine % p.heads;
-        if (p.row_slot[r] >= 0) hi = min(min(plan.own[r], p.row_pos[r] + 1), it.key1);
+        if (p.row_slot[r] >= 0) hi = min(p.row_pos[r] + 1, it.key1);
+      }
+      if (n == 0) {                                            // nothing for any of its rows
+        if (r >= 0 && set == 0 && rank == 0)
+          *reinterpret_cast<float2*>(plan.part_ml + 2 * ((1ll * plan.cell[r] + it.part) * p.heads + h)) = make_float2(-INFINITY, 0.f);
+        continue;
       }
       // queries into tensor memory, the sets in turn: all of a thread's loads are under way together
       {
@@ -382,6 +398,16 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
         if (!ok) break;
         tc_fence_after();
         tmem_st_32x32(lanes + kPlP, w);
+        if (it.tail && key0 + kPlKeys > end) {
+          // Places behind the last position belong to nobody, and a weight of zero does not take a NaN or an infinity away: their values
+          // become zeros, two threads to a place.
+          const int key = mine & (kPlKeys - 1);
+          if (key0 + key >= end)
+            for (int i = 8 * (mine / kPlKeys); i < 8 * v_chunks; i += (i & 7) == 7 ? 9 : 1)
+              *reinterpret_cast<uint4*>(s_kv + tile % p.stages * stage_bytes + (i >> 3) * kPlChunk + key * 128 + (i & 7) * 16) =
+                  make_uint4(0, 0, 0, 0);
+          fence_async_smem();
+        }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -402,10 +428,10 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
       m = all;
       if (ok) {
         const bool write = r >= 0, seen = hi > it.key0;
-        const long long cell = write ? (1ll * plan.cell[r] + it.split) * p.heads + h : 0;
+        const long long cell = write ? (1ll * plan.cell[r] + it.part) * p.heads + h : 0;
         if (write && set == 0 && rank == 0)
           *reinterpret_cast<float2*>(plan.part_ml + 2 * cell) =
-              make_float2(seen ? m * 0.6931471805599453f : -INFINITY, seen ? l : 0.f);
+              make_float2(seen ? m : -INFINITY, seen ? l : 0.f);
         float* dst = plan.part_o + cell * p.kvp + v0;
         for (int c = 16 * set; c < v1 - v0; c += 16 * kPlSets) {
           uint32_t o[16];
@@ -442,7 +468,7 @@ static int launch_form(const CUtensorMap& pool, const CUtensorMap& chunks, const
 // cudaErrorNotSupported: these sizes are for the simple form
 int launch_prefix_latent(const ds41_latent_attend_args& a, const ds41_prefix_plan& plan, int n_pages, cudaStream_t st) {
   const int rp = a.row_len - a.kv_pad, v_chunks = (a.kv_pad + 63) / 64;
-  if (a.f32 || (a.kv_pad & 15) || (rp & 15) || a.kv_pad > 512 || plan.rows_per_item * a.heads > kPlQueries || (a.ld_q_abs & 7) ||
+  if (a.f32 || (a.kv_pad & 15) || (rp & 15) || a.kv_pad > 512 || plan.rows_per_unit * a.heads > kPlQueries || (a.ld_q_abs & 7) ||
       (a.ld_q_rot & 7) || (a.q_rot_stride & 7) || 1ll * n_pages * a.page_tokens >= (1ll << 31) - 1 ||
       ((reinterpret_cast<uintptr_t>(a.q_abs) | reinterpret_cast<uintptr_t>(a.q_rot) | reinterpret_cast<uintptr_t>(a.pool)) & 15))
     return cudaErrorNotSupported;

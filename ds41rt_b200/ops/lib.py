@@ -139,8 +139,7 @@ def dir_functions():
         "ds41_latent_prefill", "ds41_mlstm_chunk",
         "ds41_mlstm_step", "ds41_gemm_f32", "ds41_side_act", "ds41_softcap_rows", "ds41_attn_post", "ds41_group_attend",
         "ds41_group_prefill", "ds41_route_softmax", "ds41_gated_act",
-        "ds41_prefix_group_shared", "ds41_prefix_group_own", "ds41_prefix_latent_shared", "ds41_prefix_latent_own",
-        "ds41_prefix_latent_merge",
+        "ds41_prefix_group", "ds41_prefix_latent",
     ]
 
 

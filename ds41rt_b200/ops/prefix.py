@@ -14,25 +14,23 @@ new one.
 from __future__ import annotations
 
 import ctypes as C
-from typing import List, Optional, Sequence, Tuple
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
 
 from . import lib
 from . import stack as S
+from .stack import ceil_to
 
 BF16, F32, I32 = torch.bfloat16, torch.float32, torch.int32
 SMS = 148                # of a B200: plans do not depend on the device found
-ITEM = 8                 # numbers of an item (ds41_prefix_plan)
-MAX_PARTS = 160          # parts of a row's prefix that a join takes
-MAX_OWN = 32             # splits of a row's own keys (latent attention)
+UNIT = 8                 # numbers of a unit (ds41_prefix_plan)
 
 
 class PlanArgs(C.Structure):
-    _fields_ = [("items", C.c_void_p), ("n_items", C.c_void_p), ("order", C.c_void_p), ("own", C.c_void_p), ("cell", C.c_void_p),
-                ("parts", C.c_void_p), ("part_o", C.c_void_p), ("part_ml", C.c_void_p), ("max_items", C.c_int),
-                ("rows_per_item", C.c_int), ("grid", C.c_int)]
+    _fields_ = [("units", C.c_void_p), ("n_units", C.c_void_p), ("order", C.c_void_p), ("cell", C.c_void_p), ("parts", C.c_void_p),
+                ("part_o", C.c_void_p), ("part_ml", C.c_void_p), ("max_units", C.c_int), ("rows_per_unit", C.c_int), ("grid", C.c_int)]
 
 
 def common_runs(tables: np.ndarray) -> List[Tuple[List[int], int]]:
@@ -63,35 +61,42 @@ def common_runs(tables: np.ndarray) -> List[Tuple[List[int], int]]:
     return out
 
 
-def key_span(work: Sequence[Tuple[int, int]], budget: int, unit: int) -> int:
-    """Keys of an item, where `work` lists (pieces, keys) of every prefix and `budget` items run at once: the shortest range that
-    keeps one wave of items, or of two waves where shorter ones win by more than an item's fixed cost."""
-    longest = max(keys for _, keys in work)
-    best = None
-    for waves in (1, 2):
-        lo, hi = 1, -(-longest // unit)
-        if sum(n for n, _ in work) > budget * waves:
-            continue
-        while lo < hi:
-            mid = (lo + hi) // 2
-            if sum(n * -(-keys // (mid * unit)) for n, keys in work) <= budget * waves:
-                hi = mid
-            else:
-                lo = mid + 1
-        cost = waves * (lo * unit + ITEM_COST)
-        if best is None or cost < best[0]:
-            best = (cost, lo * unit)
-    return max(best[1] if best else longest, -(-longest // (MAX_PARTS * unit)) * unit)
+class Cost:
+    """What a plan goes by, in us: of a unit, of a key in it, of a byte of partial results on their way to the join."""
+
+    def __init__(self, unit: float, key: float):
+        self.unit, self.key, self.byte = unit, key, 1 / 4e6
 
 
-ITEM_COST = 512          # fixed cost of an item, in keys
+COSTS = {"grouped": Cost(3.0, 0.006), "latent": Cost(4.0, 0.02)}
+
+
+def key_span(work: Sequence[Tuple[int, int, int]], width: int, part_bytes: int, most: int, unit: int, cost: Cost) -> int:
+    """Keys of a unit, where `work` lists (pieces, rows, keys) of every range of pages and `width` units run at once: the length with
+    the least estimate of the time until the last unit is done plus that of moving the partial results, at most `most` units."""
+    pieces, rows, keys = (np.array(x, dtype=np.float64) for x in zip(*work))
+    best, longest = None, int(keys.max())
+    for k in (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256, 512, 1024, 4096, 1 << 20):
+        span = k * unit
+        count = np.maximum(1, np.ceil(keys / span))
+        if (pieces * count).sum() <= most:
+            total = (pieces * (count * cost.unit + keys * cost.key)).sum() / width
+            last = cost.unit + min(span, longest) * cost.key
+            # the units that the busiest block gets are whole ones
+            estimate = max(total, last, np.ceil((pieces * count).sum() / width) * cost.unit + last - cost.unit) \
+                + (rows * count).sum() * part_bytes * cost.byte
+            if best is None or estimate < best[0]:
+                best = (estimate, span)
+        if span >= longest:
+            break
+    return best[1] if best else ceil_to(longest, unit)
 
 
 class PrefixPlan:
     """Rows that share leading pages, how their attention is divided, and the workspace of the calls.
 
     `kind`: "grouped" or "latent"; `rows`: most rows of a pass; `heads`, `kv_heads`, `vdim`: of the attention (latent: one key / value
-    head, `vdim` the padded latent width)."""
+    head, `vdim` the padded latent width).  Prefixes shorter than `min_tokens` are left to the rows."""
 
     def __init__(self, kind: str, *, rows: int, heads: int, vdim: int, page_tokens: int, device, kv_heads: int = 1, dtype=BF16,
                  min_tokens: int = 64):
@@ -106,39 +111,33 @@ class PrefixPlan:
         self.kind, self.rows, self.heads, self.kv_heads, self.vdim = kind, rows, heads, kv_heads, vdim
         self.page_tokens, self.dtype, self.device = page_tokens, dtype, torch.device(device)
         self.min_tokens = min_tokens
-        per_lane = heads // kv_heads
-        self.rows_per_item = max(1, (256 if kind == "grouped" else 128) // per_lane)
-        pair = kind == "latent" and vdim > 256               # two CTAs to an item
-        self.budget = max(1, (SMS // 2 if pair else SMS) // kv_heads)
-        self.max_items = 2 * self.budget + rows
-        self.max_cells = 2 * self.budget * min(self.rows_per_item, rows) + rows
-        self.own_cells = rows * self._own_splits(rows, 1 << 30) if kind == "latent" else 0
+        self.rows_per_unit = max(1, (256 if kind == "grouped" else 128) // (heads // kv_heads))
+        self.grid = SMS // 2 if kind == "latent" and vdim > 256 else SMS               # two CTAs to a unit
+        self.extra = 3 * -(-self.grid // kv_heads)               # items beyond one for every piece of a prefix and every request
+        self.max_items = self.extra + 2 * rows
+        self.max_units = ceil_to(self.max_items * kv_heads, self.grid)
+        self.max_cells = self.extra * min(self.rows_per_unit, rows) + 2 * rows
         z = lambda n, d: torch.zeros(max(n, 4), dtype=d, device=self.device)
-        # [count, 3 unused | items | order | own | cell | parts]
-        self._at = np.cumsum([4, ITEM * self.max_items, rows, rows, rows]).tolist()
+        # [count, 3 unused | units | order | cell | parts]
+        self._at = np.cumsum([4, UNIT * self.max_units, rows, rows]).tolist()
         self.data = z(self._at[-1] + rows, I32)
         self.part_o, self.part_ml = z(self.max_cells * heads * vdim, F32), z(self.max_cells * heads * 2, F32)
-        self.own_o, self.own_ml = z(self.own_cells * heads * vdim, F32), z(self.own_cells * heads * 2, F32)
         self.status = lib.new_status(self.device)
-        self.n_items = 0
+        self.n_units = 0
         self.shared: List[Tuple[List[int], int]] = []      # rows and tokens of every prefix
-        self.least_own = 0
         a, base = PlanArgs(), self.data.data_ptr()
-        a.n_items, (a.items, a.order, a.own, a.cell, a.parts) = base, (base + 4 * x for x in self._at)
+        a.n_units, (a.units, a.order, a.cell, a.parts) = base, (base + 4 * x for x in self._at)
         a.part_o, a.part_ml = self.part_o.data_ptr(), self.part_ml.data_ptr()
-        a.max_items, a.rows_per_item = self.max_items, self.rows_per_item
-        a.grid = min(self.max_items * kv_heads, SMS)
+        a.max_units, a.rows_per_unit, a.grid = self.max_units, self.rows_per_unit, self.grid
         self.args = a
 
-    def _own_splits(self, rows: int, tokens: int) -> int:
-        return max(1, min(2 * SMS // (rows * -(-self.heads // 32)), MAX_OWN, -(-tokens // 64)))
-
     def nbytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in (self.data, self.part_o, self.part_ml, self.own_o, self.own_ml))
+        return sum(t.numel() * t.element_size() for t in (self.data, self.part_o, self.part_ml))
 
-    def set(self, slots: Sequence[int], tables) -> None:
+    def set(self, slots: Sequence[int], tables, lengths: Optional[Sequence[int]] = None) -> None:
         """`slots`: the slot of every row of the passes to come (-1: none); `tables`: the page table on the host, [slots, pages],
-        negative where no page is leased."""
+        negative where no page is leased.  `lengths`: how many tokens each row's request has now (default: what its pages hold); only
+        the division of the work goes by it."""
         t = tables.numpy() if isinstance(tables, torch.Tensor) else np.asarray(tables)
         s = np.asarray(slots, dtype=np.int64)
         if t.ndim != 2 or t.dtype != np.int32:
@@ -147,7 +146,9 @@ class PrefixPlan:
             raise ValueError(f"a plan for {self.rows} rows does not take {s.shape}")
         if len(s) and int(s.max()) >= len(t):
             raise ValueError(f"slot {int(s.max())} of {len(t)}")
-        of = {}                                                # rows of every slot
+        if lengths is not None and len(lengths) != len(s):
+            raise ValueError("lengths has an entry per row")
+        of: Dict[int, List[int]] = {}                          # rows of every slot
         for r, slot in enumerate(s.tolist()):
             if slot >= 0:
                 of.setdefault(slot, []).append(r)
@@ -155,34 +156,69 @@ class PrefixPlan:
         runs = common_runs(t[keep]) if len(keep) > 1 else []
         self.shared = [(sorted(r for i in members for r in of[keep[i]]), pages * self.page_tokens) for members, pages in runs
                        if pages * self.page_tokens >= self.min_tokens]
-        self._lay_out(s)
+        begin = np.zeros(len(s), dtype=np.int64)               # where a row's own keys begin
+        for rows, tokens in self.shared:
+            begin[rows] = tokens
+        leased = {slot: self.page_tokens * int((np.append(t[slot], -1) < 0).argmax()) for slot in keep}
+        tails = []                                             # (first row, rows, first key, keys there are now)
+        for slot, rows in of.items():
+            at = 0
+            while at < len(rows):                              # neighbours, as many as a unit takes
+                n = 1
+                while at + n < len(rows) and n < self.rows_per_unit and rows[at + n] == rows[at] + n:
+                    n += 1
+                have = leased[slot] if lengths is None else max(int(lengths[r]) for r in rows[at:at + n])
+                tails.append((rows[at], n, int(begin[rows[at]]), max(1, have - int(begin[rows[at]]))))
+                at += n
+        self._lay_out(s, tails, t.shape[1] * self.page_tokens)
 
-    def _lay_out(self, slots: np.ndarray) -> None:
+    def _lay_out(self, slots: np.ndarray, tails, limit: int) -> None:
         host = np.zeros(self.data.numel(), dtype=np.int32)
-        items, order, own, cell, parts = (host[a:b] for a, b in zip(self._at, self._at[1:] + [len(host)]))
-        pieces = [-(-len(rows) // self.rows_per_item) for rows, _ in self.shared]
-        n = at = cells = 0
-        if self.shared:
-            span = key_span([(p, tokens) for p, (_, tokens) in zip(pieces, self.shared)], self.budget, max(128, self.page_tokens))
-            todo = []
+        units, order, cell, parts = (host[a:b] for a, b in zip(self._at, self._at[1:] + [len(host)]))
+        pieces = [-(-len(rows) // self.rows_per_unit) for rows, _ in self.shared]
+        work = [(p, len(rows), tokens) for p, (rows, tokens) in zip(pieces, self.shared)] + [(1, n, keys) for _, n, _, keys in tails]
+        n = 0
+        if work:
+            unit, part_bytes = max(128, self.page_tokens), 8 * self.heads * self.vdim
+            span = key_span(work, max(1, self.grid // self.kv_heads), part_bytes, sum(w[0] for w in work) + self.extra, unit,
+                            COSTS[self.kind])
+            items, at = [], 0
             for p, (rows, tokens) in zip(pieces, self.shared):
                 count = -(-tokens // span)
                 order[at:at + len(rows)] = rows
-                own[rows], parts[rows] = tokens, count
-                cell[rows] = cells + count * np.arange(len(rows))
-                cells += count * len(rows)
+                parts[rows] = count
                 for i in range(p):
                     lo, hi = (len(rows) * j // p for j in (i, i + 1))
-                    todo += [(int(slots[rows[0]]), at + lo, hi - lo, k * span, min(tokens, (k + 1) * span), k, 0, 0) for k in range(count)]
+                    items += [(int(slots[rows[0]]), at + lo, hi - lo, k * span, min(tokens, (k + 1) * span), k, 0) for k in range(count)]
                 at += len(rows)
-            todo.sort(key=lambda x: x[3] - x[4])               # the longest ranges first
-            n = len(todo)
-            assert n <= self.max_items and cells <= self.max_cells, (n, cells)
-            items[:ITEM * n] = np.asarray(todo, dtype=np.int32).ravel()
-        host[0] = self.n_items = n
-        live = [r for r in range(len(slots)) if slots[r] >= 0]
-        self.least_own = int(own[live].min()) if live else 0
+            for first, rows, key0, keys in tails:
+                count = max(1, keys // span)                   # the last one goes on to wherever the request gets
+                part = int(parts[first])
+                items += [(int(slots[first]), first, rows, key0 + k * span, key0 + (k + 1) * span if k + 1 < count else limit, part + k, 1)
+                          for k in range(count)]
+                parts[first:first + rows] += count
+            cell[:] = np.cumsum(parts) - parts
+            assert len(items) <= self.max_items and int(parts.sum()) <= self.max_cells, (len(items), int(parts.sum()))
+            n = self._deal(np.array(items, dtype=np.int32), units, {x[0]: x[2] + x[3] for x in tails})
+        host[0] = self.n_units = n
         self.data.copy_(torch.from_numpy(host))
+
+    def _deal(self, items: np.ndarray, units: np.ndarray, ends: Dict[int, int]) -> int:
+        """Items and key/value heads as units, the longest first, dealt to the blocks there and back: block b takes the units b, b + grid,
+        b + 2 grid ...  Returns how many places were dealt (a place may stay empty)."""
+        keys = items[:, 4] - items[:, 3]
+        for i in np.flatnonzero(items[:, 6]):
+            keys[i] = min(keys[i], max(1, ends[int(items[i, 1])] - items[i, 3]))
+        ranked = items[np.argsort(-keys, kind="stable")]
+        every = np.repeat(ranked, self.kv_heads, 0)
+        heads = np.tile(np.arange(self.kv_heads, dtype=np.int32), len(items))
+        i = np.arange(len(every))
+        turn, place = i // self.grid, i % self.grid
+        place = np.where(turn % 2 == 1, self.grid - 1 - place, place)
+        n = ceil_to(len(every), self.grid) if len(every) > self.grid else len(every)
+        table = units.reshape(-1, UNIT)
+        table[turn * self.grid + place] = np.concatenate([every, heads[:, None]], 1)
+        return n
 
     def check_status(self, what: str = "attention over a shared prefix"):
         lib.raise_on_status(self.status, what)
@@ -190,31 +226,14 @@ class PrefixPlan:
 
 # ---------------------------------------------------------------------------------------------------- launches
 def launch_group(a: S.GroupAttendArgs, plan: PrefixPlan) -> None:
-    """Both launches of grouped attention; `a` as for ds41_group_attend."""
-    k, st = lib.kernels("stack"), lib.stream()
-    if plan.n_items or torch.cuda.is_current_stream_capturing():
-        lib.check(k.ds41_prefix_group_shared(C.byref(a), C.byref(plan.args), st), "ds41_prefix_group_shared")
-    lib.check(k.ds41_prefix_group_own(C.byref(a), C.byref(plan.args), st), "ds41_prefix_group_own")
+    """Grouped attention; `a` as for ds41_group_attend."""
+    lib.check(lib.kernels("stack").ds41_prefix_group(C.byref(a), C.byref(plan.args), lib.stream()), "ds41_prefix_group")
 
 
 def launch_latent(a: S.LatentAttendArgs, plan: PrefixPlan, n_pages: int, sink, out: torch.Tensor, ld_out: int) -> None:
-    """The launches of latent attention; `a` as for ds41_latent_attend, whose partial results lie in the plan."""
-    k, st = lib.kernels("stack"), lib.stream()
-    tokens = a.max_pages * a.page_tokens - (plan.least_own if not torch.cuda.is_current_stream_capturing() else 0)
-    a.n_splits = plan._own_splits(a.rows, max(tokens, 1))
-    a.part_o, a.part_ml = plan.own_o.data_ptr(), plan.own_ml.data_ptr()
-    if plan.n_items or torch.cuda.is_current_stream_capturing():
-        lib.check(k.ds41_prefix_latent_shared(C.byref(a), C.byref(plan.args), n_pages, st), "ds41_prefix_latent_shared")
-    lib.check(k.ds41_prefix_latent_own(C.byref(a), C.byref(plan.args), st), "ds41_prefix_latent_own")
-    lib.check(k.ds41_prefix_latent_merge(lib.ptr(plan.own_o), lib.ptr(plan.own_ml), lib.ptr(sink), C.byref(plan.args), a.n_splits, a.rows,
-                                         a.heads, a.kv_pad, lib.ptr(out), ld_out, a.f32, st), "ds41_prefix_latent_merge")
-
-
-def own_cluster(rows: int, heads: int, kv_heads: int, tokens: int) -> int:
-    """CTAs that share a row's own keys in grouped attention."""
-    blocks = rows * kv_heads * -(-(heads // kv_heads) // 16)
-    n = max(1, min(SMS // blocks, 16, -(-tokens // 128)))
-    return n if n <= 8 else (16 if n == 16 and blocks <= 4 else 8)
+    """Latent attention and the join of its parts; `a` as for ds41_latent_attend."""
+    lib.check(lib.kernels("stack").ds41_prefix_latent(C.byref(a), C.byref(plan.args), n_pages, lib.ptr(sink), lib.ptr(out), ld_out,
+                                                      lib.stream()), "ds41_prefix_latent")
 
 
 # ---------------------------------------------------------------------------------------------------- front end
@@ -287,8 +306,6 @@ def group_attend(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, 
     a.rows, a.heads, a.kv_heads, a.dim_pad, a.vdim_pad = R, H, plan.kv_heads, D, plan.vdim
     a.max_pages, a.page_tokens, a.f32, a.n_pages = page_table.shape[1], plan.page_tokens, int(plan.dtype == F32), \
         pool.shape[0] // plan.page_tokens
-    span = a.max_pages * plan.page_tokens - (0 if torch.cuda.is_current_stream_capturing() else plan.least_own)
-    a.n_splits = own_cluster(R, H, plan.kv_heads, max(1, min(span, chunk or span)))
     launch_group(a, plan)
     return out
 

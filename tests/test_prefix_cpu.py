@@ -70,11 +70,11 @@ def test_the_first_group_saves_most_and_groups_are_true(seed):
     assert max([(len(m) - 1) * p for m, p in groups], default=0) == best_saving(t)
 
 
-@pytest.mark.parametrize("seed", range(20))
-def test_items_cover_every_prefix_once(seed):
+@pytest.mark.parametrize("seed", range(30))
+def test_units_cover_every_position_of_every_row_once(seed):
     rng = random.Random(seed)
     P = rng.choice([32, 64, 128])
-    kind, heads, kv = rng.choice([("grouped", 16, 4), ("grouped", 6, 2), ("latent", 16, 1), ("latent", 5, 1)])
+    kind, heads, kv, vdim = rng.choice([("grouped", 16, 4, 64), ("grouped", 6, 2, 64), ("latent", 16, 1, 512), ("latent", 5, 1, 64)])
     rows = rng.randint(2, 90)
     width = 80
     t = np.full((rows + 4, width), -1, dtype=np.int32)
@@ -86,33 +86,43 @@ def test_items_cover_every_prefix_once(seed):
         row = lead + [next(pages) for _ in range(rng.randint(1, width - len(lead)))]
         t[s, :len(row)] = row
     row_slots = [s if rng.random() < 0.9 else -1 for s in slots]
-    plan = PrefixPlan(kind, rows=rows, heads=heads, kv_heads=kv, vdim=64, page_tokens=P, device="cpu")
-    plan.set(row_slots, torch.from_numpy(t))
+    if seed % 3 == 0:                                          # several rows of a request
+        row_slots = [s for s in row_slots[:rows // 3] for _ in range(3)]
+    lengths = [rng.randint(1, width * P) for _ in row_slots] if seed % 2 else None
+    plan = PrefixPlan(kind, rows=rows, heads=heads, kv_heads=kv, vdim=vdim, page_tokens=P, device="cpu")
+    plan.set(row_slots, torch.from_numpy(t), lengths)
     d = plan.data.numpy()
-    items, order, own, cell, count = (d[a:b] for a, b in zip(plan._at, plan._at[1:] + [len(d)]))
-    assert d[0] == plan.n_items <= plan.max_items
-    covered = {}
-    for slot, first, n, k0, k1, part, _, _ in items[:8 * plan.n_items].reshape(-1, 8):
-        assert 0 < n <= plan.rows_per_item and 0 <= k0 < k1 and k0 % P == 0 and k1 % P == 0
-        for r in order[first:first + n]:
-            assert (t[row_slots[r], :k1 // P] == t[slot, :k1 // P]).all() and row_slots[r] >= 0
-            assert part < count[r] and cell[r] + count[r] <= plan.max_cells
-            covered.setdefault(int(r), []).append((int(k0), int(k1), int(part)))
-    for r in range(rows):
-        got = sorted(covered.get(r, []))
-        assert [x[2] for x in got] == list(range(count[r]))
-        assert [x[0] for x in got] + [own[r]] == [0] + [x[1] for x in got]          # adjacent, from 0 to the row's own keys
-    used = [c for r in covered for c in range(cell[r], cell[r] + count[r])]
-    assert len(used) == len(set(used))                                                # no cell has two writers
+    units, order, cell, count = (d[a:b] for a, b in zip(plan._at, plan._at[1:] + [len(d)]))
+    assert d[0] == plan.n_units <= plan.max_units and not units[8 * plan.n_units:].any()
+    covered, used = {}, set()
+    for slot, first, n, k0, k1, part, tail, head in units[:8 * plan.n_units].reshape(-1, 8).tolist():
+        if n == 0:                                             # a place that was not dealt
+            continue
+        assert 0 < n <= plan.rows_per_unit and 0 <= k0 < k1 and k0 % P == 0 and k1 % P == 0 and 0 <= head < kv
+        for r in range(first, first + n) if tail else order[first:first + n].tolist():
+            s = row_slots[r]
+            assert s >= 0 and (t[s, :k1 // P] == t[slot, :k1 // P]).all() and (not tail or s == slot)
+            assert part < count[r]
+            cells = (int(cell[r]) + part, head)
+            assert cells not in used and cells[0] < plan.max_cells       # no cell has two writers
+            used.add(cells)
+            covered.setdefault((r, head), []).append((k0, k1, part))
+    for r, s in enumerate(row_slots):
+        for head in range(kv):
+            got = sorted(covered.get((r, head), []))
+            assert [x[2] for x in got] == list(range(count[r]))
+            assert [x[0] for x in got] + [width * P] == [0] + [x[1] for x in got] if s >= 0 else not got
 
 
 def test_a_new_plan_replaces_the_old_one_whole():
     t = table([1, 2, 3, 4], [1, 2, 3, 5], [9, 8])
     plan = PrefixPlan("grouped", rows=3, heads=4, kv_heads=2, vdim=16, page_tokens=64, device="cpu")
     plan.set([0, 1, 2], t)
-    assert plan.n_items > 0 and plan.shared == [([0, 1], 192)]
+    assert plan.n_units > 0 and plan.shared == [([0, 1], 192)]
     plan.set([0, 2], t)
-    assert plan.n_items == 0 and plan.shared == [] and int(plan.data.abs().sum()) == 0
+    assert plan.shared == []
+    plan.set([-1, -1], t)
+    assert plan.n_units == 0 and int(plan.data.abs().sum()) == 0
 
 
 def test_rows_of_one_slot_share_with_other_slots_only():
@@ -128,14 +138,23 @@ def test_short_prefixes_are_left_to_the_rows():
     t = table([1, 2], [1, 3])
     plan = PrefixPlan("grouped", rows=2, heads=4, kv_heads=2, vdim=16, page_tokens=32, device="cpu", min_tokens=64)
     plan.set([0, 1], t)
-    assert plan.shared == [] and plan.n_items == 0
+    assert plan.shared == []
 
 
-def test_key_ranges_fill_one_wave_and_stay_within_the_parts_of_a_row():
-    assert key_span([(1, 4096)], 18, 128) == 256              # 16 ranges of 18
-    for pieces, keys in ((1, 100), (3, 100000), (40, 5000), (200, 300), (1, 1 << 24)):
-        span = key_span([(pieces, keys)], 37, 128)
-        assert span >= 1 and -(-keys // span) <= prefix.MAX_PARTS
+@pytest.mark.parametrize("kind", ["grouped", "latent"])
+def test_key_ranges_stay_within_what_the_plan_holds(kind):
+    for pieces, rows, keys in ((1, 4, 100), (3, 100, 100000), (40, 2000, 5000), (200, 300, 300), (1, 2, 1 << 24)):
+        for most in (pieces, pieces + 40):
+            span = key_span([(pieces, rows, keys)], 37, 4096, most, 128, prefix.COSTS[kind])
+            assert span >= 128 and span % 128 == 0 and pieces * -(-keys // span) <= most
+
+
+def test_short_requests_are_not_divided_and_long_ones_are():
+    t = table(*[[10 * i + k for k in range(1, 3)] for i in range(4)], list(range(1000, 1700)), width=800)
+    plan = PrefixPlan("grouped", rows=5, heads=8, kv_heads=2, vdim=128, page_tokens=64, device="cpu")
+    plan.set(range(5), t)
+    at = plan._at[3]
+    assert plan.data[at:at + 5].tolist()[:4] == [1, 1, 1, 1] and plan.data[at + 4] > 8
 
 
 @pytest.mark.parametrize("kw", [dict(kind="other"), dict(heads=0), dict(heads=6, kv_heads=4), dict(vdim=24), dict(rows=0),
@@ -155,6 +174,8 @@ def test_plans_refuse_rows_and_tables_that_do_not_fit(slots, tables):
     plan = PrefixPlan("grouped", rows=4, heads=8, kv_heads=2, vdim=32, page_tokens=64, device="cpu")
     with pytest.raises(ValueError):
         plan.set(slots, tables)
+    with pytest.raises(ValueError):
+        plan.set([0], table([1]), [1, 2])
 
 
 def call(kind="grouped", **change):
