@@ -1,14 +1,16 @@
 // Parts of grouped-query attention for rows that share prefixes, on tcgen05.
 //
 // The queries of one key/value head are packed: (row, head) pairs of a unit's rows are the 128 rows of a tensor-core tile, so that a
-// tile of keys and values is read once for all of them and the products have the shape of a prompt's.  A CTA walks units, its copies
-// running ahead into the next one, and has two tiles:
-//   more than 128 queries : two tiles of queries that walk the same keys;
-//   up to 128             : the same queries twice, over the even and the odd tiles of keys, joined through tensor memory at the end.
-// Either way one tile's softmax runs while the tensor core works on the other's products.
-//   warps 0-3, 4-7 : queries into shared memory, softmax of tile 0 / 1 (one thread per query), partial results
-//   warp 8         : TMA producer: key and value tiles of 128 positions, page by page, into rings of stages
-//   warp 9         : tcgen05.mma issue: S = Q K^T into TMEM, O += P V with P in TMEM where it replaces its S
+// tile of keys and values is read once for all of them and the products have the shape of a prompt's.  A CTA has two tiles: units
+// come in twos, and where both of them walk the same keys each copy serves two tiles.  One tile's softmax runs while the tensor core
+// works on the other's products, and nothing but the order of the copies ties the two together.
+//   warps 0-3, 4-7 : softmax of tile 0 / 1 (one thread per query), partial results
+//   warp 8         : TMA producer: what the next units are, for everybody (a ring of four); key and value tiles of 128 positions, page
+//                    by page
+//   warp 9         : tcgen05.mma issue, in whichever order their inputs come: S = Q K^T, O += P V with P in TMEM where it replaces its S
+//   warps 10, 11   : queries of tile 0 / 1, and what each of them sees
+// A CTA walks its units, and every role but the softmax runs ahead into the next ones: a request's own keys are a few tiles, which the
+// chain of loads that a unit begins with (its description, its rows' positions, their pages, their queries) would take as long as.
 // The running maximum is raised when it grew by more than 2^8 only; what leaves is (m, l, unnormalised O) in 32 bits.  P is rounded
 // to bf16 as the operand of the second product; l sums the unrounded weights.
 #include <cuda.h>
@@ -19,9 +21,10 @@
 
 namespace ds41 {
 
-constexpr int kPgThreads = 320;
+constexpr int kPgThreads = 384;
 constexpr int kPgTile = 128;                   // queries per tile, keys per tile
 constexpr int kPgChunk = kPgTile * 128;        // bytes of 128 rows x 64 bf16 columns
+constexpr int kPgInfos = 4;
 
 struct PrefixGroupParams {
   const __nv_bfloat16* q;
@@ -33,6 +36,34 @@ struct PrefixGroupParams {
   int* status;
 };
 
+// What a CTA's two tiles do next, as the producer found it: unit t walks `tiles[t]` key tiles from `first[t]` on, and nobody sees
+// `end[t]` or what follows.  both: they walk the same ones.
+struct __align__(16) GroupWork {
+  PrefixUnit unit[2];
+  int first[2], end[2], tiles[2], base, both;              // base: number of the first key tile in the order of the copies
+};
+static_assert(sizeof(GroupWork) == 96, "whole 16-byte pieces");
+
+// Number of key tile j of tile t in the order of the copies: one after the other, or in turn as long as both have some.
+__device__ __forceinline__ int copy_index(const GroupWork& w, int t, int j) {
+  if (w.both) return w.base + j;
+  const int least = min(w.tiles[0], w.tiles[1]);
+  return w.base + (j < least ? 2 * j + t : least + j);
+}
+
+struct GroupShared {                           // behind the tiles
+  uint64_t info_full[kPgInfos], info_empty[kPgInfos];
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+  // per tile:
+  uint64_t q_full[2], q_empty[2];
+  uint64_t s_full[2];                          // S complete (and every earlier MMA of the issuing thread)
+  uint64_t p_full[2];                          // P written, O rescaled
+  uint64_t o_full[2];                          // the unit's last product
+  uint32_t tmem, pad[3];
+  GroupWork info[kPgInfos];
+  int4 query[2][kPgTile];                      // of a packed query: pass row (-1: none), visible keys [y, z)
+};
+
 __global__ void __launch_bounds__(kPgThreads, 1)
 prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupParams p, const ds41_prefix_plan plan) {
   extern __shared__ uint8_t pg_raw[];
@@ -41,382 +72,440 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
   uint8_t* s_q = smem;                                   // two tiles
   uint8_t* s_k = s_q + 2 * q_bytes;
   uint8_t* s_v = s_k + p.k_stages * k_bytes;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(s_v + p.v_stages * v_bytes);
-  uint64_t* q_full = bars;
-  uint64_t* k_full = bars + 1;        // [2]
-  uint64_t* k_empty = bars + 3;
-  uint64_t* v_full = bars + 5;
-  uint64_t* v_empty = bars + 7;
-  uint64_t* s_full = bars + 9;        // [2] per tile: S complete (and every earlier MMA of the issuing thread)
-  uint64_t* p_full = bars + 11;       // [2] per tile: P written, O rescaled
-  uint64_t* o_full = bars + 13;       // [2] per tile: the unit's last product
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 15);
-  int* s_row = reinterpret_cast<int*>(bars + 16);        // [256] pass row of a packed query, -1: none
-  float2* s_ml = reinterpret_cast<float2*>(s_row + 2 * kPgTile);      // [2][128]
+  GroupShared& sh = *reinterpret_cast<GroupShared*>(s_v + p.v_stages * v_bytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 2 * kPgTile);
+    for (int i = 0; i < kPgInfos; ++i) {
+      mbar_init(&sh.info_full[i], 1);
+      mbar_init(&sh.info_empty[i], 12);                  // eight softmax warps, two of queries, the products of either tile
+    }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&k_full[i], 1);
-      mbar_init(&k_empty[i], 1);
-      mbar_init(&v_full[i], 1);
-      mbar_init(&v_empty[i], 1);
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], kPgTile);
-      mbar_init(&o_full[i], 1);
+      mbar_init(&sh.q_full[i], 1);
+      mbar_init(&sh.q_empty[i], 5);                      // four softmax warps, the products
+      mbar_init(&sh.k_full[i], 1);
+      mbar_init(&sh.k_empty[i], 1);
+      mbar_init(&sh.v_full[i], 1);
+      mbar_init(&sh.v_empty[i], 1);
+      mbar_init(&sh.s_full[i], 1);
+      mbar_init(&sh.p_full[i], 4);
+      mbar_init(&sh.o_full[i], 1);
     }
     mbar_init_fence();
     tma_prefetch_desc(&pool);
   }
   if (warp == 9) {
-    tmem_alloc(tmem_slot, 512);
+    tmem_alloc(&sh.tmem, 512);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = sh.tmem;
   pdl_wait();
 
-  const int units = *plan.n_units;
-  // the key tiles of a unit (whole warps)
-  auto span = [&](const PrefixUnit& it, int& first, int& end) {
-    prefix_span(plan, it, p.row_pos, p.row_slot, p.chunk, p.page_tokens, first, end);
-    return (end - first + kPgTile - 1) / kPgTile;
-  };
+  // this CTA's twos of units: number i is blockIdx.x + i * gridDim.x
+  const int twos = (*plan.n_units + 1) / 2, turns = (twos - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+  bool ok = true;
 
   if (warp == 8) {
     const int boxes = kPgTile / p.box;
     int kt = 0, k_stage = 0, v_stage = 0;                // key tiles so far, places in the rings
     uint32_t k_free = 1, v_free = 1;
-    bool ok = true;
-    for (int unit = blockIdx.x; unit < units && ok; unit += gridDim.x) {
-      const PrefixUnit it = prefix_unit(plan, unit);
-      if (it.rows == 0) continue;
-      const int g = it.head;
-      int first, end;
-      const int n = span(it, first, end);
-      const int* table = p.page_table + 1ll * it.slot * p.max_pages;
-      int row = 0, u = 0;                                // lane i: pool row of box i of the walk, 32 boxes at a time
-      for (int j = 0; j < n; ++j, ++kt, u += boxes) {
-        if ((u & 31) == 0) {                             // boxes divides 32
-          const int key = first + (u + lane) * p.box, pg = key / p.page_tokens;
-          const int id = key < end && pg < p.max_pages ? table[pg] : -1;
-          row = id >= 0 ? id * p.page_tokens + (key - pg * p.page_tokens) : p.hidden_row;
-        }
-        // one tile of keys or values: `chunks` chunks of 64 columns from column x on
-        auto fetch = [&](uint8_t* dst, uint64_t* bar, int x, int chunks) {
-          if (lane == 0) mbar_expect_tx(bar, chunks * kPgChunk);
+    // lane i: pool row of box i of the 32 boxes from box u of a walk on
+    auto locate = [&](const GroupWork& w, int t, int u) {
+      const int key = w.first[t] + (u + lane) * p.box, pg = key / p.page_tokens;
+      const int id = key < w.end[t] && pg < p.max_pages ? p.page_table[1ll * w.unit[t].slot * p.max_pages + pg] : -1;
+      return id >= 0 ? id * p.page_tokens + (key - pg * p.page_tokens) : p.hidden_row;
+    };
+    GroupWork next = {};
+    int next_row[2] = {0, 0};
+    auto prepare = [&](int turn) {                       // behind the copies of the units before
+      if (turn >= turns) return;
+      const int at = 2 * (static_cast<int>(blockIdx.x) + turn * static_cast<int>(gridDim.x));
+#pragma unroll
+      for (int t = 0; t < 2; ++t) next.unit[t] = prefix_unit(plan, at + t);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        prefix_span(plan, next.unit[t], p.row_pos, p.row_slot, p.chunk, p.page_tokens, next.first[t], next.end[t]);
+      const PrefixUnit &a = next.unit[0], &b = next.unit[1];
+      next.both = b.rows > 0 && !a.tail && !b.tail && a.slot == b.slot && a.key0 == b.key0 && a.key1 == b.key1 && a.head == b.head;
+      if (next.both && next.first[0] < next.end[0] && next.first[1] < next.end[1]) {
+        next.first[0] = next.first[1] = min(next.first[0], next.first[1]);
+        next.end[0] = next.end[1] = max(next.end[0], next.end[1]);
+      } else {
+        next.both = 0;                                   // one of them sees nothing
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        next.tiles[t] = (next.end[t] - next.first[t] + kPgTile - 1) / kPgTile;
+        if (!(t == 1 && next.both)) next_row[t] = locate(next, t, 0);
+      }
+    };
+    prepare(0);
+    for (int turn = 0; turn < turns && ok; ++turn) {
+      GroupWork w = next;
+      int row[2] = {next_row[0], next_row[1]};
+      w.base = kt;
+      ok = __all_sync(0xffffffffu, mbar_wait(&sh.info_empty[turn % kPgInfos], ((turn / kPgInfos) & 1) ^ 1, p.status, 459)) != 0;
+      if (!ok) break;
+      if (lane == 0) {
+        sh.info[turn % kPgInfos] = w;
+        mbar_arrive(&sh.info_full[turn % kPgInfos]);
+      }
+      const int most = w.both ? w.tiles[0] : max(w.tiles[0], w.tiles[1]);
+      if (most == 0) prepare(turn + 1);
+      for (int j = 0; j < most && ok; ++j) {
+        const int u = j * boxes;
 #pragma unroll 1
-          for (int i = 0; i < boxes; ++i) {
-            const int at = __shfl_sync(0xffffffffu, row, (u + i) & 31);
-            if (lane == 0)
-#pragma unroll 1
-              for (int c = 0; c < chunks; ++c) tma_load_3d(dst + c * kPgChunk + i * p.box * 128, &pool, bar, x + 64 * c, at, 0);
-            __syncwarp();
+        for (int t = 0; t < (w.both ? 1 : 2); ++t) {
+          if (j >= (t ? w.tiles[1] : w.tiles[0])) continue;
+          if (u > 0 && (u & 31) == 0) {                  // boxes divides 32
+            if (t) row[1] = locate(w, 1, u);
+            else row[0] = locate(w, 0, u);
           }
-        };
-        ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[k_stage], k_free, p.status, 460)) != 0;
-        if (!ok) break;
-        fetch(s_k + k_stage * k_bytes, &k_full[k_stage], g * p.dp, p.kd);
-        if (++k_stage == p.k_stages) {
-          k_stage = 0;
-          k_free ^= 1;
-        }
-        ok = __all_sync(0xffffffffu, mbar_wait(&v_empty[v_stage], v_free, p.status, 461)) != 0;
-        if (!ok) {
+          const int here = t ? row[1] : row[0], g = t ? w.unit[1].head : w.unit[0].head;
+          // one tile of keys or values: `chunks` chunks of 64 columns from column x on
+          auto fetch = [&](uint8_t* dst, uint64_t* bar, int x, int chunks) {
+            if (lane == 0) mbar_expect_tx(bar, chunks * kPgChunk);
+#pragma unroll 1
+            for (int i = 0; i < boxes; ++i) {
+              const int at = __shfl_sync(0xffffffffu, here, (u + i) & 31);
+              if (lane == 0)
+#pragma unroll 1
+                for (int c = 0; c < chunks; ++c) tma_load_3d(dst + c * kPgChunk + i * p.box * 128, &pool, bar, x + 64 * c, at, 0);
+              __syncwarp();
+            }
+          };
+          ok = __all_sync(0xffffffffu, mbar_wait(&sh.k_empty[k_stage], k_free, p.status, 460)) != 0;
+          if (!ok) break;
+          fetch(s_k + k_stage * k_bytes, &sh.k_full[k_stage], g * p.dp, p.kd);
+          if (++k_stage == p.k_stages) {
+            k_stage = 0;
+            k_free ^= 1;
+          }
           ++kt;
-          break;
+          ok = __all_sync(0xffffffffu, mbar_wait(&sh.v_empty[v_stage], v_free, p.status, 461)) != 0;
+          if (!ok) break;
+          fetch(s_v + v_stage * v_bytes, &sh.v_full[v_stage], p.kv_heads * p.dp + g * p.vp, p.vc);
+          if (++v_stage == p.v_stages) {
+            v_stage = 0;
+            v_free ^= 1;
+          }
         }
-        fetch(s_v + v_stage * v_bytes, &v_full[v_stage], p.kv_heads * p.dp + g * p.vp, p.vc);
-        if (++v_stage == p.v_stages) {
-          v_stage = 0;
-          v_free ^= 1;
-        }
+        if (j == 0 && ok) prepare(turn + 1);
       }
     }
     if (!ok && lane == 0) {
       // something else gave up: let the copies under way land before the shared memory goes away
       for (int b = max(0, kt - 2); b < kt; ++b) {
-        for (int i = 0; i < (1 << 20) && !mbar_test_wait(&k_full[b % p.k_stages], (b / p.k_stages) & 1); ++i) {
+        for (int i = 0; i < (1 << 18) && !mbar_test_wait(&sh.k_full[b % p.k_stages], (b / p.k_stages) & 1); ++i) {
         }
-        for (int i = 0; i < (1 << 20) && !mbar_test_wait(&v_full[b % p.v_stages], (b / p.v_stages) & 1); ++i) {
+        for (int i = 0; i < (1 << 18) && !mbar_test_wait(&sh.v_full[b % p.v_stages], (b / p.v_stages) & 1); ++i) {
         }
       }
     }
   } else if (warp == 9) {
-    const bool leader = elect_one();
-    const uint32_t idesc_s = umma_idesc(kPgTile, kPgTile, 1u, 1u);
-    const uint32_t idesc_pv = umma_idesc_bmn(kPgTile, p.vp, 1u, 1u);
-    const uint64_t q_desc = umma_desc_sw128(smem_u32(s_q)), k_desc = umma_desc_sw128(smem_u32(s_k));
-    const uint64_t v_desc = umma_desc_sw128_mn(smem_u32(s_v), kPgChunk, 1024);
-    const int whole = p.dp / 64, rest = p.dp / 16 - 4 * whole;
-    bool ok = true;
-    int kt = 0, done[2] = {0, 0}, live = 0;              // key tiles; products of each tile; units with work so far
-    for (int unit = blockIdx.x; unit < units && ok; unit += gridDim.x) {
-      const PrefixUnit it = prefix_unit(plan, unit);
-      if (it.rows == 0) continue;
-      int first, end;
-      const int n = span(it, first, end);
-      if (n == 0) continue;
-      if (leader) {                                      // one thread: votes and the like between two products cost as much as the products
-        ok = mbar_wait(q_full, live & 1, p.status, 470);
-        ++live;
-        tc_fence_after();
-        const bool both = it.rows * p.n <= kPgTile;
-        const int step = both ? 2 : 1;
-        // per tile: its next scores and next values, as numbers of key tiles; scores overwrite the P that the values before them read
-        int sj[2] = {0, both ? 1 : 0}, pj[2] = {0, both ? 1 : 0};
-        uint32_t idle = 0;
-        long long since = 0;
-        while (ok && (pj[0] < n || pj[1] < n)) {
-          bool moved = false;
+    // one thread: votes and the like between two products cost as much as the products
+    if (elect_one()) {
+      const uint32_t idesc_s = umma_idesc(kPgTile, kPgTile, 1u, 1u);
+      const uint32_t idesc_pv = umma_idesc_bmn(kPgTile, p.vp, 1u, 1u);
+      const uint64_t q_desc = umma_desc_sw128(smem_u32(s_q)), k_desc = umma_desc_sw128(smem_u32(s_k));
+      const uint64_t v_desc = umma_desc_sw128_mn(smem_u32(s_v), kPgChunk, 1024);
+      const int whole = p.dp / 64, rest = p.dp / 16 - 4 * whole;
+      // per tile: the turn it is at, its key tiles (0: not begun), the next scores and values of that turn, and counts of units and
+      // products for the barriers' phases.  Scores overwrite the P that the values before them read.
+      int turn[2] = {0, 0}, n[2] = {0, 0}, sj[2] = {0, 0}, pj[2] = {0, 0}, begun[2] = {0, 0}, done[2] = {0, 0};
+      uint32_t idle = 0;
+      long long since = 0;
+      while (ok && (turn[0] < turns || turn[1] < turns)) {
+        bool moved = false;
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if (pj[t] < sj[t] && pj[t] < n) {
-              const int at = kt + pj[t], stage = p.v_stages == 2 ? at & 1 : 0, phase = p.v_stages == 2 ? (at >> 1) & 1 : at & 1;
-              if (mbar_test_wait(&p_full[t], done[t] & 1) && mbar_test_wait(&v_full[stage], phase)) {
-                tc_fence_after();
-                const uint64_t vd = v_desc + static_cast<uint64_t>(stage * v_bytes / 16);
-                const uint32_t o = tmem + 256 + t * 128, a = tmem + t * 128;
-                umma4_ts<128>(o, a, vd, idesc_pv, pj[t] >= step);
-                umma4_ts<128>(o, a + 32, vd + 512, idesc_pv, 1u);
-                ++done[t];
-                if (both || pj[t ^ 1] > pj[t]) tc_commit_if(true, &v_empty[stage]);      // the tile's last reader
-                pj[t] += step;
-                if (pj[t] >= n) tc_commit_if(true, &o_full[t]);
-                moved = true;
-              }
+        for (int t = 0; t < 2; ++t) {
+          if (turn[t] >= turns) continue;
+          const GroupWork& w = sh.info[turn[t] % kPgInfos];
+          uint64_t* read = &sh.info_empty[turn[t] % kPgInfos];
+          if (n[t] == 0) {
+            if (!mbar_test_wait(&sh.info_full[turn[t] % kPgInfos], (turn[t] / kPgInfos) & 1)) continue;
+            moved = true;
+            n[t] = w.tiles[t];
+            sj[t] = pj[t] = 0;
+            if (n[t] == 0) {
+              mbar_arrive(read);
+              ++turn[t];
+              continue;
             }
-            if (sj[t] < n && sj[t] == pj[t]) {
-              const int at = kt + sj[t], stage = p.k_stages == 2 ? at & 1 : 0, phase = p.k_stages == 2 ? (at >> 1) & 1 : at & 1;
-              if (mbar_test_wait(&k_full[stage], phase)) {
-                tc_fence_after();
-                uint64_t a = q_desc + static_cast<uint64_t>(both ? 0 : t * q_bytes / 16), b = k_desc + static_cast<uint64_t>(stage * k_bytes / 16);
-#pragma unroll 1
-                for (int c = 0; c < whole; ++c, a += kPgChunk / 16, b += kPgChunk / 16) umma4_ss<2, 2>(tmem + t * 128, a, b, idesc_s, c);
-#pragma unroll 1
-                for (int k = 0; k < rest; ++k) umma_bf16(tmem + t * 128, a + 2 * k, b + 2 * k, idesc_s, whole > 0 || k > 0);
-                tc_commit_if(true, &s_full[t]);
-                if (both || sj[t ^ 1] > sj[t]) tc_commit_if(true, &k_empty[stage]);
-                sj[t] += step;
-                moved = true;
+          }
+          const bool both = w.both != 0;
+          const int o = t ^ 1;
+          if (pj[t] < sj[t]) {
+            const int at = copy_index(w, t, pj[t]), stage = p.v_stages == 2 ? at & 1 : 0, phase = p.v_stages == 2 ? (at >> 1) & 1 : at & 1;
+            if (mbar_test_wait(&sh.p_full[t], done[t] & 1) && mbar_test_wait(&sh.v_full[stage], phase)) {
+              tc_fence_after();
+              const uint64_t vd = v_desc + static_cast<uint64_t>(stage * v_bytes / 16);
+              const uint32_t to = tmem + 256 + t * 128, a = tmem + t * 128;
+              umma4_ts<128>(to, a, vd, idesc_pv, pj[t] > 0);
+              umma4_ts<128>(to, a + 32, vd + 512, idesc_pv, 1u);
+              ++done[t];
+              if (!both || turn[o] > turn[t] || (turn[o] == turn[t] && pj[o] > pj[t])) tc_commit_if(true, &sh.v_empty[stage]);      // its last reader
+              ++pj[t];
+              moved = true;
+              if (pj[t] == n[t]) {
+                tc_commit_if(true, &sh.o_full[t]);
+                mbar_arrive(read);
+                ++turn[t];
+                n[t] = 0;
+                continue;
               }
             }
           }
-          if (moved) {
-            idle = 0;
-            since = 0;
-          } else if ((++idle & 0x3ff) == 0) {            // as long as any other wait: see mbar_wait
-            if (since == 0) since = clock64();
-            if (clock64() - since > DS41_WAIT_LIMIT_CYCLES ||
-                (p.status != nullptr && *reinterpret_cast<volatile int*>(p.status) != kStatusOk)) {
-              if (p.status != nullptr && atomicCAS(p.status, kStatusOk, kStatusMbarTimeout) == kStatusOk) {
-                p.status[1] = 471;
-                p.status[2] = static_cast<int>(blockIdx.x);
-                p.status[3] = pj[0];
-              }
-              ok = false;
+          if (sj[t] < n[t] && sj[t] == pj[t]) {
+            const int at = copy_index(w, t, sj[t]), stage = p.k_stages == 2 ? at & 1 : 0, phase = p.k_stages == 2 ? (at >> 1) & 1 : at & 1;
+            if (mbar_test_wait(&sh.k_full[stage], phase) && (sj[t] > 0 || mbar_test_wait(&sh.q_full[t], begun[t] & 1))) {
+              tc_fence_after();
+              uint64_t a = q_desc + static_cast<uint64_t>(t * q_bytes / 16), b = k_desc + static_cast<uint64_t>(stage * k_bytes / 16);
+#pragma unroll 1
+              for (int c = 0; c < whole; ++c, a += kPgChunk / 16, b += kPgChunk / 16) umma4_ss<2, 2>(tmem + t * 128, a, b, idesc_s, c);
+#pragma unroll 1
+              for (int k = 0; k < rest; ++k) umma_bf16(tmem + t * 128, a + 2 * k, b + 2 * k, idesc_s, whole > 0 || k > 0);
+              tc_commit_if(true, &sh.s_full[t]);
+              if (!both || turn[o] > turn[t] || (turn[o] == turn[t] && sj[o] > sj[t])) tc_commit_if(true, &sh.k_empty[stage]);
+              if (sj[t] == 0) ++begun[t];
+              ++sj[t];
+              if (sj[t] == n[t]) tc_commit_if(true, &sh.q_empty[t]);
+              moved = true;
             }
           }
         }
-        kt += n;
+        if (moved) {
+          idle = 0;
+          since = 0;
+        } else if ((++idle & 0x3ff) == 0) {              // as long as any other wait: see mbar_wait
+          if (since == 0) since = clock64();
+          if (clock64() - since > DS41_WAIT_LIMIT_CYCLES ||
+              (p.status != nullptr && *reinterpret_cast<volatile int*>(p.status) != kStatusOk)) {
+            if (p.status != nullptr && atomicCAS(p.status, kStatusOk, kStatusMbarTimeout) == kStatusOk) {
+              p.status[1] = 471;
+              p.status[2] = static_cast<int>(blockIdx.x);
+              p.status[3] = turn[0];
+            }
+            ok = false;
+          }
+        }
       }
-      ok = __ballot_sync(0xffffffffu, leader && ok) != 0;
     }
+    __syncwarp();
   } else {
-    const int t = warp >> 2, quad = warp & 3, mine = quad * 32 + lane;
-    const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
-    const uint32_t s_t = tmem + lanes + t * 128, o_t = tmem + lanes + 256 + t * 128;
-    int kt = 0, tiles = 0, outs[2] = {0, 0};             // key tiles so far; tiles of S seen by this half; finished results of both
-    bool ok = true;
-    // the loop runs to its end whatever happened: its barriers are for all eight warps
-    for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
-      const PrefixUnit it = prefix_unit(plan, unit);
-      if (it.rows == 0) continue;
-      const int g = it.head, count = it.rows * p.n;
-      const bool both = count <= kPgTile;                // the same queries in both tiles
-      int first, end;
-      const int n = span(it, first, end);
-      const int mine_q = both ? mine : t * kPgTile + mine;
-      int r = -1, lo = 0, hi = 0;
-      if (mine_q < count) {
-        r = prefix_row(plan, it, mine_q / p.n);
-        const int pos = p.row_pos[r];
-        if (p.row_slot[r] >= 0) {
-          lo = chunk_start(pos, p.chunk);
-          hi = min(pos + 1, it.key1);
-        }
-      }
-      s_row[t * kPgTile + mine] = r;                     // equal in both halves where the queries are
-      named_barrier(1, 2 * kPgTile);
-      if (n > 0) {
-        // a row's 16-byte pieces by neighbouring lanes, four rows of a lane under way together
-        const int pieces = p.dp / 8, per = 32 / pieces, sub = lane / pieces, c = lane % pieces, rows = (both ? 1 : 2) * kPgTile;
-        for (int x0 = warp * per + sub; x0 < rows; x0 += 32 * per) {
-          uint4 v[4];
+    // the roles that follow one tile: its work at a turn, once it is known; whole warps
+    auto work = [&](int turn, int t, PrefixUnit& unit, int& first, int& end, int& last) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&sh.info_full[turn % kPgInfos], (turn / kPgInfos) & 1, p.status, 462)) != 0;
+      if (!ok) return 0;
+      const GroupWork& w = sh.info[turn % kPgInfos];
+      unit = w.unit[t];
+      first = w.first[t];
+      end = w.end[t];
+      last = copy_index(w, t, w.tiles[t] > 0 ? w.tiles[t] - 1 : 0);
+      return w.tiles[t];
+    };
+    auto work_read = [&](int turn) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.info_empty[turn % kPgInfos]);
+    };
+    PrefixUnit unit;
+    int first, end, last;                                // last: the last tile's number
+    if (warp >= 10) {
+      const int t = warp - 10, pieces = p.dp / 8, per = 32 / pieces, sub = lane / pieces, c = lane % pieces;
+      int filled = 0;
+      for (int turn = 0; turn < turns; ++turn) {
+        const int n = work(turn, t, unit, first, end, last);
+        if (!ok) break;
+        work_read(turn);
+        if (n == 0) continue;
+        const int here = unit.rows * p.n;
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_empty[t], (filled & 1) ^ 1, p.status, 463)) != 0;
+        if (!ok) break;
+        ++filled;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int x = x0 + 8 * per * k, row = sub < per && x < rows ? s_row[x] : -1;
-            v[k] = make_uint4(0, 0, 0, 0);
-            if (row >= 0) v[k] = *reinterpret_cast<const uint4*>(p.q + row * p.ld_q + 1ll * (g * p.n + x % p.n) * p.dp + 8 * c);
+        for (int x = lane; x < kPgTile; x += 32) {       // what a query sees
+          int4 v = make_int4(-1, 0, 0, 0);
+          if (x < here) {
+            v.x = prefix_row(plan, unit, x / p.n);
+            const int pos = p.row_pos[v.x];
+            if (p.row_slot[v.x] >= 0) {
+              v.y = chunk_start(pos, p.chunk);
+              v.z = min(pos + 1, unit.key1);
+            }
+          }
+          sh.query[t][x] = v;
+        }
+        // a row's 16-byte pieces by neighbouring lanes, eight rows of a lane under way together; rows without a query stay as they are
+        for (int x0 = sub; x0 < here; x0 += 8 * per) {
+          uint4 v[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int x = x0 + per * k;
+            if (sub < per && x < here)
+              v[k] = *reinterpret_cast<const uint4*>(p.q + 1ll * prefix_row(plan, unit, x / p.n) * p.ld_q +
+                                                     1ll * (unit.head * p.n + x % p.n) * p.dp + 8 * c);
           }
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int x = x0 + 8 * per * k, y = x & (kPgTile - 1);
-            if (sub < per && x < rows)
-              *reinterpret_cast<uint4*>(s_q + (x >> 7) * q_bytes + (c >> 3) * kPgChunk + y * 128 + (((c & 7) ^ (y & 7)) << 4)) = v[k];
+          for (int k = 0; k < 8; ++k) {
+            const int x = x0 + per * k;
+            if (sub < per && x < here)
+              *reinterpret_cast<uint4*>(s_q + t * q_bytes + (c >> 3) * kPgChunk + x * 128 + (((c & 7) ^ (x & 7)) << 4)) = v[k];
           }
         }
         fence_async_smem();
-        mbar_arrive(q_full);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.q_full[t]);
       }
-      // limits of the warp's queries: tiles between them need no look at single keys
-      int low = hi > lo ? lo : 0, high = hi > lo ? hi : 0x7fffffff;
-#pragma unroll
-      for (int o = 16; o; o >>= 1) {
-        low = max(low, __shfl_xor_sync(0xffffffffu, low, o));
-        high = min(high, __shfl_xor_sync(0xffffffffu, high, o));
-      }
-      float m = -INFINITY, l = 0.f;
-      const int step = both ? 2 : 1, from = both ? t : 0;
-      for (int j = from; j < n && ok; j += step) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], tiles & 1, p.status, 480 + t)) != 0;
+    } else {
+      const int t = warp >> 2, quad = warp & 3, mine = quad * 32 + lane;
+      const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+      const uint32_t s_t = tmem + lanes + t * 128, o_t = tmem + lanes + 256 + t * 128;
+      int tiles = 0, done = 0;                           // tiles of S, units with keys so far
+      for (int turn = 0; turn < turns; ++turn) {
+        const int n = work(turn, t, unit, first, end, last);
         if (!ok) break;
-        ++tiles;
-        tc_fence_after();
-        const int key0 = first + j * kPgTile;
-        const bool edge = key0 < low || key0 + kPgTile > high;
-        const int shown = hi - key0, hidden = lo - key0;             // columns [hidden, shown) of this tile are visible
-        // Two halves of 64 columns, each read twice: the loops' bodies have to stay in the instruction cache, which this code shares
-        // with the other roles' (unrolled over the tile, 42 % of all cycles were waits for instructions)
-        float top = -INFINITY;
-        uint32_t v[64];
-        auto load = [&](int c) {
-          tmem_ld_32x32(s_t + c, reinterpret_cast<uint32_t(&)[32]>(v[0]));
-          tmem_ld_32x32(s_t + c + 32, reinterpret_cast<uint32_t(&)[32]>(v[32]));
-          tmem_wait_ld();
-          if (edge) {
-#pragma unroll
-            for (int i = 0; i < 64; ++i) v[i] = c + i < shown && c + i >= hidden ? v[i] : 0xff800000u;
+        work_read(turn);
+        if (n == 0) {                                    // nothing for any of its rows
+          if (mine < unit.rows * p.n) {
+            const long long cell = (1ll * plan.cell[prefix_row(plan, unit, mine / p.n)] + unit.part) * p.heads + unit.head * p.n +
+                                   mine % p.n;
+            *reinterpret_cast<float2*>(plan.part_ml + 2 * cell) = make_float2(-INFINITY, 0.f);
           }
-        };
-#pragma unroll 1
-        for (int c = 0; c < kPgTile; c += 64) {
-          load(c);
-          float tops[4] = {top, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int i = 0; i < 64; i += 2) tops[(i >> 1) & 3] = fmaxf(tops[(i >> 1) & 3], fmaxf(__uint_as_float(v[i]), __uint_as_float(v[i + 1])));
-          top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+          continue;
         }
-        top *= p.scale_log2;
-        const bool grow = top > m + 8.f || (m == -INFINITY && top > m);
-        if (__any_sync(0xffffffffu, grow)) {
-          const float m_new = grow ? top : m;
-          const float alpha = m == -INFINITY ? 0.f : ex2_approx(m - m_new);
-          if (grow) l *= alpha;
-          m = m_new;
-          if (j > from) {
-            const float keep = grow ? alpha : 1.f;
-#pragma unroll 1
-            for (int c = 0; c < p.vp; c += 16) {
-              uint32_t o[16];
-              tmem_ld_32x16(o_t + c, o);
-              tmem_wait_ld();
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_full[t], done & 1, p.status, 482 + t)) != 0;
+        if (!ok) break;
+        const int4 me = sh.query[t][mine];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.q_empty[t]);
+        const int r = me.x, lo = me.y, hi = me.z;
+        // limits of the warp's queries: tiles between them need no look at single keys
+        int low = hi > lo ? lo : 0, high = hi > lo ? hi : 0x7fffffff;
 #pragma unroll
-              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
-              tmem_st_32x16(o_t + c, o);
-            }
-          }
+        for (int o = 16; o; o >>= 1) {
+          low = max(low, __shfl_xor_sync(0xffffffffu, low, o));
+          high = min(high, __shfl_xor_sync(0xffffffffu, high, o));
         }
-        const float neg = m == -INFINITY ? 0.f : -m;
-        const float2 by = make_float2(p.scale_log2, p.scale_log2), off = make_float2(neg, neg);
-        float2 sums[2] = {};
-#pragma unroll 1
-        for (int c = 0; c < kPgTile; c += 64) {
-          load(c);
-          uint32_t w[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            float2 e = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), by, off);
-            e = make_float2(ex2_approx(e.x), ex2_approx(e.y));
-            sums[i & 1] = add2(sums[i & 1], e);
-            const __nv_bfloat162 q = __floats2bfloat162_rn(e.x, e.y);
-            w[i] = *reinterpret_cast<const uint32_t*>(&q);
-          }
-          tmem_st_32x32(s_t + c / 2, w);                 // columns whose S this thread has read
-        }
-        sums[0] = add2(sums[0], sums[1]);
-        l += sums[0].x + sums[0].y;
-        if (it.tail && key0 + kPgTile > end) {
-          // Places behind the last position belong to nobody, and a weight of zero does not take a NaN or an infinity away: their values
-          // become zeros, a thread to a place.
-          const int at = kt + j, stage = p.v_stages == 2 ? at & 1 : 0, phase = p.v_stages == 2 ? (at >> 1) & 1 : at & 1;
-          ok = __all_sync(0xffffffffu, mbar_wait(&v_full[stage], phase, p.status, 484 + t)) != 0;
+        const bool idle = high == 0x7fffffff;            // no query of this warp sees anything
+        float m = -INFINITY, l = 0.f;
+        for (int j = 0; j < n; ++j) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&sh.s_full[t], tiles & 1, p.status, 480 + t)) != 0;
           if (!ok) break;
-          if (key0 + mine >= end)
-            for (int i = 0; i < 8 * p.vc; ++i)
-              *reinterpret_cast<uint4*>(s_v + stage * v_bytes + (i >> 3) * kPgChunk + mine * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
-          fence_async_smem();
-        }
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(&p_full[t]);
-      }
-      kt += n;
-      if (hi <= lo) {                                    // a query that sees nothing here: tiles without an edge did not look
-        m = -INFINITY;
-        l = 0.f;
-      }
-      if (both) s_ml[t * kPgTile + mine] = make_float2(m, l);
-      // which results exist: tile x has one where it had a tile of keys
-      const bool has[2] = {n > 0, both ? n > 1 : n > 0};
+          ++tiles;
+          const int key0 = first + j * kPgTile;
+          if (!idle) {
+            tc_fence_after();
+            const bool edge = key0 < low || key0 + kPgTile > high;
+            const int shown = hi - key0, hidden = lo - key0;             // columns [hidden, shown) of this tile are visible
+            // Two halves of 64 columns, each read twice: the loops' bodies have to stay in the instruction cache, which this code shares
+            // with the other roles' (unrolled over the tile, 42 % of all cycles were waits for instructions)
+            float top = -INFINITY;
+            uint32_t v[64];
+            auto load = [&](int c) {
+              tmem_ld_32x32(s_t + c, reinterpret_cast<uint32_t(&)[32]>(v[0]));
+              tmem_ld_32x32(s_t + c + 32, reinterpret_cast<uint32_t(&)[32]>(v[32]));
+              tmem_wait_ld();
+              if (edge) {
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        if (!has[x]) continue;
-        if (ok && (both || x == t)) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[x], outs[x] & 1, p.status, 490 + x)) != 0;
-        ++outs[x];
-      }
-      tc_fence_after();
-      named_barrier(1, 2 * kPgTile);                     // s_ml is there
-      const bool write = ok && r >= 0;
-      const long long cell = write ? (1ll * plan.cell[r] + it.part) * p.heads + g * p.n + mine_q % p.n : 0;
-      float f0 = 1.f, f1 = 0.f;                          // factors on the two tiles' results
-      if (both) {
-        const float2 a = s_ml[mine], b = s_ml[kPgTile + mine];
-        m = fmaxf(a.x, b.x);
-        f0 = a.x == -INFINITY ? 0.f : ex2_approx(a.x - m);
-        f1 = b.x == -INFINITY ? 0.f : ex2_approx(b.x - m);
-        l = a.y * f0 + b.y * f1;
-      }
-      if (write && !(both && t == 1)) *reinterpret_cast<float2*>(plan.part_ml + 2 * cell) = make_float2(m, l);
-      if (ok && n > 0) {                                 // whole warps: tensor memory is read by all lanes
-        float* dst = plan.part_o + cell * p.vp;
-        const int half = p.vp / 32 * 16, c0 = both && t == 1 ? half : 0, c1 = both && t == 0 ? half : p.vp;
-        for (int c = c0; c < c1; c += 16) {
-          uint32_t a[16], b[16];
-          tmem_ld_32x16((both ? tmem + lanes + 256 : o_t) + c, a);
-          if (has[1] && both) tmem_ld_32x16(tmem + lanes + 384 + c, b);
-          tmem_wait_ld();
-          if (write) {
-#pragma unroll
-            for (int i = 0; i < 16; i += 8) {
-              float o[8];
-#pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                o[e] = f0 * __uint_as_float(a[i + e]);
-                if (has[1] && both) o[e] += f1 * __uint_as_float(b[i + e]);
+                for (int i = 0; i < 64; ++i) v[i] = c + i < shown && c + i >= hidden ? v[i] : 0xff800000u;
               }
-              store8(dst + c + i, o);
+            };
+#pragma unroll 1
+            for (int c = 0; c < kPgTile; c += 64) {
+              load(c);
+              float tops[4] = {top, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+              for (int i = 0; i < 64; i += 2)
+                tops[(i >> 1) & 3] = fmaxf(tops[(i >> 1) & 3], fmaxf(__uint_as_float(v[i]), __uint_as_float(v[i + 1])));
+              top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
             }
+            top *= p.scale_log2;
+            const bool grow = hi > lo && (top > m + 8.f || (m == -INFINITY && top > m));
+            if (__any_sync(0xffffffffu, grow)) {
+              const float m_new = grow ? top : m;
+              const float alpha = m == -INFINITY ? 0.f : ex2_approx(m - m_new);
+              if (grow) l *= alpha;
+              m = m_new;
+              if (j > 0) {
+                const float keep = grow ? alpha : 1.f;
+#pragma unroll 1
+                for (int c = 0; c < p.vp; c += 16) {
+                  uint32_t o[16];
+                  tmem_ld_32x16(o_t + c, o);
+                  tmem_wait_ld();
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
+                  tmem_st_32x16(o_t + c, o);
+                }
+              }
+            }
+            const float neg = m == -INFINITY ? 0.f : -m;
+            const float2 by = make_float2(p.scale_log2, p.scale_log2), off = make_float2(neg, neg);
+            float2 sums[2] = {};
+#pragma unroll 1
+            for (int c = 0; c < kPgTile; c += 64) {
+              load(c);
+              uint32_t e2[32];
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                float2 e = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), by, off);
+                e = make_float2(ex2_approx(e.x), ex2_approx(e.y));
+                sums[i & 1] = add2(sums[i & 1], e);
+                const __nv_bfloat162 b = __floats2bfloat162_rn(e.x, e.y);
+                e2[i] = *reinterpret_cast<const uint32_t*>(&b);
+              }
+              tmem_st_32x32(s_t + c / 2, e2);            // columns whose S this thread has read
+            }
+            sums[0] = add2(sums[0], sums[1]);
+            l += sums[0].x + sums[0].y;
           }
+          if (unit.tail && key0 + kPgTile > end) {
+            // Places behind the last position belong to nobody, and a weight of zero does not take a NaN or an infinity away: their
+            // values become zeros, a thread to a place.  It is the last tile.
+            const int stage = p.v_stages == 2 ? last & 1 : 0, phase = p.v_stages == 2 ? (last >> 1) & 1 : last & 1;
+            ok = __all_sync(0xffffffffu, mbar_wait(&sh.v_full[stage], phase, p.status, 484 + t)) != 0;
+            if (!ok) break;
+            if (key0 + mine >= end)
+              for (int i = 0; i < 8 * p.vc; ++i)
+                *reinterpret_cast<uint4*>(s_v + stage * v_bytes + (i >> 3) * kPgChunk + mine * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+            fence_async_smem();
+          }
+          tmem_wait_st();
+          tc_fence_before();
           __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.p_full[t]);
         }
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_full[t], done & 1, p.status, 490 + t)) != 0;
+        if (!ok) break;
+        ++done;
+        tc_fence_after();
+        if (hi <= lo) {                                  // a query that sees nothing here: tiles without an edge did not look
+          m = -INFINITY;
+          l = 0.f;
+        }
+        const bool write = r >= 0;
+        const long long cell = write ? (1ll * plan.cell[r] + unit.part) * p.heads + unit.head * p.n + mine % p.n : 0;
+        if (write) *reinterpret_cast<float2*>(plan.part_ml + 2 * cell) = make_float2(m, l);
+        if (!idle) {                                     // whole warps: tensor memory is read by all lanes
+          float* dst = plan.part_o + cell * p.vp;
+#pragma unroll 1
+          for (int c = 0; c < p.vp; c += 16) {
+            uint32_t a[16];
+            tmem_ld_32x16(o_t + c, a);
+            tmem_wait_ld();
+            if (write) {
+              store8(dst + c, reinterpret_cast<const float(&)[8]>(a[0]));
+              store8(dst + c + 8, reinterpret_cast<const float(&)[8]>(a[8]));
+            }
+            __syncwarp();
+          }
+        }
+        tc_fence_before();
       }
-      tc_fence_before();
-      named_barrier(1, 2 * kPgTile);                     // tensor memory and s_ml may be written again
     }
   }
   __syncthreads();
@@ -429,7 +518,7 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
 // Stages and shared memory of a launch; false: the sizes do not fit.
 static bool plan_prefix_group(const ds41_group_attend_args& a, const ds41_prefix_plan& plan, PrefixGroupParams& p, int& smem) {
   p.n = a.heads / a.kv_heads;
-  if (a.f32 || a.n_pages <= 0 || a.vdim_pad > 128 || (a.ld_q & 7) || plan.rows_per_unit * p.n > 2 * kPgTile ||
+  if (a.f32 || a.n_pages <= 0 || a.vdim_pad > 128 || (a.ld_q & 7) || plan.rows_per_unit * p.n > kPgTile ||
       ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.pool)) & 15) ||
       1ll * a.n_pages * a.page_tokens >= (1ll << 31) - 1)
     return false;
@@ -439,7 +528,7 @@ static bool plan_prefix_group(const ds41_group_attend_args& a, const ds41_prefix
   p.kd = (a.dim_pad + 63) / 64;
   p.vc = (a.vdim_pad + 63) / 64;
   const int qk = p.kd * kPgChunk, v = p.vc * kPgChunk;
-  constexpr int kExtra = 1024 + 128 + 4 * 2 * kPgTile + 8 * 2 * kPgTile, kLimit = 227 * 1024 - kExtra;
+  constexpr int kExtra = 1024 + static_cast<int>(sizeof(GroupShared)), kLimit = 227 * 1024 - kExtra;
   p.k_stages = p.v_stages = 1;
   if (3 * qk + v > kLimit) return false;
   if (4 * qk + v <= kLimit) p.k_stages = 2;

@@ -68,7 +68,7 @@ class Cost:
         self.unit, self.key, self.byte = unit, key, 1 / 4e6
 
 
-COSTS = {"grouped": Cost(3.0, 0.006), "latent": Cost(4.0, 0.02)}
+COSTS = {"grouped": Cost(5.0, 0.02), "latent": Cost(4.0, 0.02)}
 
 
 def key_span(work: Sequence[Tuple[int, int, int]], width: int, part_bytes: int, most: int, unit: int, cost: Cost) -> int:
@@ -111,11 +111,12 @@ class PrefixPlan:
         self.kind, self.rows, self.heads, self.kv_heads, self.vdim = kind, rows, heads, kv_heads, vdim
         self.page_tokens, self.dtype, self.device = page_tokens, dtype, torch.device(device)
         self.min_tokens = min_tokens
-        self.rows_per_unit = max(1, (256 if kind == "grouped" else 128) // (heads // kv_heads))
+        self.rows_per_unit = max(1, 128 // (heads // kv_heads))
+        self.together = 2 if kind == "grouped" else 1            # units that a block (latent, wide: two blocks) has at a time
         self.grid = SMS // 2 if kind == "latent" and vdim > 256 else SMS               # two CTAs to a unit
-        self.extra = 3 * -(-self.grid // kv_heads)               # items beyond one for every piece of a prefix and every request
+        self.extra = 3 * -(-self.grid * self.together // kv_heads)      # items beyond one for every piece of a prefix and every request
         self.max_items = self.extra + 2 * rows
-        self.max_units = ceil_to(self.max_items * kv_heads, self.grid)
+        self.max_units = ceil_to(self.max_items * kv_heads, self.grid * self.together)
         self.max_cells = self.extra * min(self.rows_per_unit, rows) + 2 * rows
         z = lambda n, d: torch.zeros(max(n, 4), dtype=d, device=self.device)
         # [count, 3 unused | units | order | cell | parts]
@@ -180,7 +181,7 @@ class PrefixPlan:
         n = 0
         if work:
             unit, part_bytes = max(128, self.page_tokens), 8 * self.heads * self.vdim
-            span = key_span(work, max(1, self.grid // self.kv_heads), part_bytes, sum(w[0] for w in work) + self.extra, unit,
+            span = key_span(work, max(1, self.grid * self.together // self.kv_heads), part_bytes, sum(w[0] for w in work) + self.extra, unit,
                             COSTS[self.kind])
             items, at = [], 0
             for p, (rows, tokens) in zip(pieces, self.shared):
@@ -204,21 +205,27 @@ class PrefixPlan:
         self.data.copy_(torch.from_numpy(host))
 
     def _deal(self, items: np.ndarray, units: np.ndarray, ends: Dict[int, int]) -> int:
-        """Items and key/value heads as units, the longest first, dealt to the blocks there and back: block b takes the units b, b + grid,
-        b + 2 grid ...  Returns how many places were dealt (a place may stay empty)."""
+        """Items and key/value heads as units, those that a block has at a time side by side (pieces that walk the same keys if there are
+        two), the longest first, dealt to the blocks there and back: block b takes the units b, b + grid, b + 2 grid ...  Returns how
+        many places were dealt (a place may stay empty)."""
         keys = items[:, 4] - items[:, 3]
         for i in np.flatnonzero(items[:, 6]):
             keys[i] = min(keys[i], max(1, ends[int(items[i, 1])] - items[i, 3]))
-        ranked = items[np.argsort(-keys, kind="stable")]
-        every = np.repeat(ranked, self.kv_heads, 0)
-        heads = np.tile(np.arange(self.kv_heads, dtype=np.int32), len(items))
+        ranked = items[np.lexsort((items[:, 1], items[:, 3], items[:, 0], -keys))]
+        # by head, then by item: pieces of one range stand side by side
+        every = np.concatenate([np.tile(ranked, (self.kv_heads, 1)), np.repeat(np.arange(self.kv_heads, dtype=np.int32), len(items))[:, None]], 1)
+        length = np.tile(np.sort(keys)[::-1], self.kv_heads)
+        w = self.together
+        if len(every) % w:
+            every, length = np.concatenate([every, np.zeros((1, UNIT), dtype=np.int32)]), np.append(length, 0)
+        every, length = every.reshape(-1, w, UNIT), length.reshape(-1, w).max(1)
+        every = every[np.argsort(-length, kind="stable")]
         i = np.arange(len(every))
         turn, place = i // self.grid, i % self.grid
         place = np.where(turn % 2 == 1, self.grid - 1 - place, place)
         n = ceil_to(len(every), self.grid) if len(every) > self.grid else len(every)
-        table = units.reshape(-1, UNIT)
-        table[turn * self.grid + place] = np.concatenate([every, heads[:, None]], 1)
-        return n
+        units.reshape(-1, w, UNIT)[turn * self.grid + place] = every
+        return n * w
 
     def check_status(self, what: str = "attention over a shared prefix"):
         lib.raise_on_status(self.status, what)
