@@ -5,10 +5,10 @@
 // come in twos, and where both of them walk the same keys each copy serves two tiles.  One tile's softmax runs while the tensor core
 // works on the other's products, and nothing but the order of the copies ties the two together.
 //   warps 0-3, 4-7 : softmax of tile 0 / 1 (one thread per query), partial results
-//   warp 8         : TMA producer: what the next units are, for everybody (a ring of four); key and value tiles of 128 positions, page
-//                    by page
+//   warps 8, 12    : TMA producers: key / value tiles of 128 positions, page by page
 //   warp 9         : tcgen05.mma issue, in whichever order their inputs come: S = Q K^T, O += P V with P in TMEM where it replaces its S
 //   warps 10, 11   : queries of tile 0 / 1, and what each of them sees
+//   warp 13        : what the next units are and where their keys lie, for everybody (a ring of four)
 // A CTA walks its units, and every role but the softmax runs ahead into the next ones: a request's own keys are a few tiles, which the
 // chain of loads that a unit begins with (its description, its rows' positions, their pages, their queries) would take as long as.
 // The running maximum is raised when it grew by more than 2^8 only; what leaves is (m, l, unnormalised O) in 32 bits.  P is rounded
@@ -21,7 +21,7 @@
 
 namespace ds41 {
 
-constexpr int kPgThreads = 384;
+constexpr int kPgThreads = 448;
 constexpr int kPgTile = 128;                   // queries per tile, keys per tile
 constexpr int kPgChunk = kPgTile * 128;        // bytes of 128 rows x 64 bf16 columns
 constexpr int kPgInfos = 4;
@@ -41,8 +41,8 @@ struct PrefixGroupParams {
 struct __align__(16) GroupWork {
   PrefixUnit unit[2];
   int first[2], end[2], tiles[2], base, both;              // base: number of the first key tile in the order of the copies
+  int row[2][32];                                          // pool rows of the first 32 boxes of their keys
 };
-static_assert(sizeof(GroupWork) == 96, "whole 16-byte pieces");
 
 // Number of key tile j of tile t in the order of the copies: one after the other, or in turn as long as both have some.
 __device__ __forceinline__ int copy_index(const GroupWork& w, int t, int j) {
@@ -59,6 +59,7 @@ struct GroupShared {                           // behind the tiles
   uint64_t s_full[2];                          // S complete (and every earlier MMA of the issuing thread)
   uint64_t p_full[2];                          // P written, O rescaled
   uint64_t o_full[2];                          // the unit's last product
+  uint64_t v_here[2];                          // the values of a tail's last tile, for the softmax
   uint32_t tmem, pad[3];
   GroupWork info[kPgInfos];
   int4 query[2][kPgTile];                      // of a packed query: pass row (-1: none), visible keys [y, z)
@@ -79,7 +80,7 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
   if (threadIdx.x == 0) {
     for (int i = 0; i < kPgInfos; ++i) {
       mbar_init(&sh.info_full[i], 1);
-      mbar_init(&sh.info_empty[i], 12);                  // eight softmax warps, two of queries, the products of either tile
+      mbar_init(&sh.info_empty[i], 14);                  // eight softmax warps, two of queries, two of copies, the products of either tile
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.q_full[i], 1);
@@ -91,6 +92,7 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
       mbar_init(&sh.s_full[i], 1);
       mbar_init(&sh.p_full[i], 4);
       mbar_init(&sh.o_full[i], 1);
+      mbar_init(&sh.v_here[i], 1);
     }
     mbar_init_fence();
     tma_prefetch_desc(&pool);
@@ -103,109 +105,115 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
+  // The plan was copied to the device, not computed there by a kernel: it may be read before the wait.  Places behind the last unit
+  // are empty units.
+  const PrefixUnit first_a = prefix_unit(plan, min(2 * static_cast<int>(blockIdx.x), plan.max_units - 2));
+  const PrefixUnit first_b = prefix_unit(plan, min(2 * static_cast<int>(blockIdx.x) + 1, plan.max_units - 1));
+  const int n_units = *plan.n_units;
   pdl_wait();
 
   // this CTA's twos of units: number i is blockIdx.x + i * gridDim.x
-  const int twos = (*plan.n_units + 1) / 2, turns = (twos - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+  const int twos = (n_units + 1) / 2, turns = (twos - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
   bool ok = true;
 
-  if (warp == 8) {
-    const int boxes = kPgTile / p.box;
-    int kt = 0, k_stage = 0, v_stage = 0;                // key tiles so far, places in the rings
-    uint32_t k_free = 1, v_free = 1;
-    // lane i: pool row of box i of the 32 boxes from box u of a walk on
-    auto locate = [&](const GroupWork& w, int t, int u) {
-      const int key = w.first[t] + (u + lane) * p.box, pg = key / p.page_tokens;
-      const int id = key < w.end[t] && pg < p.max_pages ? p.page_table[1ll * w.unit[t].slot * p.max_pages + pg] : -1;
-      return id >= 0 ? id * p.page_tokens + (key - pg * p.page_tokens) : p.hidden_row;
-    };
-    GroupWork next = {};
-    int next_row[2] = {0, 0};
-    auto prepare = [&](int turn) {                       // behind the copies of the units before
-      if (turn >= turns) return;
+  // lane i: pool row of box i of the 32 boxes from box u of a walk on
+  auto locate = [&](int slot, int first, int end, int u) {
+    const int key = first + (u + lane) * p.box, pg = key / p.page_tokens;
+    const int id = key < end && pg < p.max_pages ? p.page_table[1ll * slot * p.max_pages + pg] : -1;
+    return id >= 0 ? id * p.page_tokens + (key - pg * p.page_tokens) : p.hidden_row;
+  };
+
+  if (warp == 13) {
+    int base = 0;
+    for (int turn = 0; turn < turns; ++turn) {
       const int at = 2 * (static_cast<int>(blockIdx.x) + turn * static_cast<int>(gridDim.x));
-#pragma unroll
-      for (int t = 0; t < 2; ++t) next.unit[t] = prefix_unit(plan, at + t);
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-        prefix_span(plan, next.unit[t], p.row_pos, p.row_slot, p.chunk, p.page_tokens, next.first[t], next.end[t]);
-      const PrefixUnit &a = next.unit[0], &b = next.unit[1];
-      next.both = b.rows > 0 && !a.tail && !b.tail && a.slot == b.slot && a.key0 == b.key0 && a.key1 == b.key1 && a.head == b.head;
-      if (next.both && next.first[0] < next.end[0] && next.first[1] < next.end[1]) {
-        next.first[0] = next.first[1] = min(next.first[0], next.first[1]);
-        next.end[0] = next.end[1] = max(next.end[0], next.end[1]);
-      } else {
-        next.both = 0;                                   // one of them sees nothing
+      const PrefixUnit a = turn == 0 ? first_a : prefix_unit(plan, at), b = turn == 0 ? first_b : prefix_unit(plan, at + 1);
+      // without chunks a walk begins at its first key: its pages are looked up together with its rows' positions
+      int row_a = locate(a.slot, a.key0, a.key1, 0), row_b = locate(b.slot, b.key0, b.key1, 0);
+      int first[2], end[2];
+      prefix_span(plan, a, p.row_pos, p.row_slot, p.chunk, p.page_tokens, first[0], end[0]);
+      prefix_span(plan, b, p.row_pos, p.row_slot, p.chunk, p.page_tokens, first[1], end[1]);
+      const bool seen[2] = {first[0] < end[0], first[1] < end[1]};
+      const bool both = b.rows > 0 && !a.tail && !b.tail && a.slot == b.slot && a.key0 == b.key0 && a.key1 == b.key1 &&
+                        a.head == b.head && seen[0] && seen[1];
+      if (both) {
+        first[0] = first[1] = min(first[0], first[1]);
+        end[0] = end[1] = max(end[0], end[1]);
       }
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        next.tiles[t] = (next.end[t] - next.first[t] + kPgTile - 1) / kPgTile;
-        if (!(t == 1 && next.both)) next_row[t] = locate(next, t, 0);
-      }
-    };
-    prepare(0);
-    for (int turn = 0; turn < turns && ok; ++turn) {
-      GroupWork w = next;
-      int row[2] = {next_row[0], next_row[1]};
-      w.base = kt;
+      if (first[0] != a.key0) row_a = locate(a.slot, first[0], end[0], 0);
+      if (first[1] != b.key0) row_b = locate(b.slot, first[1], end[1], 0);
+      if (first[0] + lane * p.box >= end[0]) row_a = p.hidden_row;
+      if (first[1] + lane * p.box >= end[1]) row_b = p.hidden_row;
       ok = __all_sync(0xffffffffu, mbar_wait(&sh.info_empty[turn % kPgInfos], ((turn / kPgInfos) & 1) ^ 1, p.status, 459)) != 0;
       if (!ok) break;
-      if (lane == 0) {
-        sh.info[turn % kPgInfos] = w;
-        mbar_arrive(&sh.info_full[turn % kPgInfos]);
+      GroupWork& w = sh.info[turn % kPgInfos];
+      const int tiles[2] = {(end[0] - first[0] + kPgTile - 1) / kPgTile, (end[1] - first[1] + kPgTile - 1) / kPgTile};
+      w.row[0][lane] = row_a;
+      w.row[1][lane] = row_b;
+      if (lane < 2) {
+        w.unit[lane] = lane ? b : a;
+        w.first[lane] = lane ? first[1] : first[0];
+        w.end[lane] = lane ? end[1] : end[0];
+        w.tiles[lane] = lane ? tiles[1] : tiles[0];
+        w.base = base;
+        w.both = both;
       }
-      const int most = w.both ? w.tiles[0] : max(w.tiles[0], w.tiles[1]);
-      if (most == 0) prepare(turn + 1);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.info_full[turn % kPgInfos]);
+      base += both ? tiles[0] : tiles[0] + tiles[1];
+    }
+  } else if (warp == 8 || warp == 12) {
+    const bool values = warp == 12;
+    const int boxes = kPgTile / p.box, chunks = values ? p.vc : p.kd, stages = values ? p.v_stages : p.k_stages;
+    const int bytes = chunks * kPgChunk;
+    uint64_t *full = values ? sh.v_full : sh.k_full, *empty = values ? sh.v_empty : sh.k_empty;
+    uint8_t* tiles = values ? s_v : s_k;
+    int count = 0, stage = 0;
+    uint32_t free_phase = 1;
+    for (int turn = 0; turn < turns && ok; ++turn) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&sh.info_full[turn % kPgInfos], (turn / kPgInfos) & 1, p.status, 462)) != 0;
+      if (!ok) break;
+      const GroupWork& w = sh.info[turn % kPgInfos];
+      const int n0 = w.tiles[0], n1 = w.both ? 0 : w.tiles[1], most = max(n0, n1);
+      int row0 = w.row[0][lane], row1 = w.row[1][lane];
+      const int x0 = values ? p.kv_heads * p.dp + w.unit[0].head * p.vp : w.unit[0].head * p.dp;
+      const int x1 = values ? p.kv_heads * p.dp + w.unit[1].head * p.vp : w.unit[1].head * p.dp;
       for (int j = 0; j < most && ok; ++j) {
         const int u = j * boxes;
-#pragma unroll 1
-        for (int t = 0; t < (w.both ? 1 : 2); ++t) {
-          if (j >= (t ? w.tiles[1] : w.tiles[0])) continue;
-          if (u > 0 && (u & 31) == 0) {                  // boxes divides 32
-            if (t) row[1] = locate(w, 1, u);
-            else row[0] = locate(w, 0, u);
-          }
-          const int here = t ? row[1] : row[0], g = t ? w.unit[1].head : w.unit[0].head;
-          // one tile of keys or values: `chunks` chunks of 64 columns from column x on
-          auto fetch = [&](uint8_t* dst, uint64_t* bar, int x, int chunks) {
-            if (lane == 0) mbar_expect_tx(bar, chunks * kPgChunk);
-#pragma unroll 1
-            for (int i = 0; i < boxes; ++i) {
-              const int at = __shfl_sync(0xffffffffu, here, (u + i) & 31);
-              if (lane == 0)
-#pragma unroll 1
-                for (int c = 0; c < chunks; ++c) tma_load_3d(dst + c * kPgChunk + i * p.box * 128, &pool, bar, x + 64 * c, at, 0);
-              __syncwarp();
-            }
-          };
-          ok = __all_sync(0xffffffffu, mbar_wait(&sh.k_empty[k_stage], k_free, p.status, 460)) != 0;
-          if (!ok) break;
-          fetch(s_k + k_stage * k_bytes, &sh.k_full[k_stage], g * p.dp, p.kd);
-          if (++k_stage == p.k_stages) {
-            k_stage = 0;
-            k_free ^= 1;
-          }
-          ++kt;
-          ok = __all_sync(0xffffffffu, mbar_wait(&sh.v_empty[v_stage], v_free, p.status, 461)) != 0;
-          if (!ok) break;
-          fetch(s_v + v_stage * v_bytes, &sh.v_full[v_stage], p.kv_heads * p.dp + g * p.vp, p.vc);
-          if (++v_stage == p.v_stages) {
-            v_stage = 0;
-            v_free ^= 1;
-          }
+        if (u > 0 && (u & 31) == 0) {                    // boxes divides 32
+          row0 = locate(w.unit[0].slot, w.first[0], w.end[0], u);
+          row1 = locate(w.unit[1].slot, w.first[1], w.end[1], u);
         }
-        if (j == 0 && ok) prepare(turn + 1);
-      }
-    }
-    if (!ok && lane == 0) {
-      // something else gave up: let the copies under way land before the shared memory goes away
-      for (int b = max(0, kt - 2); b < kt; ++b) {
-        for (int i = 0; i < (1 << 18) && !mbar_test_wait(&sh.k_full[b % p.k_stages], (b / p.k_stages) & 1); ++i) {
-        }
-        for (int i = 0; i < (1 << 18) && !mbar_test_wait(&sh.v_full[b % p.v_stages], (b / p.v_stages) & 1); ++i) {
+#pragma unroll 1
+        for (int t = 0; t < 2; ++t) {
+          if (j >= (t ? n1 : n0)) continue;
+          const int row = t ? row1 : row0, x = t ? x1 : x0;
+          ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], free_phase, p.status, values ? 461 : 460)) != 0;
+          if (!ok) break;
+          uint8_t* dst = tiles + stage * bytes;
+          if (lane == 0) mbar_expect_tx(&full[stage], bytes);
+#pragma unroll 1
+          for (int i = 0; i < boxes; ++i, dst += p.box * 128) {
+            const int at = __shfl_sync(0xffffffffu, row, (u + i) & 31);
+            if (lane == 0)
+#pragma unroll 1
+              for (int c = 0; c < chunks; ++c) tma_load_3d(dst + c * kPgChunk, &pool, &full[stage], x + 64 * c, at, 0);
+            __syncwarp();
+          }
+          ++count;
+          if (++stage == stages) {
+            stage = 0;
+            free_phase ^= 1;
+          }
         }
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.info_empty[turn % kPgInfos]);
     }
+    if (!ok && lane == 0)                                // something gave up: let the copies under way land before the memory goes away
+      for (int b = max(0, count - stages); b < count; ++b)
+        for (int i = 0; i < (1 << 18) && !mbar_test_wait(&full[b % stages], (b / stages) & 1); ++i) {
+        }
   } else if (warp == 9) {
     // one thread: votes and the like between two products cost as much as the products
     if (elect_one()) {
@@ -217,6 +225,20 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
       // per tile: the turn it is at, its key tiles (0: not begun), the next scores and values of that turn, and counts of units and
       // products for the barriers' phases.  Scores overwrite the P that the values before them read.
       int turn[2] = {0, 0}, n[2] = {0, 0}, sj[2] = {0, 0}, pj[2] = {0, 0}, begun[2] = {0, 0}, done[2] = {0, 0};
+      bool told[2] = {false, false};
+      // A tile's place in its ring has been filled at most as often as its last tenants were used: one tile may ask for copies far ahead
+      // of the other's, whose barrier would still show a phase of the same parity.
+      int k_used[2] = {-p.k_stages, 1 - p.k_stages}, v_used[2] = {-p.v_stages, 1 - p.v_stages};
+      auto key_here = [&](int at) {
+        const int stage = p.k_stages == 2 ? at & 1 : 0;
+        return (stage ? k_used[1] : k_used[0]) == at - p.k_stages &&
+               mbar_test_wait(&sh.k_full[stage], p.k_stages == 2 ? (at >> 1) & 1 : at & 1);
+      };
+      auto value_here = [&](int at) {
+        const int stage = p.v_stages == 2 ? at & 1 : 0;
+        return (stage ? v_used[1] : v_used[0]) == at - p.v_stages &&
+               mbar_test_wait(&sh.v_full[stage], p.v_stages == 2 ? (at >> 1) & 1 : at & 1);
+      };
       uint32_t idle = 0;
       long long since = 0;
       while (ok && (turn[0] < turns || turn[1] < turns)) {
@@ -230,7 +252,6 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
             if (!mbar_test_wait(&sh.info_full[turn[t] % kPgInfos], (turn[t] / kPgInfos) & 1)) continue;
             moved = true;
             n[t] = w.tiles[t];
-            sj[t] = pj[t] = 0;
             if (n[t] == 0) {
               mbar_arrive(read);
               ++turn[t];
@@ -240,29 +261,38 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
           const bool both = w.both != 0;
           const int o = t ^ 1;
           if (pj[t] < sj[t]) {
-            const int at = copy_index(w, t, pj[t]), stage = p.v_stages == 2 ? at & 1 : 0, phase = p.v_stages == 2 ? (at >> 1) & 1 : at & 1;
-            if (mbar_test_wait(&sh.p_full[t], done[t] & 1) && mbar_test_wait(&sh.v_full[stage], phase)) {
+            const int at = copy_index(w, t, pj[t]), stage = p.v_stages == 2 ? at & 1 : 0;
+            if (!told[t] && pj[t] + 1 == n[t] && w.unit[t].tail && value_here(at)) {
+              mbar_arrive(&sh.v_here[t]);
+              told[t] = moved = true;
+            }
+            if (mbar_test_wait(&sh.p_full[t], done[t] & 1) && value_here(at)) {
               tc_fence_after();
               const uint64_t vd = v_desc + static_cast<uint64_t>(stage * v_bytes / 16);
               const uint32_t to = tmem + 256 + t * 128, a = tmem + t * 128;
               umma4_ts<128>(to, a, vd, idesc_pv, pj[t] > 0);
               umma4_ts<128>(to, a + 32, vd + 512, idesc_pv, 1u);
               ++done[t];
-              if (!both || turn[o] > turn[t] || (turn[o] == turn[t] && pj[o] > pj[t])) tc_commit_if(true, &sh.v_empty[stage]);      // its last reader
+              if (!both || turn[o] > turn[t] || (turn[o] == turn[t] && pj[o] > pj[t])) {      // its last reader
+                tc_commit_if(true, &sh.v_empty[stage]);
+                if (stage) v_used[1] = at;
+                else v_used[0] = at;
+              }
               ++pj[t];
               moved = true;
               if (pj[t] == n[t]) {
                 tc_commit_if(true, &sh.o_full[t]);
                 mbar_arrive(read);
                 ++turn[t];
-                n[t] = 0;
+                n[t] = sj[t] = pj[t] = 0;                // the other tile compares itself with these
+                told[t] = false;
                 continue;
               }
             }
           }
           if (sj[t] < n[t] && sj[t] == pj[t]) {
-            const int at = copy_index(w, t, sj[t]), stage = p.k_stages == 2 ? at & 1 : 0, phase = p.k_stages == 2 ? (at >> 1) & 1 : at & 1;
-            if (mbar_test_wait(&sh.k_full[stage], phase) && (sj[t] > 0 || mbar_test_wait(&sh.q_full[t], begun[t] & 1))) {
+            const int at = copy_index(w, t, sj[t]), stage = p.k_stages == 2 ? at & 1 : 0;
+            if (key_here(at) && (sj[t] > 0 || mbar_test_wait(&sh.q_full[t], begun[t] & 1))) {
               tc_fence_after();
               uint64_t a = q_desc + static_cast<uint64_t>(t * q_bytes / 16), b = k_desc + static_cast<uint64_t>(stage * k_bytes / 16);
 #pragma unroll 1
@@ -270,7 +300,11 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
 #pragma unroll 1
               for (int k = 0; k < rest; ++k) umma_bf16(tmem + t * 128, a + 2 * k, b + 2 * k, idesc_s, whole > 0 || k > 0);
               tc_commit_if(true, &sh.s_full[t]);
-              if (!both || turn[o] > turn[t] || (turn[o] == turn[t] && sj[o] > sj[t])) tc_commit_if(true, &sh.k_empty[stage]);
+              if (!both || turn[o] > turn[t] || (turn[o] == turn[t] && sj[o] > sj[t])) {
+                tc_commit_if(true, &sh.k_empty[stage]);
+                if (stage) k_used[1] = at;
+                else k_used[0] = at;
+              }
               if (sj[t] == 0) ++begun[t];
               ++sj[t];
               if (sj[t] == n[t]) tc_commit_if(true, &sh.q_empty[t]);
@@ -326,18 +360,16 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
         ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_empty[t], (filled & 1) ^ 1, p.status, 463)) != 0;
         if (!ok) break;
         ++filled;
+        int4 me[4];                                      // what a query sees: asked for now, looked at behind the queries
 #pragma unroll
-        for (int x = lane; x < kPgTile; x += 32) {       // what a query sees
-          int4 v = make_int4(-1, 0, 0, 0);
+        for (int k = 0; k < 4; ++k) {
+          const int x = lane + 32 * k;
+          me[k] = make_int4(-1, 0, 0, 0);
           if (x < here) {
-            v.x = prefix_row(plan, unit, x / p.n);
-            const int pos = p.row_pos[v.x];
-            if (p.row_slot[v.x] >= 0) {
-              v.y = chunk_start(pos, p.chunk);
-              v.z = min(pos + 1, unit.key1);
-            }
+            me[k].x = prefix_row(plan, unit, x / p.n);
+            me[k].y = p.row_pos[me[k].x];
+            me[k].z = p.row_slot[me[k].x];
           }
-          sh.query[t][x] = v;
         }
         // a row's 16-byte pieces by neighbouring lanes, eight rows of a lane under way together; rows without a query stay as they are
         for (int x0 = sub; x0 < here; x0 += 8 * per) {
@@ -356,6 +388,12 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
               *reinterpret_cast<uint4*>(s_q + t * q_bytes + (c >> 3) * kPgChunk + x * 128 + (((c & 7) ^ (x & 7)) << 4)) = v[k];
           }
         }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const bool live = me[k].x >= 0 && me[k].z >= 0;
+          const int pos = me[k].y;
+          sh.query[t][lane + 32 * k] = make_int4(me[k].x, live ? chunk_start(pos, p.chunk) : 0, live ? min(pos + 1, unit.key1) : 0, 0);
+        }
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.q_full[t]);
@@ -364,7 +402,7 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
       const int t = warp >> 2, quad = warp & 3, mine = quad * 32 + lane;
       const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
       const uint32_t s_t = tmem + lanes + t * 128, o_t = tmem + lanes + 256 + t * 128;
-      int tiles = 0, done = 0;                           // tiles of S, units with keys so far
+      int tiles = 0, done = 0, tails = 0;                // tiles of S, units with keys, tails among them so far
       for (int turn = 0; turn < turns; ++turn) {
         const int n = work(turn, t, unit, first, end, last);
         if (!ok) break;
@@ -401,25 +439,29 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
             tc_fence_after();
             const bool edge = key0 < low || key0 + kPgTile > high;
             const int shown = hi - key0, hidden = lo - key0;             // columns [hidden, shown) of this tile are visible
-            // Two halves of 64 columns, each read twice: the loops' bodies have to stay in the instruction cache, which this code shares
-            // with the other roles' (unrolled over the tile, 42 % of all cycles were waits for instructions)
-            float top = -INFINITY;
-            uint32_t v[64];
-            auto load = [&](int c) {
-              tmem_ld_32x32(s_t + c, reinterpret_cast<uint32_t(&)[32]>(v[0]));
-              tmem_ld_32x32(s_t + c + 32, reinterpret_cast<uint32_t(&)[32]>(v[32]));
-              tmem_wait_ld();
-              if (edge) {
-#pragma unroll
-                for (int i = 0; i < 64; ++i) v[i] = c + i < shown && c + i >= hidden ? v[i] : 0xff800000u;
-              }
-            };
+            // Pieces of 32 columns, read twice.  The bodies of these loops are short on purpose: with the tile unrolled, 42 % of all cycles
+            // were waits for instructions, and a small call, which runs all code for the first time, took 6400 cycles for its one tile.
+            if (edge) {
 #pragma unroll 1
-            for (int c = 0; c < kPgTile; c += 64) {
-              load(c);
+              for (int c = 0; c < kPgTile; c += 32) {
+                uint32_t v[32];
+                tmem_ld_32x32(s_t + c, v);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = i < shown - c && i >= hidden - c ? v[i] : 0xff800000u;
+                tmem_st_32x32(s_t + c, v);
+              }
+              tmem_wait_st();
+            }
+            float top = -INFINITY;
+#pragma unroll 1
+            for (int c = 0; c < kPgTile; c += 32) {
+              uint32_t v[32];
+              tmem_ld_32x32(s_t + c, v);
+              tmem_wait_ld();
               float tops[4] = {top, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-              for (int i = 0; i < 64; i += 2)
+              for (int i = 0; i < 32; i += 2)
                 tops[(i >> 1) & 3] = fmaxf(tops[(i >> 1) & 3], fmaxf(__uint_as_float(v[i]), __uint_as_float(v[i + 1])));
               top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
             }
@@ -447,28 +489,30 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
             const float2 by = make_float2(p.scale_log2, p.scale_log2), off = make_float2(neg, neg);
             float2 sums[2] = {};
 #pragma unroll 1
-            for (int c = 0; c < kPgTile; c += 64) {
-              load(c);
-              uint32_t e2[32];
+            for (int c = 0; c < kPgTile; c += 32) {
+              uint32_t v[32], e2[16];
+              tmem_ld_32x32(s_t + c, v);
+              tmem_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) {
+              for (int i = 0; i < 16; ++i) {
                 float2 e = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), by, off);
                 e = make_float2(ex2_approx(e.x), ex2_approx(e.y));
                 sums[i & 1] = add2(sums[i & 1], e);
                 const __nv_bfloat162 b = __floats2bfloat162_rn(e.x, e.y);
                 e2[i] = *reinterpret_cast<const uint32_t*>(&b);
               }
-              tmem_st_32x32(s_t + c / 2, e2);            // columns whose S this thread has read
+              tmem_st_32x16(s_t + c / 2, e2);            // columns whose S this thread has read
             }
             sums[0] = add2(sums[0], sums[1]);
             l += sums[0].x + sums[0].y;
           }
-          if (unit.tail && key0 + kPgTile > end) {
+          if (unit.tail && j + 1 == n) {
             // Places behind the last position belong to nobody, and a weight of zero does not take a NaN or an infinity away: their
-            // values become zeros, a thread to a place.  It is the last tile.
-            const int stage = p.v_stages == 2 ? last & 1 : 0, phase = p.v_stages == 2 ? (last >> 1) & 1 : last & 1;
-            ok = __all_sync(0xffffffffu, mbar_wait(&sh.v_full[stage], phase, p.status, 484 + t)) != 0;
+            // values become zeros, a thread to a place.
+            const int stage = p.v_stages == 2 ? last & 1 : 0;
+            ok = __all_sync(0xffffffffu, mbar_wait(&sh.v_here[t], tails & 1, p.status, 484 + t)) != 0;
             if (!ok) break;
+            ++tails;
             if (key0 + mine >= end)
               for (int i = 0; i < 8 * p.vc; ++i)
                 *reinterpret_cast<uint4*>(s_v + stage * v_bytes + (i >> 3) * kPgChunk + mine * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
