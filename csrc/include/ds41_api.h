@@ -556,7 +556,8 @@ int ds41_latent_merge(const float* part_o, const float* part_ml, const float* si
 // read once for all rows that share them.  Device arrays of the plan, made on the host:
 typedef struct ds41_prefix_plan {
   const int* units;               // [max_units][8]: {slot, first row, rows (0: none), first key, end key, part, tail, key/value head}
-  const int* n_units;             // how many there are
+  const int* n_units;             // how many places the list has
+  const int* turns;               // [grid] how many times a block comes to the list (a grid's width of places further on each time)
   const int* order;               // pass rows by prefix: a unit's rows are order[first] .. order[first + rows - 1]; a tail's: first + i
   const int* cell;                // [rows] the row's first cell of part_o / part_ml
   const int* parts;               // [rows] how many it has

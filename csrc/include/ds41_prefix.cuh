@@ -25,26 +25,34 @@ __device__ __forceinline__ PrefixUnit prefix_unit(const ds41_prefix_plan& p, int
 __device__ __forceinline__ int prefix_row(const ds41_prefix_plan& p, const PrefixUnit& u, int i) {
   return u.tail ? u.first + i : p.order[u.first + i];
 }
-// Whole warps: the keys [first, end) that a unit's rows see.  A chunk's border may lie inside; `first` is a page's.
-__device__ __forceinline__ void prefix_span(const ds41_prefix_plan& p, const PrefixUnit& u, const int* row_pos, const int* row_slot,
-                                            int chunk, int page_tokens, int& first, int& end) {
-  first = u.key0;
-  end = u.key1;
-  if (chunk == 0 && !u.tail) return;
-  int low = u.key1, high = 0;
+// Whole warps: the keys [first, end) that a unit's rows see.  A chunk's border may lie inside; `first` is a page's.  In two steps, so
+// that the positions of several units can be under way together.
+struct PrefixRows {
+  int low, high;                       // of this lane's rows
+};
+__device__ __forceinline__ PrefixRows prefix_rows(const ds41_prefix_plan& p, const PrefixUnit& u, const int* row_pos, const int* row_slot,
+                                                  int chunk) {
+  PrefixRows v = {u.key1, 0};
+  if (chunk == 0 && !u.tail) return v;
   for (int i = threadIdx.x & 31; i < u.rows; i += 32) {
     const int r = prefix_row(p, u, i), pos = row_pos[r];
     if (row_slot[r] < 0) continue;
-    low = min(low, chunk > 0 ? pos - pos % chunk : 0);
-    high = max(high, pos + 1);
+    v.low = min(v.low, chunk > 0 ? pos - pos % chunk : 0);
+    v.high = max(v.high, pos + 1);
   }
+  return v;
+}
+__device__ __forceinline__ void prefix_span(const PrefixUnit& u, PrefixRows v, int chunk, int page_tokens, int& first, int& end) {
+  first = u.key0;
+  end = u.key1;
+  if (chunk == 0 && !u.tail) return;
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
-    low = min(low, __shfl_xor_sync(0xffffffffu, low, o));
-    high = max(high, __shfl_xor_sync(0xffffffffu, high, o));
+    v.low = min(v.low, __shfl_xor_sync(0xffffffffu, v.low, o));
+    v.high = max(v.high, __shfl_xor_sync(0xffffffffu, v.high, o));
   }
-  first = max(first, low - low % page_tokens);
-  end = max(first, min(end, high));
+  first = max(first, v.low - v.low % page_tokens);
+  end = max(first, min(end, v.high));
 }
 
 // Two 32-bit operations in one instruction.
@@ -102,7 +110,7 @@ __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
 }
 
 inline bool prefix_plan_ok(const ds41_prefix_plan* p) {
-  return p != nullptr && p->units != nullptr && p->n_units != nullptr && p->order != nullptr && p->cell != nullptr &&
+  return p != nullptr && p->units != nullptr && p->n_units != nullptr && p->turns != nullptr && p->order != nullptr && p->cell != nullptr &&
          p->parts != nullptr && p->part_o != nullptr && p->part_ml != nullptr && p->max_units > 0 && p->rows_per_unit > 0 &&
          p->grid > 0 && !(reinterpret_cast<uintptr_t>(p->units) & 15) && !(reinterpret_cast<uintptr_t>(p->part_o) & 31) &&
          !(reinterpret_cast<uintptr_t>(p->part_ml) & 7);

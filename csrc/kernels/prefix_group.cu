@@ -109,11 +109,9 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
   // are empty units.
   const PrefixUnit first_a = prefix_unit(plan, min(2 * static_cast<int>(blockIdx.x), plan.max_units - 2));
   const PrefixUnit first_b = prefix_unit(plan, min(2 * static_cast<int>(blockIdx.x) + 1, plan.max_units - 1));
-  const int n_units = *plan.n_units;
+  const int turns = plan.turns[blockIdx.x];
   pdl_wait();
 
-  // this CTA's twos of units: number i is blockIdx.x + i * gridDim.x
-  const int twos = (n_units + 1) / 2, turns = (twos - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
   bool ok = true;
 
   // lane i: pool row of box i of the 32 boxes from box u of a walk on
@@ -130,9 +128,10 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
       const PrefixUnit a = turn == 0 ? first_a : prefix_unit(plan, at), b = turn == 0 ? first_b : prefix_unit(plan, at + 1);
       // without chunks a walk begins at its first key: its pages are looked up together with its rows' positions
       int row_a = locate(a.slot, a.key0, a.key1, 0), row_b = locate(b.slot, b.key0, b.key1, 0);
+      const PrefixRows rows_a = prefix_rows(plan, a, p.row_pos, p.row_slot, p.chunk), rows_b = prefix_rows(plan, b, p.row_pos, p.row_slot, p.chunk);
       int first[2], end[2];
-      prefix_span(plan, a, p.row_pos, p.row_slot, p.chunk, p.page_tokens, first[0], end[0]);
-      prefix_span(plan, b, p.row_pos, p.row_slot, p.chunk, p.page_tokens, first[1], end[1]);
+      prefix_span(a, rows_a, p.chunk, p.page_tokens, first[0], end[0]);
+      prefix_span(b, rows_b, p.chunk, p.page_tokens, first[1], end[1]);
       const bool seen[2] = {first[0] < end[0], first[1] < end[1]};
       const bool both = b.rows > 0 && !a.tail && !b.tail && a.slot == b.slot && a.key0 == b.key0 && a.key1 == b.key1 &&
                         a.head == b.head && seen[0] && seen[1];
@@ -350,17 +349,13 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
     int first, end, last;                                // last: the last tile's number
     if (warp >= 10) {
       const int t = warp - 10, pieces = p.dp / 8, per = 32 / pieces, sub = lane / pieces, c = lane % pieces;
+      constexpr int kUnder = 12;                         // rows of a lane whose pieces are under way together
       int filled = 0;
       for (int turn = 0; turn < turns; ++turn) {
-        const int n = work(turn, t, unit, first, end, last);
-        if (!ok) break;
-        work_read(turn);
-        if (n == 0) continue;
+        // asked for before it is known whether the unit has keys
+        unit = turn == 0 ? (t ? first_b : first_a) : prefix_unit(plan, 2 * (static_cast<int>(blockIdx.x) + turn * static_cast<int>(gridDim.x)) + t);
         const int here = unit.rows * p.n;
-        ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_empty[t], (filled & 1) ^ 1, p.status, 463)) != 0;
-        if (!ok) break;
-        ++filled;
-        int4 me[4];                                      // what a query sees: asked for now, looked at behind the queries
+        int4 me[4];                                      // what a query sees
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int x = lane + 32 * k;
@@ -371,18 +366,29 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
             me[k].z = p.row_slot[me[k].x];
           }
         }
-        // a row's 16-byte pieces by neighbouring lanes, eight rows of a lane under way together; rows without a query stay as they are
-        for (int x0 = sub; x0 < here; x0 += 8 * per) {
-          uint4 v[8];
+        uint4 v[kUnder];
+        auto ask = [&](int x0) {                         // a row's 16-byte pieces by neighbouring lanes
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
+          for (int k = 0; k < kUnder; ++k) {
             const int x = x0 + per * k;
             if (sub < per && x < here)
               v[k] = *reinterpret_cast<const uint4*>(p.q + 1ll * prefix_row(plan, unit, x / p.n) * p.ld_q +
                                                      1ll * (unit.head * p.n + x % p.n) * p.dp + 8 * c);
           }
+        };
+        ask(sub);
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh.info_full[turn % kPgInfos], (turn / kPgInfos) & 1, p.status, 464)) != 0;
+        if (!ok) break;
+        const int n = sh.info[turn % kPgInfos].tiles[t];
+        work_read(turn);
+        if (n == 0) continue;
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_empty[t], (filled & 1) ^ 1, p.status, 463)) != 0;
+        if (!ok) break;
+        ++filled;
+        for (int x0 = sub; x0 < here; x0 += kUnder * per) {      // rows without a query stay as they are
+          if (x0 != sub) ask(x0);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
+          for (int k = 0; k < kUnder; ++k) {
             const int x = x0 + per * k;
             if (sub < per && x < here)
               *reinterpret_cast<uint4*>(s_q + t * q_bytes + (c >> 3) * kPgChunk + x * 128 + (((c & 7) ^ (x & 7)) << 4)) = v[k];
@@ -439,7 +445,7 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
             tc_fence_after();
             const bool edge = key0 < low || key0 + kPgTile > high;
             const int shown = hi - key0, hidden = lo - key0;             // columns [hidden, shown) of this tile are visible
-            // Pieces of 32 columns, read twice.  The bodies of these loops are short on purpose: with the tile unrolled, 42 % of all cycles
+            // Two pieces of 64 columns, read twice.  The bodies of these loops are short on purpose: with the tile unrolled, 42 % of all cycles
             // were waits for instructions, and a small call, which runs all code for the first time, took 6400 cycles for its one tile.
             if (edge) {
 #pragma unroll 1
@@ -455,13 +461,14 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
             }
             float top = -INFINITY;
 #pragma unroll 1
-            for (int c = 0; c < kPgTile; c += 32) {
-              uint32_t v[32];
-              tmem_ld_32x32(s_t + c, v);
+            for (int c = 0; c < kPgTile; c += 64) {
+              uint32_t v[64];
+              tmem_ld_32x32(s_t + c, reinterpret_cast<uint32_t(&)[32]>(v[0]));
+              tmem_ld_32x32(s_t + c + 32, reinterpret_cast<uint32_t(&)[32]>(v[32]));
               tmem_wait_ld();
               float tops[4] = {top, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-              for (int i = 0; i < 32; i += 2)
+              for (int i = 0; i < 64; i += 2)
                 tops[(i >> 1) & 3] = fmaxf(tops[(i >> 1) & 3], fmaxf(__uint_as_float(v[i]), __uint_as_float(v[i + 1])));
               top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
             }
@@ -489,19 +496,20 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
             const float2 by = make_float2(p.scale_log2, p.scale_log2), off = make_float2(neg, neg);
             float2 sums[2] = {};
 #pragma unroll 1
-            for (int c = 0; c < kPgTile; c += 32) {
-              uint32_t v[32], e2[16];
-              tmem_ld_32x32(s_t + c, v);
+            for (int c = 0; c < kPgTile; c += 64) {
+              uint32_t v[64], e2[32];
+              tmem_ld_32x32(s_t + c, reinterpret_cast<uint32_t(&)[32]>(v[0]));
+              tmem_ld_32x32(s_t + c + 32, reinterpret_cast<uint32_t(&)[32]>(v[32]));
               tmem_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
+              for (int i = 0; i < 32; ++i) {
                 float2 e = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), by, off);
                 e = make_float2(ex2_approx(e.x), ex2_approx(e.y));
                 sums[i & 1] = add2(sums[i & 1], e);
                 const __nv_bfloat162 b = __floats2bfloat162_rn(e.x, e.y);
                 e2[i] = *reinterpret_cast<const uint32_t*>(&b);
               }
-              tmem_st_32x16(s_t + c / 2, e2);            // columns whose S this thread has read
+              tmem_st_32x32(s_t + c / 2, e2);            // columns whose S this thread has read
             }
             sums[0] = add2(sums[0], sums[1]);
             l += sums[0].x + sums[0].y;

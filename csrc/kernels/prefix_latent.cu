@@ -115,13 +115,14 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
 
-  const int units = *plan.n_units, first_unit = PAIR ? blockIdx.x >> 1 : blockIdx.x, unit_step = PAIR ? gridDim.x >> 1 : gridDim.x;
+  const int first_unit = PAIR ? blockIdx.x >> 1 : blockIdx.x, unit_step = PAIR ? gridDim.x >> 1 : gridDim.x;
+  const int units = first_unit + plan.turns[first_unit] * unit_step;      // one past the last one's place
   const int v0 = p.v_col[rank], v1 = p.v_col[rank + 1], r0 = p.rot_step[rank], r1 = p.rot_step[rank + 1];
   const int v_chunks = (v1 - v0 + 63) / 64, r_chunk0 = r0 >> 2, r_chunks = r1 > r0 ? (r1 + 3) / 4 - r_chunk0 : 0;
 
   auto span = [&](const PrefixUnit& it, int& end) {            // the key tiles of a unit (whole warps)
     int first;
-    prefix_span(plan, it, p.row_pos, p.row_slot, 0, p.page_tokens, first, end);
+    prefix_span(it, prefix_rows(plan, it, p.row_pos, p.row_slot, 0), 0, p.page_tokens, first, end);
     return (end - first + kPlKeys - 1) / kPlKeys;
   };
 
@@ -461,8 +462,7 @@ static int launch_form(const CUtensorMap& pool, const CUtensorMap& chunks, const
   const cudaError_t e = cudaFuncSetAttribute(prefix_latent_kernel<PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   if (!PAIR) return launch_pdl(prefix_latent_kernel<PAIR>, dim3(plan.grid), dim3(kPlThreads), smem, st, pool, chunks, p, plan);
-  const int pairs = plan.grid < sm_count() / 2 ? plan.grid : sm_count() / 2;
-  return launch_pdl_cluster(prefix_latent_kernel<PAIR>, dim3(2 * pairs), dim3(kPlThreads), 2, smem, st, pool, chunks, p, plan);
+  return launch_pdl_cluster(prefix_latent_kernel<PAIR>, dim3(2 * plan.grid), dim3(kPlThreads), 2, smem, st, pool, chunks, p, plan);
 }
 
 // cudaErrorNotSupported: these sizes are for the simple form

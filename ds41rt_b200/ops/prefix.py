@@ -14,6 +14,7 @@ new one.
 from __future__ import annotations
 
 import ctypes as C
+import heapq
 from typing import Dict, List, Optional, Sequence, Tuple
 
 import numpy as np
@@ -29,7 +30,7 @@ UNIT = 8                 # numbers of a unit (ds41_prefix_plan)
 
 
 class PlanArgs(C.Structure):
-    _fields_ = [("units", C.c_void_p), ("n_units", C.c_void_p), ("order", C.c_void_p), ("cell", C.c_void_p), ("parts", C.c_void_p),
+    _fields_ = [("units", C.c_void_p), ("n_units", C.c_void_p), ("turns", C.c_void_p), ("order", C.c_void_p), ("cell", C.c_void_p), ("parts", C.c_void_p),
                 ("part_o", C.c_void_p), ("part_ml", C.c_void_p), ("max_units", C.c_int), ("rows_per_unit", C.c_int), ("grid", C.c_int)]
 
 
@@ -62,13 +63,14 @@ def common_runs(tables: np.ndarray) -> List[Tuple[List[int], int]]:
 
 
 class Cost:
-    """What a plan goes by, in us: of a unit, of a key in it, of a byte of partial results on their way to the join."""
+    """What a plan goes by, in us: of a unit and of one of its keys (a unit alone), of a block's turn and of a key in it, where `apart`
+    says what the keys of two units count that do not walk the same ones, and of a byte of partial results on their way to the join."""
 
-    def __init__(self, unit: float, key: float):
-        self.unit, self.key, self.byte = unit, key, 1 / 4e6
+    def __init__(self, unit: float, key: float, turn: float, walk: float, apart: float):
+        self.unit, self.key, self.turn, self.walk, self.apart, self.byte = unit, key, turn, walk, apart, 1 / 4e6
 
 
-COSTS = {"grouped": Cost(5.0, 0.02), "latent": Cost(4.0, 0.02)}
+COSTS = {"grouped": Cost(5.0, 0.02, 4.0, 0.015, 0.75), "latent": Cost(4.0, 0.02, 4.0, 0.02, 1.0)}
 
 
 def key_span(work: Sequence[Tuple[int, int, int]], width: int, part_bytes: int, most: int, unit: int, cost: Cost) -> int:
@@ -116,18 +118,19 @@ class PrefixPlan:
         self.grid = SMS // 2 if kind == "latent" and vdim > 256 else SMS               # two CTAs to a unit
         self.extra = 3 * -(-self.grid * self.together // kv_heads)      # items beyond one for every piece of a prefix and every request
         self.max_items = self.extra + 2 * rows
-        self.max_units = ceil_to(self.max_items * kv_heads, self.grid * self.together)
+        self.max_turns = -(-self.max_items * kv_heads // (self.grid * self.together)) + 2
+        self.max_units = self.max_turns * self.grid * self.together
         self.max_cells = self.extra * min(self.rows_per_unit, rows) + 2 * rows
         z = lambda n, d: torch.zeros(max(n, 4), dtype=d, device=self.device)
-        # [count, 3 unused | units | order | cell | parts]
-        self._at = np.cumsum([4, UNIT * self.max_units, rows, rows]).tolist()
+        # [count, 3 unused | units | turns | order | cell | parts]
+        self._at = np.cumsum([4, UNIT * self.max_units, self.grid, rows, rows]).tolist()
         self.data = z(self._at[-1] + rows, I32)
         self.part_o, self.part_ml = z(self.max_cells * heads * vdim, F32), z(self.max_cells * heads * 2, F32)
         self.status = lib.new_status(self.device)
         self.n_units = 0
         self.shared: List[Tuple[List[int], int]] = []      # rows and tokens of every prefix
         a, base = PlanArgs(), self.data.data_ptr()
-        a.n_units, (a.units, a.order, a.cell, a.parts) = base, (base + 4 * x for x in self._at)
+        a.n_units, (a.units, a.turns, a.order, a.cell, a.parts) = base, (base + 4 * x for x in self._at)
         a.part_o, a.part_ml = self.part_o.data_ptr(), self.part_ml.data_ptr()
         a.max_units, a.rows_per_unit, a.grid = self.max_units, self.rows_per_unit, self.grid
         self.args = a
@@ -175,7 +178,7 @@ class PrefixPlan:
 
     def _lay_out(self, slots: np.ndarray, tails, limit: int) -> None:
         host = np.zeros(self.data.numel(), dtype=np.int32)
-        units, order, cell, parts = (host[a:b] for a, b in zip(self._at, self._at[1:] + [len(host)]))
+        units, turns, order, cell, parts = (host[a:b] for a, b in zip(self._at, self._at[1:] + [len(host)]))
         pieces = [-(-len(rows) // self.rows_per_unit) for rows, _ in self.shared]
         work = [(p, len(rows), tokens) for p, (rows, tokens) in zip(pieces, self.shared)] + [(1, n, keys) for _, n, _, keys in tails]
         n = 0
@@ -200,32 +203,36 @@ class PrefixPlan:
                 parts[first:first + rows] += count
             cell[:] = np.cumsum(parts) - parts
             assert len(items) <= self.max_items and int(parts.sum()) <= self.max_cells, (len(items), int(parts.sum()))
-            n = self._deal(np.array(items, dtype=np.int32), units, {x[0]: x[2] + x[3] for x in tails})
+            n = self._deal(np.array(items, dtype=np.int32), units, turns, {x[0]: x[2] + x[3] for x in tails})
         host[0] = self.n_units = n
         self.data.copy_(torch.from_numpy(host))
 
-    def _deal(self, items: np.ndarray, units: np.ndarray, ends: Dict[int, int]) -> int:
+    def _deal(self, items: np.ndarray, units: np.ndarray, turns: np.ndarray, ends: Dict[int, int]) -> int:
         """Items and key/value heads as units, those that a block has at a time side by side (pieces that walk the same keys if there are
-        two), the longest first, dealt to the blocks there and back: block b takes the units b, b + grid, b + 2 grid ...  Returns how
-        many places were dealt (a place may stay empty)."""
+        two), the longest first, each to the block that has least to do: block b takes the places b, b + grid, b + 2 grid ...  Returns
+        how many places there are (one may stay empty)."""
         keys = items[:, 4] - items[:, 3]
         for i in np.flatnonzero(items[:, 6]):
             keys[i] = min(keys[i], max(1, ends[int(items[i, 1])] - items[i, 3]))
-        ranked = items[np.lexsort((items[:, 1], items[:, 3], items[:, 0], -keys))]
+        order = np.lexsort((items[:, 1], items[:, 3], items[:, 0], -keys))
         # by head, then by item: pieces of one range stand side by side
-        every = np.concatenate([np.tile(ranked, (self.kv_heads, 1)), np.repeat(np.arange(self.kv_heads, dtype=np.int32), len(items))[:, None]], 1)
-        length = np.tile(np.sort(keys)[::-1], self.kv_heads)
-        w = self.together
+        every = np.concatenate([np.tile(items[order], (self.kv_heads, 1)), np.repeat(np.arange(self.kv_heads, dtype=np.int32), len(items))[:, None]], 1)
+        length = np.tile(keys[order], self.kv_heads)
+        w, cost = self.together, COSTS[self.kind]
         if len(every) % w:
             every, length = np.concatenate([every, np.zeros((1, UNIT), dtype=np.int32)]), np.append(length, 0)
-        every, length = every.reshape(-1, w, UNIT), length.reshape(-1, w).max(1)
-        every = every[np.argsort(-length, kind="stable")]
-        i = np.arange(len(every))
-        turn, place = i // self.grid, i % self.grid
-        place = np.where(turn % 2 == 1, self.grid - 1 - place, place)
-        n = ceil_to(len(every), self.grid) if len(every) > self.grid else len(every)
-        units.reshape(-1, w, UNIT)[turn * self.grid + place] = every
-        return n * w
+        every, length = every.reshape(-1, w, UNIT), length.reshape(-1, w)
+        same = (every[:, 0, [0, 3, 4, 7]] == every[:, -1, [0, 3, 4, 7]]).all(1) & (every[:, 0, 6] == 0) & (every[:, -1, 2] > 0)
+        need = cost.turn + cost.walk * np.where(same, length[:, 0], length.sum(1) * cost.apart)
+        blocks = [(0.0, 0, b) for b in range(self.grid)]               # (time so far, turns, block)
+        table = units.reshape(-1, w, UNIT)
+        for i in np.argsort(-need, kind="stable").tolist():
+            time, turn, b = heapq.heappop(blocks)
+            table[turn * self.grid + b] = every[i]
+            turns[b] = turn + 1
+            if turn + 1 < self.max_turns:
+                heapq.heappush(blocks, (time + float(need[i]), turn + 1, b))
+        return int(turns.max()) * self.grid * w
 
     def check_status(self, what: str = "attention over a shared prefix"):
         lib.raise_on_status(self.status, what)

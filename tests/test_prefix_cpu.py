@@ -92,8 +92,10 @@ def test_units_cover_every_position_of_every_row_once(seed):
     plan = PrefixPlan(kind, rows=rows, heads=heads, kv_heads=kv, vdim=vdim, page_tokens=P, device="cpu")
     plan.set(row_slots, torch.from_numpy(t), lengths)
     d = plan.data.numpy()
-    units, order, cell, count = (d[a:b] for a, b in zip(plan._at, plan._at[1:] + [len(d)]))
+    units, turns, order, cell, count = (d[a:b] for a, b in zip(plan._at, plan._at[1:] + [len(d)]))
     assert d[0] == plan.n_units <= plan.max_units and not units[8 * plan.n_units:].any()
+    listed = units.reshape(plan.max_turns, plan.grid, -1, 8)[..., 2].any(2)
+    assert (listed == (np.arange(plan.max_turns)[:, None] < turns[None])).all()          # a block's turns are its first places
     covered, used = {}, set()
     for slot, first, n, k0, k1, part, tail, head in units[:8 * plan.n_units].reshape(-1, 8).tolist():
         if n == 0:                                             # a place that was not dealt
@@ -153,7 +155,7 @@ def test_short_requests_are_not_divided_and_long_ones_are():
     t = table(*[[10 * i + k for k in range(1, 3)] for i in range(4)], list(range(1000, 1700)), width=800)
     plan = PrefixPlan("grouped", rows=5, heads=8, kv_heads=2, vdim=128, page_tokens=64, device="cpu")
     plan.set(range(5), t)
-    at = plan._at[3]
+    at = plan._at[4]
     assert plan.data[at:at + 5].tolist()[:4] == [1, 1, 1, 1] and plan.data[at + 4] > 8
 
 
