@@ -62,7 +62,7 @@ struct GroupShared {                           // behind the tiles
   uint64_t v_here[2];                          // the values of a tail's last tile, for the softmax
   uint32_t tmem, pad[3];
   GroupWork info[kPgInfos];
-  int4 query[2][kPgTile];                      // of a packed query: pass row (-1: none), visible keys [y, z)
+  int4 row[2][kPgTile];                        // of a unit's row: pass row, visible keys [y, z)
 };
 
 __global__ void __launch_bounds__(kPgThreads, 1)
@@ -348,35 +348,21 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
     PrefixUnit unit;
     int first, end, last;                                // last: the last tile's number
     if (warp >= 10) {
-      const int t = warp - 10, pieces = p.dp / 8, per = 32 / pieces, sub = lane / pieces, c = lane % pieces;
-      constexpr int kUnder = 12;                         // rows of a lane whose pieces are under way together
+      // A row's queries lie side by side: pieces of 16 bytes by neighbouring lanes, or whole rows where they are shorter than a warp.
+      const int t = warp - 10, pieces = p.n * p.dp / 8, per = max(1, 32 / pieces), sub = pieces < 32 ? lane / pieces : 0;
+      const int piece0 = pieces < 32 ? lane % pieces : lane;
       int filled = 0;
       for (int turn = 0; turn < turns; ++turn) {
-        // asked for before it is known whether the unit has keys
+        // rows and positions: asked for before it is known whether the unit has keys
         unit = turn == 0 ? (t ? first_b : first_a) : prefix_unit(plan, 2 * (static_cast<int>(blockIdx.x) + turn * static_cast<int>(gridDim.x)) + t);
-        const int here = unit.rows * p.n;
-        int4 me[4];                                      // what a query sees
+        int row[4], pos[4], slot[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int x = lane + 32 * k;
-          me[k] = make_int4(-1, 0, 0, 0);
-          if (x < here) {
-            me[k].x = prefix_row(plan, unit, x / p.n);
-            me[k].y = p.row_pos[me[k].x];
-            me[k].z = p.row_slot[me[k].x];
+        for (int k = 0; k < 4; ++k)
+          if (lane + 32 * k < unit.rows) {
+            row[k] = prefix_row(plan, unit, lane + 32 * k);
+            pos[k] = p.row_pos[row[k]];
+            slot[k] = p.row_slot[row[k]];
           }
-        }
-        uint4 v[kUnder];
-        auto ask = [&](int x0) {                         // a row's 16-byte pieces by neighbouring lanes
-#pragma unroll
-          for (int k = 0; k < kUnder; ++k) {
-            const int x = x0 + per * k;
-            if (sub < per && x < here)
-              v[k] = *reinterpret_cast<const uint4*>(p.q + 1ll * prefix_row(plan, unit, x / p.n) * p.ld_q +
-                                                     1ll * (unit.head * p.n + x % p.n) * p.dp + 8 * c);
-          }
-        };
-        ask(sub);
         ok = __all_sync(0xffffffffu, mbar_wait(&sh.info_full[turn % kPgInfos], (turn / kPgInfos) & 1, p.status, 464)) != 0;
         if (!ok) break;
         const int n = sh.info[turn % kPgInfos].tiles[t];
@@ -385,20 +371,27 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
         ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_empty[t], (filled & 1) ^ 1, p.status, 463)) != 0;
         if (!ok) break;
         ++filled;
-        for (int x0 = sub; x0 < here; x0 += kUnder * per) {      // rows without a query stay as they are
-          if (x0 != sub) ask(x0);
 #pragma unroll
-          for (int k = 0; k < kUnder; ++k) {
-            const int x = x0 + per * k;
-            if (sub < per && x < here)
-              *reinterpret_cast<uint4*>(s_q + t * q_bytes + (c >> 3) * kPgChunk + x * 128 + (((c & 7) ^ (x & 7)) << 4)) = v[k];
+        for (int k = 0; k < 4; ++k)
+          if (lane + 32 * k < unit.rows)
+            sh.row[t][lane + 32 * k] = make_int4(row[k], slot[k] >= 0 ? chunk_start(pos[k], p.chunk) : 0,
+                                                 slot[k] >= 0 ? min(pos[k] + 1, unit.key1) : 0, 0);
+        __syncwarp();
+        for (int piece = piece0; piece < pieces && sub < per; piece += 32) {
+          const int head = piece * 8 / p.dp, c = piece - head * (p.dp / 8);
+          const __nv_bfloat16* src = p.q + unit.head * p.n * p.dp + 8 * piece;
+          uint8_t* dst = s_q + t * q_bytes + (c >> 3) * kPgChunk;
+          for (int i0 = sub; i0 < unit.rows; i0 += 8 * per) {      // eight rows of a lane under way together
+            uint4 v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if (i0 + k * per < unit.rows) v[k] = *reinterpret_cast<const uint4*>(src + sh.row[t][i0 + k * per].x * p.ld_q);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const int x = (i0 + k * per) * p.n + head;
+              if (i0 + k * per < unit.rows) *reinterpret_cast<uint4*>(dst + x * 128 + (((c & 7) ^ (x & 7)) << 4)) = v[k];
+            }
           }
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const bool live = me[k].x >= 0 && me[k].z >= 0;
-          const int pos = me[k].y;
-          sh.query[t][lane + 32 * k] = make_int4(me[k].x, live ? chunk_start(pos, p.chunk) : 0, live ? min(pos + 1, unit.key1) : 0, 0);
         }
         fence_async_smem();
         __syncwarp();
@@ -408,22 +401,22 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
       const int t = warp >> 2, quad = warp & 3, mine = quad * 32 + lane;
       const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
       const uint32_t s_t = tmem + lanes + t * 128, o_t = tmem + lanes + 256 + t * 128;
+      const int mine_row = mine / p.n, mine_head = mine - mine_row * p.n;
       int tiles = 0, done = 0, tails = 0;                // tiles of S, units with keys, tails among them so far
       for (int turn = 0; turn < turns; ++turn) {
         const int n = work(turn, t, unit, first, end, last);
         if (!ok) break;
         work_read(turn);
         if (n == 0) {                                    // nothing for any of its rows
-          if (mine < unit.rows * p.n) {
-            const long long cell = (1ll * plan.cell[prefix_row(plan, unit, mine / p.n)] + unit.part) * p.heads + unit.head * p.n +
-                                   mine % p.n;
+          if (mine_row < unit.rows) {
+            const long long cell = (1ll * plan.cell[prefix_row(plan, unit, mine_row)] + unit.part) * p.heads + unit.head * p.n + mine_head;
             *reinterpret_cast<float2*>(plan.part_ml + 2 * cell) = make_float2(-INFINITY, 0.f);
           }
           continue;
         }
         ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_full[t], done & 1, p.status, 482 + t)) != 0;
         if (!ok) break;
-        const int4 me = sh.query[t][mine];
+        const int4 me = mine_row < unit.rows ? sh.row[t][mine_row] : make_int4(-1, 0, 0, 0);
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.q_empty[t]);
         const int r = me.x, lo = me.y, hi = me.z;
@@ -540,7 +533,7 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
           l = 0.f;
         }
         const bool write = r >= 0;
-        const long long cell = write ? (1ll * plan.cell[r] + unit.part) * p.heads + unit.head * p.n + mine % p.n : 0;
+        const long long cell = write ? (1ll * plan.cell[r] + unit.part) * p.heads + unit.head * p.n + mine_head : 0;
         if (write) *reinterpret_cast<float2*>(plan.part_ml + 2 * cell) = make_float2(m, l);
         if (!idle) {                                     // whole warps: tensor memory is read by all lanes
           float* dst = plan.part_o + cell * p.vp;
