@@ -217,16 +217,17 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const ds41_prefix_plan
   const long long w = 4ll * blockIdx.x + (threadIdx.x >> 5);
   const int r = static_cast<int>(w / (heads * strips)), h = static_cast<int>(w / strips % heads), c = static_cast<int>(w % strips) * 128 + 4 * lane;
   pdl_launch_dependents();
+  // the plan was copied to the device, not computed there: it may be read before the wait
+  const int n = r < rows ? plan.parts[r] : 0;
+  const long long cell = r < rows ? 1ll * plan.cell[r] * heads + h : 0;
   pdl_wait();
   if (r >= rows) return;
+  const float sk = sink != nullptr ? sink[h] * 1.4426950408889634f : -INFINITY;
   if (keep.taps > 1 && keep.row_slot[r] >= 0)
     keep_inputs(keep, r, keep.row_slot[r], keep.row_pos[r], static_cast<int>(w % (heads * strips)), heads * strips, lane, 32);
-  const int n = plan.parts[r];
-  const long long cell = 1ll * plan.cell[r] * heads + h;
   const float2* ml = reinterpret_cast<const float2*>(plan.part_ml) + cell;
   const float* part = plan.part_o + cell * vp + c;
   const long long step = 1ll * heads * vp;
-  const float sk = sink != nullptr ? sink[h] * 1.4426950408889634f : -INFINITY;
   float all = sk;
   for (int s = lane; s < n; s += 32) all = fmaxf(all, ml[1ll * s * heads].x);
   all = warp_max(all);

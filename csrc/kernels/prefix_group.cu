@@ -16,6 +16,7 @@
 #include <cuda.h>
 
 #include "ds41_group.cuh"
+#include "ds41_mma.cuh"
 #include "ds41_prefix.cuh"
 #include "ds41_tma.h"
 
@@ -62,7 +63,7 @@ struct GroupShared {                           // behind the tiles
   uint64_t v_here[2];                          // the values of a tail's last tile, for the softmax
   uint32_t tmem, pad[3];
   GroupWork info[kPgInfos];
-  int4 row[2][kPgTile];                        // of a unit's row: pass row, visible keys [y, z)
+  int4 row[2][kPgTile];                        // of a unit's row: pass row, visible keys [y, z), cell
 };
 
 __global__ void __launch_bounds__(kPgThreads, 1)
@@ -353,46 +354,42 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
       const int piece0 = pieces < 32 ? lane % pieces : lane;
       int filled = 0;
       for (int turn = 0; turn < turns; ++turn) {
-        // rows and positions: asked for before it is known whether the unit has keys
+        // everything is asked for before it is known whether the unit has keys
         unit = turn == 0 ? (t ? first_b : first_a) : prefix_unit(plan, 2 * (static_cast<int>(blockIdx.x) + turn * static_cast<int>(gridDim.x)) + t);
-        int row[4], pos[4], slot[4];
+        int row[4], pos[4], slot[4], cell[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           if (lane + 32 * k < unit.rows) {
             row[k] = prefix_row(plan, unit, lane + 32 * k);
             pos[k] = p.row_pos[row[k]];
             slot[k] = p.row_slot[row[k]];
+            cell[k] = plan.cell[row[k]];
           }
-        ok = __all_sync(0xffffffffu, mbar_wait(&sh.info_full[turn % kPgInfos], (turn / kPgInfos) & 1, p.status, 464)) != 0;
-        if (!ok) break;
-        const int n = sh.info[turn % kPgInfos].tiles[t];
-        work_read(turn);
-        if (n == 0) continue;
         ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_empty[t], (filled & 1) ^ 1, p.status, 463)) != 0;
         if (!ok) break;
-        ++filled;
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           if (lane + 32 * k < unit.rows)
             sh.row[t][lane + 32 * k] = make_int4(row[k], slot[k] >= 0 ? chunk_start(pos[k], p.chunk) : 0,
-                                                 slot[k] >= 0 ? min(pos[k] + 1, unit.key1) : 0, 0);
+                                                 slot[k] >= 0 ? min(pos[k] + 1, unit.key1) : 0, cell[k] + unit.part);
         __syncwarp();
         for (int piece = piece0; piece < pieces && sub < per; piece += 32) {
           const int head = piece * 8 / p.dp, c = piece - head * (p.dp / 8);
           const __nv_bfloat16* src = p.q + unit.head * p.n * p.dp + 8 * piece;
           uint8_t* dst = s_q + t * q_bytes + (c >> 3) * kPgChunk;
-          for (int i0 = sub; i0 < unit.rows; i0 += 8 * per) {      // eight rows of a lane under way together
-            uint4 v[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              if (i0 + k * per < unit.rows) v[k] = *reinterpret_cast<const uint4*>(src + sh.row[t][i0 + k * per].x * p.ld_q);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const int x = (i0 + k * per) * p.n + head;
-              if (i0 + k * per < unit.rows) *reinterpret_cast<uint4*>(dst + x * 128 + (((c & 7) ^ (x & 7)) << 4)) = v[k];
-            }
+#pragma unroll 4
+          for (int i = sub; i < unit.rows; i += per) {
+            const int x = i * p.n + head;
+            cp_async_16(dst + x * 128 + (((c & 7) ^ (x & 7)) << 4), src + sh.row[t][i].x * p.ld_q);
           }
         }
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh.info_full[turn % kPgInfos], (turn / kPgInfos) & 1, p.status, 464)) != 0;
+        cp_async_wait_all();
+        if (!ok) break;
+        const int n = sh.info[turn % kPgInfos].tiles[t];
+        work_read(turn);
+        if (n == 0) continue;
+        ++filled;
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.q_full[t]);
@@ -490,19 +487,23 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
             float2 sums[2] = {};
 #pragma unroll 1
             for (int c = 0; c < kPgTile; c += 64) {
-              uint32_t v[64], e2[32];
+              uint32_t v[64];
               tmem_ld_32x32(s_t + c, reinterpret_cast<uint32_t(&)[32]>(v[0]));
               tmem_ld_32x32(s_t + c + 32, reinterpret_cast<uint32_t(&)[32]>(v[32]));
               tmem_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                float2 e = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), by, off);
-                e = make_float2(ex2_approx(e.x), ex2_approx(e.y));
-                sums[i & 1] = add2(sums[i & 1], e);
-                const __nv_bfloat162 b = __floats2bfloat162_rn(e.x, e.y);
-                e2[i] = *reinterpret_cast<const uint32_t*>(&b);
+              for (int h = 0; h < 2; ++h) {
+                uint32_t e2[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  float2 e = fma2(make_float2(__uint_as_float(v[32 * h + 2 * i]), __uint_as_float(v[32 * h + 2 * i + 1])), by, off);
+                  e = make_float2(ex2_approx(e.x), ex2_approx(e.y));
+                  sums[i & 1] = add2(sums[i & 1], e);
+                  const __nv_bfloat162 b = __floats2bfloat162_rn(e.x, e.y);
+                  e2[i] = *reinterpret_cast<const uint32_t*>(&b);
+                }
+                tmem_st_32x16(s_t + c / 2 + 16 * h, e2);       // columns whose S this thread has read
               }
-              tmem_st_32x32(s_t + c / 2, e2);            // columns whose S this thread has read
             }
             sums[0] = add2(sums[0], sums[1]);
             l += sums[0].x + sums[0].y;
@@ -533,18 +534,19 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
           l = 0.f;
         }
         const bool write = r >= 0;
-        const long long cell = write ? (1ll * plan.cell[r] + unit.part) * p.heads + unit.head * p.n + mine_head : 0;
+        const long long cell = write ? 1ll * me.w * p.heads + unit.head * p.n + mine_head : 0;
         if (write) *reinterpret_cast<float2*>(plan.part_ml + 2 * cell) = make_float2(m, l);
         if (!idle) {                                     // whole warps: tensor memory is read by all lanes
           float* dst = plan.part_o + cell * p.vp;
 #pragma unroll 1
-          for (int c = 0; c < p.vp; c += 16) {
-            uint32_t a[16];
-            tmem_ld_32x16(o_t + c, a);
+          for (int c = 0; c < p.vp; c += 32) {             // a last half piece reads columns that nobody stores
+            uint32_t a[32];
+            tmem_ld_32x32(o_t + c, a);
             tmem_wait_ld();
             if (write) {
-              store8(dst + c, reinterpret_cast<const float(&)[8]>(a[0]));
-              store8(dst + c + 8, reinterpret_cast<const float(&)[8]>(a[8]));
+#pragma unroll
+              for (int i = 0; i < 32; i += 8)
+                if (c + i < p.vp) store8(dst + c + i, reinterpret_cast<const float(&)[8]>(a[i]));
             }
             __syncwarp();
           }
