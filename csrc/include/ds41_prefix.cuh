@@ -102,6 +102,13 @@ __device__ __forceinline__ void umma4_ss(uint32_t d, uint64_t a, uint64_t b, uin
       : "memory");
 }
 
+// Thirty-two bytes, 32-byte aligned.
+__device__ __forceinline__ void load32(const void* p, uint32_t (&v)[8]) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "l"(p)
+               : "memory");
+}
 // Eight neighbouring values, 32-byte aligned: a whole sector of L2 per thread, as neighbouring threads store to rows far apart.
 __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
   asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]),

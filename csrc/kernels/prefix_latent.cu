@@ -39,6 +39,7 @@ struct PrefixLatentParams {
   int v_col[3], rot_step[3];                                // CTA c: latent columns [v_col[c], v_col[c + 1]), rotated steps of 16 likewise
   int max_pages, page_tokens, box, hidden_row;
   int deep;                                                 // a CTA's latent chunks of a box in one copy
+  int wide;                                                 // queries may be read 32 bytes at a time
   float scale_log2;
   int* status;
 };
@@ -113,10 +114,12 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
   if (PAIR) cluster_meet();                                  // the other CTA's barriers are ready, too
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  pdl_wait();
-
+  // The plan was copied to the device, not computed there by a kernel: it may be read before the wait.
   const int first_unit = PAIR ? blockIdx.x >> 1 : blockIdx.x, unit_step = PAIR ? gridDim.x >> 1 : gridDim.x;
   const int units = first_unit + plan.turns[first_unit] * unit_step;      // one past the last one's place
+  const PrefixUnit begin = prefix_unit(plan, first_unit);
+  pdl_wait();
+
   const int v0 = p.v_col[rank], v1 = p.v_col[rank + 1], r0 = p.rot_step[rank], r1 = p.rot_step[rank + 1];
   const int v_chunks = (v1 - v0 + 63) / 64, r_chunk0 = r0 >> 2, r_chunks = r1 > r0 ? (r1 + 3) / 4 - r_chunk0 : 0;
 
@@ -134,7 +137,7 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
     uint32_t free_phase = 1;
     bool ok = true;
     for (int unit = first_unit; unit < units && ok; unit += unit_step) {
-      const PrefixUnit it = prefix_unit(plan, unit);
+      const PrefixUnit it = unit == first_unit ? begin : prefix_unit(plan, unit);
       if (it.rows == 0) continue;
       int end;
       const int n = span(it, end);
@@ -181,7 +184,7 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
     int kt = 0, live = 0, s_stage = 0, p_stage = 0;            // tiles so far; the ring's places of the next scores and values
     uint32_t s_phase = 0;
     for (int unit = first_unit; unit < units && ok; unit += unit_step) {
-      const PrefixUnit it = prefix_unit(plan, unit);
+      const PrefixUnit it = unit == first_unit ? begin : prefix_unit(plan, unit);
       if (it.rows == 0) continue;
       int end;
       const int n = span(it, end);
@@ -249,27 +252,38 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
     const int before = (set + kPlSets - 1) % kPlSets;              // the set of the last tile
     int kt = 0;
     bool ok = true;
-    // the loop runs to its end whatever happened: the warps of a quadrant meet at barriers
-    for (int unit = first_unit; unit < units; unit += unit_step) {
-      const PrefixUnit it = prefix_unit(plan, unit);
-      if (it.rows == 0) continue;
-      int end;
-      const int n = span(it, end);
-      int r = -1, hi = 0, h = 0;
-      if (mine < it.rows * p.heads) {
-        r = prefix_row(plan, it, mine / p.heads);
-        h = mine % p.heads;
+    // What a thread has to know of a unit, found while the last product of the one before it is under way.
+    PrefixUnit it = begin;
+    int n = 0, end = 0, r = -1, hi = 0, cell = 0;
+    const int my_row = mine / p.heads, h = mine - my_row * p.heads;
+    auto look = [&](const PrefixUnit& next) {
+      it = next;
+      const PrefixRows rows = prefix_rows(plan, it, p.row_pos, p.row_slot, 0);
+      r = -1;
+      hi = 0;
+      if (my_row < it.rows) {
+        r = prefix_row(plan, it, my_row);
+        cell = plan.cell[r] + it.part;
         if (p.row_slot[r] >= 0) hi = min(p.row_pos[r] + 1, it.key1);
       }
+      int first;
+      prefix_span(it, rows, 0, p.page_tokens, first, end);
+      n = (end - first + kPlKeys - 1) / kPlKeys;
+    };
+    if (first_unit < units) look(begin);
+    // the loop runs to its end whatever happened: the warps of a quadrant meet at barriers
+    for (int unit = first_unit; unit < units; unit += unit_step) {
+      const PrefixUnit next = unit + unit_step < units ? prefix_unit(plan, unit + unit_step) : it;
       if (n == 0) {                                            // nothing for any of its rows
         if (r >= 0 && set == 0 && rank == 0)
-          *reinterpret_cast<float2*>(plan.part_ml + 2 * ((1ll * plan.cell[r] + it.part) * p.heads + h)) = make_float2(-INFINITY, 0.f);
+          *reinterpret_cast<float2*>(plan.part_ml + 2 * (1ll * cell * p.heads + h)) = make_float2(-INFINITY, 0.f);
+        look(next);
         continue;
       }
       // queries into tensor memory, the sets in turn: all of a thread's loads are under way together
       {
         constexpr int kMine = 2 * kPlMost / kPlSets;             // pieces of 32 values
-        uint4 v[kMine][4];
+        uint32_t v[kMine][16];
 #pragma unroll
         for (int k = 0; k < kMine; ++k) {
           const int c = set + kPlSets * k;
@@ -277,15 +291,34 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
           const int d0 = lat ? v0 + 32 * c : 64 * r_chunk0 + 32 * (c - 2 * v_chunks), width = lat ? v1 : p.rp;
           const __nv_bfloat16* src = lat ? p.q_abs + r * p.ld_q_abs + 1ll * h * p.kvp + d0
                                          : p.q_rot + r * p.ld_q_rot + 1ll * h * p.q_rot_stride + d0;
+          const bool there = r >= 0 && c < 2 * (v_chunks + r_chunks);
+          // neighbouring threads read rows far apart: a sector of 32 bytes each
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            v[k][i] = r >= 0 && c < 2 * (v_chunks + r_chunks) && d0 + 8 * i < width ? *reinterpret_cast<const uint4*>(src + 8 * i)
-                                                                                   : make_uint4(0, 0, 0, 0);
+          for (int i = 0; i < 2; ++i) {
+            uint32_t(&to)[8] = reinterpret_cast<uint32_t(&)[8]>(v[k][8 * i]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) to[e] = 0;
+            if (there && d0 + 16 * i < width) {
+              if (p.wide) {
+                load32(src + 16 * i, to);
+              } else {
+                const uint4 a = *reinterpret_cast<const uint4*>(src + 16 * i), b = *reinterpret_cast<const uint4*>(src + 16 * i + 8);
+                to[0] = a.x;
+                to[1] = a.y;
+                to[2] = a.z;
+                to[3] = a.w;
+                to[4] = b.x;
+                to[5] = b.y;
+                to[6] = b.z;
+                to[7] = b.w;
+              }
+            }
+          }
         }
 #pragma unroll
         for (int k = 0; k < kMine; ++k) {
           const int c = set + kPlSets * k;
-          if (c < 2 * (v_chunks + r_chunks)) tmem_st_32x16(lanes + kPlQ + 16 * c, reinterpret_cast<const uint32_t(&)[16]>(v[k][0]));
+          if (c < 2 * (v_chunks + r_chunks)) tmem_st_32x16(lanes + kPlQ + 16 * c, v[k]);
         }
       }
       tmem_wait_st();
@@ -418,6 +451,9 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
       // the last maximum is there; and the set of the last tile has seen the products up to the one before the last complete, so that the
       // wait that follows cannot take an earlier phase for its own
       named_barrier(1 + quad, 32 * kPlSets);
+      const int key0 = it.key0, this_r = r, this_hi = hi;
+      const long long this_cell = 1ll * cell * p.heads + h;
+      if (unit + unit_step < units) look(next);
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[(kt - 1) % kPlSets], ((kt - 1) / kPlSets) & 1, p.status, 526)) != 0;
       tc_fence_after();
       const float all = s_top[mine];
@@ -428,12 +464,11 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
       for (int i = 1; i < kPlSets; ++i) l += s_sum[i * kPlQueries + mine];
       m = all;
       if (ok) {
-        const bool write = r >= 0, seen = hi > it.key0;
-        const long long cell = write ? (1ll * plan.cell[r] + it.part) * p.heads + h : 0;
+        const bool write = this_r >= 0, seen = this_hi > key0;
         if (write && set == 0 && rank == 0)
-          *reinterpret_cast<float2*>(plan.part_ml + 2 * cell) =
+          *reinterpret_cast<float2*>(plan.part_ml + 2 * this_cell) =
               make_float2(seen ? m : -INFINITY, seen ? l : 0.f);
-        float* dst = plan.part_o + cell * p.kvp + v0;
+        float* dst = plan.part_o + (write ? this_cell : 0) * p.kvp + v0;
         for (int c = 16 * set; c < v1 - v0; c += 16 * kPlSets) {
           uint32_t o[16];
           tmem_ld_32x16(lanes + c, o);
@@ -503,6 +538,8 @@ int launch_prefix_latent(const ds41_latent_attend_args& a, const ds41_prefix_pla
   p.ld_q_abs = a.ld_q_abs; p.ld_q_rot = a.ld_q_rot; p.q_rot_stride = a.q_rot_stride;
   p.heads = a.heads; p.kvp = a.kv_pad; p.rp = rp;
   p.max_pages = a.max_pages; p.page_tokens = a.page_tokens; p.hidden_row = n_pages * a.page_tokens;
+  p.wide = !((a.ld_q_abs | a.ld_q_rot | a.q_rot_stride) & 15) &&
+           !((reinterpret_cast<uintptr_t>(a.q_abs) | reinterpret_cast<uintptr_t>(a.q_rot)) & 31);
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.status = a.status;
   CUtensorMap pool;
