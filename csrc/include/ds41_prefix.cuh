@@ -116,6 +116,34 @@ __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
                : "memory");
 }
 
+// A warp's 32 rows of 32 columns, a thread to a row as tensor memory hands them out, into rows of global memory: the eight threads of a
+// group exchange their rows' pieces of 16 bytes (8 x 8 of them, in three steps), so that a store covers whole lines of 128 bytes.
+// Thread-wise every store is 32 requests: 128 rows of 256 columns took 7500 cycles, 4600 so, of 32 live rows the other way 2000 and
+// 3900.  `at`: this thread's row, < 0: none.
+__device__ __forceinline__ void store_rows(float* base, long long at, uint32_t (&v)[32]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int m = 1; m < 8; m *= 2) {
+    const bool up = (lane & m) != 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if ((j & m) == 0) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t &low = v[4 * j + e], &high = v[4 * (j | m) + e];
+          const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? low : high, m);
+          if (up) low = got;
+          else high = got;
+        }
+      }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const long long row = __shfl_sync(0xffffffffu, at, (lane & 24) + j);
+    if (row >= 0) *reinterpret_cast<uint4*>(base + row + 4 * (lane & 7)) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+  }
+}
+
 inline bool prefix_plan_ok(const ds41_prefix_plan* p) {
   return p != nullptr && p->units != nullptr && p->n_units != nullptr && p->turns != nullptr && p->order != nullptr && p->cell != nullptr &&
          p->parts != nullptr && p->part_o != nullptr && p->part_ml != nullptr && p->max_units > 0 && p->rows_per_unit > 0 &&

@@ -451,7 +451,7 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
       // the last maximum is there; and the set of the last tile has seen the products up to the one before the last complete, so that the
       // wait that follows cannot take an earlier phase for its own
       named_barrier(1 + quad, 32 * kPlSets);
-      const int key0 = it.key0, this_r = r, this_hi = hi;
+      const int key0 = it.key0, this_r = r, this_hi = hi, queries = it.rows * p.heads;
       const long long this_cell = 1ll * cell * p.heads + h;
       if (unit + unit_step < units) look(next);
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[(kt - 1) % kPlSets], ((kt - 1) / kPlSets) & 1, p.status, 526)) != 0;
@@ -469,15 +469,21 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
           *reinterpret_cast<float2*>(plan.part_ml + 2 * this_cell) =
               make_float2(seen ? m : -INFINITY, seen ? l : 0.f);
         float* dst = plan.part_o + (write ? this_cell : 0) * p.kvp + v0;
-        for (int c = 16 * set; c < v1 - v0; c += 16 * kPlSets) {
-          uint32_t o[16];
-          tmem_ld_32x16(lanes + c, o);
-          tmem_wait_ld();
-          if (write) {
-            store8(dst + c, reinterpret_cast<const float(&)[8]>(o[0]));
-            store8(dst + c + 8, reinterpret_cast<const float(&)[8]>(o[8]));
+        if (__any_sync(0xffffffffu, write)) {
+#pragma unroll 1
+          for (int c = 32 * set; c < v1 - v0; c += 32 * kPlSets) {
+            uint32_t o[32];
+            tmem_ld_32x32(lanes + c, o);
+            tmem_wait_ld();
+            if (queries > kPlQueries / 2 && c + 32 <= v1 - v0) {
+              store_rows(plan.part_o + v0 + c, write ? this_cell * p.kvp : -1, o);
+            } else if (write) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 8)
+                if (c + i < v1 - v0) store8(dst + c + i, reinterpret_cast<const float(&)[8]>(o[i]));
+            }
+            __syncwarp();
           }
-          __syncwarp();
         }
       }
       tc_fence_before();
