@@ -5,8 +5,9 @@
 // come in twos, and where both of them walk the same keys each copy serves two tiles.  One tile's softmax runs while the tensor core
 // works on the other's products, and nothing but the order of the copies ties the two together.
 //   warps 0-3, 4-7 : softmax of tile 0 / 1 (one thread per query), partial results
-//   warps 8, 12    : TMA producers: key / value tiles of 128 positions, page by page
-//   warp 9         : tcgen05.mma issue, in whichever order their inputs come: S = Q K^T, O += P V with P in TMEM where it replaces its S
+//   warps 8, 12    : TMA producers: key / value tiles of 64 positions, page by page
+//   warps 9, 14    : tcgen05.mma issue for tile 0 / 1: S = Q K^T, O += P V with P in TMEM where it replaces its S.  S has two places,
+//                    and the next tile's are asked for before this one's values
 //   warps 10, 11   : queries of tile 0 / 1, and what each of them sees
 //   warp 13        : what the next units are and where their keys lie, for everybody (a ring of four)
 // A CTA walks its units, and every role but the softmax runs ahead into the next ones: a request's own keys are a few tiles, which the
@@ -22,17 +23,19 @@
 
 namespace ds41 {
 
-constexpr int kPgThreads = 448;
-constexpr int kPgTile = 128;                   // queries per tile, keys per tile
-constexpr int kPgChunk = kPgTile * 128;        // bytes of 128 rows x 64 bf16 columns
-constexpr int kPgInfos = 4;
+constexpr int kPgThreads = 480;
+constexpr int kPgTile = 128, kPgKeys = 64;     // queries of a tile, keys of a tile
+constexpr int kPgChunk = kPgTile * 128;        // bytes of 128 queries x 64 bf16 columns
+constexpr int kPgKeyChunk = kPgKeys * 128;     // of 64 keys
+constexpr int kPgInfos = 4, kPgStages = 8;
 
 struct PrefixGroupParams {
   const __nv_bfloat16* q;
   const int *page_table, *row_pos, *row_slot;
   long long ld_q;
-  int heads, kv_heads, n, dp, vp, kd, vc, k_stages, v_stages;
+  int heads, kv_heads, n, dp, vp, kd, vc, stages, shift;             // tiles of keys and of values: 2^shift
   int chunk, max_pages, page_tokens, box, hidden_row;      // a row beyond the pool: reads as zeros
+  int deep;                                                // all chunks of a box in one copy
   float scale_log2;
   int* status;
 };
@@ -46,35 +49,36 @@ struct __align__(16) GroupWork {
 };
 
 // Number of key tile j of tile t in the order of the copies: one after the other, or in turn as long as both have some.
-__device__ __forceinline__ int copy_index(const GroupWork& w, int t, int j) {
-  if (w.both) return w.base + j;
-  const int least = min(w.tiles[0], w.tiles[1]);
-  return w.base + (j < least ? 2 * j + t : least + j);
+__device__ __forceinline__ int copy_index(bool both, int base, int least, int t, int j) {
+  return base + (both ? j : j < least ? 2 * j + t : least + j);
 }
 
 struct GroupShared {                           // behind the tiles
   uint64_t info_full[kPgInfos], info_empty[kPgInfos];
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t k_full[kPgStages], k_empty[kPgStages], v_full[kPgStages], v_empty[kPgStages];
   // per tile:
   uint64_t q_full[2], q_empty[2];
-  uint64_t s_full[2];                          // S complete (and every earlier MMA of the issuing thread)
-  uint64_t p_full[2];                          // P written, O rescaled
+  uint64_t s_full[2][2];                       // by place of S: complete (and every earlier MMA of the issuing thread)
+  uint64_t p_full[2][2];                       // P written, O rescaled
+  uint64_t o_next[2];                          // the unit's last product but one
   uint64_t o_full[2];                          // the unit's last product
   uint64_t v_here[2];                          // the values of a tail's last tile, for the softmax
-  uint32_t tmem, pad[3];
+  int k_asked, v_asked;                        // copies under way or done: a place's barrier is at the phase of the last of these
+  uint32_t tmem, pad[1];
   GroupWork info[kPgInfos];
   int4 row[2][kPgTile];                        // of a unit's row: pass row, visible keys [y, z), cell
 };
 
 __global__ void __launch_bounds__(kPgThreads, 1)
-prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupParams p, const ds41_prefix_plan plan) {
+prefix_group_kernel(const __grid_constant__ CUtensorMap keys, const __grid_constant__ CUtensorMap values, const PrefixGroupParams p,
+                    const ds41_prefix_plan plan) {
   extern __shared__ uint8_t pg_raw[];
   uint8_t* smem = pg_raw + ((1024u - (smem_u32(pg_raw) & 1023u)) & 1023u);
-  const int q_bytes = p.kd * kPgChunk, k_bytes = q_bytes, v_bytes = p.vc * kPgChunk;
+  const int q_bytes = p.kd * kPgChunk, k_bytes = p.kd * kPgKeyChunk, v_bytes = p.vc * kPgKeyChunk;
   uint8_t* s_q = smem;                                   // two tiles
   uint8_t* s_k = s_q + 2 * q_bytes;
-  uint8_t* s_v = s_k + p.k_stages * k_bytes;
-  GroupShared& sh = *reinterpret_cast<GroupShared*>(s_v + p.v_stages * v_bytes);
+  uint8_t* s_v = s_k + p.stages * k_bytes;
+  GroupShared& sh = *reinterpret_cast<GroupShared*>(s_v + p.stages * v_bytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   pdl_launch_dependents();
@@ -86,17 +90,24 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.q_full[i], 1);
       mbar_init(&sh.q_empty[i], 5);                      // four softmax warps, the products
-      mbar_init(&sh.k_full[i], 1);
-      mbar_init(&sh.k_empty[i], 1);
-      mbar_init(&sh.v_full[i], 1);
-      mbar_init(&sh.v_empty[i], 1);
-      mbar_init(&sh.s_full[i], 1);
-      mbar_init(&sh.p_full[i], 4);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&sh.s_full[i][b], 1);
+        mbar_init(&sh.p_full[i][b], 4);
+      }
+      mbar_init(&sh.o_next[i], 1);
       mbar_init(&sh.o_full[i], 1);
       mbar_init(&sh.v_here[i], 1);
     }
+    for (int i = 0; i < kPgStages; ++i) {
+      mbar_init(&sh.k_full[i], 1);
+      mbar_init(&sh.k_empty[i], 2);                      // the products of either tile, or twice those of one
+      mbar_init(&sh.v_full[i], 1);
+      mbar_init(&sh.v_empty[i], 2);
+    }
+    sh.k_asked = sh.v_asked = 0;
     mbar_init_fence();
-    tma_prefetch_desc(&pool);
+    tma_prefetch_desc(&keys);
+    tma_prefetch_desc(&values);
   }
   if (warp == 9) {
     tmem_alloc(&sh.tmem, 512);
@@ -147,7 +158,7 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
       ok = __all_sync(0xffffffffu, mbar_wait(&sh.info_empty[turn % kPgInfos], ((turn / kPgInfos) & 1) ^ 1, p.status, 459)) != 0;
       if (!ok) break;
       GroupWork& w = sh.info[turn % kPgInfos];
-      const int tiles[2] = {(end[0] - first[0] + kPgTile - 1) / kPgTile, (end[1] - first[1] + kPgTile - 1) / kPgTile};
+      const int tiles[2] = {(end[0] - first[0] + kPgKeys - 1) / kPgKeys, (end[1] - first[1] + kPgKeys - 1) / kPgKeys};
       w.row[0][lane] = row_a;
       w.row[1][lane] = row_b;
       if (lane < 2) {
@@ -163,11 +174,13 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
       base += both ? tiles[0] : tiles[0] + tiles[1];
     }
   } else if (warp == 8 || warp == 12) {
-    const bool values = warp == 12;
-    const int boxes = kPgTile / p.box, chunks = values ? p.vc : p.kd, stages = values ? p.v_stages : p.k_stages;
-    const int bytes = chunks * kPgChunk;
-    uint64_t *full = values ? sh.v_full : sh.k_full, *empty = values ? sh.v_empty : sh.k_empty;
-    uint8_t* tiles = values ? s_v : s_k;
+    const bool second = warp == 12;                      // values
+    const int boxes = kPgKeys / p.box, chunks = second ? p.vc : p.kd, stages = p.stages;
+    const int bytes = chunks * kPgKeyChunk;
+    const CUtensorMap* map = second ? &values : &keys;
+    uint64_t *full = second ? sh.v_full : sh.k_full, *empty = second ? sh.v_empty : sh.k_empty;
+    uint8_t* tiles = second ? s_v : s_k;
+    int* asked = second ? &sh.v_asked : &sh.k_asked;
     int count = 0, stage = 0;
     uint32_t free_phase = 1;
     for (int turn = 0; turn < turns && ok; ++turn) {
@@ -176,8 +189,8 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
       const GroupWork& w = sh.info[turn % kPgInfos];
       const int n0 = w.tiles[0], n1 = w.both ? 0 : w.tiles[1], most = max(n0, n1);
       int row0 = w.row[0][lane], row1 = w.row[1][lane];
-      const int x0 = values ? p.kv_heads * p.dp + w.unit[0].head * p.vp : w.unit[0].head * p.dp;
-      const int x1 = values ? p.kv_heads * p.dp + w.unit[1].head * p.vp : w.unit[1].head * p.dp;
+      const int x0 = second ? p.kv_heads * p.dp + w.unit[0].head * p.vp : w.unit[0].head * p.dp;
+      const int x1 = second ? p.kv_heads * p.dp + w.unit[1].head * p.vp : w.unit[1].head * p.dp;
       for (int j = 0; j < most && ok; ++j) {
         const int u = j * boxes;
         if (u > 0 && (u & 31) == 0) {                    // boxes divides 32
@@ -188,16 +201,25 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
         for (int t = 0; t < 2; ++t) {
           if (j >= (t ? n1 : n0)) continue;
           const int row = t ? row1 : row0, x = t ? x1 : x0;
-          ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], free_phase, p.status, values ? 461 : 460)) != 0;
+          ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], free_phase, p.status, second ? 461 : 460)) != 0;
           if (!ok) break;
           uint8_t* dst = tiles + stage * bytes;
-          if (lane == 0) mbar_expect_tx(&full[stage], bytes);
+          if (lane == 0) {
+            mbar_expect_tx(&full[stage], bytes);
+            *reinterpret_cast<volatile int*>(asked) = count + 1;
+          }
 #pragma unroll 1
           for (int i = 0; i < boxes; ++i, dst += p.box * 128) {
             const int at = __shfl_sync(0xffffffffu, row, (u + i) & 31);
-            if (lane == 0)
+            if (lane == 0) {
+              // a copy costs its thread 50 to 100 cycles: all chunks of a page's rows in one where they lie side by side in whole chunks
+              if (p.deep) {
+                tma_load_3d(dst, map, &full[stage], 0, at, x >> 6);
+              } else {
 #pragma unroll 1
-              for (int c = 0; c < chunks; ++c) tma_load_3d(dst + c * kPgChunk, &pool, &full[stage], x + 64 * c, at, 0);
+                for (int c = 0; c < chunks; ++c) tma_load_3d(dst + c * kPgKeyChunk, map, &full[stage], x + 64 * c, at, 0);
+              }
+            }
             __syncwarp();
           }
           ++count;
@@ -214,118 +236,79 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
       for (int b = max(0, count - stages); b < count; ++b)
         for (int i = 0; i < (1 << 18) && !mbar_test_wait(&full[b % stages], (b / stages) & 1); ++i) {
         }
-  } else if (warp == 9) {
-    // one thread: votes and the like between two products cost as much as the products
+  } else if (warp == 9 || warp == 14) {
+    // One thread: votes and the like between two products cost as much as the products.  One of either tile: a single one for both,
+    // that looked in turn for what could be asked next, took 800 cycles for every step of 250 to 400 cycles of products.
     if (elect_one()) {
-      const uint32_t idesc_s = umma_idesc(kPgTile, kPgTile, 1u, 1u);
+      const int t = warp == 14;
+      const uint32_t idesc_s = umma_idesc(kPgTile, kPgKeys, 1u, 1u);
       const uint32_t idesc_pv = umma_idesc_bmn(kPgTile, p.vp, 1u, 1u);
-      const uint64_t q_desc = umma_desc_sw128(smem_u32(s_q)), k_desc = umma_desc_sw128(smem_u32(s_k));
-      const uint64_t v_desc = umma_desc_sw128_mn(smem_u32(s_v), kPgChunk, 1024);
-      const int whole = p.dp / 64, rest = p.dp / 16 - 4 * whole;
-      // per tile: the turn it is at, its key tiles (0: not begun), the next scores and values of that turn, and counts of units and
-      // products for the barriers' phases.  Scores overwrite the P that the values before them read.
-      int turn[2] = {0, 0}, n[2] = {0, 0}, sj[2] = {0, 0}, pj[2] = {0, 0}, begun[2] = {0, 0}, done[2] = {0, 0};
-      bool told[2] = {false, false};
-      // A tile's place in its ring has been filled at most as often as its last tenants were used: one tile may ask for copies far ahead
-      // of the other's, whose barrier would still show a phase of the same parity.
-      int k_used[2] = {-p.k_stages, 1 - p.k_stages}, v_used[2] = {-p.v_stages, 1 - p.v_stages};
-      auto key_here = [&](int at) {
-        const int stage = p.k_stages == 2 ? at & 1 : 0;
-        return (stage ? k_used[1] : k_used[0]) == at - p.k_stages &&
-               mbar_test_wait(&sh.k_full[stage], p.k_stages == 2 ? (at >> 1) & 1 : at & 1);
-      };
-      auto value_here = [&](int at) {
-        const int stage = p.v_stages == 2 ? at & 1 : 0;
-        return (stage ? v_used[1] : v_used[0]) == at - p.v_stages &&
-               mbar_test_wait(&sh.v_full[stage], p.v_stages == 2 ? (at >> 1) & 1 : at & 1);
-      };
-      uint32_t idle = 0;
-      long long since = 0;
-      while (ok && (turn[0] < turns || turn[1] < turns)) {
-        bool moved = false;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (turn[t] >= turns) continue;
-          const GroupWork& w = sh.info[turn[t] % kPgInfos];
-          uint64_t* read = &sh.info_empty[turn[t] % kPgInfos];
-          if (n[t] == 0) {
-            if (!mbar_test_wait(&sh.info_full[turn[t] % kPgInfos], (turn[t] / kPgInfos) & 1)) continue;
-            moved = true;
-            n[t] = w.tiles[t];
-            if (n[t] == 0) {
-              mbar_arrive(read);
-              ++turn[t];
-              continue;
-            }
-          }
-          const bool both = w.both != 0;
-          const int o = t ^ 1;
-          if (pj[t] < sj[t]) {
-            const int at = copy_index(w, t, pj[t]), stage = p.v_stages == 2 ? at & 1 : 0;
-            if (!told[t] && pj[t] + 1 == n[t] && w.unit[t].tail && value_here(at)) {
-              mbar_arrive(&sh.v_here[t]);
-              told[t] = moved = true;
-            }
-            if (mbar_test_wait(&sh.p_full[t], done[t] & 1) && value_here(at)) {
-              tc_fence_after();
-              const uint64_t vd = v_desc + static_cast<uint64_t>(stage * v_bytes / 16);
-              const uint32_t to = tmem + 256 + t * 128, a = tmem + t * 128;
-              umma4_ts<128>(to, a, vd, idesc_pv, pj[t] > 0);
-              umma4_ts<128>(to, a + 32, vd + 512, idesc_pv, 1u);
-              ++done[t];
-              if (!both || turn[o] > turn[t] || (turn[o] == turn[t] && pj[o] > pj[t])) {      // its last reader
-                tc_commit_if(true, &sh.v_empty[stage]);
-                if (stage) v_used[1] = at;
-                else v_used[0] = at;
+      const uint64_t q_desc = umma_desc_sw128(smem_u32(s_q + t * q_bytes)), k_desc = umma_desc_sw128(smem_u32(s_k));
+      const uint64_t v_desc = umma_desc_sw128_mn(smem_u32(s_v), kPgKeyChunk, 1024);
+      const int whole = p.dp / 64, rest = p.dp / 16 - 4 * whole, mask = p.stages - 1;
+      int begun = 0, tiles = 0, done = 0, k_seen = 0, v_seen = 0;        // units, tiles of S, products so far; copies known to be asked for
+      // Copy `at` of a ring has landed.  Its place's barrier alone does not say so: while the copy before it in this place, the other
+      // tile's, is under way, the one before that shows the same parity.
+      auto landed = [&](const int* asked, int& seen, uint64_t* full, int at, int where) {
+        if (seen <= at) {
+          const long long start = clock64();
+          for (uint32_t spins = 1; (seen = *reinterpret_cast<const volatile int*>(asked)) <= at; ++spins)
+            if ((spins & 0x3ff) == 0 && (clock64() - start > DS41_WAIT_LIMIT_CYCLES ||
+                                         (p.status != nullptr && *reinterpret_cast<volatile int*>(p.status) != kStatusOk))) {
+              if (p.status != nullptr && atomicCAS(p.status, kStatusOk, kStatusMbarTimeout) == kStatusOk) {
+                p.status[1] = where;
+                p.status[2] = static_cast<int>(blockIdx.x);
+                p.status[3] = at;
               }
-              ++pj[t];
-              moved = true;
-              if (pj[t] == n[t]) {
-                tc_commit_if(true, &sh.o_full[t]);
-                mbar_arrive(read);
-                ++turn[t];
-                n[t] = sj[t] = pj[t] = 0;                // the other tile compares itself with these
-                told[t] = false;
-                continue;
-              }
+              return false;
             }
-          }
-          if (sj[t] < n[t] && sj[t] == pj[t]) {
-            const int at = copy_index(w, t, sj[t]), stage = p.k_stages == 2 ? at & 1 : 0;
-            if (key_here(at) && (sj[t] > 0 || mbar_test_wait(&sh.q_full[t], begun[t] & 1))) {
-              tc_fence_after();
-              uint64_t a = q_desc + static_cast<uint64_t>(t * q_bytes / 16), b = k_desc + static_cast<uint64_t>(stage * k_bytes / 16);
-#pragma unroll 1
-              for (int c = 0; c < whole; ++c, a += kPgChunk / 16, b += kPgChunk / 16) umma4_ss<2, 2>(tmem + t * 128, a, b, idesc_s, c);
-#pragma unroll 1
-              for (int k = 0; k < rest; ++k) umma_bf16(tmem + t * 128, a + 2 * k, b + 2 * k, idesc_s, whole > 0 || k > 0);
-              tc_commit_if(true, &sh.s_full[t]);
-              if (!both || turn[o] > turn[t] || (turn[o] == turn[t] && sj[o] > sj[t])) {
-                tc_commit_if(true, &sh.k_empty[stage]);
-                if (stage) k_used[1] = at;
-                else k_used[0] = at;
-              }
-              if (sj[t] == 0) ++begun[t];
-              ++sj[t];
-              if (sj[t] == n[t]) tc_commit_if(true, &sh.q_empty[t]);
-              moved = true;
-            }
-          }
         }
-        if (moved) {
-          idle = 0;
-          since = 0;
-        } else if ((++idle & 0x3ff) == 0) {              // as long as any other wait: see mbar_wait
-          if (since == 0) since = clock64();
-          if (clock64() - since > DS41_WAIT_LIMIT_CYCLES ||
-              (p.status != nullptr && *reinterpret_cast<volatile int*>(p.status) != kStatusOk)) {
-            if (p.status != nullptr && atomicCAS(p.status, kStatusOk, kStatusMbarTimeout) == kStatusOk) {
-              p.status[1] = 471;
-              p.status[2] = static_cast<int>(blockIdx.x);
-              p.status[3] = turn[0];
-            }
-            ok = false;
-          }
+        return mbar_wait(&full[at & mask], (at >> p.shift) & 1, p.status, where);
+      };
+      for (int turn = 0; turn < turns && ok; ++turn) {
+        ok = mbar_wait(&sh.info_full[turn % kPgInfos], (turn / kPgInfos) & 1, p.status, 470);
+        if (!ok) break;
+        const GroupWork& w = sh.info[turn % kPgInfos];
+        const int n = w.tiles[t], base = w.base, least = min(w.tiles[0], w.tiles[1]);
+        const bool both = w.both != 0, tail = w.unit[t].tail != 0;
+        mbar_arrive(&sh.info_empty[turn % kPgInfos]);
+        if (n == 0) continue;
+        auto scores = [&](int j) {
+          const int at = copy_index(both, base, least, t, j), stage = at & mask, place = tiles & 1;
+          if (!landed(&sh.k_asked, k_seen, sh.k_full, at, 471)) return false;
+          tc_fence_after();
+          const uint32_t to = tmem + t * 128 + 64 * place;
+          uint64_t a = q_desc, b = k_desc + static_cast<uint64_t>(stage * k_bytes / 16);
+#pragma unroll 1
+          for (int c = 0; c < whole; ++c, a += kPgChunk / 16, b += kPgKeyChunk / 16) umma4_ss<2, 2>(to, a, b, idesc_s, c);
+#pragma unroll 1
+          for (int k = 0; k < rest; ++k) umma_bf16(to, a + 2 * k, b + 2 * k, idesc_s, whole > 0 || k > 0);
+          tc_commit(&sh.s_full[t][place]);
+          if (!both) mbar_arrive(&sh.k_empty[stage]);
+          tc_commit(&sh.k_empty[stage]);
+          ++tiles;
+          if (j + 1 == n) tc_commit(&sh.q_empty[t]);
+          return true;
+        };
+        ok = mbar_wait(&sh.q_full[t], begun & 1, p.status, 472) && scores(0);
+        ++begun;
+        for (int j = 0; j < n && ok; ++j) {
+          // they overwrite the P that the values before this tile's read
+          if (j + 1 < n) ok = scores(j + 1);
+          if (!ok) break;
+          const int at = copy_index(both, base, least, t, j), stage = at & mask, place = done & 1;
+          ok = landed(&sh.v_asked, v_seen, sh.v_full, at, 473);
+          if (!ok) break;
+          if (tail && j + 1 == n) mbar_arrive(&sh.v_here[t]);
+          ok = mbar_wait(&sh.p_full[t][place], (done >> 1) & 1, p.status, 474);
+          if (!ok) break;
+          tc_fence_after();
+          umma4_ts<128>(tmem + 256 + t * 128, tmem + t * 128 + 64 * place, v_desc + static_cast<uint64_t>(stage * v_bytes / 16), idesc_pv, j > 0);
+          ++done;
+          if (!both) mbar_arrive(&sh.v_empty[stage]);
+          tc_commit(&sh.v_empty[stage]);
+          if (j + 2 == n) tc_commit(&sh.o_next[t]);
+          if (j + 1 == n) tc_commit(&sh.o_full[t]);
         }
       }
     }
@@ -339,7 +322,7 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
       unit = w.unit[t];
       first = w.first[t];
       end = w.end[t];
-      last = copy_index(w, t, w.tiles[t] > 0 ? w.tiles[t] - 1 : 0);
+      last = copy_index(w.both != 0, w.base, min(w.tiles[0], w.tiles[1]), t, w.tiles[t] - 1);
       return w.tiles[t];
     };
     auto work_read = [&](int turn) {
@@ -397,9 +380,9 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
     } else {
       const int t = warp >> 2, quad = warp & 3, mine = quad * 32 + lane;
       const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
-      const uint32_t s_t = tmem + lanes + t * 128, o_t = tmem + lanes + 256 + t * 128;
+      const uint32_t o_t = tmem + lanes + 256 + t * 128;
       const int mine_row = mine / p.n, mine_head = mine - mine_row * p.n;
-      int tiles = 0, done = 0, tails = 0;                // tiles of S, units with keys, tails among them so far
+      int tiles = 0, done = 0, pairs = 0, tails = 0;     // tiles of S, units with keys, those with two tiles or more, tails so far
       for (int turn = 0; turn < turns; ++turn) {
         const int n = work(turn, t, unit, first, end, last);
         if (!ok) break;
@@ -427,42 +410,42 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
         const bool idle = high == 0x7fffffff;            // no query of this warp sees anything
         float m = -INFINITY, l = 0.f;
         for (int j = 0; j < n; ++j) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&sh.s_full[t], tiles & 1, p.status, 480 + t)) != 0;
+          const int place = tiles & 1;
+          const uint32_t s_t = tmem + lanes + t * 128 + 64 * place;
+          ok = __all_sync(0xffffffffu, mbar_wait(&sh.s_full[t][place], (tiles >> 1) & 1, p.status, 480 + t)) != 0;
           if (!ok) break;
           ++tiles;
-          const int key0 = first + j * kPgTile;
+          // the last tile: the product before it is complete; for the others the next scores say so
+          if (j > 0 && j + 1 == n) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_next[t], pairs & 1, p.status, 486 + t)) != 0;
+            if (!ok) break;
+            ++pairs;
+          }
+          const int key0 = first + j * kPgKeys;
           if (!idle) {
             tc_fence_after();
-            const bool edge = key0 < low || key0 + kPgTile > high;
+            const bool edge = key0 < low || key0 + kPgKeys > high;
             const int shown = hi - key0, hidden = lo - key0;             // columns [hidden, shown) of this tile are visible
-            // Two pieces of 64 columns, read twice.  The bodies of these loops are short on purpose: with the tile unrolled, 42 % of all cycles
-            // were waits for instructions, and a small call, which runs all code for the first time, took 6400 cycles for its one tile.
-            if (edge) {
-#pragma unroll 1
-              for (int c = 0; c < kPgTile; c += 32) {
-                uint32_t v[32];
-                tmem_ld_32x32(s_t + c, v);
-                tmem_wait_ld();
-#pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = i < shown - c && i >= hidden - c ? v[i] : 0xff800000u;
-                tmem_st_32x32(s_t + c, v);
-              }
-              tmem_wait_st();
-            }
-            float top = -INFINITY;
-#pragma unroll 1
-            for (int c = 0; c < kPgTile; c += 64) {
-              uint32_t v[64];
-              tmem_ld_32x32(s_t + c, reinterpret_cast<uint32_t(&)[32]>(v[0]));
-              tmem_ld_32x32(s_t + c + 32, reinterpret_cast<uint32_t(&)[32]>(v[32]));
+            // The code of this loop is short on purpose: with tiles unrolled over 128 columns, 42 % of all cycles were waits for
+            // instructions, and a small call, which runs everything for the first time, took 6400 cycles for its one tile.
+            float2 v[kPgKeys / 2];
+            {
+              uint32_t(&raw)[64] = reinterpret_cast<uint32_t(&)[64]>(v);
+              tmem_ld_32x32(s_t, reinterpret_cast<uint32_t(&)[32]>(raw[0]));
+              tmem_ld_32x32(s_t + 32, reinterpret_cast<uint32_t(&)[32]>(raw[32]));
               tmem_wait_ld();
-              float tops[4] = {top, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-              for (int i = 0; i < 64; i += 2)
-                tops[(i >> 1) & 3] = fmaxf(tops[(i >> 1) & 3], fmaxf(__uint_as_float(v[i]), __uint_as_float(v[i + 1])));
-              top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
             }
-            top *= p.scale_log2;
+            if (edge) {
+#pragma unroll
+              for (int i = 0; i < kPgKeys / 2; ++i) {
+                v[i].x = 2 * i < shown && 2 * i >= hidden ? v[i].x : -INFINITY;
+                v[i].y = 2 * i + 1 < shown && 2 * i + 1 >= hidden ? v[i].y : -INFINITY;
+              }
+            }
+            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int i = 0; i < kPgKeys / 2; ++i) tops[i & 3] = fmaxf(tops[i & 3], fmaxf(v[i].x, v[i].y));
+            const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * p.scale_log2;
             const bool grow = hi > lo && (top > m + 8.f || (m == -INFINITY && top > m));
             if (__any_sync(0xffffffffu, grow)) {
               const float m_new = grow ? top : m;
@@ -470,6 +453,11 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
               if (grow) l *= alpha;
               m = m_new;
               if (j > 0) {
+                if (j + 1 < n) {                         // the next scores were issued behind the last values
+                  ok = __all_sync(0xffffffffu, mbar_wait(&sh.s_full[t][place ^ 1], (tiles >> 1) & 1, p.status, 488 + t)) != 0;
+                  if (!ok) break;
+                  tc_fence_after();
+                }
                 const float keep = grow ? alpha : 1.f;
 #pragma unroll 1
                 for (int c = 0; c < p.vp; c += 16) {
@@ -485,45 +473,39 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap pool, const PrefixGroupP
             const float neg = m == -INFINITY ? 0.f : -m;
             const float2 by = make_float2(p.scale_log2, p.scale_log2), off = make_float2(neg, neg);
             float2 sums[2] = {};
-#pragma unroll 1
-            for (int c = 0; c < kPgTile; c += 64) {
-              uint32_t v[64];
-              tmem_ld_32x32(s_t + c, reinterpret_cast<uint32_t(&)[32]>(v[0]));
-              tmem_ld_32x32(s_t + c + 32, reinterpret_cast<uint32_t(&)[32]>(v[32]));
-              tmem_wait_ld();
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                uint32_t e2[16];
+            for (int h = 0; h < 2; ++h) {
+              uint32_t e2[16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                  float2 e = fma2(make_float2(__uint_as_float(v[32 * h + 2 * i]), __uint_as_float(v[32 * h + 2 * i + 1])), by, off);
-                  e = make_float2(ex2_approx(e.x), ex2_approx(e.y));
-                  sums[i & 1] = add2(sums[i & 1], e);
-                  const __nv_bfloat162 b = __floats2bfloat162_rn(e.x, e.y);
-                  e2[i] = *reinterpret_cast<const uint32_t*>(&b);
-                }
-                tmem_st_32x16(s_t + c / 2 + 16 * h, e2);       // columns whose S this thread has read
+              for (int i = 0; i < 16; ++i) {
+                float2 e = fma2(v[16 * h + i], by, off);
+                e = make_float2(ex2_approx(e.x), ex2_approx(e.y));
+                sums[i & 1] = add2(sums[i & 1], e);
+                const __nv_bfloat162 b = __floats2bfloat162_rn(e.x, e.y);
+                e2[i] = *reinterpret_cast<const uint32_t*>(&b);
               }
+              tmem_st_32x16(s_t + 16 * h, e2);           // this thread has read all of its S
             }
             sums[0] = add2(sums[0], sums[1]);
             l += sums[0].x + sums[0].y;
           }
           if (unit.tail && j + 1 == n) {
             // Places behind the last position belong to nobody, and a weight of zero does not take a NaN or an infinity away: their
-            // values become zeros, a thread to a place.
-            const int stage = p.v_stages == 2 ? last & 1 : 0;
+            // values become zeros, two threads to a place.
             ok = __all_sync(0xffffffffu, mbar_wait(&sh.v_here[t], tails & 1, p.status, 484 + t)) != 0;
             if (!ok) break;
             ++tails;
-            if (key0 + mine >= end)
-              for (int i = 0; i < 8 * p.vc; ++i)
-                *reinterpret_cast<uint4*>(s_v + stage * v_bytes + (i >> 3) * kPgChunk + mine * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+            const int key = mine & (kPgKeys - 1);
+            if (key0 + key >= end)
+              for (int i = 8 * (mine / kPgKeys); i < 8 * p.vc; i += (i & 7) == 7 ? 9 : 1)
+                *reinterpret_cast<uint4*>(s_v + (last & (p.stages - 1)) * v_bytes + (i >> 3) * kPgKeyChunk + key * 128 + (i & 7) * 16) =
+                    make_uint4(0, 0, 0, 0);
             fence_async_smem();
           }
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.p_full[t]);
+          if (lane == 0) mbar_arrive(&sh.p_full[t][place]);
         }
         if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_full[t], done & 1, p.status, 490 + t)) != 0;
         if (!ok) break;
@@ -569,18 +551,19 @@ static bool plan_prefix_group(const ds41_group_attend_args& a, const ds41_prefix
       ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.pool)) & 15) ||
       1ll * a.n_pages * a.page_tokens >= (1ll << 31) - 1)
     return false;
-  if (a.page_tokens % kPgTile == 0) p.box = kPgTile;
-  else if (kPgTile % a.page_tokens == 0 && a.page_tokens >= 8) p.box = a.page_tokens;
+  if (a.page_tokens % kPgKeys == 0) p.box = kPgKeys;
+  else if (kPgKeys % a.page_tokens == 0 && a.page_tokens >= 8) p.box = a.page_tokens;
   else return false;
   p.kd = (a.dim_pad + 63) / 64;
   p.vc = (a.vdim_pad + 63) / 64;
-  const int qk = p.kd * kPgChunk, v = p.vc * kPgChunk;
+  p.deep = p.box == kPgKeys && a.dim_pad % 64 == 0 && a.vdim_pad % 64 == 0;
+  const int q = p.kd * kPgChunk, k = p.kd * kPgKeyChunk, v = p.vc * kPgKeyChunk;
   constexpr int kExtra = 1024 + static_cast<int>(sizeof(GroupShared)), kLimit = 227 * 1024 - kExtra;
-  p.k_stages = p.v_stages = 1;
-  if (3 * qk + v > kLimit) return false;
-  if (4 * qk + v <= kLimit) p.k_stages = 2;
-  if ((2 + p.k_stages) * qk + 2 * v <= kLimit) p.v_stages = 2;
-  smem = (2 + p.k_stages) * qk + p.v_stages * v + kExtra;
+  const int fit = (kLimit - 2 * q) / (k + v);
+  if (fit < 1) return false;
+  while (p.shift < 3 && 2 << p.shift <= fit) ++p.shift;  // kPgStages at most
+  p.stages = 1 << p.shift;
+  smem = 2 * q + p.stages * (k + v) + kExtra;
   return true;
 }
 
@@ -595,13 +578,19 @@ int launch_prefix_group(const ds41_group_attend_args& a, const ds41_prefix_plan&
   p.chunk = a.chunk; p.max_pages = a.max_pages; p.page_tokens = a.page_tokens; p.hidden_row = a.n_pages * a.page_tokens;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.status = a.status;
-  CUtensorMap pool;
   const int row_len = a.kv_heads * (a.dim_pad + a.vdim_pad);
-  cudaError_t e = make_tensor_map_3d(&pool, a.pool, TmaDtype::kBF16, row_len, p.hidden_row, 1, 2ull * row_len, 0, 64, p.box, true);
+  // keys and values are columns of the same rows; deep: as chunks of 64 columns, all of a head's in one box
+  CUtensorMap keys, values;
+  for (int i = 0; i < 2; ++i) {
+    const cudaError_t e =
+        p.deep ? make_tensor_map_3d(i ? &values : &keys, a.pool, TmaDtype::kBF16, 64, p.hidden_row, row_len / 64, 2ull * row_len, 128, 64, p.box,
+                                    true, i ? p.vc : p.kd)
+               : make_tensor_map_3d(i ? &values : &keys, a.pool, TmaDtype::kBF16, row_len, p.hidden_row, 1, 2ull * row_len, 0, 64, p.box, true);
+    if (e != cudaSuccess) return e;
+  }
+  const cudaError_t e = cudaFuncSetAttribute(prefix_group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  e = cudaFuncSetAttribute(prefix_group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return e;
-  return launch_pdl(prefix_group_kernel, dim3(plan.grid), dim3(kPgThreads), smem, st, pool, p, plan);
+  return launch_pdl(prefix_group_kernel, dim3(plan.grid), dim3(kPgThreads), smem, st, keys, values, p, plan);
 }
 
 }  // namespace ds41
