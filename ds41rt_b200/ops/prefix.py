@@ -15,7 +15,7 @@ from __future__ import annotations
 
 import ctypes as C
 import heapq
-from typing import Dict, List, Optional, Sequence, Tuple
+from typing import Dict, List, NamedTuple, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
@@ -62,36 +62,21 @@ def common_runs(tables: np.ndarray) -> List[Tuple[List[int], int]]:
     return out
 
 
-class Cost:
-    """What a plan goes by, in us: of a unit and of one of its keys (a unit alone), of a block's turn and of a key in it, where `apart`
-    says what the keys of two units count that do not walk the same ones, and of a byte of partial results on their way to the join."""
+class Cost(NamedTuple):
+    """What a plan goes by, in us (measured on units of 64 to 16000 keys): of a block's turn, of a row of its units, of a key of the
+    longer of the units that it has at a time and of one of the shorter, of a byte of partial results on their way to the join and of a
+    part of the row that has most of them."""
+    turn: float
+    row: float
+    longer: float
+    shorter: float
+    byte: float
+    part: float = 0.2
 
-    def __init__(self, unit: float, key: float, turn: float, walk: float, apart: float):
-        self.unit, self.key, self.turn, self.walk, self.apart, self.byte = unit, key, turn, walk, apart, 1 / 4e6
 
-
-COSTS = {"grouped": Cost(5.0, 0.02, 4.0, 0.015, 0.75), "latent": Cost(4.0, 0.02, 4.0, 0.02, 1.0)}
-
-
-def key_span(work: Sequence[Tuple[int, int, int]], width: int, part_bytes: int, most: int, unit: int, cost: Cost) -> int:
-    """Keys of a unit, where `work` lists (pieces, rows, keys) of every range of pages and `width` units run at once: the length with
-    the least estimate of the time until the last unit is done plus that of moving the partial results, at most `most` units."""
-    pieces, rows, keys = (np.array(x, dtype=np.float64) for x in zip(*work))
-    best, longest = None, int(keys.max())
-    for k in (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256, 512, 1024, 4096, 1 << 20):
-        span = k * unit
-        count = np.maximum(1, np.ceil(keys / span))
-        if (pieces * count).sum() <= most:
-            total = (pieces * (count * cost.unit + keys * cost.key)).sum() / width
-            last = cost.unit + min(span, longest) * cost.key
-            # the units that the busiest block gets are whole ones
-            estimate = max(total, last, np.ceil((pieces * count).sum() / width) * cost.unit + last - cost.unit) \
-                + (rows * count).sum() * part_bytes * cost.byte
-            if best is None or estimate < best[0]:
-                best = (estimate, span)
-        if span >= longest:
-            break
-    return best[1] if best else ceil_to(longest, unit)
+COSTS = {"grouped": Cost(1.4, 0.10, 0.0105, 0.0055, 1 / 6e6), "latent": Cost(4.0, 0.0, 0.0205, 0.0, 1 / 8e6)}
+COST_F32 = Cost(5.0, 0.0, 0.2, 0.2, 1 / 6e6)
+SPANS = (1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 28, 32, 40, 48, 64, 96, 128, 192, 256, 384, 512, 1024, 2048, 4096)    # tried, in tiles or pages
 
 
 class PrefixPlan:
@@ -112,7 +97,7 @@ class PrefixPlan:
             raise ValueError(f"cache rows are bf16 or fp32, not {dtype}")
         self.kind, self.rows, self.heads, self.kv_heads, self.vdim = kind, rows, heads, kv_heads, vdim
         self.page_tokens, self.dtype, self.device = page_tokens, dtype, torch.device(device)
-        self.min_tokens = min_tokens
+        self.min_tokens, self.cost = min_tokens, COSTS[kind] if dtype == BF16 else COST_F32
         self.rows_per_unit = max(1, 128 // (heads // kv_heads))
         self.together = 2 if kind == "grouped" else 1            # units that a block (latent, wide: two blocks) has at a time
         self.grid = SMS // 2 if kind == "latent" and vdim > 256 else SMS               # two CTAs to a unit
@@ -127,7 +112,7 @@ class PrefixPlan:
         self.data = z(self._at[-1] + rows, I32)
         self.part_o, self.part_ml = z(self.max_cells * heads * vdim, F32), z(self.max_cells * heads * 2, F32)
         self.status = lib.new_status(self.device)
-        self.n_units = 0
+        self.n_units = self.span = 0
         self.shared: List[Tuple[List[int], int]] = []      # rows and tokens of every prefix
         a, base = PlanArgs(), self.data.data_ptr()
         a.n_units, (a.units, a.turns, a.order, a.cell, a.parts) = base, (base + 4 * x for x in self._at)
@@ -177,62 +162,96 @@ class PrefixPlan:
         self._lay_out(s, tails, t.shape[1] * self.page_tokens)
 
     def _lay_out(self, slots: np.ndarray, tails, limit: int) -> None:
+        pieces = [-(-len(rows) // self.rows_per_unit) for rows, _ in self.shared]
         host = np.zeros(self.data.numel(), dtype=np.int32)
         units, turns, order, cell, parts = (host[a:b] for a, b in zip(self._at, self._at[1:] + [len(host)]))
-        pieces = [-(-len(rows) // self.rows_per_unit) for rows, _ in self.shared]
-        work = [(p, len(rows), tokens) for p, (rows, tokens) in zip(pieces, self.shared)] + [(1, n, keys) for _, n, _, keys in tails]
+        at = 0
+        for rows, _ in self.shared:
+            order[at:at + len(rows)] = rows
+            at += len(rows)
+        best = None
+        if tails:
+            unit, most = ceil_to(128, self.page_tokens), sum(pieces) + len(tails) + self.extra
+            longest = max([tokens for _, tokens in self.shared] + [t[3] for t in tails])
+            for span in self._spans(longest, unit):
+                if sum(p * -(-x[1] // span) for p, x in zip(pieces, self.shared)) + sum(max(1, x[3] // span) for x in tails) <= most:
+                    items, n_parts = self._items(slots, pieces, tails, limit, span)
+                    every, need = self._pairs(items, {x[0]: x[2] + x[3] for x in tails})
+                    join = 8 * int(n_parts.sum()) * self.heads * self.vdim * self.cost.byte + int(n_parts.max()) * self.cost.part
+                    if best is None or max(need.sum() / self.grid, need.max()) + join < best[0]:
+                        place, time = self._deal(need)
+                        if best is None or time + join < best[0]:
+                            best = (time + join, span, every, place, n_parts)
         n = 0
-        if work:
-            unit, part_bytes = max(128, self.page_tokens), 8 * self.heads * self.vdim
-            span = key_span(work, max(1, self.grid * self.together // self.kv_heads), part_bytes, sum(w[0] for w in work) + self.extra, unit,
-                            COSTS[self.kind])
-            items, at = [], 0
-            for p, (rows, tokens) in zip(pieces, self.shared):
-                count = -(-tokens // span)
-                order[at:at + len(rows)] = rows
-                parts[rows] = count
-                for i in range(p):
-                    lo, hi = (len(rows) * j // p for j in (i, i + 1))
-                    items += [(int(slots[rows[0]]), at + lo, hi - lo, k * span, min(tokens, (k + 1) * span), k, 0) for k in range(count)]
-                at += len(rows)
-            for first, rows, key0, keys in tails:
-                count = max(1, keys // span)                   # the last one goes on to wherever the request gets
-                part = int(parts[first])
-                items += [(int(slots[first]), first, rows, key0 + k * span, key0 + (k + 1) * span if k + 1 < count else limit, part + k, 1)
-                          for k in range(count)]
-                parts[first:first + rows] += count
+        self.span = 0
+        if best is not None:
+            _, self.span, every, place, n_parts = best
+            assert int(n_parts.sum()) <= self.max_cells, int(n_parts.sum())
+            units.reshape(-1, self.together, UNIT)[place] = every
+            turns[:] = np.bincount(place % self.grid, minlength=self.grid)
+            parts[:len(n_parts)] = n_parts
             cell[:] = np.cumsum(parts) - parts
-            assert len(items) <= self.max_items and int(parts.sum()) <= self.max_cells, (len(items), int(parts.sum()))
-            n = self._deal(np.array(items, dtype=np.int32), units, turns, {x[0]: x[2] + x[3] for x in tails})
+            n = int(turns.max()) * self.grid * self.together
         host[0] = self.n_units = n
         self.data.copy_(torch.from_numpy(host))
 
-    def _deal(self, items: np.ndarray, units: np.ndarray, turns: np.ndarray, ends: Dict[int, int]) -> int:
+    def _spans(self, longest: int, unit: int) -> List[int]:
+        return [k * unit for k in SPANS if k * unit < longest] + [ceil_to(longest, unit)]        # the last one divides nothing
+
+    def _items(self, slots: np.ndarray, pieces, tails, limit: int, span: int) -> Tuple[np.ndarray, np.ndarray]:
+        """What there is to do with at most `span` keys at a time, as units without their head, and the partial results of every row."""
+        items, at, parts = [], 0, np.zeros(len(slots), dtype=np.int32)
+        for p, (rows, tokens) in zip(pieces, self.shared):
+            count = -(-tokens // span)
+            parts[rows] = count
+            for i in range(p):
+                lo, hi = (len(rows) * j // p for j in (i, i + 1))
+                items += [(int(slots[rows[0]]), at + lo, hi - lo, k * span, min(tokens, (k + 1) * span), k, 0) for k in range(count)]
+            at += len(rows)
+        for first, rows, key0, keys in tails:
+            count = max(1, keys // span)                       # the last one goes on to wherever the request gets
+            part = int(parts[first])
+            items += [(int(slots[first]), first, rows, key0 + k * span, key0 + (k + 1) * span if k + 1 < count else limit, part + k, 1)
+                      for k in range(count)]
+            parts[first:first + rows] += count
+        return np.array(items, dtype=np.int32), parts
+
+    def _pairs(self, items: np.ndarray, ends: Dict[int, int]) -> Tuple[np.ndarray, np.ndarray]:
         """Items and key/value heads as units, those that a block has at a time side by side (pieces that walk the same keys if there are
-        two), the longest first, each to the block that has least to do: block b takes the places b, b + grid, b + 2 grid ...  Returns
-        how many places there are (one may stay empty)."""
+        two), and what each such group takes."""
         keys = items[:, 4] - items[:, 3]
-        for i in np.flatnonzero(items[:, 6]):
-            keys[i] = min(keys[i], max(1, ends[int(items[i, 1])] - items[i, 3]))
+        last = np.array([ends.get(i, 0) for i in items[:, 1].tolist()])
+        keys = np.where(items[:, 6] == 1, np.minimum(keys, np.maximum(1, last - items[:, 3])), keys)
         order = np.lexsort((items[:, 1], items[:, 3], items[:, 0], -keys))
         # by head, then by item: pieces of one range stand side by side
         every = np.concatenate([np.tile(items[order], (self.kv_heads, 1)), np.repeat(np.arange(self.kv_heads, dtype=np.int32), len(items))[:, None]], 1)
         length = np.tile(keys[order], self.kv_heads)
-        w, cost = self.together, COSTS[self.kind]
+        w, cost = self.together, self.cost
         if len(every) % w:
             every, length = np.concatenate([every, np.zeros((1, UNIT), dtype=np.int32)]), np.append(length, 0)
         every, length = every.reshape(-1, w, UNIT), length.reshape(-1, w)
-        same = (every[:, 0, [0, 3, 4, 7]] == every[:, -1, [0, 3, 4, 7]]).all(1) & (every[:, 0, 6] == 0) & (every[:, -1, 2] > 0)
-        need = cost.turn + cost.walk * np.where(same, length[:, 0], length.sum(1) * cost.apart)
-        blocks = [(0.0, 0, b) for b in range(self.grid)]               # (time so far, turns, block)
-        table = units.reshape(-1, w, UNIT)
-        for i in np.argsort(-need, kind="stable").tolist():
-            time, turn, b = heapq.heappop(blocks)
-            table[turn * self.grid + b] = every[i]
-            turns[b] = turn + 1
-            if turn + 1 < self.max_turns:
-                heapq.heappush(blocks, (time + float(need[i]), turn + 1, b))
-        return int(turns.max()) * self.grid * w
+        longer = length.max(1)
+        return every, cost.turn + cost.row * every[:, :, 2].max(1) + cost.longer * longer + cost.shorter * (length.sum(1) - longer)
+
+    def _deal(self, need: np.ndarray) -> Tuple[np.ndarray, float]:
+        """Groups of units to blocks, the longest first, each to the block that has least to do: block b takes the places b, b + grid,
+        b + 2 grid ...  Returns their places, and the time until the last block is done."""
+        place = np.zeros(len(need), dtype=np.int64)
+        order = np.argsort(-need, kind="stable")
+        place[order[:self.grid]] = np.arange(min(self.grid, len(need)))
+        last = float(need.max())
+        if len(need) > self.grid:
+            blocks = [(time, 1, b) for b, time in enumerate(need[order[:self.grid]].tolist())]     # (time so far, turns, block)
+            heapq.heapify(blocks)
+            for i, time in zip(order[self.grid:].tolist(), need[order[self.grid:]].tolist()):
+                so_far, turn, b = blocks[0]
+                place[i] = turn * self.grid + b
+                last = max(last, so_far + time)
+                if turn + 1 < self.max_turns:
+                    heapq.heapreplace(blocks, (so_far + time, turn + 1, b))
+                else:
+                    heapq.heappop(blocks)
+        return place, last
 
     def check_status(self, what: str = "attention over a shared prefix"):
         lib.raise_on_status(self.status, what)

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from ds41rt_b200.ops import prefix
-from ds41rt_b200.ops.prefix import PrefixPlan, common_runs, key_span
+from ds41rt_b200.ops.prefix import PrefixPlan, common_runs
 
 BF16 = torch.bfloat16
 
@@ -143,12 +143,16 @@ def test_short_prefixes_are_left_to_the_rows():
     assert plan.shared == []
 
 
-@pytest.mark.parametrize("kind", ["grouped", "latent"])
-def test_key_ranges_stay_within_what_the_plan_holds(kind):
-    for pieces, rows, keys in ((1, 4, 100), (3, 100, 100000), (40, 2000, 5000), (200, 300, 300), (1, 2, 1 << 24)):
-        for most in (pieces, pieces + 40):
-            span = key_span([(pieces, rows, keys)], 37, 4096, most, 128, prefix.COSTS[kind])
-            assert span >= 128 and span % 128 == 0 and pieces * -(-keys // span) <= most
+@pytest.mark.parametrize("kind,P", [("grouped", 32), ("grouped", 48), ("grouped", 192), ("latent", 16), ("latent", 160)])
+def test_key_ranges_are_whole_pages_and_fit_the_plan(kind, P):
+    for rows, pages in ((2, 3), (2, 40), (90, 30), (150, 600)):
+        shared = list(range(1, pages + 1))
+        t = table(*[shared + [100000 + 10 * i] for i in range(rows)], width=pages + 4)
+        plan = PrefixPlan(kind, rows=rows, heads=8, kv_heads=2 if kind == "grouped" else 1, vdim=64, page_tokens=P, device="cpu")
+        plan.set(range(rows), t)
+        assert plan.span > 0 and plan.span % P == 0 and 0 < plan.n_units <= plan.max_units
+        units = plan.data[4:4 + 8 * plan.n_units].reshape(-1, 8)
+        assert bool((units[:, 3] % P == 0).all()) and bool((units[:, 4] % P == 0).all())
 
 
 def test_short_requests_are_not_divided_and_long_ones_are():
