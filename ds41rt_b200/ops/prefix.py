@@ -270,44 +270,45 @@ def launch_latent(a: S.LatentAttendArgs, plan: PrefixPlan, n_pages: int, sink, o
 
 
 # ---------------------------------------------------------------------------------------------------- front end
-def _check(plan: PrefixPlan, kind: str, q: torch.Tensor, pool, page_table, row_pos, row_slot, out, width: int, scale: float,
-           named) -> int:
+def _check(plan: PrefixPlan, kind: str, rows: int, tensors, pool, page_table, row_pos, row_slot, out, width: int, scale: float) -> None:
+    """`tensors`: name, tensor or None, and type of every argument."""
     if plan.kind != kind:
         raise ValueError(f"the plan is for {plan.kind} attention")
     if not scale > 0:
         raise ValueError("scale must be positive")
-    R = q.shape[0]
-    if not 0 < R <= plan.rows:
-        raise ValueError(f"a pass has 1 to {plan.rows} rows, not {R}")
-    for name, t in (("pool", pool), ("out", out)) + named:
-        if t is not None and t.dtype != (F32 if name in ("gate", "sink") else plan.dtype):
-            raise ValueError(f"{name} is {t.dtype}")
-    for name, t in (("page_table", page_table), ("row_pos", row_pos), ("row_slot", row_slot)):
-        if t.dtype != I32 or not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous 32-bit integers")
-    if page_table.dim() != 2 or row_pos.dim() != 1 or row_slot.dim() != 1 or row_pos.numel() < R or row_slot.numel() < R:
+    if not 0 < rows <= plan.rows:
+        raise ValueError(f"a pass has 1 to {plan.rows} rows, not {rows}")
+    for name, t, dtype in tensors:
+        if t is not None and t.dtype != dtype:
+            raise ValueError(f"{name} must be 32-bit integers, not {t.dtype}" if dtype == I32 else f"{name} is {t.dtype}")
+    if not (page_table.is_contiguous() and row_pos.is_contiguous() and row_slot.is_contiguous()):
+        raise ValueError("page_table, row_pos and row_slot must be contiguous")
+    if page_table.dim() != 2 or row_pos.dim() != 1 or row_slot.dim() != 1 or row_pos.numel() < rows or row_slot.numel() < rows:
         raise ValueError("page_table is [slots, pages], row_pos and row_slot have an entry per row")
-    if pool.dim() != 2 or not pool.is_contiguous() or pool.shape[1] != width or pool.shape[0] == 0 or pool.shape[0] % plan.page_tokens:
+    shape = pool.shape
+    if len(shape) != 2 or not pool.is_contiguous() or shape[1] != width or shape[0] == 0 or shape[0] % plan.page_tokens:
         raise ValueError(f"pool must be contiguous rows of {width} values, whole pages of {plan.page_tokens} of them")
-    if pool.shape[0] >= 1 << 31:
+    if shape[0] >= 1 << 31:
         raise ValueError("a pool has fewer than 2^31 rows")
-    if out.shape != (R, plan.heads, plan.vdim) or out.stride(2) != 1 or out.stride(1) != plan.vdim or out.stride(0) % 8:
-        raise ValueError(f"out must be [{R}, {plan.heads}, {plan.vdim}], a row's heads side by side and rows at multiples of 8 values")
-    if out.data_ptr() % 16:
-        raise ValueError("out must be 16-byte aligned")
-    here = torch.device("cuda", torch.cuda.current_device()) if plan.device.type == "cuda" and torch.cuda.is_available() else None
-    for name, t in (("pool", pool), ("out", out), ("page_table", page_table), ("row_pos", row_pos), ("row_slot", row_slot),
-                    ("plan", plan.data)) + named:
-        if t is not None and t.device != here:
+    if out.shape != (rows, plan.heads, plan.vdim):
+        raise ValueError(f"out must be [{rows}, {plan.heads}, {plan.vdim}]")
+    step, head, one = out.stride()
+    if one != 1 or head != plan.vdim or step % 8 or step < plan.heads * plan.vdim or out.data_ptr() % 16:
+        raise ValueError("out must be 16-byte aligned, a row's heads side by side and rows apart, at multiples of 8 values")
+    here = torch.cuda.current_device() if plan.device.type == "cuda" else None
+    for name, t, _ in tensors:
+        if t is not None and t.get_device() != here:
             raise ValueError(f"{name} is on {t.device}, not on the current CUDA device")
-    return R
 
 
-def _heads(name: str, q: torch.Tensor, heads: int, dtype):
-    if q.dim() != 3 or q.shape[1] != heads or q.dtype != dtype or q.shape[2] % 16 or q.shape[2] == 0:
+def _heads(name: str, q: torch.Tensor, heads: int, dtype) -> int:
+    shape = q.shape
+    if len(shape) != 3 or shape[1] != heads or q.dtype != dtype or shape[2] % 16 or shape[2] == 0:
         raise ValueError(f"{name} must be [rows, {heads}, a multiple of 16] of {dtype}")
-    if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16 or q.stride(0) < q.stride(1) * (heads - 1) + q.shape[2]:
+    row, head, one = q.stride()
+    if one != 1 or row % 8 or head % 8 or q.data_ptr() % 16 or row < head * (heads - 1) + shape[2]:
         raise ValueError(f"{name}: values of a head side by side, rows and heads at multiples of 8 values, 16-byte aligned")
+    return row
 
 
 def group_attend(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, row_pos: torch.Tensor, row_slot: torch.Tensor,
@@ -318,27 +319,24 @@ def group_attend(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, 
     q [rows, heads, dim]; pool [pages * page_tokens, kv_heads * (dim + vdim)]: keys of all key/value heads, then their values; row r
     stands at row_pos[r] of slot row_slot[r] (negative: the row's result is zero) and sees the positions up to its own, within its
     chunk of `chunk` of them where that is not 0.  `gate` [rows, heads] fp32: a head's result times sigmoid(gate)."""
-    _heads("q", q, plan.heads, plan.dtype)
+    ld_q, dtype = _heads("q", q, plan.heads, plan.dtype), plan.dtype
     R, H, D = q.shape
     if q.stride(1) != D:
         raise ValueError("q: a row's heads must lie side by side")
     if out is None:
-        out = torch.empty(R, H, plan.vdim, dtype=plan.dtype, device=q.device)
-    _check(plan, "grouped", q, pool, page_table, row_pos, row_slot, out, plan.kv_heads * (D + plan.vdim), scale,
-           (("q", q), ("gate", gate)))
+        out = torch.empty(R, H, plan.vdim, dtype=dtype, device=q.device)
+    _check(plan, "grouped", R, (("pool", pool, dtype), ("out", out, dtype), ("page_table", page_table, I32), ("row_pos", row_pos, I32),
+                                ("row_slot", row_slot, I32), ("q", q, dtype), ("gate", gate, F32), ("plan", plan.data, I32)),
+           pool, page_table, row_pos, row_slot, out, plan.kv_heads * (D + plan.vdim), scale)
     if chunk < 0:
         raise ValueError("chunk must not be negative")
     if gate is not None and (gate.shape != (R, H) or gate.stride(1) != 1):
         raise ValueError(f"gate must be [{R}, {H}] with a row's values side by side")
-    a = S.GroupAttendArgs()
-    a.q, a.pool, a.out, a.status = lib.ptr(q), lib.ptr(pool), lib.ptr(out), lib.ptr(plan.status)
-    a.page_table, a.row_pos, a.row_slot = lib.ptr(page_table), lib.ptr(row_pos), lib.ptr(row_slot)
-    a.gate = S.Proj(gate, gate.stride(0)).args() if gate is not None else S.NO_PROJ
-    a.u, a.taps, a.slots = S.NO_PROJ, 1, page_table.shape[0]
-    a.ld_q, a.ld_out, a.scale, a.chunk = q.stride(0), out.stride(0), scale, chunk
-    a.rows, a.heads, a.kv_heads, a.dim_pad, a.vdim_pad = R, H, plan.kv_heads, D, plan.vdim
-    a.max_pages, a.page_tokens, a.f32, a.n_pages = page_table.shape[1], plan.page_tokens, int(plan.dtype == F32), \
-        pool.shape[0] // plan.page_tokens
+    slots, max_pages = page_table.shape
+    a = S.GroupAttendArgs(q.data_ptr(), pool.data_ptr(), page_table.data_ptr(), row_pos.data_ptr(), row_slot.data_ptr(), out.data_ptr(),
+                          plan.status.data_ptr(), S.Proj(gate, gate.stride(0)).args() if gate is not None else S.NO_PROJ, S.NO_PROJ, None,
+                          ld_q, scale, R, H, plan.kv_heads, D, plan.vdim, chunk, 1, slots, 0, out.stride(0), max_pages, plan.page_tokens,
+                          int(dtype == F32), pool.shape[0] // plan.page_tokens, 0)
     launch_group(a, plan)
     return out
 
@@ -351,29 +349,30 @@ def latent_attend(q_abs: torch.Tensor, q_rot: Optional[torch.Tensor], pool: torc
     q_abs [rows, heads, latent], q_rot [rows, heads, rot] (None: no rotated part); pool [pages * page_tokens, latent + rot]: a
     position's latent, which is key and value of every head, and its rotated key part.  `sink` [heads] fp32: an extra logit in a
     head's denominator."""
-    _heads("q_abs", q_abs, plan.heads, plan.dtype)
+    ld_abs, dtype = _heads("q_abs", q_abs, plan.heads, plan.dtype), plan.dtype
     R, H, V = q_abs.shape
     if V != plan.vdim:
         raise ValueError(f"q_abs: {V} latent values, the plan has {plan.vdim}")
     if q_abs.stride(1) != V:
         raise ValueError("q_abs: a row's heads must lie side by side")
+    rot = ld_rot = rot_head = 0
     if q_rot is not None:
-        _heads("q_rot", q_rot, H, plan.dtype)
+        ld_rot = _heads("q_rot", q_rot, H, dtype)
         if q_rot.shape[0] != R:
             raise ValueError("q_rot must have as many rows as q_abs")
-    rot = 0 if q_rot is None else q_rot.shape[2]
+        rot, rot_head = q_rot.shape[2], q_rot.stride(1)
     if out is None:
-        out = torch.empty(R, H, V, dtype=plan.dtype, device=q_abs.device)
-    _check(plan, "latent", q_abs, pool, page_table, row_pos, row_slot, out, V + rot, scale,
-           (("q_abs", q_abs), ("q_rot", q_rot), ("sink", sink)))
+        out = torch.empty(R, H, V, dtype=dtype, device=q_abs.device)
+    _check(plan, "latent", R, (("pool", pool, dtype), ("out", out, dtype), ("page_table", page_table, I32), ("row_pos", row_pos, I32),
+                               ("row_slot", row_slot, I32), ("q_abs", q_abs, dtype), ("q_rot", q_rot, dtype), ("sink", sink, F32),
+                               ("plan", plan.data, I32)),
+           pool, page_table, row_pos, row_slot, out, V + rot, scale)
     if sink is not None and (sink.shape != (H,) or not sink.is_contiguous()):
         raise ValueError(f"sink must be {H} contiguous values")
     a = S.LatentAttendArgs()
-    a.q_abs, a.ld_q_abs = lib.ptr(q_abs), q_abs.stride(0)
-    if q_rot is not None:
-        a.q_rot, a.ld_q_rot, a.q_rot_stride = lib.ptr(q_rot), q_rot.stride(0), q_rot.stride(1)
-    a.pool, a.page_table, a.row_pos, a.row_slot = lib.ptr(pool), lib.ptr(page_table), lib.ptr(row_pos), lib.ptr(row_slot)
+    a.q_abs, a.ld_q_abs, a.q_rot, a.ld_q_rot, a.q_rot_stride = q_abs.data_ptr(), ld_abs, q_rot.data_ptr() if rot else None, ld_rot, rot_head
+    a.pool, a.page_table, a.row_pos, a.row_slot = pool.data_ptr(), page_table.data_ptr(), row_pos.data_ptr(), row_slot.data_ptr()
     a.scale, a.rows, a.heads, a.kv_pad, a.row_len = scale, R, H, V, V + rot
-    a.max_pages, a.page_tokens, a.f32, a.status = page_table.shape[1], plan.page_tokens, int(plan.dtype == F32), lib.ptr(plan.status)
+    a.max_pages, a.page_tokens, a.f32, a.status = page_table.shape[1], plan.page_tokens, int(dtype == F32), plan.status.data_ptr()
     launch_latent(a, plan, pool.shape[0] // plan.page_tokens, sink, out, out.stride(0))
     return out
