@@ -490,6 +490,9 @@ def cmd_serve(args) -> int:
         if wanted:
             print(f"{cfg.name}: {', '.join(wanted)} not available for {fam.name} models", file=sys.stderr)
             return 2
+    if args.shared_prefix and not fam.shared_prefix:
+        print(f"{cfg.name}: --shared-prefix not available for {fam.name} models", file=sys.stderr)
+        return 2
     fabric = Fabric.create() if "WORLD_SIZE" in os.environ else Fabric.single(torch.device("cuda", args.device))
     rank, world, dev = fabric.rank, fabric.world, fabric.device
     ctl = make_control_group(fabric)
@@ -512,7 +515,8 @@ def cmd_serve(args) -> int:
         print(f"rank {rank}: only {n_pages} KV pages fit; lower --max-context or --concurrency", file=sys.stderr)
         return 2
     eng = fam.engine(cfg, weights, fabric, max_rows=max(8, args.concurrency, args.prefill_chunk), slots=args.concurrency,
-                     max_ctx=args.max_context, kv_dtype=args.kv_dtype, n_pages=n_pages)
+                     max_ctx=args.max_context, kv_dtype=args.kv_dtype, n_pages=n_pages,
+                     **({"shared_prefix": True} if args.shared_prefix else {}))
     engram_layers = _attach_engram(args, cfg, eng, dev)
     hb = None
     if world > 1:
@@ -665,6 +669,8 @@ def main(argv=None) -> int:
     ps.add_argument("--vision", action="store_true",
                     help="accept image parts in chat messages: vision tower from the checkpoint (or a small random one "
                          "for a random-init model); one-rank serving")
+    ps.add_argument("--shared-prefix", action="store_true",
+                    help="layer-stack models: attention reads the cache pages that active requests have in common once for all of them")
     ps.add_argument("--speculative", action="store_true",
                     help="decode with dSpark draft + verify rounds: a lone request, or up to four active requests sharing "
                          "a round (random-init drafter unless the checkpoint provides one)")

@@ -103,6 +103,10 @@ class RowsEngine:
     def sp_rows(self, n: int) -> int:
         return n
 
+    def describe(self, positions, slots):
+        """What the rows of the passes to come are, for engines that plan by it.  set_rows() calls it; whoever hands the rows to the
+        device in another way does so before the pass."""
+
     # ------------------------------------------------------------------ graphs
     @contextlib.contextmanager
     def rehearsal(self):

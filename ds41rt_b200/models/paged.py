@@ -21,6 +21,7 @@ class PagedSlots:
         self.page_table = self.page_table_host.to(device)
         from ..runtime import core as K
         self.alloc = K.KvAllocator(self.n_pages, slots, page_tokens)
+        self.version = 0      # counts leases that begin or end; pages appended to a lease are not counted
 
     @property
     def free_pages(self) -> int:
@@ -44,6 +45,7 @@ class PagedSlots:
     def _publish(self, slot: int, first: int = 0):
         pages = self.alloc.pages(slot)
         n = len(pages)
+        self.version += first == 0
         if n > first:
             self.page_table_host[slot, first:n] = torch.tensor(pages[first:], dtype=I32)
             self.page_table[slot, first:n].copy_(self.page_table_host[slot, first:n], non_blocking=True)
@@ -68,6 +70,7 @@ class PagedSlots:
         g = self.alloc.generation(slot)
         if g:
             self.alloc.retire(slot, g)
+        self.version += 1
         self.page_table_host[slot].fill_(-1)
         self.page_table[slot].fill_(-1)
 

@@ -18,6 +18,7 @@ class Family:
     name = ""
     presets: tuple = ()
     dtypes: tuple = ("bf16",)
+    shared_prefix = False     # do its engines take `shared_prefix`?
 
     def matches(self, doc: dict) -> bool:
         raise NotImplementedError
@@ -68,6 +69,7 @@ class DS41Family(Family):
 class StackFamily(Family):
     """Layer-stack models (models/stack.py); `module` reads the family's configuration and names its tensors."""
     dtypes = ("bf16", "f32")
+    shared_prefix = True
 
     def __init__(self, name: str, module):
         self.name, self.module, self.presets = name, module, module.PRESETS

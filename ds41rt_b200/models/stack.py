@@ -19,7 +19,7 @@ import numpy as np
 import torch
 
 from ..config import rope_inv_freq
-from ..ops import lib
+from ..ops import lib, prefix
 from ..ops import stack as S
 from ..ops.stack import Matrix, Proj, ceil_to
 from ..stack_config import GroupedAttentionSpec, LatentAttentionSpec, MLSTMSpec, MoESpec, StackConfig
@@ -223,6 +223,9 @@ class LatentAttention:
         a.n_keys, a.pos0, a.ld_out = n, n - R, H * self.vp
         e._run("latent_prefill", k.ds41_latent_prefill, C.byref(a), lib.stream())
 
+    def prefix_shape(self):
+        return "latent", self.spec.heads, 1, self.kvp
+
     def _absorbed(self, e: "StackEngine", R: int, ldq: int, pool, gate: Proj):
         sp, k, H = self.spec, e.k, self.spec.heads
         q = e.q.view(-1)
@@ -232,6 +235,7 @@ class LatentAttention:
             e._run("absorb_q", S.per_head, qr, ldq, self.hs, n, H, self.w_ukt, self.kvp, self.dp, self.dp, e.q_abs,
                    H * self.kvp, e.status)
             splits = e.attn_splits(n, H)
+            plan = e.prefix_plan(self, R)
             a = S.LatentAttendArgs()
             a.q_abs, a.ld_q_abs = e.q_abs.data_ptr(), H * self.kvp
             a.q_rot, a.ld_q_rot, a.q_rot_stride = qr[self.dp:].data_ptr(), ldq, self.hs
@@ -240,9 +244,12 @@ class LatentAttention:
             a.part_o, a.part_ml = e.part_o.data_ptr(), e.part_ml.data_ptr()
             a.scale, a.rows, a.heads, a.kv_pad, a.row_len, a.n_splits = sp.scale, n, H, self.kvp, self.row_len, splits
             a.max_pages, a.page_tokens, a.f32, a.status = e.cache.max_pages, e.cache.page_tokens, e.f32, lib.ptr(e.status)
-            e._run("latent_attend", k.ds41_latent_attend, C.byref(a), lib.stream())
-            e._run("latent_merge", k.ds41_latent_merge, lib.ptr(e.part_o), lib.ptr(e.part_ml), lib.ptr(self.sink), splits, n,
-                   H, self.kvp, lib.ptr(e.o_lat), H * self.kvp, e.f32, lib.stream())
+            if plan is not None:
+                e._run("prefix_attend", prefix.launch_latent, a, plan, e.cache.n_pages, self.sink, e.o_lat, H * self.kvp)
+            else:
+                e._run("latent_attend", k.ds41_latent_attend, C.byref(a), lib.stream())
+                e._run("latent_merge", k.ds41_latent_merge, lib.ptr(e.part_o), lib.ptr(e.part_ml), lib.ptr(self.sink), splits, n,
+                       H, self.kvp, lib.ptr(e.o_lat), H * self.kvp, e.f32, lib.stream())
             o = e.o_heads.view(-1)[r0 * H * self.vp:]
             e._run("values", S.per_head, e.o_lat, H * self.kvp, self.kvp, n, H, self.w_uv, self.vp, self.kvp, self.kvp, o,
                    H * self.vp, e.status)
@@ -340,6 +347,9 @@ class GroupedAttention:
     def matrices(self):
         return {"a": [(self.w_in.n, self.w_in.k)], "b": [(self.w_o.n, self.w_o.k)]}
 
+    def prefix_shape(self):
+        return "grouped", self.spec.heads, self.spec.kv_heads, self.vp
+
     def splits(self, e: "StackEngine", rows: int) -> int:
         """CTAs that share a row's keys: enough to fill the GPU, static per batch size (a captured pass replays while the
         context grows)."""
@@ -377,6 +387,8 @@ class GroupedAttention:
         if long:
             b.pos0, b.n_splits = long - R, 1
             e._run("group_prefill", k.ds41_group_prefill, C.byref(b), lib.stream())
+        elif e.prefix_plan(self, R) is not None:
+            e._run("prefix_attend", prefix.launch_group, b, e.prefix_plan(self, R))
         else:
             b.n_splits = self.splits(e, R)
             e._run("group_attend", k.ds41_group_attend, C.byref(b), lib.stream())
@@ -595,7 +607,8 @@ class StackEngine(RowsEngine):
     taps = None
 
     def __init__(self, cfg: StackConfig, weights: StackWeights, *, max_rows: int = 8, slots: int = 1, max_ctx: int = 4096,
-                 page_tokens: int = 64, n_pages: Optional[int] = None, moe_rows: int = 32):
+                 page_tokens: int = 64, n_pages: Optional[int] = None, moe_rows: int = 32,
+                 shared_prefix: bool = False):
         self.cfg, self.w, self.device = cfg, weights, weights.device
         self.rank, self.world = 0, 1
         self.max_rows = R = max_rows
@@ -661,6 +674,7 @@ class StackEngine(RowsEngine):
             self.q_abs, self.o_lat = z((self.attn_rows * lat,), dt), z((self.attn_rows * lat,), dt)
             self.part_o, self.part_ml = z((cells,), F32), z((cells // 8 + 2,), F32)
         self._init_experts(R, moe_rows, z, dt)
+        self._init_prefix_plans(shared_prefix)
         # head
         self.head_cap = min(R, 64)
         self.last_head_row = 0
@@ -688,6 +702,39 @@ class StackEngine(RowsEngine):
         size = lambda f: max([n * Rm * f(m) for n, m in live if m is not None], default=8)
         self.moe_act, self.moe_out = z((size(lambda m: m.ffp),), dt), z((size(lambda m: m.ld),), F32)
         self.moe_up = z((size(lambda m: 2 * m.ffp) if self.f32 else 8,), F32)
+
+    def _init_prefix_plans(self, shared_prefix: bool):
+        """`shared_prefix`: passes of up to `attn_rows` rows read the pages that requests have in common once for all of them, by a
+        plan per shape of attention that follows the rows and their leases.  32-bit passes read them row by row."""
+        self.prefix_plans: Dict[tuple, prefix.PrefixPlan] = {}
+        self._planned, self._plan_until = None, 0
+        if not shared_prefix or self.f32:
+            return
+        for lw in self.w.layers:
+            if not hasattr(lw.mixer, "prefix_shape"):
+                continue
+            kind, heads, kv_heads, vdim = key = lw.mixer.prefix_shape()
+            if key not in self.prefix_plans:
+                self.prefix_plans[key] = prefix.PrefixPlan(kind, rows=self.attn_rows, heads=heads, kv_heads=kv_heads, vdim=vdim,
+                                                           page_tokens=self.cache.page_tokens, device=self.device)
+
+    def prefix_plan(self, mixer, rows: int) -> Optional[prefix.PrefixPlan]:
+        """Static per batch size, as a captured pass needs it: the plan's contents follow the rows."""
+        return self.prefix_plans.get(mixer.prefix_shape()) if self.prefix_plans and rows <= self.attn_rows else None
+
+    def describe(self, positions, slots):
+        """Plans hold as long as the rows belong to the same leases; they are also renewed as requests grow, for the sake of an even
+        division."""
+        if not self.prefix_plans:
+            return
+        n = min(len(slots), self.attn_rows)
+        slots, positions = [int(s) for s in slots[:n]], [int(p) for p in positions[:n]]
+        key, last = (slots, self.cache.version), max(positions, default=0)
+        if key == self._planned and last < self._plan_until:
+            return
+        for plan in self.prefix_plans.values():
+            plan.set(slots, self.cache.page_table_host, [p + 1 for p in positions])
+        self._planned, self._plan_until = key, last + 256
 
     def max_active(self, m: MoESpec) -> int:
         """Most experts that a planned pass can use."""
@@ -753,6 +800,7 @@ class StackEngine(RowsEngine):
             self.in_tokens.copy_(row_values(tokens, self.max_rows, 0), non_blocking=True)
         self.row_pos.copy_(pos, non_blocking=True)
         self.row_slot.copy_(slot, non_blocking=True)
+        self.describe(p, s)
 
     def _resid(self, R: int, *, y: Optional[Proj] = None, gate: Optional[Proj] = None, bias=None, post=None, x_in=None,
                x_out=None, layer: Optional[int] = None, next_w=None, post_rms: bool = False):

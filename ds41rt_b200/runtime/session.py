@@ -67,6 +67,7 @@ class DecodeSession:
             except (TypeError, ValueError, OverflowError):       # other numbers, or one for all rows
                 self._in[i * n:(i + 1) * n] = whole_numbers(values)
         self.h2d_bytes += 3 * 4 * n
+        e.describe(self._in[n:2 * n], self._in[2 * n:3 * n])
         g = self.graph(n)
         src, dst, s = lib.ptr(self.h_in), lib.ptr(self.h_chosen), lib.stream()
         rows = (lib.ptr(e.in_tokens), lib.ptr(e.row_pos), lib.ptr(e.row_slot))

@@ -241,3 +241,69 @@ def test_grouped_calls_refuse(change):
 def test_latent_calls_refuse(change):
     with pytest.raises(ValueError):
         call("latent", **change)
+
+
+class Leases:
+    """What StackEngine.describe() asks of an engine and its cache."""
+    from ds41rt_b200.models.stack import StackEngine
+    describe = StackEngine.describe
+
+    def __init__(self):
+        from ds41rt_b200.models.paged import PagedSlots
+        self.cache = PagedSlots()
+        self.cache._init_pages(4, 1024, "cpu", 64, 40)
+        self.attn_rows, self._planned, self._plan_until = 3, None, 0
+        self.prefix_plans = {"x": PrefixPlan("grouped", rows=3, heads=4, kv_heads=2, vdim=16, page_tokens=64, device="cpu")}
+        self.plan, self.sets = self.prefix_plans["x"], 0
+        real = self.plan.set
+
+        def counted(*a):
+            self.sets += 1
+            real(*a)
+        self.plan.set = counted
+
+    def share(self, slot, n):
+        """A lease of the first n pages of slot 0."""
+        pages = self.cache.alloc.retain(0, self.cache._gen(0), n)
+        self.cache.alloc.share(slot, self.cache._gen(slot), pages)
+        self.cache._publish(slot)
+
+
+def test_plans_of_an_engine_follow_its_rows_and_their_leases():
+    e = Leases()
+    assert e.cache.ensure(0, 300)
+    e.share(1, 3)
+    e.share(2, 2)
+    assert e.cache.ensure(1, 400) and e.cache.ensure(2, 400)
+    e.describe([300, 301, 302], [0, 1, 2])
+    assert e.sets == 1 and e.plan.shared == [([0, 1, 2], 128)]
+    e.describe(np.array([301, 302, 303]), np.array([0, 1, 2]))         # the same requests a step later
+    assert e.cache.ensure(0, 700)                                      # pages appended to a lease
+    e.describe([302, 303, 304], [0, 1, 2])
+    assert e.sets == 1
+    e.describe([600, 303, 304], [0, 1, 2])                             # longer by a few tiles
+    assert e.sets == 2
+    e.describe([601, 304], [0, 1])
+    assert e.sets == 3 and e.plan.shared == [([0, 1], 192)]
+    e.describe([304, 601], [1, 0])
+    assert e.sets == 4
+    e.cache.release(1)                                                 # the slot's next request shares nothing
+    assert e.cache.ensure(1, 400)
+    e.describe([304, 601], [1, 0])
+    assert e.sets == 5 and e.plan.shared == []
+    e.describe([1, 2, 3, 4], [0, 0, 0, 0])                             # more rows than passes of this form have
+    assert e.sets == 6 and int(e.plan.data[e.plan._at[4]:].count_nonzero()) == 3
+    e.describe([], [])
+    assert e.plan.n_units == 0
+
+
+def test_engines_without_plans_ignore_the_rows():
+    e = Leases()
+    e.prefix_plans = {}
+    e.describe([1], [0])
+    assert e.sets == 0
+
+
+def test_only_layer_stacks_are_served_with_shared_prefixes():
+    from ds41rt_b200.models.registry import FAMILIES
+    assert {n for n, f in FAMILIES.items() if f.shared_prefix} == {"genesun", "belasun"}
