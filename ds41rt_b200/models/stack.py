@@ -604,6 +604,7 @@ class StackEngine(RowsEngine):
     partial_prefix = False        # recurrent states belong to a snapshot's whole length
     replay_window = 1 << 30       # the prefix banks then never prefer a truncated snapshot
     engram: dict = {}
+    prefix_plans: Dict[tuple, prefix.PrefixPlan] = {}      # by shape of attention, of engines made with `shared_prefix`
     taps = None
 
     def __init__(self, cfg: StackConfig, weights: StackWeights, *, max_rows: int = 8, slots: int = 1, max_ctx: int = 4096,
@@ -706,7 +707,7 @@ class StackEngine(RowsEngine):
     def _init_prefix_plans(self, shared_prefix: bool):
         """`shared_prefix`: passes of up to `attn_rows` rows read the pages that requests have in common once for all of them, by a
         plan per shape of attention that follows the rows and their leases.  32-bit passes read them row by row."""
-        self.prefix_plans: Dict[tuple, prefix.PrefixPlan] = {}
+        self.prefix_plans = {}
         self._planned, self._plan_until = None, 0
         if not shared_prefix or self.f32:
             return

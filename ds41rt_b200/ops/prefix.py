@@ -171,17 +171,15 @@ class PrefixPlan:
             at += len(rows)
         best = None
         if tails:
-            unit, most = ceil_to(128, self.page_tokens), sum(pieces) + len(tails) + self.extra
-            longest = max([tokens for _, tokens in self.shared] + [t[3] for t in tails])
-            for span in self._spans(longest, unit):
-                if sum(p * -(-x[1] // span) for p, x in zip(pieces, self.shared)) + sum(max(1, x[3] // span) for x in tails) <= most:
+            ends = {x[0]: x[2] + x[3] for x in tails}
+            for least, span in self._spans(pieces, tails):
+                if best is None or least < best[0]:
                     items, n_parts = self._items(slots, pieces, tails, limit, span)
-                    every, need = self._pairs(items, {x[0]: x[2] + x[3] for x in tails})
-                    join = 8 * int(n_parts.sum()) * self.heads * self.vdim * self.cost.byte + int(n_parts.max()) * self.cost.part
-                    if best is None or max(need.sum() / self.grid, need.max()) + join < best[0]:
-                        place, time = self._deal(need)
-                        if best is None or time + join < best[0]:
-                            best = (time + join, span, every, place, n_parts)
+                    every, need = self._pairs(items, ends)
+                    place, time = self._deal(need)
+                    time += self._join_time(int(n_parts.sum()), int(n_parts.max()))
+                    if best is None or time < best[0]:
+                        best = (time, span, every, place, n_parts)
         n = 0
         self.span = 0
         if best is not None:
@@ -195,8 +193,25 @@ class PrefixPlan:
         host[0] = self.n_units = n
         self.data.copy_(torch.from_numpy(host))
 
-    def _spans(self, longest: int, unit: int) -> List[int]:
-        return [k * unit for k in SPANS if k * unit < longest] + [ceil_to(longest, unit)]        # the last one divides nothing
+    def _join_time(self, parts: int, most: int) -> float:
+        return 8 * parts * self.heads * self.vdim * self.cost.byte + most * self.cost.part
+
+    def _spans(self, pieces, tails) -> List[Tuple[float, int]]:
+        """Lengths that the keys may be divided by: the time that a plan with it takes at least, length; the shortest time first."""
+        p, rows, tokens, n, keys = (np.array(x, dtype=np.int64) for x in (
+            pieces, [len(x) for x, _ in self.shared], [x for _, x in self.shared], [x[1] for x in tails], [x[3] for x in tails]))
+        longest, unit, cost = int(max(tokens.max(initial=0), keys.max())), ceil_to(128, self.page_tokens), self.cost
+        at_a_time = self.grid * self.together / self.kv_heads
+        per_key = cost.longer if self.together == 1 else (cost.longer + cost.shorter) / 2
+        out = []
+        for span in [k * unit for k in SPANS if k * unit < longest] + [ceil_to(longest, unit)]:      # the last one divides nothing
+            shared, own = -(-tokens // span), np.maximum(1, keys // span)
+            items = int((p * shared).sum() + own.sum())
+            if items <= len(tails) + sum(pieces) + self.extra:
+                busy = (items * cost.turn + float((p * tokens).sum() + keys.sum()) * per_key) / at_a_time
+                last = cost.turn + cost.longer * min(span, longest)
+                out.append((max(busy, last) + self._join_time(int((rows * shared).sum() + (n * own).sum()), 0), span))
+        return sorted(out)
 
     def _items(self, slots: np.ndarray, pieces, tails, limit: int, span: int) -> Tuple[np.ndarray, np.ndarray]:
         """What there is to do with at most `span` keys at a time, as units without their head, and the partial results of every row."""
