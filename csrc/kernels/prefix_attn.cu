@@ -1,8 +1,10 @@
 // Attention of rows that share prefixes: its parts for every type and size, and their join.
 //
 // A block takes sixteen queries (head and row) of a unit and walks its keys 32 at a time through shared memory, so that a cached
-// value that was read once serves sixteen queries: scores by 256 threads of two (query, key) pairs each, a softmax state per query
-// (running maximum and sum), results in registers.  It serves 32-bit rows and the sizes that the tensor-core forms
+// value that was read once serves sixteen queries: scores by warps of 8 queries x 8 keys (6 rows of 16 heads and 576 values over 500 keys
+// in 32 bits: 25 us, 46 with two pairs to a thread, which narrow rows take: 64 and 46 us with 32 values), a softmax state per query
+// (running maximum and sum), results in registers.  A warp fetches four of the keys, whose places it looks up a tile ahead; values that
+// are a part of their key (a latent) are fetched once.  It serves 32-bit rows and the sizes that the tensor-core forms
 // (prefix_group.cu, prefix_latent.cu) leave out, and is bound by its 32-bit products and their operands from shared memory.
 #include "ds41_group.cuh"
 #include "ds41_prefix.cuh"
@@ -15,6 +17,7 @@ int launch_prefix_latent(const ds41_latent_attend_args& a, const ds41_prefix_pla
 
 constexpr int kSimpleQueries = 16;
 constexpr int kSimpleKeys = 32;
+constexpr int kSimpleLd = kSimpleQueries + 4;      // of the weights: a key's lie side by side, four of them in one load
 
 struct SimpleArgs {
   const void *q, *q2, *pool;         // a query is [d1 values of q | d2 of q2]
@@ -23,13 +26,14 @@ struct SimpleArgs {
   int q_head, q2_head;               // values between a row's heads
   int d1, d2, vp, row_len;
   int k_lane, v_at, v_lane;          // key / value head g of a cache row: keys at g * k_lane, values at v_at + g * v_lane
+  int inside;                        // the values are the first values of the key
   int lanes, per_lane, heads, chunk, max_pages, page_tokens;
   float scale;
 };
 
 inline int simple_smem(const SimpleArgs& p) {
   const int dp = p.d1 + p.d2;
-  return 4 * (kSimpleQueries * (dp + 4) + kSimpleKeys * (dp + 4) + kSimpleKeys * p.vp + kSimpleQueries * (kSimpleKeys + 1)) +
+  return 4 * (kSimpleQueries * (dp + 4) + kSimpleKeys * (dp + 4) + (p.inside ? 0 : kSimpleKeys * p.vp) + kSimpleKeys * kSimpleLd) +
          16 * kSimpleQueries;
 }
 
@@ -40,16 +44,17 @@ __device__ __forceinline__ float4 four(const __nv_bfloat16* p) {
                      __uint_as_float(v.y & 0xffff0000u));
 }
 
-// QPT: queries whose columns a thread accumulates
-template <typename T, int QPT>
-__global__ void __launch_bounds__(256) prefix_simple_kernel(const SimpleArgs p, const ds41_prefix_plan plan) {
+// QPT: queries whose columns a thread accumulates.  WIDE: rows of more than 64 values.
+template <typename T, int QPT, bool WIDE>
+__global__ void __launch_bounds__(256, QPT <= 4 ? 2 : 1) prefix_simple_kernel(const SimpleArgs p, const ds41_prefix_plan plan) {
   extern __shared__ __align__(16) float ps_smem[];
   const int dp = p.d1 + p.d2, ds = dp + 4, nc = p.vp / 4;
   float* qs = ps_smem;                                        // [16][ds]
   float* ks = qs + kSimpleQueries * ds;                       // [32][ds]
-  float* vs = ks + kSimpleKeys * ds;                          // [32][vp]
-  float* sc = vs + kSimpleKeys * p.vp;                        // [16][33] scores, then weights
-  float* ms = sc + kSimpleQueries * (kSimpleKeys + 1);        // [16] maxima
+  float* vs = p.inside ? ks : ks + kSimpleKeys * ds;          // [32][vs_ld]
+  const int vs_ld = p.inside ? ds : p.vp;
+  float* sc = p.inside ? ks + kSimpleKeys * ds : vs + kSimpleKeys * p.vp;      // [32][20] scores, then weights
+  float* ms = sc + kSimpleKeys * kSimpleLd;                   // [16] maxima
   float* ls = ms + kSimpleQueries;                            // [16] sums
   float* keep = ls + kSimpleQueries;                          // [16] factor on what was summed before
   int* lim = reinterpret_cast<int*>(keep + kSimpleQueries);   // [16] end of what a query sees
@@ -58,10 +63,12 @@ __global__ void __launch_bounds__(256) prefix_simple_kernel(const SimpleArgs p, 
   pdl_launch_dependents();
   pdl_wait();
   const int subs = (plan.rows_per_unit * p.per_lane + kSimpleQueries - 1) / kSimpleQueries;
-  const int units = *plan.n_units * subs;
-  for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
-    const PrefixUnit it = prefix_unit(plan, unit / subs);
-    const int g = it.head, i0 = unit % subs * kSimpleQueries, count = it.rows * p.per_lane;
+  // every unit's first sixteen queries, then the second sixteen of those that have them: a block's next ones are not always the ones
+  // that only full units have
+  const int places = *plan.n_units;
+  for (int unit = blockIdx.x; unit < places * subs; unit += gridDim.x) {
+    const PrefixUnit it = prefix_unit(plan, unit % places);
+    const int g = it.head, i0 = unit / places * kSimpleQueries, count = it.rows * p.per_lane;
     if (i0 >= count) continue;
     __syncthreads();                     // the last unit's shared memory is no longer read
     if (tid < kSimpleQueries) {
@@ -81,13 +88,13 @@ __global__ void __launch_bounds__(256) prefix_simple_kernel(const SimpleArgs p, 
       ls[tid] = 0.f;
     }
     __syncthreads();
-    for (int i = 4 * tid; i < kSimpleQueries * dp; i += 1024) {
-      const int u = i / dp, d = i % dp, r = row_of[u], h = g * p.per_lane + (i0 + u) % p.per_lane;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (r >= 0)
-        v = d < p.d1 ? four(static_cast<const T*>(p.q) + r * p.ld_q + 1ll * h * p.q_head + d)
-                     : four(static_cast<const T*>(p.q2) + r * p.ld_q2 + 1ll * h * p.q2_head + (d - p.d1));
-      *reinterpret_cast<float4*>(qs + u * ds + d) = v;
+    for (int u = warp; u < kSimpleQueries; u += 8) {
+      const int r = row_of[u], h = g * p.per_lane + (i0 + u) % p.per_lane;
+      const T* q = static_cast<const T*>(p.q) + r * p.ld_q + 1ll * h * p.q_head;
+      const T* q2 = static_cast<const T*>(p.q2) + r * p.ld_q2 + 1ll * h * p.q2_head - p.d1;
+#pragma unroll 4
+      for (int d = 4 * lane; d < dp; d += 128)
+        *reinterpret_cast<float4*>(qs + u * ds + d) = r >= 0 ? four((d < p.d1 ? q : q2) + d) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     int from = INT_MAX, to = 0;
 #pragma unroll
@@ -100,38 +107,89 @@ __global__ void __launch_bounds__(256) prefix_simple_kernel(const SimpleArgs p, 
 #pragma unroll
     for (int u = 0; u < QPT; ++u) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
     const int col = tid % nc, u0 = tid / nc * QPT;
+    auto row_at = [&](int key) {           // pool row of a key, -1: none
+      const int pg = key / p.page_tokens;
+      const int id = key >= from && key < to && pg < p.max_pages ? p.page_table[1ll * it.slot * p.max_pages + pg] : -1;
+      return id >= 0 ? id * p.page_tokens + (key - pg * p.page_tokens) : -1;
+    };
+    int next = lane < 4 && from < to ? row_at(from + warp + 8 * lane) : -1;
+    const T* pool_k = static_cast<const T*>(p.pool) + g * p.k_lane;
+    const T* pool_v = static_cast<const T*>(p.pool) + p.v_at + g * p.v_lane;
     for (int t0 = from; t0 < to; t0 += kSimpleKeys) {
       __syncthreads();
-      for (int i = 4 * tid; i < kSimpleKeys * (dp + p.vp); i += 1024) {
-        const int j = i / (dp + p.vp), d = i % (dp + p.vp), key = t0 + j, pg = key / p.page_tokens;
-        const int id = key < to && pg < p.max_pages ? p.page_table[1ll * it.slot * p.max_pages + pg] : -1;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (id >= 0) {
-          const T* row = static_cast<const T*>(p.pool) + (1ll * id * p.page_tokens + (key - pg * p.page_tokens)) * p.row_len;
-          v = four(d < dp ? row + g * p.k_lane + d : row + p.v_at + g * p.v_lane + (d - dp));
-        }
-        *reinterpret_cast<float4*>(d < dp ? ks + j * ds + d : vs + j * p.vp + (d - dp)) = v;
+      long long at[4];
+      bool there[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int row = __shfl_sync(0xffffffffu, next, k);
+        there[k] = row >= 0;
+        at[k] = 1ll * row * p.row_len;
       }
+      auto fetch = [&](const T* src, float* dst, int ld, int width) {
+#pragma unroll 2
+        for (int d = 4 * lane; d < width; d += 128) {
+          float4 v[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[k] = there[k] ? four(src + at[k] + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) *reinterpret_cast<float4*>(dst + (warp + 8 * k) * ld + d) = v[k];
+        }
+      };
+      fetch(pool_k, ks, ds, dp);
+      if (!p.inside) fetch(pool_v, vs, vs_ld, p.vp);
+      next = lane < 4 ? row_at(t0 + kSimpleKeys + warp + 8 * lane) : -1;
       __syncthreads();
-      {
+      if constexpr (!WIDE) {             // a thread's two keys of a query: narrow rows leave most lanes of the other form without columns
         const int u = tid >> 4, j = tid & 15;
         float a = 0.f, b = 0.f;
+#pragma unroll 4
         for (int d = 0; d < dp; d += 4) {
           const float4 x = four(qs + u * ds + d), y = four(ks + j * ds + d), z = four(ks + (j + 16) * ds + d);
           a += x.x * y.x + x.y * y.y + x.z * y.z + x.w * y.w;
           b += x.x * z.x + x.y * z.y + x.z * z.z + x.w * z.w;
         }
         const int key = t0 + j;
-        sc[u * 33 + j] = key >= low[u] && key < lim[u] ? a * p.scale : -INFINITY;
-        sc[u * 33 + j + 16] = key + 16 >= low[u] && key + 16 < lim[u] ? b * p.scale : -INFINITY;
+        sc[j * kSimpleLd + u] = key >= low[u] && key < lim[u] ? a * p.scale : -INFINITY;
+        sc[(j + 16) * kSimpleLd + u] = key + 16 >= low[u] && key + 16 < lim[u] ? b * p.scale : -INFINITY;
+      } else {
+        // a warp's 8 queries x 8 keys, the columns by lane: 16 loads for 256 products, then the lanes' sums are added and shared out
+        const float *x = qs + (warp & 1) * 8 * ds, *y = ks + (warp >> 1) * 8 * ds;
+        float s[64];
+#pragma unroll
+        for (int i = 0; i < 64; ++i) s[i] = 0.f;
+#pragma unroll 1
+        for (int d = 4 * lane; d < dp; d += 128) {
+          float4 q[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) q[u] = four(x + u * ds + d);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float4 k = four(y + j * ds + d);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s[8 * u + j] += q[u].x * k.x + q[u].y * k.y + q[u].z * k.z + q[u].w * k.w;
+          }
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1)
+#pragma unroll
+          for (int i = 0; i < 2 * o; ++i) {
+            const bool up = lane & o;
+            const float mine = up ? s[i + 2 * o] : s[i], other = up ? s[i] : s[i + 2 * o];
+            s[i] = mine + __shfl_xor_sync(0xffffffffu, other, o);
+          }
+        // this lane's: query lane / 4, keys 2 (lane % 4) and the next
+        const int u = (warp & 1) * 8 + (lane >> 2), j = (warp >> 1) * 8 + 2 * (lane & 3);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          sc[(j + i) * kSimpleLd + u] = t0 + j + i >= low[u] && t0 + j + i < lim[u] ? s[i] * p.scale : -INFINITY;
       }
       __syncthreads();
       for (int u = 2 * warp; u < 2 * warp + 2; ++u) {
-        const float s = sc[u * 33 + lane], top = fmaxf(ms[u], warp_max(s));
+        const float s = sc[lane * kSimpleLd + u], top = fmaxf(ms[u], warp_max(s));
         const float e = s == -INFINITY ? 0.f : expf(s - top);
         const float f = ms[u] == -INFINITY ? 0.f : expf(ms[u] - top), sum = warp_sum(e);
         __syncwarp();
-        sc[u * 33 + lane] = e;
+        sc[lane * kSimpleLd + u] = e;
         if (lane == 0) {
           ls[u] = ls[u] * f + sum;
           ms[u] = top;
@@ -148,18 +206,25 @@ __global__ void __launch_bounds__(256) prefix_simple_kernel(const SimpleArgs p, 
           acc[u].z *= f;
           acc[u].w *= f;
         }
+#pragma unroll 4
         for (int j = 0; j < kSimpleKeys; ++j) {
-          const float4 v = four(vs + j * p.vp + 4 * col);
+          const float4 v = four(vs + j * vs_ld + 4 * col);
+          alignas(16) float w[QPT];
+          if constexpr (QPT >= 4) {
 #pragma unroll
-          for (int u = 0; u < QPT; ++u) {
-            const float w = sc[(u0 + u) * 33 + j];
-            if (w != 0.f) {              // what a query does not see may be anything
-              acc[u].x += w * v.x;
-              acc[u].y += w * v.y;
-              acc[u].z += w * v.z;
-              acc[u].w += w * v.w;
-            }
+            for (int u = 0; u < QPT; u += 4) *reinterpret_cast<float4*>(w + u) = four(sc + j * kSimpleLd + u0 + u);
+          } else {
+#pragma unroll
+            for (int u = 0; u < QPT; ++u) w[u] = sc[j * kSimpleLd + u0 + u];
           }
+#pragma unroll
+          for (int u = 0; u < QPT; ++u)
+            if (w[u] != 0.f) {           // what a query does not see may be anything
+              acc[u].x += w[u] * v.x;
+              acc[u].y += w[u] * v.y;
+              acc[u].z += w[u] * v.z;
+              acc[u].w += w[u] * v.w;
+            }
         }
       }
     }
@@ -177,25 +242,25 @@ __global__ void __launch_bounds__(256) prefix_simple_kernel(const SimpleArgs p, 
   }
 }
 
-template <typename T, int QPT>
+template <typename T, int QPT, bool WIDE>
 static int launch_simple(const SimpleArgs& p, const ds41_prefix_plan& plan, cudaStream_t st) {
   const int smem = simple_smem(p);
   if (smem > 220 * 1024) return cudaErrorInvalidValue;
-  const cudaError_t e = cudaFuncSetAttribute(prefix_simple_kernel<T, QPT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  const cudaError_t e = cudaFuncSetAttribute(prefix_simple_kernel<T, QPT, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   const long long most = 1ll * plan.max_units * ((plan.rows_per_unit * p.per_lane + kSimpleQueries - 1) / kSimpleQueries);
   const int blocks = static_cast<int>(most < 4 * sm_count() ? most : 4 * sm_count());
-  return launch_pdl(prefix_simple_kernel<T, QPT>, dim3(blocks), dim3(256), smem, st, p, plan);
+  return launch_pdl(prefix_simple_kernel<T, QPT, WIDE>, dim3(blocks), dim3(256), smem, st, p, plan);
 }
 
-template <typename T>
+template <typename T, bool WIDE>
 static int dispatch_simple(const SimpleArgs& p, const ds41_prefix_plan& plan, cudaStream_t st) {
   const int nc = p.vp / 4;
-  if (16 * nc <= 256) return launch_simple<T, 1>(p, plan, st);
-  if (8 * nc <= 256) return launch_simple<T, 2>(p, plan, st);
-  if (4 * nc <= 256) return launch_simple<T, 4>(p, plan, st);
-  if (2 * nc <= 256) return launch_simple<T, 8>(p, plan, st);
-  if (nc <= 256) return launch_simple<T, 16>(p, plan, st);
+  if (16 * nc <= 256) return launch_simple<T, 1, WIDE>(p, plan, st);
+  if (8 * nc <= 256) return launch_simple<T, 2, WIDE>(p, plan, st);
+  if (4 * nc <= 256) return launch_simple<T, 4, WIDE>(p, plan, st);
+  if (2 * nc <= 256) return launch_simple<T, 8, WIDE>(p, plan, st);
+  if (nc <= 256) return launch_simple<T, 16, WIDE>(p, plan, st);
   return cudaErrorInvalidValue;
 }
 
@@ -204,7 +269,8 @@ static int run_simple(const SimpleArgs& p, const ds41_prefix_plan& plan, int f32
   if ((p.ld_q & 3) || (p.ld_q2 & 3) || (p.q_head & 3) || (p.q2_head & 3) || (p.row_len & 3) || (p.d1 & 3) || (p.d2 & 3) || (p.vp & 3) ||
       ((reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.q2) | reinterpret_cast<uintptr_t>(p.pool)) & (f32 ? 15 : 7)))
     return cudaErrorInvalidValue;
-  return f32 ? dispatch_simple<float>(p, plan, st) : dispatch_simple<__nv_bfloat16>(p, plan, st);
+  if (p.d1 + p.d2 > 64) return f32 ? dispatch_simple<float, true>(p, plan, st) : dispatch_simple<__nv_bfloat16, true>(p, plan, st);
+  return f32 ? dispatch_simple<float, false>(p, plan, st) : dispatch_simple<__nv_bfloat16, false>(p, plan, st);
 }
 
 // A warp joins 128 columns of a (row, head): the lanes find the parts' weights, then every lane sums four columns over the parts, eight
@@ -312,7 +378,7 @@ extern "C" int ds41_prefix_latent(const ds41_latent_attend_args* a, const ds41_p
     p.page_table = a->page_table; p.row_pos = a->row_pos; p.row_slot = a->row_slot;
     p.ld_q = a->ld_q_abs; p.q_head = a->kv_pad; p.ld_q2 = a->ld_q_rot; p.q2_head = a->q_rot_stride;
     p.d1 = a->kv_pad; p.d2 = a->row_len - a->kv_pad; p.vp = a->kv_pad; p.row_len = a->row_len;
-    p.lanes = 1; p.per_lane = a->heads; p.heads = a->heads;
+    p.lanes = 1; p.per_lane = a->heads; p.heads = a->heads; p.inside = 1;
     p.max_pages = a->max_pages; p.page_tokens = a->page_tokens;
     p.scale = a->scale;
     e = run_simple(p, *plan, a->f32, st);

@@ -75,7 +75,7 @@ class Cost(NamedTuple):
 
 
 COSTS = {"grouped": Cost(1.4, 0.10, 0.0105, 0.0055, 1 / 6e6), "latent": Cost(4.0, 0.0, 0.0205, 0.0, 1 / 8e6)}
-COST_F32 = Cost(5.0, 0.0, 0.2, 0.2, 1 / 6e6)
+COST_F32 = Cost(1.0, 0.0, 0.3, 0.3, 1 / 6e6)
 SPANS = (1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 28, 32, 40, 48, 64, 96, 128, 192, 256, 384, 512, 1024, 2048, 4096)    # tried, in tiles or pages
 
 
@@ -200,7 +200,8 @@ class PrefixPlan:
         """Lengths that the keys may be divided by: the time that a plan with it takes at least, length; the shortest time first."""
         p, rows, tokens, n, keys = (np.array(x, dtype=np.int64) for x in (
             pieces, [len(x) for x, _ in self.shared], [x for _, x in self.shared], [x[1] for x in tails], [x[3] for x in tails]))
-        longest, unit, cost = int(max(tokens.max(initial=0), keys.max())), ceil_to(128, self.page_tokens), self.cost
+        longest, cost = int(max(tokens.max(initial=0), keys.max())), self.cost
+        unit = ceil_to(128 if self.dtype == BF16 else 32, self.page_tokens)
         at_a_time = self.grid * self.together / self.kv_heads
         per_key = cost.longer if self.together == 1 else (cost.longer + cost.shorter) / 2
         out = []
