@@ -7,9 +7,11 @@ share them; each row reads only what follows by itself, and the parts are joined
 
 Which rows share what is a `PrefixPlan`, made on the host from the page tables.  It holds as long as the rows belong to the same
 slots and those keep their leading pages: pages added at a table's end leave it valid, so a decode loop makes it once for a batch.
-It also holds the workspace of the calls, so calls with one plan follow one another on one stream; concurrent streams, or graphs
-that replay at the same time, need a plan each.  A captured call reads the plan from device memory: after `set()` a replay uses the
-new one.
+It also holds the workspace of the calls, so calls with one plan, and `set()`, follow one another on one stream; concurrent streams,
+or graphs that replay at the same time, need a plan each.  A captured call reads the plan from device memory: after `set()` a replay
+uses the new one, which may not have more rows than the call that was captured.
+
+What no row of a pass sees may hold anything, NaN included.
 """
 from __future__ import annotations
 
@@ -113,6 +115,8 @@ class PrefixPlan:
         self.part_o, self.part_ml = z(self.max_cells * heads * vdim, F32), z(self.max_cells * heads * 2, F32)
         self.status = lib.new_status(self.device)
         self.n_units = self.span = 0
+        self.n_rows, self.table_shape = 0, None            # of the last set(): what calls have to match
+        self.captured: Optional[int] = None                # least rows of the calls that graphs hold
         self.shared: List[Tuple[List[int], int]] = []      # rows and tokens of every prefix
         a, base = PlanArgs(), self.data.data_ptr()
         a.n_units, (a.units, a.turns, a.order, a.cell, a.parts) = base, (base + 4 * x for x in self._at)
@@ -137,6 +141,9 @@ class PrefixPlan:
             raise ValueError(f"slot {int(s.max())} of {len(t)}")
         if lengths is not None and len(lengths) != len(s):
             raise ValueError("lengths has an entry per row")
+        if self.captured is not None and (len(s) > self.captured or t.shape != self.table_shape):
+            raise ValueError(f"a captured call has {self.captured} rows and a page table of {tuple(self.table_shape)}")
+        self.n_rows, self.table_shape = len(s), t.shape
         of: Dict[int, List[int]] = {}                          # rows of every slot
         for r, slot in enumerate(s.tolist()):
             if slot >= 0:
@@ -315,6 +322,10 @@ def _check(plan: PrefixPlan, kind: str, rows: int, tensors, pool, page_table, ro
     for name, t, _ in tensors:
         if t is not None and t.get_device() != here:
             raise ValueError(f"{name} is on {t.device}, not on the current CUDA device")
+    if rows != plan.n_rows or page_table.shape != plan.table_shape:
+        raise ValueError(f"the plan was set for {plan.n_rows} rows and a page table of {plan.table_shape and tuple(plan.table_shape)}")
+    if torch.cuda.is_current_stream_capturing():
+        plan.captured = rows if plan.captured is None else min(rows, plan.captured)
 
 
 def _heads(name: str, q: torch.Tensor, heads: int, dtype) -> int:

@@ -307,3 +307,43 @@ def test_engines_without_plans_ignore_the_rows():
 def test_only_layer_stacks_are_served_with_shared_prefixes():
     from ds41rt_b200.models.registry import FAMILIES
     assert {n for n, f in FAMILIES.items() if f.shared_prefix} == {"genesun", "belasun"}
+
+
+def matching(plan, monkeypatch, rows, shape, capturing=False):
+    """The last of a call's checks, which stand behind that of the device."""
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
+    monkeypatch.setattr(plan, "device", torch.device("cuda"))
+    z = lambda *s, dtype=torch.int32: torch.zeros(*s, dtype=dtype)
+    pool, out = z(128, 32, dtype=BF16), z(rows, 4, 16, dtype=BF16)
+    named = (("pool", pool, BF16), ("out", out, BF16))
+    prefix._check(plan, "latent", rows, named, pool, z(*shape), z(rows), z(rows), out, 32, 1.0)
+
+
+def test_calls_match_the_rows_and_the_table_of_their_plan(monkeypatch):
+    plan = PrefixPlan("latent", rows=6, heads=4, vdim=16, page_tokens=64, device="cpu")
+    with pytest.raises(ValueError, match="set for 0 rows"):
+        matching(plan, monkeypatch, 3, (3, 5))
+    t = table([1, 2], [1, 3], [4], width=5)
+    plan.set([0, 1, 2], t)
+    matching(plan, monkeypatch, 3, (3, 5))
+    for rows, shape in ((2, (3, 5)), (4, (3, 5)), (3, (2, 5)), (3, (3, 6)), (3, (3, 4))):
+        with pytest.raises(ValueError, match="set for 3 rows"):
+            matching(plan, monkeypatch, rows, shape)
+
+
+def test_plans_of_captured_calls_do_not_outgrow_them(monkeypatch):
+    plan = PrefixPlan("latent", rows=6, heads=4, vdim=16, page_tokens=64, device="cpu")
+    t = table([1, 2], [1, 3], [4], width=5)
+    plan.set([0, 1, 2, -1], t)
+    matching(plan, monkeypatch, 4, (3, 5))
+    plan.set([0, 1, 2, -1, -1], t)
+    matching(plan, monkeypatch, 5, (3, 5), capturing=True)
+    plan.set([0, 1, 2], t)
+    matching(plan, monkeypatch, 3, (3, 5), capturing=True)
+    with pytest.raises(ValueError, match="captured call has 3 rows"):
+        plan.set([0, 1, 2, -1], t)
+    with pytest.raises(ValueError, match="captured"):
+        plan.set([0, 1, 2], table([1, 2], [1, 3], [4], [5], width=5))
+    plan.set([2, -1], t)
+    assert plan.n_rows == 2
