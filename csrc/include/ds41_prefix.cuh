@@ -25,15 +25,15 @@ __device__ __forceinline__ PrefixUnit prefix_unit(const ds41_prefix_plan& p, int
 __device__ __forceinline__ int prefix_row(const ds41_prefix_plan& p, const PrefixUnit& u, int i) {
   return u.tail ? u.first + i : p.order[u.first + i];
 }
-// Whole warps: the keys [first, end) that a unit's rows see.  A chunk's border may lie inside; `first` is a page's.  In two steps, so
-// that the positions of several units can be under way together.
+// Whole warps: the keys [first, end) that a unit's rows see.  `first` is a page's; a chunk's border may lie inside.  Behind `end` even
+// shared pages may hold anything, as rows may stand inside them.  In two steps, so that the positions of several units can be under
+// way together.
 struct PrefixRows {
   int low, high;                       // of this lane's rows
 };
 __device__ __forceinline__ PrefixRows prefix_rows(const ds41_prefix_plan& p, const PrefixUnit& u, const int* row_pos, const int* row_slot,
                                                   int chunk) {
   PrefixRows v = {u.key1, 0};
-  if (chunk == 0 && !u.tail) return v;
   for (int i = threadIdx.x & 31; i < u.rows; i += 32) {
     const int r = prefix_row(p, u, i), pos = row_pos[r];
     if (row_slot[r] < 0) continue;
@@ -43,16 +43,13 @@ __device__ __forceinline__ PrefixRows prefix_rows(const ds41_prefix_plan& p, con
   return v;
 }
 __device__ __forceinline__ void prefix_span(const PrefixUnit& u, PrefixRows v, int chunk, int page_tokens, int& first, int& end) {
-  first = u.key0;
-  end = u.key1;
-  if (chunk == 0 && !u.tail) return;
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
     v.low = min(v.low, __shfl_xor_sync(0xffffffffu, v.low, o));
     v.high = max(v.high, __shfl_xor_sync(0xffffffffu, v.high, o));
   }
-  first = max(first, v.low - v.low % page_tokens);
-  end = max(first, min(end, v.high));
+  first = chunk > 0 ? max(u.key0, v.low - v.low % page_tokens) : u.key0;
+  end = max(first, min(u.key1, v.high));
 }
 
 // Two 32-bit operations in one instruction.

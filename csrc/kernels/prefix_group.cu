@@ -62,7 +62,7 @@ struct GroupShared {                           // behind the tiles
   uint64_t p_full[2][2];                       // P written, O rescaled
   uint64_t o_next[2];                          // the unit's last product but one
   uint64_t o_full[2];                          // the unit's last product
-  uint64_t v_here[2];                          // the values of a tail's last tile, for the softmax
+  uint64_t v_here[2];                          // the values of a last tile that nobody sees whole, for the softmax
   int k_asked, v_asked;                        // copies under way or done: a place's barrier is at the phase of the last of these
   uint32_t tmem, pad[1];
   GroupWork info[kPgInfos];
@@ -270,7 +270,7 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap keys, const __grid_const
         if (!ok) break;
         const GroupWork& w = sh.info[turn % kPgInfos];
         const int n = w.tiles[t], base = w.base, least = min(w.tiles[0], w.tiles[1]);
-        const bool both = w.both != 0, tail = w.unit[t].tail != 0;
+        const bool both = w.both != 0, partial = w.end[t] < w.unit[t].key1;
         mbar_arrive(&sh.info_empty[turn % kPgInfos]);
         if (n == 0) continue;
         auto scores = [&](int j) {
@@ -299,7 +299,7 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap keys, const __grid_const
           const int at = copy_index(both, base, least, t, j), stage = at & mask, place = done & 1;
           ok = landed(&sh.v_asked, v_seen, sh.v_full, at, 473);
           if (!ok) break;
-          if (tail && j + 1 == n) mbar_arrive(&sh.v_here[t]);
+          if (partial && j + 1 == n) mbar_arrive(&sh.v_here[t]);
           ok = mbar_wait(&sh.p_full[t][place], (done >> 1) & 1, p.status, 474);
           if (!ok) break;
           tc_fence_after();
@@ -382,7 +382,7 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap keys, const __grid_const
       const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
       const uint32_t o_t = tmem + lanes + 256 + t * 128;
       const int mine_row = mine / p.n, mine_head = mine - mine_row * p.n;
-      int tiles = 0, done = 0, pairs = 0, tails = 0;     // tiles of S, units with keys, those with two tiles or more, tails so far
+      int tiles = 0, done = 0, pairs = 0, tails = 0;     // tiles of S, units with keys, those with two tiles or more, with a last tile like that
       for (int turn = 0; turn < turns; ++turn) {
         const int n = work(turn, t, unit, first, end, last);
         if (!ok) break;
@@ -489,8 +489,8 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap keys, const __grid_const
             sums[0] = add2(sums[0], sums[1]);
             l += sums[0].x + sums[0].y;
           }
-          if (unit.tail && j + 1 == n) {
-            // Places behind the last position belong to nobody, and a weight of zero does not take a NaN or an infinity away: their
+          if (end < unit.key1 && j + 1 == n) {
+            // Places behind the last position that a row sees may hold anything, and a weight of zero does not take a NaN or an infinity away: their
             // values become zeros, two threads to a place.
             ok = __all_sync(0xffffffffu, mbar_wait(&sh.v_here[t], tails & 1, p.status, 484 + t)) != 0;
             if (!ok) break;

@@ -432,8 +432,8 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
         if (!ok) break;
         tc_fence_after();
         tmem_st_32x32(lanes + kPlP, w);
-        if (it.tail && key0 + kPlKeys > end) {
-          // Places behind the last position belong to nobody, and a weight of zero does not take a NaN or an infinity away: their values
+        if (key0 + kPlKeys > end && end < it.key1) {
+          // Places behind the last position that a row sees may hold anything, and a weight of zero does not take a NaN or an infinity away: their values
           // become zeros, two threads to a place.
           const int key = mine & (kPlKeys - 1);
           if (key0 + key >= end)

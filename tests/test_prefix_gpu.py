@@ -198,6 +198,35 @@ def test_hidden_places_may_hold_anything(kind):
     Pass(kind, groups=[(9, 5), (3, 2)], alone=1, pads=1, poison=True, own=150, **SMALL[kind]).check()
 
 
+@pytest.mark.parametrize("rows", [2, 20, 60])
+@pytest.mark.parametrize("kind", KINDS)
+def test_rows_inside_a_prefix_do_not_see_what_follows_them(kind, rows):
+    """Shared pages whose last positions nobody stands behind yet."""
+    for seed in range(4):
+        Pass(kind, groups=[(rows, 9), (3, 4)], early=True, poison=True, seed=seed, P=(64, 32, 128, 16)[seed], **SMALL[kind]).check()
+    Pass(kind, groups=[(rows, 9)], early=True, poison=True, dtype=F32, **SMALL[kind]).check()
+    if kind == "grouped":
+        Pass(kind, groups=[(rows, 9)], early=True, poison=True, chunk=200, **SMALL[kind]).check()
+
+
+# rings of one to eight tiles, blocks that come to the list many times, walks that several pieces of a range share
+DEPTHS = [("grouped", dict(heads=8, kv_heads=4, dim=256, vdim=128, groups=[(9, 12)], own=200)),
+          ("grouped", dict(heads=8, kv_heads=4, dim=256, vdim=64, groups=[(9, 12)], own=200)),
+          ("grouped", dict(heads=8, kv_heads=4, dim=16, vdim=32, groups=[(9, 12)], own=200)),
+          ("grouped", dict(heads=32, kv_heads=8, dim=64, vdim=64, groups=[(130, 2), (60, 1), (40, 3)], own=80)),
+          ("grouped", dict(heads=32, kv_heads=8, dim=128, vdim=128, groups=[(150, 3)], own=80, P=16)),
+          ("grouped", dict(heads=32, kv_heads=4, dim=128, vdim=128, groups=[(64, 40)], own=30, P=32, chunk=700)),
+          ("grouped", dict(heads=32, kv_heads=32, dim=64, vdim=64, groups=[(40, 2)], own=300)),
+          ("latent", dict(heads=64, dim=576, vdim=512, groups=[(100, 2), (60, 1)], own=80)),
+          ("latent", dict(heads=16, dim=64, vdim=64, groups=[(150, 3)], own=300, P=16))]
+
+
+@pytest.mark.parametrize("i", range(len(DEPTHS)))
+def test_many_units_and_rings_of_every_depth(i):
+    kind, kw = DEPTHS[i]
+    Pass(kind, seed=200 + i, **kw).check()
+
+
 @pytest.mark.parametrize("kind", KINDS)
 def test_scores_that_differ_widely(kind):
     """Scores of hundreds: parts whose weights vanish beside another part's, and a running maximum that grows late."""
