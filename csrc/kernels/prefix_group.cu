@@ -7,13 +7,21 @@
 //   warps 0-3, 4-7 : softmax of tile 0 / 1 (one thread per query), partial results
 //   warps 8, 12    : TMA producers: key / value tiles of 64 positions, page by page
 //   warps 9, 14    : tcgen05.mma issue for tile 0 / 1: S = Q K^T, O += P V with P in TMEM where it replaces its S.  S has two places,
-//                    and the next tile's are asked for before this one's values
+//                    and the next tile's are asked for before this one's values.  200 rows of 32 heads over 16000 shared keys and up to
+//                    700 own ones take 129 us so, 138 with one place for 128 keys (a tile's S, softmax and values are then a chain), and 185 with
+//                    two places whose products one thread asked for: every step took it 800 cycles
 //   warps 10, 11   : queries of tile 0 / 1, and what each of them sees
 //   warp 13        : what the next units are and where their keys lie, for everybody (a ring of four)
 // A CTA walks its units, and every role but the softmax runs ahead into the next ones: a request's own keys are a few tiles, which the
 // chain of loads that a unit begins with (its description, its rows' positions, their pages, their queries) would take as long as.
 // The running maximum is raised when it grew by more than 2^8 only; what leaves is (m, l, unnormalised O) in 32 bits.  P is rounded
 // to bf16 as the operand of the second product; l sums the unrounded weights.
+//
+// What bounds it: 64 keys of two tiles take 2000 cycles, of which the tensor core works 1300 (the scores' two operands from shared memory
+// 48 per 128 x 64 x 16, the values' 64) and the 128 exponentials of a scheduler's two warps 1024; the softmax warps are the longest chain.
+// Letting them take turns at the exponentials, or taking a quarter of these by a polynomial, made steps of 1900 cycles and no call
+// shorter.  A unit costs 1.4 us beside its keys and 0.1 us per row (queries in, results out); requests' own keys are tiles of a few live
+// queries at the same price, and almost half of the call above (123 us with units dealt by these costs).
 #include <cuda.h>
 
 #include "ds41_group.cuh"
@@ -237,8 +245,7 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap keys, const __grid_const
         for (int i = 0; i < (1 << 18) && !mbar_test_wait(&full[b % stages], (b / stages) & 1); ++i) {
         }
   } else if (warp == 9 || warp == 14) {
-    // One thread: votes and the like between two products cost as much as the products.  One of either tile: a single one for both,
-    // that looked in turn for what could be asked next, took 800 cycles for every step of 250 to 400 cycles of products.
+    // one thread: votes and the like between two products cost as much as the products
     if (elect_one()) {
       const int t = warp == 14;
       const uint32_t idesc_s = umma_idesc(kPgTile, kPgKeys, 1u, 1u);
@@ -303,7 +310,8 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap keys, const __grid_const
           ok = mbar_wait(&sh.p_full[t][place], (done >> 1) & 1, p.status, 474);
           if (!ok) break;
           tc_fence_after();
-          umma4_ts<128>(tmem + 256 + t * 128, tmem + t * 128 + 64 * place, v_desc + static_cast<uint64_t>(stage * v_bytes / 16), idesc_pv, j > 0);
+          umma4_ts<128>(tmem + 256 + t * 128, tmem + t * 128 + 64 * place, v_desc + static_cast<uint64_t>(stage * v_bytes / 16), idesc_pv,
+                        j > 0);
           ++done;
           if (!both) mbar_arrive(&sh.v_empty[stage]);
           tc_commit(&sh.v_empty[stage]);
@@ -382,7 +390,7 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap keys, const __grid_const
       const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
       const uint32_t o_t = tmem + lanes + 256 + t * 128;
       const int mine_row = mine / p.n, mine_head = mine - mine_row * p.n;
-      int tiles = 0, done = 0, pairs = 0, tails = 0;     // tiles of S, units with keys, those with two tiles or more, with a last tile like that
+      int tiles = 0, done = 0, pairs = 0, tails = 0;     // tiles of S; units with keys, with two tiles or more, with a last one cut short
       for (int turn = 0; turn < turns; ++turn) {
         const int n = work(turn, t, unit, first, end, last);
         if (!ok) break;
@@ -426,8 +434,7 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap keys, const __grid_const
             tc_fence_after();
             const bool edge = key0 < low || key0 + kPgKeys > high;
             const int shown = hi - key0, hidden = lo - key0;             // columns [hidden, shown) of this tile are visible
-            // The code of this loop is short on purpose: with tiles unrolled over 128 columns, 42 % of all cycles were waits for
-            // instructions, and a small call, which runs everything for the first time, took 6400 cycles for its one tile.
+            // the code of this loop is short on purpose: instructions that run for the first time are waited for
             float2 v[kPgKeys / 2];
             {
               uint32_t(&raw)[64] = reinterpret_cast<uint32_t(&)[64]>(v);
@@ -490,8 +497,8 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap keys, const __grid_const
             l += sums[0].x + sums[0].y;
           }
           if (end < unit.key1 && j + 1 == n) {
-            // Places behind the last position that a row sees may hold anything, and a weight of zero does not take a NaN or an infinity away: their
-            // values become zeros, two threads to a place.
+            // Places behind the last position that a row sees may hold anything, and a weight of zero does not take a NaN or an
+            // infinity away: their values become zeros, two threads to a place.
             ok = __all_sync(0xffffffffu, mbar_wait(&sh.v_here[t], tails & 1, p.status, 484 + t)) != 0;
             if (!ok) break;
             ++tails;

@@ -61,7 +61,8 @@ __device__ __forceinline__ void cluster_meet() {
 
 template <bool PAIR>
 __global__ void __launch_bounds__(kPlThreads, 1)
-prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_constant__ CUtensorMap chunks, const PrefixLatentParams p, const ds41_prefix_plan plan) {
+prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_constant__ CUtensorMap chunks, const PrefixLatentParams p,
+                     const ds41_prefix_plan plan) {
   extern __shared__ __align__(1024) uint8_t pl_smem[];       // no room to align it here: it is a multiple of 1024 as it is
   uint8_t* smem = pl_smem;
   const int stage_bytes = p.chunks * kPlChunk;
@@ -433,8 +434,8 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
         tc_fence_after();
         tmem_st_32x32(lanes + kPlP, w);
         if (key0 + kPlKeys > end && end < it.key1) {
-          // Places behind the last position that a row sees may hold anything, and a weight of zero does not take a NaN or an infinity away: their values
-          // become zeros, two threads to a place.
+          // Places behind the last position that a row sees may hold anything, and a weight of zero does not take a NaN or an
+          // infinity away: their values become zeros, two threads to a place.
           const int key = mine & (kPlKeys - 1);
           if (key0 + key >= end)
             for (int i = 8 * (mine / kPlKeys); i < 8 * v_chunks; i += (i & 7) == 7 ? 9 : 1)
@@ -499,7 +500,8 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
 }
 
 template <bool PAIR>
-static int launch_form(const CUtensorMap& pool, const CUtensorMap& chunks, const PrefixLatentParams& p, const ds41_prefix_plan& plan, int smem, cudaStream_t st) {
+static int launch_form(const CUtensorMap& pool, const CUtensorMap& chunks, const PrefixLatentParams& p, const ds41_prefix_plan& plan, int smem,
+                       cudaStream_t st) {
   const cudaError_t e = cudaFuncSetAttribute(prefix_latent_kernel<PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   if (!PAIR) return launch_pdl(prefix_latent_kernel<PAIR>, dim3(plan.grid), dim3(kPlThreads), smem, st, pool, chunks, p, plan);

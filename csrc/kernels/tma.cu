@@ -46,7 +46,8 @@ cudaError_t make_tensor_map_3d(CUtensorMap* out, const void* base, TmaDtype dtyp
   const uint64_t align = padded4 ? 31 : 15;
   if ((reinterpret_cast<uintptr_t>(base) & align) != 0 || (row_stride_bytes & align) != 0 ||
       (batch > 1 && (batch_stride_bytes & align) != 0) || (box_smem_bytes & 15) != 0 ||
-      box_rows == 0 || box_rows > 256 || box_batch == 0 || box_batch > 256 || box_cols == 0 || box_cols > 256 || (padded4 && (box_cols != 128 || cols % 128))) {
+      box_rows == 0 || box_rows > 256 || box_batch == 0 || box_batch > 256 || box_cols == 0 || box_cols > 256 ||
+      (padded4 && (box_cols != 128 || cols % 128))) {
     return cudaErrorInvalidValue;
   }
   if (swizzle128 && box_smem_bytes != 128) return cudaErrorInvalidValue;
