@@ -224,7 +224,7 @@ class LatentAttention:
         e._run("latent_prefill", k.ds41_latent_prefill, C.byref(a), lib.stream())
 
     def prefix_shape(self):
-        return "latent", self.spec.heads, 1, self.kvp
+        return "latent", self.spec.heads, 1, self.kvp, 0
 
     def _absorbed(self, e: "StackEngine", R: int, ldq: int, pool, gate: Proj):
         sp, k, H = self.spec, e.k, self.spec.heads
@@ -348,7 +348,7 @@ class GroupedAttention:
         return {"a": [(self.w_in.n, self.w_in.k)], "b": [(self.w_o.n, self.w_o.k)]}
 
     def prefix_shape(self):
-        return "grouped", self.spec.heads, self.spec.kv_heads, self.vp
+        return "grouped", self.spec.heads, self.spec.kv_heads, self.vp, self.spec.chunk or 0
 
     def splits(self, e: "StackEngine", rows: int) -> int:
         """CTAs that share a row's keys: enough to fill the GPU, static per batch size (a captured pass replays while the
@@ -708,16 +708,16 @@ class StackEngine(RowsEngine):
         """`shared_prefix`: passes of up to `attn_rows` rows read the pages that requests have in common once for all of them, by a
         plan per shape of attention that follows the rows and their leases.  32-bit passes read them row by row."""
         self.prefix_plans = {}
-        self._planned, self._plan_until = None, 0
+        self._planned, self._plan_from, self._plan_until = None, [], 0
         if not shared_prefix or self.f32:
             return
         for lw in self.w.layers:
             if not hasattr(lw.mixer, "prefix_shape"):
                 continue
-            kind, heads, kv_heads, vdim = key = lw.mixer.prefix_shape()
+            kind, heads, kv_heads, vdim, chunk = key = lw.mixer.prefix_shape()
             if key not in self.prefix_plans:
                 self.prefix_plans[key] = prefix.PrefixPlan(kind, rows=self.attn_rows, heads=heads, kv_heads=kv_heads, vdim=vdim,
-                                                           page_tokens=self.cache.page_tokens, device=self.device)
+                                                           page_tokens=self.cache.page_tokens, device=self.device, chunk=chunk)
 
     def prefix_plan(self, mixer, rows: int) -> Optional[prefix.PrefixPlan]:
         """Static per batch size, as a captured pass needs it: the plan's contents follow the rows."""
@@ -731,11 +731,11 @@ class StackEngine(RowsEngine):
         n = min(len(slots), self.attn_rows)
         slots, positions = [int(s) for s in slots[:n]], [int(p) for p in positions[:n]]
         key, last = (slots, self.cache.version), max(positions, default=0)
-        if key == self._planned and last < self._plan_until:
+        if key == self._planned and last < self._plan_until and all(p >= q for p, q in zip(positions, self._plan_from)):
             return
         for plan in self.prefix_plans.values():
             plan.set(slots, self.cache.page_table_host, [p + 1 for p in positions])
-        self._planned, self._plan_until = key, last + 256
+        self._planned, self._plan_from, self._plan_until = key, positions, last + 256
 
     def max_active(self, m: MoESpec) -> int:
         """Most experts that a planned pass can use."""

@@ -85,20 +85,23 @@ class PrefixPlan:
     """Rows that share leading pages, how their attention is divided, and the workspace of the calls.
 
     `kind`: "grouped" or "latent"; `rows`: most rows of a pass; `heads`, `kv_heads`, `vdim`: of the attention (latent: one key / value
-    head, `vdim` the padded latent width).  Prefixes shorter than `min_tokens` are left to the rows."""
+    head, `vdim` the padded latent width).  Prefixes shorter than `min_tokens` are left to the rows.  `chunk`: the calls' chunk, if the
+    plan is to leave out what lies before the rows' chunks (see set())."""
 
     def __init__(self, kind: str, *, rows: int, heads: int, vdim: int, page_tokens: int, device, kv_heads: int = 1, dtype=BF16,
-                 min_tokens: int = 64):
+                 min_tokens: int = 64, chunk: int = 0):
         if kind not in ("grouped", "latent"):
             raise ValueError(f"a prefix plan is grouped or latent, not {kind!r}")
         if min(rows, heads, kv_heads, vdim, page_tokens) <= 0 or heads % kv_heads or vdim % 16:
             raise ValueError("sizes must be positive, kv_heads must divide heads, the value width must be a multiple of 16")
         if kind == "latent" and kv_heads != 1:
             raise ValueError("latent attention has one key / value head")
+        if chunk < 0 or (chunk and kind == "latent"):
+            raise ValueError("chunk must not be negative, and latent attention has none")
         if dtype not in (BF16, F32):
             raise ValueError(f"cache rows are bf16 or fp32, not {dtype}")
         self.kind, self.rows, self.heads, self.kv_heads, self.vdim = kind, rows, heads, kv_heads, vdim
-        self.page_tokens, self.dtype, self.device = page_tokens, dtype, torch.device(device)
+        self.page_tokens, self.dtype, self.device, self.chunk = page_tokens, dtype, torch.device(device), chunk
         self.min_tokens, self.cost = min_tokens, COSTS[kind] if dtype == BF16 else COST_F32
         self.rows_per_unit = max(1, 128 // (heads // kv_heads))
         self.together = 2 if kind == "grouped" else 1            # units that a block (latent, wide: two blocks) has at a time
@@ -118,6 +121,7 @@ class PrefixPlan:
         self.n_rows, self.table_shape = 0, None            # of the last set(): what calls have to match
         self.captured: Optional[int] = None                # least rows of the calls that graphs hold
         self.shared: List[Tuple[List[int], int]] = []      # rows and tokens of every prefix
+        self.lows: List[int] = []                          # first token of it that any of them sees
         a, base = PlanArgs(), self.data.data_ptr()
         a.n_units, (a.units, a.turns, a.order, a.cell, a.parts) = base, (base + 4 * x for x in self._at)
         a.part_o, a.part_ml = self.part_o.data_ptr(), self.part_ml.data_ptr()
@@ -129,8 +133,9 @@ class PrefixPlan:
 
     def set(self, slots: Sequence[int], tables, lengths: Optional[Sequence[int]] = None) -> None:
         """`slots`: the slot of every row of the passes to come (-1: none); `tables`: the page table on the host, [slots, pages],
-        negative where no page is leased.  `lengths`: how many tokens each row's request has now (default: what its pages hold); only
-        the division of the work goes by it."""
+        negative where no page is leased.  `lengths`: how many tokens each row's request has now (default: what its pages hold); the
+        division of the work goes by it.  A plan with a `chunk` also leaves out the keys before the chunk of a row's last token, if it
+        is given lengths: until the next set() such a row may go on, but not back behind that chunk's beginning."""
         t = tables.numpy() if isinstance(tables, torch.Tensor) else np.asarray(tables)
         s = np.asarray(slots, dtype=np.int64)
         if t.ndim != 2 or t.dtype != np.int32:
@@ -150,18 +155,26 @@ class PrefixPlan:
                 of.setdefault(slot, []).append(r)
         keep = list(of)
         runs = common_runs(t[keep]) if len(keep) > 1 else []
-        self.shared = [(sorted(r for i in members for r in of[keep[i]]), pages * self.page_tokens) for members, pages in runs
-                       if pages * self.page_tokens >= self.min_tokens]
         begin = np.zeros(len(s), dtype=np.int64)               # where a row's own keys begin
-        for rows, tokens in self.shared:
-            begin[rows] = tokens
+        if self.chunk and lengths is not None:
+            begin = np.maximum(np.asarray(lengths, dtype=np.int64) - 1, 0) // self.chunk * self.chunk // self.page_tokens * self.page_tokens
+        group = np.full(len(s), -1)
+        self.shared, self.lows = [], []
+        for members, pages in runs:
+            tokens = pages * self.page_tokens
+            rows = sorted(r for i in members for r in of[keep[i]] if begin[r] < tokens)
+            if len(set(s[rows].tolist())) > 1 and tokens - int(begin[rows].min()) >= self.min_tokens:
+                self.lows.append(int(begin[rows].min()))
+                group[rows], begin[rows] = len(self.shared), tokens
+                self.shared.append((rows, tokens))
         leased = {slot: self.page_tokens * int((np.append(t[slot], -1) < 0).argmax()) for slot in keep}
         tails = []                                             # (first row, rows, first key, keys there are now)
         for slot, rows in of.items():
             at = 0
             while at < len(rows):                              # neighbours, as many as a unit takes
                 n = 1
-                while at + n < len(rows) and n < self.rows_per_unit and rows[at + n] == rows[at] + n:
+                while at + n < len(rows) and n < self.rows_per_unit and rows[at + n] == rows[at] + n \
+                        and begin[rows[at + n]] == begin[rows[at]] and group[rows[at + n]] == group[rows[at]]:
                     n += 1
                 have = leased[slot] if lengths is None else max(int(lengths[r]) for r in rows[at:at + n])
                 tails.append((rows[at], n, int(begin[rows[at]]), max(1, have - int(begin[rows[at]]))))
@@ -206,7 +219,7 @@ class PrefixPlan:
     def _spans(self, pieces, tails) -> List[Tuple[float, int]]:
         """Lengths that the keys may be divided by: the time that a plan with it takes at least, length; the shortest time first."""
         p, rows, tokens, n, keys = (np.array(x, dtype=np.int64) for x in (
-            pieces, [len(x) for x, _ in self.shared], [x for _, x in self.shared], [x[1] for x in tails], [x[3] for x in tails]))
+            pieces, [len(x) for x, _ in self.shared], [x - low for (_, x), low in zip(self.shared, self.lows)], [x[1] for x in tails], [x[3] for x in tails]))
         longest, cost = int(max(tokens.max(initial=0), keys.max())), self.cost
         unit = ceil_to(128 if self.dtype == BF16 else 32, self.page_tokens)
         at_a_time = self.grid * self.together / self.kv_heads
@@ -224,12 +237,13 @@ class PrefixPlan:
     def _items(self, slots: np.ndarray, pieces, tails, limit: int, span: int) -> Tuple[np.ndarray, np.ndarray]:
         """What there is to do with at most `span` keys at a time, as units without their head, and the partial results of every row."""
         items, at, parts = [], 0, np.zeros(len(slots), dtype=np.int32)
-        for p, (rows, tokens) in zip(pieces, self.shared):
-            count = -(-tokens // span)
+        for p, (rows, tokens), low in zip(pieces, self.shared, self.lows):
+            count = -(-(tokens - low) // span)
             parts[rows] = count
             for i in range(p):
                 lo, hi = (len(rows) * j // p for j in (i, i + 1))
-                items += [(int(slots[rows[0]]), at + lo, hi - lo, k * span, min(tokens, (k + 1) * span), k, 0) for k in range(count)]
+                items += [(int(slots[rows[0]]), at + lo, hi - lo, low + k * span, min(tokens, low + (k + 1) * span), k, 0)
+                          for k in range(count)]
             at += len(rows)
         for first, rows, key0, keys in tails:
             count = max(1, keys // span)                       # the last one goes on to wherever the request gets
@@ -355,8 +369,8 @@ def group_attend(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, 
     _check(plan, "grouped", R, (("pool", pool, dtype), ("out", out, dtype), ("page_table", page_table, I32), ("row_pos", row_pos, I32),
                                 ("row_slot", row_slot, I32), ("q", q, dtype), ("gate", gate, F32), ("plan", plan.data, I32)),
            pool, page_table, row_pos, row_slot, out, plan.kv_heads * (D + plan.vdim), scale)
-    if chunk < 0:
-        raise ValueError("chunk must not be negative")
+    if chunk < 0 or (plan.chunk and chunk != plan.chunk):
+        raise ValueError(f"the plan is for a chunk of {plan.chunk}" if plan.chunk else "chunk must not be negative")
     if gate is not None and (gate.shape != (R, H) or gate.stride(1) != 1):
         raise ValueError(f"gate must be [{R}, {H}] with a row's values side by side")
     slots, max_pages = page_table.shape

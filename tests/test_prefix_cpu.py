@@ -252,7 +252,7 @@ class Leases:
         from ds41rt_b200.models.paged import PagedSlots
         self.cache = PagedSlots()
         self.cache._init_pages(4, 1024, "cpu", 64, 40)
-        self.attn_rows, self._planned, self._plan_until = 3, None, 0
+        self.attn_rows, self._planned, self._plan_from, self._plan_until = 3, None, [], 0
         self.prefix_plans = {"x": PrefixPlan("grouped", rows=3, heads=4, kv_heads=2, vdim=16, page_tokens=64, device="cpu")}
         self.plan, self.sets = self.prefix_plans["x"], 0
         real = self.plan.set
@@ -283,6 +283,9 @@ def test_plans_of_an_engine_follow_its_rows_and_their_leases():
     assert e.sets == 1
     e.describe([600, 303, 304], [0, 1, 2])                             # longer by a few tiles
     assert e.sets == 2
+    e.describe([599, 303, 304], [0, 1, 2])                             # one goes back
+    assert e.sets == 3
+    e.sets = 2
     e.describe([601, 304], [0, 1])
     assert e.sets == 3 and e.plan.shared == [([0, 1], 192)]
     e.describe([304, 601], [1, 0])
@@ -347,3 +350,38 @@ def test_plans_of_captured_calls_do_not_outgrow_them(monkeypatch):
         plan.set([0, 1, 2], table([1, 2], [1, 3], [4], [5], width=5))
     plan.set([2, -1], t)
     assert plan.n_rows == 2
+
+
+@pytest.mark.parametrize("seed", range(20))
+def test_plans_with_a_chunk_leave_out_what_no_row_sees(seed):
+    rng = random.Random(seed)
+    P, chunk, width = rng.choice([(32, 256), (64, 100), (64, 1024), (16, 50)]) + (60,)
+    rows = rng.randint(2, 40)
+    lead = list(range(1, 1 + rng.randint(1, 40)))
+    t = np.full((rows, width), -1, dtype=np.int32)
+    for i in range(rows):
+        own = rng.randint(1, width - len(lead))
+        t[i, :len(lead) + own] = lead + [1000 + 100 * i + k for k in range(own)]
+    slots = list(range(rows)) if seed % 2 else [i // 2 for i in range(rows)]          # two rows of a request
+    lengths = [rng.randint(1, width * P) for _ in slots] if seed % 2 else [n + k for n in [rng.randint(1, width * P - 1)
+                                                                              for _ in range(rows)] for k in range(2)][:rows]
+    plan = PrefixPlan("grouped", rows=rows, heads=8, kv_heads=2, vdim=64, page_tokens=P, device="cpu", chunk=chunk)
+    plan.set(slots, t, lengths)
+    d = plan.data.numpy()
+    units, turns, order, cell, count = (d[a:b] for a, b in zip(plan._at, plan._at[1:] + [len(d)]))
+    covered = {}
+    for slot, first, n, k0, k1, part, tail, head in units[:8 * plan.n_units].reshape(-1, 8).tolist():
+        for r in range(first, first + n) if tail else order[first:first + n].tolist():
+            assert part < count[r] and (t[slots[r], :k1 // P] == t[slot, :k1 // P]).all() and (not tail or slots[r] == slot)
+            covered.setdefault((r, head), []).append((k0, k1, part))
+    for r in range(rows):
+        for head in range(2):
+            got = sorted(covered[r, head])
+            assert [x[2] for x in got] == list(range(count[r]))
+            assert [x[0] for x in got[1:]] + [width * P] == [x[1] for x in got]         # no gap to the table's end
+            assert got[0][0] <= (lengths[r] - 1) // chunk * chunk
+    plan.set(slots, t)                                       # without lengths nothing is left out
+    first = plan.data[4:4 + 8 * plan.n_units].reshape(-1, 8)
+    assert int(first[first[:, 2] > 0][:, 3].min()) == 0
+    with pytest.raises(ValueError):
+        PrefixPlan("latent", rows=2, heads=4, vdim=16, page_tokens=64, device="cpu", chunk=64)

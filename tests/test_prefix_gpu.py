@@ -234,6 +234,21 @@ def test_scores_that_differ_widely(kind):
         Pass(kind, groups=[(10, 9)], own=200, sharp=60.0, seed=seed, **SMALL[kind]).check()
 
 
+@pytest.mark.parametrize("chunk,P", [(256, 64), (100, 32), (1000, 16)])
+def test_plans_that_leave_out_earlier_chunks(chunk, P):
+    p = Pass("grouped", groups=[(20, 700 // P), (5, 90 // P)], alone=2, pads=1, own=600, chunk=chunk, P=P, **SMALL["grouped"])
+    plan = p.plan(chunk=chunk)
+    p.check(plan)
+    plan.set(p.row_slot, p.tables, [x + 1 for x in p.row_pos])
+    p.check(plan)
+    p.row_pos = [x + 1 if x // P == (x + 1) // P else x for x in p.row_pos]         # where the page is leased
+    p.d_pos = p.dev(p.row_pos)
+    p.check(plan)
+    with pytest.raises(ValueError, match="chunk of"):
+        p.chunk = 0
+        p.run(plan)
+
+
 @pytest.mark.parametrize("kind", KINDS)
 def test_without_gate_or_sink(kind):
     Pass(kind, groups=[(5, 6)], **SMALL[kind]).check(gate=False)
