@@ -126,7 +126,7 @@ class PrefixPlan:
         a.n_units, (a.units, a.turns, a.order, a.cell, a.parts) = base, (base + 4 * x for x in self._at)
         a.part_o, a.part_ml = self.part_o.data_ptr(), self.part_ml.data_ptr()
         a.max_units, a.rows_per_unit, a.grid = self.max_units, self.rows_per_unit, self.grid
-        self.args = a
+        self.args, self.args_ref = a, C.byref(a)
 
     def nbytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in (self.data, self.part_o, self.part_ml))
@@ -295,15 +295,20 @@ class PrefixPlan:
 
 
 # ---------------------------------------------------------------------------------------------------- launches
+def _stream() -> int:
+    """The current stream's handle, without the object that torch.cuda.current_stream() makes for it (3 us, a sixth of a call)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+
+
 def launch_group(a: S.GroupAttendArgs, plan: PrefixPlan) -> None:
     """Grouped attention; `a` as for ds41_group_attend."""
-    lib.check(lib.kernels("stack").ds41_prefix_group(C.byref(a), C.byref(plan.args), lib.stream()), "ds41_prefix_group")
+    lib.check(lib.kernels("stack").ds41_prefix_group(C.byref(a), plan.args_ref, C.c_void_p(_stream())), "ds41_prefix_group")
 
 
 def launch_latent(a: S.LatentAttendArgs, plan: PrefixPlan, n_pages: int, sink, out: torch.Tensor, ld_out: int) -> None:
     """Latent attention and the join of its parts; `a` as for ds41_latent_attend."""
-    lib.check(lib.kernels("stack").ds41_prefix_latent(C.byref(a), C.byref(plan.args), n_pages, lib.ptr(sink), lib.ptr(out), ld_out,
-                                                      lib.stream()), "ds41_prefix_latent")
+    lib.check(lib.kernels("stack").ds41_prefix_latent(C.byref(a), plan.args_ref, n_pages, lib.ptr(sink), lib.ptr(out), ld_out,
+                                                      C.c_void_p(_stream())), "ds41_prefix_latent")
 
 
 # ---------------------------------------------------------------------------------------------------- front end
@@ -375,7 +380,7 @@ def group_attend(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, 
         raise ValueError(f"gate must be [{R}, {H}] with a row's values side by side")
     slots, max_pages = page_table.shape
     a = S.GroupAttendArgs(q.data_ptr(), pool.data_ptr(), page_table.data_ptr(), row_pos.data_ptr(), row_slot.data_ptr(), out.data_ptr(),
-                          plan.status.data_ptr(), S.Proj(gate, gate.stride(0)).args() if gate is not None else S.NO_PROJ, S.NO_PROJ, None,
+                          plan.status.data_ptr(), S.ProjArgs(gate.data_ptr(), 0, gate.stride(0), 1, 0, 0) if gate is not None else S.NO_PROJ, S.NO_PROJ, None,
                           ld_q, scale, R, H, plan.kv_heads, D, plan.vdim, chunk, 1, slots, 0, out.stride(0), max_pages, plan.page_tokens,
                           int(dtype == F32), pool.shape[0] // plan.page_tokens, 0)
     launch_group(a, plan)
