@@ -224,7 +224,7 @@ class LatentAttention:
         e._run("latent_prefill", k.ds41_latent_prefill, C.byref(a), lib.stream())
 
     def prefix_shape(self):
-        return "latent", self.spec.heads, 1, self.kvp, 0
+        return "latent", self.spec.heads, 1, self.row_len, self.kvp, 0
 
     def _absorbed(self, e: "StackEngine", R: int, ldq: int, pool, gate: Proj):
         sp, k, H = self.spec, e.k, self.spec.heads
@@ -348,7 +348,7 @@ class GroupedAttention:
         return {"a": [(self.w_in.n, self.w_in.k)], "b": [(self.w_o.n, self.w_o.k)]}
 
     def prefix_shape(self):
-        return "grouped", self.spec.heads, self.spec.kv_heads, self.vp, self.spec.chunk or 0
+        return "grouped", self.spec.heads, self.spec.kv_heads, self.dp, self.vp, self.spec.chunk or 0
 
     def splits(self, e: "StackEngine", rows: int) -> int:
         """CTAs that share a row's keys: enough to fill the GPU, static per batch size (a captured pass replays while the
@@ -706,7 +706,8 @@ class StackEngine(RowsEngine):
 
     def _init_prefix_plans(self, shared_prefix: bool):
         """`shared_prefix`: passes of up to `attn_rows` rows read the pages that requests have in common once for all of them, by a
-        plan per shape of attention that follows the rows and their leases.  32-bit passes read them row by row."""
+        plan per shape of attention that follows the rows and their leases.  32-bit passes, and shapes that the tensor-core forms do not
+        take, read them row by row."""
         self.prefix_plans = {}
         self._planned, self._plan_from, self._plan_until = None, [], 0
         if not shared_prefix or self.f32:
@@ -714,8 +715,8 @@ class StackEngine(RowsEngine):
         for lw in self.w.layers:
             if not hasattr(lw.mixer, "prefix_shape"):
                 continue
-            kind, heads, kv_heads, vdim, chunk = key = lw.mixer.prefix_shape()
-            if key not in self.prefix_plans:
+            kind, heads, kv_heads, dim, vdim, chunk = key = lw.mixer.prefix_shape()
+            if key not in self.prefix_plans and prefix.tiled(kind, heads, kv_heads, dim, vdim, self.cache.page_tokens):
                 self.prefix_plans[key] = prefix.PrefixPlan(kind, rows=self.attn_rows, heads=heads, kv_heads=kv_heads, vdim=vdim,
                                                            page_tokens=self.cache.page_tokens, device=self.device, chunk=chunk)
 

@@ -64,6 +64,16 @@ def common_runs(tables: np.ndarray) -> List[Tuple[List[int], int]]:
     return out
 
 
+def tiled(kind: str, heads: int, kv_heads: int, dim: int, vdim: int, page_tokens: int) -> bool:
+    """Do bf16 calls of these sizes take the tensor-core forms?  The one for everything else, whose products are 32-bit, is for sizes that
+    are small or rare: reading common pages once does not make up for it.  `dim`: of a key (latent: with its rotated part)."""
+    if page_tokens < 8 or max(page_tokens, 64) % min(page_tokens, 64):
+        return False
+    if kind == "grouped":
+        return heads // kv_heads <= 128 and vdim <= 128 and dim <= 256
+    return heads <= 128 and vdim <= 512 and dim - vdim <= 64
+
+
 class Cost(NamedTuple):
     """What a plan goes by, in us (measured on units of 64 to 16000 keys): of a block's turn, of a row of its units, of a key of the
     longer of the units that it has at a time and of one of the shorter, of a byte of partial results on their way to the join and of a

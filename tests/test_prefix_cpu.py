@@ -385,3 +385,13 @@ def test_plans_with_a_chunk_leave_out_what_no_row_sees(seed):
     assert int(first[first[:, 2] > 0][:, 3].min()) == 0
     with pytest.raises(ValueError):
         PrefixPlan("latent", rows=2, heads=4, vdim=16, page_tokens=64, device="cpu", chunk=64)
+
+
+@pytest.mark.parametrize("args,want", [
+    (("grouped", 32, 8, 128, 128, 64), True), (("grouped", 32, 8, 256, 128, 16), True), (("grouped", 32, 8, 128, 144, 64), False),
+    (("grouped", 160, 1, 64, 64, 64), False), (("grouped", 32, 8, 272, 64, 64), False), (("grouped", 32, 8, 64, 64, 48), False),
+    (("grouped", 32, 8, 64, 64, 4), False), (("grouped", 32, 8, 64, 64, 192), True), (("grouped", 32, 8, 64, 64, 96), False),
+    (("latent", 128, 1, 576, 512, 64), True), (("latent", 130, 1, 576, 512, 64), False), (("latent", 16, 1, 592, 528, 64), False),
+    (("latent", 16, 1, 592, 512, 64), False), (("latent", 16, 1, 512, 512, 8), True)])
+def test_which_shapes_engines_plan_for(args, want):
+    assert prefix.tiled(*args) is want

@@ -119,3 +119,49 @@ def test_graphs_of_a_device_loop_follow_the_requests_as_they_grow():
         want, spread = (x[130] for x in belasun.reference("tiles", common + [first], "bf16")[:2])
         err = float((got[0][i] - got[1][i]).pow(2).mean().sqrt() / want.std())
         assert err < 2 * limit("bf16", float(spread))    # either is within one of the exact values
+
+
+def test_the_scheduler_serves_requests_that_share_a_prompt():
+    """Requests that extend one prompt continue its snapshot together: every token's logit is the largest one, within what rounding may
+    move two of them (a logit is off by at most sqrt(vocabulary) times the root mean square that `limit` bounds)."""
+    from ds41rt_b200.serving.engine import GenRequest, NativeBackend
+    from ds41rt_b200.serving.protocol import Sampling
+    e = engine("belasun", "tiles", max_rows=256, slots=4, page_tokens=32)
+    seen = set()
+    describe = e.describe
+
+    def watched(*a):
+        describe(*a)
+        seen.update(len(p.shared[0][0]) for p in e.prefix_plans.values() if p.shared)
+    e.describe = watched
+    be = NativeBackend(e, eos=-1, concurrency=3, prefill_chunk=128)
+    try:
+        def submit(p, n):
+            r = GenRequest(prompt_ids=p, max_tokens=n, sampling=Sampling(temperature=0.0))
+            be.submit(r)
+            return r
+
+        def collect(r):
+            toks = []
+            while True:
+                ev = r.events.get(timeout=60)
+                assert ev.kind != "error", ev.message
+                toks += ev.tokens
+                if ev.kind == "finish":
+                    return toks
+
+        first = belasun.tokens("tiles", 120, seed=31)
+        common = first + collect(submit(first, 8))[:7]
+        prompts = [common + belasun.tokens("tiles", 5 + i, seed=40 + i) for i in range(3)]
+        outs = [collect(r) for r in [submit(p, 24) for p in prompts]]
+        assert be.error is None and seen & {2, 3}
+        for p, o in zip(prompts, outs):
+            assert len(o) == 24
+            want, spread = belasun.reference("tiles", p + o, "bf16")[:2]
+            for i, tok in enumerate(o):
+                z, at = want[len(p) + i - 1], len(p) + i - 1
+                room = 2 * len(z) ** 0.5 * limit("bf16", float(spread[at])) * float(z.std())
+                assert float(z.max() - z[tok]) <= room
+    finally:
+        be.close()
+    e.check_status()
