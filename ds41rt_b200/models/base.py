@@ -107,6 +107,9 @@ class RowsEngine:
         """What the rows of the passes to come are, for engines that plan by it.  set_rows() calls it; whoever hands the rows to the
         device in another way does so before the pass."""
 
+    def settle(self):
+        """Before a captured pass is replayed over the rows of the last set_rows(), whatever pass that was meant for."""
+
     # ------------------------------------------------------------------ graphs
     @contextlib.contextmanager
     def rehearsal(self):

@@ -387,8 +387,8 @@ class GroupedAttention:
         if long:
             b.pos0, b.n_splits = long - R, 1
             e._run("group_prefill", k.ds41_group_prefill, C.byref(b), lib.stream())
-        elif e.prefix_plan(self, R) is not None:
-            e._run("prefix_attend", prefix.launch_group, b, e.prefix_plan(self, R))
+        elif (plan := e.prefix_plan(self, R)) is not None:
+            e._run("prefix_attend", prefix.launch_group, b, plan)
         else:
             b.n_splits = self.splits(e, R)
             e._run("group_attend", k.ds41_group_attend, C.byref(b), lib.stream())
@@ -605,6 +605,7 @@ class StackEngine(RowsEngine):
     replay_window = 1 << 30       # the prefix banks then never prefer a truncated snapshot
     engram: dict = {}
     prefix_plans: Dict[tuple, prefix.PrefixPlan] = {}      # by shape of attention, of engines made with `shared_prefix`
+    _undescribed = None
     taps = None
 
     def __init__(self, cfg: StackConfig, weights: StackWeights, *, max_rows: int = 8, slots: int = 1, max_ctx: int = 4096,
@@ -710,6 +711,7 @@ class StackEngine(RowsEngine):
         take, read them row by row."""
         self.prefix_plans = {}
         self._planned, self._plan_from, self._plan_until = None, [], 0
+        self._undescribed = None      # (positions, slots) of a pass that needs no plan, until one over the same rows does
         if not shared_prefix or self.f32:
             return
         for lw in self.w.layers:
@@ -721,14 +723,19 @@ class StackEngine(RowsEngine):
                                                            page_tokens=self.cache.page_tokens, device=self.device, chunk=chunk)
 
     def prefix_plan(self, mixer, rows: int) -> Optional[prefix.PrefixPlan]:
-        """Static per batch size, as a captured pass needs it: the plan's contents follow the rows."""
-        return self.prefix_plans.get(mixer.prefix_shape()) if self.prefix_plans and rows <= self.attn_rows else None
+        """The plan that a pass takes, static per batch size, as a captured pass needs it: its contents follow the rows.  A long pass asks
+        for one, too, where a layer has no other form (its pages, its widths)."""
+        if not self.prefix_plans or rows > self.attn_rows:
+            return None
+        self.settle()
+        return self.prefix_plans.get(mixer.prefix_shape())
 
     def describe(self, positions, slots):
         """Plans hold as long as the rows belong to the same leases; they are also renewed as requests grow, for the sake of an even
         division."""
         if not self.prefix_plans:
             return
+        self._undescribed = None
         n = min(len(slots), self.attn_rows)
         slots, positions = [int(s) for s in slots[:n]], [int(p) for p in positions[:n]]
         key, last = (slots, self.cache.version), max(positions, default=0)
@@ -737,6 +744,10 @@ class StackEngine(RowsEngine):
         for plan in self.prefix_plans.values():
             plan.set(slots, self.cache.page_table_host, [p + 1 for p in positions])
         self._planned, self._plan_from, self._plan_until = key, positions, last + 256
+
+    def settle(self):
+        if self._undescribed is not None:
+            self.describe(*self._undescribed)
 
     def max_active(self, m: MoESpec) -> int:
         """Most experts that a planned pass can use."""
@@ -802,7 +813,10 @@ class StackEngine(RowsEngine):
             self.in_tokens.copy_(row_values(tokens, self.max_rows, 0), non_blocking=True)
         self.row_pos.copy_(pos, non_blocking=True)
         self.row_slot.copy_(slot, non_blocking=True)
-        self.describe(p, s)
+        if self.prefix_plans and (one or n > self.attn_rows):
+            self._undescribed = (p, s)        # a prompt's: the plan of the requests that decode between its passes stays
+        else:
+            self.describe(p, s)
 
     def _resid(self, R: int, *, y: Optional[Proj] = None, gate: Optional[Proj] = None, bias=None, post=None, x_in=None,
                x_out=None, layer: Optional[int] = None, next_w=None, post_rms: bool = False):

@@ -84,6 +84,7 @@ class DecodeSession:
     def run_device_loop(self, rows: int, steps: int):
         """`steps` decode steps with on-device token feedback (no host synchronisation inside)."""
         g = self.graph(rows, feedback=True)
+        self.e.settle()
         for _ in range(steps):
             if g is not None:
                 g.replay()

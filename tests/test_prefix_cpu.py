@@ -246,13 +246,13 @@ def test_latent_calls_refuse(change):
 class Leases:
     """What StackEngine.describe() asks of an engine and its cache."""
     from ds41rt_b200.models.stack import StackEngine
-    describe = StackEngine.describe
+    describe, settle = StackEngine.describe, StackEngine.settle
 
     def __init__(self):
         from ds41rt_b200.models.paged import PagedSlots
         self.cache = PagedSlots()
         self.cache._init_pages(4, 1024, "cpu", 64, 40)
-        self.attn_rows, self._planned, self._plan_from, self._plan_until = 3, None, [], 0
+        self.attn_rows, self._planned, self._plan_from, self._plan_until, self._undescribed = 3, None, [], 0, None
         self.prefix_plans = {"x": PrefixPlan("grouped", rows=3, heads=4, kv_heads=2, vdim=16, page_tokens=64, device="cpu")}
         self.plan, self.sets = self.prefix_plans["x"], 0
         real = self.plan.set
@@ -298,6 +298,22 @@ def test_plans_of_an_engine_follow_its_rows_and_their_leases():
     assert e.sets == 6 and int(e.plan.data[e.plan._at[4]:].count_nonzero()) == 3
     e.describe([], [])
     assert e.plan.n_units == 0
+
+
+def test_rows_that_need_no_plan_are_described_when_one_is():
+    e = Leases()
+    assert e.cache.ensure(0, 300)
+    e.describe([1], [0])
+    e.settle()
+    assert e.sets == 1
+    e._undescribed = ([2, 3], [0, 0])
+    e.settle()
+    e.settle()
+    assert e.sets == 2 and e._undescribed is None and e.plan.n_rows == 2
+    e._undescribed = ([2, 3], [0, 0])
+    e.describe([4], [0])                                     # other rows are there now
+    e.settle()
+    assert e.sets == 3 and e.plan.n_rows == 1
 
 
 def test_engines_without_plans_ignore_the_rows():

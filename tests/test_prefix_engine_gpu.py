@@ -165,3 +165,40 @@ def test_the_scheduler_serves_requests_that_share_a_prompt():
     finally:
         be.close()
     e.check_status()
+
+
+def test_prompts_between_steps_leave_the_plan_of_the_steps():
+    """A long prompt pass takes no plan; the same rows as a short pass, eager or by a captured step, do."""
+    from ds41rt_b200.runtime.session import DecodeSession
+    e = engine("belasun", "tiles", page_tokens=32)
+    sets, plans = [0], list(e.prefix_plans.values())
+    real = plans[0].set
+
+    def counted(*a):
+        sets[0] += 1
+        real(*a)
+    plans[0].set = counted
+    ses = DecodeSession(e)
+    a, b, c = (belasun.tokens("tiles", n, seed=50 + n) for n in (90, 100, 150))
+    want = [belasun.reference("tiles", t, "bf16")[:2] for t in (a, b, c)]
+    feed(e, 0, a[:70], 0, [1024])
+    feed(e, 1, b[:80], 0, [1024])
+    assert all(e.cache.ensure(s, 200) for s in range(3))
+    assert sets[0] == 0
+    for i in range(4):
+        ses.step([a[70 + i], b[80 + i]], [70 + i, 80 + i], [0, 1])
+        got = e.logits_rows(2).cpu().double()
+        for r, at in enumerate((70 + i, 80 + i)):
+            close(got[r:r + 1], want[r][0][at:at + 1], "bf16", want[r][1][at:at + 1])
+        if i == 1:
+            n = sets[0]
+            close(feed(e, 2, c[:70], 0, [1024]), want[2][0][:70], "bf16", want[2][1][:70])
+    assert n == sets[0] == 1
+    for _ in range(2):                                   # once as a prompt's pass, then as any other over the same rows
+        e.set_rows(c[:80], list(range(80)), [2] * 80)
+        e.forward_rows(80, head=False)
+        e.forward_rows(80, head=False)
+        got = e.logits_at(list(range(80))).cpu().double()
+        close(got, want[2][0][:80], "bf16", want[2][1][:80])
+    assert sets[0] == 2
+    e.check_status()
