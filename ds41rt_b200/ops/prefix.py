@@ -322,17 +322,23 @@ def launch_latent(a: S.LatentAttendArgs, plan: PrefixPlan, n_pages: int, sink, o
 
 
 # ---------------------------------------------------------------------------------------------------- front end
-def _check(plan: PrefixPlan, kind: str, rows: int, tensors, pool, page_table, row_pos, row_slot, out, width: int, scale: float) -> None:
-    """`tensors`: name, tensor or None, and type of every argument."""
+def _check(plan: PrefixPlan, kind: str, rows: int, q, q_rot, extra, pool, page_table, row_pos, row_slot, out, width: int,
+           scale: float) -> None:
+    """`extra`: the gate or the sink.  What is asked of every tensor is asked at once, as it is a call's host time; which one it is that
+    does not fit is found afterwards."""
     if plan.kind != kind:
         raise ValueError(f"the plan is for {plan.kind} attention")
     if not scale > 0:
         raise ValueError("scale must be positive")
     if not 0 < rows <= plan.rows:
         raise ValueError(f"a pass has 1 to {plan.rows} rows, not {rows}")
-    for name, t, dtype in tensors:
-        if t is not None and t.dtype != dtype:
-            raise ValueError(f"{name} must be 32-bit integers, not {t.dtype}" if dtype == I32 else f"{name} is {t.dtype}")
+    dtype = plan.dtype
+    if pool.dtype is not dtype or out.dtype is not dtype or page_table.dtype is not I32 or row_pos.dtype is not I32 \
+            or row_slot.dtype is not I32 or (extra is not None and extra.dtype is not F32):
+        for name, t, want in (("pool", pool, dtype), ("out", out, dtype), ("page_table", page_table, I32), ("row_pos", row_pos, I32),
+                              ("row_slot", row_slot, I32), ("gate" if kind == "grouped" else "sink", extra, F32)):
+            if t is not None and t.dtype != want:
+                raise ValueError(f"{name} must be 32-bit integers, not {t.dtype}" if want == I32 else f"{name} is {t.dtype}")
     if not (page_table.is_contiguous() and row_pos.is_contiguous() and row_slot.is_contiguous()):
         raise ValueError("page_table, row_pos and row_slot must be contiguous")
     if page_table.dim() != 2 or row_pos.dim() != 1 or row_slot.dim() != 1 or row_pos.numel() < rows or row_slot.numel() < rows:
@@ -348,9 +354,13 @@ def _check(plan: PrefixPlan, kind: str, rows: int, tensors, pool, page_table, ro
     if one != 1 or head != plan.vdim or step % 8 or step < plan.heads * plan.vdim or out.data_ptr() % 16:
         raise ValueError("out must be 16-byte aligned, a row's heads side by side and rows apart, at multiples of 8 values")
     here = torch.cuda.current_device() if plan.device.type == "cuda" else None
-    for name, t, _ in tensors:
-        if t is not None and t.get_device() != here:
-            raise ValueError(f"{name} is on {t.device}, not on the current CUDA device")
+    if not (pool.get_device() == here and out.get_device() == here and page_table.get_device() == here and row_pos.get_device() == here
+            and row_slot.get_device() == here and q.get_device() == here and (q_rot is None or q_rot.get_device() == here)
+            and (extra is None or extra.get_device() == here) and plan.data.get_device() == here):
+        for name, t in (("pool", pool), ("out", out), ("page_table", page_table), ("row_pos", row_pos), ("row_slot", row_slot), ("q", q),
+                        ("q_rot", q_rot), ("gate" if kind == "grouped" else "sink", extra), ("the plan", plan.data)):
+            if t is not None and t.get_device() != here:
+                raise ValueError(f"{name} is on {t.device}, not on the current CUDA device")
     if rows != plan.n_rows or page_table.shape != plan.table_shape:
         raise ValueError(f"the plan was set for {plan.n_rows} rows and a page table of {plan.table_shape and tuple(plan.table_shape)}")
     if torch.cuda.is_current_stream_capturing():
@@ -381,9 +391,7 @@ def group_attend(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, 
         raise ValueError("q: a row's heads must lie side by side")
     if out is None:
         out = torch.empty(R, H, plan.vdim, dtype=dtype, device=q.device)
-    _check(plan, "grouped", R, (("pool", pool, dtype), ("out", out, dtype), ("page_table", page_table, I32), ("row_pos", row_pos, I32),
-                                ("row_slot", row_slot, I32), ("q", q, dtype), ("gate", gate, F32), ("plan", plan.data, I32)),
-           pool, page_table, row_pos, row_slot, out, plan.kv_heads * (D + plan.vdim), scale)
+    _check(plan, "grouped", R, q, None, gate, pool, page_table, row_pos, row_slot, out, plan.kv_heads * (D + plan.vdim), scale)
     if chunk < 0 or (plan.chunk and chunk != plan.chunk):
         raise ValueError(f"the plan is for a chunk of {plan.chunk}" if plan.chunk else "chunk must not be negative")
     if gate is not None and (gate.shape != (R, H) or gate.stride(1) != 1):
@@ -419,10 +427,7 @@ def latent_attend(q_abs: torch.Tensor, q_rot: Optional[torch.Tensor], pool: torc
         rot, rot_head = q_rot.shape[2], q_rot.stride(1)
     if out is None:
         out = torch.empty(R, H, V, dtype=dtype, device=q_abs.device)
-    _check(plan, "latent", R, (("pool", pool, dtype), ("out", out, dtype), ("page_table", page_table, I32), ("row_pos", row_pos, I32),
-                               ("row_slot", row_slot, I32), ("q_abs", q_abs, dtype), ("q_rot", q_rot, dtype), ("sink", sink, F32),
-                               ("plan", plan.data, I32)),
-           pool, page_table, row_pos, row_slot, out, V + rot, scale)
+    _check(plan, "latent", R, q_abs, q_rot, sink, pool, page_table, row_pos, row_slot, out, V + rot, scale)
     if sink is not None and (sink.shape != (H,) or not sink.is_contiguous()):
         raise ValueError(f"sink must be {H} contiguous values")
     a = S.LatentAttendArgs()

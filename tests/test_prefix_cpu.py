@@ -335,8 +335,7 @@ def matching(plan, monkeypatch, rows, shape, capturing=False):
     monkeypatch.setattr(plan, "device", torch.device("cuda"))
     z = lambda *s, dtype=torch.int32: torch.zeros(*s, dtype=dtype)
     pool, out = z(128, 32, dtype=BF16), z(rows, 4, 16, dtype=BF16)
-    named = (("pool", pool, BF16), ("out", out, BF16))
-    prefix._check(plan, "latent", rows, named, pool, z(*shape), z(rows), z(rows), out, 32, 1.0)
+    prefix._check(plan, "latent", rows, out, None, None, pool, z(*shape), z(rows), z(rows), out, 32, 1.0)
 
 
 def test_calls_match_the_rows_and_the_table_of_their_plan(monkeypatch):
