@@ -350,7 +350,7 @@ def _check(plan: PrefixPlan, kind: str, rows: int, q, q_rot, extra, pool, page_t
         raise ValueError("a pool has fewer than 2^31 rows")
     if out.shape != (rows, plan.heads, plan.vdim):
         raise ValueError(f"out must be [{rows}, {plan.heads}, {plan.vdim}]")
-    step, head, one = out.stride()
+    step, head, one = _steps(out)
     if one != 1 or head != plan.vdim or step % 8 or step < plan.heads * plan.vdim or out.data_ptr() % 16:
         raise ValueError("out must be 16-byte aligned, a row's heads side by side and rows apart, at multiples of 8 values")
     here = torch.cuda.current_device() if plan.device.type == "cuda" else None
@@ -367,14 +367,23 @@ def _check(plan: PrefixPlan, kind: str, rows: int, q, q_rot, extra, pool, page_t
         plan.captured = rows if plan.captured is None else min(rows, plan.captured)
 
 
-def _heads(name: str, q: torch.Tensor, heads: int, dtype) -> int:
+def _steps(t: torch.Tensor) -> Tuple[int, int, int]:
+    """Strides of [rows, heads, values]; a dimension of one entry may have any, and gets that of entries side by side."""
+    row, head, one = t.stride()
+    rows, heads, values = t.shape
+    head = values if heads == 1 else head
+    return (heads * head if rows == 1 else row), head, one
+
+
+def _heads(name: str, q: torch.Tensor, heads: int, dtype) -> Tuple[int, int]:
+    """Values between a tensor's rows and between a row's heads."""
     shape = q.shape
     if len(shape) != 3 or shape[1] != heads or q.dtype != dtype or shape[2] % 16 or shape[2] == 0:
         raise ValueError(f"{name} must be [rows, {heads}, a multiple of 16] of {dtype}")
-    row, head, one = q.stride()
+    row, head, one = _steps(q)
     if one != 1 or row % 8 or head % 8 or q.data_ptr() % 16 or row < head * (heads - 1) + shape[2]:
         raise ValueError(f"{name}: values of a head side by side, rows and heads at multiples of 8 values, 16-byte aligned")
-    return row
+    return row, head
 
 
 def group_attend(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, row_pos: torch.Tensor, row_slot: torch.Tensor,
@@ -385,21 +394,21 @@ def group_attend(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, 
     q [rows, heads, dim]; pool [pages * page_tokens, kv_heads * (dim + vdim)]: keys of all key/value heads, then their values; row r
     stands at row_pos[r] of slot row_slot[r] (negative: the row's result is zero) and sees the positions up to its own, within its
     chunk of `chunk` of them where that is not 0.  `gate` [rows, heads] fp32: a head's result times sigmoid(gate)."""
-    ld_q, dtype = _heads("q", q, plan.heads, plan.dtype), plan.dtype
+    (ld_q, step), dtype = _heads("q", q, plan.heads, plan.dtype), plan.dtype
     R, H, D = q.shape
-    if q.stride(1) != D:
+    if step != D:
         raise ValueError("q: a row's heads must lie side by side")
     if out is None:
         out = torch.empty(R, H, plan.vdim, dtype=dtype, device=q.device)
     _check(plan, "grouped", R, q, None, gate, pool, page_table, row_pos, row_slot, out, plan.kv_heads * (D + plan.vdim), scale)
     if chunk < 0 or (plan.chunk and chunk != plan.chunk):
         raise ValueError(f"the plan is for a chunk of {plan.chunk}" if plan.chunk else "chunk must not be negative")
-    if gate is not None and (gate.shape != (R, H) or gate.stride(1) != 1):
+    if gate is not None and (gate.shape != (R, H) or (H > 1 and gate.stride(1) != 1)):
         raise ValueError(f"gate must be [{R}, {H}] with a row's values side by side")
     slots, max_pages = page_table.shape
     a = S.GroupAttendArgs(q.data_ptr(), pool.data_ptr(), page_table.data_ptr(), row_pos.data_ptr(), row_slot.data_ptr(), out.data_ptr(),
                           plan.status.data_ptr(), S.ProjArgs(gate.data_ptr(), 0, gate.stride(0), 1, 0, 0) if gate is not None else S.NO_PROJ, S.NO_PROJ, None,
-                          ld_q, scale, R, H, plan.kv_heads, D, plan.vdim, chunk, 1, slots, 0, out.stride(0), max_pages, plan.page_tokens,
+                          ld_q, scale, R, H, plan.kv_heads, D, plan.vdim, chunk, 1, slots, 0, _steps(out)[0], max_pages, plan.page_tokens,
                           int(dtype == F32), pool.shape[0] // plan.page_tokens, 0)
     launch_group(a, plan)
     return out
@@ -413,18 +422,18 @@ def latent_attend(q_abs: torch.Tensor, q_rot: Optional[torch.Tensor], pool: torc
     q_abs [rows, heads, latent], q_rot [rows, heads, rot] (None: no rotated part); pool [pages * page_tokens, latent + rot]: a
     position's latent, which is key and value of every head, and its rotated key part.  `sink` [heads] fp32: an extra logit in a
     head's denominator."""
-    ld_abs, dtype = _heads("q_abs", q_abs, plan.heads, plan.dtype), plan.dtype
+    (ld_abs, step), dtype = _heads("q_abs", q_abs, plan.heads, plan.dtype), plan.dtype
     R, H, V = q_abs.shape
     if V != plan.vdim:
         raise ValueError(f"q_abs: {V} latent values, the plan has {plan.vdim}")
-    if q_abs.stride(1) != V:
+    if step != V:
         raise ValueError("q_abs: a row's heads must lie side by side")
     rot = ld_rot = rot_head = 0
     if q_rot is not None:
-        ld_rot = _heads("q_rot", q_rot, H, dtype)
+        ld_rot, rot_head = _heads("q_rot", q_rot, H, dtype)
         if q_rot.shape[0] != R:
             raise ValueError("q_rot must have as many rows as q_abs")
-        rot, rot_head = q_rot.shape[2], q_rot.stride(1)
+        rot = q_rot.shape[2]
     if out is None:
         out = torch.empty(R, H, V, dtype=dtype, device=q_abs.device)
     _check(plan, "latent", R, q_abs, q_rot, sink, pool, page_table, row_pos, row_slot, out, V + rot, scale)
@@ -435,5 +444,5 @@ def latent_attend(q_abs: torch.Tensor, q_rot: Optional[torch.Tensor], pool: torc
     a.pool, a.page_table, a.row_pos, a.row_slot = pool.data_ptr(), page_table.data_ptr(), row_pos.data_ptr(), row_slot.data_ptr()
     a.scale, a.rows, a.heads, a.kv_pad, a.row_len = scale, R, H, V, V + rot
     a.max_pages, a.page_tokens, a.f32, a.status = page_table.shape[1], plan.page_tokens, int(dtype == F32), plan.status.data_ptr()
-    launch_latent(a, plan, pool.shape[0] // plan.page_tokens, sink, out, out.stride(0))
+    launch_latent(a, plan, pool.shape[0] // plan.page_tokens, sink, out, _steps(out)[0])
     return out

@@ -290,6 +290,22 @@ def test_rows_beyond_the_pass_and_strided_arguments(kind):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,groups,alone", [(1, [], 1), (1, [(3, 4)], 0), (8, [], 1)])
+def test_one_row_or_one_head_with_any_stride(kind, heads, groups, alone):
+    """A dimension of one entry has no neighbour: its stride means nothing."""
+    p = Pass(kind, heads=heads, dim=64, vdim=64 if kind == "grouped" else 48, groups=groups, alone=alone)
+    plan, (R, H, V) = p.plan(), (p.R, p.H, p.V)
+    want, tol = p.expected()
+    odd = lambda t: t.as_strided(t.shape, tuple(s if n > 1 else 12345 + 2 * k for k, (n, s) in enumerate(zip(t.shape, t.stride()))))
+    a, out = (p.pool, p.d_tables, p.d_pos, p.d_slot, plan), odd(torch.empty(R, H, V, dtype=BF16, device="cuda"))
+    if kind == "grouped":
+        prefix().group_attend(odd(p.q), *a, scale=p.scale, gate=odd(p.gate), out=out)
+    else:
+        prefix().latent_attend(odd(p.q[..., :V].contiguous()), odd(p.q[..., V:].contiguous()), *a, scale=p.scale, sink=p.sink, out=out)
+    assert ((out.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_repeated_calls_agree_bit_for_bit(kind, dtype):
     p = Pass(kind, groups=[(9, 8)], dtype=dtype, **SMALL[kind])
