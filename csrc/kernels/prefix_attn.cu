@@ -273,15 +273,20 @@ static int run_simple(const SimpleArgs& p, const ds41_prefix_plan& plan, int f32
   return f32 ? dispatch_simple<float, false>(p, plan, st) : dispatch_simple<__nv_bfloat16, false>(p, plan, st);
 }
 
-// A warp joins 128 columns of a (row, head): the lanes find the parts' weights, then every lane sums four columns over the parts, eight
+// A warp joins 128 columns of a (row, head): the lanes find the parts' weights, then every lane sums four columns over the parts, PARTS
 // of them under way together.  Rows without a slot have no parts and become zero.  The launch also keeps the convolution's last
 // inputs where the attention has one (ds41_group.cuh).
-template <typename T>
-__global__ void __launch_bounds__(128) prefix_join_kernel(const ds41_prefix_plan plan, const float* sink, const ds41_proj gate, int rows,
-                                                          int heads, int vp, T* out, int ld_out, const ds41_group_attend_args keep) {
+// A chain of loads from L2: small launches want many of them under way (94 registers), large ones many warps (56).  Whole calls with 8 / 4
+// parts: 37 rows of 6 heads in 13 parts 13.5 / 15.2 us, 32 rows of 32 heads 22.8 / 23.8 (1024 warps); 32 rows x 32 heads x 512 columns
+// (4096 warps) 31.7 / 30.3 us, 128 rows (16384) 204 / 198.
+template <typename T, int PARTS>
+__global__ void __launch_bounds__(128, PARTS == 8 ? 1 : 9)
+prefix_join_kernel(const ds41_prefix_plan plan, const float* sink, const ds41_proj gate, int rows, int heads, int vp, T* out, int ld_out,
+                   const ds41_group_attend_args keep) {
   const int lane = threadIdx.x & 31, strips = (vp + 127) / 128;
   const long long w = 4ll * blockIdx.x + (threadIdx.x >> 5);
-  const int r = static_cast<int>(w / (heads * strips)), h = static_cast<int>(w / strips % heads), c = static_cast<int>(w % strips) * 128 + 4 * lane;
+  const int r = static_cast<int>(w / (heads * strips)), h = static_cast<int>(w / strips % heads);
+  const int c = static_cast<int>(w % strips) * 128 + 4 * lane;
   pdl_launch_dependents();
   // the plan was copied to the device, not computed there: it may be read before the wait
   const int n = r < rows ? plan.parts[r] : 0;
@@ -294,27 +299,27 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const ds41_prefix_plan
   const float2* ml = reinterpret_cast<const float2*>(plan.part_ml) + cell;
   const float* part = plan.part_o + cell * vp + c;
   const long long step = 1ll * heads * vp;
-  float all = sk;
-  for (int s = lane; s < n; s += 32) all = fmaxf(all, ml[1ll * s * heads].x);
+  float2 mine = lane < n ? ml[1ll * lane * heads] : make_float2(-INFINITY, 0.f);
+  float all = fmaxf(sk, mine.x);
+  for (int s = lane + 32; s < n; s += 32) all = fmaxf(all, ml[1ll * s * heads].x);
   all = warp_max(all);
   float den = sink != nullptr && lane == 0 && all > -INFINITY ? exp2f(sk - all) : 0.f;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int s0 = 0; s0 < n; s0 += 32) {
-    float2 mine = make_float2(-INFINITY, 0.f);
-    if (s0 + lane < n) mine = ml[1ll * (s0 + lane) * heads];
+    if (s0 > 0) mine = s0 + lane < n ? ml[1ll * (s0 + lane) * heads] : make_float2(-INFINITY, 0.f);
     const float e = mine.x > -INFINITY ? exp2f(mine.x - all) : 0.f;
     den += e * mine.y;
-    for (int k0 = 0; k0 < 32 && s0 + k0 < n; k0 += 8) {
-      float4 o[8];
-      float f[8];
+    for (int k0 = 0; k0 < 32 && s0 + k0 < n; k0 += PARTS) {
+      float4 o[PARTS];
+      float f[PARTS];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < PARTS; ++k) {
         f[k] = __shfl_sync(0xffffffffu, e, k0 + k);
         // a part without a weight may hold anything: nothing may have been written
         if (f[k] > 0.f && c < vp) o[k] = *reinterpret_cast<const float4*>(part + (s0 + k0 + k) * step);
       }
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
+      for (int k = 0; k < PARTS; ++k)
         if (f[k] > 0.f && c < vp) {
           a.x += f[k] * o[k].x;
           a.y += f[k] * o[k].y;
@@ -332,8 +337,9 @@ template <typename T>
 static int launch_join(const ds41_prefix_plan& plan, const float* sink, const ds41_proj& gate, int rows, int heads, int vp, void* out,
                        int ld_out, const ds41_group_attend_args& keep, cudaStream_t st) {
   const long long warps = 1ll * rows * heads * ((vp + 127) / 128);
-  return launch_pdl(prefix_join_kernel<T>, dim3(static_cast<unsigned>((warps + 3) / 4)), dim3(128), 0, st, plan, sink, gate, rows, heads,
-                    vp, static_cast<T*>(out), ld_out, keep);
+  return launch_pdl(warps < 20 * sm_count() ? prefix_join_kernel<T, 8> : prefix_join_kernel<T, 4>,
+                    dim3(static_cast<unsigned>((warps + 3) / 4)), dim3(128), 0, st, plan, sink, gate, rows, heads, vp, static_cast<T*>(out),
+                    ld_out, keep);
 }
 
 }  // namespace ds41
