@@ -284,9 +284,9 @@ __global__ void __launch_bounds__(128, PARTS == 8 ? 1 : 9)
 prefix_join_kernel(const ds41_prefix_plan plan, const float* sink, const ds41_proj gate, int rows, int heads, int vp, T* out, int ld_out,
                    const ds41_group_attend_args keep) {
   const int lane = threadIdx.x & 31, strips = (vp + 127) / 128;
-  const long long w = 4ll * blockIdx.x + (threadIdx.x >> 5);
-  const int r = static_cast<int>(w / (heads * strips)), h = static_cast<int>(w / strips % heads);
-  const int c = static_cast<int>(w % strips) * 128 + 4 * lane;
+  const unsigned w = 4 * blockIdx.x + (threadIdx.x >> 5);
+  const unsigned pair = w / strips;
+  const int r = pair / heads, h = pair % heads, c = (w - pair * strips) * 128 + 4 * lane;
   pdl_launch_dependents();
   // the plan was copied to the device, not computed there: it may be read before the wait
   const int n = r < rows ? plan.parts[r] : 0;
@@ -295,7 +295,7 @@ prefix_join_kernel(const ds41_prefix_plan plan, const float* sink, const ds41_pr
   if (r >= rows) return;
   const float sk = sink != nullptr ? sink[h] * 1.4426950408889634f : -INFINITY;
   if (keep.taps > 1 && keep.row_slot[r] >= 0)
-    keep_inputs(keep, r, keep.row_slot[r], keep.row_pos[r], static_cast<int>(w % (heads * strips)), heads * strips, lane, 32);
+    keep_inputs(keep, r, keep.row_slot[r], keep.row_pos[r], w % (heads * strips), heads * strips, lane, 32);
   const float2* ml = reinterpret_cast<const float2*>(plan.part_ml) + cell;
   const float* part = plan.part_o + cell * vp + c;
   const long long step = 1ll * heads * vp;
@@ -337,6 +337,7 @@ template <typename T>
 static int launch_join(const ds41_prefix_plan& plan, const float* sink, const ds41_proj& gate, int rows, int heads, int vp, void* out,
                        int ld_out, const ds41_group_attend_args& keep, cudaStream_t st) {
   const long long warps = 1ll * rows * heads * ((vp + 127) / 128);
+  if (warps >= 1ll << 31) return cudaErrorInvalidValue;
   return launch_pdl(warps < 20 * sm_count() ? prefix_join_kernel<T, 8> : prefix_join_kernel<T, 4>,
                     dim3(static_cast<unsigned>((warps + 3) / 4)), dim3(128), 0, st, plan, sink, gate, rows, heads, vp, static_cast<T*>(out),
                     ld_out, keep);
