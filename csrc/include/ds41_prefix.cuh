@@ -25,20 +25,27 @@ __device__ __forceinline__ PrefixUnit prefix_unit(const ds41_prefix_plan& p, int
 __device__ __forceinline__ int prefix_row(const ds41_prefix_plan& p, const PrefixUnit& u, int i) {
   return u.tail ? u.first + i : p.order[u.first + i];
 }
-// Whole warps: the keys [first, end) that a unit's rows see.  `first` is a page's; a chunk's border may lie inside.  Behind `end` even
-// shared pages may hold anything, as rows may stand inside them.  In two steps, so that the positions of several units can be under
+// Whole warps: the keys [first, end) that a unit's rows see.  `first` is a page's; a chunk's border may lie inside, and between the
+// windows of rows in different chunks there may be places that nobody sees.  Those and the ones behind `end`, which shared pages have
+// as well since rows may stand inside them, may hold anything.  In two steps, so that the positions of several units can be under
 // way together.
 struct PrefixRows {
-  int low, high;                       // of this lane's rows
+  int low, high;                       // of this lane's rows that see any of the unit's keys
+  int wide_low, wide_high;             // the longest window of one of them, inside the unit
 };
 __device__ __forceinline__ PrefixRows prefix_rows(const ds41_prefix_plan& p, const PrefixUnit& u, const int* row_pos, const int* row_slot,
                                                   int chunk) {
-  PrefixRows v = {u.key1, 0};
+  PrefixRows v = {u.key1, 0, u.key0, u.key0};
   for (int i = threadIdx.x & 31; i < u.rows; i += 32) {
     const int r = prefix_row(p, u, i), pos = row_pos[r];
-    if (row_slot[r] < 0) continue;
-    v.low = min(v.low, chunk > 0 ? pos - pos % chunk : 0);
-    v.high = max(v.high, pos + 1);
+    const int low = chunk > 0 ? pos - pos % chunk : 0, from = max(low, u.key0), high = min(pos + 1, u.key1);
+    if (row_slot[r] < 0 || from >= high) continue;
+    v.low = min(v.low, low);
+    v.high = max(v.high, high);
+    if (high - from > v.wide_high - v.wide_low) {
+      v.wide_low = from;
+      v.wide_high = high;
+    }
   }
   return v;
 }
@@ -50,6 +57,30 @@ __device__ __forceinline__ void prefix_span(const PrefixUnit& u, PrefixRows v, i
   }
   first = chunk > 0 ? max(u.key0, v.low - v.low % page_tokens) : u.key0;
   end = max(first, min(u.key1, v.high));
+}
+// Whole warps: the longest window of all lanes' rows.
+__device__ __forceinline__ void prefix_widest(const PrefixRows& v, int& low, int& high) {
+  low = v.wide_low;
+  high = v.wide_high;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    const int l = __shfl_xor_sync(0xffffffffu, low, o), h = __shfl_xor_sync(0xffffffffu, high, o);
+    if (h - l > high - low) {
+      low = l;
+      high = h;
+    }
+  }
+}
+// Whole warps: which of the 64 places from `key` on are seen by one of this lane's rows of a unit.
+__device__ __forceinline__ unsigned long long prefix_seen(const ds41_prefix_plan& p, const PrefixUnit& u, const int* row_pos,
+                                                          const int* row_slot, int chunk, int key) {
+  unsigned long long seen = 0;
+  for (int i = threadIdx.x & 31; i < u.rows; i += 32) {
+    const int r = prefix_row(p, u, i), pos = row_pos[r];
+    const int from = max(pos - pos % chunk - key, 0), to = min(min(pos + 1, u.key1) - key, 64);
+    if (row_slot[r] >= 0 && from < to) seen |= (~0ull >> (64 - (to - from))) << from;
+  }
+  return seen;
 }
 
 // Two 32-bit operations in one instruction.

@@ -49,10 +49,11 @@ struct PrefixGroupParams {
 };
 
 // What a CTA's two tiles do next, as the producer found it: unit t walks `tiles[t]` key tiles from `first[t]` on, and nobody sees
-// `end[t]` or what follows.  both: they walk the same ones.
+// `end[t]` or what follows.  both: they walk the same ones.  Key tiles inside [safe[t], safe_end[t]) have no place that nobody sees.
 struct __align__(16) GroupWork {
   PrefixUnit unit[2];
   int first[2], end[2], tiles[2], base, both;              // base: number of the first key tile in the order of the copies
+  int safe[2], safe_end[2];
   int row[2][32];                                          // pool rows of the first 32 boxes of their keys
 };
 
@@ -70,9 +71,10 @@ struct GroupShared {                           // behind the tiles
   uint64_t p_full[2][2];                       // P written, O rescaled
   uint64_t o_next[2];                          // the unit's last product but one
   uint64_t o_full[2];                          // the unit's last product
-  uint64_t v_here[2];                          // the values of a last tile that nobody sees whole, for the softmax
+  uint64_t v_here[2];                          // the values of a key tile with places that nobody sees, for the softmax
   int k_asked, v_asked;                        // copies under way or done: a place's barrier is at the phase of the last of these
-  uint32_t tmem, pad[1];
+  int v_place[2];                              // where in the ring those are
+  uint32_t tmem, pad[3];
   GroupWork info[kPgInfos];
   int4 row[2][kPgTile];                        // of a unit's row: pass row, visible keys [y, z), cell
 };
@@ -159,6 +161,20 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap keys, const __grid_const
         first[0] = first[1] = min(first[0], first[1]);
         end[0] = end[1] = max(end[0], end[1]);
       }
+      // without chunks every place before `end` is seen by the row that stands last; with them, a row's window vouches for its tiles
+      int safe[2] = {first[0], first[1]}, safe_end[2] = {end[0], end[1]};
+      if (p.chunk > 0) {
+        prefix_widest(rows_a, safe[0], safe_end[0]);
+        prefix_widest(rows_b, safe[1], safe_end[1]);
+        if (both) {
+          const int t = safe_end[1] - safe[1] > safe_end[0] - safe[0];
+          safe[0] = safe[1] = t ? safe[1] : safe[0];
+          safe_end[0] = safe_end[1] = t ? safe_end[1] : safe_end[0];
+        }
+      }
+      // what lies behind the unit's keys is read as zeros
+      if (safe_end[0] == a.key1) safe_end[0] = 0x7fffffff;
+      if (safe_end[1] == b.key1) safe_end[1] = 0x7fffffff;
       if (first[0] != a.key0) row_a = locate(a.slot, first[0], end[0], 0);
       if (first[1] != b.key0) row_b = locate(b.slot, first[1], end[1], 0);
       if (first[0] + lane * p.box >= end[0]) row_a = p.hidden_row;
@@ -174,6 +190,8 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap keys, const __grid_const
         w.first[lane] = lane ? first[1] : first[0];
         w.end[lane] = lane ? end[1] : end[0];
         w.tiles[lane] = lane ? tiles[1] : tiles[0];
+        w.safe[lane] = lane ? safe[1] : safe[0];
+        w.safe_end[lane] = lane ? safe_end[1] : safe_end[0];
         w.base = base;
         w.both = both;
       }
@@ -277,7 +295,8 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap keys, const __grid_const
         if (!ok) break;
         const GroupWork& w = sh.info[turn % kPgInfos];
         const int n = w.tiles[t], base = w.base, least = min(w.tiles[0], w.tiles[1]);
-        const bool both = w.both != 0, partial = w.end[t] < w.unit[t].key1;
+        const int first = w.first[t], safe = w.safe[t], safe_end = w.safe_end[t];
+        const bool both = w.both != 0;
         mbar_arrive(&sh.info_empty[turn % kPgInfos]);
         if (n == 0) continue;
         auto scores = [&](int j) {
@@ -306,7 +325,11 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap keys, const __grid_const
           const int at = copy_index(both, base, least, t, j), stage = at & mask, place = done & 1;
           ok = landed(&sh.v_asked, v_seen, sh.v_full, at, 473);
           if (!ok) break;
-          if (partial && j + 1 == n) mbar_arrive(&sh.v_here[t]);
+          const int key0 = first + j * kPgKeys;
+          if (key0 < safe || key0 > safe_end - kPgKeys) {
+            sh.v_place[t] = stage;
+            mbar_arrive(&sh.v_here[t]);
+          }
           ok = mbar_wait(&sh.p_full[t][place], (done >> 1) & 1, p.status, 474);
           if (!ok) break;
           tc_fence_after();
@@ -323,14 +346,14 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap keys, const __grid_const
     __syncwarp();
   } else {
     // the roles that follow one tile: its work at a turn, once it is known; whole warps
-    auto work = [&](int turn, int t, PrefixUnit& unit, int& first, int& end, int& last) {
+    auto work = [&](int turn, int t, PrefixUnit& unit, int& first, int& safe, int& safe_end) {
       ok = __all_sync(0xffffffffu, mbar_wait(&sh.info_full[turn % kPgInfos], (turn / kPgInfos) & 1, p.status, 462)) != 0;
       if (!ok) return 0;
       const GroupWork& w = sh.info[turn % kPgInfos];
       unit = w.unit[t];
       first = w.first[t];
-      end = w.end[t];
-      last = copy_index(w.both != 0, w.base, min(w.tiles[0], w.tiles[1]), t, w.tiles[t] - 1);
+      safe = w.safe[t];
+      safe_end = w.safe_end[t];
       return w.tiles[t];
     };
     auto work_read = [&](int turn) {
@@ -338,7 +361,7 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap keys, const __grid_const
       if (lane == 0) mbar_arrive(&sh.info_empty[turn % kPgInfos]);
     };
     PrefixUnit unit;
-    int first, end, last;                                // last: the last tile's number
+    int first, safe, safe_end;
     if (warp >= 10) {
       // A row's queries lie side by side: pieces of 16 bytes by neighbouring lanes, or whole rows where they are shorter than a warp.
       const int t = warp - 10, pieces = p.n * p.dp / 8, per = max(1, 32 / pieces), sub = pieces < 32 ? lane / pieces : 0;
@@ -390,9 +413,9 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap keys, const __grid_const
       const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
       const uint32_t o_t = tmem + lanes + 256 + t * 128;
       const int mine_row = mine / p.n, mine_head = mine - mine_row * p.n;
-      int tiles = 0, done = 0, pairs = 0, tails = 0;     // tiles of S; units with keys, with two tiles or more, with a last one cut short
+      int tiles = 0, done = 0, pairs = 0, cut = 0;       // tiles of S; units with keys, with two tiles or more; key tiles with unseen places
       for (int turn = 0; turn < turns; ++turn) {
-        const int n = work(turn, t, unit, first, end, last);
+        const int n = work(turn, t, unit, first, safe, safe_end);
         if (!ok) break;
         work_read(turn);
         if (n == 0) {                                    // nothing for any of its rows
@@ -496,16 +519,31 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap keys, const __grid_const
             sums[0] = add2(sums[0], sums[1]);
             l += sums[0].x + sums[0].y;
           }
-          if (end < unit.key1 && j + 1 == n) {
-            // Places behind the last position that a row sees may hold anything, and a weight of zero does not take a NaN or an
-            // infinity away: their values become zeros, two threads to a place.
-            ok = __all_sync(0xffffffffu, mbar_wait(&sh.v_here[t], tails & 1, p.status, 484 + t)) != 0;
+          if (key0 < safe || key0 > safe_end - kPgKeys) {
+            // Places that no row sees may hold anything, and a weight of zero does not take a NaN or an infinity away: their values
+            // become zeros, two threads to a place.  Behind the last position of all rows that is known; a tile with a chunk's border,
+            // or between the windows of rows in different chunks, asks the rows of whoever walks these keys.
+            uint32_t seen[2];
+            if (p.chunk > 0) {
+              const PrefixUnit other = prefix_unit(plan, 2 * (static_cast<int>(blockIdx.x) + turn * static_cast<int>(gridDim.x)) + (t ^ 1));
+              unsigned long long mask = prefix_seen(plan, unit, p.row_pos, p.row_slot, p.chunk, key0);
+              if (!unit.tail && !other.tail && other.slot == unit.slot && other.key0 == unit.key0 && other.key1 == unit.key1 &&
+                  other.head == unit.head)
+                mask |= prefix_seen(plan, other, p.row_pos, p.row_slot, p.chunk, key0);
+              seen[0] = __reduce_or_sync(0xffffffffu, static_cast<uint32_t>(mask));
+              seen[1] = __reduce_or_sync(0xffffffffu, static_cast<uint32_t>(mask >> 32));
+            } else {
+              const int shown = safe_end - key0;            // 1 to 63: the tile has been asked for
+              seen[0] = shown >= 32 ? 0xffffffffu : (1u << shown) - 1;
+              seen[1] = (1u << max(shown - 32, 0)) - 1;
+            }
+            ok = __all_sync(0xffffffffu, mbar_wait(&sh.v_here[t], cut & 1, p.status, 484 + t)) != 0;
             if (!ok) break;
-            ++tails;
-            const int key = mine & (kPgKeys - 1);
-            if (key0 + key >= end)
+            ++cut;
+            const int key = mine & (kPgKeys - 1), at = sh.v_place[t];
+            if (!((key < 32 ? seen[0] : seen[1]) >> (key & 31) & 1))
               for (int i = 8 * (mine / kPgKeys); i < 8 * p.vc; i += (i & 7) == 7 ? 9 : 1)
-                *reinterpret_cast<uint4*>(s_v + (last & (p.stages - 1)) * v_bytes + (i >> 3) * kPgKeyChunk + key * 128 + (i & 7) * 16) =
+                *reinterpret_cast<uint4*>(s_v + at * v_bytes + (i >> 3) * kPgKeyChunk + key * 128 + (i & 7) * 16) =
                     make_uint4(0, 0, 0, 0);
             fence_async_smem();
           }

@@ -1,0 +1,60 @@
+"""Attention over a shared prefix where a row's window, its numbers or its plan are out of the ordinary.
+
+Tolerances and expected values are those of test_prefix_gpu.Pass.
+"""
+import math
+
+import pytest
+import torch
+
+from test_prefix_gpu import BF16, F32, SMALL, Pass
+
+pytestmark = pytest.mark.gpu
+
+
+def poison_unseen(p):
+    """NaN and infinities wherever no row of the pass sees: behind its position, and before its chunk."""
+    seen = torch.zeros(p.pages * p.P, dtype=torch.bool)
+    for s, pos in zip(p.row_slot, p.row_pos):
+        if s >= 0:
+            at = torch.arange(pos - pos % p.chunk if p.chunk else 0, pos + 1)
+            seen[p.tables[s].long()[at // p.P] * p.P + at % p.P] = True
+    hidden = (~seen).nonzero().flatten().cuda()
+    bad = torch.tensor([math.nan, math.inf, -math.inf], device="cuda")
+    p.pool[hidden] = bad[hidden % 3][:, None].to(p.dtype)
+    return hidden.numel()
+
+
+WIDE = dict(heads=32, kv_heads=8, dim=128, vdim=128)
+ODD = dict(heads=6, kv_heads=2, dim=32, vdim=48)
+CHUNKS = [
+    (SMALL["grouped"], dict(chunk=96, P=64, groups=[(1, 1)], own=60)),
+    (SMALL["grouped"], dict(chunk=100, P=32, groups=[(20, 9)], own=300)),
+    (SMALL["grouped"], dict(chunk=100, P=32, groups=[(60, 9), (3, 2)], early=True)),
+    (SMALL["grouped"], dict(chunk=200, P=64, groups=[(70, 5)], early=True, own=150)),
+    (SMALL["grouped"], dict(chunk=96, P=128, groups=[(9, 3)], early=True)),
+    (SMALL["grouped"], dict(chunk=40, P=256, groups=[(40, 2)], early=True)),
+    (SMALL["grouped"], dict(chunk=100, P=16, groups=[(33, 20)], early=True, pads=2, alone=2)),
+    (SMALL["grouped"], dict(chunk=30, P=8, groups=[(12, 30)], own=90)),
+    (SMALL["grouped"], dict(chunk=50, P=64, groups=[(12, 4)], per_slot=3)),
+    (SMALL["grouped"], dict(chunk=7, P=64, groups=[(130, 6)], early=True)),
+    (WIDE, dict(chunk=300, P=64, groups=[(65, 12)], early=True)),
+    (WIDE, dict(chunk=1000, P=64, groups=[(40, 15)], own=300)),
+    (ODD, dict(chunk=96, P=32, groups=[(90, 9)], early=True, alone=3)),
+    (dict(heads=8, kv_heads=8, dim=64, vdim=64), dict(chunk=100, P=64, groups=[(130, 5)], early=True)),
+    (SMALL["grouped"], dict(chunk=100, P=48, groups=[(20, 5)], early=True)),
+    (SMALL["grouped"], dict(chunk=100, P=32, groups=[(20, 9)], early=True, dtype=F32)),
+]
+
+
+@pytest.mark.parametrize("i", range(len(CHUNKS)))
+def test_places_outside_every_chunk_may_hold_anything(i):
+    """A chunk's border inside a page, and gaps between the windows of rows that share a range."""
+    sizes, kw = CHUNKS[i]
+    p = Pass("grouped", seed=300 + i, **sizes, **kw)
+    assert poison_unseen(p) > 0
+    plan = p.plan()
+    p.check(plan)
+    later = p.plan(chunk=p.chunk)                            # a plan that leaves out what lies before the rows' chunks
+    later.set(p.row_slot, p.tables, [x + 1 for x in p.row_pos])
+    p.check(later)
