@@ -294,8 +294,9 @@ prefix_join_kernel(const ds41_prefix_plan plan, const float* sink, const ds41_pr
   pdl_wait();
   if (r >= rows) return;
   const float sk = sink != nullptr ? sink[h] * 1.4426950408889634f : -INFINITY;
-  if (keep.taps > 1 && keep.row_slot[r] >= 0)
-    keep_inputs(keep, r, keep.row_slot[r], keep.row_pos[r], w % (heads * strips), heads * strips, lane, 32);
+  const int slot = keep.row_slot[r];
+  if (keep.taps > 1 && slot >= 0)
+    keep_inputs(keep, r, slot, keep.row_pos[r], w % (heads * strips), heads * strips, lane, 32);
   const float2* ml = reinterpret_cast<const float2*>(plan.part_ml) + cell;
   const float* part = plan.part_o + cell * vp + c;
   const long long step = 1ll * heads * vp;
@@ -329,7 +330,8 @@ prefix_join_kernel(const ds41_prefix_plan plan, const float* sink, const ds41_pr
     }
   }
   den = warp_sum(den);
-  const float f = (den > 0.f ? 1.0f / den : 0.f) * (gate.data != nullptr ? sigmoid_f32(proj_at(gate, r, h)) : 1.f);
+  // a NaN among the scores leaves its part a sum of NaN, whatever the maximum is
+  const float f = slot < 0 ? 0.f : (den > 0.f ? 1.0f / den : den) * (gate.data != nullptr ? sigmoid_f32(proj_at(gate, r, h)) : 1.f);
   if (c < vp) store4(out + 1ll * r * ld_out + h * vp + c, make_float4(a.x * f, a.y * f, a.z * f, a.w * f));
 }
 
@@ -394,6 +396,7 @@ extern "C" int ds41_prefix_latent(const ds41_latent_attend_args* a, const ds41_p
   const ds41_proj none{};
   ds41_group_attend_args keep{};
   keep.taps = 1;
+  keep.row_slot = a->row_slot;
   return a->f32 ? launch_join<float>(*plan, sink, none, a->rows, a->heads, a->kv_pad, out, ld_out, keep, st)
                 : launch_join<__nv_bfloat16>(*plan, sink, none, a->rows, a->heads, a->kv_pad, out, ld_out, keep, st);
 }

@@ -463,7 +463,7 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[(kt - 1) % kPlSets], ((kt - 1) / kPlSets) & 1, p.status, 526)) != 0;
       tc_fence_after();
       const float all = s_top[mine];
-      s_sum[set * kPlQueries + mine] = m == -INFINITY ? 0.f : l * ex2_approx(m - all);
+      s_sum[set * kPlQueries + mine] = m == -INFINITY ? l : l * ex2_approx(m - all);      // without a maximum: 0, or NaN
       named_barrier(1 + quad, 32 * kPlSets);
       l = s_sum[mine];
 #pragma unroll

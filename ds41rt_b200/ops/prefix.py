@@ -11,7 +11,9 @@ It also holds the workspace of the calls, so calls with one plan, and `set()`, f
 or graphs that replay at the same time, need a plan each.  A captured call reads the plan from device memory: after `set()` a replay
 uses the new one, which may not have more rows than the call that was captured.
 
-What no row of a pass sees may hold anything, NaN included.
+What no row of a pass sees may hold anything, NaN included.  A NaN that a row does meet, in its query, a key, a value, a gate or a
+sink, is in its result; one in a value that only some rows of a range see may be in the others' as well, as the tensor cores multiply
+it by their weight of zero.
 """
 from __future__ import annotations
 

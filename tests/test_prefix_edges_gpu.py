@@ -58,3 +58,47 @@ def test_places_outside_every_chunk_may_hold_anything(i):
     later = p.plan(chunk=p.chunk)                            # a plan that leaves out what lies before the rows' chunks
     later.set(p.row_slot, p.tables, [x + 1 for x in p.row_pos])
     p.check(later)
+
+
+FORMS = [("grouped", dict(SMALL["grouped"])), ("grouped", dict(SMALL["grouped"], P=48)), ("grouped", dict(SMALL["grouped"], dtype=F32)),
+         ("grouped", dict(WIDE)), ("latent", dict(SMALL["latent"])), ("latent", dict(heads=16, dim=576, vdim=512)),
+         ("latent", dict(SMALL["latent"], P=48)), ("latent", dict(heads=4, dim=48, vdim=32, dtype=F32))]
+
+
+@pytest.mark.parametrize("i", range(len(FORMS)))
+def test_results_that_are_no_numbers_are_not_hidden(i):
+    """NaN and infinities in a query, in a request's only own key, in a value, in a sink or gate: the definition's NaN, and nobody else's."""
+    kind, sizes = FORMS[i]
+    for case in range(6):
+        p = Pass(kind, groups=[(9, 5), (4, 2)], alone=2, pads=1, own=130, seed=10 * i + case, **sizes)
+        live = [r for r, s in enumerate(p.row_slot) if s >= 0]
+        a, b = live[0], live[-1]
+        none = p.row_slot.index(-1)                          # a row without a slot gives zeros whatever stands in it
+        p.q[none], p.gate[none] = math.nan, math.nan
+        if case == 0:
+            p.q[a, 1] = math.nan
+            p.q[b] = math.nan
+        elif case == 1:
+            p.q[a, :, 3] = math.inf
+            p.q[b, 0, 0] = -math.inf
+        elif case == 2:                                      # the request's own part is this key alone
+            r = next(r for r in live if p.row_pos[r] > 2 * p.P)
+            lead = p.tables[p.row_slot[r]].tolist()
+            shared = next(k for k, page in enumerate(lead) if not any(page == int(p.tables[s][k]) for s in p.row_slot if s >= 0 and s != p.row_slot[r]))
+            p.row_pos[r] = shared * p.P
+            p.d_pos = p.dev(p.row_pos)
+            p.pool[lead[shared] * p.P] = math.nan
+        elif case == 3:
+            s, pos = p.row_slot[a], p.row_pos[a]
+            p.pool[int(p.tables[s, pos // p.P]) * p.P + pos % p.P, -1 if kind == "grouped" else 5] = math.nan
+        elif kind == "latent":
+            p.sink[:3] = torch.tensor([math.nan, -math.inf, math.inf] if case == 4 else [1e30, -1e30, 80.0])
+        else:
+            p.gate[a, 0], p.gate[b, 1], p.gate[b, 0] = (math.nan, math.inf, -math.inf) if case == 4 else (1e30, -1e30, 80.0)
+        plan = p.plan()
+        got = p.run(plan)
+        plan.check_status()
+        want, tol = p.expected()
+        assert case == 5 or want.isnan().any()
+        assert torch.equal(got.isnan(), want.isnan()), (case, got.isnan().sum().item(), want.isnan().sum().item())
+        assert ((got.double() - want).abs() <= tol)[~want.isnan()].all(), case
