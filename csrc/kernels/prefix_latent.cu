@@ -14,6 +14,9 @@
 //                   own is known
 //   warp 8        : TMA producer, page by page
 //   warp 9        : tcgen05.mma issue, in whichever order their inputs come: S = Q K^T as soon as the last S is in registers, O += P V
+//   warp 10       : tells the other CTA which of its scores have been read.  That takes a release that the whole cluster sees, which
+//                   also waits for the scores that a softmax warp has just sent: by those warps 128 rows of 32 heads over 16000 keys take
+//                   236 us, 212 so
 // The running maximum is raised when it grew by more than 2^8 only.  P is rounded to bf16 as the operand of the second product; sums
 // stay in 32 bits.
 //
@@ -28,7 +31,7 @@
 
 namespace ds41 {
 
-constexpr int kPlSets = 2, kPlThreads = 128 * kPlSets + 64, kPlTma = 4 * kPlSets, kPlMma = kPlTma + 1;
+constexpr int kPlSets = 2, kPlThreads = 128 * kPlSets + 96, kPlTma = 4 * kPlSets, kPlMma = kPlTma + 1, kPlRelay = kPlTma + 2;
 constexpr int kPlQueries = 128, kPlKeys = 64;
 constexpr int kPlChunk = kPlKeys * 128;        // bytes of a tile's keys x 64 bf16 columns
 constexpr int kPlMost = 5;                     // chunks of columns of a CTA
@@ -56,9 +59,22 @@ __device__ __forceinline__ void remote_store(uint32_t addr, uint32_t bar, float 
                "f"(a), "f"(b), "f"(c), "f"(d)
                : "memory");
 }
-// The other CTA's barrier.  What was read before has been used by now, so nothing needs to be ordered but the arrival itself.
+// The other CTA's barrier: what this thread knows to have been read may be overwritten from there.
 __device__ __forceinline__ void remote_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// mbar_wait for what the other CTA arrives with: its release is met by an acquire of the same scope.
+__device__ __forceinline__ bool cluster_wait(uint64_t* bar, uint32_t parity, int* status, int where) {
+  if (!mbar_wait(bar, parity, status, where)) return false;
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred P;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 P, [%1], %2;\n\t"
+      "selp.b32 %0, 1, 0, P;\n\t}"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
 }
 __device__ __forceinline__ void cluster_meet() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -84,7 +100,8 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
   uint64_t* pv_done = s_full + kPlSets;                      // [2] O += P V complete
   uint64_t* x_full = pv_done + kPlSets;                      // [2] the other CTA's scores are here
   uint64_t* x_free = x_full + kPlSets;                       // [2] this CTA's have been read there
-  uint64_t* known = x_free + kPlSets;                        // [2][4] the maximum after a tile, by quadrant
+  uint64_t* x_read = x_free + kPlSets;                       // [2] the other CTA's have been read here
+  uint64_t* known = x_read + kPlSets;                        // [2][4] the maximum after a tile, by quadrant
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(known + 4 * kPlSets);
   float* s_top = reinterpret_cast<float*>(tmem_slot + 2);    // [128] the running maximum
   float* s_sum = s_top + kPlQueries;                         // [2][128] the sets' sums
@@ -104,7 +121,8 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
       mbar_init(&s_full[i], 1);
       mbar_init(&pv_done[i], 1);
       mbar_init(&x_full[i], 1);
-      mbar_init(&x_free[i], 4);
+      mbar_init(&x_free[i], 1);
+      mbar_init(&x_read[i], 4);
       for (int q = 0; q < 4; ++q) mbar_init(&known[4 * i + q], 1);
     }
     mbar_init_fence();
@@ -249,12 +267,32 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
       }
       ok = __ballot_sync(0xffffffffu, leader && ok) != 0;
     }
+  } else if (warp == kPlRelay) {
+    if (PAIR) {
+      uint32_t free_there[kPlSets];
+#pragma unroll
+      for (int i = 0; i < kPlSets; ++i) free_there[i] = cluster_addr(smem_u32(&x_free[i]), rank ^ 1);
+      bool ok = true;
+      int kt = 0;
+      for (int unit = first_unit; unit < units && ok; unit += unit_step) {
+        const PrefixUnit it = unit == first_unit ? begin : prefix_unit(plan, unit);
+        if (it.rows == 0) continue;
+        int end;
+        const int n = span(it, end);
+        if (lane == 0)
+          for (int j = 0; j < n && ok; ++j, ++kt) {
+            const int set = kt % kPlSets;
+            ok = mbar_wait(&x_read[set], (kt / kPlSets) & 1, p.status, 530);
+            if (ok) remote_arrive(set ? free_there[1] : free_there[0]);
+          }
+        ok = __shfl_sync(0xffffffffu, ok, 0) != 0;
+      }
+    }
   } else {
     const int set = warp >> 2, quad = warp & 3, mine = quad * 32 + lane;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     const uint32_t x_there = PAIR ? cluster_addr(smem_u32(s_x) + 16 * mine, rank ^ 1) : 0;
     const uint32_t full_there = PAIR ? cluster_addr(smem_u32(&x_full[set]), rank ^ 1) : 0;
-    const uint32_t free_there = PAIR ? cluster_addr(smem_u32(&x_free[set]), rank ^ 1) : 0;
     const int before = (set + kPlSets - 1) % kPlSets;              // the set of the last tile
     int kt = 0;
     bool ok = true;
@@ -358,7 +396,7 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
         if (PAIR) {                                            // [column / 4][query]: neighbouring lanes, neighbouring 16 bytes
           const uint32_t buf = (tile & 1) * kPlKeys * kPlQueries;      // its last scores, of the tile before last, have been read
           if (tile > 1)
-            ok = __all_sync(0xffffffffu, mbar_wait(&x_free[(tile - 2) % kPlSets], ((tile - 2) / kPlSets) & 1, p.status, 521)) != 0;
+            ok = __all_sync(0xffffffffu, cluster_wait(&x_free[(tile - 2) % kPlSets], ((tile - 2) / kPlSets) & 1, p.status, 521)) != 0;
           if (!ok) break;
           if (quad == 0 && lane == 0) mbar_expect_tx(&x_full[set], 4 * kPlKeys * kPlQueries);
 #pragma unroll
@@ -387,7 +425,10 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
 #pragma unroll
         for (int i = 0; i < kPlKeys / 2; ++i) tops[i & 3] = fmaxf(tops[i & 3], fmaxf(s[i].x, s[i].y));
         const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * p.scale_log2;
-        if (PAIR && lane == 0) remote_arrive(free_there);          // every score has been used for the maximum
+        if (PAIR) {                                            // every lane's scores are in registers
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&x_read[set]);
+        }
         if (tile > 0) ok = __all_sync(0xffffffffu, mbar_wait(&known[4 * before + quad], ((tile - 1) / kPlSets) & 1, p.status, 523)) != 0;
         if (!ok) break;
         float now = j > 0 ? s_top[mine] : -INFINITY;           // what O is relative to
@@ -540,7 +581,7 @@ int launch_prefix_latent(const ds41_latent_attend_args& a, const ds41_prefix_pla
     if (n > kPlMost || p.v_col[c + 1] <= p.v_col[c]) return cudaErrorNotSupported;
     p.chunks = n > p.chunks ? n : p.chunks;
   }
-  constexpr int kExtra = 8 * (2 * kPlStages + 2 + 9 * kPlSets) + 8 + 4 * (1 + kPlSets) * kPlQueries;
+  constexpr int kExtra = 8 * (2 * kPlStages + 2 + 10 * kPlSets) + 8 + 4 * (1 + kPlSets) * kPlQueries;
   const int room = 227 * 1024 - kExtra - (pair ? 2 * 4 * kPlKeys * kPlQueries : 0);
   p.stages = room / (p.chunks * kPlChunk);
   if (p.stages > kPlStages) p.stages = kPlStages;

@@ -102,3 +102,13 @@ def test_results_that_are_no_numbers_are_not_hidden(i):
         assert case == 5 or want.isnan().any()
         assert torch.equal(got.isnan(), want.isnan()), (case, got.isnan().sum().item(), want.isnan().sum().item())
         assert ((got.double() - want).abs() <= tol)[~want.isnan()].all(), case
+
+
+@pytest.mark.parametrize("groups,P,heads", [([(40, 90)], 64, 32), ([(3, 150), (2, 70)], 32, 16), ([(1, 200)], 64, 128)])
+def test_exchanged_scores_are_read_before_they_are_overwritten(groups, P, heads):
+    """Long walks of CTA pairs, again and again: each call gives the bits of the first, which are right."""
+    p = Pass("latent", heads=heads, dim=576, vdim=512, groups=groups, P=P, own=400, seed=5)
+    plan = p.plan()
+    first = p.check(plan)
+    for _ in range(40):
+        assert torch.equal(p.run(plan), first)
