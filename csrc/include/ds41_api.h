@@ -560,6 +560,7 @@ typedef struct ds41_prefix_plan {
   const int* turns;               // [grid] how many times a block comes to the list (a grid's width of places further on each time)
   const int* order;               // pass rows by prefix: a unit's rows are order[first] .. order[first + rows - 1]; a tail's: first + i
   const int* cell;                // [rows] the row's first cell of part_o / part_ml
+  const int* owner;               // [rows] one more than the slot that the row was planned for (0: none)
   const int* parts;               // [rows] how many it has
   float* part_o;                  // [cells][heads][value width] unnormalised results
   float* part_ml;                 // [cells][heads]{maximum in units of log 2, sum}

@@ -174,7 +174,7 @@ __device__ __forceinline__ void store_rows(float* base, long long at, uint32_t (
 
 inline bool prefix_plan_ok(const ds41_prefix_plan* p) {
   return p != nullptr && p->units != nullptr && p->n_units != nullptr && p->turns != nullptr && p->order != nullptr && p->cell != nullptr &&
-         p->parts != nullptr && p->part_o != nullptr && p->part_ml != nullptr && p->max_units > 0 && p->rows_per_unit > 0 &&
+         p->owner != nullptr && p->parts != nullptr && p->part_o != nullptr && p->part_ml != nullptr && p->max_units > 0 && p->rows_per_unit > 0 &&
          p->grid > 0 && !(reinterpret_cast<uintptr_t>(p->units) & 15) && !(reinterpret_cast<uintptr_t>(p->part_o) & 31) &&
          !(reinterpret_cast<uintptr_t>(p->part_ml) & 7);
 }

@@ -274,8 +274,8 @@ static int run_simple(const SimpleArgs& p, const ds41_prefix_plan& plan, int f32
 }
 
 // A warp joins 128 columns of a (row, head): the lanes find the parts' weights, then every lane sums four columns over the parts, PARTS
-// of them under way together.  Rows without a slot have no parts and become zero.  The launch also keeps the convolution's last
-// inputs where the attention has one (ds41_group.cuh).
+// of them under way together.  Rows without a slot become zero; rows of another slot than the plan's become NaN and are reported.
+// The launch also keeps the convolution's last inputs where the attention has one (ds41_group.cuh).
 // A chain of loads from L2: small launches want many of them under way (94 registers), large ones many warps (56).  Whole calls with 8 / 4
 // parts: 37 rows of 6 heads in 13 parts 13.5 / 15.2 us, 32 rows of 32 heads 22.8 / 23.8 (1024 warps); 32 rows x 32 heads x 512 columns
 // (4096 warps) 31.7 / 30.3 us, 128 rows (16384) 204 / 198.
@@ -289,12 +289,20 @@ prefix_join_kernel(const ds41_prefix_plan plan, const float* sink, const ds41_pr
   const int r = pair / heads, h = pair % heads, c = (w - pair * strips) * 128 + 4 * lane;
   pdl_launch_dependents();
   // the plan was copied to the device, not computed there: it may be read before the wait
-  const int n = r < rows ? plan.parts[r] : 0;
+  const int n = r < rows ? plan.parts[r] : 0, owner = r < rows ? plan.owner[r] : 0;
   const long long cell = r < rows ? 1ll * plan.cell[r] * heads + h : 0;
   pdl_wait();
   if (r >= rows) return;
   const float sk = sink != nullptr ? sink[h] * 1.4426950408889634f : -INFINITY;
   const int slot = keep.row_slot[r];
+  // a row of another slot than the one that the plan holds its keys for: no result is right
+  const bool stray = slot >= 0 && slot + 1 != owner;
+  if (stray && w % (heads * strips) == 0 && lane == 0 && keep.status != nullptr &&
+      atomicCAS(keep.status, kStatusOk, kStatusBadArgument) == kStatusOk) {
+    keep.status[1] = 540;
+    keep.status[2] = r;
+    keep.status[3] = slot;
+  }
   if (keep.taps > 1 && slot >= 0)
     keep_inputs(keep, r, slot, keep.row_pos[r], w % (heads * strips), heads * strips, lane, 32);
   const float2* ml = reinterpret_cast<const float2*>(plan.part_ml) + cell;
@@ -331,7 +339,8 @@ prefix_join_kernel(const ds41_prefix_plan plan, const float* sink, const ds41_pr
   }
   den = warp_sum(den);
   // a NaN among the scores leaves its part a sum of NaN, whatever the maximum is
-  const float f = slot < 0 ? 0.f : (den > 0.f ? 1.0f / den : den) * (gate.data != nullptr ? sigmoid_f32(proj_at(gate, r, h)) : 1.f);
+  float f = (den > 0.f ? 1.0f / den : den) * (gate.data != nullptr ? sigmoid_f32(proj_at(gate, r, h)) : 1.f);
+  f = slot < 0 ? 0.f : stray ? NAN : f;
   if (c < vp) store4(out + 1ll * r * ld_out + h * vp + c, make_float4(a.x * f, a.y * f, a.z * f, a.w * f));
 }
 
@@ -397,6 +406,7 @@ extern "C" int ds41_prefix_latent(const ds41_latent_attend_args* a, const ds41_p
   ds41_group_attend_args keep{};
   keep.taps = 1;
   keep.row_slot = a->row_slot;
+  keep.status = a->status;
   return a->f32 ? launch_join<float>(*plan, sink, none, a->rows, a->heads, a->kv_pad, out, ld_out, keep, st)
                 : launch_join<__nv_bfloat16>(*plan, sink, none, a->rows, a->heads, a->kv_pad, out, ld_out, keep, st);
 }

@@ -9,7 +9,8 @@ Which rows share what is a `PrefixPlan`, made on the host from the page tables. 
 slots and those keep their leading pages: pages added at a table's end leave it valid, so a decode loop makes it once for a batch.
 It also holds the workspace of the calls, so calls with one plan, and `set()`, follow one another on one stream; concurrent streams,
 or graphs that replay at the same time, need a plan each.  A captured call reads the plan from device memory: after `set()` a replay
-uses the new one, which may not have more rows than the call that was captured.
+uses the new one, which may not have more rows than the call that was captured.  A row that belongs to another slot than its plan says
+gets NaN, and check_status() raises; that a slot's leading pages are the ones it was set for is the caller's to see to.
 
 What no row of a pass sees may hold anything, NaN included.  A NaN that a row does meet, in its query, a key, a value, a gate or a
 sink, is in its result; one in a value that only some rows of a range see may be in the others' as well, as the tensor cores multiply
@@ -34,7 +35,7 @@ UNIT = 8                 # numbers of a unit (ds41_prefix_plan)
 
 
 class PlanArgs(C.Structure):
-    _fields_ = [("units", C.c_void_p), ("n_units", C.c_void_p), ("turns", C.c_void_p), ("order", C.c_void_p), ("cell", C.c_void_p), ("parts", C.c_void_p),
+    _fields_ = [("units", C.c_void_p), ("n_units", C.c_void_p), ("turns", C.c_void_p), ("order", C.c_void_p), ("cell", C.c_void_p), ("owner", C.c_void_p), ("parts", C.c_void_p),
                 ("part_o", C.c_void_p), ("part_ml", C.c_void_p), ("max_units", C.c_int), ("rows_per_unit", C.c_int), ("grid", C.c_int)]
 
 
@@ -124,8 +125,8 @@ class PrefixPlan:
         self.max_units = self.max_turns * self.grid * self.together
         self.max_cells = self.extra * min(self.rows_per_unit, rows) + 2 * rows
         z = lambda n, d: torch.zeros(max(n, 4), dtype=d, device=self.device)
-        # [count, 3 unused | units | turns | order | cell | parts]
-        self._at = np.cumsum([4, UNIT * self.max_units, self.grid, rows, rows]).tolist()
+        # [count, 3 unused | units | turns | order | cell, owner | parts]
+        self._at = np.cumsum([4, UNIT * self.max_units, self.grid, rows, 2 * rows]).tolist()
         self.data = z(self._at[-1] + rows, I32)
         self.part_o, self.part_ml = z(self.max_cells * heads * vdim, F32), z(self.max_cells * heads * 2, F32)
         self.status = lib.new_status(self.device)
@@ -136,6 +137,7 @@ class PrefixPlan:
         self.lows: List[int] = []                          # first token of it that any of them sees
         a, base = PlanArgs(), self.data.data_ptr()
         a.n_units, (a.units, a.turns, a.order, a.cell, a.parts) = base, (base + 4 * x for x in self._at)
+        a.owner = a.cell + 4 * rows
         a.part_o, a.part_ml = self.part_o.data_ptr(), self.part_ml.data_ptr()
         a.max_units, a.rows_per_unit, a.grid = self.max_units, self.rows_per_unit, self.grid
         self.args, self.args_ref = a, C.byref(a)
@@ -220,7 +222,8 @@ class PrefixPlan:
             units.reshape(-1, self.together, UNIT)[place] = every
             turns[:] = np.bincount(place % self.grid, minlength=self.grid)
             parts[:len(n_parts)] = n_parts
-            cell[:] = np.cumsum(parts) - parts
+            cell[:self.rows] = np.cumsum(parts) - parts
+            cell[self.rows:self.rows + len(slots)] = np.maximum(slots, -1) + 1
             n = int(turns.max()) * self.grid * self.together
         host[0] = self.n_units = n
         self.data.copy_(torch.from_numpy(host))

@@ -112,3 +112,39 @@ def test_exchanged_scores_are_read_before_they_are_overwritten(groups, P, heads)
     first = p.check(plan)
     for _ in range(40):
         assert torch.equal(p.run(plan), first)
+
+
+@pytest.mark.parametrize("i", range(len(FORMS)))
+def test_rows_of_other_slots_than_the_plan_says_are_reported(i):
+    from ds41rt_b200.ops.lib import KernelError
+    kind, sizes = FORMS[i]
+    p = Pass(kind, groups=[(9, 5)], alone=2, pads=1, own=130, seed=i, **sizes)
+    plan, none = p.plan(), p.row_slot.index(-1)
+    a, b, c = [r for r, s in enumerate(p.row_slot) if s >= 0][:3]
+    out = torch.empty(p.R, p.H, p.V, dtype=p.dtype, device="cuda")
+    want, tol = p.expected()
+    p.run(plan, out=out)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        p.run(plan, out=out)
+    for call in (lambda: p.run(plan, out=out), g.replay):
+        p.d_slot[c] = -1                                     # a row that the plan knows may have no slot
+        call()
+        plan.check_status()
+        assert not out[c].any()
+        for rows, slots in (((a, b), (p.row_slot[b], p.row_slot[a])), ((none,), (p.row_slot[a],))):
+            p.d_slot[list(rows)] = p.dev(slots)
+            call()
+            with pytest.raises(KernelError, match="bad argument"):
+                plan.check_status()
+            plan.status.zero_()
+            assert out[list(rows)].isnan().all()
+            right = [r for r in range(p.R) if r not in rows and r != c]
+            assert ((out.double() - want).abs() <= tol)[right].all()
+            p.d_slot[:] = p.dev(p.row_slot)
+            p.d_slot[c] = -1
+        p.d_slot[:] = p.dev(p.row_slot)
+        call()
+        plan.check_status()
+        assert ((out.double() - want).abs() <= tol).all()
