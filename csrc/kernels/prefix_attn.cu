@@ -27,7 +27,7 @@ struct SimpleArgs {
   int d1, d2, vp, row_len;
   int k_lane, v_at, v_lane;          // key / value head g of a cache row: keys at g * k_lane, values at v_at + g * v_lane
   int inside;                        // the values are the first values of the key
-  int lanes, per_lane, heads, chunk, max_pages, page_tokens;
+  int per_lane, heads, chunk, max_pages, page_tokens, n_pages;
   float scale;
 };
 
@@ -59,6 +59,7 @@ __global__ void __launch_bounds__(256, QPT <= 4 ? 2 : 1) prefix_simple_kernel(co
   float* keep = ls + kSimpleQueries;                          // [16] factor on what was summed before
   int* lim = reinterpret_cast<int*>(keep + kSimpleQueries);   // [16] end of what a query sees
   __shared__ int low[kSimpleQueries], row_of[kSimpleQueries];
+  __shared__ bool leased[kSimpleKeys];                        // a key without a page is not there
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_launch_dependents();
   pdl_wait();
@@ -110,7 +111,7 @@ __global__ void __launch_bounds__(256, QPT <= 4 ? 2 : 1) prefix_simple_kernel(co
     auto row_at = [&](int key) {           // pool row of a key, -1: none
       const int pg = key / p.page_tokens;
       const int id = key >= from && key < to && pg < p.max_pages ? p.page_table[1ll * it.slot * p.max_pages + pg] : -1;
-      return id >= 0 ? id * p.page_tokens + (key - pg * p.page_tokens) : -1;
+      return static_cast<unsigned>(id) < static_cast<unsigned>(p.n_pages) ? id * p.page_tokens + (key - pg * p.page_tokens) : -1;
     };
     int next = lane < 4 && from < to ? row_at(from + warp + 8 * lane) : -1;
     const T* pool_k = static_cast<const T*>(p.pool) + g * p.k_lane;
@@ -135,6 +136,7 @@ __global__ void __launch_bounds__(256, QPT <= 4 ? 2 : 1) prefix_simple_kernel(co
           for (int k = 0; k < 4; ++k) *reinterpret_cast<float4*>(dst + (warp + 8 * k) * ld + d) = v[k];
         }
       };
+      if (lane < 4) leased[warp + 8 * lane] = next >= 0;
       fetch(pool_k, ks, ds, dp);
       if (!p.inside) fetch(pool_v, vs, vs_ld, p.vp);
       next = lane < 4 ? row_at(t0 + kSimpleKeys + warp + 8 * lane) : -1;
@@ -149,8 +151,8 @@ __global__ void __launch_bounds__(256, QPT <= 4 ? 2 : 1) prefix_simple_kernel(co
           b += x.x * z.x + x.y * z.y + x.z * z.z + x.w * z.w;
         }
         const int key = t0 + j;
-        sc[j * kSimpleLd + u] = key >= low[u] && key < lim[u] ? a * p.scale : -INFINITY;
-        sc[(j + 16) * kSimpleLd + u] = key + 16 >= low[u] && key + 16 < lim[u] ? b * p.scale : -INFINITY;
+        sc[j * kSimpleLd + u] = leased[j] && key >= low[u] && key < lim[u] ? a * p.scale : -INFINITY;
+        sc[(j + 16) * kSimpleLd + u] = leased[j + 16] && key + 16 >= low[u] && key + 16 < lim[u] ? b * p.scale : -INFINITY;
       } else {
         // a warp's 8 queries x 8 keys, the columns by lane: 16 loads for 256 products, then the lanes' sums are added and shared out
         const float *x = qs + (warp & 1) * 8 * ds, *y = ks + (warp >> 1) * 8 * ds;
@@ -181,7 +183,8 @@ __global__ void __launch_bounds__(256, QPT <= 4 ? 2 : 1) prefix_simple_kernel(co
         const int u = (warp & 1) * 8 + (lane >> 2), j = (warp >> 1) * 8 + 2 * (lane & 3);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          sc[(j + i) * kSimpleLd + u] = t0 + j + i >= low[u] && t0 + j + i < lim[u] ? s[i] * p.scale : -INFINITY;
+          sc[(j + i) * kSimpleLd + u] =
+              leased[j + i] && t0 + j + i >= low[u] && t0 + j + i < lim[u] ? s[i] * p.scale : -INFINITY;
       }
       __syncthreads();
       for (int u = 2 * warp; u < 2 * warp + 2; ++u) {
@@ -312,7 +315,8 @@ prefix_join_kernel(const ds41_prefix_plan plan, const float* sink, const ds41_pr
   float all = fmaxf(sk, mine.x);
   for (int s = lane + 32; s < n; s += 32) all = fmaxf(all, ml[1ll * s * heads].x);
   all = warp_max(all);
-  float den = sink != nullptr && lane == 0 && all > -INFINITY ? exp2f(sk - all) : 0.f;
+  // parts of a row without a slot are empty, so that its sum stays zero
+  float den = stray ? NAN : sink != nullptr && slot >= 0 && lane == 0 && all > -INFINITY ? exp2f(sk - all) : 0.f;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int s0 = 0; s0 < n; s0 += 32) {
     if (s0 > 0) mine = s0 + lane < n ? ml[1ll * (s0 + lane) * heads] : make_float2(-INFINITY, 0.f);
@@ -338,9 +342,8 @@ prefix_join_kernel(const ds41_prefix_plan plan, const float* sink, const ds41_pr
     }
   }
   den = warp_sum(den);
-  // a NaN among the scores leaves its part a sum of NaN, whatever the maximum is
-  float f = (den > 0.f ? 1.0f / den : den) * (gate.data != nullptr ? sigmoid_f32(proj_at(gate, r, h)) : 1.f);
-  f = slot < 0 ? 0.f : stray ? NAN : f;
+  // nothing seen: zeros, whatever the gate is; a NaN among the scores left its part a sum of NaN, whatever the maximum was
+  const float f = den > 0.f ? (gate.data != nullptr ? sigmoid_f32(proj_at(gate, r, h)) : 1.f) * (1.0f / den) : den;
   if (c < vp) store4(out + 1ll * r * ld_out + h * vp + c, make_float4(a.x * f, a.y * f, a.z * f, a.w * f));
 }
 
@@ -359,7 +362,8 @@ static int launch_join(const ds41_prefix_plan& plan, const float* sink, const ds
 using namespace ds41;
 
 extern "C" int ds41_prefix_group(const ds41_group_attend_args* a, const ds41_prefix_plan* plan, void* stream) {
-  if (!prefix_plan_ok(plan) || !group_attend_ok(a) || (a->ld_out & 3) || (reinterpret_cast<uintptr_t>(a->out) & (a->f32 ? 15 : 7)))
+  if (!prefix_plan_ok(plan) || !group_attend_ok(a) || a->n_pages <= 0 ||
+      1ll * a->n_pages * a->page_tokens >= 1ll << 31 || (a->ld_out & 3) || (reinterpret_cast<uintptr_t>(a->out) & (a->f32 ? 15 : 7)))
     return cudaErrorInvalidValue;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int e = launch_prefix_group(*a, *plan, st);
@@ -370,8 +374,8 @@ extern "C" int ds41_prefix_group(const ds41_group_attend_args* a, const ds41_pre
     p.ld_q = a->ld_q; p.q_head = a->dim_pad; p.d1 = a->dim_pad; p.vp = a->vdim_pad;
     p.row_len = a->kv_heads * (a->dim_pad + a->vdim_pad);
     p.k_lane = a->dim_pad; p.v_at = a->kv_heads * a->dim_pad; p.v_lane = a->vdim_pad;
-    p.lanes = a->kv_heads; p.per_lane = a->heads / a->kv_heads; p.heads = a->heads;
-    p.chunk = a->chunk; p.max_pages = a->max_pages; p.page_tokens = a->page_tokens;
+    p.per_lane = a->heads / a->kv_heads; p.heads = a->heads;
+    p.chunk = a->chunk; p.max_pages = a->max_pages; p.page_tokens = a->page_tokens; p.n_pages = a->n_pages;
     p.scale = a->scale;
     e = run_simple(p, *plan, a->f32, st);
   }
@@ -383,7 +387,8 @@ extern "C" int ds41_prefix_group(const ds41_group_attend_args* a, const ds41_pre
 extern "C" int ds41_prefix_latent(const ds41_latent_attend_args* a, const ds41_prefix_plan* plan, int n_pages, const float* sink, void* out,
                                   int ld_out, void* stream) {
   if (!prefix_plan_ok(plan) || a == nullptr || a->rows <= 0 || a->heads <= 0 || a->heads > 65535 || a->kv_pad <= 0 || (a->kv_pad & 3) ||
-      a->row_len < a->kv_pad || (a->row_len & 3) || n_pages <= 0 || a->max_pages <= 0 || a->page_tokens <= 0 || a->q_abs == nullptr ||
+      a->row_len < a->kv_pad || (a->row_len & 3) || n_pages <= 0 || a->max_pages <= 0 || a->page_tokens <= 0 ||
+      1ll * n_pages * a->page_tokens >= 1ll << 31 || a->q_abs == nullptr ||
       (a->row_len > a->kv_pad && a->q_rot == nullptr) || a->pool == nullptr || a->page_table == nullptr || a->row_pos == nullptr ||
       a->row_slot == nullptr || out == nullptr || ld_out < a->heads * a->kv_pad || (ld_out & 3) ||
       (reinterpret_cast<uintptr_t>(out) & (a->f32 ? 15 : 7)))
@@ -396,8 +401,8 @@ extern "C" int ds41_prefix_latent(const ds41_latent_attend_args* a, const ds41_p
     p.page_table = a->page_table; p.row_pos = a->row_pos; p.row_slot = a->row_slot;
     p.ld_q = a->ld_q_abs; p.q_head = a->kv_pad; p.ld_q2 = a->ld_q_rot; p.q2_head = a->q_rot_stride;
     p.d1 = a->kv_pad; p.d2 = a->row_len - a->kv_pad; p.vp = a->kv_pad; p.row_len = a->row_len;
-    p.lanes = 1; p.per_lane = a->heads; p.heads = a->heads; p.inside = 1;
-    p.max_pages = a->max_pages; p.page_tokens = a->page_tokens;
+    p.per_lane = a->heads; p.heads = a->heads; p.inside = 1;
+    p.max_pages = a->max_pages; p.page_tokens = a->page_tokens; p.n_pages = n_pages;
     p.scale = a->scale;
     e = run_simple(p, *plan, a->f32, st);
   }

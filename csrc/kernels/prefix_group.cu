@@ -42,7 +42,7 @@ struct PrefixGroupParams {
   const int *page_table, *row_pos, *row_slot;
   long long ld_q;
   int heads, kv_heads, n, dp, vp, kd, vc, stages, shift;             // tiles of keys and of values: 2^shift
-  int chunk, max_pages, page_tokens, box, hidden_row;      // a row beyond the pool: reads as zeros
+  int chunk, max_pages, page_tokens, n_pages, box, hidden_row;      // a row beyond the pool: reads as zeros
   int deep;                                                // all chunks of a box in one copy
   float scale_log2;
   int* status;
@@ -140,7 +140,7 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap keys, const __grid_const
   auto locate = [&](int slot, int first, int end, int u) {
     const int key = first + (u + lane) * p.box, pg = key / p.page_tokens;
     const int id = key < end && pg < p.max_pages ? p.page_table[1ll * slot * p.max_pages + pg] : -1;
-    return id >= 0 ? id * p.page_tokens + (key - pg * p.page_tokens) : p.hidden_row;
+    return static_cast<unsigned>(id) < static_cast<unsigned>(p.n_pages) ? id * p.page_tokens + (key - pg * p.page_tokens) : p.hidden_row;
   };
 
   if (warp == 13) {
@@ -620,7 +620,8 @@ int launch_prefix_group(const ds41_group_attend_args& a, const ds41_prefix_plan&
   p.q = static_cast<const __nv_bfloat16*>(a.q);
   p.page_table = a.page_table; p.row_pos = a.row_pos; p.row_slot = a.row_slot;
   p.ld_q = a.ld_q; p.heads = a.heads; p.kv_heads = a.kv_heads; p.dp = a.dim_pad; p.vp = a.vdim_pad;
-  p.chunk = a.chunk; p.max_pages = a.max_pages; p.page_tokens = a.page_tokens; p.hidden_row = a.n_pages * a.page_tokens;
+  p.chunk = a.chunk; p.max_pages = a.max_pages; p.page_tokens = a.page_tokens; p.n_pages = a.n_pages;
+  p.hidden_row = a.n_pages * a.page_tokens;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.status = a.status;
   const int row_len = a.kv_heads * (a.dim_pad + a.vdim_pad);

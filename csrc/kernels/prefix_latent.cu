@@ -45,7 +45,7 @@ struct PrefixLatentParams {
   int q_rot_stride, heads, kvp, rp;
   int chunks, stages;                                       // of a stage, of the ring
   int v_col[3], rot_step[3];                                // CTA c: latent columns [v_col[c], v_col[c + 1]), rotated steps of 16 likewise
-  int max_pages, page_tokens, box, hidden_row;
+  int max_pages, page_tokens, n_pages, box, hidden_row;
   int deep;                                                 // a CTA's latent chunks of a box in one copy
   int wide;                                                 // queries may be read 32 bytes at a time
   float scale_log2;
@@ -177,7 +177,7 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
           if ((u & 31) == 0) {
             const int key = it.key0 + (u + lane) * p.box, pg = key / p.page_tokens;
             const int id = key < end && pg < p.max_pages ? table[pg] : -1;
-            row = id >= 0 ? id * p.page_tokens + (key - pg * p.page_tokens) : p.hidden_row;
+            row = static_cast<unsigned>(id) < static_cast<unsigned>(p.n_pages) ? id * p.page_tokens + (key - pg * p.page_tokens) : p.hidden_row;
           }
           const int at = __shfl_sync(0xffffffffu, row, u & 31);
           if (lane == 0) {
@@ -591,7 +591,7 @@ int launch_prefix_latent(const ds41_latent_attend_args& a, const ds41_prefix_pla
   p.page_table = a.page_table; p.row_pos = a.row_pos; p.row_slot = a.row_slot;
   p.ld_q_abs = a.ld_q_abs; p.ld_q_rot = a.ld_q_rot; p.q_rot_stride = a.q_rot_stride;
   p.heads = a.heads; p.kvp = a.kv_pad; p.rp = rp;
-  p.max_pages = a.max_pages; p.page_tokens = a.page_tokens; p.hidden_row = n_pages * a.page_tokens;
+  p.max_pages = a.max_pages; p.page_tokens = a.page_tokens; p.n_pages = n_pages; p.hidden_row = n_pages * a.page_tokens;
   p.wide = !((a.ld_q_abs | a.ld_q_rot | a.q_rot_stride) & 15) &&
            !((reinterpret_cast<uintptr_t>(a.q_abs) | reinterpret_cast<uintptr_t>(a.q_rot)) & 31);
   p.scale_log2 = a.scale * 1.4426950408889634f;

@@ -12,6 +12,8 @@ or graphs that replay at the same time, need a plan each.  A captured call reads
 uses the new one, which may not have more rows than the call that was captured.  A row that belongs to another slot than its plan says
 gets NaN, and check_status() raises; that a slot's leading pages are the ones it was set for is the caller's to see to.
 
+The pages of what a row sees have to be leased, by numbers that the pool has; those that are not are left out where products are 32-bit
+and read as zeros by the tensor-core forms, as in the operators that read row by row.
 What no row of a pass sees may hold anything, NaN included.  A NaN that a row does meet, in its query, a key, a value, a gate or a
 sink, is in its result; one in a value that only some rows of a range see may be in the others' as well, as the tensor cores multiply
 it by their weight of zero.

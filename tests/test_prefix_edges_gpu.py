@@ -148,3 +148,44 @@ def test_rows_of_other_slots_than_the_plan_says_are_reported(i):
         call()
         plan.check_status()
         assert ((out.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("page", [-1, "n", 1 << 25, (1 << 31) - 1, -(1 << 31)])
+@pytest.mark.parametrize("i", range(len(FORMS)))
+def test_pages_that_the_pool_does_not_have(i, page):
+    """A page inside what a row sees that is not leased, or whose number is none of the pool's: not there, or zeros in tensor-core forms."""
+    kind, sizes = FORMS[i]
+    p = Pass(kind, groups=[(5, 3)], alone=2, own=200, seed=i, **sizes)
+    plan = p.plan()
+    tiled = p.dtype == BF16 and p.P == 64
+    r = next(r for r, s in enumerate(p.row_slot) if p.row_pos[r] >= 4 * p.P)
+    s, hole = p.row_slot[r], 3                               # behind the common pages, before the row's last one
+    want, tol = p.expected()
+    p.d_tables[s, hole] = p.pool.shape[0] // p.P if page == "n" else page
+    got = p.run(plan)
+    torch.cuda.synchronize()
+    plan.check_status()
+    others = [x for x in range(p.R) if x != r]
+    assert ((got.double() - want).abs() <= tol)[others].all()
+    at = torch.arange(p.row_pos[r] + 1)
+    rows = p.pool[(p.tables[s].long()[at // p.P] * p.P + at % p.P).cuda()].double()
+    gone = (at // p.P == hole).cuda()
+    rows[gone] = 0
+    n = p.H // p.G
+    for h in range(p.H):
+        g = h // n
+        k, v = (rows[:, g * p.D:(g + 1) * p.D], rows[:, p.G * p.D + g * p.V:p.G * p.D + (g + 1) * p.V]) if kind == "grouped" else (rows, rows[:, :p.V])
+        z = k @ p.q[r, h].double() * p.scale
+        if not tiled:
+            z[gone] = -math.inf
+        if kind == "latent":
+            z = torch.cat([z, p.sink[h:h + 1].double()])
+        w = torch.softmax(z, 0)[:len(at)]
+        o, A = w @ v, w @ v.abs()
+        u = 2.0 ** -8 if p.dtype == BF16 else 2.0 ** -24
+        d = float((k.abs() @ p.q[r, h].double().abs()).max()) * p.scale * (p.D + 2) * 2.0 ** -23
+        t = (2 * d * (1 + d) + 2.0 ** -20 + 2 * len(at) * 2.0 ** -23 + (u if p.dtype == BF16 else 0)) * A
+        if kind == "grouped":
+            f = torch.sigmoid(p.gate[r, h].double())
+            o, t = o * f, (t + 2.0 ** -21 * o.abs()) * f
+        assert ((got[r, h].double() - o).abs() <= t + u * (o.abs() + t) + 1e-30).all(), h
