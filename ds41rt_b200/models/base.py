@@ -108,7 +108,7 @@ class RowsEngine:
         device in another way does so before the pass."""
 
     def settle(self):
-        """Before a captured pass is replayed over the rows of the last set_rows(), whatever pass that was meant for."""
+        """Before a pass is captured, or replayed over the rows of the last set_rows(), whatever pass that was meant for."""
 
     # ------------------------------------------------------------------ graphs
     @contextlib.contextmanager
@@ -128,6 +128,7 @@ class RowsEngine:
     def capture(self, enqueue) -> torch.cuda.CUDAGraph:
         """Graph of the launches that `enqueue` makes; one eager pass first sets function attributes and warms every
         code path."""
+        self.settle()             # nothing may be planned inside the capture
         with self.rehearsal():
             enqueue()
             torch.cuda.synchronize()

@@ -189,3 +189,23 @@ def test_pages_that_the_pool_does_not_have(i, page):
             f = torch.sigmoid(p.gate[r, h].double())
             o, t = o * f, (t + 2.0 ** -21 * o.abs()) * f
         assert ((got[r, h].double() - o).abs() <= t + u * (o.abs() + t) + 1e-30).all(), h
+
+
+def test_graphs_are_captured_right_behind_a_long_prompt():
+    """The rows of the last set_rows() took the long form, which needs no plan; the captured pass over them does."""
+    import test_belasun_gpu as belasun
+    from ds41rt_b200.runtime.session import DecodeSession
+    from test_stack_gpu import close
+    e = belasun.engine("tiles", "bf16", shared_prefix=True, page_tokens=32)
+    toks = belasun.tokens("tiles", 110, seed=12)
+    want, spread = belasun.reference("tiles", toks, "bf16")[:2]
+    assert e.cache.ensure(0, 200)
+    e.set_rows(toks[:100], list(range(100)), [0] * 100)
+    e.forward_rows(100, head=False)
+    e.set_rows(toks[:80], list(range(80)), [0] * 80)
+    ses = DecodeSession(e)
+    assert ses.graph(80) is not None
+    for at in range(100, 110):
+        ses.step([toks[at]], [at], [0])
+        close(e.logits_rows(1).cpu().double(), want[at:at + 1], "bf16", spread[at:at + 1])
+    e.check_status()
