@@ -21,8 +21,7 @@ it by their weight of zero.
 from __future__ import annotations
 
 import ctypes as C
-import heapq
-from typing import Dict, List, NamedTuple, Optional, Sequence, Tuple
+from typing import List, NamedTuple, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
@@ -41,32 +40,27 @@ class PlanArgs(C.Structure):
                 ("part_o", C.c_void_p), ("part_ml", C.c_void_p), ("max_units", C.c_int), ("rows_per_unit", C.c_int), ("grid", C.c_int)]
 
 
-def common_runs(tables: np.ndarray) -> List[Tuple[List[int], int]]:
-    """Groups of rows of a page table that begin with the same leased pages: (rows, common pages), a row in one group at most.
+class PlanShape(C.Structure):
+    """What the host's division of the work goes by (csrc/core/prefix_plan.cc)."""
+    _fields_ = [(n, C.c_int) for n in ("rows", "heads", "kv_heads", "vdim", "page_tokens", "chunk", "rows_per_unit", "together", "grid",
+                                       "min_tokens", "max_turns", "max_units", "max_cells", "extra", "least_span", "reserved")] + \
+               [(n, C.c_double) for n in ("turn", "row", "longer", "shorter", "byte", "part")]
 
-    Sorted, rows with a common beginning stand next to each other, and a range of them shares the least of the runs between
-    neighbours.  The range that saves most reads, (rows - 1) x pages, is a group; the rows on either side of it are divided again."""
-    order = sorted(range(len(tables)), key=lambda i: tables[i].tobytes())
-    t = tables[order]
-    same = (t[1:] == t[:-1]) & (t[1:] >= 0)
-    runs = np.where(same.all(1), t.shape[1], same.argmin(1)) if len(t) > 1 else np.zeros(0, dtype=np.int64)
-    out, todo = [], [(0, len(runs))]
-    while todo:
-        lo, hi = todo.pop()
-        best = (0, 0, 0, 0)
-        rising: List[Tuple[int, int]] = []               # (first run, height) of the ranges that are still open
-        for i in range(lo, hi + 1):
-            h, at = (int(runs[i]) if i < hi else 0), i
-            while rising and rising[-1][1] >= h:
-                at, top = rising.pop()
-                best = max(best, ((i - at) * top, top, at, i))
-            rising.append((at, h))
-        gain, pages, a, b = best
-        if gain == 0:
-            continue
-        out.append(([order[i] for i in range(a, b + 1)], pages))
-        todo += [(lo, max(lo, a - 1)), (min(hi, b + 1), hi)]
-    return out
+
+def _failed(err: int):
+    raise (MemoryError("no memory to divide the work of a pass") if err == -2 else RuntimeError("a plan's arrays do not hold its rows' division"))
+
+
+def common_runs(tables: np.ndarray) -> List[Tuple[List[int], int]]:
+    """Groups of rows of a page table that begin with the same leased pages: (rows, common pages), a row in one group at most.  Which
+    they are: find_groups() of csrc/core/prefix_plan.cc."""
+    t = np.ascontiguousarray(tables, dtype=np.int32)
+    n, width = t.shape
+    order, bounds, pages = (np.zeros(max(n, 1) * k, dtype=np.int32) for k in (1, 2, 1))
+    count = lib.core().ds41_prefix_groups(C.c_void_p(t.ctypes.data), n, width, *(C.c_void_p(x.ctypes.data) for x in (order, bounds, pages)))
+    if count < 0:
+        _failed(count)
+    return [(order[bounds[2 * i]:bounds[2 * i + 1]].tolist(), int(pages[i])) for i in range(count)]
 
 
 def tiled(kind: str, heads: int, kv_heads: int, dim: int, vdim: int, page_tokens: int) -> bool:
@@ -93,7 +87,6 @@ class Cost(NamedTuple):
 
 COSTS = {"grouped": Cost(1.4, 0.10, 0.0105, 0.0055, 1 / 6e6), "latent": Cost(4.0, 0.0, 0.0205, 0.0, 1 / 8e6)}
 COST_F32 = Cost(1.0, 0.0, 0.3, 0.3, 1 / 6e6)
-SPANS = (1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 28, 32, 40, 48, 64, 96, 128, 192, 256, 384, 512, 1024, 2048, 4096)    # tried, in tiles or pages
 
 
 class PrefixPlan:
@@ -123,20 +116,30 @@ class PrefixPlan:
         self.grid = SMS // 2 if kind == "latent" and vdim > 256 else SMS               # two CTAs to a unit
         self.extra = 3 * -(-self.grid * self.together // kv_heads)      # items beyond one for every piece of a prefix and every request
         self.max_items = self.extra + 2 * rows
-        self.max_turns = -(-self.max_items * kv_heads // (self.grid * self.together)) + 2
+        # a head's items go in twos (one may stay alone), the heads are dealt one like the other
+        self.max_turns = -(-(self.max_items + 1) * kv_heads // (self.grid * self.together)) + 2
         self.max_units = self.max_turns * self.grid * self.together
         self.max_cells = self.extra * min(self.rows_per_unit, rows) + 2 * rows
-        z = lambda n, d: torch.zeros(max(n, 4), dtype=d, device=self.device)
         # [count, 3 unused | units | turns | order | cell, owner | parts]
         self._at = np.cumsum([4, UNIT * self.max_units, self.grid, rows, 2 * rows]).tolist()
-        self.data = z(self._at[-1] + rows, I32)
-        self.part_o, self.part_ml = z(self.max_cells * heads * vdim, F32), z(self.max_cells * heads * 2, F32)
+        self._size = self._at[-1] + rows
+        self.data = torch.zeros(self._size, dtype=I32, device=self.device)
+        # parts without a weight are not read
+        self.part_o = torch.empty(self.max_cells * heads * vdim, dtype=F32, device=self.device)
+        self.part_ml = torch.empty(self.max_cells * heads * 2, dtype=F32, device=self.device)
         self.status = lib.new_status(self.device)
         self.n_units = self.span = 0
         self.n_rows, self.table_shape = 0, None            # of the last set(): what calls have to match
         self.captured: Optional[int] = None                # least rows of the calls that graphs hold
-        self.shared: List[Tuple[List[int], int]] = []      # rows and tokens of every prefix
-        self.lows: List[int] = []                          # first token of it that any of them sees
+        self._groups, self._result = np.zeros(3 * rows, dtype=np.int32), np.zeros(3, dtype=np.int32)
+        self._order, self._used = np.zeros(0, dtype=np.int32), 0
+        shape = PlanShape(rows=rows, heads=heads, kv_heads=kv_heads, vdim=vdim, page_tokens=page_tokens, chunk=chunk,
+                          rows_per_unit=self.rows_per_unit, together=self.together, grid=self.grid, min_tokens=min_tokens,
+                          max_turns=self.max_turns, max_units=self.max_units, max_cells=self.max_cells, extra=self.extra,
+                          least_span=ceil_to(128 if dtype == BF16 else 32, page_tokens), **self.cost._asdict())
+        at = (C.c_int32 * 5)(*self._at)
+        self._divide = lib.core().ds41_prefix_divide
+        self._shape = (shape, at, C.byref(shape), C.c_void_p(self._groups.ctypes.data), C.c_void_p(self._result.ctypes.data))
         a, base = PlanArgs(), self.data.data_ptr()
         a.n_units, (a.units, a.turns, a.order, a.cell, a.parts) = base, (base + 4 * x for x in self._at)
         a.owner = a.cell + 4 * rows
@@ -144,168 +147,57 @@ class PrefixPlan:
         a.max_units, a.rows_per_unit, a.grid = self.max_units, self.rows_per_unit, self.grid
         self.args, self.args_ref = a, C.byref(a)
 
-    def nbytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in (self.data, self.part_o, self.part_ml))
+    @property
+    def shared(self) -> List[Tuple[List[int], int]]:
+        """Rows and tokens of every prefix."""
+        out, at = [], 0
+        for i in range(int(self._result[2])):
+            n, tokens = self._groups[3 * i:3 * i + 2].tolist()
+            out.append((self._order[at:at + n].tolist(), tokens))
+            at += n
+        return out
 
     def set(self, slots: Sequence[int], tables, lengths: Optional[Sequence[int]] = None) -> None:
         """`slots`: the slot of every row of the passes to come (-1: none); `tables`: the page table on the host, [slots, pages],
         negative where no page is leased.  `lengths`: how many tokens each row's request has now (default: what its pages hold); the
         division of the work goes by it.  A plan with a `chunk` also leaves out the keys before the chunk of a row's last token, if it
-        is given lengths: until the next set() such a row may go on, but not back behind that chunk's beginning."""
+        is given lengths: until the next set() such a row may go on, but not back behind that chunk's beginning.  Not inside a capture;
+        the device's copy is made on the current stream, and the host does not wait for it."""
         t = tables.numpy() if isinstance(tables, torch.Tensor) else np.asarray(tables)
-        s = np.asarray(slots, dtype=np.int64)
+        s = np.ascontiguousarray(slots, dtype=np.int64)
         if t.ndim != 2 or t.dtype != np.int32:
             raise ValueError("the page table is a matrix of 32-bit integers")
-        if s.ndim != 1 or len(s) > self.rows:
+        n, (n_slots, width) = len(s), t.shape
+        if s.ndim != 1 or n > self.rows:
             raise ValueError(f"a plan for {self.rows} rows does not take {s.shape}")
-        if len(s) and int(s.max()) >= len(t):
-            raise ValueError(f"slot {int(s.max())} of {len(t)}")
-        if lengths is not None and len(lengths) != len(s):
+        if n and int(s.max()) >= n_slots:
+            raise ValueError(f"slot {int(s.max())} of {n_slots}")
+        if lengths is not None and len(lengths) != n:
             raise ValueError("lengths has an entry per row")
-        if self.captured is not None and (len(s) > self.captured or t.shape != self.table_shape):
+        if width * self.page_tokens >= 1 << 31:
+            raise ValueError("a request has fewer than 2^31 tokens")
+        if self.captured is not None and (n > self.captured or t.shape != self.table_shape):
             raise ValueError(f"a captured call has {self.captured} rows and a page table of {tuple(self.table_shape)}")
-        self.n_rows, self.table_shape = len(s), t.shape
-        of: Dict[int, List[int]] = {}                          # rows of every slot
-        for r, slot in enumerate(s.tolist()):
-            if slot >= 0:
-                of.setdefault(slot, []).append(r)
-        keep = list(of)
-        runs = common_runs(t[keep]) if len(keep) > 1 else []
-        begin = np.zeros(len(s), dtype=np.int64)               # where a row's own keys begin
-        if self.chunk and lengths is not None:
-            begin = np.maximum(np.asarray(lengths, dtype=np.int64) - 1, 0) // self.chunk * self.chunk // self.page_tokens * self.page_tokens
-        group = np.full(len(s), -1)
-        self.shared, self.lows = [], []
-        for members, pages in runs:
-            tokens = pages * self.page_tokens
-            rows = sorted(r for i in members for r in of[keep[i]] if begin[r] < tokens)
-            if len(set(s[rows].tolist())) > 1 and tokens - int(begin[rows].min()) >= self.min_tokens:
-                self.lows.append(int(begin[rows].min()))
-                group[rows], begin[rows] = len(self.shared), tokens
-                self.shared.append((rows, tokens))
-        leased = {slot: self.page_tokens * int((np.append(t[slot], -1) < 0).argmax()) for slot in keep}
-        tails = []                                             # (first row, rows, first key, keys there are now)
-        for slot, rows in of.items():
-            at = 0
-            while at < len(rows):                              # neighbours, as many as a unit takes
-                n = 1
-                while at + n < len(rows) and n < self.rows_per_unit and rows[at + n] == rows[at] + n \
-                        and begin[rows[at + n]] == begin[rows[at]] and group[rows[at + n]] == group[rows[at]]:
-                    n += 1
-                have = leased[slot] if lengths is None else max(int(lengths[r]) for r in rows[at:at + n])
-                tails.append((rows[at], n, int(begin[rows[at]]), max(1, have - int(begin[rows[at]]))))
-                at += n
-        self._lay_out(s, tails, t.shape[1] * self.page_tokens)
-
-    def _lay_out(self, slots: np.ndarray, tails, limit: int) -> None:
-        pieces = [-(-len(rows) // self.rows_per_unit) for rows, _ in self.shared]
-        host = np.zeros(self.data.numel(), dtype=np.int32)
-        units, turns, order, cell, parts = (host[a:b] for a, b in zip(self._at, self._at[1:] + [len(host)]))
-        at = 0
-        for rows, _ in self.shared:
-            order[at:at + len(rows)] = rows
-            at += len(rows)
-        best = None
-        if tails:
-            ends = {x[0]: x[2] + x[3] for x in tails}
-            for least, span in self._spans(pieces, tails):
-                if best is None or least < best[0]:
-                    items, n_parts = self._items(slots, pieces, tails, limit, span)
-                    every, need = self._pairs(items, ends)
-                    place, time = self._deal(need)
-                    time += self._join_time(int(n_parts.sum()), int(n_parts.max()))
-                    if best is None or time < best[0]:
-                        best = (time, span, every, place, n_parts)
-        n = 0
-        self.span = 0
-        if best is not None:
-            _, self.span, every, place, n_parts = best
-            assert int(n_parts.sum()) <= self.max_cells, int(n_parts.sum())
-            units.reshape(-1, self.together, UNIT)[place] = every
-            turns[:] = np.bincount(place % self.grid, minlength=self.grid)
-            parts[:len(n_parts)] = n_parts
-            cell[:self.rows] = np.cumsum(parts) - parts
-            cell[self.rows:self.rows + len(slots)] = np.maximum(slots, -1) + 1
-            n = int(turns.max()) * self.grid * self.together
-        host[0] = self.n_units = n
-        self.data.copy_(torch.from_numpy(host))
-
-    def _join_time(self, parts: int, most: int) -> float:
-        return 8 * parts * self.heads * self.vdim * self.cost.byte + most * self.cost.part
-
-    def _spans(self, pieces, tails) -> List[Tuple[float, int]]:
-        """Lengths that the keys may be divided by: the time that a plan with it takes at least, length; the shortest time first."""
-        p, rows, tokens, n, keys = (np.array(x, dtype=np.int64) for x in (
-            pieces, [len(x) for x, _ in self.shared], [x - low for (_, x), low in zip(self.shared, self.lows)], [x[1] for x in tails], [x[3] for x in tails]))
-        longest, cost = int(max(tokens.max(initial=0), keys.max())), self.cost
-        unit = ceil_to(128 if self.dtype == BF16 else 32, self.page_tokens)
-        at_a_time = self.grid * self.together / self.kv_heads
-        per_key = cost.longer if self.together == 1 else (cost.longer + cost.shorter) / 2
-        out = []
-        for span in [k * unit for k in SPANS if k * unit < longest] + [ceil_to(longest, unit)]:      # the last one divides nothing
-            shared, own = -(-tokens // span), np.maximum(1, keys // span)
-            items = int((p * shared).sum() + own.sum())
-            if items <= len(tails) + sum(pieces) + self.extra:
-                busy = (items * cost.turn + float((p * tokens).sum() + keys.sum()) * per_key) / at_a_time
-                last = cost.turn + cost.longer * min(span, longest)
-                out.append((max(busy, last) + self._join_time(int((rows * shared).sum() + (n * own).sum()), 0), span))
-        return sorted(out)
-
-    def _items(self, slots: np.ndarray, pieces, tails, limit: int, span: int) -> Tuple[np.ndarray, np.ndarray]:
-        """What there is to do with at most `span` keys at a time, as units without their head, and the partial results of every row."""
-        items, at, parts = [], 0, np.zeros(len(slots), dtype=np.int32)
-        for p, (rows, tokens), low in zip(pieces, self.shared, self.lows):
-            count = -(-(tokens - low) // span)
-            parts[rows] = count
-            for i in range(p):
-                lo, hi = (len(rows) * j // p for j in (i, i + 1))
-                items += [(int(slots[rows[0]]), at + lo, hi - lo, low + k * span, min(tokens, low + (k + 1) * span), k, 0)
-                          for k in range(count)]
-            at += len(rows)
-        for first, rows, key0, keys in tails:
-            count = max(1, keys // span)                       # the last one goes on to wherever the request gets
-            part = int(parts[first])
-            items += [(int(slots[first]), first, rows, key0 + k * span, key0 + (k + 1) * span if k + 1 < count else limit, part + k, 1)
-                      for k in range(count)]
-            parts[first:first + rows] += count
-        return np.array(items, dtype=np.int32), parts
-
-    def _pairs(self, items: np.ndarray, ends: Dict[int, int]) -> Tuple[np.ndarray, np.ndarray]:
-        """Items and key/value heads as units, those that a block has at a time side by side (pieces that walk the same keys if there are
-        two), and what each such group takes."""
-        keys = items[:, 4] - items[:, 3]
-        last = np.array([ends.get(i, 0) for i in items[:, 1].tolist()])
-        keys = np.where(items[:, 6] == 1, np.minimum(keys, np.maximum(1, last - items[:, 3])), keys)
-        order = np.lexsort((items[:, 1], items[:, 3], items[:, 0], -keys))
-        # by head, then by item: pieces of one range stand side by side
-        every = np.concatenate([np.tile(items[order], (self.kv_heads, 1)), np.repeat(np.arange(self.kv_heads, dtype=np.int32), len(items))[:, None]], 1)
-        length = np.tile(keys[order], self.kv_heads)
-        w, cost = self.together, self.cost
-        if len(every) % w:
-            every, length = np.concatenate([every, np.zeros((1, UNIT), dtype=np.int32)]), np.append(length, 0)
-        every, length = every.reshape(-1, w, UNIT), length.reshape(-1, w)
-        longer = length.max(1)
-        return every, cost.turn + cost.row * every[:, :, 2].max(1) + cost.longer * longer + cost.shorter * (length.sum(1) - longer)
-
-    def _deal(self, need: np.ndarray) -> Tuple[np.ndarray, float]:
-        """Groups of units to blocks, the longest first, each to the block that has least to do: block b takes the places b, b + grid,
-        b + 2 grid ...  Returns their places, and the time until the last block is done."""
-        place = np.zeros(len(need), dtype=np.int64)
-        order = np.argsort(-need, kind="stable")
-        place[order[:self.grid]] = np.arange(min(self.grid, len(need)))
-        last = float(need.max())
-        if len(need) > self.grid:
-            blocks = [(time, 1, b) for b, time in enumerate(need[order[:self.grid]].tolist())]     # (time so far, turns, block)
-            heapq.heapify(blocks)
-            for i, time in zip(order[self.grid:].tolist(), need[order[self.grid:]].tolist()):
-                so_far, turn, b = blocks[0]
-                place[i] = turn * self.grid + b
-                last = max(last, so_far + time)
-                if turn + 1 < self.max_turns:
-                    heapq.heapreplace(blocks, (so_far + time, turn + 1, b))
-                else:
-                    heapq.heappop(blocks)
-        return place, last
+        t = np.ascontiguousarray(t)
+        have = np.ascontiguousarray(lengths, dtype=np.int64) if lengths is not None else None
+        cuda = self.data.is_cuda
+        if cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a plan is not set inside a capture")
+        # torch keeps a pinned buffer until the copies from it are done
+        to = torch.empty(self._size, dtype=I32, pin_memory=True) if cuda else self.data
+        _, at, shape, groups, result = self._shape
+        err = self._divide(shape, C.c_void_p(t.ctypes.data), n_slots, width, C.c_void_p(s.ctypes.data), n,
+                           C.c_void_p(have.ctypes.data if have is not None else 0), self._used, C.c_void_p(to.data_ptr()), at, groups, result)
+        if err:
+            _failed(err)
+        self.n_units, self.span, n_groups = self._result.tolist()
+        self.n_rows, self.table_shape = n, t.shape
+        a, b = self._at[0] + UNIT * max(self.n_units, self._used), self._at[1]
+        self._order = to[self._at[2]:self._at[2] + (int(self._groups[:3 * n_groups:3].sum()) if n_groups else 0)].numpy().copy()
+        self._used = self.n_units
+        if cuda:
+            self.data[:a].copy_(to[:a], non_blocking=True)
+            self.data[b:].copy_(to[b:], non_blocking=True)
 
     def check_status(self, what: str = "attention over a shared prefix"):
         lib.raise_on_status(self.status, what)

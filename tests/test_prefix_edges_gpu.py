@@ -209,3 +209,49 @@ def test_graphs_are_captured_right_behind_a_long_prompt():
         ses.step([toks[at]], [at], [0])
         close(e.logits_rows(1).cpu().double(), want[at:at + 1], "bf16", spread[at:at + 1])
     e.check_status()
+
+
+@pytest.mark.parametrize("kind", ["grouped", "latent"])
+def test_plans_are_made_while_the_gpu_is_busy(kind):
+    """set() orders its copies on the stream and does not wait for it; a later call takes the plan, an earlier one had its own."""
+    a = Pass(kind, groups=[(9, 12)], seed=1, **SMALL[kind])
+    b = Pass(kind, groups=[(5, 3)], alone=4, seed=2, **SMALL[kind])
+    width, slots = max(x.tables.shape[1] for x in (a, b)), max(x.tables.shape[0] for x in (a, b))
+    for x in (a, b):
+        t = torch.full((slots, width), -1, dtype=torch.int32)
+        t[:x.tables.shape[0], :x.tables.shape[1]] = x.tables
+        x.tables, x.d_tables = t, t.cuda()
+    plan = a.plan()
+    a.run(plan), b.plan()                                    # pinned memory and kernels are there
+    torch.cuda.synchronize()
+    torch.cuda._sleep(400_000_000)
+    busy = torch.cuda.Event()
+    busy.record()
+    got = []
+    for _ in range(4):
+        for x in (a, b):
+            plan.set(x.row_slot, x.tables)
+            got.append((x, x.run(plan)))
+    assert not busy.query()
+    torch.cuda.synchronize()
+    plan.check_status()
+    for x, out in got:
+        want, tol = x.expected()
+        assert ((out.double() - want).abs() <= tol).all()
+
+
+def test_plans_are_not_set_inside_a_capture():
+    p = Pass("grouped", groups=[(3, 4)], **SMALL["grouped"])
+    plan = p.plan()
+    out = torch.empty(p.R, p.H, p.V, dtype=BF16, device="cuda")
+    p.run(plan, out=out)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(RuntimeError, match="capture"):
+            plan.set(p.row_slot, p.tables)
+        p.run(plan, out=out)
+    g.replay()
+    torch.cuda.synchronize()
+    want, tol = p.expected()
+    assert ((out.double() - want).abs() <= tol).all()
