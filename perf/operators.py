@@ -158,9 +158,10 @@ def prepare(case, seed):
         s["groups"].append((torch.tensor(rows, device="cuda"), shared[rows[0]], max(last[i] for i in rows) + 1))
     if own:
         from ds41rt_b200.ops import prefix
+        # workspace; the division of a pass's work is a part of the pass.  A program keeps its page table on the host, too
         s["plan"] = prefix.PrefixPlan(case["kind"], rows=n + pads, heads=H, kv_heads=case["kv_heads"], vdim=case["vdim"],
                                       page_tokens=P, device="cuda", dtype=dt)
-        s["plan"].set(row_slot.tolist(), tables)
+        s["host"] = (row_slot.tolist(), tables)
     return s
 
 
@@ -210,6 +211,7 @@ def run(s):
     case = s["case"]
     if own:
         from ds41rt_b200.ops import prefix
+        s["plan"].set(*s["host"])
         if case["kind"] == "grouped":
             return prefix.group_attend(s["q"], s["pool"], s["tables"], s["row_pos"], s["row_slot"], s["plan"], scale=_scale(case),
                                        chunk=case["chunk"], gate=s["gate"], out=s["out"])
