@@ -411,6 +411,7 @@ int divide(const void* shape, const int32_t* table, int slots, int width, const 
   }
   data[0] = places;
   data[1] = data[2] = data[3] = 0;
+  std::copy(order.begin(), order.end(), groups + 3 * shared.size());
   for (size_t i = 0; i < shared.size(); ++i) {
     groups[3 * i] = shared[i].rows;
     groups[3 * i + 1] = shared[i].tokens;
@@ -446,7 +447,8 @@ int ds41_prefix_groups(const int32_t* table, int n, int width, int32_t* order, i
 // The plan of `n` rows of slots row_slot[] (negative: none) over the page table [slots][width]; `lengths`: tokens of each row's request
 // (null: what its pages hold).  `data`: [4 | units | turns | order | cell, owner | parts], the parts at at[0] .. at[4]; units of the
 // `used` places that the last plan had and this one has not become zeros.  groups[3 i]: rows of prefix i, its tokens, the first of them
-// that any of its rows sees; result: places, length of the ranges, prefixes.  0; -1: the plan's arrays do not hold the division; -2: no memory.
+// that any of its rows sees, behind the last prefix all their rows; result: places, length of the ranges, prefixes.
+// 0; -1: the plan's arrays do not hold the division; -2: no memory.
 int ds41_prefix_divide(const void* shape, const int32_t* table, int slots, int width, const int64_t* row_slot, int n, const int64_t* lengths,
                        int used, int32_t* data, const int32_t* at, int32_t* groups, int32_t* result) try {
   return divide(shape, table, slots, width, row_slot, n, lengths, used, data, at, groups, result);

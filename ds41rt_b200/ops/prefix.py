@@ -131,8 +131,11 @@ class PrefixPlan:
         self.n_units = self.span = 0
         self.n_rows, self.table_shape = 0, None            # of the last set(): what calls have to match
         self.captured: Optional[int] = None                # least rows of the calls that graphs hold
-        self._groups, self._result = np.zeros(3 * rows, dtype=np.int32), np.zeros(3, dtype=np.int32)
-        self._order, self._used = np.zeros(0, dtype=np.int32), 0
+        # prefixes: {rows, tokens, first of them that is seen} of each, then their rows; {places, length of the ranges, prefixes}
+        self._groups, self._result = np.zeros(4 * rows, dtype=np.int32), np.zeros(3, dtype=np.int32)
+        # one copy of everything costs less than two of what is used, if it is small (64 KB: 3 us of the host, 7 with the slices of two)
+        self._whole = self._size <= 1 << 14
+        self._used = 0
         shape = PlanShape(rows=rows, heads=heads, kv_heads=kv_heads, vdim=vdim, page_tokens=page_tokens, chunk=chunk,
                           rows_per_unit=self.rows_per_unit, together=self.together, grid=self.grid, min_tokens=min_tokens,
                           max_turns=self.max_turns, max_units=self.max_units, max_cells=self.max_cells, extra=self.extra,
@@ -150,10 +153,11 @@ class PrefixPlan:
     @property
     def shared(self) -> List[Tuple[List[int], int]]:
         """Rows and tokens of every prefix."""
-        out, at = [], 0
-        for i in range(int(self._result[2])):
+        out, n_groups = [], int(self._result[2])
+        at = 3 * n_groups
+        for i in range(n_groups):
             n, tokens = self._groups[3 * i:3 * i + 2].tolist()
-            out.append((self._order[at:at + n].tolist(), tokens))
+            out.append((self._groups[at:at + n].tolist(), tokens))
             at += n
         return out
 
@@ -187,17 +191,19 @@ class PrefixPlan:
         to = torch.empty(self._size, dtype=I32, pin_memory=True) if cuda else self.data
         _, at, shape, groups, result = self._shape
         err = self._divide(shape, C.c_void_p(t.ctypes.data), n_slots, width, C.c_void_p(s.ctypes.data), n,
-                           C.c_void_p(have.ctypes.data if have is not None else 0), self._used, C.c_void_p(to.data_ptr()), at, groups, result)
+                           C.c_void_p(have.ctypes.data if have is not None else 0), self.max_units if self._whole else self._used,
+                           C.c_void_p(to.data_ptr()), at, groups, result)
         if err:
             _failed(err)
-        self.n_units, self.span, n_groups = self._result.tolist()
+        self.n_units, self.span, _ = self._result.tolist()
         self.n_rows, self.table_shape = n, t.shape
-        a, b = self._at[0] + UNIT * max(self.n_units, self._used), self._at[1]
-        self._order = to[self._at[2]:self._at[2] + (int(self._groups[:3 * n_groups:3].sum()) if n_groups else 0)].numpy().copy()
-        self._used = self.n_units
-        if cuda:
+        if cuda and self._whole:
+            self.data.copy_(to, non_blocking=True)
+        elif cuda:
+            a, b = self._at[0] + UNIT * max(self.n_units, self._used), self._at[1]
             self.data[:a].copy_(to[:a], non_blocking=True)
             self.data[b:].copy_(to[b:], non_blocking=True)
+        self._used = self.n_units
 
     def check_status(self, what: str = "attention over a shared prefix"):
         lib.raise_on_status(self.status, what)
