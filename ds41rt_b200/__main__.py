@@ -507,14 +507,16 @@ def cmd_serve(args) -> int:
     from .runtime.memory import plan_pool
     torch.cuda.synchronize()
     free_now = torch.cuda.mem_get_info(dev)[0]
+    max_rows = max(8, args.concurrency, args.prefill_chunk)
+    workspace = fam.shared_prefix_bytes(weights, max_rows) if args.shared_prefix else 0
     plan = plan_pool(cfg, n_layers=cfg.n_layers, slots=args.concurrency, max_context=args.max_context,
                      free_bytes=free_now, kv_dtype=args.kv_dtype, retained=args.prompt_snapshots + args.turn_snapshots,
-                     ring_rows=cfg.window + max(16, args.prefill_chunk), reserve_bytes=args.reserve_gb << 30)
+                     ring_rows=cfg.window + max(16, args.prefill_chunk), reserve_bytes=(args.reserve_gb << 30) + workspace)
     n_pages = int(fabric.all_reduce_max(-plan.pages) * -1) if world > 1 else plan.pages     # the smallest rank decides
     if n_pages < (args.max_context + 63) // 64 + 1:
         print(f"rank {rank}: only {n_pages} KV pages fit; lower --max-context or --concurrency", file=sys.stderr)
         return 2
-    eng = fam.engine(cfg, weights, fabric, max_rows=max(8, args.concurrency, args.prefill_chunk), slots=args.concurrency,
+    eng = fam.engine(cfg, weights, fabric, max_rows=max_rows, slots=args.concurrency,
                      max_ctx=args.max_context, kv_dtype=args.kv_dtype, n_pages=n_pages,
                      **({"shared_prefix": True} if args.shared_prefix else {}))
     engram_layers = _attach_engram(args, cfg, eng, dev)

@@ -20,6 +20,10 @@ class Family:
     dtypes: tuple = ("bf16",)
     shared_prefix = False     # do its engines take `shared_prefix`?
 
+    def shared_prefix_bytes(self, weights, max_rows: int) -> int:
+        """Device memory that `shared_prefix` takes."""
+        return 0
+
     def matches(self, doc: dict) -> bool:
         raise NotImplementedError
 
@@ -73,6 +77,10 @@ class StackFamily(Family):
 
     def __init__(self, name: str, module):
         self.name, self.module, self.presets = name, module, module.PRESETS
+
+    def shared_prefix_bytes(self, weights, max_rows):
+        from .stack import prefix_plan_bytes
+        return prefix_plan_bytes(weights, max_rows)
 
     def matches(self, doc):
         return self.module.matches(doc)

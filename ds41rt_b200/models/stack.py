@@ -600,6 +600,27 @@ def row_requests(pos: np.ndarray, slot: np.ndarray) -> int:
     return n
 
 
+ABSORBED_ROWS = 256           # most rows of passes that read the cache row by row, or by a plan
+
+
+def prefix_plan_sizes(weights: "StackWeights", max_rows: int, page_tokens: int) -> Dict[tuple, dict]:
+    """What the plans of shared prefixes are made with, by shape of attention: those whose tensor-core forms take the shape."""
+    out = {}
+    for lw in weights.layers if weights.dtype != "f32" else ():
+        if not hasattr(lw.mixer, "prefix_shape"):
+            continue
+        kind, heads, kv_heads, dim, vdim, chunk = key = lw.mixer.prefix_shape()
+        if prefix.tiled(kind, heads, kv_heads, dim, vdim, page_tokens):
+            out[key] = dict(kind=kind, rows=min(max_rows, ABSORBED_ROWS), heads=heads, kv_heads=kv_heads, vdim=vdim,
+                            page_tokens=page_tokens, chunk=chunk)
+    return out
+
+
+def prefix_plan_bytes(weights: "StackWeights", max_rows: int, page_tokens: int = 64) -> int:
+    """Device memory of an engine's plans of shared prefixes."""
+    return sum(prefix.PrefixPlan.nbytes(**sizes) for sizes in prefix_plan_sizes(weights, max_rows, page_tokens).values())
+
+
 class StackEngine(RowsEngine):
     partial_prefix = False        # recurrent states belong to a snapshot's whole length
     replay_window = 1 << 30       # the prefix banks then never prefer a truncated snapshot
@@ -635,7 +656,7 @@ class StackEngine(RowsEngine):
         act = heads = q = 8
         q_rank = 8
         lat = 0
-        self.attn_rows = min(R, 256)
+        self.attn_rows = min(R, ABSORBED_ROWS)
         cells = 1
         for lw in weights.layers:
             for m in lw.parts():
@@ -712,15 +733,9 @@ class StackEngine(RowsEngine):
         self.prefix_plans = {}
         self._planned, self._plan_from, self._plan_until = None, [], 0
         self._undescribed = None      # (positions, slots) of a pass that needs no plan, until one over the same rows does
-        if not shared_prefix or self.f32:
-            return
-        for lw in self.w.layers:
-            if not hasattr(lw.mixer, "prefix_shape"):
-                continue
-            kind, heads, kv_heads, dim, vdim, chunk = key = lw.mixer.prefix_shape()
-            if key not in self.prefix_plans and prefix.tiled(kind, heads, kv_heads, dim, vdim, self.cache.page_tokens):
-                self.prefix_plans[key] = prefix.PrefixPlan(kind, rows=self.attn_rows, heads=heads, kv_heads=kv_heads, vdim=vdim,
-                                                           page_tokens=self.cache.page_tokens, device=self.device, chunk=chunk)
+        if shared_prefix:
+            self.prefix_plans = {key: prefix.PrefixPlan(device=self.device, **sizes)
+                                 for key, sizes in prefix_plan_sizes(self.w, self.max_rows, self.cache.page_tokens).items()}
 
     def prefix_plan(self, mixer, rows: int) -> Optional[prefix.PrefixPlan]:
         """The plan that a pass takes, static per batch size, as a captured pass needs it: its contents follow the rows.  A long pass asks

@@ -111,18 +111,7 @@ class PrefixPlan:
         self.kind, self.rows, self.heads, self.kv_heads, self.vdim = kind, rows, heads, kv_heads, vdim
         self.page_tokens, self.dtype, self.device, self.chunk = page_tokens, dtype, torch.device(device), chunk
         self.min_tokens, self.cost = min_tokens, COSTS[kind] if dtype == BF16 else COST_F32
-        self.rows_per_unit = max(1, 128 // (heads // kv_heads))
-        self.together = 2 if kind == "grouped" else 1            # units that a block (latent, wide: two blocks) has at a time
-        self.grid = SMS // 2 if kind == "latent" and vdim > 256 else SMS               # two CTAs to a unit
-        self.extra = 3 * -(-self.grid * self.together // kv_heads)      # items beyond one for every piece of a prefix and every request
-        self.max_items = self.extra + 2 * rows
-        # a head's items go in twos (one may stay alone), the heads are dealt one like the other
-        self.max_turns = -(-(self.max_items + 1) * kv_heads // (self.grid * self.together)) + 2
-        self.max_units = self.max_turns * self.grid * self.together
-        self.max_cells = self.extra * min(self.rows_per_unit, rows) + 2 * rows
-        # [count, 3 unused | units | turns | order | cell, owner | parts]
-        self._at = np.cumsum([4, UNIT * self.max_units, self.grid, rows, 2 * rows]).tolist()
-        self._size = self._at[-1] + rows
+        self._sizes(kind, rows, heads, vdim, kv_heads)
         self.data = torch.zeros(self._size, dtype=I32, device=self.device)
         # parts without a weight are not read
         self.part_o = torch.empty(self.max_cells * heads * vdim, dtype=F32, device=self.device)
@@ -149,6 +138,27 @@ class PrefixPlan:
         a.part_o, a.part_ml = self.part_o.data_ptr(), self.part_ml.data_ptr()
         a.max_units, a.rows_per_unit, a.grid = self.max_units, self.rows_per_unit, self.grid
         self.args, self.args_ref = a, C.byref(a)
+
+    def _sizes(self, kind: str, rows: int, heads: int, vdim: int, kv_heads: int):
+        self.rows_per_unit = max(1, 128 // (heads // kv_heads))
+        self.together = 2 if kind == "grouped" else 1            # units that a block (latent, wide: two blocks) has at a time
+        self.grid = SMS // 2 if kind == "latent" and vdim > 256 else SMS               # two CTAs to a unit
+        self.extra = 3 * -(-self.grid * self.together // kv_heads)      # items beyond one for every piece of a prefix and every request
+        self.max_items = self.extra + 2 * rows
+        # a head's items go in twos (one may stay alone), the heads are dealt one like the other
+        self.max_turns = -(-(self.max_items + 1) * kv_heads // (self.grid * self.together)) + 2
+        self.max_units = self.max_turns * self.grid * self.together
+        self.max_cells = self.extra * min(self.rows_per_unit, rows) + 2 * rows
+        # [count, 3 unused | units | turns | order | cell, owner | parts]
+        self._at = np.cumsum([4, UNIT * self.max_units, self.grid, rows, 2 * rows]).tolist()
+        self._size = self._at[-1] + rows
+
+    @classmethod
+    def nbytes(cls, kind: str, *, rows: int, heads: int, vdim: int, kv_heads: int = 1, **_) -> int:
+        """Device memory that a plan of these sizes takes."""
+        p = cls.__new__(cls)
+        p._sizes(kind, rows, heads, vdim, kv_heads)
+        return 4 * (p._size + p.max_cells * heads * (vdim + 2) + 4)
 
     @property
     def shared(self) -> List[Tuple[List[int], int]]:

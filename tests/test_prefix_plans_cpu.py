@@ -111,3 +111,21 @@ def test_heads_whose_units_do_not_come_in_twos():
         for spans in seen.values():
             spans.sort()
             assert spans[0][0] == 0 and spans[-1][1] == 320 and all(a[1] == b[0] for a, b in zip(spans, spans[1:]))
+
+
+def test_the_memory_of_plans_is_known_before_they_are_made():
+    from types import SimpleNamespace as N
+    from ds41rt_b200.models.registry import FAMILIES
+    from ds41rt_b200.models.stack import prefix_plan_bytes, prefix_plan_sizes
+    from ds41rt_b200.ops.prefix import PrefixPlan
+    shapes = [("grouped", 32, 8, 128, 128, 0), ("grouped", 32, 8, 128, 128, 8192), ("grouped", 32, 8, 128, 128, 0),
+              ("latent", 16, 1, 576, 512, 0), ("latent", 4, 1, 96, 64, 0), ("grouped", 4, 2, 320, 64, 0)]
+    layers = [N(mixer=N(prefix_shape=lambda s=s: s)) for s in shapes] + [N(mixer=N())]
+    w = N(dtype="bf16", layers=layers)
+    sizes = prefix_plan_sizes(w, 40, 64)
+    assert set(sizes) == set(shapes[:5])                     # wide keys are read row by row
+    made = [PrefixPlan(device="cpu", **s) for s in sizes.values()]
+    assert prefix_plan_bytes(w, 40) == sum(t.numel() * t.element_size() for p in made for t in (p.data, p.part_o, p.part_ml, p.status))
+    assert prefix_plan_bytes(w, 5000) == prefix_plan_bytes(w, 256) > prefix_plan_bytes(w, 40)
+    assert prefix_plan_bytes(N(dtype="f32", layers=layers), 40) == 0
+    assert FAMILIES["belasun"].shared_prefix_bytes(w, 40) == prefix_plan_bytes(w, 40) and FAMILIES["ds41"].shared_prefix_bytes(w, 40) == 0
