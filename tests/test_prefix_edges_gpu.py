@@ -255,3 +255,31 @@ def test_plans_are_not_set_inside_a_capture():
     torch.cuda.synchronize()
     want, tol = p.expected()
     assert ((out.double() - want).abs() <= tol).all()
+
+
+def test_a_device_loop_gives_the_logits_of_its_own_tokens():
+    """Steps that feed themselves across pages, as requests outgrow the lengths that the plan was made with, against the plain CPU statement
+    of the tokens that came out."""
+    import test_belasun_gpu as belasun
+    from ds41rt_b200.runtime.session import DecodeSession
+    from test_stack_gpu import close, feed
+    e = belasun.engine("tiles", "bf16", shared_prefix=True, page_tokens=32)
+    common = belasun.tokens("tiles", 130, seed=8)
+    feed(e, 0, common, 0, [1024])
+    snap = e.cache.snapshot(0, 130)
+    assert e.cache.restore(1, snap) and all(e.cache.ensure(s, 300) for s in (0, 1))
+    ses = DecodeSession(e)
+    e.set_rows([3, 200], [130, 130], [0, 1])
+    toks, seen = [[3], [200]], {}
+    for step in range(120):
+        ses.run_device_loop(2, 1)
+        if step % 13 == 0 or step == 119:
+            seen[130 + step] = e.logits_rows(2).cpu().double()
+        for t, new in zip(toks, e.in_tokens[:2].tolist()):
+            t.append(new)
+    e.check_status()
+    assert e.row_pos[:2].tolist() == [250, 250]
+    for r in range(2):
+        want, spread = belasun.reference("tiles", common + toks[r][:120], "bf16")[:2]
+        for at, got in seen.items():
+            close(got[r:r + 1], want[at:at + 1], "bf16", spread[at:at + 1])
