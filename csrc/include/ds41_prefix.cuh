@@ -30,7 +30,7 @@ __device__ __forceinline__ int prefix_row(const ds41_prefix_plan& p, const Prefi
 // as well since rows may stand inside them, may hold anything.  In two steps, so that the positions of several units can be under
 // way together.
 struct PrefixRows {
-  int low, high;                       // of this lane's rows that see any of the unit's keys
+  int low, high;                       // of this lane's rows that see any of the unit's keys; of all lanes' behind prefix_span()
   int wide_low, wide_high;             // the longest window of one of them, inside the unit
 };
 __device__ __forceinline__ PrefixRows prefix_rows(const ds41_prefix_plan& p, const PrefixUnit& u, const int* row_pos, const int* row_slot,
@@ -49,7 +49,7 @@ __device__ __forceinline__ PrefixRows prefix_rows(const ds41_prefix_plan& p, con
   }
   return v;
 }
-__device__ __forceinline__ void prefix_span(const PrefixUnit& u, PrefixRows v, int chunk, int page_tokens, int& first, int& end) {
+__device__ __forceinline__ void prefix_span(const PrefixUnit& u, PrefixRows& v, int chunk, int page_tokens, int& first, int& end) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
     v.low = min(v.low, __shfl_xor_sync(0xffffffffu, v.low, o));

@@ -296,7 +296,6 @@ prefix_join_kernel(const ds41_prefix_plan plan, const float* sink, const ds41_pr
   const long long cell = r < rows ? 1ll * plan.cell[r] * heads + h : 0;
   pdl_wait();
   if (r >= rows) return;
-  const float sk = sink != nullptr ? sink[h] * 1.4426950408889634f : -INFINITY;
   const int slot = keep.row_slot[r];
   // a row of another slot than the one that the plan holds its keys for: no result is right
   const bool stray = slot >= 0 && slot + 1 != owner;
@@ -306,6 +305,8 @@ prefix_join_kernel(const ds41_prefix_plan plan, const float* sink, const ds41_pr
     keep.status[2] = r;
     keep.status[3] = slot;
   }
+  // parts of a row without a slot are empty, so that its sum stays zero; that of a stray one becomes NaN
+  const float sk = stray ? NAN : sink != nullptr && slot >= 0 ? sink[h] * 1.4426950408889634f : -INFINITY;
   if (keep.taps > 1 && slot >= 0)
     keep_inputs(keep, r, slot, keep.row_pos[r], w % (heads * strips), heads * strips, lane, 32);
   const float2* ml = reinterpret_cast<const float2*>(plan.part_ml) + cell;
@@ -315,8 +316,7 @@ prefix_join_kernel(const ds41_prefix_plan plan, const float* sink, const ds41_pr
   float all = fmaxf(sk, mine.x);
   for (int s = lane + 32; s < n; s += 32) all = fmaxf(all, ml[1ll * s * heads].x);
   all = warp_max(all);
-  // parts of a row without a slot are empty, so that its sum stays zero
-  float den = stray ? NAN : sink != nullptr && slot >= 0 && lane == 0 && all > -INFINITY ? exp2f(sk - all) : 0.f;
+  float den = lane > 0 || sk == -INFINITY ? 0.f : exp2f(sk - all);
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int s0 = 0; s0 < n; s0 += 32) {
     if (s0 > 0) mine = s0 + lane < n ? ml[1ll * (s0 + lane) * heads] : make_float2(-INFINITY, 0.f);

@@ -49,11 +49,12 @@ struct PrefixGroupParams {
 };
 
 // What a CTA's two tiles do next, as the producer found it: unit t walks `tiles[t]` key tiles from `first[t]` on, and nobody sees
-// `end[t]` or what follows.  both: they walk the same ones.  Key tiles inside [safe[t], safe_end[t]) have no place that nobody sees.
+// `end[t]` or what follows.  both: they walk the same ones.  Key tiles inside [safe[t], safe_end[t]) have no place that nobody sees; of
+// the places outside all are unseen, or it takes a look at the rows (gaps).
 struct __align__(16) GroupWork {
   PrefixUnit unit[2];
   int first[2], end[2], tiles[2], base, both;              // base: number of the first key tile in the order of the copies
-  int safe[2], safe_end[2];
+  int safe[2], safe_end[2], gaps[2];
   int row[2][32];                                          // pool rows of the first 32 boxes of their keys
 };
 
@@ -150,7 +151,7 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap keys, const __grid_const
       const PrefixUnit a = turn == 0 ? first_a : prefix_unit(plan, at), b = turn == 0 ? first_b : prefix_unit(plan, at + 1);
       // without chunks a walk begins at its first key: its pages are looked up together with its rows' positions
       int row_a = locate(a.slot, a.key0, a.key1, 0), row_b = locate(b.slot, b.key0, b.key1, 0);
-      const PrefixRows rows_a = prefix_rows(plan, a, p.row_pos, p.row_slot, p.chunk), rows_b = prefix_rows(plan, b, p.row_pos, p.row_slot, p.chunk);
+      PrefixRows rows_a = prefix_rows(plan, a, p.row_pos, p.row_slot, p.chunk), rows_b = prefix_rows(plan, b, p.row_pos, p.row_slot, p.chunk);
       int first[2], end[2];
       prefix_span(a, rows_a, p.chunk, p.page_tokens, first[0], end[0]);
       prefix_span(b, rows_b, p.chunk, p.page_tokens, first[1], end[1]);
@@ -162,15 +163,19 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap keys, const __grid_const
         end[0] = end[1] = max(end[0], end[1]);
       }
       // without chunks every place before `end` is seen by the row that stands last; with them, a row's window vouches for its tiles
-      int safe[2] = {first[0], first[1]}, safe_end[2] = {end[0], end[1]};
+      int safe[2] = {first[0], first[1]}, safe_end[2] = {end[0], end[1]}, gaps[2] = {0, 0};
       if (p.chunk > 0) {
         prefix_widest(rows_a, safe[0], safe_end[0]);
         prefix_widest(rows_b, safe[1], safe_end[1]);
+        int low[2] = {max(rows_a.low, a.key0), max(rows_b.low, b.key0)};
         if (both) {
           const int t = safe_end[1] - safe[1] > safe_end[0] - safe[0];
           safe[0] = safe[1] = t ? safe[1] : safe[0];
           safe_end[0] = safe_end[1] = t ? safe_end[1] : safe_end[0];
+          low[0] = low[1] = min(low[0], low[1]);
         }
+        gaps[0] = low[0] < safe[0] || end[0] > safe_end[0];
+        gaps[1] = low[1] < safe[1] || end[1] > safe_end[1];
       }
       // what lies behind the unit's keys is read as zeros
       if (safe_end[0] == a.key1) safe_end[0] = 0x7fffffff;
@@ -192,6 +197,7 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap keys, const __grid_const
         w.tiles[lane] = lane ? tiles[1] : tiles[0];
         w.safe[lane] = lane ? safe[1] : safe[0];
         w.safe_end[lane] = lane ? safe_end[1] : safe_end[0];
+        w.gaps[lane] = lane ? gaps[1] : gaps[0];
         w.base = base;
         w.both = both;
       }
@@ -346,7 +352,7 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap keys, const __grid_const
     __syncwarp();
   } else {
     // the roles that follow one tile: its work at a turn, once it is known; whole warps
-    auto work = [&](int turn, int t, PrefixUnit& unit, int& first, int& safe, int& safe_end) {
+    auto work = [&](int turn, int t, PrefixUnit& unit, int& first, int& safe, int& safe_end, bool& gaps) {
       ok = __all_sync(0xffffffffu, mbar_wait(&sh.info_full[turn % kPgInfos], (turn / kPgInfos) & 1, p.status, 462)) != 0;
       if (!ok) return 0;
       const GroupWork& w = sh.info[turn % kPgInfos];
@@ -354,6 +360,7 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap keys, const __grid_const
       first = w.first[t];
       safe = w.safe[t];
       safe_end = w.safe_end[t];
+      gaps = w.gaps[t] != 0;
       return w.tiles[t];
     };
     auto work_read = [&](int turn) {
@@ -362,6 +369,7 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap keys, const __grid_const
     };
     PrefixUnit unit;
     int first, safe, safe_end;
+    bool gaps;
     if (warp >= 10) {
       // A row's queries lie side by side: pieces of 16 bytes by neighbouring lanes, or whole rows where they are shorter than a warp.
       const int t = warp - 10, pieces = p.n * p.dp / 8, per = max(1, 32 / pieces), sub = pieces < 32 ? lane / pieces : 0;
@@ -415,7 +423,7 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap keys, const __grid_const
       const int mine_row = mine / p.n, mine_head = mine - mine_row * p.n;
       int tiles = 0, done = 0, pairs = 0, cut = 0;       // tiles of S; units with keys, with two tiles or more; key tiles with unseen places
       for (int turn = 0; turn < turns; ++turn) {
-        const int n = work(turn, t, unit, first, safe, safe_end);
+        const int n = work(turn, t, unit, first, safe, safe_end, gaps);
         if (!ok) break;
         work_read(turn);
         if (n == 0) {                                    // nothing for any of its rows
@@ -521,10 +529,9 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap keys, const __grid_const
           }
           if (key0 < safe || key0 > safe_end - kPgKeys) {
             // Places that no row sees may hold anything, and a weight of zero does not take a NaN or an infinity away: their values
-            // become zeros, two threads to a place.  Behind the last position of all rows that is known; a tile with a chunk's border,
-            // or between the windows of rows in different chunks, asks the rows of whoever walks these keys.
+            // become zeros, two threads to a place.  Where rows stand in different chunks, those of whoever walks these keys are asked.
             uint32_t seen[2];
-            if (p.chunk > 0) {
+            if (gaps) {
               const PrefixUnit other = prefix_unit(plan, 2 * (static_cast<int>(blockIdx.x) + turn * static_cast<int>(gridDim.x)) + (t ^ 1));
               unsigned long long mask = prefix_seen(plan, unit, p.row_pos, p.row_slot, p.chunk, key0);
               if (!unit.tail && !other.tail && other.slot == unit.slot && other.key0 == unit.key0 && other.key1 == unit.key1 &&
@@ -533,9 +540,10 @@ prefix_group_kernel(const __grid_constant__ CUtensorMap keys, const __grid_const
               seen[0] = __reduce_or_sync(0xffffffffu, static_cast<uint32_t>(mask));
               seen[1] = __reduce_or_sync(0xffffffffu, static_cast<uint32_t>(mask >> 32));
             } else {
-              const int shown = safe_end - key0;            // 1 to 63: the tile has been asked for
-              seen[0] = shown >= 32 ? 0xffffffffu : (1u << shown) - 1;
-              seen[1] = (1u << max(shown - 32, 0)) - 1;
+              const int from = max(safe - key0, 0), to = min(safe_end - key0, kPgKeys);
+              const unsigned long long mask = from < to ? (~0ull >> (64 - (to - from))) << from : 0ull;
+              seen[0] = static_cast<uint32_t>(mask);
+              seen[1] = static_cast<uint32_t>(mask >> 32);
             }
             ok = __all_sync(0xffffffffu, mbar_wait(&sh.v_here[t], cut & 1, p.status, 484 + t)) != 0;
             if (!ok) break;

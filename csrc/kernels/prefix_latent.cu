@@ -149,7 +149,8 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
 
   auto span = [&](const PrefixUnit& it, int& end) {            // the key tiles of a unit (whole warps)
     int first;
-    prefix_span(it, prefix_rows(plan, it, p.row_pos, p.row_slot, 0), 0, p.page_tokens, first, end);
+    PrefixRows rows = prefix_rows(plan, it, p.row_pos, p.row_slot, 0);
+    prefix_span(it, rows, 0, p.page_tokens, first, end);
     return (end - first + kPlKeys - 1) / kPlKeys;
   };
 
@@ -302,7 +303,7 @@ prefix_latent_kernel(const __grid_constant__ CUtensorMap pool, const __grid_cons
     const int my_row = mine / p.heads, h = mine - my_row * p.heads;
     auto look = [&](const PrefixUnit& next) {
       it = next;
-      const PrefixRows rows = prefix_rows(plan, it, p.row_pos, p.row_slot, 0);
+      PrefixRows rows = prefix_rows(plan, it, p.row_pos, p.row_slot, 0);
       r = -1;
       hi = 0;
       if (my_row < it.rows) {
