@@ -1,8 +1,9 @@
 // Attention of rows that share prefixes: its parts for every type and size, and their join.
 //
 // A block takes sixteen queries (head and row) of a unit and walks its keys 32 at a time through shared memory, so that a cached
-// value that was read once serves sixteen queries: scores by warps of 8 queries x 8 keys (6 rows of 16 heads and 576 values over 500 keys
-// in 32 bits: 25 us, 46 with two pairs to a thread, which narrow rows take: 64 and 46 us with 32 values), a softmax state per query
+// value that was read once serves sixteen queries: scores by warps of 8 queries x 8 keys, or two pairs to a thread where a key has at most
+// 64 values (32 bits, the first and the second: 6 rows of 16 heads over 500 keys of 576 values 23.9 and 29.8 us, of 48 values 28.5 and
+// 25.3; 8 rows of 16 heads over 1000 keys of 128 values 21.8 and 22.3, of 32 values 22.5 and 19.3), a softmax state per query
 // (running maximum and sum), results in registers.  A warp fetches four of the keys, whose places it looks up a tile ahead; values that
 // are a part of their key (a latent) are fetched once.  It serves 32-bit rows and the sizes that the tensor-core forms
 // (prefix_group.cu, prefix_latent.cu) leave out, and is bound by its 32-bit products and their operands from shared memory.
@@ -279,9 +280,9 @@ static int run_simple(const SimpleArgs& p, const ds41_prefix_plan& plan, int f32
 // A warp joins 128 columns of a (row, head): the lanes find the parts' weights, then every lane sums four columns over the parts, PARTS
 // of them under way together.  Rows without a slot become zero; rows of another slot than the plan's become NaN and are reported.
 // The launch also keeps the convolution's last inputs where the attention has one (ds41_group.cuh).
-// A chain of loads from L2: small launches want many of them under way (94 registers), large ones many warps (56).  Whole calls with 8 / 4
-// parts: 37 rows of 6 heads in 13 parts 13.5 / 15.2 us, 32 rows of 32 heads 22.8 / 23.8 (1024 warps); 32 rows x 32 heads x 512 columns
-// (4096 warps) 31.7 / 30.3 us, 128 rows (16384) 204 / 198.
+// A chain of loads from L2: small launches want many of them under way (101 registers), large ones many warps (56).  Whole calls with 8 / 4
+// parts: 37 rows of 6 heads in 13 parts 15.7 / 18.3 us, 32 rows of 32 heads 22.8 / 24.5 (1024 warps); 32 rows x 32 heads x 512 columns
+// (4096 warps) 33.0 / 31.6 us, 128 rows (16384) 214 / 207.
 template <typename T, int PARTS>
 __global__ void __launch_bounds__(128, PARTS == 8 ? 1 : 9)
 prefix_join_kernel(const ds41_prefix_plan plan, const float* sink, const ds41_proj gate, int rows, int heads, int vp, T* out, int ld_out,

@@ -21,7 +21,7 @@
 // 48 per 128 x 64 x 16, the values' 64) and the 128 exponentials of a scheduler's two warps 1024; the softmax warps are the longest chain.
 // Letting them take turns at the exponentials, or taking a quarter of these by a polynomial, made steps of 1900 cycles and no call
 // shorter.  A unit costs 1.4 us beside its keys and 0.1 us per row (queries in, results out); requests' own keys are tiles of a few live
-// queries at the same price, and almost half of the call above (123 us with units dealt by these costs).
+// queries at the same price, and almost half of the call above (124 us with units dealt by these costs).
 #include <cuda.h>
 
 #include "ds41_group.cuh"

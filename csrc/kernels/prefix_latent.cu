@@ -15,15 +15,16 @@
 //   warp 8        : TMA producer, page by page
 //   warp 9        : tcgen05.mma issue, in whichever order their inputs come: S = Q K^T as soon as the last S is in registers, O += P V
 //   warp 10       : tells the other CTA which of its scores have been read.  That takes a release that the whole cluster sees, which
-//                   also waits for the scores that a softmax warp has just sent: by those warps 128 rows of 32 heads over 16000 keys take
-//                   236 us, 212 so
+//                   also waits for the scores that a softmax warp has just sent: calls of 128 rows of 32 heads over 16000 keys take
+//                   236 us where those warps make it, 212 so
 // The running maximum is raised when it grew by more than 2^8 only.  P is rounded to bf16 as the operand of the second product; sums
 // stay in 32 bits.
 //
-// What bounds it: 64 keys take a pair 2470 cycles (128 rows of 32 heads over 16000 shared keys and up to 700 own ones: 198 us with the
+// What bounds it: 64 keys take a pair 2600 cycles (128 rows of 32 heads over 16000 shared keys and up to 700 own ones: 207 us with the
 // join), of which the tensor core works 1150.  Sending a tile's scores takes 1200 and they share the way into an SM with the next tiles,
-// which need a deep ring: with three sets and a third exchange buffer in a place of the ring the call takes 238 us, with three sets and
-// two buffers 212.  In one CTA (256 latent values: 73 us) 64 keys take 1425: a tile's P waits for the values before it to let go of it.
+// which need a deep ring: with three sets and a third exchange buffer in a place of the ring the call took 238 us, with three sets and
+// two buffers 212, when with two sets it took 203.  In one CTA (256 latent values: 73 us) 64 keys take 1425: a tile's P waits for the
+// values before it to let go of it.
 #include <cuda.h>
 
 #include "ds41_prefix.cuh"
