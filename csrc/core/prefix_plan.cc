@@ -116,7 +116,7 @@ struct Item {
 };
 // A block as one number that compares as (time that it is busy, turns, block): the time in tenths of a nanosecond.
 using Block = uint64_t;
-constexpr int kTurnBits = 16, kIdBits = 10;
+constexpr int kTurnBits = 20, kIdBits = 8;
 Block block(double busy, int turns, int id) {
   return (static_cast<uint64_t>(busy * 1e4) << kTurnBits | static_cast<uint64_t>(turns)) << kIdBits | static_cast<uint64_t>(id);
 }
@@ -300,6 +300,7 @@ int divide(const void* shape, const int32_t* table, int slots, int width, const 
            int used, int32_t* data, const int32_t* at, int32_t* groups, int32_t* result) {
   const Shape& s = *static_cast<const Shape*>(shape);
   const int P = s.page_tokens, limit = width * P;
+  if (s.grid > 1 << kIdBits || s.max_turns > 1 << kTurnBits) return -1;
   std::vector<int> index(slots, -1), keep, rows_of, first_of, begin(n, 0), group(n, -1);
   for (int r = 0; r < n; ++r)
     if (row_slot[r] >= 0 && index[row_slot[r]] < 0) {

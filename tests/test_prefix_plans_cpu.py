@@ -129,3 +129,15 @@ def test_the_memory_of_plans_is_known_before_they_are_made():
     assert prefix_plan_bytes(w, 5000) == prefix_plan_bytes(w, 256) > prefix_plan_bytes(w, 40)
     assert prefix_plan_bytes(N(dtype="f32", layers=layers), 40) == 0
     assert FAMILIES["belasun"].shared_prefix_bytes(w, 40) == prefix_plan_bytes(w, 40) and FAMILIES["ds41"].shared_prefix_bytes(w, 40) == 0
+
+
+def test_blocks_that_come_back_very_often():
+    """Thousands of heads: each block takes its turns by the thousand, and no place is dealt twice."""
+    p = plan(rows=40, heads=8192, kv_heads=8192, vdim=16)
+    p.set(range(40), many(40, pages=2, own=3, width=6))
+    d = p.data.numpy()
+    units = d[4:4 + 8 * p.n_units].reshape(-1, 8)
+    alive = units[units[:, 2] > 0]
+    assert len({(u[1], u[3], u[6], u[7]) for u in alive.tolist()}) == len(alive)
+    turns = d[p._at[1]:p._at[2]]
+    assert turns.max() <= p.max_turns and int(turns.sum()) >= len(alive) // 2 and turns.max() - turns.min() <= 2
