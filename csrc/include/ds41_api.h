@@ -677,6 +677,65 @@ int ds41_gemm_f32(const float* A, const float* B, float* out, int M, int N, int 
                   long long ldo, int batch, long long a_batch_stride, long long b_batch_stride,
                   long long out_batch_stride, const int* batch_map, const int* n_active, void* stream);
 
+// ---------------------------------------------------------------------------------------------------
+// Ragged passes (ragged.cu, ragged_attend.cu): requests with any number of new tokens each over a paged cache.  Request i brings news[i]
+// tokens, the last of lengths[i], in slot slots[i]; its rows follow those of request i - 1.  What a pass is made of, and the workspace of
+// its calls, is written on the device from the requests' lengths:
+typedef struct ds41_ragged_pass {
+  int* header;                    // [16] {units, rows of all requests}
+  int* row_pos;                   // [rows] position, slot (-1: none) and row of the pool (-1: none) of every row; rows behind the last
+  int* row_slot;                  //   request's: 0, -1, -1
+  int* row_place;
+  int* units;                     // [max_units][12] {slot, first row, tokens, first position, key/value head, first key tile, key tiles,
+                                  //   piece, pieces, first cell, counter, cells between pieces}
+  unsigned int* counters;         // [max_blocks * kv_heads][2] finished pieces of both tiles, zero between calls
+  float* part_o;                  // [max_cells][vdim] unnormalised results of pieces
+  float* part_ml;                 // [max_cells]{maximum in units of log 2, sum}
+  int* status;
+  int rows, requests;             // most of them
+  int heads, kv_heads, dim, vdim, page_tokens;
+  int window, first;              // a row at p sees j <= p with j > p - window (0: all) or j < first
+  int f32, tiled;                 // 32-bit rows; the tensor-core form
+  int unit_tokens, key_tile;      // most tokens of a unit, keys of a tile
+  int max_blocks, max_units, max_cells, grid;
+} ds41_ragged_pass;
+int ds41_ragged_describe(const ds41_ragged_pass* pass, const int* slots, const int* news, const int* lengths, int n,
+                         const int* page_table, int n_slots, int max_pages, int n_pages, void* stream);
+
+// RMS norm of every head of q and k (weights [dim], or [heads][dim] with a stride; NULL: none), rotation of the first rot_dim values by
+// row_pos * freq, q as a matrix, keys and values into the pool's rows row_place.  Rows with a negative place are left as they are.
+typedef struct ds41_ragged_heads_args {
+  ds41_proj q, k, v;              // heads * dim, kv_heads * dim, kv_heads * vdim columns
+  const float* q_norm;
+  const float* k_norm;
+  const float* freq;              // [rot_dim / 2]
+  const int* row_pos;
+  const int* row_place;
+  void* q_out;                    // [rows][ld_q]
+  void* pool;                     // [pool_rows][kv_heads * (dim + vdim)]
+  long long ld_q;
+  float eps;
+  int q_norm_stride, k_norm_stride;   // values between two heads' weights (0: shared)
+  int width;                      // values of a head in its mean square (the rest is padding)
+  int rows, heads, kv_heads, dim, vdim, rot_dim, pool_rows, f32;
+} ds41_ragged_heads_args;
+int ds41_ragged_heads(const ds41_ragged_heads_args* args, void* stream);
+
+// Attention of a described pass's rows: [rows][heads][vdim], divided by the sums (with exp(sink), if any) times sigmoid(gate).  Rows
+// without a slot become zeros, rows behind the last request's are left as they are.
+typedef struct ds41_ragged_attend_args {
+  const void* q;                  // row r, head h at r * q_row + h * q_head
+  const void* pool;
+  const int* page_table;
+  void* out;                      // row r, head h at r * out_row + h * vdim
+  const float* gate;              // [rows][gate_row] or NULL
+  const float* sink;              // [heads] or NULL
+  long long q_row, q_head, out_row, gate_row;
+  float scale;
+  int q_rows, max_pages, n_pages;
+} ds41_ragged_attend_args;
+int ds41_ragged_attend(const ds41_ragged_attend_args* args, const ds41_ragged_pass* pass, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,626 @@
+// Ragged passes: several requests with any number of new tokens each over a paged cache.
+//
+//  ragged_describe : positions, slots and cache rows of all new tokens from the requests' lengths, and how the attention's work is
+//                    divided; nothing of it comes to the host, so that a captured pass follows its requests
+//  ragged_heads    : RMS norm of every query and key head, rotation, queries as a matrix, keys and values into their cache rows
+//  ragged_simple   : attention of a described pass for every type and size (ragged_attend.cu: bf16 on tcgen05)
+#include <algorithm>
+#include <atomic>
+#include <climits>
+
+#include "ds41_ragged.cuh"
+#include "ds41_tma.h"
+
+namespace ds41 {
+
+constexpr int kDescribeThreads = 1024;
+constexpr int kMostRequests = 4096, kMostBlocks = 12288;
+constexpr int kCandidates = 16, kBins = 256;
+
+struct DescribeArgs {
+  const int *slots, *news, *lengths, *page_table;
+  int n, n_slots, max_pages, n_pages;
+};
+
+// Sum of the block's values before this thread's, and of all of them; two numbers of 32 bits in one.
+__device__ __forceinline__ unsigned long long block_scan(unsigned long long v, unsigned long long* warps, unsigned long long& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  unsigned long long x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const unsigned long long y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) warps[warp] = x;
+  __syncthreads();
+  unsigned long long w = warps[lane];                  // as many warps as lanes
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const unsigned long long y = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += y;
+  }
+  total = __shfl_sync(0xffffffffu, w, 31);
+  const unsigned long long before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+  return (warp ? before : 0) + x - v;
+}
+
+// Last entry of an ascending list that is not above x; list[0] <= x.
+__device__ __forceinline__ int find_last(const int* list, int n, int x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (list[mid] <= x) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ void bad_argument(int* status, int where, int detail) {
+  if (atomicCAS(status, kStatusOk, kStatusBadArgument) == kStatusOk) {
+    status[1] = where;
+    status[2] = static_cast<int>(blockIdx.x);
+    status[3] = detail;
+  }
+}
+
+__global__ void __launch_bounds__(kDescribeThreads) ragged_describe_kernel(const ds41_ragged_pass p, const DescribeArgs a) {
+  extern __shared__ int rd_smem[];
+  __shared__ unsigned long long warps[32];
+  __shared__ int units_of[kCandidates], cells_of[kCandidates], bins[kBins], bin_sums[kBins / 32];
+  __shared__ unsigned long long cost_of[kCandidates];
+  __shared__ int longest, chosen;
+  const int tid = threadIdx.x, lane = tid & 31, n = a.n, G = p.kv_heads, group = p.heads / p.kv_heads;
+  int* row_first = rd_smem;             // [n] of every request: its first row, its first block, tokens, first token's position, slot
+  int* block_first = row_first + n;
+  int* tokens = block_first + n;
+  int* begin = tokens + n;
+  int* slot_of = begin + n;
+  int* tiles = slot_of + n;             // [blocks] key tiles; then the number of the block's first unit
+  int* cells = tiles + p.max_blocks;    // [blocks] first cell
+  pdl_launch_dependents();
+  pdl_wait();
+  unsigned long long base = 0;
+  for (int i0 = 0; i0 < n; i0 += kDescribeThreads) {
+    const int i = i0 + tid;
+    int slot = -1, count = 0, length = 0;
+    if (i < n) {
+      slot = a.slots[i];
+      count = a.news[i];
+      length = a.lengths[i];
+      if (count < 0 || length < count || slot >= a.n_slots || (slot >= 0 && length > 1ll * a.max_pages * p.page_tokens)) {
+        if (blockIdx.x == 0) bad_argument(p.status, 500, i);
+        slot = -1;
+      }
+    }
+    const int wanted = max(count, 0), most = min(wanted, p.rows);
+    unsigned long long total;
+    const unsigned long long at = base + block_scan(static_cast<unsigned long long>(most) << 32, warps, total);
+    base += total;
+    // rows beyond the pass's are left out
+    const int first = static_cast<int>(min(at >> 32, static_cast<unsigned long long>(p.rows))), kept = min(most, p.rows - first);
+    if (kept < wanted && blockIdx.x == 0) bad_argument(p.status, 501, i);
+    if (i < n) {
+      row_first[i] = first;
+      tokens[i] = kept;
+      begin[i] = max(0, length - wanted);
+      slot_of[i] = slot;
+    }
+  }
+  const int rows = static_cast<int>(min(base >> 32, static_cast<unsigned long long>(p.rows)));
+  __syncthreads();
+
+  if (blockIdx.x > 0) {
+    const int r = (blockIdx.x - 1) * kDescribeThreads + tid;
+    if (r < p.rows) {
+      int pos = 0, slot = -1, place = -1;
+      if (r < rows) {
+        const int i = find_last(row_first, n, r);
+        pos = begin[i] + r - row_first[i];
+        slot = slot_of[i];
+        if (slot >= 0) {
+          const int pg = pos / p.page_tokens, id = a.page_table[1ll * slot * a.max_pages + pg];
+          if (static_cast<unsigned>(id) < static_cast<unsigned>(a.n_pages)) place = id * p.page_tokens + (pos - pg * p.page_tokens);
+        }
+      }
+      p.row_pos[r] = pos;
+      p.row_slot[r] = slot;
+      p.row_place[r] = place;
+    }
+    // counters of calls that gave up
+    for (int i = r; i < 2 * p.max_blocks * G; i += (gridDim.x - 1) * kDescribeThreads) p.counters[i] = 0;
+    return;
+  }
+
+  // blocks
+  unsigned long long blocks64 = 0;
+  for (int i0 = 0; i0 < n; i0 += kDescribeThreads) {
+    const int i = i0 + tid;
+    const int mine = i < n ? (tokens[i] + p.unit_tokens - 1) / p.unit_tokens : 0;
+    unsigned long long total;
+    const unsigned long long at = blocks64 + block_scan(mine, warps, total);
+    blocks64 += total;
+    if (i < n) block_first[i] = static_cast<int>(at);
+  }
+  const int blocks = min(static_cast<int>(blocks64), p.max_blocks);
+  if (tid < kCandidates) units_of[tid] = cells_of[tid] = 0, cost_of[tid] = 0;
+  if (tid < kBins) bins[tid] = 0;
+  if (tid == 0) longest = 0;
+  __syncthreads();
+  const int align = min(p.page_tokens, p.key_tile);
+  auto block_of = [&](int b, int& i, int& t0, int& count, int& pos0) {
+    i = find_last(block_first, n, b);
+    t0 = (b - block_first[i]) * p.unit_tokens;
+    count = min(p.unit_tokens, tokens[i] - t0);
+    pos0 = begin[i] + t0;
+  };
+  int most = 0;
+  for (int b = tid; b < blocks; b += kDescribeThreads) {
+    int i, t0, count, pos0, k = 0;
+    block_of(b, i, t0, count, pos0);
+    if (slot_of[i] >= 0) {
+      const RaggedWalk w = ragged_walk(pos0, pos0 + count - 1, p.window, p.first, align);
+      k = (w.places + p.key_tile - 1) / p.key_tile;
+    }
+    tiles[b] = k;
+    cells[b] = count * group;
+    most = max(most, k);
+  }
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (lane == 0) atomicMax(&longest, most);
+  __syncthreads();
+  const int longest_walk = max(longest, 1);
+  // How long a piece may be.  A CTA's time is its pieces' tiles, two tiles' time for what a piece begins and ends with, and for a part
+  // of `unit_tokens` tokens that has to be joined one more to write and one to read; the join comes last.
+  auto limit = [&](int k) {
+    constexpr int kDivide[kCandidates] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256};
+    int d = 1;
+#pragma unroll
+    for (int j = 0; j < kCandidates; ++j) d = k == j ? kDivide[j] : d;
+    return (longest_walk + d - 1) / d;
+  };
+  const int full = p.unit_tokens * group;
+#pragma unroll 1
+  for (int k = 0; k < kCandidates; ++k) {
+    const int most_tiles = limit(k);
+    int units = 0, parts = 0;
+    unsigned long long cost = 0;                        // whole numbers: the choice is the same every time
+    for (int b = tid; b < blocks; b += kDescribeThreads) {
+      const int pieces = max(1, (tiles[b] + most_tiles - 1) / most_tiles);
+      units += pieces;
+      cost += 4ull * tiles[b] + 8 * pieces;
+      if (pieces > 1) {
+        parts += min(pieces * cells[b], 1 << 20);
+        cost += 8 * pieces * cells[b] / full;
+      }
+    }
+    units = __reduce_add_sync(0xffffffffu, units);
+    parts = __reduce_add_sync(0xffffffffu, min(parts, 1 << 22));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) cost += __shfl_xor_sync(0xffffffffu, cost, o);
+    if (lane == 0 && units > 0) {
+      atomicAdd(&units_of[k], units);
+      atomicAdd(&cells_of[k], min(parts, 1 << 25));
+      atomicAdd(&cost_of[k], cost);
+    }
+  }
+  __syncthreads();
+  if (tid < 32) {
+    float time = INFINITY;
+    if (lane < kCandidates && (lane == 0 || (1ll * units_of[lane] * G <= p.max_units && 1ll * cells_of[lane] * G <= p.max_cells))) {
+      const float units = static_cast<float>(units_of[lane]) * G, turns = ceilf(units / p.grid);
+      const float cost = static_cast<float>(cost_of[lane]) * 0.25f * G;
+      time = fmaxf(limit(lane) + 2.f, turns * cost / fmaxf(units, 1.f)) + (cells_of[lane] > 0 ? 3.f : 0.f);
+    }
+    float best = time;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) best = fminf(best, __shfl_xor_sync(0xffffffffu, best, o));
+    const unsigned who = __ballot_sync(0xffffffffu, time == best);
+    if (lane == 0) chosen = limit(__ffs(who) - 1);
+  }
+  __syncthreads();
+  const int most_tiles = chosen;
+  // the longest pieces first
+  auto bin_of = [&](int t) { return kBins - 1 - static_cast<int>(static_cast<long long>(t) * (kBins - 1) / most_tiles); };
+  unsigned long long sums = 0;
+  for (int b0 = 0; b0 < blocks; b0 += kDescribeThreads) {
+    const int b = b0 + tid;
+    int pieces = 0, parts = 0, k = 0;
+    if (b < blocks) {
+      k = tiles[b];
+      pieces = max(1, (k + most_tiles - 1) / most_tiles);
+      parts = pieces > 1 ? pieces * cells[b] * G : 0;
+      const int more = k % pieces;                     // pieces of one tile more than the others
+      if (more) atomicAdd(&bins[bin_of(k / pieces + 1)], more * G);
+      atomicAdd(&bins[bin_of(k / pieces)], (pieces - more) * G);
+    }
+    unsigned long long total;
+    const unsigned long long at = sums + block_scan(static_cast<unsigned long long>(pieces * G) << 32 | parts, warps, total);
+    sums += total;
+    if (b < blocks) {
+      tiles[b] = static_cast<int>(at >> 32);           // of the list by blocks: the block's first
+      cells[b] = static_cast<int>(at & 0xffffffffu);
+    }
+  }
+  const int units = static_cast<int>(sums >> 32);
+  __syncthreads();
+  // where a bin's units begin
+  int count = tid < kBins ? bins[tid] : 0, upto = count;
+  if (tid < kBins) {
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int y = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += y;
+    }
+    if (lane == 31) bin_sums[tid >> 5] = upto;
+  }
+  __syncthreads();
+  if (tid < kBins) {
+    int before = 0;
+    for (int w = 0; w < (tid >> 5); ++w) before += bin_sums[w];
+    bins[tid] = before + upto - count;
+  }
+  __syncthreads();
+  for (int u = tid; u < units; u += kDescribeThreads) {
+    const int b = find_last(tiles, blocks, u);
+    int i, t0, tk, pos0;
+    block_of(b, i, t0, tk, pos0);
+    int k = 0;
+    if (slot_of[i] >= 0) {
+      const RaggedWalk w = ragged_walk(pos0, pos0 + tk - 1, p.window, p.first, align);
+      k = (w.places + p.key_tile - 1) / p.key_tile;
+    }
+    const int pieces = max(1, (k + most_tiles - 1) / most_tiles), x = u - tiles[b], head = x / pieces, piece = x - head * pieces;
+    const int least = k / pieces, more = k - least * pieces;
+    const int mine = least + (piece < more), tile0 = piece * least + min(piece, more);
+    const int step = tk * group;
+    const int at = atomicAdd(&bins[bin_of(mine)], 1);
+    int4* out = reinterpret_cast<int4*>(p.units + 1ll * at * kRaggedInts);
+    out[0] = make_int4(slot_of[i], row_first[i] + t0, tk, pos0);
+    out[1] = make_int4(head, tile0, mine, piece);
+    out[2] = make_int4(pieces, cells[b] + head * pieces * step, 2 * (b * G + head), step);
+  }
+  if (tid == 0) {
+    p.header[0] = units;
+    p.header[1] = rows;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------- heads
+constexpr int kHeadsThreads = 256;
+
+// Cosine and sine of pos * freq.  The product has up to 31 + 24 bits: it is formed, and brought into half a turn, in 64.
+__device__ __forceinline__ float2 turn_at(int pos, float freq) {
+  const double x = static_cast<double>(pos) * static_cast<double>(freq);
+  const double k = rint(x * 0.15915494309189535);
+  float s, c;
+  sincosf(static_cast<float>(fma(-k, 6.283185307179586, x)), &s, &c);
+  return make_float2(c, s);
+}
+
+// Any sizes: one block per row, whose heads stay in shared memory between the norm and the rotation.
+template <typename T>
+__global__ void __launch_bounds__(kHeadsThreads) ragged_heads_kernel(const ds41_ragged_heads_args p) {
+  extern __shared__ __align__(16) float rh_row[];       // [(heads + kv_heads) * dim], then [rot_dim / 2] turns
+  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, half = p.rot_dim / 2;
+  const int H = p.heads, G = p.kv_heads, D = p.dim, V = p.vdim;
+  float2* turns = reinterpret_cast<float2*>(rh_row + (H + G) * D);
+  pdl_launch_dependents();
+  pdl_wait();
+  const int place = p.row_place[r], pos = p.row_pos[r];
+  if (place < 0 || place >= p.pool_rows) return;
+  for (int i = tid; i < half; i += kHeadsThreads) turns[i] = turn_at(pos, p.freq[i]);
+  __syncthreads();
+  T* row = static_cast<T*>(p.pool) + 1ll * place * (G * (D + V));
+  T* q = static_cast<T*>(p.q_out) + r * p.ld_q;
+  for (int h = warp; h < H + G; h += kHeadsThreads / 32) {
+    const bool key = h >= H;
+    const int g = key ? h - H : h;
+    float* x = rh_row + h * D;
+    float sum = 0.f;
+    for (int d = lane; d < D; d += 32) {
+      const float v = proj_at(key ? p.k : p.q, r, g * D + d);
+      x[d] = v;
+      sum += v * v;
+    }
+    const float* w = key ? p.k_norm : p.q_norm;
+    const float f = w != nullptr ? 1.0f / sqrtf(warp_sum(sum) / p.width + p.eps) : 1.f;
+    if (w != nullptr) w += 1ll * g * (key ? p.k_norm_stride : p.q_norm_stride);
+    __syncwarp();
+    T* dst = key ? row + g * D : q + g * D;
+    for (int d = lane; d < D; d += 32) {
+      float v = x[d] * f * (w != nullptr ? w[d] : 1.f);
+      if (d < 2 * half) {
+        const int e = d < half ? d + half : d - half;
+        const float o = x[e] * f * (w != nullptr ? w[e] : 1.f);
+        const float2 t = turns[d < half ? d : e];
+        v = d < half ? v * t.x - o * t.y : v * t.x + o * t.y;
+      }
+      dst[d] = from_f32<T>(v);
+    }
+  }
+  for (int c = tid; c < G * V; c += kHeadsThreads) row[G * D + c] = from_f32<T>(proj_at(p.v, r, c));
+}
+
+// ---------------------------------------------------------------------------------------------------- attention, any type and size
+constexpr int kSimpleRows = 64, kSimpleKeyTile = 32, kRaggedThreads = 256;
+
+__device__ __forceinline__ float4 four_at(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 four_at(const __nv_bfloat16* p) {
+  const uint2 v = *reinterpret_cast<const uint2*>(p);
+  return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16),
+                     __uint_as_float(v.y & 0xffff0000u));
+}
+
+inline int ragged_simple_smem(const ds41_ragged_pass& p) {
+  const int ds = p.dim + 4;
+  return 4 * (kSimpleRows * ds + kSimpleKeyTile * ds + kSimpleKeyTile * p.vdim + kSimpleRows * (kSimpleKeyTile + 1) + 3 * kSimpleRows);
+}
+
+// A unit's (token, head) rows, 64 at a time, against its keys, 32 at a time, both through shared memory: scores of 2 x 4 a thread, four
+// threads to a row's softmax, and RPT rows x 4 columns of the result in a thread's registers.
+template <typename T, int RPT>
+__global__ void __launch_bounds__(kRaggedThreads) ragged_simple_kernel(const ds41_ragged_attend_args a, const ds41_ragged_pass p) {
+  extern __shared__ __align__(16) float rs_smem[];
+  __shared__ int flag;
+  const int D = p.dim, V = p.vdim, G = p.kv_heads, group = p.heads / G, ds = D + 4, nc = V / 4, row_len = G * (D + V);
+  float* qs = rs_smem;                                 // [64][ds]
+  float* ks = qs + kSimpleRows * ds;                   // [32][ds]
+  float* vs = ks + kSimpleKeyTile * ds;                // [32][V]
+  float* sc = vs + kSimpleKeyTile * V;                 // [64][33] scores, then weights
+  float* ms = sc + kSimpleRows * (kSimpleKeyTile + 1); // [64] maxima, sums, factors on what was summed before
+  float* ls = ms + kSimpleRows;
+  float* keep = ls + kSimpleRows;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int units = p.header[0];
+  const int align = min(p.page_tokens, p.key_tile);
+  const float scale = a.scale * kLog2E;
+  for (int it = blockIdx.x; it < units; it += gridDim.x) {
+    const RaggedUnit u = ragged_unit(p, it);
+    const int n = u.tokens * group;
+    if (u.slot < 0) {
+      for (int i = tid; i < n * nc; i += kRaggedThreads) {
+        const int r = i / nc, row = u.row0 + r / group, h = u.head * group + r % group;
+        store4(static_cast<T*>(a.out) + row * a.out_row + 1ll * h * V + 4 * (i - r * nc), make_float4(0.f, 0.f, 0.f, 0.f));
+      }
+      continue;
+    }
+    const RaggedWalk walk = ragged_walk(u.pos0, u.pos0 + u.tokens - 1, p.window, p.first, align);
+    const int v0 = u.tile0 * p.key_tile, v1 = min(walk.places, v0 + u.tiles * p.key_tile);
+    for (int r0 = 0; r0 < n; r0 += kSimpleRows) {
+      const int rows = min(kSimpleRows, n - r0);
+      __syncthreads();
+      for (int r = warp; r < kSimpleRows; r += kRaggedThreads / 32) {
+        const int row = u.row0 + (r0 + r) / group, h = u.head * group + (r0 + r) % group;
+        const T* q = static_cast<const T*>(a.q) + row * a.q_row + h * a.q_head;
+        for (int d = 4 * lane; d < D; d += 128)
+          *reinterpret_cast<float4*>(qs + r * ds + d) = r < rows ? four_at(q + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      if (tid < kSimpleRows) {
+        ms[tid] = -INFINITY;
+        ls[tid] = 0.f;
+      }
+      float4 acc[RPT];
+#pragma unroll
+      for (int i = 0; i < RPT; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      const int col = tid % nc, own = tid / nc * RPT;
+      for (int t0 = v0; t0 < v1; t0 += kSimpleKeyTile) {
+        __syncthreads();
+        for (int k = warp; k < kSimpleKeyTile; k += kRaggedThreads / 32) {
+          const int place = t0 + k, pos = place < walk.lead ? place : place + walk.shift, pg = pos / p.page_tokens;
+          // a key that some row sees; other places may hold anything
+          const bool seen = place < v1 && (pos < p.first || pos >= ragged_low(u.pos0, p.window));
+          const int id = seen && pg < a.max_pages ? a.page_table[1ll * u.slot * a.max_pages + pg] : -1;
+          const bool there = static_cast<unsigned>(id) < static_cast<unsigned>(a.n_pages);
+          const T* src = static_cast<const T*>(a.pool) + (1ll * id * p.page_tokens + (pos - pg * p.page_tokens)) * row_len;
+          for (int d = 4 * lane; d < D; d += 128)
+            *reinterpret_cast<float4*>(ks + k * ds + d) = there ? four_at(src + u.head * D + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int d = 4 * lane; d < V; d += 128)
+            *reinterpret_cast<float4*>(vs + k * V + d) =
+                there ? four_at(src + G * D + u.head * V + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        __syncthreads();
+        const int ty = tid >> 3, tx = tid & 7;
+        if (2 * ty < rows) {
+          float s[2][4] = {};
+          for (int d = 0; d < D; d += 4) {
+            const float4 q0 = *reinterpret_cast<const float4*>(qs + 2 * ty * ds + d);
+            const float4 q1 = *reinterpret_cast<const float4*>(qs + (2 * ty + 1) * ds + d);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float4 x = *reinterpret_cast<const float4*>(ks + (tx + 8 * k) * ds + d);
+              s[0][k] += q0.x * x.x + q0.y * x.y + q0.z * x.z + q0.w * x.w;
+              s[1][k] += q1.x * x.x + q1.y * x.y + q1.z * x.z + q1.w * x.w;
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sc[(2 * ty + j) * (kSimpleKeyTile + 1) + tx + 8 * k] = s[j][k] * scale;
+        }
+        __syncthreads();
+        {
+          const int r = tid >> 2, part = tid & 3, pos = u.pos0 + (r0 + r) / group, low = ragged_low(pos, p.window);
+          float* mine = sc + r * (kSimpleKeyTile + 1);
+          float v[8], top = -INFINITY;
+          bool bad = false;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int place = t0 + part + 4 * k, at = place < walk.lead ? place : place + walk.shift;
+            const bool seen = r < rows && place < v1 && at <= pos && (at >= low || at < p.first);
+            v[k] = seen ? mine[part + 4 * k] : -INFINITY;
+            bad |= v[k] != v[k];
+            top = fmaxf(top, v[k]);
+          }
+          if (bad) top = NAN;
+#pragma unroll
+          for (int o = 1; o < 4; o *= 2) {
+            const float y = __shfl_xor_sync(0xffffffffu, top, o);
+            top = top != top || y != y ? NAN : fmaxf(top, y);
+          }
+          const float m = ms[r];
+          const float m_new = top != top || m != m ? NAN : fmaxf(m, top), base = m_new == -INFINITY ? 0.f : m_new;
+          float sum = 0.f;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float w = exp2f(v[k] - base);
+            mine[part + 4 * k] = w;
+            sum += w;
+          }
+#pragma unroll
+          for (int o = 1; o < 4; o *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          __syncwarp();
+          if (part == 0) {
+            const float f = m == -INFINITY ? 0.f : exp2f(m - base);
+            ms[r] = m_new;
+            ls[r] = ls[r] * f + sum;
+            keep[r] = f;
+          }
+        }
+        __syncthreads();
+        if (own < rows) {
+#pragma unroll
+          for (int i = 0; i < RPT; ++i) {
+            const float f = keep[own + i];
+            acc[i].x *= f;
+            acc[i].y *= f;
+            acc[i].z *= f;
+            acc[i].w *= f;
+          }
+#pragma unroll 4
+          for (int k = 0; k < kSimpleKeyTile; ++k) {
+            const float4 v = *reinterpret_cast<const float4*>(vs + k * V + 4 * col);
+#pragma unroll
+            for (int i = 0; i < RPT; ++i) {
+              const float w = sc[(own + i) * (kSimpleKeyTile + 1) + k];
+              acc[i].x += w * v.x;
+              acc[i].y += w * v.y;
+              acc[i].z += w * v.z;
+              acc[i].w += w * v.w;
+            }
+          }
+        }
+      }
+      __syncthreads();
+      if (own < kSimpleRows) {
+#pragma unroll
+        for (int i = 0; i < RPT; ++i) {
+          const int r = own + i;
+          if (r >= rows) continue;
+          const float m = ms[r], l = ls[r];
+          const int row = u.row0 + (r0 + r) / group, h = u.head * group + (r0 + r) % group;
+          if (u.pieces > 1) {
+            const long long cell = 1ll * u.cell + 1ll * u.piece * u.step + r0 + r;
+            store4(p.part_o + cell * V + 4 * col, acc[i]);
+            if (col == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * cell) = make_float2(m, l);
+            continue;
+          }
+          const float sink = a.sink != nullptr ? a.sink[h] * kLog2E : -INFINITY;
+          const float whole = fmaxf(m, sink), base = whole == -INFINITY ? 0.f : whole;
+          const float w = m == -INFINITY ? 0.f : exp2f(m - base);
+          const float den = l * w + (a.sink != nullptr ? exp2f(sink - base) : 0.f);
+          float f = den != 0.f ? w / den : 0.f;
+          if (a.gate != nullptr) f *= sigmoid_f32(a.gate[row * a.gate_row + h]);
+          store4(static_cast<T*>(a.out) + row * a.out_row + 1ll * h * V + 4 * col,
+                 make_float4(acc[i].x * f, acc[i].y * f, acc[i].z * f, acc[i].w * f));
+        }
+      }
+    }
+    if (u.pieces > 1 && ragged_last(p.counters + u.counter, u.pieces, tid == 0, 1, kRaggedThreads, &flag))
+      ragged_join<T>(p, a, u, warp, n, kRaggedThreads / 32);
+  }
+}
+
+template <typename T, int RPT>
+cudaError_t launch_simple(const ds41_ragged_attend_args& a, const ds41_ragged_pass& p, cudaStream_t st) {
+  static std::atomic<unsigned long long> ready{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 64 || !(ready.load() >> dev & 1)) {
+    e = cudaFuncSetAttribute(ragged_simple_kernel<T, RPT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) ready.fetch_or(1ull << dev);
+  }
+  return launch_pdl(ragged_simple_kernel<T, RPT>, dim3(p.grid), dim3(kRaggedThreads), ragged_simple_smem(p), st, a, p);
+}
+
+template <typename T>
+cudaError_t launch_ragged_simple(const ds41_ragged_attend_args& a, const ds41_ragged_pass& p, cudaStream_t st) {
+  const int groups = kRaggedThreads / (p.vdim / 4), need = (kSimpleRows + groups - 1) / groups;
+  if (need <= 1) return launch_simple<T, 1>(a, p, st);
+  if (need <= 2) return launch_simple<T, 2>(a, p, st);
+  if (need <= 4) return launch_simple<T, 4>(a, p, st);
+  if (need <= 8) return launch_simple<T, 8>(a, p, st);
+  return launch_simple<T, 16>(a, p, st);
+}
+
+inline bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+inline bool ragged_pass_ok(const ds41_ragged_pass* p) {
+  if (p == nullptr || p->header == nullptr || p->row_pos == nullptr || p->row_slot == nullptr || p->row_place == nullptr ||
+      p->units == nullptr || p->counters == nullptr || p->part_o == nullptr || p->part_ml == nullptr || p->status == nullptr)
+    return false;
+  if (p->rows <= 0 || p->rows > 1 << 18 || p->requests <= 0 || p->requests > kMostRequests || p->heads <= 0 || p->kv_heads <= 0 ||
+      p->heads % p->kv_heads || p->heads / p->kv_heads > 1024 || p->dim <= 0 || p->dim > 256 || (p->dim & 15) || p->vdim <= 0 ||
+      p->vdim > 256 || (p->vdim & 15) || p->page_tokens <= 0 || p->window < 0 || p->first < 0 || p->unit_tokens <= 0 || p->grid <= 0)
+    return false;
+  return p->max_blocks >= p->rows / p->unit_tokens + std::min(p->requests, p->rows) && p->max_blocks <= kMostBlocks &&
+         p->max_units >= 1ll * p->max_blocks * p->kv_heads && p->max_units < 1 << 22 && p->max_cells > 0 && p->max_cells < 1 << 22 &&
+         aligned(p->units, 16) && aligned(p->part_o, 16) && aligned(p->part_ml, 8) && (p->tiled ? p->key_tile == 128 : p->key_tile == 32);
+}
+
+}  // namespace ds41
+
+using namespace ds41;
+
+extern "C" int ds41_ragged_describe(const ds41_ragged_pass* p, const int* slots, const int* news, const int* lengths, int n,
+                                    const int* page_table, int n_slots, int max_pages, int n_pages, void* stream) {
+  if (!ragged_pass_ok(p) || n < 0 || n > p->requests || n_slots <= 0 || max_pages <= 0 || n_pages <= 0 || page_table == nullptr ||
+      (n > 0 && (slots == nullptr || news == nullptr || lengths == nullptr)) || 1ll * n_pages * p->page_tokens > INT_MAX)
+    return cudaErrorInvalidValue;
+  const int smem = 4 * (5 * n + 2 * p->max_blocks);
+  static std::atomic<unsigned long long> ready{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 64 || !(ready.load() >> dev & 1)) {
+    e = cudaFuncSetAttribute(ragged_describe_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * (5 * kMostRequests + 2 * kMostBlocks));
+    if (e != cudaSuccess) return e;
+    if (dev < 64) ready.fetch_or(1ull << dev);
+  }
+  const DescribeArgs a{slots, news, lengths, page_table, n, n_slots, max_pages, n_pages};
+  const int grid = 1 + (p->rows + kDescribeThreads - 1) / kDescribeThreads;
+  return launch_pdl(ragged_describe_kernel, dim3(grid), dim3(kDescribeThreads), smem, static_cast<cudaStream_t>(stream), *p, a);
+}
+
+extern "C" int ds41_ragged_heads(const ds41_ragged_heads_args* a, void* stream) {
+  if (a == nullptr || a->rows <= 0 || a->heads <= 0 || a->kv_heads <= 0 || a->dim <= 0 || a->vdim <= 0 || a->dim > 1024 ||
+      a->heads > 4096 || a->kv_heads > 4096 || a->rot_dim < 0 || (a->rot_dim & 1) || a->rot_dim > a->dim || a->width <= 0 || a->width > a->dim ||
+      !proj_ok(a->q) || !proj_ok(a->k) || !proj_ok(a->v) || (a->rot_dim > 0 && a->freq == nullptr) || a->row_pos == nullptr ||
+      a->row_place == nullptr || a->q_out == nullptr || a->pool == nullptr || a->pool_rows <= 0 || a->ld_q < 1ll * a->heads * a->dim ||
+      a->q_norm_stride < 0 || a->k_norm_stride < 0 || (a->heads + a->kv_heads) * a->dim * 4 + a->rot_dim * 4 > 200 * 1024)
+    return cudaErrorInvalidValue;
+  const int smem = (a->heads + a->kv_heads) * a->dim * 4 + a->rot_dim * 4;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto kernel = a->f32 ? ragged_heads_kernel<float> : ragged_heads_kernel<__nv_bfloat16>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(kernel, dim3(a->rows), dim3(kHeadsThreads), smem, st, *a);
+}
+
+extern "C" int ds41_ragged_attend(const ds41_ragged_attend_args* a, const ds41_ragged_pass* p, void* stream) {
+  if (!ragged_pass_ok(p) || a == nullptr || a->q == nullptr || a->pool == nullptr || a->page_table == nullptr || a->out == nullptr ||
+      a->q_rows < p->rows || a->max_pages <= 0 || a->n_pages <= 0 || 1ll * a->n_pages * p->page_tokens > INT_MAX || !(a->scale > 0.f) ||
+      a->q_head < p->dim || a->q_row < 0 || a->out_row < 1ll * p->heads * p->vdim)
+    return cudaErrorInvalidValue;
+  const int size = p->f32 ? 4 : 2;
+  if (!aligned(a->q, 16) || !aligned(a->pool, 16) || !aligned(a->out, 16) || (a->q_row * size & 15) || (a->q_head * size & 15) ||
+      (a->out_row * size & 15))
+    return cudaErrorInvalidValue;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (p->tiled) return launch_ragged_tiled(*a, *p, st);
+  return p->f32 ? launch_ragged_simple<float>(*a, *p, st) : launch_ragged_simple<__nv_bfloat16>(*a, *p, st);
+}
