@@ -5,11 +5,12 @@
 // walk the same keys; a block of a few rows (decode) has them twice, and its two copies take the key tiles in turn.  Either way one
 // tile's softmax runs while the tensor core works on the other's products.
 //   warps 0-3, 4-7 : softmax of tile 0 / 1 (one thread per row), results
-//   warp 8, 11     : TMA producers: queries and keys / values, page by page, a lane per copy
-//   warp 9         : tcgen05.mma issue: S = Q K^T into TMEM, O += P V with P read from TMEM where it replaces its S
-//   warp 10        : zeros in place of values that no row of the unit sees: their weights are zeros, but they may hold anything
-// The running maximum is raised when it grew by more than 2^8 only, so the accumulated output is rarely rescaled.  P is rounded to bf16
-// as the operand of the second product; the sums take the unrounded weights.
+//   warp 8         : TMA producer: queries, keys and values, 128 positions at a time, page by page, a lane per copy
+//   warps 9, 10    : tcgen05.mma issue for tile 0 / 1: S = Q K^T into TMEM, O += P V with P read from TMEM where it replaces its S, the
+//                    first 96 keys' share while the others' weights are made
+//   warp 11        : zeros in place of values that no row of the unit sees: their weights are zeros, but they may hold anything
+// The running maximum is raised when it grew by more than 2^8 only, so the accumulated output is rarely rescaled, and a tile's weights
+// need not wait for its maximum.  P is rounded to bf16 as the operand of the second product; the sums take the unrounded weights.
 //
 // A CTA walks the units blockIdx.x, 2 * grid - 1 - blockIdx.x, ... of a list with the longest first; all roles but the softmax run ahead.
 #include <cuda.h>
@@ -23,8 +24,9 @@
 namespace ds41 {
 
 constexpr int kRtThreads = 384;
-constexpr int kRtTile = 128;                   // rows of a tile, keys of a tile
+constexpr int kRtTile = 128, kRtKeys = 128;    // rows of a tile, keys of a tile
 constexpr int kRtChunk = kRtTile * 128;        // bytes of 128 rows x 64 bf16 columns
+constexpr int kRtKeyChunk = kRtKeys * 128;     // of its keys
 constexpr int kRtStages = 4, kRtSlotRows = 64;
 
 struct TiledParams {
@@ -42,13 +44,29 @@ struct TiledShared {
   uint64_t q_full, q_free;                     // queries are there; the unit's last scores are done
   uint64_t k_full[kRtStages], k_empty[kRtStages], v_full[kRtStages], v_empty[kRtStages];
   uint64_t v_clean[kRtStages];                 // places that nobody sees are zeros
-  uint64_t s_full[2], p_full[2], o_full[2];    // per tile: S complete (and every earlier product); P written, O rescaled; O complete
+  // per tile:
+  uint64_t s_full[2];                          // S complete, and every product before it
+  uint64_t p_full[2][2];                       // P written, O rescaled: of the first 96 keys, of the others
+  uint64_t most_done[2];                       // the product with the former is complete
+  uint64_t o_full[2];                          // the unit's last product is complete
   uint64_t half_full, half_read[2];            // the second tile's half of a unit whose keys were taken in turn
   float2 half_ml[kRtSlotRows];
   uint32_t tmem;
   int flag[2];
+  int busy[4];                                 // per scheduler: one of its two softmax warps is at its exponentials
 };
 
+// Two products of 16 columns of K each (see umma4_ts).
+template <int BSTEP>
+__device__ __forceinline__ void umma2_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t.reg .b32 x;\n\t.reg .b64 y;\n\t"
+      "setp.eq.b32 q, 0, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, q;\n\t"
+      "add.s32 x, %1, 8;\n\tadd.s64 y, %2, %4;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %3, q;\n\t}"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "n"(BSTEP)
+      : "memory");
+}
 // What every role knows of a unit.
 struct TiledUnit {
   RaggedUnit u;
@@ -70,7 +88,7 @@ __device__ __forceinline__ TiledUnit tiled_unit(const TiledParams& t, int i) {
     x.n[1] = u.tiles / 2;
   } else {
     const int seen = u.pos0 + x.tok0 - x.walk.shift;                     // places up to tile 0's last row
-    x.n[0] = min(max((seen + kRtTile - 1) / kRtTile - u.tile0, 0), u.tiles);
+    x.n[0] = min(max((seen + kRtKeys - 1) / kRtKeys - u.tile0, 0), u.tiles);
     x.n[1] = u.tokens > x.tok0 ? u.tiles : 0;
   }
   return x;
@@ -82,14 +100,52 @@ __device__ __forceinline__ int unit_at(int turn) {
          (turn & 1 ? static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x));
 }
 
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+__device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
+}
+__device__ __forceinline__ float largest(const uint32_t (&v)[32]) {
+  auto f = [&](int k) { return __uint_as_float(v[k]); };
+  float x[2];
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    x[c] = max3(f(c), f(2 + c), f(4 + c));
+#pragma unroll
+    for (int k = 6; k + 2 < 32; k += 4) x[c] = max3(x[c], f(k + c), f(k + 2 + c));
+  }
+  return fmaxf(max3(x[0], f(30), f(31)), x[1]);
+}
+// The wait as something that the loaded registers depend on.
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                 "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),
+                 "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
+                 "+r"(r[28]), "+r"(r[29])
+               :: "memory");
+  asm volatile("" : "+r"(r[30]), "+r"(r[31])::"memory");
+}
+__device__ __forceinline__ void mbar_arrive_if(bool issue, uint64_t* bar) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t@q mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}"
+               ::"r"(smem_u32(bar)), "r"(static_cast<uint32_t>(issue))
+               : "memory");
 }
 // The lowest n bits.
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
 
+// A scheduler's two softmax warps take turns at the exponentials: at the same time they would take each as long as both after one another,
+// and the tensor core would have both tiles' products at once, and none afterwards.  Who has waited long enough goes on without.
+__device__ __forceinline__ void take_turn(int* busy, int lane) {
+  if (lane == 0)
+    for (int i = 0; i < 1024 && atomicCAS(busy, 0, 1) != 0; ++i) {
+    }
+  __syncwarp();
+}
+__device__ __forceinline__ void end_turn(int* busy, int lane) {
+  __syncwarp();
+  if (lane == 0) atomicExch(busy, 0);
+}
 // All lanes, or one thread by itself.
 #define WARP_WAIT(bar, parity, where) (__all_sync(0xffffffffu, mbar_wait(bar, parity, t.p.status, where)) != 0)
 
@@ -98,7 +154,7 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
                     const __grid_constant__ TiledParams t) {
   extern __shared__ uint8_t rt_raw[];
   uint8_t* smem = rt_raw + ((1024u - (smem_u32(rt_raw) & 1023u)) & 1023u);
-  const int q_bytes = t.kd * kRtChunk, k_bytes = q_bytes, v_bytes = t.vc * kRtChunk;
+  const int q_bytes = t.kd * kRtChunk, k_bytes = t.kd * kRtKeyChunk, v_bytes = t.vc * kRtKeyChunk;
   uint8_t* s_q = smem;                                   // two tiles
   uint8_t* s_k = s_q + 2 * q_bytes;
   uint8_t* s_v = s_k + t.k_stages * k_bytes;
@@ -109,18 +165,21 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
     mbar_init(&sh.q_full, 1);
-    mbar_init(&sh.q_free, 1);
+    mbar_init(&sh.q_free, 2);                            // the products of either tile
     for (int i = 0; i < kRtStages; ++i) {
       mbar_init(&sh.k_full[i], 1);
-      mbar_init(&sh.k_empty[i], 1);
+      mbar_init(&sh.k_empty[i], 2);                      // the products of either tile, or that they do not take it
       mbar_init(&sh.v_full[i], 1);
       mbar_init(&sh.v_clean[i], 1);
-      mbar_init(&sh.v_empty[i], 2);                      // the products, the cleaner
+      mbar_init(&sh.v_empty[i], 3);                      // the same, and the cleaner
     }
     mbar_init(&sh.half_full, 4);
+    for (int i = 0; i < 4; ++i) sh.busy[i] = 0;
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.s_full[i], 1);
-      mbar_init(&sh.p_full[i], 4);
+      mbar_init(&sh.p_full[i][0], 4);
+      mbar_init(&sh.p_full[i][1], 4);
+      mbar_init(&sh.most_done[i], 1);
       mbar_init(&sh.o_full[i], 1);
       mbar_init(&sh.half_read[i], 4);
     }
@@ -139,154 +198,213 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
   pdl_wait();
   const int units = t.p.header[0];
 
-  if (warp == 8 || warp == 11) {
-    const bool values = warp == 11;
-    const int chunks = values ? t.vc : t.kd, stages = values ? t.v_stages : t.k_stages, bytes = values ? v_bytes : k_bytes;
-    uint8_t* ring = values ? s_v : s_k;
-    uint64_t *full = values ? sh.v_full : sh.k_full, *empty = values ? sh.v_empty : sh.k_empty;
-    const int box = lane / chunks, chunk = lane - box * chunks;          // this lane's copy of a tile
-    const bool copies = box < kRtTile / t.box;
-    uint8_t* const dst = ring + chunk * kRtChunk + box * t.box * 128;
-    int count = 0, stage = 0, done = 0, halves = 0;
-    uint32_t phase = 1;
-    bool ok = true;
+  if (warp == 8) {
+    // this lane's copies of a tile of keys and of one of values: some rows of one chunk of columns
+    const int boxes = kRtKeys / t.box, k_box = lane / t.kd, k_chunk = lane - k_box * t.kd, v_box = lane / t.vc, v_chunk = lane - v_box * t.vc;
+    const bool k_copies = k_box < boxes, v_copies = v_box < boxes;
+    uint8_t *const k_to = s_k + k_chunk * kRtKeyChunk + k_box * t.box * 128, *const v_to = s_v + v_chunk * kRtKeyChunk + v_box * t.box * 128;
+    int k_count = 0, v_count = 0, ks = 0, vs = 0, done = 0, halves = 0, v_row = 0, v_col = 0;
+    uint32_t k_phase = 1, v_phase = 1;
+    bool ok = true, behind = false;
+    // values follow the keys one tile behind: by then their place is free as well
+    auto values = [&]() {
+      ok = WARP_WAIT(&sh.v_empty[vs], v_phase, 603);
+      if (!ok) return;
+      if (lane == 0) mbar_expect_tx(&sh.v_full[vs], v_bytes);
+      __syncwarp();
+      if (v_copies) tma_load_3d(v_to + vs * v_bytes, &pool, &sh.v_full[vs], v_col, v_row, 0);
+      ++v_count;
+      if (++vs == t.v_stages) {
+        vs = 0;
+        v_phase ^= 1;
+      }
+    };
     for (int turn = 0; unit_at(turn) < units && ok; ++turn) {
       const TiledUnit x = tiled_unit(t, unit_at(turn));
-      if (x.u.tiles == 0) continue;
-      auto locate = [&](int s) {
-        const int place = (x.u.tile0 + s) * kRtTile + box * t.box, pos = place < x.walk.lead ? place : place + x.walk.shift;
+      const int n = x.u.tiles;
+      auto locate = [&](int s, int box, bool copies) {
+        const int place = (x.u.tile0 + s) * kRtKeys + box * t.box, pos = place < x.walk.lead ? place : place + x.walk.shift;
         const int pg = pos / t.p.page_tokens;
         const int id = copies && place < x.walk.places && pg < t.a.max_pages
                            ? __ldg(t.a.page_table + 1ll * x.u.slot * t.a.max_pages + pg) : -1;
         return static_cast<unsigned>(id) < static_cast<unsigned>(t.a.n_pages) ? id * t.p.page_tokens + (pos - pg * t.p.page_tokens)
                                                                               : t.hidden_row;
       };
-      int row = locate(0);
-      if (!values) {
-        ok = WARP_WAIT(&sh.q_free, (done & 1) ^ 1, 600);
-        // the second tile's place holds halves of units that went in turns
-        for (int h = max(0, halves - 2); h < halves && ok && !x.turns; ++h) ok = WARP_WAIT(&sh.half_read[h & 1], (h >> 1) & 1, 601);
-        if (!ok) break;
-        const bool second = !x.turns && x.u.tokens > x.tok0;
-        if (lane == 0) mbar_expect_tx(&sh.q_full, (second ? 2 : 1) * t.kd * t.per_tile * t.group * 128);
-        __syncwarp();
-        if (lane < (second ? 2 : 1) * t.kd) {
-          const int k = lane / t.kd, c = lane - k * t.kd;
-          tma_load_3d(s_q + k * q_bytes + c * kRtChunk, &queries, &sh.q_full, 64 * c, x.u.head * t.group, x.u.row0 + k * x.tok0);
+      int k_next = n > 0 ? locate(0, k_box, k_copies) : 0, v_next = n > 0 ? locate(0, v_box, v_copies) : 0;
+      for (int s = 0; s < n; ++s) {
+        const int k_row = k_next, v_later = v_next;
+        if (s + 1 < n) {
+          k_next = locate(s + 1, k_box, k_copies);
+          v_next = locate(s + 1, v_box, v_copies);
         }
-        ++done;
-        if (x.turns && x.u.tiles > 1) ++halves;
-      }
-      const int col = (values ? t.p.kv_heads * dp + x.u.head * vp : x.u.head * dp) + 64 * chunk;
-      for (int s = 0; s < x.u.tiles; ++s) {
-        const int at = row;
-        if (s + 1 < x.u.tiles) row = locate(s + 1);
-        ok = WARP_WAIT(&empty[stage], phase, values ? 603 : 602);
+        ok = WARP_WAIT(&sh.k_empty[ks], k_phase, 602);
         if (!ok) break;
-        if (lane == 0) mbar_expect_tx(&full[stage], bytes);
+        if (lane == 0) mbar_expect_tx(&sh.k_full[ks], k_bytes);
         __syncwarp();
-        if (copies) tma_load_3d(dst + stage * bytes, &pool, &full[stage], col, at, 0);
-        ++count;
-        if (++stage == stages) {
-          stage = 0;
-          phase ^= 1;
+        if (k_copies) tma_load_3d(k_to + ks * k_bytes, &pool, &sh.k_full[ks], x.u.head * dp + 64 * k_chunk, k_row, 0);
+        ++k_count;
+        if (++ks == t.k_stages) {
+          ks = 0;
+          k_phase ^= 1;
+        }
+        if (behind) values();
+        if (!ok) break;
+        behind = true;
+        v_row = v_later;
+        v_col = t.p.kv_heads * dp + x.u.head * vp + 64 * v_chunk;
+        // queries behind as many key tiles as there are places for: those do not wait for the last unit's queries
+        if (s + 1 == min(n, t.k_stages)) {
+          ok = WARP_WAIT(&sh.q_free, (done & 1) ^ 1, 600);
+          // the second tile's place holds halves of units that went in turns
+          for (int h = max(0, halves - 2); h < halves && ok && !x.turns; ++h) ok = WARP_WAIT(&sh.half_read[h & 1], (h >> 1) & 1, 601);
+          if (!ok) break;
+          const bool second = !x.turns && x.u.tokens > x.tok0;
+          if (lane == 0) mbar_expect_tx(&sh.q_full, (second ? 2 : 1) * t.kd * t.per_tile * t.group * 128);
+          __syncwarp();
+          if (lane < (second ? 2 : 1) * t.kd) {
+            const int k = lane / t.kd, c = lane - k * t.kd;
+            tma_load_3d(s_q + k * q_bytes + c * kRtChunk, &queries, &sh.q_full, 64 * c, x.u.head * t.group, x.u.row0 + k * x.tok0);
+          }
+          ++done;
+          if (x.turns && n > 1) ++halves;
         }
       }
     }
+    if (ok && behind) values();
     if (!ok && lane == 0) {                              // something gave up: the copies under way land before the memory goes away
       auto drain = [](uint64_t* bar, uint32_t parity) {
         for (int i = 0; i < (1 << 18) && !mbar_test_wait(bar, parity); ++i) {
         }
       };
-      if (!values && done > 0) drain(&sh.q_full, (done - 1) & 1);
-      for (int b = max(0, count - stages); b < count; ++b) drain(&full[b % stages], (b / stages) & 1);
+      if (done > 0) drain(&sh.q_full, (done - 1) & 1);
+      for (int b = max(0, k_count - t.k_stages); b < k_count; ++b) drain(&sh.k_full[b % t.k_stages], (b / t.k_stages) & 1);
+      for (int b = max(0, v_count - t.v_stages); b < v_count; ++b) drain(&sh.v_full[b % t.v_stages], (b / t.v_stages) & 1);
     }
-  } else if (warp == 9) {
+  } else if (warp == 9 || warp == 10) {
+    // one thread: votes and the like between two products cost as much as the products
     if (elect_one()) {
-      const uint32_t idesc_s = umma_idesc(kRtTile, kRtTile, 1u, 1u), idesc_pv = umma_idesc_bmn(kRtTile, vp, 1u, 1u);
+      const int i = warp - 9;
+      const uint32_t idesc_s = umma_idesc(kRtTile, kRtKeys, 1u, 1u), idesc_pv = umma_idesc_bmn(kRtTile, vp, 1u, 1u);
       const uint64_t q_desc = umma_desc_sw128(smem_u32(s_q)), k_desc = umma_desc_sw128(smem_u32(s_k));
-      const uint64_t v_desc = umma_desc_sw128_mn(smem_u32(s_v), kRtChunk, 1024);
+      const uint64_t v_desc = umma_desc_sw128_mn(smem_u32(s_v), kRtKeyChunk, 1024);
+      const uint64_t k_step = k_bytes / 16, v_step = v_bytes / 16;
       const int whole = dp / 64, rest = dp / 16 - 4 * whole;
-      int begun = 0, count = 0, products[2] = {0, 0};     // units, key tiles, products of either tile
+      const uint32_t o_t = tmem + 256 + i * 128;
+      int begun = 0, done = 0;                           // units, tiles
+      int ks = 0, vs = 0;                                // places of the next keys and values, and their phases
+      uint32_t k_phase = 0, v_phase = 0;
       bool ok = true;
+      auto next_k = [&]() {
+        if (++ks == t.k_stages) {
+          ks = 0;
+          k_phase ^= 1;
+        }
+      };
+      auto next_v = [&]() {
+        if (++vs == t.v_stages) {
+          vs = 0;
+          v_phase ^= 1;
+        }
+      };
+      // tiles of the other one's, up to `upto`: every place of the rings is watched, or its phases could be mistaken
+      auto skip_k = [&](int& at, int upto) {
+        for (; at < upto && ok; ++at) {
+          ok = mbar_wait(&sh.k_full[ks], k_phase, t.p.status, 610);
+          if (ok) mbar_arrive(&sh.k_empty[ks]);
+          next_k();
+        }
+      };
+      auto skip_v = [&](int& at, int upto) {
+        for (; at < upto && ok; ++at) {
+          ok = mbar_wait(&sh.v_full[vs], v_phase, t.p.status, 611);
+          if (ok) mbar_arrive(&sh.v_empty[vs]);
+          next_v();
+        }
+      };
       for (int turn = 0; unit_at(turn) < units && ok; ++turn) {
         const TiledUnit x = tiled_unit(t, unit_at(turn));
-        const int n = x.u.tiles, ahead = x.turns ? 2 : 1;
-        if (n == 0) continue;
+        const int n = x.n[i], first = x.turns ? i : 0, step = x.turns ? 2 : 1;
+        if (x.u.tiles == 0) continue;
         const int low = ragged_low(x.u.pos0, t.p.window) - x.walk.shift;
-        auto takes = [&](int i, int s) { return x.turns ? s < n && (s & 1) == i : s < x.n[i]; };
-        auto scores = [&](int i, int s) {                // the tile's keys have landed
-          uint64_t a = q_desc + (x.turns ? 0u : static_cast<uint64_t>(i * q_bytes / 16));
-          uint64_t b = k_desc + static_cast<uint64_t>((count + s) % t.k_stages * (k_bytes / 16));
+        const uint64_t q = q_desc + (i && !x.turns ? static_cast<uint64_t>(q_bytes / 16) : 0u);
+        const uint32_t s_t = tmem + i * 128;
+        int k_at = 0, v_at = 0;
+        auto keys = [&](int j) {                         // of its tile j
+          skip_k(k_at, first + j * step);
+          if (ok) ok = mbar_wait(&sh.k_full[ks], k_phase, t.p.status, 612);
+        };
+        auto scores = [&](int j) {
+          uint64_t a = q, b = k_desc + ks * k_step;
 #pragma unroll 1
-          for (int c = 0; c < whole; ++c, a += kRtChunk / 16, b += kRtChunk / 16) umma4_ss<2, 2>(tmem + i * 128, a, b, idesc_s, c);
+          for (int c = 0; c < whole; ++c, a += kRtChunk / 16, b += kRtKeyChunk / 16) umma4_ss<2, 2>(s_t, a, b, idesc_s, c);
 #pragma unroll 1
-          for (int k = 0; k < rest; ++k) umma_bf16(tmem + i * 128, a + 2 * k, b + 2 * k, idesc_s, whole > 0 || k > 0);
+          for (int k = 0; k < rest; ++k) umma_bf16(s_t, a + 2 * k, b + 2 * k, idesc_s, whole > 0 || k > 0);
           tc_commit(&sh.s_full[i]);
+          tc_commit(&sh.k_empty[ks]);
+          ++k_at;
+          next_k();
+          if (j == n - 1) tc_commit(&sh.q_free);
         };
-        auto keys = [&](int s) {
-          const int at = count + s;
-          if (!mbar_wait(&sh.k_full[at % t.k_stages], (at / t.k_stages) & 1, t.p.status, 610)) return false;
-          tc_fence_after();
-          return true;
-        };
-        auto keys_read = [&](int s) {
-          tc_commit(&sh.k_empty[(count + s) % t.k_stages]);
-          if (s == n - 1) tc_commit(&sh.q_free);
-        };
-        ok = mbar_wait(&sh.q_full, begun & 1, t.p.status, 611);
+        ok = mbar_wait(&sh.q_full, begun & 1, t.p.status, 613);
         ++begun;
-        for (int s = 0; s < ahead && s < n && ok; ++s) {
-          ok = keys(s);
+        if (ok && n == 0) mbar_arrive(&sh.q_free);
+        if (ok && n > 0) {
+          keys(0);
           if (!ok) break;
-          for (int i = 0; i < 2; ++i)
-            if (takes(i, s)) scores(i, s);
-          keys_read(s);
+          tc_fence_after();
+          scores(0);
         }
-        for (int s = 0; s < n && ok; ++s) {
-          const int at = count + s, vs = at % t.v_stages, place0 = (x.u.tile0 + s) * kRtTile;
-          const bool unseen = place0 + kRtTile > x.walk.places || (max(place0, t.p.first) < min(place0 + kRtTile, low));
-          ok = mbar_wait(unseen ? &sh.v_clean[vs] : &sh.v_full[vs], (at / t.v_stages) & 1, t.p.status, 612);
-          if (ok && s + ahead < n) ok = keys(s + ahead);
+        for (int j = 0; j < n && ok; ++j) {
+          const int s = first + j * step, place0 = (x.u.tile0 + s) * kRtKeys;
+          const bool unseen = place0 + kRtKeys > x.walk.places || max(place0, t.p.first) < min(place0 + kRtKeys, low);
+          skip_v(v_at, s);
+          // they have landed, so that the cleaner is past the ones before them in this place; only then can its phase be told
+          if (ok) ok = mbar_wait(&sh.v_full[vs], v_phase, t.p.status, 614);
+          if (ok && unseen) ok = mbar_wait(&sh.v_clean[vs], v_phase, t.p.status, 617);
+          if (j + 1 < n) keys(j + 1);
+          const uint64_t v = v_desc + vs * v_step;
+          if (ok) ok = mbar_wait(&sh.p_full[i][0], done & 1, t.p.status, 615);
           if (!ok) break;
-          for (int i = 0; i < 2 && ok; ++i) {
-            if (takes(i, s)) {
-              ok = mbar_wait(&sh.p_full[i], products[i] & 1, t.p.status, 614 + i);
-              if (!ok) break;
-              tc_fence_after();
-              const uint64_t v = v_desc + static_cast<uint64_t>(vs * (v_bytes / 16));
-              const bool first = s == (x.turns ? i : 0);
-              umma4_ts<128>(tmem + 256 + i * 128, tmem + i * 128, v, idesc_pv, !first);
-              umma4_ts<128>(tmem + 256 + i * 128, tmem + i * 128 + 32, v + 512, idesc_pv, 1);
-              ++products[i];
-              if (!takes(i, s + ahead)) tc_commit(&sh.o_full[i]);
-            }
-            if (x.turns ? takes(i, s) : i == 1) tc_commit(&sh.v_empty[vs]);
-            if (takes(i, s + ahead)) scores(i, s + ahead);
-          }
-          if (ok && s + ahead < n) keys_read(s + ahead);
+          tc_fence_after();
+          umma4_ts<128>(o_t, s_t, v, idesc_pv, j > 0);
+          umma2_ts<128>(o_t, s_t + 32, v + 512, idesc_pv);
+          tc_commit(&sh.most_done[i]);
+          ok = mbar_wait(&sh.p_full[i][1], done & 1, t.p.status, 616);
+          if (!ok) break;
+          tc_fence_after();
+          umma2_ts<128>(o_t, s_t + 48, v + 768, idesc_pv);
+          if (j + 1 < n) scores(j + 1);                  // over the P that these products read
+          else tc_commit(&sh.o_full[i]);
+          tc_commit(&sh.v_empty[vs]);
+          ++done;
+          ++v_at;
+          next_v();
         }
-        count += n;
+        for (int s = min(k_at, v_at); s < x.u.tiles && ok; ++s) {
+          skip_k(k_at, s + 1);
+          skip_v(v_at, s + 1);
+        }
       }
     }
     __syncwarp();
-  } else if (warp == 10) {
-    int count = 0;
+  } else if (warp == 11) {
+    int vs = 0;
+    uint32_t phase = 0;
     bool ok = true;
     for (int turn = 0; unit_at(turn) < units && ok; ++turn) {
       const TiledUnit x = tiled_unit(t, unit_at(turn));
       const int low = ragged_low(x.u.pos0, t.p.window) - x.walk.shift;
-      for (int s = 0; s < x.u.tiles; ++s, ++count) {
-        const int vs = count % t.v_stages, place0 = (x.u.tile0 + s) * kRtTile;
-        ok = WARP_WAIT(&sh.v_full[vs], (count / t.v_stages) & 1, 620);
+      for (int s = 0; s < x.u.tiles; ++s) {
+        const int place0 = (x.u.tile0 + s) * kRtKeys;
+        ok = WARP_WAIT(&sh.v_full[vs], phase, 620);
         if (!ok) break;
         // places [a, b) and [c, 128) of the tile are seen by nobody
-        const int a = max(0, t.p.first - place0), b = min(kRtTile, low - place0), c = min(kRtTile, x.walk.places - place0);
-        if (a < b || c < kRtTile) {
+        const int a = max(0, t.p.first - place0), b = min(kRtKeys, low - place0), c = min(kRtKeys, x.walk.places - place0);
+        if (a < b || c < kRtKeys) {
           for (int k = 0; k < t.vc; ++k) {
-            uint8_t* v = s_v + vs * v_bytes + k * kRtChunk + 16 * (lane & 7);
+            uint8_t* v = s_v + vs * v_bytes + k * kRtKeyChunk + 16 * (lane & 7);
             for (int r = a + (lane >> 3); r < b; r += 4) *reinterpret_cast<uint4*>(v + r * 128) = make_uint4(0, 0, 0, 0);
-            for (int r = c + (lane >> 3); r < kRtTile; r += 4) *reinterpret_cast<uint4*>(v + r * 128) = make_uint4(0, 0, 0, 0);
+            for (int r = c + (lane >> 3); r < kRtKeys; r += 4) *reinterpret_cast<uint4*>(v + r * 128) = make_uint4(0, 0, 0, 0);
           }
           fence_async_smem();
         }
@@ -295,118 +413,177 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
           mbar_arrive(&sh.v_clean[vs]);
           mbar_arrive(&sh.v_empty[vs]);
         }
+        if (++vs == t.v_stages) {
+          vs = 0;
+          phase ^= 1;
+        }
       }
     }
   } else {
     // Where a wait gave up, `ok` stays false and later ones are left out, but every barrier that warps share is reached.
     const int i = warp >> 2, quad = warp & 3, mine = quad * 32 + lane, tid = mine;
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
-    const uint32_t s_t = tmem + lanes + i * 128, o_t = tmem + lanes + 256 + i * 128;
+    const uint32_t o_t = tmem + lanes + 256 + i * 128;
     const int mine_tok = mine / t.group, mine_head = mine - mine_tok * t.group;
+    const uint32_t s_t = tmem + lanes + i * 128;
+    const float2 scale2 = make_float2(t.scale_log2, t.scale_log2);
     int tiles = 0, outputs = 0, halves = 0;
     bool ok = true;
     for (int turn = 0; unit_at(turn) < units; ++turn) {
-      const TiledUnit x = tiled_unit(t, unit_at(turn));
-      const RaggedUnit& u = x.u;
-      if (u.tiles == 0) {
-        for (int r = threadIdx.x; r < u.tokens * t.group; r += 256) {
-          uint4* out = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(t.a.out) + (u.row0 + r / t.group) * t.a.out_row +
-                                                1ll * (u.head * t.group + r % t.group) * vp);
-          for (int c = 0; c < vp / 8; ++c) out[c] = make_uint4(0, 0, 0, 0);
+      // Of this thread's row: visible are the places [0, a) and [b, e); of all of its warp's rows up to a_all, from b_all to e_all.
+      int n, a, b, e, a_all, b_all, e_all, place0, place_step;
+      bool live;
+      {
+        const TiledUnit x = tiled_unit(t, unit_at(turn));
+        const RaggedUnit& u = x.u;
+        if (u.tiles == 0) {
+          for (int r = threadIdx.x; r < u.tokens * t.group; r += 256) {
+            uint4* out = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(t.a.out) + (u.row0 + r / t.group) * t.a.out_row +
+                                                  1ll * (u.head * t.group + r % t.group) * vp);
+            for (int c = 0; c < vp / 8; ++c) out[c] = make_uint4(0, 0, 0, 0);
+          }
+          continue;
         }
-        continue;
+        const int toks = x.turns ? u.tokens : (i ? u.tokens - x.tok0 : x.tok0);
+        live = mine_tok < toks;
+        const int pos = u.pos0 + (i && !x.turns ? x.tok0 : 0) + min(mine_tok, toks - 1);
+        e = pos + 1 - x.walk.shift;
+        b = ragged_low(pos, t.p.window) - x.walk.shift;
+        a = min(t.p.first, e);
+        b_all = __shfl_sync(0xffffffffu, b, 31);
+        e_all = __shfl_sync(0xffffffffu, e, 0);
+        a_all = min(t.p.first, e_all);
+        n = x.n[i];
+        place0 = (u.tile0 + (x.turns ? i : 0)) * kRtKeys;
+        place_step = x.turns ? 2 * kRtKeys : kRtKeys;
       }
-      const int first_tok = i && !x.turns ? x.tok0 : 0, toks = x.turns ? u.tokens : (i ? u.tokens - x.tok0 : x.tok0);
-      const bool live = mine_tok < toks && mine < t.per_tile * t.group;
-      const int pos = u.pos0 + first_tok + min(mine_tok, toks - 1);
-      // visible places of this thread's row: [0, a) and [b, e); of all of its warp's: up to a_all, from b_all to e_all
-      const int shift = x.walk.shift;
-      const int e = pos + 1 - shift, b = ragged_low(pos, t.p.window) - shift, a = min(t.p.first, e);
-      const int b_all = __shfl_sync(0xffffffffu, b, 31), e_all = __shfl_sync(0xffffffffu, e, 0), a_all = min(t.p.first, e_all);
       const bool idle = !__any_sync(0xffffffffu, live);
-      float m = -INFINITY, l = 0.f;
-      const int n = x.n[i];
-      for (int j = 0; j < n; ++j) {
+      float m = -INFINITY, l = 0.f, after = -INFINITY;   // `after`: largest score of the last tile's last keys
+      for (int j = 0; j < n; ++j, ++tiles, place0 += place_step) {
         if (ok) ok = WARP_WAIT(&sh.s_full[i], tiles & 1, 630 + i);
-        ++tiles;
-        if (!ok) continue;
-        if (!idle) {
-          tc_fence_after();
-          const int place0 = (u.tile0 + (x.turns ? 2 * j + i : j)) * kRtTile;
-          if ((place0 < b_all || place0 + kRtTile > e_all) && place0 + kRtTile > a_all) {
-#pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              uint32_t v[32];
-              tmem_ld_32x32(s_t + 32 * c, v);
-              const int at = place0 + 32 * c;
-              const uint32_t seen = low_bits(a - at) | (low_bits(e - at) & ~low_bits(b - at));
-              tmem_wait_ld();
+        const bool work = ok && !idle;
+        // Weights are relative to the maximum so far.  Where that of the first 96 keys, or of the last tile's others, is above it by more
+        // than 2^8, it is raised and they are taken once more.  The others' product follows one that is under way and has to be
+        // relative to the same maximum: up to 2^64 it is.
+        uint32_t x[2][32], w[32];
+        float2 sums[2], neg2;
+        auto begin = [&]() {
+          const float neg = m == -INFINITY ? 0.f : -m;
+          neg2 = make_float2(neg, neg);
+          sums[0] = sums[1] = make_float2(0.f, 0.f);
+        };
+        auto weights = [&](const uint32_t (&v)[32], int from, int to, int at) {
 #pragma unroll
-              for (int k = 0; k < 32; ++k) v[k] = seen >> k & 1 ? v[k] : 0xff800000u;
-              tmem_st_32x32(s_t + 32 * c, v);
+          for (int k = 0; k < 16; ++k) {
+            if (k < from || k >= to) continue;
+            float2 y = fma2(make_float2(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])), scale2, neg2);
+            y.x = ex2_approx(y.x);
+            y.y = ex2_approx(y.y);
+            sums[k & 1] = add2(sums[k & 1], y);
+            const __nv_bfloat162 q = __floats2bfloat162_rn(y.x, y.y);
+            w[at + k] = *reinterpret_cast<const uint32_t*>(&q);
+          }
+        };
+        auto raise = [&](float top, bool grow) {           // O and the sum follow
+          const float m_new = grow ? top : m, keep = grow ? (m == -INFINITY ? 0.f : ex2_approx(m - m_new)) : 1.f;
+          l *= keep;
+          m = m_new;
+#pragma unroll 1
+          for (int c = 0; c < vp; c += 16) {
+            uint32_t o[16];
+            tmem_ld_32x16(o_t + c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
+            tmem_st_32x16(o_t + c, o);
+          }
+        };
+        if (work) {
+          tc_fence_after();
+          const bool edge = (place0 < b_all || place0 + kRtKeys > e_all) && place0 + kRtKeys > a_all;
+          if (edge || j == 0) {
+            float top = -INFINITY;
+#pragma unroll 1
+            for (int c = 0; c < kRtKeys; c += 32) {
+              tmem_ld_32x32(s_t + c, x[0]);
+              const int at = place0 + c;
+              const uint32_t seen = edge ? low_bits(a - at) | (low_bits(e - at) & ~low_bits(b - at)) : ~0u;
+              tmem_wait_ld(x[0]);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) x[0][k] = seen >> k & 1 ? x[0][k] : 0xff800000u;
+              top = fmaxf(top, largest(x[0]));
+              tmem_st_32x32(s_t + c, x[0]);
             }
             tmem_wait_st();
+            if (j == 0) m = top * t.scale_log2;
           }
-          float v[kRtTile];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_t + 32 * c, reinterpret_cast<uint32_t(&)[32]>(v[32 * c]));
-          tmem_wait_ld();
-          float top4[4];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            top4[c] = max3_nan(v[c], v[4 + c], v[8 + c]);
-#pragma unroll
-            for (int k = 12; k + 4 < kRtTile; k += 8) top4[c] = max3_nan(top4[c], v[k + c], v[k + 4 + c]);
-            top4[c] = max3_nan(top4[c], top4[c], v[kRtTile - 4 + c]);
-          }
-          const float top = max3_nan(max3_nan(top4[0], top4[1], top4[2]), top4[3], top4[3]) * t.scale_log2;
-          const bool grow = !(top <= m + 8.f);           // a NaN as well
+          tmem_ld_32x32(s_t, x[0]);
+          tmem_ld_32x32(s_t + 32, x[1]);
+          take_turn(&sh.busy[quad], lane);
+          tmem_wait_ld(x[0]);
+          tmem_wait_ld(x[1]);
+          begin();
+          weights(x[0], 0, 16, 0);
+          float top = largest(x[0]);
+          tmem_ld_32x32(s_t + 64, x[0]);
+          weights(x[1], 0, 16, 16);
+          top = fmaxf(top, largest(x[1]));
+          tmem_ld_32x32(s_t + 96, x[1]);
+          tmem_wait_ld(x[0]);
+          top = fmaxf(fmaxf(top, largest(x[0])) * t.scale_log2, after);
+          const bool grow = top > m + 8.f;
           if (__any_sync(0xffffffffu, grow)) {
-            const float m_new = grow ? top : m;
-            const float keep = grow ? (m == -INFINITY ? 0.f : ex2_approx(m - m_new)) : 1.f;
-            l *= keep;
-            m = m_new;
-            if (j > 0) {
-#pragma unroll 1
-              for (int c = 0; c < vp; c += 16) {
-                uint32_t o[16];
-                tmem_ld_32x16(o_t + c, o);
-                tmem_wait_ld();
-#pragma unroll
-                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
-                tmem_st_32x16(o_t + c, o);
-              }
-            }
+            raise(top, grow);
+            tmem_ld_32x32(s_t, x[0]);
+            tmem_ld_32x32(s_t + 32, x[1]);
+            tmem_wait_ld(x[0]);
+            tmem_wait_ld(x[1]);
+            begin();
+            weights(x[0], 0, 16, 0);
+            weights(x[1], 0, 16, 16);
+            tmem_ld_32x32(s_t + 64, x[0]);
+            tmem_ld_32x32(s_t + 96, x[1]);
+            tmem_wait_ld(x[0]);
           }
-          const float neg = m == -INFINITY ? 0.f : -m;
-          const float2 scale2 = make_float2(t.scale_log2, t.scale_log2), neg2 = make_float2(neg, neg);
-          float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t w[32];
-#pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              float2 y = fma2(make_float2(v[64 * h + 2 * k], v[64 * h + 2 * k + 1]), scale2, neg2);
-              y.x = ex2_approx(y.x);
-              y.y = ex2_approx(y.y);
-              sum[k & 1] = add2(sum[k & 1], y);
-              const __nv_bfloat162 q = __floats2bfloat162_rn(y.x, y.y);
-              w[k] = *reinterpret_cast<const uint32_t*>(&q);
-            }
-            tmem_st_32x32(s_t + 32 * h, w);              // columns whose S this thread has read
-          }
-          l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+          tmem_st_32x32(s_t, w);                         // columns whose S this thread has read
+          weights(x[0], 0, 16, 0);
+          tmem_st_32x16(s_t + 32, reinterpret_cast<uint32_t(&)[16]>(w[0]));
+          end_turn(&sh.busy[quad], lane);
+          tmem_wait_ld(x[1]);
+          l += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
+          begin();
+          weights(x[1], 0, 8, 16);
           tmem_wait_st();
           tc_fence_before();
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.p_full[i]);
+        mbar_arrive_if(ok && lane == 0, &sh.p_full[i][0]);
+        if (work) {
+          weights(x[1], 8, 16, 16);
+          after = largest(x[1]) * t.scale_log2;
+          if (__any_sync(0xffffffffu, after > m + 64.f)) {
+            if (ok) ok = WARP_WAIT(&sh.most_done[i], tiles & 1, 632 + i);
+            tc_fence_after();
+            raise(after, after > m + 64.f);
+            begin();
+            weights(x[1], 0, 16, 16);
+          }
+          l += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
+          tmem_st_32x16(s_t + 48, reinterpret_cast<uint32_t(&)[16]>(w[16]));
+          tmem_wait_st();
+          tc_fence_before();
+        }
+        __syncwarp();
+        mbar_arrive_if(ok && lane == 0, &sh.p_full[i][1]);
       }
       if (n > 0) {
-        if (ok) ok = WARP_WAIT(&sh.o_full[i], outputs & 1, 632 + i);
+        if (ok) ok = WARP_WAIT(&sh.o_full[i], outputs & 1, 634 + i);
         ++outputs;
         tc_fence_after();
       }
+      const TiledUnit x = tiled_unit(t, unit_at(turn));  // once more: it takes registers
+      const RaggedUnit& u = x.u;
+      const int first_tok = i && !x.turns ? x.tok0 : 0, toks = x.turns ? u.tokens : (i ? u.tokens - x.tok0 : x.tok0);
       if (x.turns && i == 1) {
         // this half goes to the first tile's warps
         if (u.tiles > 1) {
@@ -430,7 +607,7 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
           tc_fence_before();
           ++halves;
           __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.half_full);
+          mbar_arrive_if(lane == 0, &sh.half_full);
         }
         continue;
       }
@@ -441,7 +618,7 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
         if (ok) ok = WARP_WAIT(&sh.half_full, halves & 1, 635);
         if (live) {
           const float2 ml = sh.half_ml[mine];
-          const float top = max3_nan(m, ml.x, ml.x), base = top == -INFINITY ? 0.f : top;
+          const float top = fmaxf(m, ml.x), base = top == -INFINITY ? 0.f : top;
           w_own = ex2_approx(m - base);
           w_half = ex2_approx(ml.x - base);
           l = l * w_own + ml.y * w_half;
@@ -456,7 +633,7 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
         if (live) *reinterpret_cast<float2*>(t.p.part_ml + 2 * cell) = make_float2(m, l);
       } else if (live) {
         const float sink = t.a.sink != nullptr ? t.a.sink[h] * kLog2E : -INFINITY;
-        const float top = max3_nan(m, sink, sink), base = top == -INFINITY ? 0.f : top;
+        const float top = fmaxf(m, sink), base = top == -INFINITY ? 0.f : top;
         const float w = ex2_approx(m - base), den = l * w + (t.a.sink != nullptr ? ex2_approx(sink - base) : 0.f);
         f = den != 0.f ? w / den : 0.f;
         if (t.a.gate != nullptr) f *= sigmoid_f32(t.a.gate[row * t.a.gate_row + h]);
@@ -505,7 +682,7 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
       if (joined) {
         fence_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.half_read[halves & 1]);
+        mbar_arrive_if(lane == 0, &sh.half_read[halves & 1]);
         ++halves;
       }
       if (u.pieces > 1 && ragged_last(t.p.counters + u.counter + i, u.pieces, tid == 0, 1 + i, kRtTile, &sh.flag[i]))
@@ -519,22 +696,22 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
   }
 }
 
-// Stages of the rings and the launch's shared memory; 0: the sizes do not fit.
+// Places of the rings and the launch's shared memory; 0: the sizes do not fit.
 inline int tiled_smem(TiledParams& t) {
   t.kd = (t.p.dim + 63) / 64;
   t.vc = (t.p.vdim + 63) / 64;
-  const int qk = t.kd * kRtChunk, v = t.vc * kRtChunk;
+  const int q = 2 * t.kd * kRtChunk, k = t.kd * kRtKeyChunk, v = t.vc * kRtKeyChunk;
   constexpr int kFixed = 1024 + static_cast<int>(sizeof(TiledShared)), kLimit = 227 * 1024;
   t.k_stages = t.v_stages = 1;
-  if (kFixed + 3 * qk + v > kLimit) return 0;
-  while (true) {                                         // keys first: they are needed earlier
-    const int left = kLimit - kFixed - 2 * qk - t.k_stages * qk - t.v_stages * v;
-    if (t.k_stages <= t.v_stages && t.k_stages < kRtStages && left >= qk) ++t.k_stages;
-    else if (t.v_stages < kRtStages && left >= v) ++t.v_stages;
-    else if (t.k_stages < kRtStages && left >= qk) ++t.k_stages;
+  int left = kLimit - kFixed - q - k - v;
+  if (left < 0) return 0;
+  while (true) {                                         // values first: they are held until their weights are there
+    if (t.v_stages <= t.k_stages && t.v_stages < kRtStages && left >= v) ++t.v_stages, left -= v;
+    else if (t.k_stages < kRtStages && left >= k) ++t.k_stages, left -= k;
+    else if (t.v_stages < kRtStages && left >= v) ++t.v_stages, left -= v;
     else break;
   }
-  return kFixed + 2 * qk + t.k_stages * qk + t.v_stages * v;
+  return kLimit - left;
 }
 
 cudaError_t launch_ragged_tiled(const ds41_ragged_attend_args& a, const ds41_ragged_pass& p, cudaStream_t stream) {
@@ -542,14 +719,15 @@ cudaError_t launch_ragged_tiled(const ds41_ragged_attend_args& a, const ds41_rag
   t.a = a;
   t.p = p;
   t.group = p.heads / p.kv_heads;
-  if (p.f32 || t.group > kRtTile || p.vdim > 128 || p.page_tokens < 16 || (p.page_tokens < kRtTile ? kRtTile % p.page_tokens : p.page_tokens % kRtTile))
+  if (p.f32 || t.group > kRtTile || p.vdim > 128 || p.key_tile != kRtKeys || p.page_tokens < 16 ||
+      (p.page_tokens < kRtKeys ? kRtKeys % p.page_tokens : p.page_tokens % kRtKeys))
     return cudaErrorInvalidValue;
   t.per_tile = kRtTile / t.group;
   if (p.unit_tokens != 2 * t.per_tile) return cudaErrorInvalidValue;
   const int smem = tiled_smem(t);
   if (smem == 0) return cudaErrorInvalidValue;
-  t.box = p.page_tokens < kRtTile ? p.page_tokens : kRtTile;
-  if (kRtTile / t.box * (t.kd > t.vc ? t.kd : t.vc) > 32) return cudaErrorInvalidValue;
+  t.box = p.page_tokens < kRtKeys ? p.page_tokens : kRtKeys;
+  if (kRtKeys / t.box * (t.kd > t.vc ? t.kd : t.vc) > 32) return cudaErrorInvalidValue;
   t.slot_rows = t.kd * kRtChunk / (4 * p.vdim);          // their results have to fit the second tile's place
   if (t.slot_rows > kRtSlotRows) t.slot_rows = kRtSlotRows;
   t.hidden_row = a.n_pages * p.page_tokens;

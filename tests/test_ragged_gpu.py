@@ -137,8 +137,8 @@ RUNS = {
 }
 # (heads, kv_heads, dim, vdim, page): those of the tensor-core form, then others
 TILED = [(8, 2, 64, 64, 64), (32, 8, 128, 128, 64), (6, 2, 32, 48, 32), (12, 1, 128, 128, 16), (4, 4, 192, 128, 128), (20, 4, 80, 16, 256),
-         (128, 1, 64, 128, 64), (3, 1, 256, 32, 32)]
-OTHERS = [(8, 2, 64, 64, 24), (4, 1, 128, 256, 64), (2, 2, 16, 16, 8), (200, 1, 32, 32, 64)]
+         (128, 1, 64, 128, 64), (3, 1, 256, 32, 32), (5, 5, 256, 128, 16)]
+OTHERS = [(8, 2, 64, 64, 24), (4, 1, 128, 256, 64), (2, 2, 16, 16, 4), (200, 1, 32, 32, 64)]
 
 
 def test_describe_rows_and_units():
