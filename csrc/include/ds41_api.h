@@ -697,6 +697,7 @@ typedef struct ds41_ragged_pass {
   int window, first;              // a row at p sees j <= p with j > p - window (0: all) or j < first
   int f32, tiled;                 // 32-bit rows; the tensor-core form
   int unit_tokens, key_tile;      // most tokens of a unit, keys of a tile
+  int turn_rows;                  // most (token, head) rows of a unit whose two tiles take the keys in turn
   int max_blocks, max_units, max_cells, grid;
 } ds41_ragged_pass;
 int ds41_ragged_describe(const ds41_ragged_pass* pass, const int* slots, const int* news, const int* lengths, int n,

@@ -14,7 +14,7 @@
 namespace ds41 {
 
 constexpr int kDescribeThreads = 1024;
-constexpr int kMostRequests = 4096, kMostBlocks = 12288;
+constexpr int kMostRequests = 4096, kMostBlocks = 8192;
 constexpr int kCandidates = 16, kBins = 256;
 
 struct DescribeArgs {
@@ -64,23 +64,30 @@ __device__ __forceinline__ void bad_argument(int* status, int where, int detail)
   }
 }
 
+// A tile's time in tenths of that of a tensor-core tile pair of 128 keys, and that of what a unit begins and ends with.
+constexpr int kPairTile = 10, kTurnTile = 7, kUnitCost = 20;
+__device__ __forceinline__ int tile_cost(const ds41_ragged_pass& p, int rows) { return !p.tiled || rows > p.turn_rows ? kPairTile : kTurnTile; }
+
 __global__ void __launch_bounds__(kDescribeThreads) ragged_describe_kernel(const ds41_ragged_pass p, const DescribeArgs a) {
   extern __shared__ int rd_smem[];
-  __shared__ unsigned long long warps[32];
-  __shared__ int units_of[kCandidates], cells_of[kCandidates], bins[kBins], bin_sums[kBins / 32];
-  __shared__ unsigned long long cost_of[kCandidates];
-  __shared__ int longest, chosen;
-  const int tid = threadIdx.x, lane = tid & 31, n = a.n, G = p.kv_heads, group = p.heads / p.kv_heads;
+  __shared__ unsigned long long warps[32], cost_of[kCandidates];
+  __shared__ int units_of[kCandidates], cells_of[kCandidates], bins[kBins], bin_sums[kBins / 32], longest;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.n, G = p.kv_heads, group = p.heads / p.kv_heads;
   int* row_first = rd_smem;             // [n] of every request: its first row, its first block, tokens, first token's position, slot
   int* block_first = row_first + n;
   int* tokens = block_first + n;
   int* begin = tokens + n;
   int* slot_of = begin + n;
-  int* tiles = slot_of + n;             // [blocks] key tiles; then the number of the block's first unit
-  int* cells = tiles + p.max_blocks;    // [blocks] first cell
+  int* owner = slot_of + n;             // [blocks] request
+  int* tiles = owner + p.max_blocks;    // [blocks] key tiles
+  int* first = tiles + p.max_blocks;    // [blocks] first unit of the list by blocks, first cell
+  int* cells = first + p.max_blocks;
   pdl_launch_dependents();
+  if (tid < kCandidates) units_of[tid] = cells_of[tid] = 0, cost_of[tid] = 0;
+  if (tid < kBins) bins[tid] = 0;
+  if (tid == 0) longest = 1;
   pdl_wait();
-  unsigned long long base = 0;
+  unsigned long long base = 0;          // rows, blocks
   for (int i0 = 0; i0 < n; i0 += kDescribeThreads) {
     const int i = i0 + tid;
     int slot = -1, count = 0, length = 0;
@@ -95,19 +102,22 @@ __global__ void __launch_bounds__(kDescribeThreads) ragged_describe_kernel(const
     }
     const int wanted = max(count, 0), most = min(wanted, p.rows);
     unsigned long long total;
-    const unsigned long long at = base + block_scan(static_cast<unsigned long long>(most) << 32, warps, total);
-    base += total;
+    unsigned long long at = block_scan(static_cast<unsigned long long>(most) << 32 | (most + p.unit_tokens - 1) / p.unit_tokens, warps, total);
     // rows beyond the pass's are left out
-    const int first = static_cast<int>(min(at >> 32, static_cast<unsigned long long>(p.rows))), kept = min(most, p.rows - first);
+    const int row = static_cast<int>(min((base + at) >> 32, static_cast<unsigned long long>(p.rows))), kept = min(most, p.rows - row);
     if (kept < wanted && blockIdx.x == 0) bad_argument(p.status, 501, i);
+    if (((base + total) >> 32) > static_cast<unsigned>(p.rows))
+      at = block_scan(static_cast<unsigned long long>(kept) << 32 | (kept + p.unit_tokens - 1) / p.unit_tokens, warps, total);
     if (i < n) {
-      row_first[i] = first;
+      row_first[i] = row;
+      block_first[i] = static_cast<int>((base + at) & 0xffffffffu);
       tokens[i] = kept;
       begin[i] = max(0, length - wanted);
       slot_of[i] = slot;
     }
+    base += total;
   }
-  const int rows = static_cast<int>(min(base >> 32, static_cast<unsigned long long>(p.rows)));
+  const int rows = static_cast<int>(base >> 32), blocks = min(static_cast<int>(base & 0xffffffffu), p.max_blocks);
   __syncthreads();
 
   if (blockIdx.x > 0) {
@@ -132,46 +142,27 @@ __global__ void __launch_bounds__(kDescribeThreads) ragged_describe_kernel(const
     return;
   }
 
-  // blocks
-  unsigned long long blocks64 = 0;
-  for (int i0 = 0; i0 < n; i0 += kDescribeThreads) {
-    const int i = i0 + tid;
-    const int mine = i < n ? (tokens[i] + p.unit_tokens - 1) / p.unit_tokens : 0;
-    unsigned long long total;
-    const unsigned long long at = blocks64 + block_scan(mine, warps, total);
-    blocks64 += total;
-    if (i < n) block_first[i] = static_cast<int>(at);
-  }
-  const int blocks = min(static_cast<int>(blocks64), p.max_blocks);
-  if (tid < kCandidates) units_of[tid] = cells_of[tid] = 0, cost_of[tid] = 0;
-  if (tid < kBins) bins[tid] = 0;
-  if (tid == 0) longest = 0;
-  __syncthreads();
+  // blocks: request, key tiles
   const int align = min(p.page_tokens, p.key_tile);
-  auto block_of = [&](int b, int& i, int& t0, int& count, int& pos0) {
-    i = find_last(block_first, n, b);
-    t0 = (b - block_first[i]) * p.unit_tokens;
-    count = min(p.unit_tokens, tokens[i] - t0);
-    pos0 = begin[i] + t0;
-  };
   int most = 0;
   for (int b = tid; b < blocks; b += kDescribeThreads) {
-    int i, t0, count, pos0, k = 0;
-    block_of(b, i, t0, count, pos0);
+    const int i = find_last(block_first, n, b), t0 = (b - block_first[i]) * p.unit_tokens, count = min(p.unit_tokens, tokens[i] - t0);
+    int k = 0;
     if (slot_of[i] >= 0) {
-      const RaggedWalk w = ragged_walk(pos0, pos0 + count - 1, p.window, p.first, align);
+      const RaggedWalk w = ragged_walk(begin[i] + t0, begin[i] + t0 + count - 1, p.window, p.first, align);
       k = (w.places + p.key_tile - 1) / p.key_tile;
     }
+    owner[b] = i;
     tiles[b] = k;
     cells[b] = count * group;
-    most = max(most, k);
+    most = max(most, k * tile_cost(p, count * group));
   }
   most = __reduce_max_sync(0xffffffffu, most);
-  if (lane == 0) atomicMax(&longest, most);
+  if (lane == 0 && most > 0) atomicMax(&longest, most);
   __syncthreads();
-  const int longest_walk = max(longest, 1);
-  // How long a piece may be.  A CTA's time is its pieces' tiles, two tiles' time for what a piece begins and ends with, and for a part
-  // of `unit_tokens` tokens that has to be joined one more to write and one to read; the join comes last.
+  // How long a piece may be.  A CTA's time is its pieces' tiles and what they begin and end with, and for a part of `unit_tokens` tokens
+  // that has to be joined as much again to write and read it; the join comes last.
+  const int longest_walk = longest;
   auto limit = [&](int k) {
     constexpr int kDivide[kCandidates] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256};
     int d = 1;
@@ -179,104 +170,103 @@ __global__ void __launch_bounds__(kDescribeThreads) ragged_describe_kernel(const
     for (int j = 0; j < kCandidates; ++j) d = k == j ? kDivide[j] : d;
     return (longest_walk + d - 1) / d;
   };
+  auto pieces_of = [&](int tiles, int cells, int most_cost) {
+    return max(1, min(tiles, (tiles * tile_cost(p, cells) + most_cost - 1) / most_cost));
+  };
   const int full = p.unit_tokens * group;
-#pragma unroll 1
-  for (int k = 0; k < kCandidates; ++k) {
-    const int most_tiles = limit(k);
+  {
+    static_assert(kDescribeThreads / 32 == 2 * kCandidates, "two warps to a length");
+    const int k = warp % kCandidates, most_cost = limit(k);
     int units = 0, parts = 0;
     unsigned long long cost = 0;                        // whole numbers: the choice is the same every time
-    for (int b = tid; b < blocks; b += kDescribeThreads) {
-      const int pieces = max(1, (tiles[b] + most_tiles - 1) / most_tiles);
+    for (int b = lane + 32 * (warp / kCandidates); b < blocks; b += 64) {
+      const int pieces = pieces_of(tiles[b], cells[b], most_cost);
       units += pieces;
-      cost += 4ull * tiles[b] + 8 * pieces;
+      cost += 1ull * tiles[b] * tile_cost(p, cells[b]) + kUnitCost * pieces;
       if (pieces > 1) {
         parts += min(pieces * cells[b], 1 << 20);
-        cost += 8 * pieces * cells[b] / full;
+        cost += kUnitCost * pieces * cells[b] / full;
       }
     }
     units = __reduce_add_sync(0xffffffffu, units);
-    parts = __reduce_add_sync(0xffffffffu, min(parts, 1 << 22));
+    parts = __reduce_add_sync(0xffffffffu, min(parts, 1 << 24));
 #pragma unroll
     for (int o = 16; o; o >>= 1) cost += __shfl_xor_sync(0xffffffffu, cost, o);
     if (lane == 0 && units > 0) {
       atomicAdd(&units_of[k], units);
-      atomicAdd(&cells_of[k], min(parts, 1 << 25));
+      atomicAdd(&cells_of[k], min(parts, 1 << 29));
       atomicAdd(&cost_of[k], cost);
     }
   }
   __syncthreads();
-  if (tid < 32) {
-    float time = INFINITY;
+  int most_cost;
+  {
+    float time = INFINITY;                              // every warp finds the same
     if (lane < kCandidates && (lane == 0 || (1ll * units_of[lane] * G <= p.max_units && 1ll * cells_of[lane] * G <= p.max_cells))) {
-      const float units = static_cast<float>(units_of[lane]) * G, turns = ceilf(units / p.grid);
-      const float cost = static_cast<float>(cost_of[lane]) * 0.25f * G;
-      time = fmaxf(limit(lane) + 2.f, turns * cost / fmaxf(units, 1.f)) + (cells_of[lane] > 0 ? 3.f : 0.f);
+      const float units = static_cast<float>(units_of[lane]) * G, turns = ceilf(units / p.grid), cost = static_cast<float>(cost_of[lane]) * G;
+      time = fmaxf(static_cast<float>(limit(lane) + kUnitCost), turns * cost / fmaxf(units, 1.f)) + (cells_of[lane] > 0 ? 1.5f * kUnitCost : 0.f);
     }
     float best = time;
 #pragma unroll
     for (int o = 16; o; o >>= 1) best = fminf(best, __shfl_xor_sync(0xffffffffu, best, o));
-    const unsigned who = __ballot_sync(0xffffffffu, time == best);
-    if (lane == 0) chosen = limit(__ffs(who) - 1);
+    most_cost = limit(__ffs(__ballot_sync(0xffffffffu, time == best)) - 1);
   }
-  __syncthreads();
-  const int most_tiles = chosen;
   // the longest pieces first
-  auto bin_of = [&](int t) { return kBins - 1 - static_cast<int>(static_cast<long long>(t) * (kBins - 1) / most_tiles); };
+  const int widest = longest_walk < most_cost + kPairTile ? longest_walk : most_cost + kPairTile;
+  const float per_cost = (kBins - 1) / static_cast<float>(widest);
+  auto bin_of = [&](int cost) { return kBins - 1 - min(kBins - 1, static_cast<int>(cost * per_cost)); };
   unsigned long long sums = 0;
   for (int b0 = 0; b0 < blocks; b0 += kDescribeThreads) {
     const int b = b0 + tid;
-    int pieces = 0, parts = 0, k = 0;
+    int pieces = 0, parts = 0;
     if (b < blocks) {
-      k = tiles[b];
-      pieces = max(1, (k + most_tiles - 1) / most_tiles);
+      const int k = tiles[b], c = tile_cost(p, cells[b]);
+      pieces = pieces_of(k, cells[b], most_cost);
       parts = pieces > 1 ? pieces * cells[b] * G : 0;
-      const int more = k % pieces;                     // pieces of one tile more than the others
-      if (more) atomicAdd(&bins[bin_of(k / pieces + 1)], more * G);
-      atomicAdd(&bins[bin_of(k / pieces)], (pieces - more) * G);
+      const int least = k / pieces, more = k - least * pieces;             // pieces of one tile more than the others
+      if (more) atomicAdd(&bins[bin_of((least + 1) * c)], more * G);
+      atomicAdd(&bins[bin_of(least * c)], (pieces - more) * G);
     }
     unsigned long long total;
     const unsigned long long at = sums + block_scan(static_cast<unsigned long long>(pieces * G) << 32 | parts, warps, total);
     sums += total;
     if (b < blocks) {
-      tiles[b] = static_cast<int>(at >> 32);           // of the list by blocks: the block's first
+      first[b] = static_cast<int>(at >> 32);
       cells[b] = static_cast<int>(at & 0xffffffffu);
     }
   }
   const int units = static_cast<int>(sums >> 32);
   __syncthreads();
   // where a bin's units begin
-  int count = tid < kBins ? bins[tid] : 0, upto = count;
-  if (tid < kBins) {
+  const int count = tid < kBins ? bins[tid] : 0;
+  int upto = count;
 #pragma unroll
-    for (int o = 1; o < 32; o *= 2) {
-      const int y = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += y;
-    }
-    if (lane == 31) bin_sums[tid >> 5] = upto;
+  for (int o = 1; o < 32; o *= 2) {
+    const int y = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += y;
   }
+  if (tid < kBins && lane == 31) bin_sums[warp] = upto;
   __syncthreads();
   if (tid < kBins) {
     int before = 0;
-    for (int w = 0; w < (tid >> 5); ++w) before += bin_sums[w];
+    for (int w = 0; w < warp; ++w) before += bin_sums[w];
     bins[tid] = before + upto - count;
   }
   __syncthreads();
   for (int u = tid; u < units; u += kDescribeThreads) {
-    const int b = find_last(tiles, blocks, u);
-    int i, t0, tk, pos0;
-    block_of(b, i, t0, tk, pos0);
-    int k = 0;
-    if (slot_of[i] >= 0) {
-      const RaggedWalk w = ragged_walk(pos0, pos0 + tk - 1, p.window, p.first, align);
-      k = (w.places + p.key_tile - 1) / p.key_tile;
-    }
-    const int pieces = max(1, (k + most_tiles - 1) / most_tiles), x = u - tiles[b], head = x / pieces, piece = x - head * pieces;
+    const int b = find_last(first, blocks, u), i = owner[b], k = tiles[b];
+    const int t0 = (b - block_first[i]) * p.unit_tokens, tk = min(p.unit_tokens, tokens[i] - t0), step = tk * group;
+    const int pieces = pieces_of(k, step, most_cost), x = u - first[b], head = x / pieces, piece = x - head * pieces;
     const int least = k / pieces, more = k - least * pieces;
     const int mine = least + (piece < more), tile0 = piece * least + min(piece, more);
-    const int step = tk * group;
-    const int at = atomicAdd(&bins[bin_of(mine)], 1);
+    // one thread asks for all of its warp's of a bin
+    const int bin = bin_of(mine * tile_cost(p, step));
+    const unsigned same = __match_any_sync(__activemask(), bin);
+    const int leader = __ffs(same) - 1;
+    int at = lane == leader ? atomicAdd(&bins[bin], __popc(same)) : 0;
+    at = __shfl_sync(same, at, leader) + __popc(same & ((1u << lane) - 1));
     int4* out = reinterpret_cast<int4*>(p.units + 1ll * at * kRaggedInts);
-    out[0] = make_int4(slot_of[i], row_first[i] + t0, tk, pos0);
+    out[0] = make_int4(slot_of[i], row_first[i] + t0, tk, begin[i] + t0);
     out[1] = make_int4(head, tile0, mine, piece);
     out[2] = make_int4(pieces, cells[b] + head * pieces * step, 2 * (b * G + head), step);
   }
@@ -287,15 +277,33 @@ __global__ void __launch_bounds__(kDescribeThreads) ragged_describe_kernel(const
 }
 
 // ---------------------------------------------------------------------------------------------------- heads
+inline bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
 constexpr int kHeadsThreads = 256;
 
-// Cosine and sine of pos * freq.  The product has up to 31 + 24 bits: it is formed, and brought into half a turn, in 64.
+// Cosine and sine of pos * freq, pos >= 0.  In turns that is pos * (freq / 2 pi), of which only the fraction counts: with freq / 2 pi as
+// a whole number of 2^-64 turns it is what 64 bits hold of a product of whole numbers, as exact for far positions as for near ones (with
+// the product and its reduction in 64-bit floating point, which is slow here, the rotations of 8192 rows took 12 us).
+__device__ __forceinline__ unsigned long long turns_of(float freq) {
+  constexpr unsigned long long kInverse = 11743562013128004906ull;       // 2^66 / (2 pi)
+  const uint32_t bits = __float_as_uint(freq), exponent = bits >> 23 & 0xff;
+  const unsigned long long m = (bits & 0x7fffffu) | (exponent ? 0x800000u : 0u);
+  const int right = 152 - static_cast<int>(exponent ? exponent : 1);       // freq = m 2^(exponent - 150)
+  const unsigned long long low = m * kInverse, high = __umul64hi(m, kInverse);
+  unsigned long long x;
+  if (right <= 0) x = right > -64 ? low << -right : 0;
+  else if (right < 64) x = low >> right | high << (64 - right);
+  else x = right < 128 ? high >> (right - 64) : 0;
+  return bits >> 31 ? 0ull - x : x;
+}
 __device__ __forceinline__ float2 turn_at(int pos, float freq) {
-  const double x = static_cast<double>(pos) * static_cast<double>(freq);
-  const double k = rint(x * 0.15915494309189535);
+  if (!(fabsf(freq) < INFINITY)) return make_float2(NAN, NAN);
+  const uint32_t part = static_cast<uint32_t>(static_cast<unsigned long long>(pos) * turns_of(freq) >> 32);       // of a turn, in 2^-32
+  const uint32_t quarter = (part + 0x20000000u) >> 30;
   float s, c;
-  sincosf(static_cast<float>(fma(-k, 6.283185307179586, x)), &s, &c);
-  return make_float2(c, s);
+  sincospif(static_cast<float>(static_cast<int>(part - (quarter << 30))) * 4.6566128730773926e-10f, &s, &c);     // within an eighth; 2^-31
+  const float x = quarter & 1 ? -s : c, y = quarter & 1 ? c : s;
+  return quarter & 2 ? make_float2(-x, -y) : make_float2(x, y);
 }
 
 // Any sizes: one block per row, whose heads stay in shared memory between the norm and the rotation.
@@ -340,6 +348,188 @@ __global__ void __launch_bounds__(kHeadsThreads) ragged_heads_kernel(const ds41_
     }
   }
   for (int c = tid; c < G * V; c += kHeadsThreads) row[G * D + c] = from_f32<T>(proj_at(p.v, r, c));
+}
+
+// Heads of multiples of 16 values and rotations of multiples of 16, rows of whole 16 bytes.  A lane has 16 values of a head: in its rotated
+// part eight and the eight that they turn with, else neighbours; as many lanes as a head has sixteens (or the next power of two) share
+// it.  A warp takes `per` steps of one row, in each of which its lanes have neighbouring heads, and keeps its lanes' turns and weights.
+// Bound by memory: what is read and written is read and written once, in whole lines.
+struct Sixteen {
+  float v[16];
+};
+template <bool PACKED>
+struct RawSixteen {
+  uint4 a, b;
+  __device__ __forceinline__ void load(const ds41_proj& p, long long r, int ca, int cb) {
+    const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(p.data) + r * p.ld + p.col;
+    a = *reinterpret_cast<const uint4*>(row + ca);
+    b = *reinterpret_cast<const uint4*>(row + cb);
+  }
+  __device__ __forceinline__ Sixteen get() const {
+    const uint32_t q[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    Sixteen x;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x.v[2 * i] = __uint_as_float(q[i] << 16);
+      x.v[2 * i + 1] = __uint_as_float(q[i] & 0xffff0000u);
+    }
+    return x;
+  }
+};
+template <>
+struct RawSixteen<false> {
+  float4 q[4];
+  __device__ __forceinline__ void load(const ds41_proj& p, long long r, int ca, int cb) {
+    q[0] = proj_at4(p, r, ca);
+    q[1] = proj_at4(p, r, ca + 4);
+    q[2] = proj_at4(p, r, cb);
+    q[3] = proj_at4(p, r, cb + 4);
+  }
+  __device__ __forceinline__ Sixteen get() const {
+    Sixteen x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x.v[4 * i] = q[i].x;
+      x.v[4 * i + 1] = q[i].y;
+      x.v[4 * i + 2] = q[i].z;
+      x.v[4 * i + 3] = q[i].w;
+    }
+    return x;
+  }
+};
+__device__ __forceinline__ void store_eight(float* to, const float* v) {
+  store4(to, make_float4(v[0], v[1], v[2], v[3]));
+  store4(to + 4, make_float4(v[4], v[5], v[6], v[7]));
+}
+__device__ __forceinline__ void store_eight(__nv_bfloat16* to, const float* v) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 q = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&q);
+  }
+  *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+struct HeadsSteps {
+  int lanes;                 // to a head
+  int q, qk, all;            // steps of queries, of queries and keys, and with the values
+  int per, parts;            // steps of a warp, warps of a row
+};
+
+template <typename T, bool PACKED>
+__global__ void __launch_bounds__(kHeadsThreads) ragged_heads_wide_kernel(const ds41_ragged_heads_args p, const HeadsSteps h) {
+  extern __shared__ __align__(16) float2 rw_turns[];     // [warps][rot_dim / 2]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = p.rot_dim / 2;
+  const int G = p.kv_heads, D = p.dim, V = p.vdim, per_step = 32 / h.lanes, unit = lane % h.lanes;
+  const long long w = 1ll * blockIdx.x * (kHeadsThreads / 32) + warp;
+  const int r = static_cast<int>(w / h.parts), s0 = static_cast<int>(w % h.parts) * h.per, s1 = min(h.all, s0 + h.per);
+  const bool turned = 16 * unit < p.rot_dim;
+  const int ca = turned ? 8 * unit : 16 * unit, cb = turned ? half + 8 * unit : ca + 8;
+  pdl_launch_dependents();
+  pdl_wait();
+  if (r >= p.rows) return;
+  const int place = p.row_place[r], pos = p.row_pos[r];
+  // step s of this lane: which projection, its columns there
+  auto fetch = [&](int s, RawSixteen<PACKED>& raw) {
+    if (s < h.qk) {
+      const bool key = s >= h.q;
+      const int g = (s - (key ? h.q : 0)) * per_step + lane / h.lanes;
+      if (16 * unit < D && g < (key ? G : p.heads)) raw.load(key ? p.k : p.q, r, g * D + ca, g * D + cb);
+    } else {
+      const int c = ((s - h.qk) * 32 + lane) * 16;
+      if (c < G * V) raw.load(p.v, r, c, c + 8);
+    }
+  };
+  RawSixteen<PACKED> next;
+  fetch(s0, next);
+  if (place < 0 || place >= p.pool_rows) return;
+  float2 turn[8];
+  if (half > 0 && s0 < h.qk) {
+    float2* mine = rw_turns + warp * half;
+    for (int i = lane; i < half; i += 32) mine[i] = turn_at(pos, p.freq[i]);
+    __syncwarp();
+#pragma unroll
+    for (int e = 0; e < 8; ++e) turn[e] = turned ? mine[8 * unit + e] : make_float2(1.f, 0.f);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) turn[e] = make_float2(1.f, 0.f);
+  }
+  T* row = static_cast<T*>(p.pool) + 1ll * place * (G * (D + V));
+  T* q = static_cast<T*>(p.q_out) + r * p.ld_q;
+  float weight[16];
+  bool first = true;
+  for (int s = s0; s < s1; ++s) {
+    Sixteen x = next.get();
+    if (s + 1 < s1) fetch(s + 1, next);
+    if (s >= h.qk) {
+      const int c = ((s - h.qk) * 32 + lane) * 16;
+      if (c < G * V) {
+        store_eight(row + G * D + c, x.v);
+        store_eight(row + G * D + c + 8, x.v + 8);
+      }
+      continue;
+    }
+    const bool key = s >= h.q;
+    const int g = (s - (key ? h.q : 0)) * per_step + lane / h.lanes;
+    const bool live = 16 * unit < D && g < (key ? G : p.heads);
+    const float* norm = key ? p.k_norm : p.q_norm;
+    const int stride = key ? p.k_norm_stride : p.q_norm_stride;
+    if (norm != nullptr) {
+      if (first || s == h.q || stride > 0) {
+        if (live) {
+          const float* at = norm + 1ll * g * stride;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float4 u = *reinterpret_cast<const float4*>(at + ca + 4 * e), v = *reinterpret_cast<const float4*>(at + cb + 4 * e);
+            weight[4 * e] = u.x, weight[4 * e + 1] = u.y, weight[4 * e + 2] = u.z, weight[4 * e + 3] = u.w;
+            weight[8 + 4 * e] = v.x, weight[9 + 4 * e] = v.y, weight[10 + 4 * e] = v.z, weight[11 + 4 * e] = v.w;
+          }
+        }
+        first = !live;                                   // a lane without a head here may have one in a later step
+      }
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sum += x.v[e] * x.v[e];
+      sum = live ? sum : 0.f;
+      for (int o = h.lanes / 2; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      const float f = 1.0f / sqrtf(sum / p.width + p.eps);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x.v[e] *= f * weight[e];
+    }
+    if (!live) continue;
+    float y[16];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      y[e] = x.v[e] * turn[e].x - x.v[8 + e] * turn[e].y;
+      y[8 + e] = x.v[8 + e] * turn[e].x + x.v[e] * turn[e].y;
+    }
+    T* to = key ? row + g * D : q + 1ll * g * D;
+    store_eight(to + ca, y);
+    store_eight(to + cb, y + 8);
+  }
+}
+
+template <typename T, bool PACKED>
+cudaError_t launch_heads_wide(const ds41_ragged_heads_args& a, cudaStream_t st) {
+  HeadsSteps h{};
+  h.lanes = 1;
+  while (16 * h.lanes < a.dim) h.lanes *= 2;
+  const int per_step = 32 / h.lanes;
+  h.q = (a.heads + per_step - 1) / per_step;
+  h.qk = h.q + (a.kv_heads + per_step - 1) / per_step;
+  h.all = h.qk + (a.kv_heads * a.vdim + 511) / 512;
+  // few rows: a warp for every step; many: whole rows, whose turns are made once
+  h.per = static_cast<int>(std::min<long long>(h.all, std::max<long long>(1, 1ll * a.rows * h.all / (148 * 48))));
+  h.parts = (h.all + h.per - 1) / h.per;
+  const long long blocks = (1ll * a.rows * h.parts + kHeadsThreads / 32 - 1) / (kHeadsThreads / 32);
+  if (blocks > INT_MAX) return cudaErrorInvalidValue;
+  const int smem = kHeadsThreads / 32 * a.rot_dim / 2 * static_cast<int>(sizeof(float2));
+  return launch_pdl(ragged_heads_wide_kernel<T, PACKED>, dim3(static_cast<unsigned>(blocks)), dim3(kHeadsThreads), smem, st, a, h);
+}
+
+inline bool packed_row(const ds41_proj& p) {
+  return p.bf16 && !(p.ld & 7) && !(p.col & 7) && !(reinterpret_cast<uintptr_t>(p.data) & 15);
 }
 
 // ---------------------------------------------------------------------------------------------------- attention, any type and size
@@ -557,15 +747,13 @@ cudaError_t launch_ragged_simple(const ds41_ragged_attend_args& a, const ds41_ra
   return launch_simple<T, 16>(a, p, st);
 }
 
-inline bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
-
 inline bool ragged_pass_ok(const ds41_ragged_pass* p) {
   if (p == nullptr || p->header == nullptr || p->row_pos == nullptr || p->row_slot == nullptr || p->row_place == nullptr ||
       p->units == nullptr || p->counters == nullptr || p->part_o == nullptr || p->part_ml == nullptr || p->status == nullptr)
     return false;
   if (p->rows <= 0 || p->rows > 1 << 18 || p->requests <= 0 || p->requests > kMostRequests || p->heads <= 0 || p->kv_heads <= 0 ||
       p->heads % p->kv_heads || p->heads / p->kv_heads > 1024 || p->dim <= 0 || p->dim > 256 || (p->dim & 15) || p->vdim <= 0 ||
-      p->vdim > 256 || (p->vdim & 15) || p->page_tokens <= 0 || p->window < 0 || p->first < 0 || p->unit_tokens <= 0 || p->grid <= 0)
+      p->vdim > 256 || (p->vdim & 15) || p->page_tokens <= 0 || p->window < 0 || p->first < 0 || p->unit_tokens <= 0 || p->grid <= 0 || p->turn_rows < 0)
     return false;
   return p->max_blocks >= p->rows / p->unit_tokens + std::min(p->requests, p->rows) && p->max_blocks <= kMostBlocks &&
          p->max_units >= 1ll * p->max_blocks * p->kv_heads && p->max_units < 1 << 22 && p->max_cells > 0 && p->max_cells < 1 << 22 &&
@@ -581,13 +769,13 @@ extern "C" int ds41_ragged_describe(const ds41_ragged_pass* p, const int* slots,
   if (!ragged_pass_ok(p) || n < 0 || n > p->requests || n_slots <= 0 || max_pages <= 0 || n_pages <= 0 || page_table == nullptr ||
       (n > 0 && (slots == nullptr || news == nullptr || lengths == nullptr)) || 1ll * n_pages * p->page_tokens > INT_MAX)
     return cudaErrorInvalidValue;
-  const int smem = 4 * (5 * n + 2 * p->max_blocks);
+  const int smem = 4 * (5 * n + 4 * p->max_blocks);
   static std::atomic<unsigned long long> ready{0};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev >= 64 || !(ready.load() >> dev & 1)) {
-    e = cudaFuncSetAttribute(ragged_describe_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * (5 * kMostRequests + 2 * kMostBlocks));
+    e = cudaFuncSetAttribute(ragged_describe_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * (5 * kMostRequests + 4 * kMostBlocks));
     if (e != cudaSuccess) return e;
     if (dev < 64) ready.fetch_or(1ull << dev);
   }
@@ -603,8 +791,16 @@ extern "C" int ds41_ragged_heads(const ds41_ragged_heads_args* a, void* stream) 
       a->row_place == nullptr || a->q_out == nullptr || a->pool == nullptr || a->pool_rows <= 0 || a->ld_q < 1ll * a->heads * a->dim ||
       a->q_norm_stride < 0 || a->k_norm_stride < 0 || (a->heads + a->kv_heads) * a->dim * 4 + a->rot_dim * 4 > 200 * 1024)
     return cudaErrorInvalidValue;
-  const int smem = (a->heads + a->kv_heads) * a->dim * 4 + a->rot_dim * 4;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (!(a->dim & 15) && a->dim <= 512 && !(a->rot_dim & 15) && !(a->kv_heads * a->vdim & 15) && !(a->ld_q & 7) && aligned(a->q_out, 16) &&
+      aligned(a->pool, 16) && (a->q_norm == nullptr || aligned(a->q_norm, 16)) && (a->k_norm == nullptr || aligned(a->k_norm, 16)) &&
+      !(a->q_norm_stride & 3) && !(a->k_norm_stride & 3)) {
+    if (packed_row(a->q) && packed_row(a->k) && packed_row(a->v))
+      return a->f32 ? launch_heads_wide<float, true>(*a, st) : launch_heads_wide<__nv_bfloat16, true>(*a, st);
+    if (proj_vec4(a->q) && proj_vec4(a->k) && proj_vec4(a->v))
+      return a->f32 ? launch_heads_wide<float, false>(*a, st) : launch_heads_wide<__nv_bfloat16, false>(*a, st);
+  }
+  const int smem = (a->heads + a->kv_heads) * a->dim * 4 + a->rot_dim * 4;
   auto kernel = a->f32 ? ragged_heads_kernel<float> : ragged_heads_kernel<__nv_bfloat16>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
   if (e != cudaSuccess) return e;

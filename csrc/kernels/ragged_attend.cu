@@ -27,7 +27,7 @@ constexpr int kRtThreads = 384;
 constexpr int kRtTile = 128, kRtKeys = 128;    // rows of a tile, keys of a tile
 constexpr int kRtChunk = kRtTile * 128;        // bytes of 128 rows x 64 bf16 columns
 constexpr int kRtKeyChunk = kRtKeys * 128;     // of its keys
-constexpr int kRtStages = 4, kRtSlotRows = 64;
+constexpr int kRtStages = 4, kRtTurnRows = 64;
 
 struct TiledParams {
   ds41_ragged_attend_args a;
@@ -35,7 +35,7 @@ struct TiledParams {
   int group, per_tile;       // query heads of a key/value head, tokens of a tile
   int kd, vc;                // 64-column chunks of a key and a value
   int k_stages, v_stages;
-  int box, slot_rows;        // rows of a copy; most rows of a block whose tiles take the keys in turn
+  int box;                   // rows of a copy
   int hidden_row;            // beyond the pool: reads as zeros
   float scale_log2;
 };
@@ -50,7 +50,7 @@ struct TiledShared {
   uint64_t most_done[2];                       // the product with the former is complete
   uint64_t o_full[2];                          // the unit's last product is complete
   uint64_t half_full, half_read[2];            // the second tile's half of a unit whose keys were taken in turn
-  float2 half_ml[kRtSlotRows];
+  float2 half_ml[kRtTurnRows];
   uint32_t tmem;
   int flag[2];
   int busy[4];                                 // per scheduler: one of its two softmax warps is at its exponentials
@@ -80,7 +80,7 @@ __device__ __forceinline__ TiledUnit tiled_unit(const TiledParams& t, int i) {
   TiledUnit x;
   x.u = ragged_unit(t.p, i);
   const RaggedUnit& u = x.u;
-  x.turns = u.tokens * t.group <= t.slot_rows;
+  x.turns = u.tokens * t.group <= t.p.turn_rows;
   x.tok0 = x.turns ? u.tokens : (u.tokens + 1) / 2;
   x.walk = ragged_walk(u.pos0, u.pos0 + u.tokens - 1, t.p.window, t.p.first, t.box);
   if (x.turns) {
@@ -728,8 +728,8 @@ cudaError_t launch_ragged_tiled(const ds41_ragged_attend_args& a, const ds41_rag
   if (smem == 0) return cudaErrorInvalidValue;
   t.box = p.page_tokens < kRtKeys ? p.page_tokens : kRtKeys;
   if (kRtKeys / t.box * (t.kd > t.vc ? t.kd : t.vc) > 32) return cudaErrorInvalidValue;
-  t.slot_rows = t.kd * kRtChunk / (4 * p.vdim);          // their results have to fit the second tile's place
-  if (t.slot_rows > kRtSlotRows) t.slot_rows = kRtSlotRows;
+  // the results of tiles in turns have to fit the second tile's place
+  if (p.turn_rows > kRtTurnRows || p.turn_rows * 4 * p.vdim > t.kd * kRtChunk) return cudaErrorInvalidValue;
   t.hidden_row = a.n_pages * p.page_tokens;
   t.scale_log2 = a.scale * kLog2E;
   const int row_len = p.kv_heads * (p.dim + p.vdim);

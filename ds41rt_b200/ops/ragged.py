@@ -27,18 +27,19 @@ import torch
 
 from . import lib
 from . import stack as S
-from .prefix import _heads, _steps, _stream
+from .prefix import _heads, _steps
 
 BF16, F32, I32 = torch.bfloat16, torch.float32, torch.int32
 SMS = 148                       # of a B200: passes do not depend on the device found
+_raw_stream = torch._C._cuda_getCurrentRawStream      # without the object that torch.cuda.current_stream() makes for it (3 us)
 UNIT = 12                       # numbers of a unit (ds41_ragged_pass)
-MOST_ROWS, MOST_REQUESTS, MOST_BLOCKS = 1 << 18, 4096, 12288
+MOST_ROWS, MOST_REQUESTS, MOST_BLOCKS = 1 << 18, 4096, 8192
 
 
 class PassArgs(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("header", "row_pos", "row_slot", "row_place", "units", "counters", "part_o", "part_ml", "status")] + \
                [(n, C.c_int) for n in ("rows", "requests", "heads", "kv_heads", "dim", "vdim", "page_tokens", "window", "first", "f32", "tiled",
-                                       "unit_tokens", "key_tile", "max_blocks", "max_units", "max_cells", "grid")]
+                                       "unit_tokens", "key_tile", "turn_rows", "max_blocks", "max_units", "max_cells", "grid")]
 
 
 class HeadsArgs(C.Structure):
@@ -81,6 +82,7 @@ class RaggedPass:
             raise ValueError(f"cache rows are bf16 or fp32, not {dtype}")
         self.rows, self.requests, self.heads, self.kv_heads, self.dim, self.vdim = rows, requests, heads, kv_heads, dim, vdim
         self.page_tokens, self.window, self.first, self.dtype, self.device = page_tokens, window, first, dtype, torch.device(device)
+        self.columns = kv_heads * (dim + vdim)
         self._sizes()
         i32 = lambda n: torch.zeros(n, dtype=I32, device=self.device)
         self.header, self.units, self.counters = i32(16), i32(UNIT * self.max_units), i32(2 * self.max_blocks * kv_heads)
@@ -93,7 +95,7 @@ class RaggedPass:
         a = PassArgs(*(t.data_ptr() for t in (self.header, self.row_pos, self.row_slot, self.row_place, self.units, self.counters,
                                               self.part_o, self.part_ml, self.status)),
                      rows, requests, heads, kv_heads, dim, vdim, page_tokens, window, first, int(dtype == F32), int(self.tiled),
-                     self.unit_tokens, self.key_tile, self.max_blocks, self.max_units, self.max_cells, SMS)
+                     self.unit_tokens, self.key_tile, self.turn_rows, self.max_blocks, self.max_units, self.max_cells, SMS)
         self.args, self.args_ref = a, C.byref(a)
 
     def _sizes(self):
@@ -101,6 +103,8 @@ class RaggedPass:
         self.tiled = self.dtype == BF16 and tiled(self.heads, self.kv_heads, self.dim, self.vdim, self.page_tokens)
         self.unit_tokens = 2 * (128 // group) if self.tiled else max(1, 64 // group)
         self.key_tile = 128 if self.tiled else 32
+        # of the tensor-core form: blocks of so few rows have them in both of a CTA's tiles, which take the keys in turn
+        self.turn_rows = min(64, -(-self.dim // 64) * 16384 // (4 * self.vdim)) if self.tiled else 0
         self.max_blocks = self.rows // self.unit_tokens + min(self.requests, self.rows)
         if self.max_blocks > MOST_BLOCKS:
             raise ValueError(f"{self.rows} rows of {group} heads to a key/value head are more than a pass divides")
@@ -119,52 +123,54 @@ class RaggedPass:
         a slot, and rows beyond the pass's are left out; check_status() then raises."""
         n = slots.numel()
         for name, t in (("slots", slots), ("new", new), ("lengths", lengths)):
-            if t.dtype is not I32 or t.dim() != 1 or not t.is_contiguous() or t.numel() != n:
+            if t.dtype is not I32 or t.shape != (n,) or not t.is_contiguous():
                 raise ValueError(f"{name} must be contiguous 32-bit integers, one per request")
         if n > self.requests:
             raise ValueError(f"a pass for {self.requests} requests does not take {n}")
-        _table(page_table, n_pages, self.page_tokens)
-        _here((("slots", slots), ("new", new), ("lengths", lengths), ("page_table", page_table), ("the pass", self.header)))
-        lib.check(lib.kernels("stack").ds41_ragged_describe(self.args_ref, C.c_void_p(slots.data_ptr()), C.c_void_p(new.data_ptr()),
-                                                            C.c_void_p(lengths.data_ptr()), n, C.c_void_p(page_table.data_ptr()),
-                                                            page_table.shape[0], page_table.shape[1], n_pages, C.c_void_p(_stream())),
-                  "ds41_ragged_describe")
-        self.table_shape, self.n_pages = page_table.shape, n_pages
+        n_slots, width = shape = page_table.shape if page_table.dim() == 2 else (0, 0)
+        if page_table.dtype is not I32 or n_slots == 0 or width == 0 or not page_table.is_contiguous():
+            raise ValueError("page_table is a contiguous matrix of 32-bit integers, [slots, pages]")
+        if n_pages <= 0 or n_pages * self.page_tokens >= 1 << 31 or width * self.page_tokens >= 1 << 31:
+            raise ValueError("a pool and a request have fewer than 2^31 rows")
+        here = torch.cuda.current_device()
+        if not (slots.get_device() == here and new.get_device() == here and lengths.get_device() == here and page_table.get_device() == here
+                and self.header.get_device() == here):
+            _elsewhere(here, (("slots", slots), ("new", new), ("lengths", lengths), ("page_table", page_table), ("the pass", self.header)))
+        err = lib.kernels("stack").ds41_ragged_describe(self.args_ref, C.c_void_p(slots.data_ptr()), C.c_void_p(new.data_ptr()),
+                                                        C.c_void_p(lengths.data_ptr()), n, C.c_void_p(page_table.data_ptr()), n_slots,
+                                                        width, n_pages, C.c_void_p(_raw_stream(here)))
+        if err:
+            lib.check(err, "ds41_ragged_describe")
+        self.table_shape, self.n_pages = shape, n_pages
         return self.row_pos, self.row_slot, self.row_place
 
     def check_status(self, what: str = "ragged pass"):
         lib.raise_on_status(self.status, what)
 
 
-def _table(page_table: torch.Tensor, n_pages: int, page_tokens: int):
-    if page_table.dtype is not I32 or page_table.dim() != 2 or not page_table.is_contiguous() or page_table.numel() == 0:
-        raise ValueError("page_table is a contiguous matrix of 32-bit integers, [slots, pages]")
-    if n_pages <= 0 or n_pages * page_tokens >= 1 << 31 or page_table.shape[1] * page_tokens >= 1 << 31:
-        raise ValueError("a pool and a request have fewer than 2^31 rows")
-
-
-def _here(tensors):
-    here = torch.cuda.current_device()
+def _elsewhere(here: int, tensors):
     for name, t in tensors:
         if t is not None and t.get_device() != here:
             raise ValueError(f"{name} is on {t.device}, not on the current CUDA device")
 
 
-def _projection(name: str, x: torch.Tensor, rows: int, heads: int, dim: int) -> S.ProjArgs:
-    if x.dim() != 3 or tuple(x.shape) != (rows, heads, dim) or x.dtype not in (BF16, F32):
+def _projection(name: str, x: torch.Tensor, rows: int, heads: int, dim: int) -> Tuple[int, int, int, int, int, int]:
+    shape, dtype = x.shape, x.dtype
+    if shape != (rows, heads, dim) or (dtype is not BF16 and dtype is not F32):
         raise ValueError(f"{name} must be [{rows}, {heads}, {dim}] of bf16 or fp32")
-    row, head, one = _steps(x)
+    row, head, one = x.stride()
     if one != 1 or head != dim or row < heads * dim or row >= 1 << 31:
-        raise ValueError(f"{name}: a row's heads must lie side by side")
-    return S.ProjArgs(x.data_ptr(), 0, row, 1, int(x.dtype == BF16), 0)
+        row, head, one = _steps(x)
+        if one != 1 or head != dim or row < heads * dim or row >= 1 << 31:
+            raise ValueError(f"{name}: a row's heads must lie side by side")
+    return x.data_ptr(), 0, row, 1, dtype is BF16, 0
 
 
-def _weight(name: str, w: Optional[torch.Tensor], heads: int, dim: int) -> int:
-    if w is None:
-        return 0
-    if w.dtype is not F32 or not w.is_contiguous() or tuple(w.shape) not in ((dim,), (heads, dim)):
+def _weight(name: str, w: torch.Tensor, heads: int, dim: int) -> Tuple[int, int]:
+    shape = w.shape
+    if w.dtype is not F32 or not w.is_contiguous() or (shape != (dim,) and shape != (heads, dim)):
         raise ValueError(f"{name} must be contiguous fp32, [{dim}] or [{heads}, {dim}]")
-    return dim if w.dim() == 2 else 0
+    return w.data_ptr(), dim if len(shape) == 2 else 0
 
 
 def heads_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, row_pos: torch.Tensor, row_place: torch.Tensor, pool: torch.Tensor, *,
@@ -173,45 +179,52 @@ def heads_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, row_pos: t
     """Queries [rows, heads, dim] as attention reads them; keys and values go into `pool`.
 
     q, k [rows, kv_heads, dim], v [rows, kv_heads, vdim]: bf16 or fp32, a row's heads side by side.  Every head of q and k becomes
-    x / sqrt(mean(x^2) + eps) * weight where a weight (fp32, [dim], or [heads, dim]) is given, the mean over the first `width` values
+    x / sqrt(mean(x^2) + eps) * weight where a weight (fp32, [dim], or [heads, dim]) is given, the mean over `width` values
     (0: all; the others are padding, zeros); its values j and j + len(freq), j < len(freq), are then turned by row_pos * freq[j].
     pool [pages * page_tokens, kv_heads * (dim + vdim)], bf16 or fp32: row row_place[r] becomes the keys of all heads, then the values.
-    Rows with a negative place are left out.  Two rows with one place leave one of theirs."""
+    Rows with a negative place are left out.  Two rows with one place leave a mixture of theirs."""
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise ValueError("q, k and v are [rows, heads, values]")
-    R, H, D = q.shape
-    G, V = k.shape[1], v.shape[2]
-    if pool.dtype not in (BF16, F32) or pool.dim() != 2 or not pool.is_contiguous() or pool.shape[1] != G * (D + V) or pool.shape[0] == 0 \
-            or pool.shape[0] >= 1 << 31:
-        raise ValueError(f"pool must be contiguous rows of {G * (D + V)} values, bf16 or fp32, fewer than 2^31")
-    if H == 0 or G == 0 or D == 0 or V == 0 or D > 1024 or max(H, G) > 4096 or (H + G) * D > 51200 - 512:
+    (R, H, D), G, V = q.shape, k.shape[1], v.shape[2]
+    if min(H, G, D, V) == 0 or D > 1024 or max(H, G) > 4096 or (H + G) * D > 50688:
         raise ValueError("heads of 1 to 1024 values, of all queries and keys at most 50688")
-    a = HeadsArgs()
-    a.q, a.k, a.v = _projection("q", q, R, H, D), _projection("k", k, R, G, D), _projection("v", v, R, G, V)
-    a.q_norm_stride, a.k_norm_stride = _weight("q_norm", q_norm, H, D), _weight("k_norm", k_norm, G, D)
-    if freq is not None and (freq.dtype is not F32 or freq.dim() != 1 or not freq.is_contiguous() or 2 * freq.numel() > D):
-        raise ValueError(f"freq must be at most {D // 2} contiguous fp32 values")
+    dtype, (pool_rows, columns) = pool.dtype, pool.shape if pool.dim() == 2 else (0, 0)
+    if (dtype is not BF16 and dtype is not F32) or columns != G * (D + V) or not pool.is_contiguous() or not 0 < pool_rows < 1 << 31:
+        raise ValueError(f"pool must be contiguous rows of {G * (D + V)} values, bf16 or fp32, fewer than 2^31")
+    a_q, a_k, a_v = _projection("q", q, R, H, D), _projection("k", k, R, G, D), _projection("v", v, R, G, V)
+    q_weight, q_stride = (None, 0) if q_norm is None else _weight("q_norm", q_norm, H, D)
+    k_weight, k_stride = (None, 0) if k_norm is None else _weight("k_norm", k_norm, G, D)
+    half = 0
+    if freq is not None:
+        half = freq.numel()
+        if freq.dtype is not F32 or freq.dim() != 1 or not freq.is_contiguous() or 2 * half > D:
+            raise ValueError(f"freq must be at most {D // 2} contiguous fp32 values")
     if not 0 <= width <= D or not eps >= 0:
         raise ValueError(f"width is 0 to {D}, eps is not negative")
     for name, t in (("row_pos", row_pos), ("row_place", row_place)):
-        if t.dtype is not I32 or t.dim() != 1 or not t.is_contiguous() or t.numel() < R:
+        if t.dtype is not I32 or t.dim() != 1 or t.numel() < R or not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous 32-bit integers, one per row")
     if out is None:
-        out = torch.empty(R, H, D, dtype=pool.dtype, device=q.device)
-    if tuple(out.shape) != (R, H, D) or out.dtype != pool.dtype:
+        out = torch.empty(R, H, D, dtype=dtype, device=q.device)
+    if out.shape != (R, H, D) or out.dtype is not dtype:
         raise ValueError(f"out must be [{R}, {H}, {D}] of the pool's type")
     row, head, one = _steps(out)
     if one != 1 or head != D or row < H * D:
         raise ValueError("out: a row's heads must lie side by side, rows apart")
-    _here((("q", q), ("k", k), ("v", v), ("row_pos", row_pos), ("row_place", row_place), ("pool", pool), ("q_norm", q_norm),
-           ("k_norm", k_norm), ("freq", freq), ("out", out)))
+    here = torch.cuda.current_device()
+    if not (q.get_device() == here and k.get_device() == here and v.get_device() == here and row_pos.get_device() == here
+            and row_place.get_device() == here and pool.get_device() == here and out.get_device() == here
+            and (q_norm is None or q_norm.get_device() == here) and (k_norm is None or k_norm.get_device() == here)
+            and (freq is None or freq.get_device() == here)):
+        _elsewhere(here, (("q", q), ("k", k), ("v", v), ("row_pos", row_pos), ("row_place", row_place), ("pool", pool), ("out", out),
+                          ("q_norm", q_norm), ("k_norm", k_norm), ("freq", freq)))
     if R == 0:
         return out
-    a.q_norm, a.k_norm, a.freq = lib.ptr(q_norm), lib.ptr(k_norm), lib.ptr(freq)
-    a.row_pos, a.row_place, a.q_out, a.pool = row_pos.data_ptr(), row_place.data_ptr(), out.data_ptr(), pool.data_ptr()
-    a.ld_q, a.eps, a.width, a.rows, a.heads, a.kv_heads, a.dim, a.vdim = row, eps, width or D, R, H, G, D, V
-    a.rot_dim, a.pool_rows, a.f32 = 0 if freq is None else 2 * freq.numel(), pool.shape[0], int(pool.dtype == F32)
-    lib.check(lib.kernels("stack").ds41_ragged_heads(C.byref(a), C.c_void_p(_stream())), "ds41_ragged_heads")
+    a = HeadsArgs(a_q, a_k, a_v, q_weight, k_weight, freq.data_ptr() if half else None, row_pos.data_ptr(), row_place.data_ptr(),
+                  out.data_ptr(), pool.data_ptr(), row, eps, q_stride, k_stride, width or D, R, H, G, D, V, 2 * half, pool_rows, dtype is F32)
+    err = lib.kernels("stack").ds41_ragged_heads(C.byref(a), C.c_void_p(_raw_stream(here)))
+    if err:
+        lib.check(err, "ds41_ragged_heads")
     return out
 
 
@@ -223,33 +236,49 @@ def attend(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, descri
     tokens' among them.  `sink` [heads] fp32: an extra logit in a head's denominator; `gate` [rows, heads] fp32: a head's result times
     sigmoid(gate).  Rows behind the last request's are left as `out` has them."""
     p = described
-    (q_row, q_head), R = _heads("q", q, p.heads, p.dtype), p.rows
-    if tuple(q.shape) != (R, p.heads, p.dim):
-        raise ValueError(f"q must be [{R}, {p.heads}, {p.dim}]")
+    R, H, D, V, dtype = p.rows, p.heads, p.dim, p.vdim, p.dtype
+    if q.shape != (R, H, D) or q.dtype is not dtype:
+        raise ValueError(f"q must be [{R}, {H}, {D}] of {dtype}")
+    q_row, q_head = _heads("q", q, H, dtype)
+    table_shape = page_table.shape
     if p.table_shape is None:
         raise ValueError("the pass has not been described")
-    if pool.dtype is not p.dtype or pool.dim() != 2 or not pool.is_contiguous() or pool.shape[1] != p.kv_heads * (p.dim + p.vdim) \
-            or pool.data_ptr() % 16:
-        raise ValueError(f"pool must be contiguous rows of {p.kv_heads * (p.dim + p.vdim)} values of {p.dtype}, 16-byte aligned")
-    if pool.shape[0] != p.n_pages * p.page_tokens or page_table.shape != p.table_shape:
+    pool_rows, columns = pool.shape if pool.dim() == 2 else (0, 0)
+    if pool.dtype is not dtype or columns != p.columns or not pool.is_contiguous() or pool.data_ptr() % 16:
+        raise ValueError(f"pool must be contiguous rows of {p.columns} values of {dtype}, 16-byte aligned")
+    if pool_rows != p.n_pages * p.page_tokens or table_shape != p.table_shape:
         raise ValueError(f"the pass was described for {p.n_pages} pages and a page table of {tuple(p.table_shape)}")
-    _table(page_table, p.n_pages, p.page_tokens)
+    if page_table.dtype is not I32 or not page_table.is_contiguous():
+        raise ValueError("page_table is a contiguous matrix of 32-bit integers, [slots, pages]")
     if not scale > 0:
         raise ValueError("scale must be positive")
     if out is None:
-        out = torch.empty(R, p.heads, p.vdim, dtype=p.dtype, device=q.device)
-    if tuple(out.shape) != (R, p.heads, p.vdim) or out.dtype is not p.dtype:
-        raise ValueError(f"out must be [{R}, {p.heads}, {p.vdim}] of {p.dtype}")
+        out = torch.empty(R, H, V, dtype=dtype, device=q.device)
+    if out.shape != (R, H, V) or out.dtype is not dtype:
+        raise ValueError(f"out must be [{R}, {H}, {V}] of {dtype}")
     step, head, one = _steps(out)
-    if one != 1 or head != p.vdim or step % 8 or step < p.heads * p.vdim or out.data_ptr() % 16:
+    out_at = out.data_ptr()
+    if one != 1 or head != V or step % 8 or step < H * V or out_at % 16:
         raise ValueError("out must be 16-byte aligned, a row's heads side by side and rows apart, at multiples of 8 values")
-    if sink is not None and (sink.dtype is not F32 or tuple(sink.shape) != (p.heads,) or not sink.is_contiguous()):
-        raise ValueError(f"sink must be {p.heads} contiguous fp32 values")
-    if gate is not None and (gate.dtype is not F32 or tuple(gate.shape) != (R, p.heads) or (p.heads > 1 and gate.stride(1) != 1)):
-        raise ValueError(f"gate must be fp32 [{R}, {p.heads}] with a row's values side by side")
-    _here((("q", q), ("pool", pool), ("page_table", page_table), ("out", out), ("sink", sink), ("gate", gate), ("the pass", p.header)))
-    a = AttendArgs(q.data_ptr(), pool.data_ptr(), page_table.data_ptr(), out.data_ptr(), None if gate is None else gate.data_ptr(),
-                   None if sink is None else sink.data_ptr(), q_row, q_head, step, 0 if gate is None else gate.stride(0), scale, R,
-                   page_table.shape[1], p.n_pages)
-    lib.check(lib.kernels("stack").ds41_ragged_attend(C.byref(a), p.args_ref, C.c_void_p(_stream())), "ds41_ragged_attend")
+    sink_at = gate_at = None
+    gate_row = 0
+    if sink is not None:
+        if sink.dtype is not F32 or sink.shape != (H,) or not sink.is_contiguous():
+            raise ValueError(f"sink must be {H} contiguous fp32 values")
+        sink_at = sink.data_ptr()
+    if gate is not None:
+        gate_row, one = gate.stride() if gate.dim() == 2 else (0, 0)
+        if gate.dtype is not F32 or gate.shape != (R, H) or (H > 1 and one != 1):
+            raise ValueError(f"gate must be fp32 [{R}, {H}] with a row's values side by side")
+        gate_at = gate.data_ptr()
+    here = torch.cuda.current_device()
+    if not (q.get_device() == here and pool.get_device() == here and page_table.get_device() == here and out.get_device() == here
+            and p.header.get_device() == here and (sink is None or sink.get_device() == here) and (gate is None or gate.get_device() == here)):
+        _elsewhere(here, (("q", q), ("pool", pool), ("page_table", page_table), ("out", out), ("the pass", p.header), ("sink", sink),
+                          ("gate", gate)))
+    a = AttendArgs(q.data_ptr(), pool.data_ptr(), page_table.data_ptr(), out_at, gate_at, sink_at, q_row, q_head, step, gate_row, scale, R,
+                   table_shape[1], p.n_pages)
+    err = lib.kernels("stack").ds41_ragged_attend(C.byref(a), p.args_ref, C.c_void_p(_raw_stream(here)))
+    if err:
+        lib.check(err, "ds41_ragged_attend")
     return out
