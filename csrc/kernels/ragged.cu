@@ -8,6 +8,7 @@
 #include <atomic>
 #include <climits>
 
+#include "ds41_prefix.cuh"
 #include "ds41_ragged.cuh"
 #include "ds41_tma.h"
 
@@ -354,14 +355,22 @@ __global__ void __launch_bounds__(kHeadsThreads) ragged_heads_kernel(const ds41_
 // part eight and the eight that they turn with, else neighbours; as many lanes as a head has sixteens (or the next power of two) share
 // it.  A warp takes `per` steps of one row, in each of which its lanes have neighbouring heads, and keeps its lanes' turns and weights.
 // Bound by memory: what is read and written is read and written once, in whole lines.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  return d;
+}
+// Sixteen values as two rows of eight, in pairs.
 struct Sixteen {
-  float v[16];
+  float2 a[4], b[4];
 };
 template <bool PACKED>
 struct RawSixteen {
   uint4 a, b;
-  __device__ __forceinline__ void load(const ds41_proj& p, long long r, int ca, int cb) {
-    const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(p.data) + r * p.ld + p.col;
+  __device__ __forceinline__ void load(const ds41_proj& p, long long at, int ca, int cb) {
+    const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(p.data) + at;
     a = *reinterpret_cast<const uint4*>(row + ca);
     b = *reinterpret_cast<const uint4*>(row + cb);
   }
@@ -369,9 +378,9 @@ struct RawSixteen {
     const uint32_t q[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
     Sixteen x;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x.v[2 * i] = __uint_as_float(q[i] << 16);
-      x.v[2 * i + 1] = __uint_as_float(q[i] & 0xffff0000u);
+    for (int i = 0; i < 4; ++i) {
+      x.a[i] = make_float2(__uint_as_float(q[i] << 16), __uint_as_float(q[i] & 0xffff0000u));
+      x.b[i] = make_float2(__uint_as_float(q[4 + i] << 16), __uint_as_float(q[4 + i] & 0xffff0000u));
     }
     return x;
   }
@@ -379,153 +388,182 @@ struct RawSixteen {
 template <>
 struct RawSixteen<false> {
   float4 q[4];
-  __device__ __forceinline__ void load(const ds41_proj& p, long long r, int ca, int cb) {
-    q[0] = proj_at4(p, r, ca);
-    q[1] = proj_at4(p, r, ca + 4);
-    q[2] = proj_at4(p, r, cb);
-    q[3] = proj_at4(p, r, cb + 4);
+  __device__ __forceinline__ void load(const ds41_proj& p, long long at, int ca, int cb) {
+    ds41_proj row = p;
+    row.col = 0;
+    row.data = p.bf16 ? static_cast<const void*>(static_cast<const __nv_bfloat16*>(p.data) + at)
+                      : static_cast<const void*>(static_cast<const float*>(p.data) + at);
+    q[0] = proj_at4(row, 0, ca);
+    q[1] = proj_at4(row, 0, ca + 4);
+    q[2] = proj_at4(row, 0, cb);
+    q[3] = proj_at4(row, 0, cb + 4);
   }
   __device__ __forceinline__ Sixteen get() const {
     Sixteen x;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x.v[4 * i] = q[i].x;
-      x.v[4 * i + 1] = q[i].y;
-      x.v[4 * i + 2] = q[i].z;
-      x.v[4 * i + 3] = q[i].w;
+    for (int i = 0; i < 2; ++i) {
+      x.a[2 * i] = make_float2(q[i].x, q[i].y);
+      x.a[2 * i + 1] = make_float2(q[i].z, q[i].w);
+      x.b[2 * i] = make_float2(q[2 + i].x, q[2 + i].y);
+      x.b[2 * i + 1] = make_float2(q[2 + i].z, q[2 + i].w);
     }
     return x;
   }
 };
-__device__ __forceinline__ void store_eight(float* to, const float* v) {
-  store4(to, make_float4(v[0], v[1], v[2], v[3]));
-  store4(to + 4, make_float4(v[4], v[5], v[6], v[7]));
+__device__ __forceinline__ void store_eight(float* to, const float2 (&v)[4]) {
+  store4(to, make_float4(v[0].x, v[0].y, v[1].x, v[1].y));
+  store4(to + 4, make_float4(v[2].x, v[2].y, v[3].x, v[3].y));
 }
-__device__ __forceinline__ void store_eight(__nv_bfloat16* to, const float* v) {
+__device__ __forceinline__ void store_eight(__nv_bfloat16* to, const float2 (&v)[4]) {
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const __nv_bfloat162 q = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+    const __nv_bfloat162 q = __float22bfloat162_rn(v[i]);
     w[i] = *reinterpret_cast<const uint32_t*>(&q);
   }
   *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 struct HeadsSteps {
-  int lanes;                 // to a head
   int q, qk, all;            // steps of queries, of queries and keys, and with the values
   int per, parts;            // steps of a warp, warps of a row
+  float inverse;             // 1 / width
 };
 
-template <typename T, bool PACKED>
-__global__ void __launch_bounds__(kHeadsThreads) ragged_heads_wide_kernel(const ds41_ragged_heads_args p, const HeadsSteps h) {
+template <typename T, bool PACKED, int LANES>
+__global__ void __launch_bounds__(kHeadsThreads, PACKED ? 3 : 2) ragged_heads_wide_kernel(const ds41_ragged_heads_args p, const HeadsSteps h) {
   extern __shared__ __align__(16) float2 rw_turns[];     // [warps][rot_dim / 2]
+  constexpr int kStep = 32 / LANES;                      // heads of a step
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = p.rot_dim / 2;
-  const int G = p.kv_heads, D = p.dim, V = p.vdim, per_step = 32 / h.lanes, unit = lane % h.lanes;
-  const long long w = 1ll * blockIdx.x * (kHeadsThreads / 32) + warp;
+  const int G = p.kv_heads, D = p.dim, unit = lane % LANES, own = lane / LANES;
+  const unsigned w = blockIdx.x * (kHeadsThreads / 32) + warp;
   const int r = static_cast<int>(w / h.parts), s0 = static_cast<int>(w % h.parts) * h.per, s1 = min(h.all, s0 + h.per);
-  const bool turned = 16 * unit < p.rot_dim;
+  const bool inside = 16 * unit < D, turned = 16 * unit < p.rot_dim;
   const int ca = turned ? 8 * unit : 16 * unit, cb = turned ? half + 8 * unit : ca + 8;
   pdl_launch_dependents();
   pdl_wait();
   if (r >= p.rows) return;
   const int place = p.row_place[r], pos = p.row_pos[r];
-  // step s of this lane: which projection, its columns there
+  const bool turns = half > 0 && s0 < h.qk;
+  const float freq = turns && lane < half ? p.freq[lane] : 0.f;
+  const long long q_at = 1ll * r * p.q.ld + p.q.col, k_at = 1ll * r * p.k.ld + p.k.col, v_at = 1ll * r * p.v.ld + p.v.col;
+  // this lane's head at a step of queries or keys
+  auto head = [&](int s) { return (s - (s < h.q ? 0 : h.q)) * kStep + own; };
+  auto lives = [&](int s) { return inside && head(s) < (s < h.q ? p.heads : G); };
   auto fetch = [&](int s, RawSixteen<PACKED>& raw) {
-    if (s < h.qk) {
-      const bool key = s >= h.q;
-      const int g = (s - (key ? h.q : 0)) * per_step + lane / h.lanes;
-      if (16 * unit < D && g < (key ? G : p.heads)) raw.load(key ? p.k : p.q, r, g * D + ca, g * D + cb);
+    if (s < h.q) {
+      if (lives(s)) raw.load(p.q, q_at + head(s) * D, ca, cb);
+    } else if (s < h.qk) {
+      if (lives(s)) raw.load(p.k, k_at + head(s) * D, ca, cb);
     } else {
-      const int c = ((s - h.qk) * 32 + lane) * 16;
-      if (c < G * V) raw.load(p.v, r, c, c + 8);
+      const int c = (s - h.qk) * 512 + 16 * lane;
+      if (c < G * p.vdim) raw.load(p.v, v_at + c, 0, 8);
     }
   };
+  // what the first step needs is asked for before any of it is looked at
   RawSixteen<PACKED> next;
   fetch(s0, next);
+  Sixteen weight;
+  auto weights = [&](int s) {
+    const float* norm = s < h.q ? p.q_norm : p.k_norm;
+    if (norm == nullptr || !lives(s)) return;
+    norm += 1ll * head(s) * (s < h.q ? p.q_norm_stride : p.k_norm_stride);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      weight.a[e] = *reinterpret_cast<const float2*>(norm + ca + 2 * e);
+      weight.b[e] = *reinterpret_cast<const float2*>(norm + cb + 2 * e);
+    }
+  };
+  if (s0 < h.qk) weights(s0);
   if (place < 0 || place >= p.pool_rows) return;
-  float2 turn[8];
-  if (half > 0 && s0 < h.qk) {
+  float2 cosine[4], sine[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) cosine[e] = make_float2(1.f, 1.f), sine[e] = make_float2(0.f, 0.f);
+  if (turns) {
     float2* mine = rw_turns + warp * half;
-    for (int i = lane; i < half; i += 32) mine[i] = turn_at(pos, p.freq[i]);
+    if (lane < half) mine[lane] = turn_at(pos, freq);
+    for (int i = lane + 32; i < half; i += 32) mine[i] = turn_at(pos, p.freq[i]);
     __syncwarp();
+    if (turned)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) turn[e] = turned ? mine[8 * unit + e] : make_float2(1.f, 0.f);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) turn[e] = make_float2(1.f, 0.f);
+      for (int e = 0; e < 4; ++e) {
+        const float4 t = *reinterpret_cast<const float4*>(mine + 8 * unit + 2 * e);
+        cosine[e] = make_float2(t.x, t.z);
+        sine[e] = make_float2(t.y, t.w);
+      }
   }
-  T* row = static_cast<T*>(p.pool) + 1ll * place * (G * (D + V));
+  T* row = static_cast<T*>(p.pool) + 1ll * place * (G * (D + p.vdim));
   T* q = static_cast<T*>(p.q_out) + r * p.ld_q;
-  float weight[16];
-  bool first = true;
   for (int s = s0; s < s1; ++s) {
     Sixteen x = next.get();
     if (s + 1 < s1) fetch(s + 1, next);
     if (s >= h.qk) {
-      const int c = ((s - h.qk) * 32 + lane) * 16;
-      if (c < G * V) {
-        store_eight(row + G * D + c, x.v);
-        store_eight(row + G * D + c + 8, x.v + 8);
+      const int c = (s - h.qk) * 512 + 16 * lane;
+      if (c < G * p.vdim) {
+        store_eight(row + G * D + c, x.a);
+        store_eight(row + G * D + c + 8, x.b);
       }
       continue;
     }
-    const bool key = s >= h.q;
-    const int g = (s - (key ? h.q : 0)) * per_step + lane / h.lanes;
-    const bool live = 16 * unit < D && g < (key ? G : p.heads);
-    const float* norm = key ? p.k_norm : p.q_norm;
-    const int stride = key ? p.k_norm_stride : p.q_norm_stride;
-    if (norm != nullptr) {
-      if (first || s == h.q || stride > 0) {
-        if (live) {
-          const float* at = norm + 1ll * g * stride;
+    // the last queries' step may leave lanes without a head that have one among the keys
+    if (s > s0 && (s == h.q || (s < h.q ? p.q_norm_stride : p.k_norm_stride) > 0)) weights(s);
+    const bool live = lives(s);
+    if ((s < h.q ? p.q_norm : p.k_norm) != nullptr) {
+      float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float4 u = *reinterpret_cast<const float4*>(at + ca + 4 * e), v = *reinterpret_cast<const float4*>(at + cb + 4 * e);
-            weight[4 * e] = u.x, weight[4 * e + 1] = u.y, weight[4 * e + 2] = u.z, weight[4 * e + 3] = u.w;
-            weight[8 + 4 * e] = v.x, weight[9 + 4 * e] = v.y, weight[10 + 4 * e] = v.z, weight[11 + 4 * e] = v.w;
-          }
-        }
-        first = !live;                                   // a lane without a head here may have one in a later step
+      for (int e = 0; e < 4; ++e) sum = fma2(x.b[e], x.b[e], fma2(x.a[e], x.a[e], sum));
+      float all = live ? sum.x + sum.y : 0.f;
+#pragma unroll
+      for (int o = LANES / 2; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+      const float f = rsqrtf(all * h.inverse + p.eps);
+      const float2 f2 = make_float2(f, f);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x.a[e] = mul2(mul2(x.a[e], f2), weight.a[e]);
+        x.b[e] = mul2(mul2(x.b[e], f2), weight.b[e]);
       }
-      float sum = 0.f;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) sum += x.v[e] * x.v[e];
-      sum = live ? sum : 0.f;
-      for (int o = h.lanes / 2; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      const float f = 1.0f / sqrtf(sum / p.width + p.eps);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) x.v[e] *= f * weight[e];
     }
-    if (!live) continue;
-    float y[16];
+    if (turned) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      y[e] = x.v[e] * turn[e].x - x.v[8 + e] * turn[e].y;
-      y[8 + e] = x.v[8 + e] * turn[e].x + x.v[e] * turn[e].y;
+      for (int e = 0; e < 4; ++e) {
+        const float2 u = x.a[e], v = x.b[e], minus = make_float2(-sine[e].x, -sine[e].y);
+        x.a[e] = fma2(u, cosine[e], mul2(v, minus));
+        x.b[e] = fma2(v, cosine[e], mul2(u, sine[e]));
+      }
     }
-    T* to = key ? row + g * D : q + 1ll * g * D;
-    store_eight(to + ca, y);
-    store_eight(to + cb, y + 8);
+    if (live) {
+      T* to = (s < h.q ? q : row) + head(s) * D;
+      store_eight(to + ca, x.a);
+      store_eight(to + cb, x.b);
+    }
   }
 }
 
-template <typename T, bool PACKED>
-cudaError_t launch_heads_wide(const ds41_ragged_heads_args& a, cudaStream_t st) {
+template <typename T, bool PACKED, int LANES>
+cudaError_t launch_heads_lanes(const ds41_ragged_heads_args& a, cudaStream_t st) {
   HeadsSteps h{};
-  h.lanes = 1;
-  while (16 * h.lanes < a.dim) h.lanes *= 2;
-  const int per_step = 32 / h.lanes;
-  h.q = (a.heads + per_step - 1) / per_step;
-  h.qk = h.q + (a.kv_heads + per_step - 1) / per_step;
+  constexpr int kStep = 32 / LANES;
+  h.q = (a.heads + kStep - 1) / kStep;
+  h.qk = h.q + (a.kv_heads + kStep - 1) / kStep;
   h.all = h.qk + (a.kv_heads * a.vdim + 511) / 512;
-  // few rows: a warp for every step; many: whole rows, whose turns are made once
-  h.per = static_cast<int>(std::min<long long>(h.all, std::max<long long>(1, 1ll * a.rows * h.all / (148 * 48))));
+  h.inverse = 1.f / a.width;
+  // few rows: a warp for every step; many: half of a row, whose turns are made once (8192 rows of 32 and 8 heads: 47.1 us, whole rows 47.6,
+  // thirds 50)
+  h.per = static_cast<int>(std::min<long long>(h.all, std::max<long long>(1, 1ll * a.rows * h.all / (148 * 100))));
   h.parts = (h.all + h.per - 1) / h.per;
   const long long blocks = (1ll * a.rows * h.parts + kHeadsThreads / 32 - 1) / (kHeadsThreads / 32);
-  if (blocks > INT_MAX) return cudaErrorInvalidValue;
+  if (blocks > INT_MAX / 8) return cudaErrorInvalidValue;
   const int smem = kHeadsThreads / 32 * a.rot_dim / 2 * static_cast<int>(sizeof(float2));
-  return launch_pdl(ragged_heads_wide_kernel<T, PACKED>, dim3(static_cast<unsigned>(blocks)), dim3(kHeadsThreads), smem, st, a, h);
+  return launch_pdl(ragged_heads_wide_kernel<T, PACKED, LANES>, dim3(static_cast<unsigned>(blocks)), dim3(kHeadsThreads), smem, st, a, h);
+}
+template <typename T, bool PACKED>
+cudaError_t launch_heads_wide(const ds41_ragged_heads_args& a, cudaStream_t st) {
+  if (a.dim <= 16) return launch_heads_lanes<T, PACKED, 1>(a, st);
+  if (a.dim <= 32) return launch_heads_lanes<T, PACKED, 2>(a, st);
+  if (a.dim <= 64) return launch_heads_lanes<T, PACKED, 4>(a, st);
+  if (a.dim <= 128) return launch_heads_lanes<T, PACKED, 8>(a, st);
+  if (a.dim <= 256) return launch_heads_lanes<T, PACKED, 16>(a, st);
+  return launch_heads_lanes<T, PACKED, 32>(a, st);
 }
 
 inline bool packed_row(const ds41_proj& p) {
