@@ -14,17 +14,19 @@
 
 namespace ds41 {
 
-constexpr int kDescribeThreads = 1024;
+constexpr int kDescribeThreads = 256, kDescribeWarps = kDescribeThreads / 32;
 constexpr int kMostRequests = 4096, kMostBlocks = 8192;
 constexpr int kCandidates = 16, kBins = 256;
 
 struct DescribeArgs {
   const int *slots, *news, *lengths, *page_table;
   int n, n_slots, max_pages, n_pages;
+  int dividers;              // CTAs that divide the work and each write their share of the units; the others describe rows
 };
 
-// Sum of the block's values before this thread's, and of all of them; two numbers of 32 bits in one.
-__device__ __forceinline__ unsigned long long block_scan(unsigned long long v, unsigned long long* warps, unsigned long long& total) {
+// Sum of the block's values before this thread's, and of all of them; two numbers of 32 bits in one.  `sums`: of two calls after one another.
+__device__ __forceinline__ unsigned long long block_scan(unsigned long long v, unsigned long long (&sums)[2][kDescribeWarps], int& turn,
+                                                         unsigned long long& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   unsigned long long x = v;
 #pragma unroll
@@ -32,18 +34,18 @@ __device__ __forceinline__ unsigned long long block_scan(unsigned long long v, u
     const unsigned long long y = __shfl_up_sync(0xffffffffu, x, o);
     if (lane >= o) x += y;
   }
+  turn ^= 1;
+  if (lane == 31) sums[turn][warp] = x;
   __syncthreads();
-  if (lane == 31) warps[warp] = x;
-  __syncthreads();
-  unsigned long long w = warps[lane];                  // as many warps as lanes
+  unsigned long long before = 0;
+  total = 0;
 #pragma unroll
-  for (int o = 1; o < 32; o *= 2) {
-    const unsigned long long y = __shfl_up_sync(0xffffffffu, w, o);
-    if (lane >= o) w += y;
+  for (int w = 0; w < kDescribeWarps; ++w) {
+    const unsigned long long y = sums[turn][w];
+    if (w < warp) before += y;
+    total += y;
   }
-  total = __shfl_sync(0xffffffffu, w, 31);
-  const unsigned long long before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
-  return (warp ? before : 0) + x - v;
+  return before + x - v;
 }
 
 // Last entry of an ascending list that is not above x; list[0] <= x.
@@ -71,8 +73,10 @@ __device__ __forceinline__ int tile_cost(const ds41_ragged_pass& p, int rows) { 
 
 __global__ void __launch_bounds__(kDescribeThreads) ragged_describe_kernel(const ds41_ragged_pass p, const DescribeArgs a) {
   extern __shared__ int rd_smem[];
-  __shared__ unsigned long long warps[32], cost_of[kCandidates];
-  __shared__ int units_of[kCandidates], cells_of[kCandidates], bins[kBins], bin_sums[kBins / 32], longest;
+  __shared__ unsigned long long scans[2][kDescribeWarps];
+  __shared__ float cost_of[kCandidates];
+  __shared__ int units_of[kCandidates], cells_of[kCandidates], bins[kBins], earlier[kBins], bin_sums[kBins / 32], longest, chosen;
+  int scan = 0;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.n, G = p.kv_heads, group = p.heads / p.kv_heads;
   int* row_first = rd_smem;             // [n] of every request: its first row, its first block, tokens, first token's position, slot
   int* block_first = row_first + n;
@@ -84,8 +88,7 @@ __global__ void __launch_bounds__(kDescribeThreads) ragged_describe_kernel(const
   int* first = tiles + p.max_blocks;    // [blocks] first unit of the list by blocks, first cell
   int* cells = first + p.max_blocks;
   pdl_launch_dependents();
-  if (tid < kCandidates) units_of[tid] = cells_of[tid] = 0, cost_of[tid] = 0;
-  if (tid < kBins) bins[tid] = 0;
+  for (int i = tid; i < kBins; i += kDescribeThreads) bins[i] = earlier[i] = 0;
   if (tid == 0) longest = 1;
   pdl_wait();
   unsigned long long base = 0;          // rows, blocks
@@ -103,12 +106,12 @@ __global__ void __launch_bounds__(kDescribeThreads) ragged_describe_kernel(const
     }
     const int wanted = max(count, 0), most = min(wanted, p.rows);
     unsigned long long total;
-    unsigned long long at = block_scan(static_cast<unsigned long long>(most) << 32 | (most + p.unit_tokens - 1) / p.unit_tokens, warps, total);
+    unsigned long long at = block_scan(static_cast<unsigned long long>(most) << 32 | (most + p.unit_tokens - 1) / p.unit_tokens, scans, scan, total);
     // rows beyond the pass's are left out
     const int row = static_cast<int>(min((base + at) >> 32, static_cast<unsigned long long>(p.rows))), kept = min(most, p.rows - row);
     if (kept < wanted && blockIdx.x == 0) bad_argument(p.status, 501, i);
     if (((base + total) >> 32) > static_cast<unsigned>(p.rows))
-      at = block_scan(static_cast<unsigned long long>(kept) << 32 | (kept + p.unit_tokens - 1) / p.unit_tokens, warps, total);
+      at = block_scan(static_cast<unsigned long long>(kept) << 32 | (kept + p.unit_tokens - 1) / p.unit_tokens, scans, scan, total);
     if (i < n) {
       row_first[i] = row;
       block_first[i] = static_cast<int>((base + at) & 0xffffffffu);
@@ -121,8 +124,9 @@ __global__ void __launch_bounds__(kDescribeThreads) ragged_describe_kernel(const
   const int rows = static_cast<int>(base >> 32), blocks = min(static_cast<int>(base & 0xffffffffu), p.max_blocks);
   __syncthreads();
 
-  if (blockIdx.x > 0) {
-    const int r = (blockIdx.x - 1) * kDescribeThreads + tid;
+  const int divider = blockIdx.x;
+  if (divider >= a.dividers) {
+    const int r = (divider - a.dividers) * kDescribeThreads + tid;
     if (r < p.rows) {
       int pos = 0, slot = -1, place = -1;
       if (r < rows) {
@@ -139,7 +143,7 @@ __global__ void __launch_bounds__(kDescribeThreads) ragged_describe_kernel(const
       p.row_place[r] = place;
     }
     // counters of calls that gave up
-    for (int i = r; i < 2 * p.max_blocks * G; i += (gridDim.x - 1) * kDescribeThreads) p.counters[i] = 0;
+    for (int i = r; i < 2 * p.max_blocks * G; i += (gridDim.x - a.dividers) * kDescribeThreads) p.counters[i] = 0;
     return;
   }
 
@@ -171,65 +175,74 @@ __global__ void __launch_bounds__(kDescribeThreads) ragged_describe_kernel(const
     for (int j = 0; j < kCandidates; ++j) d = k == j ? kDivide[j] : d;
     return (longest_walk + d - 1) / d;
   };
-  auto pieces_of = [&](int tiles, int cells, int most_cost) {
-    return max(1, min(tiles, (tiles * tile_cost(p, cells) + most_cost - 1) / most_cost));
+  // the same number wherever it is asked for: a product that is rounded once
+  auto pieces_of = [&](int tiles, int cells, float part) {
+    return max(1, min(tiles, static_cast<int>(ceilf(__fmul_rn(static_cast<float>(tiles * tile_cost(p, cells)), part)))));
   };
-  const int full = p.unit_tokens * group;
-  {
-    static_assert(kDescribeThreads / 32 == 2 * kCandidates, "two warps to a length");
-    const int k = warp % kCandidates, most_cost = limit(k);
+  const float per_full = 1.f / (p.unit_tokens * group);
+  static_assert(kCandidates % kDescribeWarps == 0, "some lengths to a warp");
+  for (int k = warp; k < kCandidates; k += kDescribeWarps) {
+    const float part = 1.f / limit(k);
     int units = 0, parts = 0;
-    unsigned long long cost = 0;                        // whole numbers: the choice is the same every time
-    for (int b = lane + 32 * (warp / kCandidates); b < blocks; b += 64) {
-      const int pieces = pieces_of(tiles[b], cells[b], most_cost);
+    float cost = 0.f;                                   // added in one order: the choice is the same every time
+    for (int b = lane; b < blocks; b += 32) {
+      const int pieces = pieces_of(tiles[b], cells[b], part);
       units += pieces;
-      cost += 1ull * tiles[b] * tile_cost(p, cells[b]) + kUnitCost * pieces;
+      cost += static_cast<float>(tiles[b] * tile_cost(p, cells[b]) + kUnitCost * pieces);
       if (pieces > 1) {
-        parts += min(pieces * cells[b], 1 << 20);
-        cost += kUnitCost * pieces * cells[b] / full;
+        parts += min(pieces * cells[b], 1 << 18);
+        cost += kUnitCost * per_full * static_cast<float>(pieces * cells[b]);
       }
     }
     units = __reduce_add_sync(0xffffffffu, units);
-    parts = __reduce_add_sync(0xffffffffu, min(parts, 1 << 24));
-#pragma unroll
-    for (int o = 16; o; o >>= 1) cost += __shfl_xor_sync(0xffffffffu, cost, o);
-    if (lane == 0 && units > 0) {
-      atomicAdd(&units_of[k], units);
-      atomicAdd(&cells_of[k], min(parts, 1 << 29));
-      atomicAdd(&cost_of[k], cost);
+    parts = __reduce_add_sync(0xffffffffu, min(parts, 1 << 25));
+    cost = warp_sum(cost);
+    if (lane == 0) {
+      units_of[k] = units;
+      cells_of[k] = parts;
+      cost_of[k] = cost;
     }
   }
   __syncthreads();
-  int most_cost;
-  {
-    float time = INFINITY;                              // every warp finds the same
+  if (warp == 0) {
+    float time = INFINITY;
     if (lane < kCandidates && (lane == 0 || (1ll * units_of[lane] * G <= p.max_units && 1ll * cells_of[lane] * G <= p.max_cells))) {
-      const float units = static_cast<float>(units_of[lane]) * G, turns = ceilf(units / p.grid), cost = static_cast<float>(cost_of[lane]) * G;
+      const float units = static_cast<float>(units_of[lane]) * G, turns = ceilf(units / p.grid), cost = cost_of[lane] * G;
       time = fmaxf(static_cast<float>(limit(lane) + kUnitCost), turns * cost / fmaxf(units, 1.f)) + (cells_of[lane] > 0 ? 1.5f * kUnitCost : 0.f);
     }
     float best = time;
 #pragma unroll
     for (int o = 16; o; o >>= 1) best = fminf(best, __shfl_xor_sync(0xffffffffu, best, o));
-    most_cost = limit(__ffs(__ballot_sync(0xffffffffu, time == best)) - 1);
+    const int who = __ffs(__ballot_sync(0xffffffffu, time == best)) - 1;
+    if (lane == 0) chosen = limit(who);
   }
+  __syncthreads();
+  const int most_cost = chosen;
+  const float part = 1.f / most_cost;
   // the longest pieces first
   const int widest = longest_walk < most_cost + kPairTile ? longest_walk : most_cost + kPairTile;
   const float per_cost = (kBins - 1) / static_cast<float>(widest);
   auto bin_of = [&](int cost) { return kBins - 1 - min(kBins - 1, static_cast<int>(cost * per_cost)); };
+  // this CTA's blocks
+  const int share = (blocks + a.dividers - 1) / a.dividers, b_first = min(blocks, divider * share), b_end = min(blocks, b_first + share);
   unsigned long long sums = 0;
   for (int b0 = 0; b0 < blocks; b0 += kDescribeThreads) {
     const int b = b0 + tid;
     int pieces = 0, parts = 0;
     if (b < blocks) {
       const int k = tiles[b], c = tile_cost(p, cells[b]);
-      pieces = pieces_of(k, cells[b], most_cost);
+      pieces = pieces_of(k, cells[b], part);
       parts = pieces > 1 ? pieces * cells[b] * G : 0;
-      const int least = k / pieces, more = k - least * pieces;             // pieces of one tile more than the others
+      const int least = pieces > 1 ? k / pieces : k, more = k - least * pieces;             // pieces of one tile more than the others
       if (more) atomicAdd(&bins[bin_of((least + 1) * c)], more * G);
       atomicAdd(&bins[bin_of(least * c)], (pieces - more) * G);
+      if (b < b_first) {
+        if (more) atomicAdd(&earlier[bin_of((least + 1) * c)], more * G);
+        atomicAdd(&earlier[bin_of(least * c)], (pieces - more) * G);
+      }
     }
     unsigned long long total;
-    const unsigned long long at = sums + block_scan(static_cast<unsigned long long>(pieces * G) << 32 | parts, warps, total);
+    const unsigned long long at = sums + block_scan(static_cast<unsigned long long>(pieces * G) << 32 | parts, scans, scan, total);
     sums += total;
     if (b < blocks) {
       first[b] = static_cast<int>(at >> 32);
@@ -239,26 +252,28 @@ __global__ void __launch_bounds__(kDescribeThreads) ragged_describe_kernel(const
   const int units = static_cast<int>(sums >> 32);
   __syncthreads();
   // where a bin's units begin
-  const int count = tid < kBins ? bins[tid] : 0;
+  static_assert(kBins == kDescribeThreads, "a bin to a thread");
+  const int count = bins[tid];
   int upto = count;
 #pragma unroll
   for (int o = 1; o < 32; o *= 2) {
     const int y = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= o) upto += y;
   }
-  if (tid < kBins && lane == 31) bin_sums[warp] = upto;
+  if (lane == 31) bin_sums[warp] = upto;
   __syncthreads();
-  if (tid < kBins) {
-    int before = 0;
-    for (int w = 0; w < warp; ++w) before += bin_sums[w];
-    bins[tid] = before + upto - count;
-  }
+  int before = 0;
+#pragma unroll
+  for (int w = 0; w < kDescribeWarps; ++w) before += w < warp ? bin_sums[w] : 0;
+  bins[tid] = before + upto - count + earlier[tid];
   __syncthreads();
-  for (int u = tid; u < units; u += kDescribeThreads) {
-    const int b = find_last(first, blocks, u), i = owner[b], k = tiles[b];
+  const bool whole = units == blocks * G;                // no block in pieces
+  const int u_first = b_first < blocks ? first[b_first] : units, u_end = b_end < blocks ? first[b_end] : units;
+  for (int u = u_first + tid; u < u_end; u += kDescribeThreads) {
+    const int b = whole ? u / G : find_last(first, blocks, u), i = owner[b], k = tiles[b];
     const int t0 = (b - block_first[i]) * p.unit_tokens, tk = min(p.unit_tokens, tokens[i] - t0), step = tk * group;
-    const int pieces = pieces_of(k, step, most_cost), x = u - first[b], head = x / pieces, piece = x - head * pieces;
-    const int least = k / pieces, more = k - least * pieces;
+    const int pieces = whole ? 1 : pieces_of(k, step, part), x = u - first[b], head = pieces > 1 ? x / pieces : x, piece = x - head * pieces;
+    const int least = pieces > 1 ? k / pieces : k, more = k - least * pieces;
     const int mine = least + (piece < more), tile0 = piece * least + min(piece, more);
     // one thread asks for all of its warp's of a bin
     const int bin = bin_of(mine * tile_cost(p, step));
@@ -271,7 +286,7 @@ __global__ void __launch_bounds__(kDescribeThreads) ragged_describe_kernel(const
     out[1] = make_int4(head, tile0, mine, piece);
     out[2] = make_int4(pieces, cells[b] + head * pieces * step, 2 * (b * G + head), step);
   }
-  if (tid == 0) {
+  if (divider == 0 && tid == 0) {
     p.header[0] = units;
     p.header[1] = rows;
   }
@@ -817,8 +832,10 @@ extern "C" int ds41_ragged_describe(const ds41_ragged_pass* p, const int* slots,
     if (e != cudaSuccess) return e;
     if (dev < 64) ready.fetch_or(1ull << dev);
   }
-  const DescribeArgs a{slots, news, lengths, page_table, n, n_slots, max_pages, n_pages};
-  const int grid = 1 + (p->rows + kDescribeThreads - 1) / kDescribeThreads;
+  // 456 blocks in 3648 units: 14.1 us with one divider
+  const int dividers = std::min(8, (p->max_blocks + 31) / 32);
+  const DescribeArgs a{slots, news, lengths, page_table, n, n_slots, max_pages, n_pages, dividers};
+  const int grid = dividers + (p->rows + kDescribeThreads - 1) / kDescribeThreads;
   return launch_pdl(ragged_describe_kernel, dim3(grid), dim3(kDescribeThreads), smem, static_cast<cudaStream_t>(stream), *p, a);
 }
 
