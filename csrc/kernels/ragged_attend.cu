@@ -47,7 +47,6 @@ struct TiledShared {
   // per tile:
   uint64_t s_full[2];                          // S complete, and every product before it
   uint64_t p_full[2][2];                       // P written, O rescaled: of the first 96 keys, of the others
-  uint64_t most_done[2];                       // the product with the former is complete
   uint64_t o_full[2];                          // the unit's last product is complete
   uint64_t half_full, half_read[2];            // the second tile's half of a unit whose keys were taken in turn
   float2 half_ml[kRtTurnRows];
@@ -137,14 +136,15 @@ __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 
 // A scheduler's two softmax warps take turns at the exponentials: at the same time they would take each as long as both after one another,
 // and the tensor core would have both tiles' products at once, and none afterwards.  Who has waited long enough goes on without.
 __device__ __forceinline__ void take_turn(int* busy, int lane) {
-  if (lane == 0)
-    for (int i = 0; i < 1024 && atomicCAS(busy, 0, 1) != 0; ++i) {
-    }
+  if (lane == 0) {
+    const uint32_t at = smem_u32(busy);
+    for (int i = 0, was = 1; i < 1024 && was != 0; ++i) asm volatile("atom.shared.cas.b32 %0, [%1], 0, 1;" : "=r"(was) : "r"(at) : "memory");
+  }
   __syncwarp();
 }
 __device__ __forceinline__ void end_turn(int* busy, int lane) {
   __syncwarp();
-  if (lane == 0) atomicExch(busy, 0);
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.eq.b32 q, %1, 0;\n\t@q st.shared.b32 [%0], 0;\n\t}" ::"r"(smem_u32(busy)), "r"(lane) : "memory");
 }
 // All lanes, or one thread by itself.
 #define WARP_WAIT(bar, parity, where) (__all_sync(0xffffffffu, mbar_wait(bar, parity, t.p.status, where)) != 0)
@@ -179,7 +179,6 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
       mbar_init(&sh.s_full[i], 1);
       mbar_init(&sh.p_full[i][0], 4);
       mbar_init(&sh.p_full[i][1], 4);
-      mbar_init(&sh.most_done[i], 1);
       mbar_init(&sh.o_full[i], 1);
       mbar_init(&sh.half_read[i], 4);
     }
@@ -368,7 +367,6 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
           tc_fence_after();
           umma4_ts<128>(o_t, s_t, v, idesc_pv, j > 0);
           umma2_ts<128>(o_t, s_t + 32, v + 512, idesc_pv);
-          tc_commit(&sh.most_done[i]);
           ok = mbar_wait(&sh.p_full[i][1], done & 1, t.p.status, 616);
           if (!ok) break;
           tc_fence_after();
@@ -458,13 +456,12 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
         place_step = x.turns ? 2 * kRtKeys : kRtKeys;
       }
       const bool idle = !__any_sync(0xffffffffu, live);
-      float m = -INFINITY, l = 0.f, after = -INFINITY;   // `after`: largest score of the last tile's last keys
+      float m = -INFINITY, l = 0.f;
       for (int j = 0; j < n; ++j, ++tiles, place0 += place_step) {
         if (ok) ok = WARP_WAIT(&sh.s_full[i], tiles & 1, 630 + i);
         const bool work = ok && !idle;
-        // Weights are relative to the maximum so far.  Where that of the first 96 keys, or of the last tile's others, is above it by more
-        // than 2^8, it is raised and they are taken once more.  The others' product follows one that is under way and has to be
-        // relative to the same maximum: up to 2^64 it is.
+        // Weights are relative to the maximum so far.  Where the tile's is above it by more than 2^8, it is raised and they are taken once
+        // more.
         uint32_t x[2][32], w[32];
         float2 sums[2], neg2;
         auto begin = [&]() {
@@ -482,20 +479,6 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
             sums[k & 1] = add2(sums[k & 1], y);
             const __nv_bfloat162 q = __floats2bfloat162_rn(y.x, y.y);
             w[at + k] = *reinterpret_cast<const uint32_t*>(&q);
-          }
-        };
-        auto raise = [&](float top, bool grow) {           // O and the sum follow
-          const float m_new = grow ? top : m, keep = grow ? (m == -INFINITY ? 0.f : ex2_approx(m - m_new)) : 1.f;
-          l *= keep;
-          m = m_new;
-#pragma unroll 1
-          for (int c = 0; c < vp; c += 16) {
-            uint32_t o[16];
-            tmem_ld_32x16(o_t + c, o);
-            tmem_wait_ld();
-#pragma unroll
-            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
-            tmem_st_32x16(o_t + c, o);
           }
         };
         if (work) {
@@ -530,10 +513,23 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
           top = fmaxf(top, largest(x[1]));
           tmem_ld_32x32(s_t + 96, x[1]);
           tmem_wait_ld(x[0]);
-          top = fmaxf(fmaxf(top, largest(x[0])) * t.scale_log2, after);
+          tmem_wait_ld(x[1]);
+          top = fmaxf(top, fmaxf(largest(x[0]), largest(x[1]))) * t.scale_log2;
           const bool grow = top > m + 8.f;
           if (__any_sync(0xffffffffu, grow)) {
-            raise(top, grow);
+            // O and the sum follow; the products before this tile's are complete
+            const float m_new = grow ? top : m, keep = grow ? (m == -INFINITY ? 0.f : ex2_approx(m - m_new)) : 1.f;
+            l *= keep;
+            m = m_new;
+#pragma unroll 1
+            for (int c = 0; c < vp; c += 16) {
+              uint32_t o[16];
+              tmem_ld_32x16(o_t + c, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
+              tmem_st_32x16(o_t + c, o);
+            }
             tmem_ld_32x32(s_t, x[0]);
             tmem_ld_32x32(s_t + 32, x[1]);
             tmem_wait_ld(x[0]);
@@ -544,14 +540,12 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
             tmem_ld_32x32(s_t + 64, x[0]);
             tmem_ld_32x32(s_t + 96, x[1]);
             tmem_wait_ld(x[0]);
+            tmem_wait_ld(x[1]);
           }
           tmem_st_32x32(s_t, w);                         // columns whose S this thread has read
           weights(x[0], 0, 16, 0);
           tmem_st_32x16(s_t + 32, reinterpret_cast<uint32_t(&)[16]>(w[0]));
           end_turn(&sh.busy[quad], lane);
-          tmem_wait_ld(x[1]);
-          l += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
-          begin();
           weights(x[1], 0, 8, 16);
           tmem_wait_st();
           tc_fence_before();
@@ -560,16 +554,8 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
         mbar_arrive_if(ok && lane == 0, &sh.p_full[i][0]);
         if (work) {
           weights(x[1], 8, 16, 16);
-          after = largest(x[1]) * t.scale_log2;
-          if (__any_sync(0xffffffffu, after > m + 64.f)) {
-            if (ok) ok = WARP_WAIT(&sh.most_done[i], tiles & 1, 632 + i);
-            tc_fence_after();
-            raise(after, after > m + 64.f);
-            begin();
-            weights(x[1], 0, 16, 16);
-          }
-          l += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
           tmem_st_32x16(s_t + 48, reinterpret_cast<uint32_t(&)[16]>(w[16]));
+          l += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
           tmem_wait_st();
           tc_fence_before();
         }
