@@ -24,16 +24,26 @@ __device__ __forceinline__ RaggedUnit ragged_unit(const ds41_ragged_pass& p, int
 __host__ __device__ __forceinline__ int ragged_low(int pos, int window) { return window > 0 && pos >= window ? pos - window + 1 : 0; }
 
 // The keys that rows at p0 .. p1 see, as one row of places: the first `lead` of them are positions 0 .. lead - 1, place v behind them is
-// position v + shift.  Places come in runs of `align`, within which positions follow one another and lie in one page.  A range of first
+// position v + shift.  Places come in runs, within which positions follow one another and lie in one page.  A range of first
 // tokens that reaches the window is a part of it.
 struct RaggedWalk {
   int lead, shift, places;
 };
-__host__ __device__ __forceinline__ RaggedWalk ragged_walk(int p0, int p1, int window, int first, int align) {
-  int base = ragged_low(p0, window);
-  base -= base % align;
+struct Runs {                // of a power of two
+  int mask;
+  __device__ __forceinline__ int down(int x) const { return x & ~mask; }
+  __device__ __forceinline__ int up(int x) const { return (x + mask) & ~mask; }
+};
+struct AnyRuns {
+  int align;
+  __device__ __forceinline__ int down(int x) const { return x - x % align; }
+  __device__ __forceinline__ int up(int x) const { return (x + align - 1) / align * align; }
+};
+template <typename R>
+__device__ __forceinline__ RaggedWalk ragged_walk(int p0, int p1, int window, int first, R runs) {
+  int base = runs.down(ragged_low(p0, window));
   const int f = first < p1 + 1 ? first : p1 + 1;
-  int lead = f > 0 ? (f + align - 1) / align * align : 0;
+  int lead = f > 0 ? runs.up(f) : 0;
   if (lead >= base) {
     if (lead > 0) base = 0;
     lead = 0;

@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(kDescribeThreads) ragged_describe_kernel(const
     const int i = find_last(block_first, n, b), t0 = (b - block_first[i]) * p.unit_tokens, count = min(p.unit_tokens, tokens[i] - t0);
     int k = 0;
     if (slot_of[i] >= 0) {
-      const RaggedWalk w = ragged_walk(begin[i] + t0, begin[i] + t0 + count - 1, p.window, p.first, align);
+      const RaggedWalk w = ragged_walk(begin[i] + t0, begin[i] + t0 + count - 1, p.window, p.first, AnyRuns{align});
       k = (w.places + p.key_tile - 1) / p.key_tile;
     }
     owner[b] = i;
@@ -630,7 +630,7 @@ __global__ void __launch_bounds__(kRaggedThreads) ragged_simple_kernel(const ds4
       }
       continue;
     }
-    const RaggedWalk walk = ragged_walk(u.pos0, u.pos0 + u.tokens - 1, p.window, p.first, align);
+    const RaggedWalk walk = ragged_walk(u.pos0, u.pos0 + u.tokens - 1, p.window, p.first, AnyRuns{align});
     const int v0 = u.tile0 * p.key_tile, v1 = min(walk.places, v0 + u.tiles * p.key_tile);
     for (int r0 = 0; r0 < n; r0 += kSimpleRows) {
       const int rows = min(kSimpleRows, n - r0);

@@ -77,11 +77,13 @@ struct TiledUnit {
 
 __device__ __forceinline__ TiledUnit tiled_unit(const TiledParams& t, int i) {
   TiledUnit x;
+  if (i + static_cast<int>(gridDim.x) < t.p.max_units)   // one of the next ones, or near it
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(t.p.units + 1ll * (i + static_cast<int>(gridDim.x)) * kRaggedInts));
   x.u = ragged_unit(t.p, i);
   const RaggedUnit& u = x.u;
   x.turns = u.tokens * t.group <= t.p.turn_rows;
   x.tok0 = x.turns ? u.tokens : (u.tokens + 1) / 2;
-  x.walk = ragged_walk(u.pos0, u.pos0 + u.tokens - 1, t.p.window, t.p.first, t.box);
+  x.walk = ragged_walk(u.pos0, u.pos0 + u.tokens - 1, t.p.window, t.p.first, Runs{t.box - 1});
   if (x.turns) {
     x.n[0] = (u.tiles + 1) / 2;
     x.n[1] = u.tiles / 2;
@@ -195,6 +197,7 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
   pdl_wait();
+  asm volatile("prefetch.global.L1 [%0];" ::"l"(t.p.units + 1ll * min(static_cast<int>(blockIdx.x), t.p.max_units - 1) * kRaggedInts));
   const int units = t.p.header[0];
 
   if (warp == 8) {
@@ -229,8 +232,27 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
         return static_cast<unsigned>(id) < static_cast<unsigned>(t.a.n_pages) ? id * t.p.page_tokens + (pos - pg * t.p.page_tokens)
                                                                               : t.hidden_row;
       };
+      auto load_queries = [&]() {
+        ok = WARP_WAIT(&sh.q_free, (done & 1) ^ 1, 600);
+        // the second tile's place holds halves of units that went in turns
+        for (int h = max(0, halves - 2); h < halves && ok && !x.turns; ++h) ok = WARP_WAIT(&sh.half_read[h & 1], (h >> 1) & 1, 601);
+        if (!ok) return;
+        const bool second = !x.turns && x.u.tokens > x.tok0;
+        if (lane == 0) mbar_expect_tx(&sh.q_full, (second ? 2 : 1) * t.kd * t.per_tile * t.group * 128);
+        __syncwarp();
+        if (lane < (second ? 2 : 1) * t.kd) {
+          const int k = lane / t.kd, c = lane - k * t.kd;
+          tma_load_3d(s_q + k * q_bytes + c * kRtChunk, &queries, &sh.q_full, 64 * c, x.u.head * t.group, x.u.row0 + k * x.tok0);
+        }
+        ++done;
+        if (x.turns && n > 1) ++halves;
+      };
+      // The first unit's queries before its keys; later ones behind as many key tiles as there are places for, as those do not wait for
+      // the last unit's queries.
+      const int q_after = done == 0 ? 0 : min(n, t.k_stages);
+      if (n > 0 && q_after == 0) load_queries();
       int k_next = n > 0 ? locate(0, k_box, k_copies) : 0, v_next = n > 0 ? locate(0, v_box, v_copies) : 0;
-      for (int s = 0; s < n; ++s) {
+      for (int s = 0; s < n && ok; ++s) {
         const int k_row = k_next, v_later = v_next;
         if (s + 1 < n) {
           k_next = locate(s + 1, k_box, k_copies);
@@ -251,22 +273,7 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
         behind = true;
         v_row = v_later;
         v_col = t.p.kv_heads * dp + x.u.head * vp + 64 * v_chunk;
-        // queries behind as many key tiles as there are places for: those do not wait for the last unit's queries
-        if (s + 1 == min(n, t.k_stages)) {
-          ok = WARP_WAIT(&sh.q_free, (done & 1) ^ 1, 600);
-          // the second tile's place holds halves of units that went in turns
-          for (int h = max(0, halves - 2); h < halves && ok && !x.turns; ++h) ok = WARP_WAIT(&sh.half_read[h & 1], (h >> 1) & 1, 601);
-          if (!ok) break;
-          const bool second = !x.turns && x.u.tokens > x.tok0;
-          if (lane == 0) mbar_expect_tx(&sh.q_full, (second ? 2 : 1) * t.kd * t.per_tile * t.group * 128);
-          __syncwarp();
-          if (lane < (second ? 2 : 1) * t.kd) {
-            const int k = lane / t.kd, c = lane - k * t.kd;
-            tma_load_3d(s_q + k * q_bytes + c * kRtChunk, &queries, &sh.q_full, 64 * c, x.u.head * t.group, x.u.row0 + k * x.tok0);
-          }
-          ++done;
-          if (x.turns && n > 1) ++halves;
-        }
+        if (s + 1 == q_after) load_queries();
       }
     }
     if (ok && behind) values();
@@ -423,15 +430,21 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
     const uint32_t o_t = tmem + lanes + 256 + i * 128;
     const int mine_tok = mine / t.group, mine_head = mine - mine_tok * t.group;
-    const uint32_t s_t = tmem + lanes + i * 128;
     const float2 scale2 = make_float2(t.scale_log2, t.scale_log2);
+    // a row of the second tile's half, each beginning at another column, so that neighbours do not meet in a bank
+    float4* const half = reinterpret_cast<float4*>(s_q + q_bytes) + mine * (vp / 4);
+    const int turned = mine % (vp / 4);
     int tiles = 0, outputs = 0, halves = 0;
     bool ok = true;
-    for (int turn = 0; unit_at(turn) < units; ++turn) {
+    // Before the first unit one tile of whatever the output's columns hold, into them, while the first keys are on their way:
+    // instructions that run for the first time are waited for, 2 us of a small call.
+    for (int turn = -1; turn < 0 || unit_at(turn) < units; ++turn) {
+      const bool rehearsal = turn < 0;
       // Of this thread's row: visible are the places [0, a) and [b, e); of all of its warp's rows up to a_all, from b_all to e_all.
-      int n, a, b, e, a_all, b_all, e_all, place0, place_step;
-      bool live;
-      {
+      int n = 1, a = 0, b = 0, e = 0, a_all = 0, b_all = 0, e_all = 0, place0 = 0, place_step = 0;
+      bool live = true;
+      float sink = -INFINITY, gate = 0.f;                // asked for long before they are needed
+      if (!rehearsal) {
         const TiledUnit x = tiled_unit(t, unit_at(turn));
         const RaggedUnit& u = x.u;
         if (u.tiles == 0) {
@@ -454,11 +467,15 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
         n = x.n[i];
         place0 = (u.tile0 + (x.turns ? i : 0)) * kRtKeys;
         place_step = x.turns ? 2 * kRtKeys : kRtKeys;
+        const int h = u.head * t.group + mine_head, row = u.row0 + (i && !x.turns ? x.tok0 : 0) + mine_tok;
+        if (live && t.a.sink != nullptr) sink = t.a.sink[h] * kLog2E;
+        if (live && t.a.gate != nullptr) gate = t.a.gate[row * t.a.gate_row + h];
       }
       const bool idle = !__any_sync(0xffffffffu, live);
       float m = -INFINITY, l = 0.f;
+      const uint32_t s_t = rehearsal ? o_t : tmem + lanes + i * 128;
       for (int j = 0; j < n; ++j, ++tiles, place0 += place_step) {
-        if (ok) ok = WARP_WAIT(&sh.s_full[i], tiles & 1, 630 + i);
+        if (ok && !rehearsal) ok = WARP_WAIT(&sh.s_full[i], tiles & 1, 630 + i);
         const bool work = ok && !idle;
         // Weights are relative to the maximum so far.  Where the tile's is above it by more than 2^8, it is raised and they are taken once
         // more.
@@ -551,7 +568,7 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
           tc_fence_before();
         }
         __syncwarp();
-        mbar_arrive_if(ok && lane == 0, &sh.p_full[i][0]);
+        mbar_arrive_if(ok && !rehearsal && lane == 0, &sh.p_full[i][0]);
         if (work) {
           weights(x[1], 8, 16, 16);
           tmem_st_32x16(s_t + 48, reinterpret_cast<uint32_t(&)[16]>(w[16]));
@@ -560,7 +577,11 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
           tc_fence_before();
         }
         __syncwarp();
-        mbar_arrive_if(ok && lane == 0, &sh.p_full[i][1]);
+        mbar_arrive_if(ok && !rehearsal && lane == 0, &sh.p_full[i][1]);
+      }
+      if (rehearsal) {
+        tiles = 0;
+        continue;
       }
       if (n > 0) {
         if (ok) ok = WARP_WAIT(&sh.o_full[i], outputs & 1, 634 + i);
@@ -575,18 +596,19 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
         if (u.tiles > 1) {
           if (halves > 0 && ok) ok = WARP_WAIT(&sh.half_read[(halves - 1) & 1], ((halves - 1) >> 1) & 1, 634);
           if (!idle) {
-            float4* to = reinterpret_cast<float4*>(s_q + q_bytes) + mine * (vp / 4);
+            int at = turned;
 #pragma unroll 1
-            for (int c = 0; c < vp; c += 16) {
-              uint32_t o[16];
+            for (int c = 0; c < vp; c += 32) {             // behind the last column lies something of no use
+              uint32_t o[32];
               __syncwarp();
-              tmem_ld_32x16(o_t + c, o);
-              tmem_wait_ld();
-              if (live)
+              tmem_ld_32x32(o_t + c, o);
+              tmem_wait_ld(o);
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  to[(c / 4 + k + mine) % (vp / 4)] = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]),
-                                                                  __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
+              for (int k = 0; k < 8; ++k) {
+                if (live && c + 4 * k < vp) half[at] = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]),
+                                                                   __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
+                at = at + 1 < vp / 4 ? at + 1 : 0;
+              }
             }
             if (live) sh.half_ml[mine] = make_float2(m, l);
           }
@@ -598,7 +620,6 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
         continue;
       }
       float w_own = 1.f, w_half = 0.f;                   // factors of both halves
-      const float4* half = reinterpret_cast<const float4*>(s_q + q_bytes) + mine * (vp / 4);
       const bool joined = x.turns && u.tiles > 1;
       if (joined) {
         if (ok) ok = WARP_WAIT(&sh.half_full, halves & 1, 635);
@@ -618,48 +639,54 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
         cell = 1ll * u.cell + 1ll * u.piece * u.step + first_tok * t.group + mine;
         if (live) *reinterpret_cast<float2*>(t.p.part_ml + 2 * cell) = make_float2(m, l);
       } else if (live) {
-        const float sink = t.a.sink != nullptr ? t.a.sink[h] * kLog2E : -INFINITY;
         const float top = fmaxf(m, sink), base = top == -INFINITY ? 0.f : top;
         const float w = ex2_approx(m - base), den = l * w + (t.a.sink != nullptr ? ex2_approx(sink - base) : 0.f);
         f = den != 0.f ? w / den : 0.f;
-        if (t.a.gate != nullptr) f *= sigmoid_f32(t.a.gate[row * t.a.gate_row + h]);
+        if (t.a.gate != nullptr) f *= sigmoid_f32(gate);
       }
       w_own *= f;
       w_half *= f;
       if (!idle && n > 0) {
+        float4* part = reinterpret_cast<float4*>(t.p.part_o + cell * vp);
+        uint4* out = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(t.a.out) + row * t.a.out_row + 1ll * h * vp);
+        int at = turned;
 #pragma unroll 1
-        for (int c = 0; c < vp; c += 16) {
-          uint32_t o[16];
+        for (int c = 0; c < vp; c += 32, part += 8, out += 4) {
+          uint32_t o[32];
           __syncwarp();
-          tmem_ld_32x16(o_t + c, o);
-          tmem_wait_ld();
-          float y[16];
-#pragma unroll
-          for (int k = 0; k < 16; ++k) y[k] = __uint_as_float(o[k]) * w_own;
-          if (live && joined) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float4 z = half[(c / 4 + k + mine) % (vp / 4)];
-              y[4 * k] += z.x * w_half;
-              y[4 * k + 1] += z.y * w_half;
-              y[4 * k + 2] += z.z * w_half;
-              y[4 * k + 3] += z.w * w_half;
-            }
-          }
-          if (live && u.pieces > 1) {
-            float4* to = reinterpret_cast<float4*>(t.p.part_o + cell * vp + c);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) to[k] = make_float4(y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]);
-          } else if (live) {
-            uint32_t w[8];
+          tmem_ld_32x32(o_t + c, o);
+          tmem_wait_ld(o);
+          if (joined) {
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-              const __nv_bfloat162 q = __floats2bfloat162_rn(y[2 * k], y[2 * k + 1]);
-              w[k] = *reinterpret_cast<const uint32_t*>(&q);
+              const float4 z = live ? half[at] : make_float4(0.f, 0.f, 0.f, 0.f);
+              at = at + 1 < vp / 4 ? at + 1 : 0;
+              o[4 * k] = __float_as_uint(__uint_as_float(o[4 * k]) * w_own + z.x * w_half);
+              o[4 * k + 1] = __float_as_uint(__uint_as_float(o[4 * k + 1]) * w_own + z.y * w_half);
+              o[4 * k + 2] = __float_as_uint(__uint_as_float(o[4 * k + 2]) * w_own + z.z * w_half);
+              o[4 * k + 3] = __float_as_uint(__uint_as_float(o[4 * k + 3]) * w_own + z.w * w_half);
             }
-            uint4* to = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(t.a.out) + row * t.a.out_row + 1ll * h * vp + c);
-            to[0] = make_uint4(w[0], w[1], w[2], w[3]);
-            to[1] = make_uint4(w[4], w[5], w[6], w[7]);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * w_own);
+          }
+          if (!live) {
+          } else if (u.pieces > 1) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if (c + 4 * k < vp) part[k] = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]), __uint_as_float(o[4 * k + 2]),
+                                                        __uint_as_float(o[4 * k + 3]));
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const __nv_bfloat162 q = __floats2bfloat162_rn(__uint_as_float(o[8 * k + 2 * e]), __uint_as_float(o[8 * k + 2 * e + 1]));
+                w[e] = *reinterpret_cast<const uint32_t*>(&q);
+              }
+              if (c + 8 * k < vp) out[k] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
           }
         }
         __syncwarp();
