@@ -428,7 +428,7 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
     // Where a wait gave up, `ok` stays false and later ones are left out, but every barrier that warps share is reached.
     const int i = warp >> 2, quad = warp & 3, mine = quad * 32 + lane, tid = mine;
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
-    const uint32_t o_t = tmem + lanes + 256 + i * 128;
+    const uint32_t s_t = tmem + lanes + i * 128, o_t = tmem + lanes + 256 + i * 128;
     const int mine_tok = mine / t.group, mine_head = mine - mine_tok * t.group;
     const float2 scale2 = make_float2(t.scale_log2, t.scale_log2);
     // a row of the second tile's half, each beginning at another column, so that neighbours do not meet in a bank
@@ -436,15 +436,12 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
     const int turned = mine % (vp / 4);
     int tiles = 0, outputs = 0, halves = 0;
     bool ok = true;
-    // Before the first unit one tile of whatever the output's columns hold, into them, while the first keys are on their way:
-    // instructions that run for the first time are waited for, 2 us of a small call.
-    for (int turn = -1; turn < 0 || unit_at(turn) < units; ++turn) {
-      const bool rehearsal = turn < 0;
+    for (int turn = 0; unit_at(turn) < units; ++turn) {
       // Of this thread's row: visible are the places [0, a) and [b, e); of all of its warp's rows up to a_all, from b_all to e_all.
-      int n = 1, a = 0, b = 0, e = 0, a_all = 0, b_all = 0, e_all = 0, place0 = 0, place_step = 0;
-      bool live = true;
+      int n, a, b, e, a_all, b_all, e_all, place0, place_step;
+      bool live;
       float sink = -INFINITY, gate = 0.f;                // asked for long before they are needed
-      if (!rehearsal) {
+      {
         const TiledUnit x = tiled_unit(t, unit_at(turn));
         const RaggedUnit& u = x.u;
         if (u.tiles == 0) {
@@ -473,9 +470,8 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
       }
       const bool idle = !__any_sync(0xffffffffu, live);
       float m = -INFINITY, l = 0.f;
-      const uint32_t s_t = rehearsal ? o_t : tmem + lanes + i * 128;
       for (int j = 0; j < n; ++j, ++tiles, place0 += place_step) {
-        if (ok && !rehearsal) ok = WARP_WAIT(&sh.s_full[i], tiles & 1, 630 + i);
+        if (ok) ok = WARP_WAIT(&sh.s_full[i], tiles & 1, 630 + i);
         const bool work = ok && !idle;
         // Weights are relative to the maximum so far.  Where the tile's is above it by more than 2^8, it is raised and they are taken once
         // more.
@@ -568,7 +564,7 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
           tc_fence_before();
         }
         __syncwarp();
-        mbar_arrive_if(ok && !rehearsal && lane == 0, &sh.p_full[i][0]);
+        mbar_arrive_if(ok && lane == 0, &sh.p_full[i][0]);
         if (work) {
           weights(x[1], 8, 16, 16);
           tmem_st_32x16(s_t + 48, reinterpret_cast<uint32_t(&)[16]>(w[16]));
@@ -577,11 +573,7 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
           tc_fence_before();
         }
         __syncwarp();
-        mbar_arrive_if(ok && !rehearsal && lane == 0, &sh.p_full[i][1]);
-      }
-      if (rehearsal) {
-        tiles = 0;
-        continue;
+        mbar_arrive_if(ok && lane == 0, &sh.p_full[i][1]);
       }
       if (n > 0) {
         if (ok) ok = WARP_WAIT(&sh.o_full[i], outputs & 1, 634 + i);
