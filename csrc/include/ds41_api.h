@@ -682,7 +682,7 @@ int ds41_gemm_f32(const float* A, const float* B, float* out, int M, int N, int 
 // tokens, the last of lengths[i], in slot slots[i]; its rows follow those of request i - 1.  What a pass is made of, and the workspace of
 // its calls, is written on the device from the requests' lengths:
 typedef struct ds41_ragged_pass {
-  int* header;                    // [16] {units, rows of all requests}
+  int* header;                    // [16] {units, rows of all requests, requests that cannot be, the first of them}
   int* row_pos;                   // [rows] position, slot (-1: none) and row of the pool (-1: none) of every row; rows behind the last
   int* row_slot;                  //   request's: 0, -1, -1
   int* row_place;
@@ -702,6 +702,10 @@ typedef struct ds41_ragged_pass {
 } ds41_ragged_pass;
 int ds41_ragged_describe(const ds41_ragged_pass* pass, const int* slots, const int* news, const int* lengths, int n,
                          const int* page_table, int n_slots, int max_pages, int n_pages, void* stream);
+// The same from `n` rows' positions and slots: adjacent rows of one slot at consecutive positions are a request's, rows without one a
+// request each.
+int ds41_ragged_describe_rows(const ds41_ragged_pass* pass, const int* row_pos, const int* row_slot, int n, const int* page_table,
+                              int n_slots, int max_pages, int n_pages, void* stream);
 
 // RMS norm of every head of q and k (weights [dim], or [heads][dim] with a stride; NULL: none), rotation of the first rot_dim values by
 // row_pos * freq, q as a matrix, keys and values into the pool's rows row_place.  Rows with a negative place are left as they are.
@@ -729,9 +733,9 @@ typedef struct ds41_ragged_attend_args {
   const void* pool;
   const int* page_table;
   void* out;                      // row r, head h at r * out_row + h * vdim
-  const float* gate;              // [rows][gate_row] or NULL
+  ds41_proj gate;                 // one column per head (absent: no gate)
   const float* sink;              // [heads] or NULL
-  long long q_row, q_head, out_row, gate_row;
+  long long q_row, q_head, out_row;
   float scale;
   int q_rows, max_pages, n_pages;
 } ds41_ragged_attend_args;

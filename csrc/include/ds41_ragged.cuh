@@ -90,8 +90,8 @@ __device__ __forceinline__ void ragged_join(const ds41_ragged_pass& p, const ds4
       den += ml.x == -INFINITY ? 0.f : exp2f(ml.x - base) * ml.y;
     }
     den = warp_sum(den) + (a.sink != nullptr ? exp2f(sink - base) : 0.f);
-    float f = den != 0.f ? 1.f / den : 0.f;              // a NaN in a maximum or the sink is in the sum
-    if (a.gate != nullptr) f *= sigmoid_f32(a.gate[row * a.gate_row + h]);
+    float f = 1.f / den;                                 // a NaN in a maximum or the sink is in the sum
+    if (a.gate.data != nullptr) f *= sigmoid_f32(proj_at(a.gate, row, h));
     T* out = static_cast<T*>(a.out) + row * a.out_row + 1ll * h * p.vdim;
     for (int c = 4 * lane; c < p.vdim; c += 128) {
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);

@@ -19,7 +19,7 @@ constexpr int kMostRequests = 4096, kMostBlocks = 8192;
 constexpr int kCandidates = 16, kBins = 256;
 
 struct DescribeArgs {
-  const int *slots, *news, *lengths, *page_table;
+  const int *slots, *news, *lengths, *page_table;       // news: NULL, where slots and lengths are the slots and positions of rows
   int n, n_slots, max_pages, n_pages;
   int dividers;              // CTAs that divide the work and each write their share of the units; the others describe rows
 };
@@ -59,14 +59,6 @@ __device__ __forceinline__ int find_last(const int* list, int n, int x) {
   return lo;
 }
 
-__device__ __forceinline__ void bad_argument(int* status, int where, int detail) {
-  if (atomicCAS(status, kStatusOk, kStatusBadArgument) == kStatusOk) {
-    status[1] = where;
-    status[2] = static_cast<int>(blockIdx.x);
-    status[3] = detail;
-  }
-}
-
 // A tile's time in tenths of that of a tensor-core tile pair of 128 keys, and that of what a unit begins and ends with.
 constexpr int kPairTile = 10, kTurnTile = 7, kUnitCost = 20;
 __device__ __forceinline__ int tile_cost(const ds41_ragged_pass& p, int rows) { return !p.tiled || rows > p.turn_rows ? kPairTile : kTurnTile; }
@@ -75,41 +67,80 @@ __global__ void __launch_bounds__(kDescribeThreads) ragged_describe_kernel(const
   extern __shared__ int rd_smem[];
   __shared__ unsigned long long scans[2][kDescribeWarps];
   __shared__ float cost_of[kCandidates];
-  __shared__ int units_of[kCandidates], cells_of[kCandidates], bins[kBins], earlier[kBins], bin_sums[kBins / 32], longest, chosen;
+  __shared__ int units_of[kCandidates], cells_of[kCandidates], bins[kBins], earlier[kBins], bin_sums[kBins / 32], longest, chosen, bad, first_bad;
   int scan = 0;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.n, G = p.kv_heads, group = p.heads / p.kv_heads;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = p.kv_heads, group = p.heads / p.kv_heads;
   int* row_first = rd_smem;             // [n] of every request: its first row, its first block, tokens, first token's position, slot
-  int* block_first = row_first + n;
-  int* tokens = block_first + n;
-  int* begin = tokens + n;
-  int* slot_of = begin + n;
-  int* owner = slot_of + n;             // [blocks] request
+  int* block_first = row_first + p.requests;
+  int* tokens = block_first + p.requests;
+  int* begin = tokens + p.requests;
+  int* slot_of = begin + p.requests;
+  int* owner = slot_of + p.requests;             // [blocks] request
   int* tiles = owner + p.max_blocks;    // [blocks] key tiles
   int* first = tiles + p.max_blocks;    // [blocks] first unit of the list by blocks, first cell
   int* cells = first + p.max_blocks;
   pdl_launch_dependents();
   for (int i = tid; i < kBins; i += kDescribeThreads) bins[i] = earlier[i] = 0;
-  if (tid == 0) longest = 1;
+  if (tid == 0) longest = 1, bad = 0, first_bad = INT_MAX;
   pdl_wait();
+  __syncthreads();
+  int n = a.n;
+  const bool by_rows = a.news == nullptr;
+  if (by_rows) {                        // where requests begin, then how many rows they have
+    int begun = 0;
+    for (int r0 = 0; r0 < a.n; r0 += kDescribeThreads) {
+      const int r = r0 + tid;
+      int slot = -1, pos = 0;
+      bool first = false;
+      if (r < a.n) {
+        slot = a.slots[r];
+        pos = a.lengths[r];
+        first = r == 0 || slot < 0 || a.slots[r - 1] != slot || a.lengths[r - 1] != pos - 1;
+      }
+      unsigned long long total;
+      const int i = begun + static_cast<int>(block_scan(first, scans, scan, total));
+      begun += static_cast<int>(total);
+      if (first && i < p.requests) {
+        row_first[i] = r;
+        begin[i] = pos;
+        slot_of[i] = slot;
+      }
+    }
+    __syncthreads();
+    n = min(begun, p.requests);
+    if (tid == 0 && begun > n) bad = begun - n, first_bad = n;
+    for (int i = tid; i < n; i += kDescribeThreads) tokens[i] = (i + 1 < begun && i + 1 < p.requests ? row_first[i + 1] : a.n) - row_first[i];
+    if (begun > n) {                    // the last request that has a place ends where the next one begins
+      __syncthreads();
+      if (tid == 0) {
+        int r = row_first[n - 1] + 1;
+        while (r < a.n && a.slots[r] >= 0 && a.slots[r] == slot_of[n - 1] && a.lengths[r] == begin[n - 1] + r - row_first[n - 1]) ++r;
+        tokens[n - 1] = r - row_first[n - 1];
+      }
+    }
+    __syncthreads();
+  }
   unsigned long long base = 0;          // rows, blocks
   for (int i0 = 0; i0 < n; i0 += kDescribeThreads) {
     const int i = i0 + tid;
     int slot = -1, count = 0, length = 0;
+    bool wrong = false;
     if (i < n) {
-      slot = a.slots[i];
-      count = a.news[i];
-      length = a.lengths[i];
-      if (count < 0 || length < count || slot >= a.n_slots || (slot >= 0 && length > 1ll * a.max_pages * p.page_tokens)) {
-        if (blockIdx.x == 0) bad_argument(p.status, 500, i);
-        slot = -1;
-      }
+      slot = by_rows ? slot_of[i] : a.slots[i];
+      count = by_rows ? tokens[i] : a.news[i];
+      length = by_rows ? begin[i] + count : a.lengths[i];
+      wrong = count < 0 || (slot >= 0 && length < count) || slot >= a.n_slots || (slot >= 0 && length > 1ll * a.max_pages * p.page_tokens);
+      if (wrong) slot = -1;
     }
     const int wanted = max(count, 0), most = min(wanted, p.rows);
     unsigned long long total;
     unsigned long long at = block_scan(static_cast<unsigned long long>(most) << 32 | (most + p.unit_tokens - 1) / p.unit_tokens, scans, scan, total);
     // rows beyond the pass's are left out
     const int row = static_cast<int>(min((base + at) >> 32, static_cast<unsigned long long>(p.rows))), kept = min(most, p.rows - row);
-    if (kept < wanted && blockIdx.x == 0) bad_argument(p.status, 501, i);
+    if (wrong || kept < wanted) {
+      atomicAdd(&bad, 1);
+      atomicMin(&first_bad, i);
+    }
     if (((base + total) >> 32) > static_cast<unsigned>(p.rows))
       at = block_scan(static_cast<unsigned long long>(kept) << 32 | (kept + p.unit_tokens - 1) / p.unit_tokens, scans, scan, total);
     if (i < n) {
@@ -289,6 +320,8 @@ __global__ void __launch_bounds__(kDescribeThreads) ragged_describe_kernel(const
   if (divider == 0 && tid == 0) {
     p.header[0] = units;
     p.header[1] = rows;
+    p.header[2] = bad;
+    p.header[3] = first_bad;
   }
 }
 
@@ -764,8 +797,8 @@ __global__ void __launch_bounds__(kRaggedThreads) ragged_simple_kernel(const ds4
           const float whole = fmaxf(m, sink), base = whole == -INFINITY ? 0.f : whole;
           const float w = m == -INFINITY ? 0.f : exp2f(m - base);
           const float den = l * w + (a.sink != nullptr ? exp2f(sink - base) : 0.f);
-          float f = den != 0.f ? w / den : 0.f;
-          if (a.gate != nullptr) f *= sigmoid_f32(a.gate[row * a.gate_row + h]);
+          float f = w / den;
+          if (a.gate.data != nullptr) f *= sigmoid_f32(proj_at(a.gate, row, h));
           store4(static_cast<T*>(a.out) + row * a.out_row + 1ll * h * V + 4 * col,
                  make_float4(acc[i].x * f, acc[i].y * f, acc[i].z * f, acc[i].w * f));
         }
@@ -817,12 +850,13 @@ inline bool ragged_pass_ok(const ds41_ragged_pass* p) {
 
 using namespace ds41;
 
-extern "C" int ds41_ragged_describe(const ds41_ragged_pass* p, const int* slots, const int* news, const int* lengths, int n,
-                                    const int* page_table, int n_slots, int max_pages, int n_pages, void* stream) {
-  if (!ragged_pass_ok(p) || n < 0 || n > p->requests || n_slots <= 0 || max_pages <= 0 || n_pages <= 0 || page_table == nullptr ||
-      (n > 0 && (slots == nullptr || news == nullptr || lengths == nullptr)) || 1ll * n_pages * p->page_tokens > INT_MAX)
+static int describe(const ds41_ragged_pass* p, const DescribeArgs& given, void* stream) {
+  DescribeArgs a = given;
+  if (a.n < 0 || a.n_slots <= 0 || a.max_pages <= 0 || a.n_pages <= 0 || a.page_table == nullptr ||
+      (a.n > 0 && (a.slots == nullptr || a.lengths == nullptr)) || 1ll * a.n_pages * p->page_tokens > INT_MAX ||
+      1ll * a.max_pages * p->page_tokens > 1 << 30)
     return cudaErrorInvalidValue;
-  const int smem = 4 * (5 * n + 4 * p->max_blocks);
+  const int smem = 4 * (5 * p->requests + 4 * p->max_blocks);
   static std::atomic<unsigned long long> ready{0};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -833,10 +867,22 @@ extern "C" int ds41_ragged_describe(const ds41_ragged_pass* p, const int* slots,
     if (dev < 64) ready.fetch_or(1ull << dev);
   }
   // 456 blocks in 3648 units: 14.1 us with one divider
-  const int dividers = std::min(8, (p->max_blocks + 31) / 32);
-  const DescribeArgs a{slots, news, lengths, page_table, n, n_slots, max_pages, n_pages, dividers};
-  const int grid = dividers + (p->rows + kDescribeThreads - 1) / kDescribeThreads;
+  a.dividers = std::min(8, (p->max_blocks + 31) / 32);
+  const int grid = a.dividers + (p->rows + kDescribeThreads - 1) / kDescribeThreads;
   return launch_pdl(ragged_describe_kernel, dim3(grid), dim3(kDescribeThreads), smem, static_cast<cudaStream_t>(stream), *p, a);
+}
+
+extern "C" int ds41_ragged_describe(const ds41_ragged_pass* p, const int* slots, const int* news, const int* lengths, int n,
+                                    const int* page_table, int n_slots, int max_pages, int n_pages, void* stream) {
+  static const int none = 0;
+  if (!ragged_pass_ok(p) || n > p->requests || (n > 0 && news == nullptr)) return cudaErrorInvalidValue;
+  return describe(p, DescribeArgs{slots, n > 0 ? news : &none, lengths, page_table, n, n_slots, max_pages, n_pages, 0}, stream);
+}
+
+extern "C" int ds41_ragged_describe_rows(const ds41_ragged_pass* p, const int* row_pos, const int* row_slot, int n, const int* page_table,
+                                         int n_slots, int max_pages, int n_pages, void* stream) {
+  if (!ragged_pass_ok(p) || n > p->rows) return cudaErrorInvalidValue;
+  return describe(p, DescribeArgs{row_slot, nullptr, row_pos, page_table, n, n_slots, max_pages, n_pages, 0}, stream);
 }
 
 extern "C" int ds41_ragged_heads(const ds41_ragged_heads_args* a, void* stream) {
@@ -865,7 +911,7 @@ extern "C" int ds41_ragged_heads(const ds41_ragged_heads_args* a, void* stream) 
 extern "C" int ds41_ragged_attend(const ds41_ragged_attend_args* a, const ds41_ragged_pass* p, void* stream) {
   if (!ragged_pass_ok(p) || a == nullptr || a->q == nullptr || a->pool == nullptr || a->page_table == nullptr || a->out == nullptr ||
       a->q_rows < p->rows || a->max_pages <= 0 || a->n_pages <= 0 || 1ll * a->n_pages * p->page_tokens > INT_MAX || !(a->scale > 0.f) ||
-      a->q_head < p->dim || a->q_row < 0 || a->out_row < 1ll * p->heads * p->vdim)
+      a->q_head < p->dim || a->q_row < 0 || a->out_row < 1ll * p->heads * p->vdim || (a->gate.data != nullptr && !proj_ok(a->gate)))
     return cudaErrorInvalidValue;
   const int size = p->f32 ? 4 : 2;
   if (!aligned(a->q, 16) || !aligned(a->pool, 16) || !aligned(a->out, 16) || (a->q_row * size & 15) || (a->q_head * size & 15) ||

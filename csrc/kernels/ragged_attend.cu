@@ -466,7 +466,7 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
         place_step = x.turns ? 2 * kRtKeys : kRtKeys;
         const int h = u.head * t.group + mine_head, row = u.row0 + (i && !x.turns ? x.tok0 : 0) + mine_tok;
         if (live && t.a.sink != nullptr) sink = t.a.sink[h] * kLog2E;
-        if (live && t.a.gate != nullptr) gate = t.a.gate[row * t.a.gate_row + h];
+        if (live && t.a.gate.data != nullptr) gate = proj_at(t.a.gate, row, h);
       }
       const bool idle = !__any_sync(0xffffffffu, live);
       float m = -INFINITY, l = 0.f;
@@ -633,8 +633,8 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
       } else if (live) {
         const float top = fmaxf(m, sink), base = top == -INFINITY ? 0.f : top;
         const float w = ex2_approx(m - base), den = l * w + (t.a.sink != nullptr ? ex2_approx(sink - base) : 0.f);
-        f = den != 0.f ? w / den : 0.f;
-        if (t.a.gate != nullptr) f *= sigmoid_f32(gate);
+        f = w / den;
+        if (t.a.gate.data != nullptr) f *= sigmoid_f32(gate);
       }
       w_own *= f;
       w_half *= f;

@@ -140,7 +140,7 @@ def dir_functions():
         "ds41_mlstm_step", "ds41_gemm_f32", "ds41_side_act", "ds41_softcap_rows", "ds41_attn_post", "ds41_group_attend",
         "ds41_group_prefill", "ds41_route_softmax", "ds41_gated_act",
         "ds41_prefix_group", "ds41_prefix_latent",
-        "ds41_ragged_describe", "ds41_ragged_heads", "ds41_ragged_attend",
+        "ds41_ragged_describe", "ds41_ragged_describe_rows", "ds41_ragged_heads", "ds41_ragged_attend",
     ]
 
 

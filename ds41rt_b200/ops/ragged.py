@@ -51,8 +51,8 @@ class HeadsArgs(C.Structure):
 
 
 class AttendArgs(C.Structure):
-    _fields_ = [(n, C.c_void_p) for n in ("q", "pool", "page_table", "out", "gate", "sink")] + \
-               [(n, C.c_longlong) for n in ("q_row", "q_head", "out_row", "gate_row")] + \
+    _fields_ = [(n, C.c_void_p) for n in ("q", "pool", "page_table", "out")] + [("gate", S.ProjArgs), ("sink", C.c_void_p)] + \
+               [(n, C.c_longlong) for n in ("q_row", "q_head", "out_row")] + \
                [("scale", C.c_float), ("q_rows", C.c_int), ("max_pages", C.c_int), ("n_pages", C.c_int)]
 
 
@@ -127,25 +127,54 @@ class RaggedPass:
                 raise ValueError(f"{name} must be contiguous 32-bit integers, one per request")
         if n > self.requests:
             raise ValueError(f"a pass for {self.requests} requests does not take {n}")
-        n_slots, width = shape = page_table.shape if page_table.dim() == 2 else (0, 0)
-        if page_table.dtype is not I32 or n_slots == 0 or width == 0 or not page_table.is_contiguous():
-            raise ValueError("page_table is a contiguous matrix of 32-bit integers, [slots, pages]")
-        if n_pages <= 0 or n_pages * self.page_tokens >= 1 << 31 or width * self.page_tokens >= 1 << 31:
-            raise ValueError("a pool and a request have fewer than 2^31 rows")
         here = torch.cuda.current_device()
-        if not (slots.get_device() == here and new.get_device() == here and lengths.get_device() == here and page_table.get_device() == here
-                and self.header.get_device() == here):
-            _elsewhere(here, (("slots", slots), ("new", new), ("lengths", lengths), ("page_table", page_table), ("the pass", self.header)))
+        if not (slots.get_device() == here and new.get_device() == here and lengths.get_device() == here):
+            _elsewhere(here, (("slots", slots), ("new", new), ("lengths", lengths)))
+        n_slots, width = self._table(page_table, n_pages, here)
         err = lib.kernels("stack").ds41_ragged_describe(self.args_ref, C.c_void_p(slots.data_ptr()), C.c_void_p(new.data_ptr()),
                                                         C.c_void_p(lengths.data_ptr()), n, C.c_void_p(page_table.data_ptr()), n_slots,
                                                         width, n_pages, C.c_void_p(_raw_stream(here)))
         if err:
             lib.check(err, "ds41_ragged_describe")
-        self.table_shape, self.n_pages = shape, n_pages
+        self.table_shape, self.n_pages = (n_slots, width), n_pages
         return self.row_pos, self.row_slot, self.row_place
 
+    def describe_rows(self, row_pos: torch.Tensor, row_slot: torch.Tensor, page_table: torch.Tensor, n_pages: int):
+        """The same from the positions and slots of rows, 32-bit integers on the device, as other operators take them: adjacent rows of
+        one slot at consecutive positions are a request's, a row without a slot is one by itself.  More requests than the pass takes are
+        left out, and check_status() raises."""
+        n = row_pos.numel()
+        if n > self.rows or row_pos.dtype is not I32 or row_slot.dtype is not I32 or row_pos.shape != (n,) or row_slot.shape != (n,) \
+                or not (row_pos.is_contiguous() and row_slot.is_contiguous()):
+            raise ValueError(f"row_pos and row_slot must be contiguous 32-bit integers, one per row, of at most {self.rows} rows")
+        here = torch.cuda.current_device()
+        if not (row_pos.get_device() == here and row_slot.get_device() == here):
+            _elsewhere(here, (("row_pos", row_pos), ("row_slot", row_slot)))
+        n_slots, width = self._table(page_table, n_pages, here)
+        err = lib.kernels("stack").ds41_ragged_describe_rows(self.args_ref, C.c_void_p(row_pos.data_ptr()), C.c_void_p(row_slot.data_ptr()), n,
+                                                             C.c_void_p(page_table.data_ptr()), n_slots, width, n_pages,
+                                                             C.c_void_p(_raw_stream(here)))
+        if err:
+            lib.check(err, "ds41_ragged_describe_rows")
+        self.table_shape, self.n_pages = (n_slots, width), n_pages
+        return self.row_pos, self.row_slot, self.row_place
+
+    def _table(self, page_table: torch.Tensor, n_pages: int, here: int) -> Tuple[int, int]:
+        n_slots, width = page_table.shape if page_table.dim() == 2 else (0, 0)
+        if page_table.dtype is not I32 or n_slots == 0 or width == 0 or not page_table.is_contiguous():
+            raise ValueError("page_table is a contiguous matrix of 32-bit integers, [slots, pages]")
+        if n_pages <= 0 or n_pages * self.page_tokens >= 1 << 31 or width * self.page_tokens > 1 << 30:
+            raise ValueError("a pool has fewer than 2^31 rows, a request at most 2^30")
+        if not (page_table.get_device() == here and self.header.get_device() == here):
+            _elsewhere(here, (("page_table", page_table), ("the pass", self.header)))
+        return n_slots, width
+
     def check_status(self, what: str = "ragged pass"):
+        """Raises if a wait gave up, or if the last description had requests that cannot be."""
         lib.raise_on_status(self.status, what)
+        _, _, bad, first = self.header[:4].tolist()
+        if bad:
+            raise lib.KernelError(f"{what}: {bad} requests of the description cannot be, the first of them number {first}")
 
 
 def _elsewhere(here: int, tensors):
@@ -246,8 +275,8 @@ def attend(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, descri
     pool_rows, columns = pool.shape if pool.dim() == 2 else (0, 0)
     if pool.dtype is not dtype or columns != p.columns or not pool.is_contiguous() or pool.data_ptr() % 16:
         raise ValueError(f"pool must be contiguous rows of {p.columns} values of {dtype}, 16-byte aligned")
-    if pool_rows != p.n_pages * p.page_tokens or table_shape != p.table_shape:
-        raise ValueError(f"the pass was described for {p.n_pages} pages and a page table of {tuple(p.table_shape)}")
+    if pool_rows != p.n_pages * p.page_tokens or tuple(table_shape) != p.table_shape:
+        raise ValueError(f"the pass was described for {p.n_pages} pages and a page table of {p.table_shape}")
     if page_table.dtype is not I32 or not page_table.is_contiguous():
         raise ValueError("page_table is a contiguous matrix of 32-bit integers, [slots, pages]")
     if not scale > 0:
@@ -260,24 +289,23 @@ def attend(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, descri
     out_at = out.data_ptr()
     if one != 1 or head != V or step % 8 or step < H * V or out_at % 16:
         raise ValueError("out must be 16-byte aligned, a row's heads side by side and rows apart, at multiples of 8 values")
-    sink_at = gate_at = None
-    gate_row = 0
+    sink_at, gates = None, S.NO_PROJ
     if sink is not None:
         if sink.dtype is not F32 or sink.shape != (H,) or not sink.is_contiguous():
             raise ValueError(f"sink must be {H} contiguous fp32 values")
         sink_at = sink.data_ptr()
     if gate is not None:
         gate_row, one = gate.stride() if gate.dim() == 2 else (0, 0)
-        if gate.dtype is not F32 or gate.shape != (R, H) or (H > 1 and one != 1):
+        if gate.dtype is not F32 or gate.shape != (R, H) or (H > 1 and one != 1) or (R > 1 and not H <= gate_row < 1 << 31):
             raise ValueError(f"gate must be fp32 [{R}, {H}] with a row's values side by side")
-        gate_at = gate.data_ptr()
+        gates = S.ProjArgs(gate.data_ptr(), 0, gate_row if R > 1 else H, 1, 0, 0)
     here = torch.cuda.current_device()
     if not (q.get_device() == here and pool.get_device() == here and page_table.get_device() == here and out.get_device() == here
             and p.header.get_device() == here and (sink is None or sink.get_device() == here) and (gate is None or gate.get_device() == here)):
         _elsewhere(here, (("q", q), ("pool", pool), ("page_table", page_table), ("out", out), ("the pass", p.header), ("sink", sink),
                           ("gate", gate)))
-    a = AttendArgs(q.data_ptr(), pool.data_ptr(), page_table.data_ptr(), out_at, gate_at, sink_at, q_row, q_head, step, gate_row, scale, R,
-                   table_shape[1], p.n_pages)
+    a = AttendArgs(q.data_ptr(), pool.data_ptr(), page_table.data_ptr(), out_at, gates, sink_at, q_row, q_head, step, scale, R, table_shape[1],
+                   p.n_pages)
     err = lib.kernels("stack").ds41_ragged_attend(C.byref(a), p.args_ref, C.c_void_p(_raw_stream(here)))
     if err:
         lib.check(err, "ds41_ragged_attend")

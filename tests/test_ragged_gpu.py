@@ -30,7 +30,7 @@ class Batch:
     """`requests`: (new tokens, tokens before them) of each; None: one without a slot."""
 
     def __init__(self, requests, *, heads=8, kv_heads=2, dim=64, vdim=64, P=64, window=0, first=0, dtype=BF16, seed=0, pads=0, poison=False,
-                 sharp=1.5, gate=True, sink=False, rot=None, capacity=0):
+                 sharp=1.5, gate=True, sink=False, spare=0):
         rng, gen = random.Random(seed), torch.Generator(device="cuda").manual_seed(seed)
         self.H, self.G, self.D, self.V, self.P, self.window, self.first, self.dtype = heads, kv_heads, dim, vdim, P, window, first, dtype
         n = len(requests)
@@ -74,7 +74,7 @@ class Batch:
         self.scale = dim ** -0.5
         dev = lambda x: torch.tensor(x, dtype=I32, device="cuda")
         self.d_slots, self.d_new, self.d_length, self.d_tables = dev(self.slots), dev(self.new), dev(self.length), self.tables.cuda()
-        self.p = ragged().RaggedPass(rows=capacity or self.R, requests=n, heads=heads, kv_heads=kv_heads, dim=dim, vdim=vdim, page_tokens=P,
+        self.p = ragged().RaggedPass(rows=self.R, requests=n + spare, heads=heads, kv_heads=kv_heads, dim=dim, vdim=vdim, page_tokens=P,
                                      window=window, first=first, device="cuda", dtype=dtype)
 
     def describe(self):
