@@ -702,8 +702,8 @@ typedef struct ds41_ragged_pass {
 } ds41_ragged_pass;
 int ds41_ragged_describe(const ds41_ragged_pass* pass, const int* slots, const int* news, const int* lengths, int n,
                          const int* page_table, int n_slots, int max_pages, int n_pages, void* stream);
-// The same from `n` rows' positions and slots: adjacent rows of one slot at consecutive positions are a request's, rows without one a
-// request each.
+// The same from `n` rows' positions and slots: adjacent rows of one slot at consecutive positions are a request's, rows without one together
+// one without work.
 int ds41_ragged_describe_rows(const ds41_ragged_pass* pass, const int* row_pos, const int* row_slot, int n, const int* page_table,
                               int n_slots, int max_pages, int n_pages, void* stream);
 

@@ -95,7 +95,8 @@ __global__ void __launch_bounds__(kDescribeThreads) ragged_describe_kernel(const
       if (r < a.n) {
         slot = a.slots[r];
         pos = a.lengths[r];
-        first = r == 0 || slot < 0 || a.slots[r - 1] != slot || a.lengths[r - 1] != pos - 1;
+        const int last = r > 0 ? a.slots[r - 1] : 0;
+        first = r == 0 || (slot < 0 ? last >= 0 : last != slot || a.lengths[r - 1] != pos - 1);      // rows without a slot stay together
       }
       unsigned long long total;
       const int i = begun + static_cast<int>(block_scan(first, scans, scan, total));
@@ -114,7 +115,8 @@ __global__ void __launch_bounds__(kDescribeThreads) ragged_describe_kernel(const
       __syncthreads();
       if (tid == 0) {
         int r = row_first[n - 1] + 1;
-        while (r < a.n && a.slots[r] >= 0 && a.slots[r] == slot_of[n - 1] && a.lengths[r] == begin[n - 1] + r - row_first[n - 1]) ++r;
+        const int slot = slot_of[n - 1], from = begin[n - 1] - row_first[n - 1];
+        while (r < a.n && (slot < 0 ? a.slots[r] < 0 : a.slots[r] == slot && a.lengths[r] == from + r)) ++r;
         tokens[n - 1] = r - row_first[n - 1];
       }
     }
@@ -128,7 +130,7 @@ __global__ void __launch_bounds__(kDescribeThreads) ragged_describe_kernel(const
     if (i < n) {
       slot = by_rows ? slot_of[i] : a.slots[i];
       count = by_rows ? tokens[i] : a.news[i];
-      length = by_rows ? begin[i] + count : a.lengths[i];
+      length = !by_rows ? a.lengths[i] : slot < 0 ? 0 : begin[i] + count;
       wrong = count < 0 || (slot >= 0 && length < count) || slot >= a.n_slots || (slot >= 0 && length > 1ll * a.max_pages * p.page_tokens);
       if (wrong) slot = -1;
     }
@@ -162,7 +164,7 @@ __global__ void __launch_bounds__(kDescribeThreads) ragged_describe_kernel(const
       int pos = 0, slot = -1, place = -1;
       if (r < rows) {
         const int i = find_last(row_first, n, r);
-        pos = begin[i] + r - row_first[i];
+        pos = by_rows ? a.lengths[r] : begin[i] + r - row_first[i];
         slot = slot_of[i];
         if (slot >= 0) {
           const int pg = pos / p.page_tokens, id = a.page_table[1ll * slot * a.max_pages + pg];

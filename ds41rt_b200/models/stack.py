@@ -19,10 +19,10 @@ import numpy as np
 import torch
 
 from ..config import rope_inv_freq
-from ..ops import lib, prefix
+from ..ops import lib, prefix, ragged
 from ..ops import stack as S
 from ..ops.stack import Matrix, Proj, ceil_to
-from ..stack_config import GroupedAttentionSpec, LatentAttentionSpec, MLSTMSpec, MoESpec, StackConfig
+from ..stack_config import GroupedAttentionSpec, LatentAttentionSpec, MLSTMSpec, MoESpec, StackConfig, WindowAttentionSpec
 from .base import RowsEngine, row_values, sized
 from .paged import PagedSlots
 
@@ -396,7 +396,60 @@ class GroupedAttention:
         return y, (pin.at(self.at["gate"]) if "gate" in self.at else None)
 
 
-MIXERS = {"latent_attention": LatentAttention, "grouped_attention": GroupedAttention, "mlstm": MLSTM}
+class WindowAttention:
+    """Grouped-query attention of whatever rows a pass has, several requests with several rows each among them: projection, then norm of
+    every head, rotation and cache rows in one launch, then attention over each row's window, by the engine's description of the pass."""
+
+    def __init__(self, spec: WindowAttentionSpec, cfg: StackConfig, t: Dict[str, torch.Tensor], gate: Dict[str, torch.Tensor],
+                 device, dtype):
+        self.spec, self.cfg = spec, cfg
+        H, G = spec.heads, spec.kv_heads
+        self.dp, self.vp = ceil_to(spec.dim, 16), ceil_to(spec.vdim, 16)
+        parts = [("u", torch.cat([S.pad_heads(t["q"], H, spec.dim, self.dp), S.pad_heads(t["k"], G, spec.dim, self.dp),
+                                  S.pad_heads(t["v"], G, spec.vdim, self.vp)], 0))]
+        if spec.head_gate:
+            parts += [("g", t["g"])]
+        if gate:
+            parts += [("gate", gate["w"])]
+        self.w_in, self.at = S.stack_rows(parts, device, dtype)
+        f32 = lambda x: x.to(device=device, dtype=F32).contiguous()
+        self.q_norm, self.k_norm = (f32(S.pad_heads(t[f"{n}.norm"], 1, spec.dim, self.dp)) if spec.head_norm else None for n in "qk")
+        self.sink = f32(t["sink"]) if spec.sink else None
+        self.freq = torch.tensor(rope_inv_freq(spec.rope, spec.rot_dim), dtype=F32, device=device) if spec.rot_dim else None
+        self.w_o = Matrix(S.pad_heads(t["o"].t().contiguous(), H, spec.vdim, self.vp).t(), device, dtype)
+
+    def matrices(self):
+        return {"a": [(self.w_in.n, self.w_in.k)], "b": [(self.w_o.n, self.w_o.k)]}
+
+    def ragged_shape(self):
+        sp = self.spec
+        return sp.heads, sp.kv_heads, self.dp, self.vp, sp.window, sp.first
+
+    def run(self, e: "StackEngine", l: int, R: int, src: int) -> Tuple[Proj, Optional[Proj]]:
+        sp, k, c = self.spec, e.k, e.cache
+        H, G, D, V = sp.heads, sp.kv_heads, self.dp, self.vp
+        p = e.ragged[self.ragged_shape()]
+        pin = e.project_wide("gemm_mix_in", R, self.w_in) if R >= e.long_rows and not e.f32 else \
+            e.project("gemm_mix_in", e.h, e.ldh, R, self.w_in, e.planes_a)
+        at, pool = self.at["u"], c.pools[src]
+        a = ragged.HeadsArgs()
+        a.q, a.k, a.v = pin.at(at).args(), pin.at(at + H * D).args(), pin.at(at + (H + G) * D).args()
+        a.q_norm, a.k_norm, a.freq = lib.ptr(self.q_norm), lib.ptr(self.k_norm), lib.ptr(self.freq)
+        a.row_pos, a.row_place, a.q_out, a.pool = lib.ptr(p.row_pos), lib.ptr(p.row_place), lib.ptr(e.q), lib.ptr(pool)
+        a.ld_q, a.eps, a.width, a.rows, a.heads, a.kv_heads, a.dim, a.vdim = H * D, self.cfg.norm_eps, sp.dim, R, H, G, D, V
+        a.rot_dim, a.pool_rows, a.f32 = sp.rot_dim, pool.shape[0], e.f32
+        e._run("ragged_heads", k.ds41_ragged_heads, C.byref(a), lib.stream())
+        b = ragged.AttendArgs()
+        b.q, b.pool, b.page_table, b.out, b.sink = lib.ptr(e.q), lib.ptr(pool), lib.ptr(c.page_table), lib.ptr(e.act), lib.ptr(self.sink)
+        b.gate = pin.at(self.at["g"]).args() if sp.head_gate else S.NO_PROJ
+        b.q_row, b.q_head, b.out_row, b.scale, b.q_rows = H * D, D, H * V, sp.scale, e.max_rows
+        b.max_pages, b.n_pages = c.max_pages, c.n_pages
+        e._run("ragged_attend", k.ds41_ragged_attend, C.byref(b), p.args_ref, lib.stream())
+        y = e.project("gemm_o", e.act, H * V, R, self.w_o, e.planes_b)
+        return y, (pin.at(self.at["gate"]) if "gate" in self.at else None)
+
+
+MIXERS = {"latent_attention": LatentAttention, "grouped_attention": GroupedAttention, "window_attention": WindowAttention, "mlstm": MLSTM}
 
 
 class DenseMLP:
@@ -669,7 +722,7 @@ class StackEngine(RowsEngine):
                 act = max(act, lw.mlp.ffp)
             if lw.side is not None:
                 act = max(act, lw.side.w_proj.ld)
-            if isinstance(mx, GroupedAttention):
+            if isinstance(mx, (GroupedAttention, WindowAttention)):
                 q = max(q, mx.spec.heads * mx.dp)
             if isinstance(mx, LatentAttention):
                 q = max(q, mx.spec.heads * mx.hs)
@@ -698,6 +751,7 @@ class StackEngine(RowsEngine):
             self.part_o, self.part_ml = z((cells,), F32), z((cells // 8 + 2,), F32)
         self._init_experts(R, moe_rows, z, dt)
         self._init_prefix_plans(shared_prefix)
+        self._init_ragged()
         # head
         self.head_cap = min(R, 64)
         self.last_head_row = 0
@@ -707,6 +761,8 @@ class StackEngine(RowsEngine):
         self.head_mask = None
         self._hint = None
         self.status = lib.new_status(dev)
+        for p in self.ragged.values():
+            p.args.status = self.status.data_ptr()
         self._init_instruments()
         self.on_layer = None      # callable (layer, streams [rows, width]) after every layer of an eager pass
 
@@ -736,6 +792,18 @@ class StackEngine(RowsEngine):
         if shared_prefix:
             self.prefix_plans = {key: prefix.PrefixPlan(device=self.device, **sizes)
                                  for key, sizes in prefix_plan_sizes(self.w, self.max_rows, self.cache.page_tokens).items()}
+
+    def _init_ragged(self):
+        """A description, and workspace, of the passes' rows for every shape of window attention: made on the device from the rows as the
+        pass begins, so that captured passes follow theirs."""
+        self.ragged: Dict[tuple, ragged.RaggedPass] = {}
+        for lw in self.w.layers:
+            if isinstance(lw.mixer, WindowAttention):
+                key = heads, kv_heads, dim, vdim, window, first = lw.mixer.ragged_shape()
+                if key not in self.ragged:
+                    self.ragged[key] = ragged.RaggedPass(rows=self.max_rows, requests=min(self.max_rows, ragged.MOST_REQUESTS), heads=heads,
+                                                         kv_heads=kv_heads, dim=dim, vdim=vdim, page_tokens=self.cache.page_tokens,
+                                                         window=window, first=first, device=self.device, dtype=DTYPES[self.w.dtype])
 
     def prefix_plan(self, mixer, rows: int) -> Optional[prefix.PrefixPlan]:
         """The plan that a pass takes, static per batch size, as a captured pass needs it: its contents follow the rows.  A long pass asks
@@ -862,6 +930,9 @@ class StackEngine(RowsEngine):
         if self.layer_timer is not None:
             self.layer_timer.begin()
         cur = self.kept[0]
+        for p in self.ragged.values():
+            self._run("ragged_describe", self.k.ds41_ragged_describe_rows, p.args_ref, lib.ptr(self.row_pos), lib.ptr(self.row_slot), R,
+                      lib.ptr(self.cache.page_table), self.cache.page_table.shape[0], self.cache.max_pages, self.cache.n_pages, lib.stream())
         self._resid(R, x_out=cur, next_w=layers[0].norm1)
         for l, lw in enumerate(layers):
             after = layers[l + 1].norm1 if l + 1 < len(layers) else self.w.final_norm

@@ -141,8 +141,8 @@ class RaggedPass:
 
     def describe_rows(self, row_pos: torch.Tensor, row_slot: torch.Tensor, page_table: torch.Tensor, n_pages: int):
         """The same from the positions and slots of rows, 32-bit integers on the device, as other operators take them: adjacent rows of
-        one slot at consecutive positions are a request's, a row without a slot is one by itself.  More requests than the pass takes are
-        left out, and check_status() raises."""
+        one slot at consecutive positions are a request's, and rows without a slot together one
+        that nothing is done for.  More requests than the pass takes are left out, and check_status() raises."""
         n = row_pos.numel()
         if n > self.rows or row_pos.dtype is not I32 or row_slot.dtype is not I32 or row_pos.shape != (n,) or row_slot.shape != (n,) \
                 or not (row_pos.is_contiguous() and row_slot.is_contiguous()):
@@ -150,6 +150,8 @@ class RaggedPass:
         here = torch.cuda.current_device()
         if not (row_pos.get_device() == here and row_slot.get_device() == here):
             _elsewhere(here, (("row_pos", row_pos), ("row_slot", row_slot)))
+        if n and (row_pos.data_ptr() == self.row_pos.data_ptr() or row_slot.data_ptr() == self.row_slot.data_ptr()):
+            raise ValueError("row_pos and row_slot are what the description writes: copies of them")
         n_slots, width = self._table(page_table, n_pages, here)
         err = lib.kernels("stack").ds41_ragged_describe_rows(self.args_ref, C.c_void_p(row_pos.data_ptr()), C.c_void_p(row_slot.data_ptr()), n,
                                                              C.c_void_p(page_table.data_ptr()), n_slots, width, n_pages,

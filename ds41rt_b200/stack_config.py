@@ -63,6 +63,25 @@ class GroupedAttentionSpec:
 
 
 @dataclass(frozen=True)
+class WindowAttentionSpec:
+    """Grouped-query attention over a window of positions and a few first ones that stay visible, or over everything before a position
+    (csrc/kernels/ragged.cu, ragged_attend.cu).  Every head of q and k is normed by itself."""
+    heads: int
+    kv_heads: int
+    dim: int                     # query / key width per head
+    vdim: int
+    scale: float
+    window: int = 0              # a position p sees j <= p with j > p - window (0: all of them) or j < first
+    first: int = 0
+    rot_dim: int = 0             # leading dimensions of a head that are turned (0: none)
+    rope: Optional[RopeConfig] = None
+    head_norm: bool = True       # RMS norm of every head of q and k
+    head_gate: bool = False      # one sigmoid gate per head on the output
+    sink: bool = False           # an extra logit per head in the denominator
+    kind: str = "window_attention"
+
+
+@dataclass(frozen=True)
 class MLSTMSpec:
     """Matrix-memory recurrence with a running maximum (csrc/kernels/mlstm.cu)."""
     heads: int
@@ -93,7 +112,7 @@ class MoESpec:
     kind: str = "moe"
 
 
-MixerSpec = Union[LatentAttentionSpec, GroupedAttentionSpec, MLSTMSpec]
+MixerSpec = Union[LatentAttentionSpec, GroupedAttentionSpec, WindowAttentionSpec, MLSTMSpec]
 MLPSpec = Union[DenseMLPSpec, MoESpec]
 
 
@@ -162,6 +181,12 @@ class StackConfig:
             if m.kind == "grouped_attention":
                 if min(m.heads, m.kv_heads, m.dim, m.vdim) <= 0 or m.taps < 0 or m.chunk < 0 or m.heads % m.kv_heads:
                     raise ConfigError(f"layer {l}: sizes must be positive and kv_heads must divide heads")
+                if m.rot_dim % 2 or not 0 <= m.rot_dim <= m.dim:
+                    raise ConfigError(f"layer {l}: the rotated part must be even and within the head")
+            if m.kind == "window_attention":
+                if min(m.heads, m.kv_heads, m.dim, m.vdim) <= 0 or min(m.window, m.first) < 0 or m.heads % m.kv_heads or \
+                        max(m.dim, m.vdim) > 256:
+                    raise ConfigError(f"layer {l}: sizes must be positive, heads at most 256 wide, and kv_heads must divide heads")
                 if m.rot_dim % 2 or not 0 <= m.rot_dim <= m.dim:
                     raise ConfigError(f"layer {l}: the rotated part must be even and within the head")
             if spec.mlp is not None and spec.mlp.kind == "moe" and not 0 < spec.mlp.top <= min(spec.mlp.experts, 32):

@@ -111,3 +111,12 @@ def heads_arguments(**kw):
 def test_heads_refuse(kw):
     with pytest.raises(ValueError):
         ragged.heads_to_cache(**heads_arguments(**kw))
+
+
+@pytest.mark.parametrize("kw", [dict(window=-1), dict(first=-2), dict(kv_heads=3), dict(dim=300), dict(rot_dim=7), dict(rot_dim=48)])
+def test_window_layers_that_cannot_be(kw):
+    from ds41rt_b200.stack_config import ConfigError, LayerSpec, StackConfig, WindowAttentionSpec
+    sizes = dict(heads=8, kv_heads=2, dim=32, vdim=32, scale=0.1, window=5, first=1)
+    StackConfig("w", 10, 32, (LayerSpec(WindowAttentionSpec(**sizes), None),), 1e-6).validate()
+    with pytest.raises(ConfigError):
+        StackConfig("w", 10, 32, (LayerSpec(WindowAttentionSpec(**{**sizes, **kw}), None),), 1e-6).validate()

@@ -75,6 +75,26 @@ def test_rows_of_more_requests_than_the_pass_takes():
     p.check_status()
 
 
+def test_rows_without_a_slot_are_one_request():
+    m = ragged()
+    p = m.RaggedPass(rows=900, requests=3, heads=4, kv_heads=2, dim=64, vdim=64, page_tokens=64, device="cuda")
+    table = torch.arange(10, dtype=I32, device="cuda").view(5, 2)
+    pos = torch.arange(900, dtype=I32, device="cuda") * 7919 % 2000
+    slot = torch.full_like(pos, -1)
+    pos[600:640], slot[600:640] = torch.arange(50, 90, device="cuda", dtype=I32), 2
+    got_pos, got_slot, place = p.describe_rows(pos, slot, table, 10)
+    p.check_status()
+    assert torch.equal(got_pos, pos) and torch.equal(got_slot, slot) and (place[slot < 0] == -1).all()
+    assert place[600:640].tolist() == [4 * 64 + i for i in range(50, 90)]
+    assert p.header[1].item() == 900
+    slot[700:701] = 1                       # a fourth and a fifth
+    pos[700:701] = 3
+    got_pos, got_slot, place = p.describe_rows(pos, slot, table, 10)
+    assert (got_slot[700:] == -1).all() and got_slot[639].item() == 2 and p.header[1].item() == 700
+    with pytest.raises(ValueError, match="copies"):
+        p.describe_rows(p.row_pos, slot, table, 10)
+
+
 def test_requests_that_cannot_be():
     from ds41rt_b200.ops.lib import KernelError
     b = Batch([(3, 10), (2, 60), (4, 0)])
