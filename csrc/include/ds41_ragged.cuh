@@ -72,42 +72,74 @@ __device__ __forceinline__ float4 ragged_part(const float* p) { return __ldcg(re
 
 constexpr float kLog2E = 1.4426950408889634f;
 
-// Joins rows [r, n) of a block's pieces: a warp per (token, head) row, its lanes along the columns.
+// Joins rows [r, n) of a block's pieces, the rows of warp `warp` of `warps`: 8, 16 or 32 lanes to a (token, head) row, along the pieces for
+// their maxima and sums, and along the columns for their results, eight pieces' at a time; the next row's maxima are under way meanwhile.
+// One row and one load after another, nine pieces of 63 rows of 48 columns took 28 us; 5 so.
 template <typename T>
-__device__ __forceinline__ void ragged_join(const ds41_ragged_pass& p, const ds41_ragged_attend_args& a, const RaggedUnit& u, int r,
-                                            int n, int warps) {
-  const int lane = threadIdx.x & 31, group = p.heads / p.kv_heads;
-  for (; r < n; r += warps) {
-    const int row = u.row0 + r / group, h = u.head * group + r % group;
-    float top = -INFINITY;
-    for (int i = lane; i < u.pieces; i += 32) top = fmaxf(top, __ldcg(p.part_ml + 2 * (1ll * u.cell + 1ll * i * u.step + r)));
-    top = warp_max(top);
-    const float sink = a.sink != nullptr ? a.sink[h] * kLog2E : -INFINITY;
+__device__ __forceinline__ void ragged_join(const ds41_ragged_pass& p, const ds41_ragged_attend_args& a, const RaggedUnit& u, int r0,
+                                            int n, int warp, int warps) {
+  const int span = p.vdim <= 32 ? 8 : p.vdim <= 64 ? 16 : 32, lane = threadIdx.x & (span - 1), from_lane = threadIdx.x & 31 & ~(span - 1);
+  const int group = p.heads / p.kv_heads, step = warps * (32 / span);
+  auto ml_at = [&](int r, int i) {
+    return r < n && i < u.pieces ? __ldcg(reinterpret_cast<const float2*>(p.part_ml) + (1ll * u.cell + 1ll * i * u.step + r))
+                                 : make_float2(-INFINITY, 0.f);
+  };
+  r0 += warp * (32 / span);                              // the warp's first row
+  int r = r0 + from_lane / span;
+  float2 next = ml_at(r, lane);
+  float next_gate = 0.f, next_sink = -INFINITY;
+  auto head_of = [&](int r) {                            // rows from n on have nothing, and are not stored
+    const int row = u.row0 + min(r, n - 1) / group, h = u.head * group + r % group;
+    if (a.gate.data != nullptr) next_gate = proj_at(a.gate, row, h);
+    if (a.sink != nullptr) next_sink = a.sink[h];
+  };
+  head_of(r);
+  for (; r0 < n; r0 += step, r += step) {
+    const float2 ml = next;                              // of the first pieces
+    const float gate = next_gate, sink = next_sink * kLog2E;
+    next = ml_at(r + step, lane);
+    head_of(r + step);
+    const int row = u.row0 + min(r, n - 1) / group, h = u.head * group + r % group;
+    float top = ml.x;
+    for (int i = lane + span; i < u.pieces; i += span) top = fmaxf(top, ml_at(r, i).x);
+    for (int o = span / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     const float whole = fmaxf(top, sink), base = whole == -INFINITY ? 0.f : whole;
-    float den = 0.f;
-    for (int i = lane; i < u.pieces; i += 32) {
-      const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + (1ll * u.cell + 1ll * i * u.step + r));
-      den += ml.x == -INFINITY ? 0.f : exp2f(ml.x - base) * ml.y;
+    auto weight = [&](float2 x) { return x.x == -INFINITY ? 0.f : exp2f(x.x - base); };
+    float den = weight(ml) * ml.y;
+    for (int i = lane + span; i < u.pieces; i += span) {
+      const float2 x = ml_at(r, i);
+      den += weight(x) * x.y;
     }
-    den = warp_sum(den) + (a.sink != nullptr ? exp2f(sink - base) : 0.f);
+    for (int o = span / 2; o; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
+    den += a.sink != nullptr ? exp2f(sink - base) : 0.f;
     float f = 1.f / den;                                 // a NaN in a maximum or the sink is in the sum
-    if (a.gate.data != nullptr) f *= sigmoid_f32(proj_at(a.gate, row, h));
+    if (a.gate.data != nullptr) f *= sigmoid_f32(gate);
     T* out = static_cast<T*>(a.out) + row * a.out_row + 1ll * h * p.vdim;
-    for (int c = 4 * lane; c < p.vdim; c += 128) {
+    for (int c0 = 0; c0 < p.vdim; c0 += 4 * span) {
+      const int c = c0 + 4 * lane;
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-      for (int i = 0; i < u.pieces; ++i) {
-        const long long cell = 1ll * u.cell + 1ll * i * u.step + r;
-        const float m = __ldcg(p.part_ml + 2 * cell);
-        if (m == -INFINITY) continue;
-        const float w = exp2f(m - base);
-        const float4 v = ragged_part(p.part_o + cell * p.vdim + c);
-        o.x += w * v.x;
-        o.y += w * v.y;
-        o.z += w * v.z;
-        o.w += w * v.w;
+      for (int i0 = 0; i0 < u.pieces; i0 += span) {
+        const float2 x = i0 == 0 ? ml : ml_at(r, i0 + lane);
+        const unsigned there = __ballot_sync(0xffffffffu, x.x != -INFINITY) >> from_lane;      // others saw nothing and left nothing
+        const float w = weight(x);
+        const float* from = p.part_o + (1ll * u.cell + 1ll * i0 * u.step + r) * p.vdim + c;
+#pragma unroll 1
+        for (int j = 0; j < min(span, u.pieces - i0); j += 8) {
+          float4 v[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            v[k] = c < p.vdim && there >> (j + k) & 1 ? ragged_part(from + 1ll * (j + k) * u.step * p.vdim) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float wk = __shfl_sync(0xffffffffu, w, from_lane + j + k);
+            o.x += wk * v[k].x;
+            o.y += wk * v[k].y;
+            o.z += wk * v[k].z;
+            o.w += wk * v[k].w;
+          }
+        }
       }
-      store4(out + c, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
+      if (c < p.vdim && r < n) store4(out + c, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
     }
   }
 }

@@ -621,7 +621,7 @@ inline bool packed_row(const ds41_proj& p) {
 }
 
 // ---------------------------------------------------------------------------------------------------- attention, any type and size
-constexpr int kSimpleRows = 64, kSimpleKeyTile = 32, kRaggedThreads = 256;
+constexpr int kSimpleRows = 64, kSimpleKeyTile = 32, kRaggedThreads = 256, kRaggedWarps = kRaggedThreads / 32;
 
 __device__ __forceinline__ float4 four_at(const float* p) { return *reinterpret_cast<const float4*>(p); }
 __device__ __forceinline__ float4 four_at(const __nv_bfloat16* p) {
@@ -670,11 +670,15 @@ __global__ void __launch_bounds__(kRaggedThreads) ragged_simple_kernel(const ds4
     for (int r0 = 0; r0 < n; r0 += kSimpleRows) {
       const int rows = min(kSimpleRows, n - r0);
       __syncthreads();
-      for (int r = warp; r < kSimpleRows; r += kRaggedThreads / 32) {
-        const int row = u.row0 + (r0 + r) / group, h = u.head * group + (r0 + r) % group;
-        const T* q = static_cast<const T*>(a.q) + row * a.q_row + h * a.q_head;
-        for (int d = 4 * lane; d < D; d += 128)
-          *reinterpret_cast<float4*>(qs + r * ds + d) = r < rows ? four_at(q + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int d = 4 * lane; d < D; d += 128) {          // a warp's rows together
+        float4 x[kSimpleRows / kRaggedWarps];
+#pragma unroll
+        for (int i = 0; i < kSimpleRows / kRaggedWarps; ++i) {
+          const int r = warp + i * kRaggedWarps, row = u.row0 + (r0 + r) / group, h = u.head * group + (r0 + r) % group;
+          x[i] = r < rows ? four_at(static_cast<const T*>(a.q) + row * a.q_row + h * a.q_head + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int i = 0; i < kSimpleRows / kRaggedWarps; ++i) *reinterpret_cast<float4*>(qs + (warp + i * kRaggedWarps) * ds + d) = x[i];
       }
       if (tid < kSimpleRows) {
         ms[tid] = -INFINITY;
@@ -686,18 +690,29 @@ __global__ void __launch_bounds__(kRaggedThreads) ragged_simple_kernel(const ds4
       const int col = tid % nc, own = tid / nc * RPT;
       for (int t0 = v0; t0 < v1; t0 += kSimpleKeyTile) {
         __syncthreads();
-        for (int k = warp; k < kSimpleKeyTile; k += kRaggedThreads / 32) {
-          const int place = t0 + k, pos = place < walk.lead ? place : place + walk.shift, pg = pos / p.page_tokens;
+        constexpr int kOwn = kSimpleKeyTile / kRaggedWarps;
+        const T* src[kOwn];                              // a warp's keys together
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+          const int place = t0 + warp + i * kRaggedWarps, pos = place < walk.lead ? place : place + walk.shift, pg = pos / p.page_tokens;
           // a key that some row sees; other places may hold anything
           const bool seen = place < v1 && (pos < p.first || pos >= ragged_low(u.pos0, p.window));
           const int id = seen && pg < a.max_pages ? a.page_table[1ll * u.slot * a.max_pages + pg] : -1;
-          const bool there = static_cast<unsigned>(id) < static_cast<unsigned>(a.n_pages);
-          const T* src = static_cast<const T*>(a.pool) + (1ll * id * p.page_tokens + (pos - pg * p.page_tokens)) * row_len;
-          for (int d = 4 * lane; d < D; d += 128)
-            *reinterpret_cast<float4*>(ks + k * ds + d) = there ? four_at(src + u.head * D + d) : make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int d = 4 * lane; d < V; d += 128)
-            *reinterpret_cast<float4*>(vs + k * V + d) =
-                there ? four_at(src + G * D + u.head * V + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+          src[i] = static_cast<unsigned>(id) < static_cast<unsigned>(a.n_pages)
+                       ? static_cast<const T*>(a.pool) + (1ll * id * p.page_tokens + (pos - pg * p.page_tokens)) * row_len : nullptr;
+        }
+        for (int d = 4 * lane; d < max(D, V); d += 128) {
+          float4 x[kOwn], y[kOwn];
+#pragma unroll
+          for (int i = 0; i < kOwn; ++i) {
+            x[i] = src[i] != nullptr && d < D ? four_at(src[i] + u.head * D + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+            y[i] = src[i] != nullptr && d < V ? four_at(src[i] + G * D + u.head * V + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+#pragma unroll
+          for (int i = 0; i < kOwn; ++i) {
+            if (d < D) *reinterpret_cast<float4*>(ks + (warp + i * kRaggedWarps) * ds + d) = x[i];
+            if (d < V) *reinterpret_cast<float4*>(vs + (warp + i * kRaggedWarps) * V + d) = y[i];
+          }
         }
         __syncthreads();
         const int ty = tid >> 3, tx = tid & 7;
@@ -807,7 +822,7 @@ __global__ void __launch_bounds__(kRaggedThreads) ragged_simple_kernel(const ds4
       }
     }
     if (u.pieces > 1 && ragged_last(p.counters + u.counter, u.pieces, tid == 0, 1, kRaggedThreads, &flag))
-      ragged_join<T>(p, a, u, warp, n, kRaggedThreads / 32);
+      ragged_join<T>(p, a, u, 0, n, warp, kRaggedWarps);
   }
 }
 

@@ -691,7 +691,7 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
         ++halves;
       }
       if (u.pieces > 1 && ragged_last(t.p.counters + u.counter + i, u.pieces, tid == 0, 1 + i, kRtTile, &sh.flag[i]))
-        ragged_join<__nv_bfloat16>(t.p, t.a, u, first_tok * t.group + quad, (first_tok + toks) * t.group, 4);
+        ragged_join<__nv_bfloat16>(t.p, t.a, u, first_tok * t.group, (first_tok + toks) * t.group, quad, 4);
     }
   }
   __syncthreads();

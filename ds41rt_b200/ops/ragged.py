@@ -21,6 +21,7 @@ a block see may be in the others' as well, as the tensor cores multiply it by th
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -54,6 +55,17 @@ class AttendArgs(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("q", "pool", "page_table", "out")] + [("gate", S.ProjArgs), ("sink", C.c_void_p)] + \
                [(n, C.c_longlong) for n in ("q_row", "q_head", "out_row")] + \
                [("scale", C.c_float), ("q_rows", C.c_int), ("max_pages", C.c_int), ("n_pages", C.c_int)]
+
+
+def packed(arguments) -> struct.Struct:
+    """A C structure's layout, by which its bytes are made in a fifth of the time that its object takes (1 us instead of 5)."""
+    letters = {C.c_void_p: "P", C.c_longlong: "q", C.c_int: "i", C.c_float: "f"}
+    form = lambda a: "".join(letters[t] if t in letters else form(t) for _, t in a._fields_)
+    return struct.Struct("@" + form(arguments))
+
+
+_HEADS_BYTES, _ATTEND_BYTES = packed(HeadsArgs), packed(AttendArgs)
+_NO_GATE = (0, 0, 0, 0, 0, 0)
 
 
 def tiled(heads: int, kv_heads: int, dim: int, vdim: int, page_tokens: int) -> bool:
@@ -223,8 +235,8 @@ def heads_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, row_pos: t
     if (dtype is not BF16 and dtype is not F32) or columns != G * (D + V) or not pool.is_contiguous() or not 0 < pool_rows < 1 << 31:
         raise ValueError(f"pool must be contiguous rows of {G * (D + V)} values, bf16 or fp32, fewer than 2^31")
     a_q, a_k, a_v = _projection("q", q, R, H, D), _projection("k", k, R, G, D), _projection("v", v, R, G, V)
-    q_weight, q_stride = (None, 0) if q_norm is None else _weight("q_norm", q_norm, H, D)
-    k_weight, k_stride = (None, 0) if k_norm is None else _weight("k_norm", k_norm, G, D)
+    q_weight, q_stride = (0, 0) if q_norm is None else _weight("q_norm", q_norm, H, D)
+    k_weight, k_stride = (0, 0) if k_norm is None else _weight("k_norm", k_norm, G, D)
     half = 0
     if freq is not None:
         half = freq.numel()
@@ -239,7 +251,9 @@ def heads_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, row_pos: t
         out = torch.empty(R, H, D, dtype=dtype, device=q.device)
     if out.shape != (R, H, D) or out.dtype is not dtype:
         raise ValueError(f"out must be [{R}, {H}, {D}] of the pool's type")
-    row, head, one = _steps(out)
+    row, head, one = out.stride()
+    if one != 1 or head != D or row < H * D:
+        row, head, one = _steps(out)
     if one != 1 or head != D or row < H * D:
         raise ValueError("out: a row's heads must lie side by side, rows apart")
     here = torch.cuda.current_device()
@@ -251,9 +265,10 @@ def heads_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, row_pos: t
                           ("q_norm", q_norm), ("k_norm", k_norm), ("freq", freq)))
     if R == 0:
         return out
-    a = HeadsArgs(a_q, a_k, a_v, q_weight, k_weight, freq.data_ptr() if half else None, row_pos.data_ptr(), row_place.data_ptr(),
-                  out.data_ptr(), pool.data_ptr(), row, eps, q_stride, k_stride, width or D, R, H, G, D, V, 2 * half, pool_rows, dtype is F32)
-    err = lib.kernels("stack").ds41_ragged_heads(C.byref(a), C.c_void_p(_raw_stream(here)))
+    a = _HEADS_BYTES.pack(*a_q, *a_k, *a_v, q_weight, k_weight, freq.data_ptr() if half else 0, row_pos.data_ptr(), row_place.data_ptr(),
+                          out.data_ptr(), pool.data_ptr(), row, eps, q_stride, k_stride, width or D, R, H, G, D, V, 2 * half, pool_rows,
+                          dtype is F32)
+    err = lib.kernels("stack").ds41_ragged_heads(a, C.c_void_p(_raw_stream(here)))
     if err:
         lib.check(err, "ds41_ragged_heads")
     return out
@@ -291,7 +306,7 @@ def attend(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, descri
     out_at = out.data_ptr()
     if one != 1 or head != V or step % 8 or step < H * V or out_at % 16:
         raise ValueError("out must be 16-byte aligned, a row's heads side by side and rows apart, at multiples of 8 values")
-    sink_at, gates = None, S.NO_PROJ
+    sink_at, gates = 0, _NO_GATE
     if sink is not None:
         if sink.dtype is not F32 or sink.shape != (H,) or not sink.is_contiguous():
             raise ValueError(f"sink must be {H} contiguous fp32 values")
@@ -300,15 +315,15 @@ def attend(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, descri
         gate_row, one = gate.stride() if gate.dim() == 2 else (0, 0)
         if gate.dtype is not F32 or gate.shape != (R, H) or (H > 1 and one != 1) or (R > 1 and not H <= gate_row < 1 << 31):
             raise ValueError(f"gate must be fp32 [{R}, {H}] with a row's values side by side")
-        gates = S.ProjArgs(gate.data_ptr(), 0, gate_row if R > 1 else H, 1, 0, 0)
+        gates = gate.data_ptr(), 0, gate_row if R > 1 else H, 1, 0, 0
     here = torch.cuda.current_device()
     if not (q.get_device() == here and pool.get_device() == here and page_table.get_device() == here and out.get_device() == here
             and p.header.get_device() == here and (sink is None or sink.get_device() == here) and (gate is None or gate.get_device() == here)):
         _elsewhere(here, (("q", q), ("pool", pool), ("page_table", page_table), ("out", out), ("the pass", p.header), ("sink", sink),
                           ("gate", gate)))
-    a = AttendArgs(q.data_ptr(), pool.data_ptr(), page_table.data_ptr(), out_at, gates, sink_at, q_row, q_head, step, scale, R, table_shape[1],
-                   p.n_pages)
-    err = lib.kernels("stack").ds41_ragged_attend(C.byref(a), p.args_ref, C.c_void_p(_raw_stream(here)))
+    a = _ATTEND_BYTES.pack(q.data_ptr(), pool.data_ptr(), page_table.data_ptr(), out_at, *gates, sink_at, q_row, q_head, step, scale, R,
+                           table_shape[1], p.n_pages)
+    err = lib.kernels("stack").ds41_ragged_attend(a, p.args_ref, C.c_void_p(_raw_stream(here)))
     if err:
         lib.check(err, "ds41_ragged_attend")
     return out

@@ -120,3 +120,26 @@ def test_window_layers_that_cannot_be(kw):
     StackConfig("w", 10, 32, (LayerSpec(WindowAttentionSpec(**sizes), None),), 1e-6).validate()
     with pytest.raises(ConfigError):
         StackConfig("w", 10, 32, (LayerSpec(WindowAttentionSpec(**{**sizes, **kw}), None),), 1e-6).validate()
+
+
+@pytest.mark.parametrize("name", ["HeadsArgs", "AttendArgs"])
+def test_arguments_as_bytes(name):
+    """The packed form is the structure, byte for byte but for what lies between two fields and behind the last."""
+    import ctypes as C
+    from ds41rt_b200.ops import ragged, stack
+    form = getattr(ragged, name)
+    values, n = [], [0]
+
+    def fill(a):
+        for field, t in a._fields_:
+            n[0] += 1
+            if t is stack.ProjArgs:
+                setattr(a, field, fill(t()))
+            else:
+                values.append(n[0] * 0.5 if t is C.c_float else n[0])
+                setattr(a, field, values[-1])
+        return a
+
+    want = bytes(fill(form()))
+    got = ragged.packed(form).pack(*values)
+    assert len(got) <= len(want) and got == want[:len(got)] and len(want) - len(got) < 8
