@@ -59,9 +59,13 @@ __device__ __forceinline__ int find_last(const int* list, int n, int x) {
   return lo;
 }
 
-// A tile's time in tenths of that of a tensor-core tile pair of 128 keys, and that of what a unit begins and ends with.
-constexpr int kPairTile = 10, kTurnTile = 7, kUnitCost = 20;
-__device__ __forceinline__ int tile_cost(const ds41_ragged_pass& p, int rows) { return !p.tiled || rows > p.turn_rows ? kPairTile : kTurnTile; }
+// A tile's time in tenths of that of a tensor-core tile pair of 128 keys, and that of what a unit begins and ends with.  Above it pieces
+// are too long for the grid (60: 4 requests at 2000 of 32 and 8 heads 22.1 us instead of 15.2), below it there are too many, and joins
+// (20: 40 requests at 4000 141 us instead of 135, 64 at up to 8192 300 instead of 275).
+constexpr int kPairTile = 10, kTurnTile = 7, kSimpleTile = 22, kUnitCost = 45;
+__device__ __forceinline__ int tile_cost(const ds41_ragged_pass& p, int rows) {
+  return !p.tiled ? kSimpleTile : rows > p.turn_rows ? kPairTile : kTurnTile;
+}
 
 __global__ void __launch_bounds__(kDescribeThreads) ragged_describe_kernel(const ds41_ragged_pass p, const DescribeArgs a) {
   extern __shared__ int rd_smem[];
@@ -253,7 +257,7 @@ __global__ void __launch_bounds__(kDescribeThreads) ragged_describe_kernel(const
   const int most_cost = chosen;
   const float part = 1.f / most_cost;
   // the longest pieces first
-  const int widest = longest_walk < most_cost + kPairTile ? longest_walk : most_cost + kPairTile;
+  const int widest = longest_walk < most_cost + kSimpleTile ? longest_walk : most_cost + kSimpleTile;
   const float per_cost = (kBins - 1) / static_cast<float>(widest);
   auto bin_of = [&](int cost) { return kBins - 1 - min(kBins - 1, static_cast<int>(cost * per_cost)); };
   // this CTA's blocks
