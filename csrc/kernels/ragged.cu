@@ -864,7 +864,7 @@ inline bool ragged_pass_ok(const ds41_ragged_pass* p) {
     return false;
   return p->max_blocks >= p->rows / p->unit_tokens + std::min(p->requests, p->rows) && p->max_blocks <= kMostBlocks &&
          p->max_units >= 1ll * p->max_blocks * p->kv_heads && p->max_units < 1 << 22 && p->max_cells > 0 && p->max_cells < 1 << 22 &&
-         aligned(p->units, 16) && aligned(p->part_o, 16) && aligned(p->part_ml, 8) && p->key_tile == (p->tiled ? 128 : 32);
+         aligned(p->units, 16) && aligned(p->part_o, 32) && aligned(p->part_ml, 8) && p->key_tile == (p->tiled ? 128 : 32);
 }
 
 }  // namespace ds41

@@ -36,6 +36,7 @@ struct TiledParams {
   int kd, vc;                // 64-column chunks of a key and a value
   int k_stages, v_stages;
   int box;                   // rows of a copy
+  bool wide_out;             // a row of the result begins at 32 bytes
   int hidden_row;            // beyond the pool: reads as zeros
   float scale_log2;
 };
@@ -444,6 +445,11 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
       {
         const TiledUnit x = tiled_unit(t, unit_at(turn));
         const RaggedUnit& u = x.u;
+        if (unit_at(turn + 1) < units) {                 // the next one, which may lie in two lines
+          const int* next = t.p.units + 1ll * unit_at(turn + 1) * kRaggedInts;
+          asm volatile("prefetch.global.L1 [%0];" ::"l"(next));
+          asm volatile("prefetch.global.L1 [%0];" ::"l"(next + kRaggedInts - 1));
+        }
         if (u.tiles == 0) {
           for (int r = threadIdx.x; r < u.tokens * t.group; r += 256) {
             uint4* out = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(t.a.out) + (u.row0 + r / t.group) * t.a.out_row +
@@ -497,13 +503,14 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
         if (work) {
           tc_fence_after();
           const bool edge = (place0 < b_all || place0 + kRtKeys > e_all) && place0 + kRtKeys > a_all;
-          if (edge || j == 0) {
+          if (edge) {
             float top = -INFINITY;
 #pragma unroll 1
             for (int c = 0; c < kRtKeys; c += 32) {
-              tmem_ld_32x32(s_t + c, x[0]);
               const int at = place0 + c;
-              const uint32_t seen = edge ? low_bits(a - at) | (low_bits(e - at) & ~low_bits(b - at)) : ~0u;
+              if (j > 0 && ((at >= b_all && at + 32 <= e_all) || at + 32 <= a_all)) continue;       // all of it is seen
+              tmem_ld_32x32(s_t + c, x[0]);
+              const uint32_t seen = low_bits(a - at) | (low_bits(e - at) & ~low_bits(b - at));
               tmem_wait_ld(x[0]);
 #pragma unroll
               for (int k = 0; k < 32; ++k) x[0][k] = seen >> k & 1 ? x[0][k] : 0xff800000u;
@@ -518,6 +525,7 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
           take_turn(&sh.busy[quad], lane);
           tmem_wait_ld(x[0]);
           tmem_wait_ld(x[1]);
+          if (j == 0 && !edge) m = fmaxf(largest(x[0]), largest(x[1])) * t.scale_log2;      // of the first half: seldom much less
           begin();
           weights(x[0], 0, 16, 0);
           float top = largest(x[0]);
@@ -535,7 +543,7 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
             l *= keep;
             m = m_new;
 #pragma unroll 1
-            for (int c = 0; c < vp; c += 16) {
+            for (int c = 0; c < vp && j > 0; c += 16) {
               uint32_t o[16];
               tmem_ld_32x16(o_t + c, o);
               tmem_wait_ld();
@@ -662,22 +670,26 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
 #pragma unroll
             for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * w_own);
           }
+          // a sector or two of L2 at a time
           if (!live) {
           } else if (u.pieces > 1) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              if (c + 4 * k < vp) part[k] = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]), __uint_as_float(o[4 * k + 2]),
-                                                        __uint_as_float(o[4 * k + 3]));
+            for (int k = 0; k < 4; ++k)
+              if (c + 8 * k < vp) store8(reinterpret_cast<float*>(part + 2 * k), reinterpret_cast<const float(&)[8]>(o[8 * k]));
           } else {
+            uint32_t w[16];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              uint32_t w[4];
+            for (int k = 0; k < 16; ++k) {
+              const __nv_bfloat162 q = __floats2bfloat162_rn(__uint_as_float(o[2 * k]), __uint_as_float(o[2 * k + 1]));
+              w[k] = *reinterpret_cast<const uint32_t*>(&q);
+            }
+            if (t.wide_out) {
+              store8(reinterpret_cast<float*>(out), reinterpret_cast<const float(&)[8]>(w[0]));
+              if (c + 16 < vp) store8(reinterpret_cast<float*>(out + 2), reinterpret_cast<const float(&)[8]>(w[8]));
+            } else {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const __nv_bfloat162 q = __floats2bfloat162_rn(__uint_as_float(o[8 * k + 2 * e]), __uint_as_float(o[8 * k + 2 * e + 1]));
-                w[e] = *reinterpret_cast<const uint32_t*>(&q);
-              }
-              if (c + 8 * k < vp) out[k] = make_uint4(w[0], w[1], w[2], w[3]);
+              for (int k = 0; k < 4; ++k)
+                if (c + 8 * k < vp) out[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
             }
           }
         }
@@ -735,6 +747,7 @@ cudaError_t launch_ragged_tiled(const ds41_ragged_attend_args& a, const ds41_rag
   if (kRtKeys / t.box * (t.kd > t.vc ? t.kd : t.vc) > 32) return cudaErrorInvalidValue;
   // the results of tiles in turns have to fit the second tile's place
   if (p.turn_rows > kRtTurnRows || p.turn_rows * 4 * p.vdim > t.kd * kRtChunk) return cudaErrorInvalidValue;
+  t.wide_out = !((reinterpret_cast<uintptr_t>(a.out) | 2 * a.out_row) & 31);
   t.hidden_row = a.n_pages * p.page_tokens;
   t.scale_log2 = a.scale * kLog2E;
   const int row_len = p.kv_heads * (p.dim + p.vdim);
