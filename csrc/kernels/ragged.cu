@@ -67,6 +67,11 @@ __device__ __forceinline__ int tile_cost(const ds41_ragged_pass& p, int rows) {
   return !p.tiled ? kSimpleTile : rows > p.turn_rows ? kPairTile : kTurnTile;
 }
 
+// A request's first row and first block are the sums of tokens and of ceil(tokens / unit_tokens) before it; a row finds its request by
+// search, and its cache row is page_table[slot][position / page] * page + position % page.  Blocks whose walk is longer than the chosen
+// length come in pieces, and the units are sorted by their length by counting.  A chain of dependent steps, not bytes (2 KB to 300 KB),
+// bounds it: 5.1 us for 4 requests, of which an empty kernel takes 2.2; 8.3 us for 240 requests of 20200 rows in 3648 units.  So the sums are
+// made by every CTA for itself rather than by a kernel before it, candidates are a warp's each, and many blocks are several CTAs'.
 __global__ void __launch_bounds__(kDescribeThreads) ragged_describe_kernel(const ds41_ragged_pass p, const DescribeArgs a) {
   extern __shared__ int rd_smem[];
   __shared__ unsigned long long scans[2][kDescribeWarps];
@@ -361,7 +366,8 @@ __device__ __forceinline__ float2 turn_at(int pos, float freq) {
   return quarter & 2 ? make_float2(-x, -y) : make_float2(x, y);
 }
 
-// Any sizes: one block per row, whose heads stay in shared memory between the norm and the rotation.
+// Any sizes: one block per row, whose heads stay in shared memory between the norm and the rotation.  For heads that are not whole
+// sixteens, and rows that do not begin at 16 bytes; 8192 rows of 32 and 8 heads of 128 take it 166 us, those of the form below 47.
 template <typename T>
 __global__ void __launch_bounds__(kHeadsThreads) ragged_heads_kernel(const ds41_ragged_heads_args p) {
   extern __shared__ __align__(16) float rh_row[];       // [(heads + kv_heads) * dim], then [rot_dim / 2] turns
@@ -408,7 +414,10 @@ __global__ void __launch_bounds__(kHeadsThreads) ragged_heads_kernel(const ds41_
 // Heads of multiples of 16 values and rotations of multiples of 16, rows of whole 16 bytes.  A lane has 16 values of a head: in its rotated
 // part eight and the eight that they turn with, else neighbours; as many lanes as a head has sixteens (or the next power of two) share
 // it.  A warp takes `per` steps of one row, in each of which its lanes have neighbouring heads, and keeps its lanes' turns and weights.
-// Bound by memory: what is read and written is read and written once, in whole lines.
+// y = x / sqrt(mean x^2 + eps) * w, then (y_j, y_{j + n}) turned by pos * freq_j.  Bound by memory: what is read and written is read and
+// written once, in whole lines.  8192 rows of 32 and 8 heads of 128 in bf16: 201 MB in 47 us, 4.3 TB/s, where a plain copy of as much takes
+// 31: 24 warps a multiprocessor, whose loads wait behind their own arithmetic (issue slots 57 % busy).  Five further layouts, with
+// 16 to 48 warps and loads one to three steps ahead, took 47 to 58.  16 rows: 3.0 us, the launch and three dependent loads.
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   float2 d;
   asm("mul.rn.f32x2 %0, %1, %2;"
@@ -640,7 +649,10 @@ inline int ragged_simple_smem(const ds41_ragged_pass& p) {
 }
 
 // A unit's (token, head) rows, 64 at a time, against its keys, 32 at a time, both through shared memory: scores of 2 x 4 a thread, four
-// threads to a row's softmax, and RPT rows x 4 columns of the result in a thread's registers.
+// threads to a row's softmax, and RPT rows x 4 columns of the result in a thread's registers.  fp32 products, since the tensor core has none
+// of 24 bits; bf16 takes it where pages are not of 16 to 128 tokens or whole 128s (16 x 1 over 4000: 738 us with pages of 48, 59 of 64).  Bound by latency
+// in small calls (3 + 2 x 50 rows over 500, 6 heads of 32 and 48: 19 to 22 us, launch and loads 3.4, a tile 5.5, the join 9) and by shared
+// memory's reads in large ones (32 and 8 heads of 128 in fp32: 1000 tokens 0.51 ms, 8 x 1000 3.3, 16 x 1 over 4000 0.68).
 template <typename T, int RPT>
 __global__ void __launch_bounds__(kRaggedThreads) ragged_simple_kernel(const ds41_ragged_attend_args a, const ds41_ragged_pass p) {
   extern __shared__ __align__(16) float rs_smem[];
