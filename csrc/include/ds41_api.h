@@ -686,10 +686,10 @@ typedef struct ds41_ragged_pass {
   int* row_pos;                   // [rows] position, slot (-1: none) and row of the pool (-1: none) of every row; rows behind the last
   int* row_slot;                  //   request's: 0, -1, -1
   int* row_place;
-  int* units;                     // [max_units][12] {slot, first row, tokens, first position, key/value head, first key tile, key tiles,
-                                  //   piece, pieces, first cell, counter, cells between pieces}
-  unsigned int* counters;         // [max_blocks * kv_heads][2] finished pieces of both tiles, zero between calls
-  float* part_o;                  // [max_cells][vdim] unnormalised results of pieces
+  int* units;                     // [max_units][12] {slot, first row, tokens, first position, v_parts * key/value head + part, first key tile,
+                                  //   key tiles, piece, pieces, first cell, counter, cells between pieces}
+  unsigned int* counters;         // [max_blocks * kv_heads * v_parts][2] finished pieces of both tiles, zero between calls
+  float* part_o;                  // [max_cells][vdim / v_parts] unnormalised results of pieces
   float* part_ml;                 // [max_cells]{maximum in units of log 2, sum}
   int* status;
   int rows, requests;             // most of them
@@ -699,6 +699,7 @@ typedef struct ds41_ragged_pass {
   int unit_tokens, key_tile;      // most tokens of a unit, keys of a tile
   int turn_rows;                  // most (token, head) rows of a unit whose two tiles take the keys in turn
   int max_blocks, max_units, max_cells, grid;
+  int v_parts;                    // units that share a value's columns: 2 where there are more than 128, else 1
 } ds41_ragged_pass;
 int ds41_ragged_describe(const ds41_ragged_pass* pass, const int* slots, const int* news, const int* lengths, int n,
                          const int* page_table, int n_slots, int max_pages, int n_pages, void* stream);

@@ -1,9 +1,9 @@
 // What the kernels of ragged passes share (ragged.cu, ragged_attend.cu).
 //
-// The new tokens of a request are divided into blocks of `unit_tokens`; a unit is a block, a key/value head and a range of key tiles
-// (a piece).  Softmax over a divided set of keys needs of every piece only its maximum m, its sum l = sum exp(s - m) and its
-// unnormalised result o = sum exp(s - m) v: with M = max m_i the whole is sum exp(m_i - M) o_i / sum exp(m_i - M) l_i.  The CTA that
-// finishes the last piece of a block and head joins them, in their order.
+// The new tokens of a request are divided into blocks of `unit_tokens`; a unit is a block, a key/value head (or half of its values'
+// columns) and a range of key tiles (a piece).  Softmax over a divided set of keys needs of every piece only its maximum m, its sum
+// l = sum exp(s - m) and its unnormalised result o = sum exp(s - m) v: with M = max m_i the whole is sum exp(m_i - M) o_i /
+// sum exp(m_i - M) l_i.  The CTA that finishes the last piece of a block and head joins them, in their order.
 #pragma once
 #include "ds41_stack.cuh"
 
@@ -13,11 +13,13 @@ constexpr int kRaggedInts = 12;
 
 struct RaggedUnit {
   int slot, row0, tokens, pos0, head, tile0, tiles, piece, pieces, cell, counter, step;
+  int v0;                    // its first column of a value
 };
 __device__ __forceinline__ RaggedUnit ragged_unit(const ds41_ragged_pass& p, int i) {
   const int4* u = reinterpret_cast<const int4*>(p.units + 1ll * i * kRaggedInts);
   const int4 a = u[0], b = u[1], c = u[2];
-  return {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, c.x, c.y, c.z, c.w};
+  const int half = b.x & (p.v_parts - 1);
+  return {a.x, a.y, a.z, a.w, b.x >> (p.v_parts - 1), b.y, b.z, b.w, c.x, c.y, c.z, c.w, half * (p.vdim >> 1)};
 }
 
 // First position that a row at `pos` sees behind the first tokens.
@@ -78,7 +80,8 @@ constexpr float kLog2E = 1.4426950408889634f;
 template <typename T>
 __device__ __forceinline__ void ragged_join(const ds41_ragged_pass& p, const ds41_ragged_attend_args& a, const RaggedUnit& u, int r0,
                                             int n, int warp, int warps) {
-  const int span = p.vdim <= 32 ? 8 : p.vdim <= 64 ? 16 : 32, lane = threadIdx.x & (span - 1), from_lane = threadIdx.x & 31 & ~(span - 1);
+  const int vp = p.vdim / p.v_parts, span = vp <= 32 ? 8 : vp <= 64 ? 16 : 32;
+  const int lane = threadIdx.x & (span - 1), from_lane = threadIdx.x & 31 & ~(span - 1);
   const int group = p.heads / p.kv_heads, step = warps * (32 / span);
   auto ml_at = [&](int r, int i) {
     return r < n && i < u.pieces ? __ldcg(reinterpret_cast<const float2*>(p.part_ml) + (1ll * u.cell + 1ll * i * u.step + r))
@@ -114,21 +117,21 @@ __device__ __forceinline__ void ragged_join(const ds41_ragged_pass& p, const ds4
     den += a.sink != nullptr ? exp2f(sink - base) : 0.f;
     float f = 1.f / den;                                 // a NaN in a maximum or the sink is in the sum
     if (a.gate.data != nullptr) f *= sigmoid_f32(gate);
-    T* out = static_cast<T*>(a.out) + row * a.out_row + 1ll * h * p.vdim;
-    for (int c0 = 0; c0 < p.vdim; c0 += 4 * span) {
+    T* out = static_cast<T*>(a.out) + row * a.out_row + 1ll * h * p.vdim + u.v0;
+    for (int c0 = 0; c0 < vp; c0 += 4 * span) {
       const int c = c0 + 4 * lane;
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
       for (int i0 = 0; i0 < u.pieces; i0 += span) {
         const float2 x = i0 == 0 ? ml : ml_at(r, i0 + lane);
         const unsigned there = __ballot_sync(0xffffffffu, x.x != -INFINITY) >> from_lane;      // others saw nothing and left nothing
         const float w = weight(x);
-        const float* from = p.part_o + (1ll * u.cell + 1ll * i0 * u.step + r) * p.vdim + c;
+        const float* from = p.part_o + (1ll * u.cell + 1ll * i0 * u.step + r) * vp + c;
 #pragma unroll 1
         for (int j = 0; j < min(span, u.pieces - i0); j += 8) {
           float4 v[8];
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            v[k] = c < p.vdim && there >> (j + k) & 1 ? ragged_part(from + 1ll * (j + k) * u.step * p.vdim) : make_float4(0.f, 0.f, 0.f, 0.f);
+            v[k] = c < vp && there >> (j + k) & 1 ? ragged_part(from + 1ll * (j + k) * u.step * vp) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const float wk = __shfl_sync(0xffffffffu, w, from_lane + j + k);
@@ -139,7 +142,7 @@ __device__ __forceinline__ void ragged_join(const ds41_ragged_pass& p, const ds4
           }
         }
       }
-      if (c < p.vdim && r < n) store4(out + c, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
+      if (c < vp && r < n) store4(out + c, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
     }
   }
 }

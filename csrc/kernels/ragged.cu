@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(kDescribeThreads) ragged_describe_kernel(const
   __shared__ float cost_of[kCandidates];
   __shared__ int units_of[kCandidates], cells_of[kCandidates], bins[kBins], earlier[kBins], bin_sums[kBins / 32], longest, chosen, bad, first_bad;
   int scan = 0;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = p.kv_heads, group = p.heads / p.kv_heads;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = p.kv_heads * p.v_parts, group = p.heads / p.kv_heads;
   int* row_first = rd_smem;             // [n] of every request: its first row, its first block, tokens, first token's position, slot
   int* block_first = row_first + p.requests;
   int* tokens = block_first + p.requests;
@@ -872,10 +872,11 @@ inline bool ragged_pass_ok(const ds41_ragged_pass* p) {
     return false;
   if (p->rows <= 0 || p->rows > 1 << 18 || p->requests <= 0 || p->requests > kMostRequests || p->heads <= 0 || p->kv_heads <= 0 ||
       p->heads % p->kv_heads || p->heads / p->kv_heads > 1024 || p->dim <= 0 || p->dim > 256 || (p->dim & 15) || p->vdim <= 0 ||
-      p->vdim > 256 || (p->vdim & 15) || p->page_tokens <= 0 || p->window < 0 || p->first < 0 || p->unit_tokens <= 0 || p->grid <= 0 || p->turn_rows < 0)
+      p->vdim > 256 || (p->vdim & 15) || p->page_tokens <= 0 || p->window < 0 || p->first < 0 || p->unit_tokens <= 0 || p->grid <= 0 ||
+      p->turn_rows < 0 || (p->v_parts != 1 && (p->v_parts != 2 || !p->tiled || p->vdim & 31)))
     return false;
   return p->max_blocks >= p->rows / p->unit_tokens + std::min(p->requests, p->rows) && p->max_blocks <= kMostBlocks &&
-         p->max_units >= 1ll * p->max_blocks * p->kv_heads && p->max_units < 1 << 22 && p->max_cells > 0 && p->max_cells < 1 << 22 &&
+         p->max_units >= 1ll * p->max_blocks * p->kv_heads * p->v_parts && p->max_units < 1 << 22 && p->max_cells > 0 && p->max_cells < 1 << 22 &&
          aligned(p->units, 16) && aligned(p->part_o, 32) && aligned(p->part_ml, 8) && p->key_tile == (p->tiled ? 128 : 32);
 }
 

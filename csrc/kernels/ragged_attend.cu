@@ -1,4 +1,5 @@
-// Attention of a ragged pass on tcgen05: bf16, up to 256 values of a key and 128 of a value, pages of 16 to 128 tokens or whole 128s.
+// Attention of a ragged pass on tcgen05: bf16, up to 256 values of a key and of a value, pages of 16 to 128 tokens or whole 128s.  Values
+// of more than 128 columns are two units' each, which both make the scores: tensor memory has no place for results of 256.
 //
 // The queries of one key/value head are packed: the (token, head) pairs of a block's tokens are the rows of a tensor-core tile, so that a
 // tile of keys and values is read once for all of them.  A CTA has two tiles of 128 rows.  A block of many tokens fills both, which then
@@ -178,7 +179,7 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
   uint8_t* s_v = s_k + t.k_stages * k_bytes;
   TiledShared& sh = *reinterpret_cast<TiledShared*>(s_v + t.v_stages * v_bytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int dp = t.p.dim, vp = t.p.vdim;
+  const int dp = t.p.dim, vp = t.p.vdim / t.p.v_parts;
 
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
@@ -288,7 +289,7 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
         if (!ok) break;
         behind = true;
         v_row = v_later;
-        v_col = t.p.kv_heads * dp + x.u.head * vp + 64 * v_chunk;
+        v_col = t.p.kv_heads * dp + x.u.head * t.p.vdim + x.u.v0 + 64 * v_chunk;
         if (s + 1 == q_after) load_queries();
       }
     }
@@ -468,7 +469,7 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
         if (u.tiles == 0) {
           for (int r = threadIdx.x; r < u.tokens * t.group; r += 256) {
             uint4* out = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(t.a.out) + (u.row0 + r / t.group) * t.a.out_row +
-                                                  1ll * (u.head * t.group + r % t.group) * vp);
+                                                  1ll * (u.head * t.group + r % t.group) * t.p.vdim + u.v0);
             for (int c = 0; c < vp / 8; ++c) out[c] = make_uint4(0, 0, 0, 0);
           }
           continue;
@@ -663,7 +664,7 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
       w_half *= f;
       if (!idle && n > 0) {
         float4* part = reinterpret_cast<float4*>(t.p.part_o + cell * vp);
-        uint4* out = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(t.a.out) + row * t.a.out_row + 1ll * h * vp);
+        uint4* out = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(t.a.out) + row * t.a.out_row + 1ll * h * t.p.vdim + u.v0);
         int at = turned;
 #pragma unroll 1
         for (int c = 0; c < vp; c += 32, part += 8, out += 4) {
@@ -731,7 +732,7 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
 // Places of the rings and the launch's shared memory; 0: the sizes do not fit.
 inline int tiled_smem(TiledParams& t) {
   t.kd = (t.p.dim + 63) / 64;
-  t.vc = (t.p.vdim + 63) / 64;
+  t.vc = (t.p.vdim / t.p.v_parts + 63) / 64;
   const int q = 2 * t.kd * kRtChunk, k = t.kd * kRtKeyChunk, v = t.vc * kRtKeyChunk;
   constexpr int kFixed = 1024 + static_cast<int>(sizeof(TiledShared)), kLimit = 227 * 1024;
   t.k_stages = t.v_stages = 1;
@@ -751,7 +752,7 @@ cudaError_t launch_ragged_tiled(const ds41_ragged_attend_args& a, const ds41_rag
   t.a = a;
   t.p = p;
   t.group = p.heads / p.kv_heads;
-  if (p.f32 || t.group > kRtTile || p.vdim > 128 || p.key_tile != kRtKeys || p.page_tokens < 16 ||
+  if (p.f32 || t.group > kRtTile || p.vdim > 128 * p.v_parts || p.key_tile != kRtKeys || p.page_tokens < 16 ||
       (p.page_tokens < kRtKeys ? kRtKeys % p.page_tokens : p.page_tokens % kRtKeys))
     return cudaErrorInvalidValue;
   t.per_tile = kRtTile / t.group;
@@ -761,7 +762,7 @@ cudaError_t launch_ragged_tiled(const ds41_ragged_attend_args& a, const ds41_rag
   t.box = p.page_tokens < kRtKeys ? p.page_tokens : kRtKeys;
   if (kRtKeys / t.box * (t.kd > t.vc ? t.kd : t.vc) > 32) return cudaErrorInvalidValue;
   // the results of tiles in turns have to fit the second tile's place
-  if (p.turn_rows > kRtTurnRows || p.turn_rows * 4 * p.vdim > t.kd * kRtChunk) return cudaErrorInvalidValue;
+  if (p.turn_rows > kRtTurnRows || p.turn_rows * 4 * (p.vdim / p.v_parts) > t.kd * kRtChunk) return cudaErrorInvalidValue;
   t.wide_out = !((reinterpret_cast<uintptr_t>(a.out) | 2 * a.out_row) & 31);
   t.hidden_row = a.n_pages * p.page_tokens;
   t.scale_log2 = a.scale * kLog2E;

@@ -40,7 +40,7 @@ MOST_ROWS, MOST_REQUESTS, MOST_BLOCKS = 1 << 18, 4096, 8192
 class PassArgs(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("header", "row_pos", "row_slot", "row_place", "units", "counters", "part_o", "part_ml", "status")] + \
                [(n, C.c_int) for n in ("rows", "requests", "heads", "kv_heads", "dim", "vdim", "page_tokens", "window", "first", "f32", "tiled",
-                                       "unit_tokens", "key_tile", "turn_rows", "max_blocks", "max_units", "max_cells", "grid")]
+                                       "unit_tokens", "key_tile", "turn_rows", "max_blocks", "max_units", "max_cells", "grid", "v_parts")]
 
 
 class HeadsArgs(C.Structure):
@@ -71,7 +71,7 @@ _NO_GATE = (0, 0, 0, 0, 0, 0)
 def tiled(heads: int, kv_heads: int, dim: int, vdim: int, page_tokens: int) -> bool:
     """Do bf16 calls of these sizes take the tensor-core form?  The one for everything else multiplies in 32 bits."""
     pages = page_tokens >= 16 and not (128 % page_tokens if page_tokens < 128 else page_tokens % 128)
-    return pages and heads // kv_heads <= 128 and dim <= 256 and vdim <= 128
+    return pages and heads // kv_heads <= 128 and dim <= 256 and (vdim <= 128 or (vdim <= 256 and vdim % 32 == 0))
 
 
 class RaggedPass:
@@ -97,9 +97,9 @@ class RaggedPass:
         self.columns = kv_heads * (dim + vdim)
         self._sizes()
         i32 = lambda n: torch.zeros(n, dtype=I32, device=self.device)
-        self.header, self.units, self.counters = i32(16), i32(UNIT * self.max_units), i32(2 * self.max_blocks * kv_heads)
+        self.header, self.units, self.counters = i32(16), i32(UNIT * self.max_units), i32(2 * self.max_blocks * kv_heads * self.v_parts)
         self.row_pos, self.row_slot, self.row_place = i32(rows), i32(rows), i32(rows)
-        self.part_o = torch.empty(self.max_cells * vdim, dtype=F32, device=self.device)     # what is read was written before
+        self.part_o = torch.empty(self.max_cells * (vdim // self.v_parts), dtype=F32, device=self.device)     # what is read was written before
         self.part_ml = torch.empty(self.max_cells * 2, dtype=F32, device=self.device)
         self.status = lib.new_status(self.device)
         self.table_shape: Optional[Tuple[int, ...]] = None           # of the last describe(): what attend has to match
@@ -107,7 +107,7 @@ class RaggedPass:
         a = PassArgs(*(t.data_ptr() for t in (self.header, self.row_pos, self.row_slot, self.row_place, self.units, self.counters,
                                               self.part_o, self.part_ml, self.status)),
                      rows, requests, heads, kv_heads, dim, vdim, page_tokens, window, first, int(dtype == F32), int(self.tiled),
-                     self.unit_tokens, self.key_tile, self.turn_rows, self.max_blocks, self.max_units, self.max_cells, SMS)
+                     self.unit_tokens, self.key_tile, self.turn_rows, self.max_blocks, self.max_units, self.max_cells, SMS, self.v_parts)
         self.args, self.args_ref = a, C.byref(a)
 
     def _sizes(self):
@@ -115,13 +115,15 @@ class RaggedPass:
         self.tiled = self.dtype == BF16 and tiled(self.heads, self.kv_heads, self.dim, self.vdim, self.page_tokens)
         self.unit_tokens = 2 * (128 // group) if self.tiled else max(1, 64 // group)
         self.key_tile = 128 if self.tiled else 32
+        self.v_parts = 2 if self.tiled and self.vdim > 128 else 1
+        columns = self.vdim // self.v_parts
         # of the tensor-core form: blocks of so few rows have them in both of a CTA's tiles, which take the keys in turn
-        self.turn_rows = min(64, -(-self.dim // 64) * 16384 // (4 * self.vdim)) if self.tiled else 0
+        self.turn_rows = min(64, -(-self.dim // 64) * 16384 // (4 * columns)) if self.tiled else 0
         self.max_blocks = self.rows // self.unit_tokens + min(self.requests, self.rows)
         if self.max_blocks > MOST_BLOCKS:
             raise ValueError(f"{self.rows} rows of {group} heads to a key/value head are more than a pass divides")
-        self.max_units = self.max_blocks * self.kv_heads + 8 * SMS
-        self.max_cells = min(2 * SMS * self.unit_tokens * group, 64 * self.rows * self.heads)
+        self.max_units = self.max_blocks * self.kv_heads * self.v_parts + 8 * SMS
+        self.max_cells = min(2 * SMS * self.unit_tokens * group, 64 * self.rows * self.heads * self.v_parts)
 
     def nbytes(self) -> int:
         """Device memory that the pass takes."""

@@ -25,7 +25,8 @@ def test_sizes_that_no_pass_has(kw):
 def test_forms():
     """Which sizes take the tensor-core form."""
     assert make().tiled and make(dim=256, vdim=128).tiled and make(page_tokens=16).tiled and make(page_tokens=256).tiled
-    assert not make(dtype=F32).tiled and not make(vdim=256).tiled and not make(page_tokens=24).tiled and not make(page_tokens=8).tiled
+    assert make(vdim=256).tiled and not make(vdim=240).tiled
+    assert not make(dtype=F32).tiled and not make(page_tokens=24).tiled and not make(page_tokens=8).tiled
     assert not make(heads=400, kv_heads=2).tiled
 
 

@@ -137,8 +137,8 @@ RUNS = {
 }
 # (heads, kv_heads, dim, vdim, page): those of the tensor-core form, then others
 TILED = [(8, 2, 64, 64, 64), (32, 8, 128, 128, 64), (6, 2, 32, 48, 32), (12, 1, 128, 128, 16), (4, 4, 192, 128, 128), (20, 4, 80, 16, 256),
-         (128, 1, 64, 128, 64), (3, 1, 256, 32, 32), (5, 5, 256, 128, 16)]
-OTHERS = [(8, 2, 64, 64, 24), (4, 1, 128, 256, 64), (2, 2, 16, 16, 4), (200, 1, 32, 32, 64)]
+         (128, 1, 64, 128, 64), (3, 1, 256, 32, 32), (5, 5, 256, 128, 16), (4, 1, 128, 256, 64), (8, 2, 256, 256, 64), (6, 3, 48, 160, 32)]
+OTHERS = [(8, 2, 64, 64, 24), (4, 1, 128, 240, 64), (2, 2, 16, 16, 4), (200, 1, 32, 32, 64)]
 
 
 def test_describe_rows_and_units():
@@ -172,7 +172,7 @@ def test_describe_rows_and_units():
             pieces.setdefault((row0, tokens, head), []).append((piece, of, tile0, tiles, cell, counter))
             if of > 1:
                 cells.append((cell + piece * step, step))
-        covered = {h: [0] * b.total for h in range(kv_heads)}
+        covered = {h: [0] * b.total for h in range(kv_heads * b.p.v_parts)}
         for (row0, tokens, head), found in pieces.items():
             found.sort()
             of = found[0][1]
@@ -286,7 +286,7 @@ def test_attend_tiled(run, sizes):
 
 
 @pytest.mark.parametrize("window,first", [(1, 0), (1, 1), (50, 4), (64, 0), (65, 64), (128, 100), (300, 1000), (257, 2), (10000, 3)])
-@pytest.mark.parametrize("sizes", [(8, 2, 64, 64, 64), (12, 1, 128, 128, 16), (6, 2, 32, 48, 32), (8, 2, 128, 128, 256)])
+@pytest.mark.parametrize("sizes", [(8, 2, 64, 64, 64), (12, 1, 128, 128, 16), (6, 2, 32, 48, 32), (8, 2, 128, 128, 256), (4, 2, 64, 192, 64)])
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_windows(window, first, sizes, dtype):
     H, G, D, V, P = sizes
