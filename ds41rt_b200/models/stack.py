@@ -805,6 +805,11 @@ class StackEngine(RowsEngine):
                                                          kv_heads=kv_heads, dim=dim, vdim=vdim, page_tokens=self.cache.page_tokens,
                                                          window=window, first=first, device=self.device, dtype=DTYPES[self.w.dtype])
 
+    def check_status(self, what: str = "engine pass"):
+        super().check_status(what)
+        for p in self.ragged.values():                   # of the last pass: rows at positions or slots that there are not
+            p.check_status(what)
+
     def prefix_plan(self, mixer, rows: int) -> Optional[prefix.PrefixPlan]:
         """The plan that a pass takes, static per batch size, as a captured pass needs it: its contents follow the rows.  A long pass asks
         for one, too, where a layer has no other form (its pages, its widths)."""

@@ -178,3 +178,19 @@ def test_a_snapshot_continues(model):
     e.set_rows(more, range(75, 95), [1] * 20)
     e.forward_rows(20, head=False)
     assert close(e.logits_at([19])[0], model.logits(t + more)[-1], "f32")
+
+
+def test_rows_that_cannot_be(model):
+    """A position that no page table reaches, and a slot that there is not: zeros from the attention, and told by the status."""
+    from ds41rt_b200.ops.lib import KernelError
+    e = engine(model, "f32")
+    e.cache.ensure(0, 100)
+    for pos, slot in ((100000, 0), (3, 9)):
+        e.set_rows([1, 2], [0, pos], [1 - min(slot, 1), slot])
+        e.forward_rows(2, head=False)
+        with pytest.raises(KernelError, match="1 requests"):
+            e.check_status()
+    e.set_rows([5, 6], [0, 1], [0, 0])
+    e.forward_rows(2, head=False)
+    e.check_status()
+    assert close(e.logits_at([1])[0], model.logits([5, 6])[-1], "f32")
