@@ -141,6 +141,21 @@ def test_strides(form):
     assert (store[:, :8] == 3).all() and (store[:, 8 + H * V:] == 3).all()
 
 
+@pytest.mark.parametrize("dim,vdim", [(64, 64), (128, 128), (64, 256), (128, 160)])
+def test_results_at_any_16_bytes(dim, vdim):
+    """Rows of the result that begin at 16 bytes but not at 32; requests in one piece and in many."""
+    b = Batch([(1, 9000), (100, 30), (7, 4000), (1, 0)], heads=8, kv_heads=2, dim=dim, vdim=vdim, pads=1, sink=True)
+    b.describe()
+    assert b.p.units.view(-1, ragged().UNIT)[:b.p.header[0].item(), 8].max() > 1
+    want = b.attend()
+    b.check(want)
+    wide = torch.full((b.R, 8 * vdim + 24), 7.0, dtype=BF16, device="cuda")
+    out = wide[:, 8:8 + 8 * vdim].unflatten(1, (8, vdim))
+    b.attend(out=out)
+    assert torch.equal(out[:b.total], want[:b.total])
+    assert (wide[:, :8] == 7).all() and (wide[:, 8 + 8 * vdim:] == 7).all() and (wide[b.total:] == 7).all()
+
+
 @pytest.mark.parametrize("form", FORMS)
 def test_pages_that_are_not_leased_read_as_zeros(form):
     """Of a visible page without a number, or with one that the pool does not have."""
