@@ -10,7 +10,7 @@ from test_ragged_gpu import BF16, F32, I32, Batch, ragged
 
 pytestmark = pytest.mark.gpu
 FORMS = [dict(heads=8, kv_heads=2, dim=64, vdim=64, P=64), dict(heads=8, kv_heads=2, dim=64, vdim=64, P=24),
-         dict(heads=8, kv_heads=2, dim=64, vdim=64, P=32, dtype=F32)]
+         dict(heads=8, kv_heads=2, dim=64, vdim=64, P=32, dtype=F32), dict(heads=8, kv_heads=2, dim=64, vdim=192, P=64)]
 MIXED = [(1, 700), (37, 5), None, (0, 40), (130, 129), (1, 63), (2, 126)]
 
 
