@@ -368,17 +368,18 @@ __device__ __forceinline__ float2 turn_at(int pos, float freq) {
 
 // Any sizes: one block per row, whose heads stay in shared memory between the norm and the rotation.  For heads that are not whole
 // sixteens, and rows that do not begin at 16 bytes; 8192 rows of 32 and 8 heads of 128 take it 166 us, those of the form below 47.
+// The turns come first, as pairs of 8 bytes: behind the heads they would lie at any multiple of 4.
 template <typename T>
 __global__ void __launch_bounds__(kHeadsThreads) ragged_heads_kernel(const ds41_ragged_heads_args p) {
-  extern __shared__ __align__(16) float rh_row[];       // [(heads + kv_heads) * dim], then [rot_dim / 2] turns
+  extern __shared__ __align__(16) float2 rh_turns[];     // [rot_dim / 2], then [(heads + kv_heads) * dim] values
   const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, half = p.rot_dim / 2;
   const int H = p.heads, G = p.kv_heads, D = p.dim, V = p.vdim;
-  float2* turns = reinterpret_cast<float2*>(rh_row + (H + G) * D);
+  float* const rh_row = reinterpret_cast<float*>(rh_turns + half);
   pdl_launch_dependents();
   pdl_wait();
   const int place = p.row_place[r], pos = p.row_pos[r];
   if (place < 0 || place >= p.pool_rows) return;
-  for (int i = tid; i < half; i += kHeadsThreads) turns[i] = turn_at(pos, p.freq[i]);
+  for (int i = tid; i < half; i += kHeadsThreads) rh_turns[i] = turn_at(pos, p.freq[i]);
   __syncthreads();
   T* row = static_cast<T*>(p.pool) + 1ll * place * (G * (D + V));
   T* q = static_cast<T*>(p.q_out) + r * p.ld_q;
@@ -402,7 +403,7 @@ __global__ void __launch_bounds__(kHeadsThreads) ragged_heads_kernel(const ds41_
       if (d < 2 * half) {
         const int e = d < half ? d + half : d - half;
         const float o = x[e] * f * (w != nullptr ? w[e] : 1.f);
-        const float2 t = turns[d < half ? d : e];
+        const float2 t = rh_turns[d < half ? d : e];
         v = d < half ? v * t.x - o * t.y : v * t.x + o * t.y;
       }
       dst[d] = from_f32<T>(v);

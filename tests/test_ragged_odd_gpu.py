@@ -1,0 +1,48 @@
+"""Heads of odd widths and odd numbers, and of the largest that a call takes, against the definition in 64 bits.
+
+Tolerances as in test_ragged_gpu.py: a mean of D squares and its root, D 2^-24 + 2^-21, relative; a rotation 2^-20 of |a| + |b|; a rounding
+to the type, 2^-24 or 2^-8."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+BF16, F32, I32 = torch.bfloat16, torch.float32, torch.int32
+
+
+def check(R, H, G, D, V, rot, dtype):
+    from ds41rt_b200.ops import ragged as m
+    gen = torch.Generator(device="cuda").manual_seed(H + D)
+    rnd = lambda *s: torch.randn(s, generator=gen, device="cuda")
+    qkv = rnd(R, (H + G) * D + G * V).to(dtype)
+    q, k, v = (x.unflatten(1, (-1, d)) for x, d in zip(qkv.split([H * D, G * D, G * V], 1), (D, D, V)))
+    pos = torch.arange(R, dtype=I32, device="cuda") * 977
+    place = torch.arange(R, dtype=I32, device="cuda").flip(0)
+    w = 1 + 0.3 * rnd(D)
+    freq = 10000.0 ** -(torch.arange(rot // 2, device="cuda", dtype=F32) / max(1, rot // 2))
+    pool = torch.zeros(R, G * (D + V), dtype=dtype, device="cuda")
+    out = m.heads_to_cache(q, k, v, pos, place, pool, q_norm=w, k_norm=w, eps=1e-5, freq=freq)
+    u, half = 2 ** -8 if dtype == BF16 else 2 ** -24, rot // 2
+
+    def reference(x):
+        x = x.double()
+        x = x / (x.square().mean(-1, keepdim=True) + 1e-5).sqrt() * w.double()
+        rel = D * 2 ** -24 + 2 ** -21
+        angle = pos.double()[:, None, None] * freq.double()
+        a, b = x[..., :half], x[..., half:rot]
+        y = torch.cat([a * angle.cos() - b * angle.sin(), b * angle.cos() + a * angle.sin(), x[..., rot:]], -1)
+        tol = x.abs() * rel
+        tol[..., :half] = tol[..., half:rot] = (a.abs() + b.abs()) * (rel + 2 ** -20)
+        return y, tol + u * y.abs() + 1e-30
+
+    y, tol = reference(q)
+    assert ((out.double() - y).abs() <= tol).all()
+    rows = pool[place.long()]
+    y, tol = reference(k)
+    assert ((rows[:, :G * D].double().unflatten(1, (G, D)) - y).abs() <= tol).all()
+    assert torch.equal(rows[:, G * D:], v.flatten(1))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("H,G,D,V,rot", [(2, 1, 15, 8, 8), (2, 1, 7, 3, 6), (1, 2, 9, 1, 2), (4, 1, 33, 16, 32), (3, 2, 1, 1, 0), (1, 1, 17, 5, 16)])
+def test_odd_heads(H, G, D, V, rot, dtype):
+    check(37, H, G, D, V, rot, dtype)
