@@ -340,6 +340,7 @@ __global__ void __launch_bounds__(kDescribeThreads) ragged_describe_kernel(const
 inline bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 constexpr int kHeadsThreads = 256;
+constexpr int kMostHeadValues = 50688, kHeadsSmem = 4 * (kMostHeadValues + 1024);      // of a row's queries and keys; with the turns of 1024
 
 // Cosine and sine of pos * freq, pos >= 0.  In turns that is pos * (freq / 2 pi), of which only the fraction counts: with freq / 2 pi as
 // a whole number of 2^-64 turns it is what 64 bits hold of a product of whole numbers, as exact for far positions as for near ones (with
@@ -925,7 +926,7 @@ extern "C" int ds41_ragged_heads(const ds41_ragged_heads_args* a, void* stream) 
       a->heads > 4096 || a->kv_heads > 4096 || a->rot_dim < 0 || (a->rot_dim & 1) || a->rot_dim > a->dim || a->width <= 0 || a->width > a->dim ||
       !proj_ok(a->q) || !proj_ok(a->k) || !proj_ok(a->v) || (a->rot_dim > 0 && a->freq == nullptr) || a->row_pos == nullptr ||
       a->row_place == nullptr || a->q_out == nullptr || a->pool == nullptr || a->pool_rows <= 0 || a->ld_q < 1ll * a->heads * a->dim ||
-      a->q_norm_stride < 0 || a->k_norm_stride < 0 || (a->heads + a->kv_heads) * a->dim * 4 + a->rot_dim * 4 > 200 * 1024)
+      a->q_norm_stride < 0 || a->k_norm_stride < 0 || (a->heads + a->kv_heads) * a->dim > kMostHeadValues)
     return cudaErrorInvalidValue;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (!(a->dim & 15) && a->dim <= 512 && !(a->rot_dim & 15) && !(a->kv_heads * a->vdim & 15) && !(a->ld_q & 7) && aligned(a->q_out, 16) &&
@@ -938,7 +939,7 @@ extern "C" int ds41_ragged_heads(const ds41_ragged_heads_args* a, void* stream) 
   }
   const int smem = (a->heads + a->kv_heads) * a->dim * 4 + a->rot_dim * 4;
   auto kernel = a->f32 ? ragged_heads_kernel<float> : ragged_heads_kernel<__nv_bfloat16>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeadsSmem);
   if (e != cudaSuccess) return e;
   return launch_pdl(kernel, dim3(a->rows), dim3(kHeadsThreads), smem, st, *a);
 }

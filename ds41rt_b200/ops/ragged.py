@@ -35,6 +35,7 @@ SMS = 148                       # of a B200: passes do not depend on the device 
 _raw_stream = torch._C._cuda_getCurrentRawStream      # without the object that torch.cuda.current_stream() makes for it (3 us)
 UNIT = 12                       # numbers of a unit (ds41_ragged_pass)
 MOST_ROWS, MOST_REQUESTS, MOST_BLOCKS = 1 << 18, 4096, 8192
+MOST_HEAD_VALUES = 50688        # of a row's queries and keys
 
 
 class PassArgs(C.Structure):
@@ -231,8 +232,8 @@ def heads_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, row_pos: t
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise ValueError("q, k and v are [rows, heads, values]")
     (R, H, D), G, V = q.shape, k.shape[1], v.shape[2]
-    if min(H, G, D, V) == 0 or D > 1024 or max(H, G) > 4096 or (H + G) * D > 50688:
-        raise ValueError("heads of 1 to 1024 values, of all queries and keys at most 50688")
+    if min(H, G, D, V) == 0 or D > 1024 or max(H, G) > 4096 or (H + G) * D > MOST_HEAD_VALUES:
+        raise ValueError(f"heads of 1 to 1024 values, of all queries and keys at most {MOST_HEAD_VALUES}")
     dtype, (pool_rows, columns) = pool.dtype, pool.shape if pool.dim() == 2 else (0, 0)
     if (dtype is not BF16 and dtype is not F32) or columns != G * (D + V) or not pool.is_contiguous() or not 0 < pool_rows < 1 << 31:
         raise ValueError(f"pool must be contiguous rows of {G * (D + V)} values, bf16 or fp32, fewer than 2^31")

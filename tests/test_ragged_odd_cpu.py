@@ -1,0 +1,14 @@
+"""What the heads' call and the other calls of ragged passes refuse at their limits (no GPU)."""
+import pytest
+import torch
+
+from ds41rt_b200.ops import ragged
+
+BF16, F32, I32 = torch.bfloat16, torch.float32, torch.int32
+
+
+@pytest.mark.parametrize("H,G,D", [(64, 3, 768), (49, 1, 1024), (396, 1, 128), (4001, 224, 12)])
+def test_rows_of_too_many_head_values(H, G, D):
+    at = torch.zeros(1, dtype=I32)
+    with pytest.raises(ValueError, match="50688"):
+        ragged.heads_to_cache(torch.zeros(1, H, D), torch.zeros(1, G, D), torch.zeros(1, G, 1), at, at, torch.zeros(1, G * (D + 1)))

@@ -46,3 +46,9 @@ def check(R, H, G, D, V, rot, dtype):
 @pytest.mark.parametrize("H,G,D,V,rot", [(2, 1, 15, 8, 8), (2, 1, 7, 3, 6), (1, 2, 9, 1, 2), (4, 1, 33, 16, 32), (3, 2, 1, 1, 0), (1, 1, 17, 5, 16)])
 def test_odd_heads(H, G, D, V, rot, dtype):
     check(37, H, G, D, V, rot, dtype)
+
+
+@pytest.mark.parametrize("H,G,D,rot", [(64, 2, 768, 768), (48, 1, 1024, 1024), (64, 2, 768, 0), (395, 1, 128, 128), (4000, 224, 12, 12)])
+def test_rows_of_the_most_head_values(H, G, D, rot):
+    """Up to 50688 values, and all of them turned."""
+    check(3, H, G, D, 4, rot, BF16)
