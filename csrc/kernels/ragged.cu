@@ -926,7 +926,8 @@ extern "C" int ds41_ragged_heads(const ds41_ragged_heads_args* a, void* stream) 
       a->heads > 4096 || a->kv_heads > 4096 || a->rot_dim < 0 || (a->rot_dim & 1) || a->rot_dim > a->dim || a->width <= 0 || a->width > a->dim ||
       !proj_ok(a->q) || !proj_ok(a->k) || !proj_ok(a->v) || (a->rot_dim > 0 && a->freq == nullptr) || a->row_pos == nullptr ||
       a->row_place == nullptr || a->q_out == nullptr || a->pool == nullptr || a->pool_rows <= 0 || a->ld_q < 1ll * a->heads * a->dim ||
-      a->q_norm_stride < 0 || a->k_norm_stride < 0 || (a->heads + a->kv_heads) * a->dim > kMostHeadValues)
+      a->q_norm_stride < 0 || a->k_norm_stride < 0 || (a->heads + a->kv_heads) * a->dim > kMostHeadValues ||
+      1ll * a->kv_heads * (1ll * a->dim + a->vdim) > INT_MAX)
     return cudaErrorInvalidValue;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (!(a->dim & 15) && a->dim <= 512 && !(a->rot_dim & 15) && !(a->kv_heads * a->vdim & 15) && !(a->ld_q & 7) && aligned(a->q_out, 16) &&

@@ -235,8 +235,9 @@ def heads_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, row_pos: t
     if min(H, G, D, V) == 0 or D > 1024 or max(H, G) > 4096 or (H + G) * D > MOST_HEAD_VALUES:
         raise ValueError(f"heads of 1 to 1024 values, of all queries and keys at most {MOST_HEAD_VALUES}")
     dtype, (pool_rows, columns) = pool.dtype, pool.shape if pool.dim() == 2 else (0, 0)
-    if (dtype is not BF16 and dtype is not F32) or columns != G * (D + V) or not pool.is_contiguous() or not 0 < pool_rows < 1 << 31:
-        raise ValueError(f"pool must be contiguous rows of {G * (D + V)} values, bf16 or fp32, fewer than 2^31")
+    if (dtype is not BF16 and dtype is not F32) or columns != G * (D + V) or not pool.is_contiguous() or not 0 < pool_rows < 1 << 31 \
+            or columns >= 1 << 31:
+        raise ValueError(f"pool must be contiguous rows of {G * (D + V)} values, bf16 or fp32, fewer than 2^31 rows and values of a row")
     a_q, a_k, a_v = _projection("q", q, R, H, D), _projection("k", k, R, G, D), _projection("v", v, R, G, V)
     q_weight, q_stride = (0, 0) if q_norm is None else _weight("q_norm", q_norm, H, D)
     k_weight, k_stride = (0, 0) if k_norm is None else _weight("k_norm", k_norm, G, D)

@@ -12,3 +12,11 @@ def test_rows_of_too_many_head_values(H, G, D):
     at = torch.zeros(1, dtype=I32)
     with pytest.raises(ValueError, match="50688"):
         ragged.heads_to_cache(torch.zeros(1, H, D), torch.zeros(1, G, D), torch.zeros(1, G, 1), at, at, torch.zeros(1, G * (D + 1)))
+
+
+def test_cache_rows_of_too_many_values():
+    """A row of 2^31 values: numbers of columns are 32-bit."""
+    at, G, V = torch.zeros(1, dtype=I32), 1024, (1 << 21) - 1
+    with pytest.raises(ValueError, match="values of a row"):
+        ragged.heads_to_cache(torch.zeros(1, 1, 1), torch.zeros(1, G, 1), torch.empty(1, G, V, device="meta"), at, at,
+                              torch.empty(1, G * (1 + V), device="meta"))
