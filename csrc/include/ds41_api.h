@@ -728,7 +728,7 @@ typedef struct ds41_ragged_heads_args {
 int ds41_ragged_heads(const ds41_ragged_heads_args* args, void* stream);
 
 // Attention of a described pass's rows: [rows][heads][vdim], divided by the sums (with exp(sink), if any) times sigmoid(gate).  Rows
-// without a slot become zeros, rows behind the last request's are left as they are.
+// without a slot, or on a page that is not leased, become zeros; rows behind the last request's are left as they are.
 typedef struct ds41_ragged_attend_args {
   const void* q;                  // row r, head h at r * q_row + h * q_head
   const void* pool;

@@ -4,6 +4,9 @@
 // columns) and a range of key tiles (a piece).  Softmax over a divided set of keys needs of every piece only its maximum m, its sum
 // l = sum exp(s - m) and its unnormalised result o = sum exp(s - m) v: with M = max m_i the whole is sum exp(m_i - M) o_i /
 // sum exp(m_i - M) l_i.  The CTA that finishes the last piece of a block and head joins them, in their order.
+//
+// The result of a token that has no place in the cache, as its page is not leased, is zeros: the heads' kernel has no query of it, and what
+// lies in its place may be of another pass.
 #pragma once
 #include "ds41_stack.cuh"
 
@@ -91,8 +94,10 @@ __device__ __forceinline__ void ragged_join(const ds41_ragged_pass& p, const ds4
   int r = r0 + from_lane / span;
   float2 next = ml_at(r, lane);
   float next_gate = 0.f, next_sink = -INFINITY;
+  int next_place = -1;
   auto head_of = [&](int r) {                            // rows from n on have nothing, and are not stored
     const int row = u.row0 + min(r, n - 1) / group, h = u.head * group + r % group;
+    next_place = p.row_place[row];
     if (a.gate.data != nullptr) next_gate = proj_at(a.gate, row, h);
     if (a.sink != nullptr) next_sink = a.sink[h];
   };
@@ -100,6 +105,7 @@ __device__ __forceinline__ void ragged_join(const ds41_ragged_pass& p, const ds4
   for (; r0 < n; r0 += step, r += step) {
     const float2 ml = next;                              // of the first pieces
     const float gate = next_gate, sink = next_sink * kLog2E;
+    const bool placed = next_place >= 0;
     next = ml_at(r + step, lane);
     head_of(r + step);
     const int row = u.row0 + min(r, n - 1) / group, h = u.head * group + r % group;
@@ -142,7 +148,7 @@ __device__ __forceinline__ void ragged_join(const ds41_ragged_pass& p, const ds4
           }
         }
       }
-      if (c < vp && r < n) store4(out + c, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
+      if (c < vp && r < n) store4(out + c, placed ? make_float4(o.x * f, o.y * f, o.z * f, o.w * f) : make_float4(0.f, 0.f, 0.f, 0.f));
     }
   }
 }

@@ -658,7 +658,7 @@ inline int ragged_simple_smem(const ds41_ragged_pass& p) {
 template <typename T, int RPT>
 __global__ void __launch_bounds__(kRaggedThreads) ragged_simple_kernel(const ds41_ragged_attend_args a, const ds41_ragged_pass p) {
   extern __shared__ __align__(16) float rs_smem[];
-  __shared__ int flag;
+  __shared__ int flag, places[kSimpleRows];
   const int D = p.dim, V = p.vdim, G = p.kv_heads, group = p.heads / G, ds = D + 4, nc = V / 4, row_len = G * (D + V);
   float* qs = rs_smem;                                 // [64][ds]
   float* ks = qs + kSimpleRows * ds;                   // [32][ds]
@@ -701,6 +701,7 @@ __global__ void __launch_bounds__(kRaggedThreads) ragged_simple_kernel(const ds4
       if (tid < kSimpleRows) {
         ms[tid] = -INFINITY;
         ls[tid] = 0.f;
+        places[tid] = tid < rows ? p.row_place[u.row0 + (r0 + tid) / group] : -1;
       }
       float4 acc[RPT];
 #pragma unroll
@@ -835,7 +836,7 @@ __global__ void __launch_bounds__(kRaggedThreads) ragged_simple_kernel(const ds4
           float f = w / den;
           if (a.gate.data != nullptr) f *= sigmoid_f32(proj_at(a.gate, row, h));
           store4(static_cast<T*>(a.out) + row * a.out_row + 1ll * h * V + 4 * col,
-                 make_float4(acc[i].x * f, acc[i].y * f, acc[i].z * f, acc[i].w * f));
+                 places[r] >= 0 ? make_float4(acc[i].x * f, acc[i].y * f, acc[i].z * f, acc[i].w * f) : make_float4(0.f, 0.f, 0.f, 0.f));
         }
       }
     }

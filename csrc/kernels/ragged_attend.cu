@@ -599,14 +599,16 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
         __syncwarp();
         mbar_arrive_if(ok && lane == 0, &sh.p_full[i][1]);
       }
+      const TiledUnit x = tiled_unit(t, unit_at(turn));  // once more: it takes registers
+      const RaggedUnit& u = x.u;
+      const int first_tok = i && !x.turns ? x.tok0 : 0, toks = x.turns ? u.tokens : (i ? u.tokens - x.tok0 : x.tok0);
+      const int row = u.row0 + first_tok + mine_tok, h = u.head * t.group + mine_head;
+      const bool placed = live && t.p.row_place[row] >= 0;
       if (n > 0) {
         if (ok) ok = WARP_WAIT(&sh.o_full[i], outputs & 1, 634 + i);
         ++outputs;
         tc_fence_after();
       }
-      const TiledUnit x = tiled_unit(t, unit_at(turn));  // once more: it takes registers
-      const RaggedUnit& u = x.u;
-      const int first_tok = i && !x.turns ? x.tok0 : 0, toks = x.turns ? u.tokens : (i ? u.tokens - x.tok0 : x.tok0);
       if (x.turns && i == 1) {
         // this half goes to the first tile's warps
         if (u.tiles > 1) {
@@ -648,7 +650,6 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
           m = top;
         }
       }
-      const int row = u.row0 + first_tok + mine_tok, h = u.head * t.group + mine_head;
       float f = 1.f;
       long long cell = 0;
       if (u.pieces > 1) {
@@ -697,7 +698,7 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
               const __nv_bfloat162 q = __floats2bfloat162_rn(__uint_as_float(o[2 * k]), __uint_as_float(o[2 * k + 1]));
-              w[k] = *reinterpret_cast<const uint32_t*>(&q);
+              w[k] = placed ? *reinterpret_cast<const uint32_t*>(&q) : 0u;
             }
             if (t.wide_out) {
               store8(reinterpret_cast<float*>(out), reinterpret_cast<const float(&)[8]>(w[0]));

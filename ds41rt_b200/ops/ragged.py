@@ -14,7 +14,8 @@ pages then hold.
 
 Rows behind the last request's are left as they were, in every output but the description, where they have position 0, slot -1 and place
 -1.  Requests without a slot (negative) have rows, too: their attention is zero, they have no place in the cache.  The pages of what a row
-sees have to be leased, by numbers that the pool has; others read as zeros, and nothing is stored in them.  What no row of a request's
+sees have to be leased, by numbers that the pool has; others read as zeros, and nothing is stored in them.  A new token whose own page is
+not leased has no place, either: `heads_to_cache` leaves its query out, and its attention is zero.  What no row of a request's
 block of tokens sees may hold anything, NaN included.  A NaN that a row does meet is in its result; one in a value that only some rows of
 a block see may be in the others' as well, as the tensor cores multiply it by their weight of zero.
 """
