@@ -333,6 +333,10 @@ __global__ void __launch_bounds__(kDescribeThreads) ragged_describe_kernel(const
     p.header[1] = rows;
     p.header[2] = bad;
     p.header[3] = first_bad;
+    if (bad > 0) {                      // stays until the host has seen it, whatever passes follow
+      if (p.report[0] == 0) p.report[1] = first_bad;
+      p.report[0] = min(p.report[0], INT_MAX - bad) + bad;
+    }
   }
 }
 
@@ -871,7 +875,7 @@ cudaError_t launch_ragged_simple(const ds41_ragged_attend_args& a, const ds41_ra
 
 inline bool ragged_pass_ok(const ds41_ragged_pass* p) {
   if (p == nullptr || p->header == nullptr || p->row_pos == nullptr || p->row_slot == nullptr || p->row_place == nullptr ||
-      p->units == nullptr || p->counters == nullptr || p->part_o == nullptr || p->part_ml == nullptr || p->status == nullptr)
+      p->units == nullptr || p->counters == nullptr || p->part_o == nullptr || p->part_ml == nullptr || p->status == nullptr || p->report == nullptr)
     return false;
   if (p->rows <= 0 || p->rows > 1 << 18 || p->requests <= 0 || p->requests > kMostRequests || p->heads <= 0 || p->kv_heads <= 0 ||
       p->heads % p->kv_heads || p->heads / p->kv_heads > 1024 || p->dim <= 0 || p->dim > 256 || (p->dim & 15) || p->vdim <= 0 ||

@@ -760,9 +760,10 @@ class StackEngine(RowsEngine):
         self.best_val, self.chosen = z((R,), F32), z((R,), I32)
         self.head_mask = None
         self._hint = None
-        self.status = lib.new_status(dev)
-        for p in self.ragged.values():
-            p.args.status = self.status.data_ptr()
+        self.told = z((4 + 4 * len(self.ragged),), I32)       # the status, then what the descriptions report, to be read together
+        self.status = self.told[:4]
+        for p, report in zip(self.ragged.values(), self.told[4:].view(-1, 4)):
+            p.tell(self.status, report)
         self._init_instruments()
         self.on_layer = None      # callable (layer, streams [rows, width]) after every layer of an eager pass
 
@@ -806,9 +807,13 @@ class StackEngine(RowsEngine):
                                                          window=window, first=first, device=self.device, dtype=DTYPES[self.w.dtype])
 
     def check_status(self, what: str = "engine pass"):
-        super().check_status(what)
-        for p in self.ragged.values():                   # of the last pass: rows at positions or slots that there are not
-            p.check_status(what)
+        values = self.told.tolist()
+        lib.raise_on_code(*values[:4], what)
+        for i in range(4, len(values), 4):               # rows at positions or slots that there are not, in any pass since the last check
+            found = ragged.told(values[i:i + 4])
+            if found:
+                self.told[4:].zero_()
+                raise lib.KernelError(f"{what}: {found}")
 
     def prefix_plan(self, mixer, rows: int) -> Optional[prefix.PrefixPlan]:
         """The plan that a pass takes, static per batch size, as a captured pass needs it: its contents follow the rows.  A long pass asks

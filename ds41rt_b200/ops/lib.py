@@ -180,6 +180,9 @@ def read_status(status: torch.Tensor):
 
 
 def raise_on_status(status: torch.Tensor, what: str = "kernel"):
-    code, where, block, detail = read_status(status)
+    raise_on_code(*read_status(status), what)
+
+
+def raise_on_code(code: int, where: int, block: int, detail: int, what: str = "kernel"):
     if code != 0:
         raise KernelError(f"{what}: {STATUS_NAMES.get(code, code)} at site {where}, block {block}, detail {detail}")

@@ -40,7 +40,8 @@ MOST_HEAD_VALUES = 50688        # of a row's queries and keys
 
 
 class PassArgs(C.Structure):
-    _fields_ = [(n, C.c_void_p) for n in ("header", "row_pos", "row_slot", "row_place", "units", "counters", "part_o", "part_ml", "status")] + \
+    _fields_ = [(n, C.c_void_p) for n in ("header", "row_pos", "row_slot", "row_place", "units", "counters", "part_o", "part_ml", "status",
+                                       "report")] + \
                [(n, C.c_int) for n in ("rows", "requests", "heads", "kv_heads", "dim", "vdim", "page_tokens", "window", "first", "f32", "tiled",
                                        "unit_tokens", "key_tile", "turn_rows", "max_blocks", "max_units", "max_cells", "grid", "v_parts")]
 
@@ -103,11 +104,11 @@ class RaggedPass:
         self.row_pos, self.row_slot, self.row_place = i32(rows), i32(rows), i32(rows)
         self.part_o = torch.empty(self.max_cells * (vdim // self.v_parts), dtype=F32, device=self.device)     # what is read was written before
         self.part_ml = torch.empty(self.max_cells * 2, dtype=F32, device=self.device)
-        self.status = lib.new_status(self.device)
+        self.status, self.report = lib.new_status(self.device), self.header[4:8]
         self.table_shape: Optional[Tuple[int, ...]] = None           # of the last describe(): what attend has to match
         self.n_pages = 0
         a = PassArgs(*(t.data_ptr() for t in (self.header, self.row_pos, self.row_slot, self.row_place, self.units, self.counters,
-                                              self.part_o, self.part_ml, self.status)),
+                                              self.part_o, self.part_ml, self.status, self.report)),
                      rows, requests, heads, kv_heads, dim, vdim, page_tokens, window, first, int(dtype == F32), int(self.tiled),
                      self.unit_tokens, self.key_tile, self.turn_rows, self.max_blocks, self.max_units, self.max_cells, SMS, self.v_parts)
         self.args, self.args_ref = a, C.byref(a)
@@ -127,6 +128,11 @@ class RaggedPass:
         self.max_units = self.max_blocks * self.kv_heads * self.v_parts + 8 * SMS
         self.max_cells = min(2 * SMS * self.unit_tokens * group, 64 * self.rows * self.heads * self.v_parts)
 
+    def tell(self, status: torch.Tensor, report: torch.Tensor):
+        """Where kernels report from now on: four numbers each, on the device."""
+        self.status, self.report = status, report
+        self.args.status, self.args.report = status.data_ptr(), report.data_ptr()
+
     def nbytes(self) -> int:
         """Device memory that the pass takes."""
         return sum(t.numel() * t.element_size() for t in (self.header, self.units, self.counters, self.row_pos, self.row_slot, self.row_place,
@@ -136,7 +142,7 @@ class RaggedPass:
         """`slots`, `new`, `lengths`: 32-bit integers, one per request, on the device: page table row (negative: none), new tokens, tokens
         with them.  `page_table` [slots, pages]; the pool has `n_pages`.  Returns (row_pos, row_slot, row_place) [rows] each: the pass's
         own tensors, which the next call overwrites.  A request whose lengths cannot be, or whose slot there is not, counts as one without
-        a slot, and rows beyond the pass's are left out; check_status() then raises."""
+        a slot, and rows beyond the pass's are left out; the next check_status() raises, whatever was described in between."""
         n = slots.numel()
         for name, t in (("slots", slots), ("new", new), ("lengths", lengths)):
             if t.dtype is not I32 or t.shape != (n,) or not t.is_contiguous():
@@ -158,7 +164,7 @@ class RaggedPass:
     def describe_rows(self, row_pos: torch.Tensor, row_slot: torch.Tensor, page_table: torch.Tensor, n_pages: int):
         """The same from the positions and slots of rows, 32-bit integers on the device, as other operators take them: adjacent rows of
         one slot at consecutive positions are a request's, and rows without a slot together one
-        that nothing is done for.  More requests than the pass takes are left out, and check_status() raises."""
+        that nothing is done for.  More requests than the pass takes are left out, and the next check_status() raises."""
         n = row_pos.numel()
         if n > self.rows or row_pos.dtype is not I32 or row_slot.dtype is not I32 or row_pos.shape != (n,) or row_slot.shape != (n,) \
                 or not (row_pos.is_contiguous() and row_slot.is_contiguous()):
@@ -188,11 +194,18 @@ class RaggedPass:
         return n_slots, width
 
     def check_status(self, what: str = "ragged pass"):
-        """Raises if a wait gave up, or if the last description had requests that cannot be."""
+        """Raises if a wait gave up, or if a description since the last check had requests that cannot be."""
         lib.raise_on_status(self.status, what)
-        _, _, bad, first = self.header[:4].tolist()
-        if bad:
-            raise lib.KernelError(f"{what}: {bad} requests of the description cannot be, the first of them number {first}")
+        found = told(self.report.tolist())
+        if found:
+            self.report.zero_()
+            raise lib.KernelError(f"{what}: {found}")
+
+
+def told(report) -> str:
+    """What descriptions have reported (ds41_ragged_pass), in words; nothing: ""."""
+    bad, first = report[:2]
+    return f"{bad} requests of the description cannot be, the first of them number {first}" if bad else ""
 
 
 def _elsewhere(here: int, tensors):

@@ -20,3 +20,24 @@ def test_cache_rows_of_too_many_values():
     with pytest.raises(ValueError, match="values of a row"):
         ragged.heads_to_cache(torch.zeros(1, 1, 1), torch.zeros(1, G, 1), torch.empty(1, G, V, device="meta"), at, at,
                               torch.empty(1, G * (1 + V), device="meta"))
+
+
+def test_reports_in_words():
+    assert ragged.told([0, 0, 0, 0]) == "" and ragged.told([0, 5, 0, 0]) == ""
+    assert ragged.told([2, 5, 0, 0]) == "2 requests of the description cannot be, the first of them number 5"
+
+
+def test_reports_go_where_they_are_sent():
+    p = ragged.RaggedPass(rows=16, requests=4, heads=8, kv_heads=2, dim=64, vdim=64, page_tokens=64, device="cpu")
+    assert p.args.report == p.report.data_ptr() == p.header.data_ptr() + 16 and p.args.status == p.status.data_ptr()
+    from ds41rt_b200.ops.lib import KernelError
+    p.report[0], p.report[1] = 1, 3
+    with pytest.raises(KernelError, match="1 requests .* number 3"):
+        p.check_status()
+    p.check_status()
+    there = torch.zeros(8, dtype=I32)
+    p.tell(there[:4], there[4:])
+    there[4] = 1
+    with pytest.raises(KernelError, match="number 0"):
+        p.check_status()
+    assert not there.any()
