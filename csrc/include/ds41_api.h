@@ -692,7 +692,8 @@ typedef struct ds41_ragged_pass {
   float* part_o;                  // [max_cells][vdim / v_parts] unnormalised results of pieces
   float* part_ml;                 // [max_cells]{maximum in units of log 2, sum}
   int* status;
-  int* report;                    // [4] {requests that cannot be, of all descriptions since it was zeros; of the first with any: the first}
+  int* report;                    // [4] of all descriptions since it was zeros: {requests that cannot be, of the first description with any the
+                                  //   first, tokens of requests on pages that are not leased, 2^31 - 1 - the lowest row of these}
   int rows, requests;             // most of them
   int heads, kv_heads, dim, vdim, page_tokens;
   int window, first;              // a row at p sees j <= p with j > p - window (0: all) or j < first

@@ -177,7 +177,12 @@ __global__ void __launch_bounds__(kDescribeThreads) ragged_describe_kernel(const
         slot = slot_of[i];
         if (slot >= 0) {
           const int pg = pos / p.page_tokens, id = a.page_table[1ll * slot * a.max_pages + pg];
-          if (static_cast<unsigned>(id) < static_cast<unsigned>(a.n_pages)) place = id * p.page_tokens + (pos - pg * p.page_tokens);
+          if (static_cast<unsigned>(id) < static_cast<unsigned>(a.n_pages)) {
+            place = id * p.page_tokens + (pos - pg * p.page_tokens);
+          } else {
+            atomicAdd(&p.report[2], 1);
+            atomicMax(&p.report[3], INT_MAX - r);
+          }
         }
       }
       p.row_pos[r] = pos;

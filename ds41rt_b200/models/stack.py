@@ -809,7 +809,7 @@ class StackEngine(RowsEngine):
     def check_status(self, what: str = "engine pass"):
         values = self.told.tolist()
         lib.raise_on_code(*values[:4], what)
-        for i in range(4, len(values), 4):               # rows at positions or slots that there are not, in any pass since the last check
+        for i in range(4, len(values), 4):               # rows at positions, slots or pages that there are not, in any pass since the last check
             found = ragged.told(values[i:i + 4])
             if found:
                 self.told[4:].zero_()

@@ -15,7 +15,7 @@ pages then hold.
 Rows behind the last request's are left as they were, in every output but the description, where they have position 0, slot -1 and place
 -1.  Requests without a slot (negative) have rows, too: their attention is zero, they have no place in the cache.  The pages of what a row
 sees have to be leased, by numbers that the pool has; others read as zeros, and nothing is stored in them.  A new token whose own page is
-not leased has no place, either: `heads_to_cache` leaves its query out, and its attention is zero.  What no row of a request's
+not leased has no place, either: `heads_to_cache` leaves its query out, its attention is zero, and check_status() tells of it.  What no row of a request's
 block of tokens sees may hold anything, NaN included.  A NaN that a row does meet is in its result; one in a value that only some rows of
 a block see may be in the others' as well, as the tensor cores multiply it by their weight of zero.
 """
@@ -194,7 +194,8 @@ class RaggedPass:
         return n_slots, width
 
     def check_status(self, what: str = "ragged pass"):
-        """Raises if a wait gave up, or if a description since the last check had requests that cannot be."""
+        """Raises if a wait gave up, or if a description since the last check had requests that cannot be, or new tokens on pages that
+        are not leased."""
         lib.raise_on_status(self.status, what)
         found = told(self.report.tolist())
         if found:
@@ -204,8 +205,11 @@ class RaggedPass:
 
 def told(report) -> str:
     """What descriptions have reported (ds41_ragged_pass), in words; nothing: ""."""
-    bad, first = report[:2]
-    return f"{bad} requests of the description cannot be, the first of them number {first}" if bad else ""
+    bad, first, lost, lowest = report
+    parts = [f"{bad} requests of the description cannot be, the first of them number {first}"] if bad else []
+    if lost:
+        parts += [f"{lost} new tokens are on pages that are not leased, the lowest row of them {2 ** 31 - 1 - lowest}"]
+    return "; ".join(parts)
 
 
 def _elsewhere(here: int, tensors):

@@ -25,6 +25,9 @@ def test_cache_rows_of_too_many_values():
 def test_reports_in_words():
     assert ragged.told([0, 0, 0, 0]) == "" and ragged.told([0, 5, 0, 0]) == ""
     assert ragged.told([2, 5, 0, 0]) == "2 requests of the description cannot be, the first of them number 5"
+    assert ragged.told([0, 0, 3, 2 ** 31 - 1 - 70]) == "3 new tokens are on pages that are not leased, the lowest row of them 70"
+    assert ragged.told([1, 2, 1, 2 ** 31 - 1]) == "1 requests of the description cannot be, the first of them number 2; " \
+        "1 new tokens are on pages that are not leased, the lowest row of them 0"
 
 
 def test_reports_go_where_they_are_sent():

@@ -74,3 +74,42 @@ def test_heads_and_attention_together(form, window, first):
     out = torch.full((b.R, H, V), math.nan, dtype=b.dtype, device="cuda")
     b.attend(out=out)
     same(b, out, lost, read)
+
+
+@pytest.mark.parametrize("by_rows", [False, True])
+@pytest.mark.parametrize("form", FORMS)
+def test_places(form, by_rows):
+    """A token whose page has no number, or one that the pool does not have, has place -1; every other one has its own; and it is told."""
+    from ds41rt_b200.ops.lib import KernelError
+    b, lost, read = taken_out(**form)
+    n = b.total
+    at = torch.tensor([p for _, p in b.rows], dtype=I32, device="cuda")
+    of = torch.tensor([b.slots[i] for i, _ in b.rows], dtype=I32, device="cuda")
+    pos, slot, place = b.p.describe_rows(at, of, b.d_tables, b.pages) if by_rows else b.describe()
+    assert torch.equal(pos[:n], at) and torch.equal(slot[:n], of)
+    want = b.d_tables[of.long(), (at // b.P).long()] * b.P + at % b.P
+    assert torch.equal(place[:n], torch.where(lost[:n], -1, want)) and (place[n:] == -1).all()
+    b.p.describe(b.d_slots[:0], b.d_new[:0], b.d_length[:0], b.d_tables, b.pages)          # a pass that has none
+    rows = lost.nonzero().flatten().tolist()
+    with pytest.raises(KernelError, match=f"{len(rows)} new tokens are on pages that are not leased, the lowest row of them {rows[0]}"):
+        b.p.check_status()
+    b.p.check_status()
+
+
+def test_an_engine_tells_of_pages_that_are_not_leased():
+    """A pass beyond a slot's lease and one within it: told once; what the second gives is as if the first had not been."""
+    from ds41rt_b200.ops.lib import KernelError
+    from test_ragged_engine_gpu import Model, close, config, engine, tokens
+    model = Model(config())
+    for dtype in ("f32", "bf16"):
+        e = engine(model, dtype)
+        t = tokens(32, 4)
+        e.cache.ensure(0, 32)                       # a page of 32
+        for n in (40, 32):
+            e.set_rows((t + t)[:n], range(n), [0] * n)
+            e.forward_rows(n, head=False)
+            got = e.logits_at(range(n))
+            assert not got.isnan().any() and close(got[31], model.logits(t)[-1], dtype)
+        with pytest.raises(KernelError, match="8 new tokens are on pages that are not leased, the lowest row of them 32"):
+            e.check_status()
+        e.check_status()
