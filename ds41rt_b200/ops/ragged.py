@@ -101,7 +101,9 @@ class RaggedPass:
         self._sizes()
         i32 = lambda n: torch.zeros(n, dtype=I32, device=self.device)
         self.header, self.units, self.counters = i32(16), i32(UNIT * self.max_units), i32(2 * self.max_blocks * kv_heads * self.v_parts)
-        self.row_pos, self.row_slot, self.row_place = i32(rows), i32(rows), i32(rows)
+        self.described = i32(3 * rows)
+        self.row_pos, self.row_slot, self.row_place = self.described.view(3, rows)
+        self._own = self.described.data_ptr(), self.described.data_ptr() + 12 * rows
         self.part_o = torch.empty(self.max_cells * (vdim // self.v_parts), dtype=F32, device=self.device)     # what is read was written before
         self.part_ml = torch.empty(self.max_cells * 2, dtype=F32, device=self.device)
         self.status, self.report = lib.new_status(self.device), self.header[4:8]
@@ -152,9 +154,11 @@ class RaggedPass:
         here = torch.cuda.current_device()
         if not (slots.get_device() == here and new.get_device() == here and lengths.get_device() == here):
             _elsewhere(here, (("slots", slots), ("new", new), ("lengths", lengths)))
+        slots_at, new_at, lengths_at = slots.data_ptr(), new.data_ptr(), lengths.data_ptr()
+        self._apart(n, slots_at, new_at, lengths_at)
         n_slots, width = self._table(page_table, n_pages, here)
-        err = lib.kernels("stack").ds41_ragged_describe(self.args_ref, C.c_void_p(slots.data_ptr()), C.c_void_p(new.data_ptr()),
-                                                        C.c_void_p(lengths.data_ptr()), n, C.c_void_p(page_table.data_ptr()), n_slots,
+        err = lib.kernels("stack").ds41_ragged_describe(self.args_ref, C.c_void_p(slots_at), C.c_void_p(new_at),
+                                                        C.c_void_p(lengths_at), n, C.c_void_p(page_table.data_ptr()), n_slots,
                                                         width, n_pages, C.c_void_p(_raw_stream(here)))
         if err:
             lib.check(err, "ds41_ragged_describe")
@@ -172,8 +176,7 @@ class RaggedPass:
         here = torch.cuda.current_device()
         if not (row_pos.get_device() == here and row_slot.get_device() == here):
             _elsewhere(here, (("row_pos", row_pos), ("row_slot", row_slot)))
-        if n and (row_pos.data_ptr() == self.row_pos.data_ptr() or row_slot.data_ptr() == self.row_slot.data_ptr()):
-            raise ValueError("row_pos and row_slot are what the description writes: copies of them")
+        self._apart(n, row_pos.data_ptr(), row_slot.data_ptr())
         n_slots, width = self._table(page_table, n_pages, here)
         err = lib.kernels("stack").ds41_ragged_describe_rows(self.args_ref, C.c_void_p(row_pos.data_ptr()), C.c_void_p(row_slot.data_ptr()), n,
                                                              C.c_void_p(page_table.data_ptr()), n_slots, width, n_pages,
@@ -182,6 +185,13 @@ class RaggedPass:
             lib.check(err, "ds41_ragged_describe_rows")
         self.table_shape, self.n_pages = (n_slots, width), n_pages
         return self.row_pos, self.row_slot, self.row_place
+
+    def _apart(self, n: int, *places: int):
+        """`places`: of n numbers each, which some blocks read while others write the description."""
+        low, high = self._own
+        for at in places:
+            if at < high and at + 4 * n > low:
+                raise ValueError("a description is not made from its own row_pos, row_slot and row_place: copies of them")
 
     def _table(self, page_table: torch.Tensor, n_pages: int, here: int) -> Tuple[int, int]:
         n_slots, width = page_table.shape if page_table.dim() == 2 else (0, 0)

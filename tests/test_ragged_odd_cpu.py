@@ -44,3 +44,19 @@ def test_reports_go_where_they_are_sent():
     with pytest.raises(KernelError, match="number 0"):
         p.check_status()
     assert not there.any()
+
+
+@pytest.mark.parametrize("name", ["row_pos", "row_slot", "row_place"])
+@pytest.mark.parametrize("first", [0, 1, 5])
+def test_descriptions_made_from_themselves(name, first, monkeypatch):
+    """From the beginning of what they write or from within it, of rows and of requests."""
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)             # where CPU tensors are
+    p = ragged.RaggedPass(rows=16, requests=4, heads=8, kv_heads=2, dim=64, vdim=64, page_tokens=64, device="cpu")
+    own, other, table = getattr(p, name)[first:first + 3], torch.zeros(3, dtype=I32), torch.zeros(4, 3, dtype=I32)
+    for pair in ((own, other), (other, own)):
+        with pytest.raises(ValueError, match="copies"):
+            p.describe_rows(*pair, table, 5)
+    for three in ((own, other, other), (other, own, other), (other, other, own)):
+        with pytest.raises(ValueError, match="copies"):
+            p.describe(*three, table, 5)
+    p._apart(3, own.clone().data_ptr(), other.data_ptr(), p.header.data_ptr())
