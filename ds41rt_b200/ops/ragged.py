@@ -312,7 +312,8 @@ def attend(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, descri
 
     q [rows, heads, dim]; pool [pages * page_tokens, kv_heads * (dim + vdim)]: keys of all key/value heads, then their values, the new
     tokens' among them.  `sink` [heads] fp32: an extra logit in a head's denominator; `gate` [rows, heads] fp32: a head's result times
-    sigmoid(gate).  Rows behind the last request's are left as `out` has them."""
+    sigmoid(gate).  Rows behind the last request's are left as `out` has them.  `out` may be `q` itself, but for bf16 values of more than
+    128 columns in the tensor-core form."""
     p = described
     R, H, D, V, dtype = p.rows, p.heads, p.dim, p.vdim, p.dtype
     if q.shape != (R, H, D) or q.dtype is not dtype:
@@ -338,6 +339,8 @@ def attend(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, descri
     out_at = out.data_ptr()
     if one != 1 or head != V or step % 8 or step < H * V or out_at % 16:
         raise ValueError("out must be 16-byte aligned, a row's heads side by side and rows apart, at multiples of 8 values")
+    if p.v_parts > 1 and out_at == q.data_ptr():
+        raise ValueError("out cannot be q where values have more than 128 columns: two units read a query, at different times")
     sink_at, gates = 0, _NO_GATE
     if sink is not None:
         if sink.dtype is not F32 or sink.shape != (H,) or not sink.is_contiguous():

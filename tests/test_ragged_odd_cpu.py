@@ -60,3 +60,11 @@ def test_descriptions_made_from_themselves(name, first, monkeypatch):
         with pytest.raises(ValueError, match="copies"):
             p.describe(*three, table, 5)
     p._apart(3, own.clone().data_ptr(), other.data_ptr(), p.header.data_ptr())
+
+
+def test_attention_in_place_of_queries_that_are_read_twice():
+    p = ragged.RaggedPass(rows=4, requests=4, heads=4, kv_heads=2, dim=256, vdim=256, page_tokens=64, device="cpu")
+    p.table_shape, p.n_pages = (4, 3), 5
+    q = torch.zeros(4, 4, 256, dtype=BF16)
+    with pytest.raises(ValueError, match="out cannot be q"):
+        ragged.attend(q, torch.zeros(5 * 64, 1024, dtype=BF16), torch.zeros(4, 3, dtype=I32), p, scale=0.1, out=q)

@@ -5,6 +5,8 @@ to the type, 2^-24 or 2^-8."""
 import pytest
 import torch
 
+from test_ragged_gpu import Batch
+
 pytestmark = pytest.mark.gpu
 BF16, F32, I32 = torch.bfloat16, torch.float32, torch.int32
 
@@ -52,3 +54,16 @@ def test_odd_heads(H, G, D, V, rot, dtype):
 def test_rows_of_the_most_head_values(H, G, D, rot):
     """Up to 50688 values, and all of them turned."""
     check(3, H, G, D, 4, rot, BF16)
+
+
+@pytest.mark.parametrize("form", [dict(heads=8, kv_heads=2, dim=128, vdim=128, P=64), dict(heads=8, kv_heads=2, dim=64, vdim=64, P=24),
+                                  dict(heads=8, kv_heads=2, dim=256, vdim=256, P=32, dtype=F32)])
+def test_attention_in_place_of_its_queries(form):
+    """Requests in many pieces, blocks of many rows and of few."""
+    b = Batch([(1, 9000), (300, 200), (7, 500), (65, 0), (1, 3)], window=0, sink=True, **form)
+    b.describe()
+    want = b.attend()
+    q = b.q.clone()
+    assert b.attend(out=b.q) is b.q and torch.equal(b.q, want)
+    b.q = q
+    b.check(want)
