@@ -29,7 +29,7 @@ import torch
 
 from . import lib
 from . import stack as S
-from .prefix import _heads, _steps
+from .prefix import _steps
 
 BF16, F32, I32 = torch.bfloat16, torch.float32, torch.int32
 SMS = 148                       # of a B200: passes do not depend on the device found
@@ -318,7 +318,10 @@ def attend(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, descri
     R, H, D, V, dtype = p.rows, p.heads, p.dim, p.vdim, p.dtype
     if q.shape != (R, H, D) or q.dtype is not dtype:
         raise ValueError(f"q must be [{R}, {H}, {D}] of {dtype}")
-    q_row, q_head = _heads("q", q, H, dtype)
+    q_row, q_head, one = _steps(q)
+    few = 7 if dtype is BF16 else 3               # rows and heads at multiples of 16 bytes
+    if one != 1 or q_row & few or q_head & few or q.data_ptr() % 16 or q_row < q_head * (H - 1) + D:
+        raise ValueError("q: values of a head side by side, rows and heads at multiples of 16 bytes")
     table_shape = page_table.shape
     if p.table_shape is None:
         raise ValueError("the pass has not been described")
@@ -337,8 +340,8 @@ def attend(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, descri
         raise ValueError(f"out must be [{R}, {H}, {V}] of {dtype}")
     step, head, one = _steps(out)
     out_at = out.data_ptr()
-    if one != 1 or head != V or step % 8 or step < H * V or out_at % 16:
-        raise ValueError("out must be 16-byte aligned, a row's heads side by side and rows apart, at multiples of 8 values")
+    if one != 1 or head != V or step & few or step < H * V or out_at % 16:
+        raise ValueError("out: a row's heads side by side, rows apart and at multiples of 16 bytes")
     if p.v_parts > 1 and out_at == q.data_ptr():
         raise ValueError("out cannot be q where values have more than 128 columns: two units read a query, at different times")
     sink_at, gates = 0, _NO_GATE

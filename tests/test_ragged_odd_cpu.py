@@ -68,3 +68,18 @@ def test_attention_in_place_of_queries_that_are_read_twice():
     q = torch.zeros(4, 4, 256, dtype=BF16)
     with pytest.raises(ValueError, match="out cannot be q"):
         ragged.attend(q, torch.zeros(5 * 64, 1024, dtype=BF16), torch.zeros(4, 3, dtype=I32), p, scale=0.1, out=q)
+
+
+@pytest.mark.parametrize("dtype,rows,fits", [(F32, 4, True), (F32, 2, False), (F32, 1, False), (BF16, 8, True), (BF16, 4, False)])
+def test_attention_takes_rows_at_16_bytes(dtype, rows, fits, monkeypatch):
+    """Queries, heads of queries, and results whose rows are so many values more than their own apart."""
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)              # not where CPU tensors are
+    p = ragged.RaggedPass(rows=4, requests=4, heads=4, kv_heads=2, dim=64, vdim=64, page_tokens=64, device="cpu", dtype=dtype)
+    p.table_shape, p.n_pages = (4, 3), 5
+    whole, pool, table = torch.zeros(4, 4, 64, dtype=dtype), torch.zeros(5 * 64, 256, dtype=dtype), torch.zeros(4, 3, dtype=I32)
+    apart = torch.zeros(4, 256 + rows, dtype=dtype)[:, :256].unflatten(1, (4, 64))
+    heads = torch.zeros(4, 4, 64 + rows, dtype=dtype)[..., :64]
+    for q, out in ((apart, whole), (heads, whole), (whole, apart)):
+        with pytest.raises(ValueError) as error:              # the device is looked at last
+            ragged.attend(q, pool, table, p, scale=0.1, out=out)
+        assert ("16 bytes" in str(error.value)) != fits

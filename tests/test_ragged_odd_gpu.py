@@ -67,3 +67,18 @@ def test_attention_in_place_of_its_queries(form):
     assert b.attend(out=b.q) is b.q and torch.equal(b.q, want)
     b.q = q
     b.check(want)
+
+
+@pytest.mark.parametrize("dtype,more", [(F32, 4), (F32, 12), (BF16, 8)])
+def test_attention_of_rows_at_16_bytes(dtype, more):
+    b = Batch([(1, 900), (70, 20), (5, 64)], heads=6, kv_heads=2, dim=64, vdim=48, P=32, dtype=dtype, pads=1)
+    b.describe()
+    want = b.attend()
+    b.check(want)
+    wide = torch.full((b.R, b.H, b.D + more), 5.0, dtype=dtype, device="cuda")
+    wide[..., :b.D] = b.q
+    b.q = wide[..., :b.D]
+    store = torch.full((b.R, b.H * b.V + more), 3.0, dtype=dtype, device="cuda")
+    out = store[:, :b.H * b.V].unflatten(1, (b.H, b.V))
+    b.attend(out=out)
+    assert torch.equal(out[:b.total], want[:b.total]) and (store[:, b.H * b.V:] == 3).all() and (store[b.total:] == 3).all()
