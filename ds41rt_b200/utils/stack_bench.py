@@ -81,6 +81,12 @@ def work(cfg: StackConfig, R: int, n_keys: int, first: int, decode: bool, active
     def seen(pos, chunk):
         return pos % chunk + 1 if chunk else pos + 1
 
+    def in_window(m, p0, p1):
+        """Positions that some row of p0 .. p1 sees."""
+        low = max(0, p0 - m.window + 1) if m.window else 0
+        return min(m.first, low) + p1 + 1 - low
+
+    described = set()                  # shapes of window attention: one description of the pass each
     for l, spec in enumerate(cfg.layers):
         m = spec.mixer
         chunk = getattr(m, "chunk", 0)
@@ -98,6 +104,20 @@ def work(cfg: StackConfig, R: int, n_keys: int, first: int, decode: bool, active
                 low = first - first % chunk if chunk else 0
                 add("group_prefill", (n_keys - low) * row * 2.0 + R * H * (m.dim + m.vdim) * 2.0,
                     2.0 * pairs * H * (m.dim + m.vdim))
+            gemm("gemm_o", W, H * m.vdim, 4)
+        elif m.kind == "window_attention":
+            H, G = m.heads, m.kv_heads
+            cols, row = H * m.dim + G * (m.dim + m.vdim), G * (m.dim + m.vdim)
+            out_bytes = 2 if R >= 64 else 4          # these take their projection in bf16 by its rows alone, decode's too
+            gemm("gemm_mix_in", cols + (H if m.head_gate else 0) + (W if cfg.residual_gate else 0), W, out_bytes)
+            shape = (H, G, m.dim, m.vdim, m.window, m.first)
+            if shape not in described:
+                described.add(shape)
+                add("ragged_describe", R * 20.0)
+            add("ragged_heads", R * cols * (out_bytes + 2.0))
+            keys = R * in_window(m, n_keys - 1, n_keys - 1) if decode else in_window(m, first, n_keys - 1)
+            pairs = keys if decode else sum(in_window(m, p, p) for p in range(first, n_keys))
+            add("ragged_attend", keys * row * 2.0 + R * H * (m.dim + m.vdim) * 2.0, 2.0 * pairs * H * (m.dim + m.vdim))
             gemm("gemm_o", W, H * m.vdim, 4)
         elif m.kind == "latent_attention":
             own = m.kv_from is None

@@ -85,3 +85,17 @@ def test_an_engine_asks_once(model, monkeypatch):
     with pytest.raises(error(), match="timed out at site 600, block 2, detail 3"):
         e.check_status()
     assert all(p.status.data_ptr() == e.status.data_ptr() == p.args.status for p in e.ragged.values())
+
+
+def test_kernel_classes_have_their_work(model):
+    """Every class of launches of a pass is one that utils/stack_bench.py counts the work of, and the other way round."""
+    from ds41rt_b200.utils.stack_bench import work
+    e = engine(model, "bf16")
+    e.cache.ensure(0, 100)
+    for n, decode in ((70, False), (1, True)):
+        e.set_rows(list(range(n)), range(n), [0] * n)
+        e.timeline = []
+        e.forward_rows(n, head=True)
+        tags = {tag for tag, _, _ in e.timeline}
+        e.timeline = None
+        assert tags == set(work(model.cfg, n, n, 0, decode))
