@@ -181,7 +181,6 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int dp = t.p.dim, vp = t.p.vdim / t.p.v_parts;
 
-  pdl_launch_dependents();
   if (threadIdx.x == 0) {
     mbar_init(&sh.q_full, 1);
     mbar_init(&sh.q_free, 2);                            // the products of either tile
@@ -208,6 +207,9 @@ ragged_tiled_kernel(const __grid_constant__ CUtensorMap queries, const __grid_co
   if (warp == 9) {
     tmem_alloc(&sh.tmem, 512);
     tmem_relinquish();
+    // Not before the allocation: a CTA of the next kernel with tensor memory of its own could take some here first, and would then wait for
+    // this kernel's end, which waits for the memory.
+    pdl_launch_dependents();
   }
   tc_fence_before();
   __syncthreads();

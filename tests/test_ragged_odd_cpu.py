@@ -83,3 +83,11 @@ def test_attention_takes_rows_at_16_bytes(dtype, rows, fits, monkeypatch):
         with pytest.raises(ValueError) as error:              # the device is looked at last
             ragged.attend(q, pool, table, p, scale=0.1, out=out)
         assert ("16 bytes" in str(error.value)) != fits
+
+
+def test_tensor_memory_before_the_next_kernel_may_begin():
+    """A CTA that lets the next kernel's begin beside it has its tensor memory by then: else either could wait for the other."""
+    from pathlib import Path
+    text = (Path(ragged.__file__).parents[2] / "csrc/kernels/ragged_attend.cu").read_text()
+    body = text[text.index("ragged_tiled_kernel(const __grid_constant__"):text.index("inline int tiled_smem")]
+    assert body.count("pdl_launch_dependents()") == 1 and body.index("tmem_alloc(") < body.index("pdl_launch_dependents()") < body.index("pdl_wait()")
