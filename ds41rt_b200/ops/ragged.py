@@ -35,7 +35,7 @@ BF16, F32, I32 = torch.bfloat16, torch.float32, torch.int32
 SMS = 148                       # of a B200: passes do not depend on the device found
 _raw_stream = torch._C._cuda_getCurrentRawStream      # without the object that torch.cuda.current_stream() makes for it (3 us)
 UNIT = 12                       # numbers of a unit (ds41_ragged_pass)
-MOST_ROWS, MOST_REQUESTS, MOST_BLOCKS = 1 << 18, 4096, 8192
+MOST_ROWS, MOST_REQUESTS, MOST_BLOCKS, MOST_UNITS = 1 << 18, 4096, 8192, 1 << 22
 MOST_HEAD_VALUES = 50688        # of a row's queries and keys
 
 
@@ -128,6 +128,8 @@ class RaggedPass:
         if self.max_blocks > MOST_BLOCKS:
             raise ValueError(f"{self.rows} rows of {group} heads to a key/value head are more than a pass divides")
         self.max_units = self.max_blocks * self.kv_heads * self.v_parts + 8 * SMS
+        if self.max_units >= MOST_UNITS:
+            raise ValueError(f"{self.rows} rows of {self.requests} requests with {self.kv_heads} key/value heads are more than a pass divides")
         self.max_cells = min(2 * SMS * self.unit_tokens * group, 64 * self.rows * self.heads * self.v_parts)
 
     def tell(self, status: torch.Tensor, report: torch.Tensor):

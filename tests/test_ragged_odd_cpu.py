@@ -91,3 +91,14 @@ def test_tensor_memory_before_the_next_kernel_may_begin():
     text = (Path(ragged.__file__).parents[2] / "csrc/kernels/ragged_attend.cu").read_text()
     body = text[text.index("ragged_tiled_kernel(const __grid_constant__"):text.index("inline int tiled_smem")]
     assert body.count("pdl_launch_dependents()") == 1 and body.index("tmem_alloc(") < body.index("pdl_launch_dependents()") < body.index("pdl_wait()")
+
+
+@pytest.mark.parametrize("kv_heads,vdim,fits", [(818, 64, True), (819, 64, False), (409, 256, True), (410, 256, False)])
+def test_as_many_units_as_a_pass_has(kv_heads, vdim, fits):
+    """Fewer than 2^22 = 4194304, the host says so and not the first call: 5120 blocks to a head (two parts of it) and 1184 more."""
+    sizes = dict(rows=1 << 18, requests=4096, heads=kv_heads, kv_heads=kv_heads, dim=64, vdim=vdim, page_tokens=64, device="meta")
+    if fits:
+        assert ragged.RaggedPass(**sizes).max_units < 1 << 22
+    else:
+        with pytest.raises(ValueError, match="more than a pass divides"):
+            ragged.RaggedPass(**sizes)

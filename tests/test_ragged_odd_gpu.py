@@ -82,3 +82,48 @@ def test_attention_of_rows_at_16_bytes(dtype, more):
     out = store[:, :b.H * b.V].unflatten(1, (b.H, b.V))
     b.attend(out=out)
     assert torch.equal(out[:b.total], want[:b.total]) and (store[:, b.H * b.V:] == 3).all() and (store[b.total:] == 3).all()
+
+
+@pytest.mark.parametrize("by_rows", [False, True])
+@pytest.mark.parametrize("window,first", [(0, 0), (300, 70)])
+def test_the_largest_description(window, first, by_rows):
+    """As many rows, requests and blocks as a pass takes: every row's numbers, and every (row, head) in one block's pieces."""
+    from ds41rt_b200.ops import ragged as m
+    R, n, P, G = 1 << 18, 4096, 64, 2
+    p = m.RaggedPass(rows=R, requests=n, heads=4 * G, kv_heads=G, dim=64, vdim=64, page_tokens=P, window=window, first=first, device="cuda")
+    assert p.max_blocks == m.MOST_BLOCKS and p.unit_tokens == 64
+    gen = torch.Generator().manual_seed(2)
+    new = torch.randint(0, 129, (n,), generator=gen)
+    new[new.cumsum(0) > R] = 0
+    new[17] = 0
+    new[-1] += R - new.sum() if new.sum() < R else 0
+    assert new.sum() == R
+    before = torch.randint(0, 3000, (n,), generator=gen)
+    length = new + before
+    width = int(length.max()) // P + 1
+    slots = torch.randperm(n, generator=gen)
+    table = torch.randperm(n * width, generator=gen).view(n, width).to(I32).cuda()
+    of = torch.repeat_interleave(torch.arange(n), new)
+    start = new.cumsum(0) - new
+    at = before[of] + torch.arange(R) - start[of]
+    dev = lambda x: x.to(I32).cuda()
+    if by_rows:
+        got = p.describe_rows(dev(at), dev(slots[of]), table, n * width)
+    else:
+        got = p.describe(dev(slots), dev(new), dev(length), table, n * width)
+    p.check_status()
+    pos, slot = dev(at), dev(slots[of])
+    place = table[slot.long(), (pos // P).long()] * P + pos % P
+    assert all(torch.equal(x, y) for x, y in zip(got, (pos, slot, place)))
+    count, total = p.header[:2].tolist()
+    assert total == R and 0 < count <= p.max_units
+    u = p.units.view(-1, m.UNIT)[:count].cpu().long()
+    s, row0, tokens, pos0, head, tile0, tiles, piece, pieces, cell, counter, step = u.T
+    assert (tokens > 0).all() and (tokens <= 64).all() and (s == slots[of[row0]]).all() and (pos0 == at[row0]).all()
+    assert (of[row0] == of[row0 + tokens - 1]).all() and (counter < p.counters.numel()).all()
+    begins = torch.zeros(G * (R + 1), dtype=torch.long)
+    first_piece = piece == 0
+    begins.index_add_(0, (head * (R + 1) + row0)[first_piece], torch.ones_like(row0[first_piece]))
+    begins.index_add_(0, (head * (R + 1) + row0 + tokens)[first_piece], -torch.ones_like(row0[first_piece]))
+    assert (begins.view(G, -1).cumsum(1)[:, :R] == 1).all()
+    assert first_piece.sum() == (1 / pieces.double()).sum().round() and ((cell + (piece + 1) * step)[pieces > 1] <= p.max_cells).all()
