@@ -15,6 +15,9 @@ class ConfigError(ValueError):
     pass
 
 
+MOST_HEAD_VALUES = 50688         # of a row's queries and keys, as ops/ragged.py has it
+
+
 def take(d, keys, where: str, optional=()):
     """Values of exactly `keys` (and possibly `optional`) of a JSON object."""
     if not isinstance(d, dict):
@@ -187,7 +190,12 @@ class StackConfig:
                 if min(m.heads, m.kv_heads, m.dim, m.vdim) <= 0 or min(m.window, m.first) < 0 or m.heads % m.kv_heads or \
                         max(m.dim, m.vdim) > 256:
                     raise ConfigError(f"layer {l}: sizes must be positive, heads at most 256 wide, and kv_heads must divide heads")
-                if m.rot_dim % 2 or not 0 <= m.rot_dim <= m.dim:
-                    raise ConfigError(f"layer {l}: the rotated part must be even and within the head")
+                if m.rot_dim % 2 or not 0 <= m.rot_dim <= m.dim or (m.rot_dim and m.rope is None):
+                    raise ConfigError(f"layer {l}: the rotated part must be even and within the head, and its frequencies given")
+                if not 0 < m.scale < math.inf or max(m.window, m.first) >= 1 << 31:
+                    raise ConfigError(f"layer {l}: the scale must be positive and finite, window and first numbers of tokens")
+                if m.heads // m.kv_heads > 1024 or (m.heads + m.kv_heads) * -(-m.dim // 16) * 16 > MOST_HEAD_VALUES:
+                    raise ConfigError(f"layer {l}: at most 1024 query heads to a key/value head, and {MOST_HEAD_VALUES} values of all queries "
+                                      "and keys in heads of whole 16s")
             if spec.mlp is not None and spec.mlp.kind == "moe" and not 0 < spec.mlp.top <= min(spec.mlp.experts, 32):
                 raise ConfigError(f"layer {l}: a token takes 1 to 32 of the layer's experts")

@@ -102,3 +102,20 @@ def test_as_many_units_as_a_pass_has(kv_heads, vdim, fits):
     else:
         with pytest.raises(ValueError, match="more than a pass divides"):
             ragged.RaggedPass(**sizes)
+
+
+@pytest.mark.parametrize("kw,fits", [
+    (dict(), True), (dict(scale=0.0), False), (dict(scale=-0.1), False), (dict(scale=float("nan")), False), (dict(scale=float("inf")), False),
+    (dict(rot_dim=8), False), (dict(window=1 << 31), False), (dict(first=1 << 31), False), (dict(heads=2048, kv_heads=1), False),
+    (dict(heads=1024, kv_heads=1), True), (dict(heads=196, kv_heads=2, dim=250), True), (dict(heads=198, kv_heads=2, dim=250), False)])
+def test_window_layers_that_an_engine_could_not_run(kw, fits):
+    """The configuration says so, not the engine's first pass."""
+    from ds41rt_b200 import stack_config
+    assert stack_config.MOST_HEAD_VALUES == ragged.MOST_HEAD_VALUES
+    spec = stack_config.WindowAttentionSpec(**{**dict(heads=8, kv_heads=2, dim=32, vdim=32, scale=0.1), **kw})
+    cfg = stack_config.StackConfig("w", 10, 32, (stack_config.LayerSpec(spec, None),), 1e-6)
+    if fits:
+        cfg.validate()
+    else:
+        with pytest.raises(stack_config.ConfigError):
+            cfg.validate()
