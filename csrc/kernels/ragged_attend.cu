@@ -1,5 +1,7 @@
-// Attention of a ragged pass on tcgen05: bf16, up to 256 values of a key and of a value, pages of 16 to 128 tokens or whole 128s.  Values
-// of more than 128 columns are two units' each, which both make the scores: tensor memory has no place for results of 256.
+// Attention of a ragged pass on tcgen05: bf16, up to 256 values of a key and of a value, pages of 16, 32, 64 or 128 tokens or whole 128s.
+// Values of more than 128 columns are two units' each, which both make the scores: beside two tiles' scores tensor memory has no place for
+// two results of 256.  (It has for one tile's, with two places for its scores: a form that is not built.)  Copies are as high as a page,
+// or 128; pages of other sizes could come in copies of their greatest common divisor with 128, which is not built either.
 //
 // The queries of one key/value head are packed: the (token, head) pairs of a block's tokens are the rows of a tensor-core tile, so that a
 // tile of keys and values is read once for all of them.  A CTA has two tiles of 128 rows.  A block of many tokens fills both, which then
@@ -20,8 +22,10 @@
 // What bounds it.  A pair of tiles takes 128 keys of 128 and 128 values in 3400 cycles, where the tensor core needs 2048, the exponentials
 // 2048 and shared memory 2048: S and P share a place in tensor memory, which holds no second one beside two results of 128 columns, so that
 // a tile's scores, softmax (2000), weights and products (600), and what tells one of the other (400) are a chain.  8192 tokens of 32 and 8
-// heads: 490 us at 1.66 GHz, 550 to 575 at the 1.5 that the power limit leaves (1.0 PFLOP/s; tensor pipe 51 %, exponentials 51 %).  Decode is
-// bound by memory: 64 requests of up to 8192, 1.6 GB, 272 to 290 us, 5.6 to 6.0 TB/s; 16 x 16384 161 us, 6.7 TB/s; one of 131072 88 us.
+// heads: 490 us at 1.66 GHz, 550 to 575 at the 1.5 that the power limit leaves (1.0 PFLOP/s; tensor pipe 51 %, exponentials 51 %).  Decode over
+// long contexts is bound by memory: 64 requests of up to 8192, 1.6 GB, 272 to 290 us, 5.6 to 6.0 TB/s; 16 x 16384 161 to 165 us, 6.5 to
+// 6.7 TB/s; one of 131072 88 us.  Of fewer or shorter ones units' begin and end are a larger share: 40 x 4000, 655 MB, 137 us, 4.8 TB/s;
+// 16 x 4000, 262 MB, 49 to 59 us.
 // A unit begins and ends with 4.5 us (256 rows) or 2 us (decode), which short windows pay: 200 requests with 1024 + 4 positions 183 us,
 // 846 MB, 12 % more than these for pages' ends.  4 requests of 300: 9.7 us.
 //

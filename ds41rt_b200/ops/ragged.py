@@ -15,9 +15,9 @@ pages then hold.
 Rows behind the last request's are left as they were, in every output but the description, where they have position 0, slot -1 and place
 -1.  Requests without a slot (negative) have rows, too: their attention is zero, they have no place in the cache.  The pages of what a row
 sees have to be leased, by numbers that the pool has; others read as zeros, and nothing is stored in them.  A new token whose own page is
-not leased has no place, either: `heads_to_cache` leaves its query out, its attention is zero, and check_status() tells of it.  What no row of a request's
-block of tokens sees may hold anything, NaN included.  A NaN that a row does meet is in its result; one in a value that only some rows of
-a block see may be in the others' as well, as the tensor cores multiply it by their weight of zero.
+not leased has no place, either: `heads_to_cache` leaves its query out, its attention is zero, and check_status() tells of it.  What no
+row of a request's block of tokens sees may hold anything, NaN included.  A NaN that a row does meet is in its result; one in a value that
+only some rows of a block see may be in the others' as well, as the tensor cores multiply it by their weight of zero.
 """
 from __future__ import annotations
 
@@ -72,7 +72,8 @@ _NO_GATE = (0, 0, 0, 0, 0, 0)
 
 
 def tiled(heads: int, kv_heads: int, dim: int, vdim: int, page_tokens: int) -> bool:
-    """Do bf16 calls of these sizes take the tensor-core form?  The one for everything else multiplies in 32 bits."""
+    """Do bf16 calls of these sizes take the tensor-core form (pages of 16, 32, 64, 128 or whole 128s)?  The one for everything else
+    multiplies in 32 bits, and takes many times as long in large calls."""
     pages = page_tokens >= 16 and not (128 % page_tokens if page_tokens < 128 else page_tokens % 128)
     return pages and heads // kv_heads <= 128 and dim <= 256 and (vdim <= 128 or (vdim <= 256 and vdim % 32 == 0))
 
@@ -169,8 +170,8 @@ class RaggedPass:
 
     def describe_rows(self, row_pos: torch.Tensor, row_slot: torch.Tensor, page_table: torch.Tensor, n_pages: int):
         """The same from the positions and slots of rows, 32-bit integers on the device, as other operators take them: adjacent rows of
-        one slot at consecutive positions are a request's, and rows without a slot together one
-        that nothing is done for.  More requests than the pass takes are left out, and the next check_status() raises."""
+        one slot at consecutive positions are a request's, and adjacent rows without a slot one that nothing is done for.  More
+        requests than the pass takes are left out, and the next check_status() raises."""
         n = row_pos.numel()
         if n > self.rows or row_pos.dtype is not I32 or row_slot.dtype is not I32 or row_pos.shape != (n,) or row_slot.shape != (n,) \
                 or not (row_pos.is_contiguous() and row_slot.is_contiguous()):
@@ -315,7 +316,7 @@ def attend(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, descri
     q [rows, heads, dim]; pool [pages * page_tokens, kv_heads * (dim + vdim)]: keys of all key/value heads, then their values, the new
     tokens' among them.  `sink` [heads] fp32: an extra logit in a head's denominator; `gate` [rows, heads] fp32: a head's result times
     sigmoid(gate).  Rows behind the last request's are left as `out` has them.  `out` may be `q` itself, but for bf16 values of more than
-    128 columns in the tensor-core form."""
+    128 columns in the tensor-core form.  Rows whose number in the pass's row_place is negative become zeros."""
     p = described
     R, H, D, V, dtype = p.rows, p.heads, p.dim, p.vdim, p.dtype
     if q.shape != (R, H, D) or q.dtype is not dtype:
